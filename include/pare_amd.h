@@ -56,6 +56,8 @@ extern "C" {
 #define PMI_BF16 1
 #define PMI_F32  2
 #define PMI_U8   3
+#define PMI_I8   4 /* signed 8-bit integer codes                   */
+#define PMI_F8   5 /* e4m3 codes (no infinities, largest value 448) */
 
 /* packed weight layouts */
 #define PMI_LAYOUT_STORAGE 0 /* pack_int4 order            */
@@ -559,6 +561,121 @@ PMI_API size_t pmi_argmax_workspace_bytes(int64_t rows, int64_t n);
 /* out[r, c] = silu(gate_up[r, c]) * gate_up[r, F + c]; gate_up [rows, 2F],
  * out [rows, F] fp16; F % 8 == 0. */
 PMI_API int pmi_silu_mul_f16(const void* gate_up, void* out, int64_t rows, int64_t F, void* stream);
+
+/* ---- Serving in 8 bits: the paged cache and integer products ----------------
+ * No reference counterpart: the reference serves through HuggingFace's cache
+ * (pare/eval/throughput.py:84-126 times HF generate) and only simulates 8-bit
+ * activations (quantize_inputs, pare/layers/linear.py:120-138).
+ *
+ * The cache of keys and values, code_dtype PMI_I8 or PMI_F8, code * scale = value:
+ *   k_cache [n_pages, KV, page_size, D]          one byte per code
+ *   v_cache [n_pages, KV, page_size / 16, D, 16] token 16 b + j of a page at [b, :, j]
+ *   k_scale, v_scale fp32 [n_pages, KV]
+ * page_size 16, 32, 64, 128 or 256; D 64 or 128; n_pages * page_size < 2^31; the
+ * caches 16-byte aligned. Position p of request r lies in page
+ * tables[r, p / page_size] at p % page_size. A page or slot number outside the
+ * cache is not read or written: its tokens are as if they were not there. */
+
+/* Block tables and slot maps of a step, on the device. Request r holds kv_lens[r]
+ * tokens (int32 [R], R <= 4096; negative counts as 0) in the first
+ * ceil(kv_lens[r] / page_size) pages of its row of tables (int32 [R, width], rows
+ * table_stride apart) and gets new_lens[r] more. The pages that this takes are the
+ * next ones of free_pages, a ring of `ring` page numbers (the cache's n_pages)
+ * whose first free entry and number of free entries are pool[0] and pool[1] (int32
+ * [4]; pool[2] counts refused requests). In request order, a request whose row is
+ * too short, or that needs pages when the needs up to it exceed pool[1], is refused:
+ * it keeps its length and its tokens get slot -1.
+ * Writes the fresh entries of tables, and
+ *   q_starts int32 [R + 1]  where each request's new tokens begin (at most total)
+ *   kv_lens_out int32 [R]   the lengths with the new tokens; may be kv_lens
+ *   first int32 [R]         the position of its first new token, -1 if refused
+ *   positions, slots int32 [total]  of every new token: its position, and
+ *                           page * page_size + offset (-1 and position 0 for refused
+ *                           ones and from q_starts[R] on)
+ *   pool_out int32 [4]      may be pool
+ * One launch up to 4096 tokens, else two. */
+PMI_API int pmi_extend_block_tables(int32_t* tables, int64_t table_stride, const int32_t* kv_lens,
+                                    const int32_t* new_lens, const int32_t* free_pages,
+                                    const int32_t* pool, int32_t* q_starts, int32_t* kv_lens_out,
+                                    int32_t* first, int32_t* positions, int32_t* slots,
+                                    int32_t* pool_out, int64_t R, int64_t width, int64_t ring,
+                                    int64_t page_size, int64_t total, void* stream);
+
+/* The pages of every request r with done[r] != 0 (u8 [R]) go to the end of the ring
+ * of free pages, in request order, and kv_lens[r] becomes 0. The tables stay. */
+PMI_API int pmi_release_block_tables(const int32_t* tables, int64_t table_stride, int32_t* kv_lens,
+                                     const uint8_t* done, int32_t* free_pages, int32_t* pool,
+                                     int64_t R, int64_t width, int64_t ring, int64_t page_size,
+                                     void* stream);
+
+/* RoPE and the cache write of T new tokens. qkv: fp16 or bf16 (dtype), rows of
+ * (H + 2 KV) * D values qkv_stride elements apart (a multiple of 8, 16-byte
+ * aligned); cos, sin fp32 [L, D/2] indexed by positions (int32 [T], clamped into
+ * the table), rotate_half on the two halves of the head. q_out [T, H, D] (dtype) is
+ * the rotated q. The rotated k and the v of token t go to slots[t]. Tokens with
+ * consecutive slots of one page are one run; a page must be in one run only. A run
+ * raises the page's scale (of a head, of k or of v) to what its values need, top =
+ * 127 (PMI_I8) or 448 (PMI_F8):
+ *   scale' = max(scale, amax / top),  code = round(value / scale')
+ * where scale counts as 0 for a run that begins at the page's first token, and
+ * where it grows the codes of the page's tokens before the run become
+ * round(code * scale / scale'). Each such step moves an older value by up to
+ * half a code. An infinity or NaN among the values makes its page and head NaN. */
+PMI_API int pmi_rope_append_kv(const void* qkv, int dtype, int64_t qkv_stride, const float* cos,
+                               const float* sin, int64_t L, const int32_t* positions,
+                               const int32_t* slots, void* q_out, void* k_cache, void* v_cache,
+                               float* k_scale, float* v_scale, int code_dtype, int64_t n_pages,
+                               int64_t page_size, int64_t T, int64_t H, int64_t KV, int64_t D,
+                               void* stream);
+
+/* Whole pages as values: k_out, v_out [n, KV, page_size, D] of out_dtype (PMI_F16,
+ * PMI_BF16 or PMI_F32, 16-byte aligned) of pages[i] (int32 [n]); zeros for a page
+ * number outside the cache. Tokens that nothing was written to read as whatever
+ * their bytes stand for. */
+PMI_API int pmi_read_kv_pages(const int32_t* pages, const void* k_cache, const void* v_cache,
+                              const float* k_scale, const float* v_scale, int code_dtype,
+                              int64_t n_pages, int64_t page_size, void* k_out, void* v_out,
+                              int out_dtype, int64_t n, int64_t KV, int64_t D, void* stream);
+
+/* Grouped-query attention over the cache. q: fp16 or bf16 (dtype), head h of token t
+ * at t * q_stride + h * q_head_stride elements (multiples of 8, 16-byte aligned); out
+ * [T, H, D] of the same type. Request r has the queries q_starts[r] ..
+ * q_starts[r + 1] - 1 (int32 [R + 1], ascending; null: query r, T = R) and
+ * kv_lens[r] keys, its own among them: query i of n sees positions p <= kv_lens[r] -
+ * n + i, and with window > 0 only the last `window` of them. A query that sees
+ * nothing gives zeros; rows of out from q_starts[R] on stay as they were.
+ * max_q and max_kv bound the queries and keys of a request (of a longer one the
+ * queries past max_q stay unwritten, and keys past max_kv unread); H / KV <= 64.
+ * workspace: device scratch of pmi_paged_attention_workspace_bytes() bytes for
+ * the same sizes, 256-byte aligned, its first 64 KiB zero before its first use
+ * (every call leaves them zero). Calls that may run concurrently must not share it. */
+PMI_API int pmi_paged_attention(const void* q, int dtype, int64_t q_stride, int64_t q_head_stride,
+                                const void* k_cache, const void* v_cache, const float* k_scale,
+                                const float* v_scale, int code_dtype, int64_t n_pages,
+                                int64_t page_size, const int32_t* tables, int64_t table_stride,
+                                const int32_t* kv_lens, const int32_t* q_starts, void* out,
+                                int64_t T, int64_t R, int64_t width, int64_t H, int64_t KV,
+                                int64_t D, int64_t max_q, int64_t max_kv, int64_t window,
+                                float scale, void* workspace, size_t workspace_bytes, void* stream);
+PMI_API size_t pmi_paged_attention_workspace_bytes(int64_t T, int64_t R, int64_t H, int64_t KV,
+                                                   int64_t D, int64_t max_q, int64_t max_kv,
+                                                   int64_t window);
+
+/* Rows of x [M, K] (PMI_F16, PMI_BF16 or PMI_F32, rows x_stride elements apart) as
+ * 8-bit integers: codes int8 [M, ld] = round(x * (127 / amax)), zeros from column K
+ * to ld = K rounded up to 16, and scales fp32 [M] = amax / 127, amax the largest |x| of the
+ * row (a row of zeros: scale 0). A row with an infinity or NaN gets such a scale.
+ * codes 16-byte aligned; K <= 131072. */
+PMI_API int pmi_quantize_rows(const void* x, int x_dtype, int64_t x_stride, int8_t* codes,
+                              float* scales, int64_t M, int64_t K, void* stream);
+
+/* y[m, n] = (sum_k x[m, k] w[n, k]) * x_scales[m] * w_scales[n] (+ bias[n]): codes int8
+ * [M, ld] and [N, ld], ld = K rounded up to 16, from pmi_quantize_rows, the sum exact in
+ * int32; y [M, N] and bias [N] (nullable) of dtype y_dtype (PMI_F16, PMI_BF16 or
+ * PMI_F32), rounded once. */
+PMI_API int pmi_matmul_w8a8(const int8_t* x, const float* x_scales, const int8_t* w,
+                            const float* w_scales, const void* bias, void* y, int y_dtype,
+                            int64_t M, int64_t N, int64_t K, void* stream);
 
 /* ---- Measurement hook ------------------------------------------------------
  * Reads `bytes` (a multiple of 16) of device memory at `buf` once, with at most

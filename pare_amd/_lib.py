@@ -22,7 +22,7 @@ PMI_ERR_UNSUPPORTED = -2
 PMI_ERR_HIP = -3
 PMI_ERR_NO_DEVICE = -4
 
-PMI_F16, PMI_BF16, PMI_F32, PMI_U8 = 0, 1, 2, 3
+PMI_F16, PMI_BF16, PMI_F32, PMI_U8, PMI_I8, PMI_F8 = 0, 1, 2, 3, 4, 5
 PMI_CHOICE_TILED, PMI_CHOICE_PERM, PMI_CHOICE_GM = 1, 2, 4
 PMI_LAYOUT_STORAGE, PMI_LAYOUT_KERNEL = 0, 1
 
@@ -92,6 +92,15 @@ SIGNATURES = {
     "pmi_decode_attention_workspace_bytes": (ctypes.c_size_t, [_i64, _i64, _i64, _i64]),
     "pmi_argmax_f16": (_i, [_vp, _i64, _i64, _vp, _i64, _vp, ctypes.c_size_t, _vp]),
     "pmi_argmax_workspace_bytes": (ctypes.c_size_t, [_i64, _i64]),
+    "pmi_extend_block_tables": (_i, [_vp, _i64, *[_vp] * 10, *[_i64] * 5, _vp]),
+    "pmi_release_block_tables": (_i, [_vp, _i64, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp]),
+    "pmi_rope_append_kv": (_i, [_vp, _i, _i64, _vp, _vp, _i64, *[_vp] * 7, _i, *[_i64] * 6, _vp]),
+    "pmi_read_kv_pages": (_i, [*[_vp] * 5, _i, _i64, _i64, _vp, _vp, _i, _i64, _i64, _i64, _vp]),
+    "pmi_paged_attention": (_i, [_vp, _i, _i64, _i64, *[_vp] * 4, _i, _i64, _i64, _vp, _i64, _vp, _vp, _vp,
+                                 *[_i64] * 9, ctypes.c_float, _vp, ctypes.c_size_t, _vp]),
+    "pmi_paged_attention_workspace_bytes": (ctypes.c_size_t, [_i64] * 8),
+    "pmi_quantize_rows": (_i, [_vp, _i, _i64, _vp, _vp, _i64, _i64, _vp]),
+    "pmi_matmul_w8a8": (_i, [*[_vp] * 6, _i, _i64, _i64, _i64, _vp]),
     "pmi_read_probe": (_i, [_vp, _i64, _i64, _vp, _vp]),
     "pmi_silu_mul_f16": (_i, [_vp, _vp, _i64, _i64, _vp]),
 }

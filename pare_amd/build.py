@@ -24,7 +24,7 @@ LIB_PATH = PKG_DIR / LIB_NAME
 
 SOURCES = ["capi.hip", "w4a16_gemv.hip", "w4a16_gemm.hip", "w4a16_gemm64.hip", "w4a16_skinny.hip",
            "w4a16_layout.hip", "decode_ops.hip", "gptq.hip", "probes.hip",
-           "w4a16_tgemm.hip", "w4a16_bgemm.hip"]
+           "w4a16_tgemm.hip", "w4a16_bgemm.hip", "paged_kv.hip", "paged_attention.hip", "w8a8.hip"]
 
 # The host path of a matmul call, a CPython extension against torch's headers.
 HOST_SOURCE = "host_ext.cpp"

@@ -9,7 +9,9 @@
 #include <atomic>
 #include <mutex>
 
+#include "paged.h"
 #include "pmi_launch.h"
+#include "w8a8.h"
 
 namespace {
 
@@ -84,6 +86,55 @@ bool bgemm_few_tiles(int64_t M, int64_t N, int64_t K, int64_t gs, const pmi::Bge
   if (!pmi::gemm64_supported(M, K, gs)) return Sp >= 4 * s || p >= 3;
   return Sp >= 5 * s || (Sp >= 4 * s && (M >= 2048 || (p > 1 && K >= 7168))) ||
          (p >= 3 && (M >= 2048 || (M >= 1024 && K <= 4096)));
+}
+
+int check_page_size(int64_t ps, const char* fn) {
+  if (ps != 16 && ps != 32 && ps != 64 && ps != 128 && ps != 256)
+    return fail(PMI_ERR_UNSUPPORTED, "%s: page_size=%lld must be 16, 32, 64, 128 or 256", fn, (long long)ps);
+  return PMI_OK;
+}
+
+int check_tables(int64_t R, int64_t width, int64_t stride, int64_t ring, int64_t ps, const char* fn) {
+  if (int rc = check_page_size(ps, fn)) return rc;
+  if (R < 0 || width < 0 || stride < width || ring < 0)
+    return fail(PMI_ERR_INVALID, "%s: need R, width, ring >= 0 and rows of tables that do not overlap (R=%lld "
+                "width=%lld stride=%lld ring=%lld)", fn, (long long)R, (long long)width, (long long)stride,
+                (long long)ring);
+  if (R > pmi::kTablesMaxRequests)
+    return fail(PMI_ERR_UNSUPPORTED, "%s: at most %d requests (got %lld)", fn, pmi::kTablesMaxRequests, (long long)R);
+  if (width >= (1ll << 31) / ps || ring >= (1ll << 31) / ps)
+    return fail(PMI_ERR_UNSUPPORTED, "%s: slots and positions are 32 bits", fn);
+  return PMI_OK;
+}
+
+int check_cache(const void* k, const void* v, const float* ks, const float* vs, int code_dtype, int64_t pages,
+                int64_t ps, int64_t H, int64_t KV, int64_t D, const char* fn) {
+  if (code_dtype != PMI_I8 && code_dtype != PMI_F8)
+    return fail(PMI_ERR_INVALID, "%s: code_dtype must be PMI_I8 or PMI_F8 (got %d)", fn, code_dtype);
+  if (int rc = check_page_size(ps, fn)) return rc;
+  if (pages < 0 || H <= 0 || KV <= 0 || H % KV != 0)
+    return fail(PMI_ERR_INVALID, "%s: need pages >= 0 and H a multiple of KV (pages=%lld H=%lld KV=%lld)", fn,
+                (long long)pages, (long long)H, (long long)KV);
+  if (D != 64 && D != 128)
+    return fail(PMI_ERR_UNSUPPORTED, "%s: head_dim=%lld must be 64 or 128", fn, (long long)D);
+  if (pages >= (1ll << 31) / ps || KV > 65535 || H > 65535)
+    return fail(PMI_ERR_UNSUPPORTED, "%s: cache too large", fn);
+  if (pages && (!k || !v || !ks || !vs)) return fail(PMI_ERR_INVALID, "%s: null cache buffer", fn);
+  if (!aligned(k, 16) || !aligned(v, 16))
+    return fail(PMI_ERR_INVALID, "%s: the caches must be 16-byte aligned", fn);
+  return PMI_OK;
+}
+
+int check_w8a8(int64_t M, int64_t N, int64_t K, const char* fn) {
+  if (M < 0 || N < 0 || K <= 0)
+    return fail(PMI_ERR_INVALID, "%s: need M, N >= 0 and K > 0 (M=%lld N=%lld K=%lld)", fn, (long long)M, (long long)N,
+                (long long)K);
+  if (K > pmi::kW8A8MaxK)
+    return fail(PMI_ERR_UNSUPPORTED, "%s: K=%lld exceeds %lld, past which int32 sums may overflow", fn, (long long)K,
+                (long long)pmi::kW8A8MaxK);
+  if (M >= (1ll << 24) || N >= (1ll << 24))
+    return fail(PMI_ERR_UNSUPPORTED, "%s: M and N must be below 2^24", fn);
+  return PMI_OK;
 }
 
 }  // namespace
@@ -1334,6 +1385,155 @@ int pmi_silu_mul_f16(const void* gate_up, void* out, int64_t rows, int64_t F, vo
     return fail(PMI_ERR_INVALID, "%s: buffers must be 16-byte aligned", fn);
   if (rows * F * 2 >= (1ll << 31)) return fail(PMI_ERR_UNSUPPORTED, "%s: too large", fn);
   return from_hip(pmi::launch_silu_mul(gate_up, out, rows, F, (hipStream_t)stream), fn);
+}
+
+// ---- serving in 8 bits ---------------------------------------------------------
+
+int pmi_extend_block_tables(int32_t* tables, int64_t table_stride, const int32_t* kv_lens,
+                            const int32_t* new_lens, const int32_t* free_pages, const int32_t* pool,
+                            int32_t* q_starts, int32_t* kv_lens_out, int32_t* first, int32_t* positions,
+                            int32_t* slots, int32_t* pool_out, int64_t R, int64_t width, int64_t ring,
+                            int64_t page_size, int64_t total, void* stream) {
+  const char* fn = "pmi_extend_block_tables";
+  if (int rc = check_tables(R, width, table_stride, ring, page_size, fn)) return rc;
+  if (total < 0 || total >= (1ll << 31))
+    return fail(PMI_ERR_INVALID, "%s: total=%lld must be in [0, 2^31)", fn, (long long)total);
+  if (!pool || !q_starts || !pool_out || (R && (!tables || !kv_lens || !new_lens || !kv_lens_out || !first)) ||
+      (ring && !free_pages) || (total && (!positions || !slots)))
+    return fail(PMI_ERR_INVALID, "%s: null buffer", fn);
+  const pmi::PagedTables t = {tables, table_stride, kv_lens, new_lens, free_pages, pool, q_starts, kv_lens_out,
+                              first, positions, slots, pool_out, R, width, ring, page_size, total};
+  return from_hip(pmi::launch_extend_tables(t, (hipStream_t)stream), fn);
+}
+
+int pmi_release_block_tables(const int32_t* tables, int64_t table_stride, int32_t* kv_lens, const uint8_t* done,
+                             int32_t* free_pages, int32_t* pool, int64_t R, int64_t width, int64_t ring,
+                             int64_t page_size, void* stream) {
+  const char* fn = "pmi_release_block_tables";
+  if (int rc = check_tables(R, width, table_stride, ring, page_size, fn)) return rc;
+  if (R == 0 || ring == 0) return ok();
+  if (!tables || !kv_lens || !done || !free_pages || !pool) return fail(PMI_ERR_INVALID, "%s: null buffer", fn);
+  return from_hip(pmi::launch_release_tables(tables, table_stride, kv_lens, done, free_pages, pool, R, width, ring,
+                                             page_size, (hipStream_t)stream), fn);
+}
+
+int pmi_rope_append_kv(const void* qkv, int dtype, int64_t qkv_stride, const float* cos_t, const float* sin_t,
+                       int64_t L, const int32_t* positions, const int32_t* slots, void* q_out, void* k_cache,
+                       void* v_cache, float* k_scale, float* v_scale, int code_dtype, int64_t n_pages,
+                       int64_t page_size, int64_t T, int64_t H, int64_t KV, int64_t D, void* stream) {
+  const char* fn = "pmi_rope_append_kv";
+  if (int rc = check_cache(k_cache, v_cache, k_scale, v_scale, code_dtype, n_pages, page_size, H, KV, D, fn)) return rc;
+  if (dtype != PMI_F16 && dtype != PMI_BF16)
+    return fail(PMI_ERR_INVALID, "%s: dtype must be PMI_F16 or PMI_BF16 (got %d)", fn, dtype);
+  if (T < 0 || L <= 0 || qkv_stride < (H + 2 * KV) * D || qkv_stride % 8 != 0)
+    return fail(PMI_ERR_INVALID, "%s: need T >= 0, L > 0 and qkv_stride >= (H + 2 KV) D, a multiple of 8 "
+                "(T=%lld L=%lld stride=%lld)", fn, (long long)T, (long long)L, (long long)qkv_stride);
+  if (T == 0) return ok();
+  if (T >= (1ll << 31) || L >= (1ll << 31) || T * (H / KV) * (D / 16) >= (1ll << 36))
+    return fail(PMI_ERR_UNSUPPORTED, "%s: too many tokens", fn);
+  if (!qkv || !cos_t || !sin_t || !positions || !slots || !q_out) return fail(PMI_ERR_INVALID, "%s: null buffer", fn);
+  for (const void* p : {qkv, (const void*)cos_t, (const void*)sin_t, (const void*)q_out})
+    if (!aligned(p, 16)) return fail(PMI_ERR_INVALID, "%s: qkv, cos, sin and q_out must be 16-byte aligned", fn);
+  const pmi::PagedCache c = {k_cache, v_cache, k_scale, v_scale, n_pages, KV, page_size, D, code_dtype == PMI_F8};
+  return from_hip(pmi::launch_append_kv(c, qkv, qkv_stride, dtype == PMI_BF16, cos_t, sin_t, L, positions, slots,
+                                        q_out, T, H, (hipStream_t)stream), fn);
+}
+
+int pmi_read_kv_pages(const int32_t* pages, const void* k_cache, const void* v_cache, const float* k_scale,
+                      const float* v_scale, int code_dtype, int64_t n_pages, int64_t page_size, void* k_out,
+                      void* v_out, int out_dtype, int64_t n, int64_t KV, int64_t D, void* stream) {
+  const char* fn = "pmi_read_kv_pages";
+  if (int rc = check_cache(k_cache, v_cache, k_scale, v_scale, code_dtype, n_pages, page_size, KV, KV, D, fn)) return rc;
+  if (out_dtype != PMI_F16 && out_dtype != PMI_BF16 && out_dtype != PMI_F32)
+    return fail(PMI_ERR_INVALID, "%s: out_dtype must be PMI_F16, PMI_BF16 or PMI_F32 (got %d)", fn, out_dtype);
+  if (n < 0) return fail(PMI_ERR_INVALID, "%s: need n >= 0", fn);
+  if (n == 0) return ok();
+  if (n >= (1ll << 31) / KV) return fail(PMI_ERR_UNSUPPORTED, "%s: too many pages", fn);
+  if (!pages || !k_out || !v_out) return fail(PMI_ERR_INVALID, "%s: null buffer", fn);
+  if (!aligned(k_out, 16) || !aligned(v_out, 16))
+    return fail(PMI_ERR_INVALID, "%s: k_out and v_out must be 16-byte aligned", fn);
+  const pmi::PagedCache c = {const_cast<void*>(k_cache), const_cast<void*>(v_cache), const_cast<float*>(k_scale),
+                             const_cast<float*>(v_scale), n_pages, KV, page_size, D, code_dtype == PMI_F8};
+  return from_hip(pmi::launch_read_pages(c, pages, out_dtype, k_out, v_out, n, (hipStream_t)stream), fn);
+}
+
+size_t pmi_paged_attention_workspace_bytes(int64_t T, int64_t R, int64_t H, int64_t KV, int64_t D, int64_t max_q,
+                                           int64_t max_kv, int64_t window) {
+  const int64_t most = 1ll << 31;
+  if (T <= 0 || R <= 0 || H <= 0 || KV <= 0 || H % KV != 0 || D <= 0 || max_q <= 0 || max_kv <= 0) return 0;
+  if (T >= most || R >= most || H > 65535 || D > 65535 || max_q >= most || max_kv >= most || window < 0) return 0;
+  pmi::PagedAttention p = {};
+  p.T = T, p.R = R, p.H = H, p.max_q = max_q, p.max_kv = max_kv, p.window = window;
+  pmi::PagedCache c = {};
+  c.KV = KV, c.D = D;
+  return pmi::paged_attention_ws_bytes(p, c);
+}
+
+int pmi_paged_attention(const void* q, int dtype, int64_t q_stride, int64_t q_head_stride, const void* k_cache,
+                        const void* v_cache, const float* k_scale, const float* v_scale, int code_dtype,
+                        int64_t n_pages, int64_t page_size, const int32_t* tables, int64_t table_stride,
+                        const int32_t* kv_lens, const int32_t* q_starts, void* out, int64_t T, int64_t R,
+                        int64_t width, int64_t H, int64_t KV, int64_t D, int64_t max_q, int64_t max_kv,
+                        int64_t window, float scale, void* workspace, size_t workspace_bytes, void* stream) {
+  const char* fn = "pmi_paged_attention";
+  if (int rc = check_cache(k_cache, v_cache, k_scale, v_scale, code_dtype, n_pages, page_size, H, KV, D, fn)) return rc;
+  if (dtype != PMI_F16 && dtype != PMI_BF16)
+    return fail(PMI_ERR_INVALID, "%s: dtype must be PMI_F16 or PMI_BF16 (got %d)", fn, dtype);
+  if (T < 0 || R < 0 || width < 0 || table_stride < width || max_q < 0 || max_kv < 0 || window < 0)
+    return fail(PMI_ERR_INVALID, "%s: T, R, width, max_q, max_kv and window may not be negative, rows of tables not "
+                "overlap", fn);
+  if (!q_starts && T != R)
+    return fail(PMI_ERR_INVALID, "%s: without q_starts every request has one query (T=%lld R=%lld)", fn, (long long)T,
+                (long long)R);
+  if (H / KV > 64)
+    return fail(PMI_ERR_UNSUPPORTED, "%s: at most 64 query heads per KV head (got %lld)", fn, (long long)(H / KV));
+  if (q_stride % 8 != 0 || q_head_stride % 8 != 0)
+    return fail(PMI_ERR_INVALID, "%s: the strides of q must be multiples of 8 elements", fn);
+  if (T == 0 || R == 0 || max_q == 0) return ok();
+  if (T >= (1ll << 31) / H || R >= (1ll << 31) / KV || width >= (1ll << 31) / page_size || max_kv >= (1ll << 31) ||
+      max_q >= (1ll << 31) / (H / KV) || window >= (1ll << 31))
+    return fail(PMI_ERR_UNSUPPORTED, "%s: too large", fn);
+  if (!q || !out || !kv_lens || (width && !tables)) return fail(PMI_ERR_INVALID, "%s: null buffer", fn);
+  if (!aligned(q, 16) || !aligned(out, 16))
+    return fail(PMI_ERR_INVALID, "%s: q and out must be 16-byte aligned", fn);
+  pmi::PagedAttention p = {q, q_stride, q_head_stride, out, tables, table_stride, kv_lens, q_starts, T, R, width, H,
+                           max_q, max_kv, window, scale, dtype == PMI_BF16};
+  const pmi::PagedCache c = {const_cast<void*>(k_cache), const_cast<void*>(v_cache), const_cast<float*>(k_scale),
+                             const_cast<float*>(v_scale), n_pages, KV, page_size, D, code_dtype == PMI_F8};
+  const size_t need = pmi_paged_attention_workspace_bytes(T, R, H, KV, D, max_q, max_kv, window);
+  if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 256)))
+    return fail(PMI_ERR_INVALID, "%s: needs a 256-byte aligned workspace of %zu bytes", fn, need);
+  return from_hip(pmi::launch_paged_attention(p, c, workspace, workspace_bytes, (hipStream_t)stream), fn);
+}
+
+int pmi_quantize_rows(const void* x, int x_dtype, int64_t x_stride, int8_t* codes, float* scales, int64_t M,
+                      int64_t K, void* stream) {
+  const char* fn = "pmi_quantize_rows";
+  if (x_dtype != PMI_F16 && x_dtype != PMI_BF16 && x_dtype != PMI_F32)
+    return fail(PMI_ERR_INVALID, "%s: x_dtype must be PMI_F16, PMI_BF16 or PMI_F32 (got %d)", fn, x_dtype);
+  if (int rc = check_w8a8(M, 1, K, fn)) return rc;
+  if (x_stride < K) return fail(PMI_ERR_INVALID, "%s: x_stride=%lld is less than K", fn, (long long)x_stride);
+  if (M == 0) return ok();
+  if (!x || !codes || !scales) return fail(PMI_ERR_INVALID, "%s: null buffer", fn);
+  if (!aligned(codes, 16) || !aligned(x, x_dtype == PMI_F32 ? 4 : 2))
+    return fail(PMI_ERR_INVALID, "%s: codes must be 16-byte aligned, x a multiple of its type", fn);
+  return from_hip(pmi::launch_quantize_rows(x, x_dtype, x_stride, codes, scales, M, K, (K + 15) / 16 * 16,
+                                            (hipStream_t)stream), fn);
+}
+
+int pmi_matmul_w8a8(const int8_t* x, const float* x_scales, const int8_t* w, const float* w_scales,
+                    const void* bias, void* y, int y_dtype, int64_t M, int64_t N, int64_t K, void* stream) {
+  const char* fn = "pmi_matmul_w8a8";
+  if (y_dtype != PMI_F16 && y_dtype != PMI_BF16 && y_dtype != PMI_F32)
+    return fail(PMI_ERR_INVALID, "%s: y_dtype must be PMI_F16, PMI_BF16 or PMI_F32 (got %d)", fn, y_dtype);
+  if (int rc = check_w8a8(M, N, K, fn)) return rc;
+  if (M == 0 || N == 0) return ok();
+  if (!x || !x_scales || !w || !w_scales || !y) return fail(PMI_ERR_INVALID, "%s: null buffer", fn);
+  const size_t size = y_dtype == PMI_F32 ? 4 : 2;
+  if (!aligned(x, 16) || !aligned(w, 16) || !aligned(y, size) || !aligned(bias, size))
+    return fail(PMI_ERR_INVALID, "%s: x and w must be 16-byte aligned, y and bias multiples of their type", fn);
+  const pmi::W8A8 p = {x, x_scales, w, w_scales, bias, y, M, N, (K + 15) / 16 * 16, y_dtype};
+  return from_hip(pmi::launch_w8a8(p, (hipStream_t)stream), fn);
 }
 
 }  // extern "C"

@@ -1,0 +1,582 @@
+"""The paged 8-bit cache against plain implementations (oracle/serving_oracle.py): block
+tables and slots, the write with RoPE, the read, attention, refusals, capture."""
+
+from __future__ import annotations
+
+import ctypes
+import random
+
+import numpy as np
+import pytest
+import torch
+
+import pare_amd as P
+from oracle import serving_oracle as S
+from pare_amd import _lib
+
+gpu = pytest.mark.gpu
+DEV = torch.device("cuda:0")
+CODES = [torch.int8, torch.float8_e4m3fn]
+
+
+def _ints(v):
+    return torch.tensor(v, dtype=torch.int32, device=DEV)
+
+
+# --- the oracle itself (CPU) ---------------------------------------------------------
+
+def test_oracle_append_error_is_half_a_code():
+    """Values written in one run are within half a code of what they were."""
+    rng = np.random.default_rng(0)
+    for dtype in CODES:
+        c = S.Cache(2, 1, 16, 64, dtype)
+        x = rng.standard_normal((16, 3 * 64)).astype(np.float32)
+        ones, zeros = np.ones((16, 32), np.float32), np.zeros((16, 32), np.float32)
+        c.append(x, ones, zeros, np.arange(16), np.arange(16, 32), 1)
+        for i in range(2):
+            want = x[:, 64 * (1 + i):64 * (2 + i)]
+            scale = c.scales[i][1, 0]
+            step = 1.0 if dtype == torch.int8 else np.maximum(np.abs(want) / scale * 2 ** -3, 2.0 ** -9)
+            assert (np.abs(c.values(i)[1, 0] - want) <= 0.5001 * scale * step).all()
+
+
+def test_oracle_tables_by_hand():
+    t, starts, lens, first, pos, slots, pool = S.extend_tables(
+        [[7, -1], [-1, -1], [3, -1]], [15, 0, 3], [2, 17, 1], [0, 1, 2], [2, 2, 0, 0], 16, 22)
+    assert t == [[7, 2], [-1, -1], [3, -1]]     # request 1 needs two pages, one is left
+    assert (starts, lens, first) == ([0, 2, 19, 20], [17, 0, 4], [15, -1, 3])
+    # pages 7 and 3 are not of a cache of three pages
+    assert slots == [-1, 32] + [-1] * 20 and pool == [0, 1, 1, 0]
+    assert pos[:2] == [15, 16] and pos[19] == 3
+    t, starts, lens, first, pos, slots, pool = S.extend_tables(
+        [[7, -1], [-1, -1], [3, -1]], [15, 0, 3], [2, 17, 1], [0, 1, 2, 9, 9, 9, 9, 9], [1, 2, 0, 0], 16, 22)
+    assert slots == [7 * 16 + 15, 16] + [-1] * 17 + [51, -1, -1] and pool == [2, 1, 1, 0]
+
+
+# --- refusals of the C ABI (CPU) -----------------------------------------------------
+
+P8 = 0x1000  # a 16-byte aligned address that is never read: validation comes first
+
+
+def _append_args(**kw):
+    a = dict(qkv=P8, dtype=_lib.PMI_F16, stride=6 * 128, cos=P8, sin=P8, L=8, positions=P8, slots=P8, q=P8, k=P8,
+             v=P8, ks=P8, vs=P8, code=_lib.PMI_I8, pages=4, ps=16, T=2, H=4, KV=1, D=128)
+    a.update(kw)
+    return [*a.values(), None]
+
+
+def _attention_args(**kw):
+    a = dict(q=P8, dtype=_lib.PMI_F16, stride=512, head=128, k=P8, v=P8, ks=P8, vs=P8, code=_lib.PMI_I8, pages=4, ps=16,
+             tables=P8, tstride=4, lens=P8, starts=P8, out=P8, T=2, R=1, width=4, H=4, KV=1, D=128, max_q=2,
+             max_kv=64, window=0, scale=1.0, ws=P8, ws_bytes=1 << 40)
+    a.update(kw)
+    return [*a.values(), None]
+
+
+@pytest.mark.parametrize("change", [dict(dtype=_lib.PMI_F32), dict(code=_lib.PMI_U8), dict(ps=24), dict(ps=0),
+                                    dict(ps=512), dict(D=96), dict(H=5, KV=2), dict(KV=0), dict(stride=760),
+                                    dict(stride=772), dict(L=0), dict(T=-1), dict(T=1 << 31), dict(qkv=None),
+                                    dict(k=None), dict(v=P8 + 8), dict(q=P8 + 2), dict(pages=-1),
+                                    dict(pages=1 << 40), dict(slots=None), dict(L=1 << 40)])
+def test_append_refuses(change):
+    rc = _lib.lib().pmi_rope_append_kv(*_append_args(**change))
+    assert rc in (_lib.PMI_ERR_INVALID, _lib.PMI_ERR_UNSUPPORTED) and "pmi_rope_append_kv" in _lib.last_error()
+
+
+@pytest.mark.parametrize("change", [dict(dtype=_lib.PMI_F32), dict(code=_lib.PMI_F16), dict(ps=48), dict(D=80),
+                                    dict(H=6, KV=4), dict(H=65, KV=1), dict(stride=513), dict(head=4), dict(T=-1),
+                                    dict(R=-1), dict(width=5), dict(max_q=-1), dict(max_kv=-1), dict(window=-1),
+                                    dict(starts=None), dict(T=1 << 40), dict(width=1 << 40, tstride=1 << 40),
+                                    dict(max_kv=1 << 40), dict(max_q=1 << 40), dict(q=None), dict(q=P8 + 8),
+                                    dict(out=None), dict(lens=None), dict(tables=None), dict(k=None),
+                                    dict(window=1 << 40), dict(R=1 << 40)])
+def test_attention_refuses(change):
+    rc = _lib.lib().pmi_paged_attention(*_attention_args(**change))
+    assert rc in (_lib.PMI_ERR_INVALID, _lib.PMI_ERR_UNSUPPORTED) and "pmi_paged_attention" in _lib.last_error()
+
+
+def test_attention_without_its_workspace_is_refused():
+    L = _lib.lib()
+    need = L.pmi_paged_attention_workspace_bytes(2, 2, 4, 1, 128, 1, 100000, 0)
+    if need:
+        args = dict(starts=None, T=2, R=2, max_q=1, max_kv=100000, width=10000, tstride=10000)
+        for bad in (dict(ws=None), dict(ws_bytes=need - 1), dict(ws=P8 + 16)):
+            assert L.pmi_paged_attention(*_attention_args(**args, **bad)) == _lib.PMI_ERR_INVALID
+
+
+@pytest.mark.parametrize("change", [dict(R=-1), dict(R=4097), dict(width=9), dict(ring=-1), dict(ps=8), dict(total=-1),
+                                    dict(total=1 << 31), dict(width=1 << 40, stride=1 << 40), dict(ring=1 << 40),
+                                    dict(tables=None), dict(pool=None), dict(slots=None), dict(free=None)])
+def test_tables_refuse(change):
+    a = dict(tables=P8, stride=8, lens=P8, new=P8, free=P8, pool=P8, starts=P8, out=P8, first=P8, positions=P8,
+             slots=P8, pool_out=P8, R=2, width=8, ring=16, ps=16, total=2)
+    a.update(change)
+    rc = _lib.lib().pmi_extend_block_tables(*a.values(), None)
+    assert rc in (_lib.PMI_ERR_INVALID, _lib.PMI_ERR_UNSUPPORTED)
+    if not {"total", "slots"} & set(change):
+        a = dict(tables=P8, stride=8, lens=P8, done=P8, free=P8, pool=P8, R=2, width=8, ring=16, ps=16)
+        a.update(change)
+        rc = _lib.lib().pmi_release_block_tables(*a.values(), None)
+        assert rc in (_lib.PMI_ERR_INVALID, _lib.PMI_ERR_UNSUPPORTED)
+
+
+def test_empty_calls_do_nothing():
+    L = _lib.lib()
+    assert L.pmi_rope_append_kv(*_append_args(T=0, qkv=None)) == _lib.PMI_OK
+    assert L.pmi_paged_attention(*_attention_args(T=0)) == _lib.PMI_OK
+    assert L.pmi_paged_attention(*_attention_args(max_q=0)) == _lib.PMI_OK
+    assert L.pmi_read_kv_pages(None, P8, P8, P8, P8, _lib.PMI_I8, 4, 16, None, None, _lib.PMI_F16, 0, 1, 64,
+                               None) == _lib.PMI_OK
+    assert L.pmi_release_block_tables(P8, 8, P8, P8, P8, P8, 0, 8, 16, 16, None) == _lib.PMI_OK
+    assert L.pmi_read_kv_pages(P8, P8, P8, P8, P8, _lib.PMI_I8, 4, 16, P8, P8, _lib.PMI_U8, 1, 1, 64,
+                               None) == _lib.PMI_ERR_INVALID
+
+
+def test_cpu_tensors_raise():
+    i = torch.zeros(1, dtype=torch.int32)
+    k, v, s = torch.zeros(1, 1, 16, 64, dtype=torch.int8), torch.zeros(1, 1, 1, 64, 16, dtype=torch.int8), torch.zeros(1, 1)
+    with pytest.raises(RuntimeError, match="HIP"):
+        P.paged_attention(torch.zeros(1, 1, 64).half(), k, v, s, s, i[None], i, scale=1.0)
+    with pytest.raises(RuntimeError, match="HIP"):
+        P.rope_append_kv(torch.zeros(1, 192).half(), s, s, i, i, k, v, s, s)
+    with pytest.raises(RuntimeError, match="HIP"):
+        P.read_kv_pages(i, k, v, s, s)
+    with pytest.raises(RuntimeError, match="HIP"):
+        P.extend_block_tables(i[None], i, i, i, torch.zeros(4, dtype=torch.int32), 16, 1)
+    with pytest.raises(ValueError):
+        P.PagedKVCache(1, 1, 16, 1, 64, "cpu", dtype=torch.float16)
+
+
+# --- block tables --------------------------------------------------------------------
+
+def _random_tables(rng, R, ps, longest, newest, spare, width=None):
+    lens = [rng.choice([0, 1, ps - 1, ps, rng.randint(0, longest)]) for _ in range(R)]
+    new = [rng.choice([0, 1, 1, rng.randint(0, newest)]) for _ in range(R)]
+    held = [-(-n // ps) for n in lens]
+    width = width or max([-(-(a + b) // ps) for a, b in zip(lens, new)] + [1])
+    lens = [min(n, width * ps) for n in lens]
+    held = [-(-n // ps) for n in lens]
+    need = sum(-(-(a + b) // ps) - h for a, b, h in zip(lens, new, held))
+    pages = sum(held) + max(0, need + spare)
+    order = rng.sample(range(pages), pages)
+    tables, at = [[-1] * width for _ in range(R)], 0
+    for r, h in enumerate(held):
+        tables[r][:h] = order[at:at + h]
+        at += h
+    ring = max(pages, 1)
+    free, head = [0] * ring, rng.randrange(ring)
+    for i, page in enumerate(order[at:]):
+        free[(head + i) % ring] = page
+    return tables, lens, new, free, [head, pages - at, 3, 0]
+
+
+@gpu
+@pytest.mark.parametrize("R,ps,longest,newest,spare,width", [
+    (1, 16, 0, 1, 0, None), (1, 64, 500, 300, 0, None), (48, 64, 4000, 3, 5, None), (70, 16, 200, 90, 4, None),
+    (70, 16, 200, 90, -20, None), (33, 32, 400, 900, -50, 12), (1025, 16, 40, 5, 0, None),
+    (4096, 128, 3000, 2, -7, None), (300, 256, 1000, 700, 9, None)])
+def test_extend_block_tables(R, ps, longest, newest, spare, width):
+    """Every output against the oracle's integers: pools that are too small, rows that are
+    too short, more tokens than one workgroup looks up, tokens behind the last request."""
+    rng = random.Random(R * ps + newest)
+    tables, lens, new, free, pool = _random_tables(rng, R, ps, longest, newest, spare, width)
+    total = sum(new) + rng.randint(0, 5)
+    want = S.extend_tables(tables, lens, new, free, pool, ps, total)
+    wide = torch.full((R, len(tables[0]) + 3), -9, dtype=torch.int32, device=DEV)  # rows of a larger table
+    t = wide[:, :len(tables[0])]
+    t.copy_(_ints(tables))
+    args = (_ints(lens), _ints(new), _ints(free), _ints(pool))
+    plan = P.extend_block_tables(t, *args, ps, total)
+    got = (t, plan.q_starts, plan.kv_lens, plan.first, plan.positions, plan.slots, plan.pool)
+    for name, g, w in zip(("tables", "q_starts", "kv_lens", "first", "positions", "slots", "pool"), got, want):
+        assert g.tolist() == w, name
+    assert (wide[:, len(tables[0]):] == -9).all()
+    assert args[0].tolist() == lens and args[3].tolist() == pool
+    # in place
+    t.copy_(_ints(tables))
+    again = P.extend_block_tables(t, *args, ps, total, kv_lens_out=args[0], pool_out=args[3])
+    assert args[0].tolist() == want[2] and args[3].tolist() == want[6]
+    assert again.slots.tolist() == want[5] and t.tolist() == want[0]
+
+
+@gpu
+def test_extend_with_negative_lengths_and_strange_pools():
+    """Lengths below zero count as zero; a head or count that no pool has, and table
+    entries outside the cache, lead to no slot outside it."""
+    t = _ints([[5, -1, 99], [-1, -1, -1]])
+    plan = P.extend_block_tables(t, _ints([-4, 3]), _ints([2, -1]), _ints([1, 0, 2]), _ints([77, 50, 0, 0]), 16, 2)
+    assert plan.q_starts.tolist() == [0, 2, 2] and plan.slots.tolist() == [16, 17]
+    plan = P.extend_block_tables(t, _ints([33, 0]), _ints([1, 0]), _ints([1, 0, 2]), _ints([0, 3, 0, 0]), 16, 1)
+    assert plan.slots.tolist() == [-1]  # its page is 99
+    none = P.extend_block_tables(t[:0], _ints([]), _ints([]), _ints([]), _ints([0, 0, 0, 0]), 16, 3)
+    assert none.slots.tolist() == [-1] * 3 and none.q_starts.tolist() == [0]
+
+
+@gpu
+@pytest.mark.parametrize("R,ps", [(1, 16), (37, 32), (1500, 16)])
+def test_extend_and_release_keep_every_page_once(R, ps):
+    """Requests that grow, end and start again: no page is ever held twice, and every
+    page is in a table or in the ring."""
+    rng = random.Random(R)
+    c = P.PagedKVCache(0, R, 40 * ps, 1, 64, DEV, page_size=ps, pages=R * 12)
+    pages = R * 12
+    for step in range(12):
+        new = [rng.choice([0, 1, rng.randint(0, 4 * ps)]) for _ in range(R)]
+        c.extend(_ints(new), sum(new))
+        done = torch.tensor([rng.random() < 0.3 for _ in range(R)], device=DEV)
+        held_before = c.kv_lens.tolist()
+        c.release(done)
+        lens, pool = c.kv_lens.tolist(), c.pool.tolist()
+        assert lens == [0 if d else n for n, d in zip(held_before, done.tolist())]
+        rows, free = c.block_tables.tolist(), c.free_pages.tolist()
+        held = [p for row, n in zip(rows, lens) for p in row[:-(-n // ps)]]
+        loose = [free[(pool[0] + i) % pages] for i in range(pool[1])]
+        assert sorted(held + loose) == list(range(pages)), step
+
+
+# --- the write and the read ----------------------------------------------------------
+
+def _rope(L, D):
+    inv = 1.0 / 10000.0 ** (np.arange(0, D, 2) / D)
+    a = np.arange(L)[:, None] * inv
+    return np.cos(a).astype(np.float32), np.sin(a).astype(np.float32)
+
+
+def _check_cache(c, k, v, ks, vs, where=""):
+    np.testing.assert_array_equal(ks.cpu().numpy(), c.scales[0], err_msg="k_scale " + where)
+    np.testing.assert_array_equal(vs.cpu().numpy(), c.scales[1], err_msg="v_scale " + where)
+    np.testing.assert_array_equal(k.cpu().view(torch.uint8).numpy(), c.codes[0], err_msg="k codes " + where)
+    np.testing.assert_array_equal(S.token_major(v), c.codes[1], err_msg="v codes " + where)
+
+
+@gpu
+@pytest.mark.parametrize("code", CODES)
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("H,KV,D,ps", [(1, 1, 64, 16), (8, 2, 128, 64), (7, 1, 128, 32), (4, 4, 64, 128),
+                                       (6, 3, 128, 256)])
+def test_append_equals_the_oracle_bit_for_bit(code, dtype, H, KV, D, ps):
+    """Prompts of odd lengths, then single tokens whose values grow (the pages' older
+    codes are rounded again), then a mix; refused tokens and slots outside the cache are
+    skipped. Scales and codes are one IEEE operation after another: equal bits."""
+    rng = np.random.default_rng(H * D + ps)
+    pages = 14
+    c = S.Cache(pages, KV, ps, D, code)
+    for i in range(2):  # old bytes nobody wrote
+        c.codes[i][:] = rng.integers(0, 127, c.codes[i].shape)
+        c.scales[i][:] = rng.uniform(0.5, 1, c.scales[i].shape)
+    k, v, ks, vs = c.tensors(DEV)
+    cos, sin = _rope(4 * ps, D)
+    tcos, tsin = torch.from_numpy(cos).to(DEV), torch.from_numpy(sin).to(DEV)
+    perm = rng.permutation(pages)
+    rows = perm[:12].reshape(3, 4)
+    lens = [0, 0, 0]
+    steps = [[ps + 5, 3, 0], [1, 1, 1], [1, 1, 1], [1, 0, 1], [ps - 6, 2, 17 if ps > 16 else 9], [1, 1, 1]]
+    for step, new in enumerate(steps):
+        positions = np.concatenate([np.arange(a, a + n) for a, n in zip(lens, new)] + [[0, 0]]).astype(np.int32)
+        slots = np.concatenate([rows[r][np.arange(a, a + n) // ps] * ps + np.arange(a, a + n) % ps
+                                for r, (a, n) in enumerate(zip(lens, new))] + [[-1, pages * ps]]).astype(np.int32)
+        lens = [a + n for a, n in zip(lens, new)]
+        x = torch.from_numpy(rng.standard_normal((len(slots), (H + 2 * KV) * D)) * (1 + step)).to(dtype)
+        wide = torch.zeros(len(slots), (H + 2 * KV) * D + 8, dtype=dtype, device=DEV)
+        wide[:, :-8] = x.to(DEV)
+        q = P.rope_append_kv(wide[:, :-8], tcos, tsin, torch.from_numpy(positions).to(DEV),
+                             torch.from_numpy(slots).to(DEV), k, v, ks, vs)
+        want = c.append(x.float().numpy(), cos, sin, positions, slots, H)
+        assert torch.equal(q.cpu(), torch.from_numpy(want).to(dtype)), step
+        _check_cache(c, k, v, ks, vs, f"step {step}")
+    some = torch.tensor([int(perm[0]), pages, -1, int(perm[5])], dtype=torch.int32, device=DEV)
+    for out in (torch.float16, torch.bfloat16, torch.float32):
+        rk, rv = P.read_kv_pages(some, k, v, ks, vs, dtype=out)
+        for got, i in ((rk, 0), (rv, 1)):
+            val = (S.decode(c.codes[i], code) * c.scales[i][..., None, None])[[perm[0], perm[5]]]
+            assert torch.equal(got[[0, 3]].cpu(), torch.from_numpy(val).to(out))
+            assert (got[[1, 2]] == 0).all()
+
+
+@gpu
+@pytest.mark.parametrize("code", CODES)
+def test_append_against_64_bits(code):
+    """Codes times scales against the rotation in 64 bits: half a code, and 2^-20 of the
+    largest for the fp32 rotation and division (a few roundings of 2^-24 each)."""
+    H, KV, D, ps, T = 4, 2, 128, 64, 150
+    g = torch.Generator().manual_seed(1)
+    qkv = torch.randn(T, (H + 2 * KV) * D, generator=g).half()
+    cos, sin = _rope(T, D)
+    c = P.PagedKVCache(1, 1, T, KV, D, DEV, page_size=ps, dtype=code)
+    plan = c.extend(_ints([T]), T)
+    q = c.append(0, qkv.to(DEV), torch.from_numpy(cos).to(DEV), torch.from_numpy(sin).to(DEV), plan)
+    x = qkv.double().numpy().reshape(T, H + 2 * KV, D)
+    turned = S.rotate(x[:, :H + KV], cos.astype(np.float64), sin.astype(np.float64))
+    assert np.abs(q.cpu().double().numpy() - turned[:, :H]).max() <= np.abs(turned).max() * (2 ** -11 + 2 ** -20)
+    k, v = P.read_kv_pages(c.block_tables[0], c.k[0], c.v[0], c.k_scale[0], c.v_scale[0], dtype=torch.float32)
+    for got, want in ((k, turned[:, H:]), (v, x[:, H + KV:])):
+        got = got.transpose(1, 2).reshape(-1, KV, D)[:T].cpu().double().numpy()
+        for page in range(-(-T // ps)):
+            a, b = got[page * ps:(page + 1) * ps], want[page * ps:min(T, (page + 1) * ps)]
+            top = np.abs(b).max((0, 2), keepdims=True)
+            half = top / 254 if code == torch.int8 else np.maximum(np.abs(b) * 2.0 ** -4, top / 448 * 2.0 ** -10)
+            assert (np.abs(a[:len(b)] - b) <= half + top * 2.0 ** -20).all()
+
+
+@gpu
+@pytest.mark.parametrize("bad", [float("inf"), float("-inf"), float("nan")])
+def test_append_shows_infinities_and_nan_in_their_page_and_head_only(bad):
+    KV, D, ps = 2, 64, 16
+    c = P.PagedKVCache(1, 1, 48, KV, D, DEV, page_size=ps)
+    g = torch.Generator(device=DEV).manual_seed(2)
+    qkv = torch.randn(40, 4 * KV * D // 2 * 1 + KV * D, generator=g, device=DEV).half()
+    H = qkv.shape[1] // D - 2 * KV
+    qkv[20, (H + KV) * D + 5] = bad  # v of head 0, second page
+    cos, sin = (torch.from_numpy(t).to(DEV) for t in _rope(48, D))
+    plan = c.extend(_ints([40]), 40)
+    c.append(0, qkv, cos, sin, plan)
+    page = c.block_tables[0].long()
+    finite = torch.isfinite(c.v_scale[0][page])
+    assert finite.tolist() == [[True, True], [False, True], [True, True]]
+    assert torch.isfinite(c.k_scale[0]).all()
+
+
+# --- attention -------------------------------------------------------------------------
+
+HALF = {torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}
+
+
+def _attention_case(code, dtype, H, KV, D, ps, lens, new, window=0, seed=0, width=None, spread=2.0):
+    """Inputs on the device, and (o, weight) in 64 bits."""
+    rng = np.random.default_rng(seed)
+    need = [-(-n // ps) for n in lens]
+    pages = sum(need) + 3
+    c = S.Cache(pages, KV, ps, D, code)
+    c.fill(rng)
+    order = rng.permutation(pages)
+    width = width or max(need + [1]) + 1
+    tables = rng.integers(0, pages, (len(lens), width)).astype(np.int32)  # entries past a request's end: any page
+    at = 0
+    for r, n in enumerate(need):
+        tables[r, :n] = order[at:at + n]
+        at += n
+    starts = np.concatenate([[0], np.cumsum(new)]).astype(np.int32)
+    q = torch.from_numpy(rng.standard_normal((int(starts[-1]), H, D)) * spread).to(dtype)
+    return c, tables, starts, q
+
+
+def _tolerance(o, weight, dtype):
+    """Half a step of the output's type, and of the probabilities': the kernels hold them
+    in fp16 (2^-11), from scores whose fp32 sums over at most 128 products are off by less
+    than 2^-13 here (|q| |k| scale sums to 14, times 130 2^-24), twice for numerator and sum."""
+    return HALF[dtype] * np.abs(o) + (2.0 ** -11 + 2.0 ** -12) * weight + 2.0 ** -25
+
+
+def _check(got, o, weight, dtype, what=""):
+    err = np.abs(got.double().cpu().numpy() - o)
+    bad = err > _tolerance(o, weight, dtype)
+    assert not bad.any(), f"{what} {bad.sum()} of {bad.size} off, at most {err.max():.3e} at {np.argwhere(bad)[0]}"
+
+
+def _run(c, tables, lens, starts, q, window=0, decode=None, **kw):
+    k, v, ks, vs = c.tensors(DEV)
+    new = np.diff(starts)
+    if decode is None:
+        decode = bool((new == 1).all())
+    return P.paged_attention(q.to(DEV), k, v, ks, vs, torch.from_numpy(tables).to(DEV), _ints(lens),
+                             None if decode else torch.from_numpy(starts).to(DEV), scale=1 / q.shape[-1] ** 0.5,
+                             window=window, max_q_len=int(max(new)), **kw)
+
+
+def _oracle(c, tables, lens, starts, q, window=0):
+    return S.attention(q.double().numpy(), c.values(0), c.values(1), tables, lens, starts, c.ps,
+                       1 / q.shape[-1] ** 0.5, window)
+
+
+HEADS = [(1, 1, 64, 16), (4, 1, 128, 64), (32, 8, 128, 64), (7, 1, 128, 128), (8, 8, 64, 32), (14, 2, 64, 256),
+         (16, 1, 128, 16), (40, 2, 128, 64), (64, 1, 64, 32)]
+
+
+@gpu
+@pytest.mark.parametrize("code", CODES)
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("H,KV,D,ps", HEADS)
+def test_decode_attention(code, dtype, H, KV, D, ps):
+    """One token for each of a ragged batch: lengths of one, around a page, a tile and a
+    split, and a request of length zero (whose row is zeros)."""
+    lens = [1, 2, ps - 1, ps, ps + 1, 63, 64, 65, 255, 257, 0, 700]
+    case = _attention_case(code, dtype, H, KV, D, ps, lens, [1] * len(lens), seed=H + D + ps)
+    got = _run(case[0], case[1], lens, case[2], case[3])
+    _check(got, *_oracle(case[0], case[1], lens, case[2], case[3]), dtype)
+    assert (got[10] == 0).all()
+    # the same with the starts given
+    assert torch.equal(got, _run(case[0], case[1], lens, case[2], case[3], decode=False))
+
+
+@gpu
+@pytest.mark.parametrize("lens", [[5000], [20000, 3], [1023, 4097, 2048, 9001]])
+def test_decode_attention_of_long_contexts(lens):
+    """Several splits of one sequence, joined; bit-identical when repeated."""
+    for code, dtype in ((CODES[0], torch.float16), (CODES[1], torch.bfloat16)):
+        case = _attention_case(code, dtype, 8, 2, 128, 64, lens, [1] * len(lens), seed=sum(lens))
+        got = _run(case[0], case[1], lens, case[2], case[3])
+        _check(got, *_oracle(case[0], case[1], lens, case[2], case[3]), dtype)
+        assert torch.equal(got, _run(case[0], case[1], lens, case[2], case[3]))
+
+
+@gpu
+@pytest.mark.parametrize("window", [1, 16, 63, 64, 65, 300, 5000])
+def test_windows(window):
+    lens = [1, 64, 130, 700, 0, 2000]
+    case = _attention_case(CODES[0], torch.float16, 8, 2, 128, 32, lens, [1] * len(lens), seed=window)
+    _check(_run(case[0], case[1], lens, case[2], case[3], window=window),
+           *_oracle(case[0], case[1], lens, case[2], case[3], window), torch.float16)
+    new = [1, 64, 30, 5, 0, 3]
+    case = _attention_case(CODES[1], torch.float16, 8, 2, 64, 32, lens, new, seed=window)
+    _check(_run(case[0], case[1], lens, case[2], case[3], window=window),
+           *_oracle(case[0], case[1], lens, case[2], case[3], window), torch.float16)
+
+
+@gpu
+@pytest.mark.parametrize("code", CODES)
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("H,KV,D,ps", HEADS)
+def test_prompt_attention(code, dtype, H, KV, D, ps):
+    """Prompts of odd lengths from nothing, behind a context, of no tokens, and (a refused
+    request's shape) with fewer keys than queries, whose first rows see nothing."""
+    new = [1, 17, 0, 64, 33, 20, 90]
+    lens = [1, 17, 40, 64, 300, 7, 129]
+    case = _attention_case(code, dtype, H, KV, D, ps, lens, new, seed=H * D + ps)
+    got = _run(case[0], case[1], lens, case[2], case[3])
+    _check(got, *_oracle(case[0], case[1], lens, case[2], case[3]), dtype)
+    a = int(case[2][5])
+    assert (got[a:a + 13] == 0).all() and (got[a + 13] != 0).any()
+
+
+@gpu
+@pytest.mark.parametrize("new,lens", [([300], [300]), ([257, 5], [1300, 4000]), ([3] * 5, [100, 3, 64, 2500, 65]),
+                                      ([8, 2], [513, 6000])])
+def test_longer_prompts_and_several_tokens(new, lens):
+    """Tiles on and off the diagonal, a few tokens over long contexts."""
+    for code, dtype in ((CODES[0], torch.bfloat16), (CODES[1], torch.float16)):
+        case = _attention_case(code, dtype, 8, 2, 128, 64, lens, new, seed=sum(lens))
+        _check(_run(case[0], case[1], lens, case[2], case[3]),
+               *_oracle(case[0], case[1], lens, case[2], case[3]), dtype)
+
+
+@gpu
+def test_attention_takes_strided_queries_and_leaves_rows_behind_the_last():
+    lens, new = [70, 9], [5, 2]
+    c, tables, starts, q = _attention_case(CODES[0], torch.float16, 4, 2, 64, 16, lens, new)
+    o, weight = _oracle(c, tables, lens, starts, q)
+    k, v, ks, vs = c.tensors(DEV)
+    wide = torch.full((10, 8, 72), 3.0, dtype=torch.float16, device=DEV)
+    view = wide[:, ::2, :64]
+    view[:7] = q.to(DEV)
+    out = torch.full((10, 4, 64), 7.0, dtype=torch.float16, device=DEV)
+    args = (k, v, ks, vs, torch.from_numpy(tables).to(DEV), _ints(lens), torch.from_numpy(starts).to(DEV))
+    got = P.paged_attention(view, *args, scale=1 / 8, max_q_len=5, out=out)
+    assert got is out and (out[7:] == 7).all()
+    _check(out[:7], o, weight, torch.float16)
+    # odd strides and an odd start go through a copy
+    odd = torch.empty(7 * 4 * 67 + 1, dtype=torch.float16, device=DEV)[1:].view(7, 4, 67)[:, :, :64]
+    odd.copy_(q.to(DEV))
+    assert torch.equal(P.paged_attention(odd, *args, scale=1 / 8, max_q_len=5), out[:7])
+    # heads first, as an attention of another framework lays them out
+    first = q.to(DEV).transpose(0, 1).contiguous().transpose(0, 1)
+    assert torch.equal(P.paged_attention(first, *args, scale=1 / 8, max_q_len=5), out[:7])
+
+
+@gpu
+@pytest.mark.parametrize("new", [1, 40])
+@pytest.mark.parametrize("code", CODES)
+def test_attention_ignores_what_lies_behind_a_sequence(code, new):
+    """Bytes that are NaN as e4m3, and scales that are infinite or NaN, in the tokens behind
+    a sequence's end, in the pages behind it and in tokens before the window: no trace."""
+    lens, ps = [50, 131, 64], 32
+    c, tables, starts, q = _attention_case(code, torch.float16, 4, 1, 128, ps, lens, [min(new, n) for n in lens],
+                                           width=8)
+    clean = _run(c, tables, lens, starts, q, window=40)
+    pages = c.codes[0].shape[0]
+    used = {int(tables[r, p // ps]) for r, n in enumerate(lens) for p in range(max(0, n - new - 39), n)}
+    for r, n in enumerate(lens):
+        if n % ps:
+            for i in range(2):
+                c.codes[i][tables[r, n // ps], :, n % ps:] = 0x7F
+    for page in set(range(pages)) - used:
+        for i in range(2):
+            c.codes[i][page] = 0xFF
+            c.scales[i][page] = [np.nan, np.inf][page % 2]
+    assert torch.equal(_run(c, tables, lens, starts, q, window=40), clean)
+
+
+@gpu
+@pytest.mark.parametrize("new", [[1, 1, 1], [9, 20, 1]])
+def test_attention_skips_pages_outside_the_cache(new):
+    """Table entries outside the cache (a request that was refused pages): their tokens are
+    as if they were not there."""
+    lens = [100, 300, 70]
+    c, tables, starts, q = _attention_case(CODES[0], torch.float16, 4, 2, 64, 32, lens, new)
+    tables[0, 1], tables[1, 4], tables[1, 0] = -1, 1 << 30, c.codes[0].shape[0]
+    tables[2, :3] = -5
+    got = _run(c, tables, lens, starts, q)
+    _check(got, *_oracle(c, tables, lens, starts, q), torch.float16)
+    assert (got[int(starts[2]):] == 0).all()
+
+
+@gpu
+@pytest.mark.parametrize("new", [1, 24])
+def test_attention_of_peaked_and_large_scores(new):
+    """Scores of several hundred (one position takes all), a scale of zero (all alike) and
+    pages whose values are 10^4 times another's."""
+    lens = [200, 513]
+    n = [min(new, x) for x in lens]
+    c, tables, starts, q = _attention_case(CODES[0], torch.float16, 4, 2, 128, 16, lens, n, spread=60.0)
+    got = _run(c, tables, lens, starts, q)
+    o, weight = _oracle(c, tables, lens, starts, q)
+    # scores are 30 times the other tests': their fp32 sums are off by up to 30 * 2^-13
+    err = np.abs(got.double().cpu().numpy() - o)
+    # (below 2^-14 a step of fp16 is 2^-24, however small the value: half of it, as in _tolerance)
+    assert (err <= HALF[torch.float16] * np.abs(o) + (2.0 ** -11 + 30 * 2.0 ** -12) * weight + 2.0 ** -25).all()
+    k, v, ks, vs = c.tensors(DEV)
+    c.scales[1][::2] *= np.float32(1e4)
+    c.scales[1][1::5] = 0
+    vs = torch.from_numpy(c.scales[1]).to(DEV)
+    flat = P.paged_attention(q.to(DEV).float().clamp(-4, 4).half(), k, v, ks, vs, torch.from_numpy(tables).to(DEV),
+                             _ints(lens), torch.from_numpy(starts).to(DEV), scale=0.0, max_q_len=max(n))
+    o, weight = S.attention(np.zeros(q.shape), c.values(0), c.values(1), tables, lens, starts, 16, 0.0)
+    fits = np.abs(o) < 65000
+    err = np.abs(flat.double().cpu().numpy() - o)
+    assert (err <= _tolerance(o, weight, torch.float16))[fits].all()
+
+
+@gpu
+def test_shared_pages_and_bounds_that_are_too_large():
+    """Two requests with a common prefix's pages, limits far above what is there."""
+    lens, new = [100, 101], [1, 1]
+    c, tables, starts, q = _attention_case(CODES[0], torch.float16, 4, 2, 128, 64, lens, new, width=40)
+    tables[1] = tables[0]
+    want = _oracle(c, tables, lens, starts, q)
+    for kw in (dict(), dict(max_kv_len=101), dict(max_kv_len=1 << 20)):
+        _check(_run(c, tables, lens, starts, q, **kw), *want, torch.float16)
+    k, v, ks, vs = c.tensors(DEV)
+    got = P.paged_attention(q.to(DEV), k, v, ks, vs, torch.from_numpy(tables).to(DEV), _ints(lens),
+                            torch.from_numpy(starts).to(DEV), scale=1 / 128 ** 0.5, max_q_len=1000)
+    _check(got, *want, torch.float16)
+
+
+@gpu
+def test_python_checks():
+    c, tables, starts, q = _attention_case(CODES[0], torch.float16, 4, 2, 64, 16, [20], [1])
+    k, v, ks, vs = c.tensors(DEV)
+    t, lens, q = torch.from_numpy(tables).to(DEV), _ints([20]), q.to(DEV)
+    ok = dict(scale=0.1)
+    for args in ((q.float(), k, v, ks, vs, t, lens), (q, k, v[:, :, :, :32], ks, vs, t, lens),
+                 (q, k, v, ks[:1], vs, t, lens), (q, k, v.view(torch.uint8), ks, vs, t, lens),
+                 (q, k, v, ks, vs, t.long(), lens), (q, k, v, ks, vs, t, lens.long()),
+                 (q[..., :32], k, v, ks, vs, t, lens), (q.expand(2, 4, 64), k, v, ks, vs, t, lens)):
+        with pytest.raises(AssertionError):
+            P.paged_attention(*args, **ok)
+    with pytest.raises(RuntimeError):
+        P.paged_attention(q, k, v, ks, vs, t.cpu(), lens, **ok)
+    with pytest.raises(AssertionError):
+        P.paged_attention(q, k, v, ks, vs, t, lens, out=q[..., :32], **ok)
+    with pytest.raises(AssertionError):
+        P.extend_block_tables(t, lens, lens.long(), lens, _ints([0, 0, 0, 0]), 16, 1)
+    with pytest.raises(_lib.PmiError):
+        P.extend_block_tables(t, lens, lens, lens, _ints([0, 0, 0, 0]), 24, 1)
