@@ -645,7 +645,8 @@ PMI_API int pmi_read_kv_pages(const int32_t* pages, const void* k_cache, const v
  * n + i, and with window > 0 only the last `window` of them. A query that sees
  * nothing gives zeros; rows of out from q_starts[R] on stay as they were.
  * max_q and max_kv bound the queries and keys of a request (of a longer one the
- * queries past max_q stay unwritten, and keys past max_kv unread); H / KV <= 64.
+ * queries past max_q stay unwritten, and keys past max_kv unread); H / KV <= 64;
+ * width * page_size <= 2^30.
  * workspace: device scratch of pmi_paged_attention_workspace_bytes() bytes for
  * the same sizes, 256-byte aligned, its first 64 KiB zero before its first use
  * (every call leaves them zero). Calls that may run concurrently must not share it. */

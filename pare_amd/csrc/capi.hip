@@ -1490,7 +1490,7 @@ int pmi_paged_attention(const void* q, int dtype, int64_t q_stride, int64_t q_he
   if (q_stride % 8 != 0 || q_head_stride % 8 != 0)
     return fail(PMI_ERR_INVALID, "%s: the strides of q must be multiples of 8 elements", fn);
   if (T == 0 || R == 0 || max_q == 0) return ok();
-  if (T >= (1ll << 31) / H || R >= (1ll << 31) / KV || width >= (1ll << 31) / page_size || max_kv >= (1ll << 31) ||
+  if (T >= (1ll << 31) / H || R >= (1ll << 31) / KV || width > (1ll << 30) / page_size || max_kv >= (1ll << 31) ||
       max_q >= (1ll << 31) / (H / KV) || window >= (1ll << 31))
     return fail(PMI_ERR_UNSUPPORTED, "%s: too large", fn);
   if (!q || !out || !kv_lens || (width && !tables)) return fail(PMI_ERR_INVALID, "%s: null buffer", fn);
@@ -1500,7 +1500,8 @@ int pmi_paged_attention(const void* q, int dtype, int64_t q_stride, int64_t q_he
                            max_q, max_kv, window, scale, dtype == PMI_BF16};
   const pmi::PagedCache c = {const_cast<void*>(k_cache), const_cast<void*>(v_cache), const_cast<float*>(k_scale),
                              const_cast<float*>(v_scale), n_pages, KV, page_size, D, code_dtype == PMI_F8};
-  const size_t need = pmi_paged_attention_workspace_bytes(T, R, H, KV, D, max_q, max_kv, window);
+  if (p.max_kv > width * page_size) p.max_kv = width * page_size;
+  const size_t need = pmi_paged_attention_workspace_bytes(T, R, H, KV, D, max_q, p.max_kv, window);
   if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 256)))
     return fail(PMI_ERR_INVALID, "%s: needs a 256-byte aligned workspace of %zu bytes", fn, need);
   return from_hip(pmi::launch_paged_attention(p, c, workspace, workspace_bytes, (hipStream_t)stream), fn);
