@@ -121,6 +121,17 @@ PMI_DEV float sum_over_h(float v) {
   return v + __shfl_xor(v, 32);
 }
 
+// (m, l, o) joined with another part of the same row; a part that saw no key is left out.
+PMI_DEV void join(float& m, float& l, f32x4& o, float pm, float pl, f32x4 po, bool use) {
+  use = use && !(pm == -INFINITY && pl == 0.f);
+  const float nm = fmaxf(m, pm);
+  const float fo = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - nm), fn = __builtin_amdgcn_exp2f(pm - nm);
+  l = use ? fmaf(l, fo, pl * fn) : l;
+#pragma unroll
+  for (int x = 0; x < 4; ++x) o[x] = use ? fmaf(o[x], fo, po[x] * fn) : o[x];
+  m = use ? nm : m;
+}
+
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kPBias = 16384.f;  // probabilities are held in fp16 times this
 
@@ -138,7 +149,7 @@ constexpr float kPBias = 16384.f;  // probabilities are held in fp16 times this
 // and 2^14, so that they use fp16's range from the top.
 // Sixteen-token blocks of a range are looked up 64 at a time, a lane a block.
 constexpr int kChunk = 1024;  // tokens per look-up
-constexpr int64_t kFewWgs = 4096;
+constexpr int64_t kFewWgs = 1024;
 
 template <typename T, int D, bool FP8>
 __global__ __launch_bounds__(256, 2) void attention_few_kernel(AttnArgs a) {
@@ -188,24 +199,68 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(AttnArgs a) {
   const int32_t* table = a.tables + (int64_t)r * a.stride;
   const int64_t cell_bytes = (int64_t)a.ps * D;
 
-  for (int c0 = p0; c0 < p1; c0 += kChunk) {
-    const int c1 = min(p1, c0 + kChunk);
-    // block `l` of the chunk
+  // The blocks of a chunk: lane l holds the page and the scales of block l. Pages are
+  // looked up two chunks ahead and scales one, so that no tile waits for a look-up.
+  auto look_up = [&](int c0) {
     const int bp = c0 + 16 * l;
-    int page = bp < c1 ? table[bp >> a.ps_log] : -1;
-    const bool there = (unsigned)page < a.n_pages;
-    page = there ? page : 0;
-    const int64_t bcell = (int64_t)page * a.KV + kh;
-    float bks = 0.f, bvs = 0.f;
+    return bp < p1 ? table[bp >> a.ps_log] : -1;
+  };
+  struct Blocks {
+    int page;  // -1: outside the cache, or past the range
+    float ks, vs;
+    // Of all blocks, the same in every lane: only shifted by uniform amounts. A 64-bit shift by
+    // a vector register that is the last of the wave's allocation has given wrong lanes here
+    // (v_lshlrev_b64 with its amount in v127 of 128).
+    uint64_t absent;
+  };
+  auto blocks_of = [&](int entry) {
+    const bool there = (unsigned)entry < a.n_pages;
+    Blocks x = {there ? entry : -1, 0.f, 0.f, ~__ballot(there)};
     if (there) {
-      bks = a.k_scale[bcell];
-      bvs = a.v_scale[bcell];
+      const int64_t cell = (int64_t)x.page * a.KV + kh;
+      x.ks = a.k_scale[cell];
+      x.vs = a.v_scale[cell];
     }
-    const uint64_t absent = ~__ballot(there);
-    float top = bvs < INFINITY ? bvs : 0.f;
+    return x;
+  };
+  u32x4 kw[D / 16], vw[DT];
+  // pages are read where they are there, page 0 of the cache elsewhere (and masked)
+  auto load_k = [&](int page, int p) {
+    const int b = (((p - p0) >> 4) & 63) + ((l >> 2) & 3);
+    const int64_t cell = (int64_t)max(__shfl(page, b), 0) * a.KV + kh;
+    const int tok = ((p + 16 * ((l >> 2) & 3)) & (a.ps - 1)) + (l & 3);
+    const uint8_t* at = a.k + cell * cell_bytes + tok * D + 16 * h;
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
-    {
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int j = 0; j < D / 64; ++j)
+        kw[t * (D / 64) + j] = *reinterpret_cast<const u32x4*>(at + 4 * t * D + 64 * j);
+  };
+  auto load_v = [&](int page, int p) {
+    const int b = (((p - p0) >> 4) & 63) + h;
+    const int64_t cell = (int64_t)max(__shfl(page, b), 0) * a.KV + kh;
+    const int blk = ((p + 16 * h) & (a.ps - 1)) >> 4;
+    const uint8_t* at = a.v + cell * cell_bytes + (blk * D + c) * 16;
+#pragma unroll
+    for (int d = 0; d < DT; ++d) vw[d] = *reinterpret_cast<const u32x4*>(at + 256 * d);
+  };
+  int p = p0 + 64 * wave;
+  int entry1 = look_up(p0 + kChunk);
+  Blocks cur = blocks_of(look_up(p0)), next = cur;
+  float vinv = 0.f;
+  if (p < p1) {
+    load_k(cur.page, p);
+    load_v(cur.page, p);
+  }
+  for (; p < p1; p += 256) {
+    if (((p - p0) & (kChunk - 1)) < 256) {  // this wave's first tile of a chunk
+      if (p - p0 >= kChunk) cur = next;
+      const int c0 = (p - p0) / kChunk * kChunk + p0;
+      next = blocks_of(entry1);
+      entry1 = look_up(c0 + 2 * kChunk);
+      float top = cur.vs < INFINITY ? cur.vs : 0.f;
+#pragma unroll
+      for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
       const float now = fmaxf(vref, top);
       if (now > vref && vref > 0.f) {
         const float f = vref / now;
@@ -213,99 +268,71 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(AttnArgs a) {
         for (int d = 0; d < DT; ++d) acc[d] *= f;
       }
       vref = now;
+      vinv = vref > 0.f ? kPBias / vref : 0.f;
     }
-    const float vinv = vref > 0.f ? kPBias / vref : 0.f;
-
-    u32x4 kw[D / 16], vw[DT];
-    // pages are read where they are there, page 0 of the cache elsewhere (and masked)
-    auto load_k = [&](int p) {
-      const int b = ((p - c0) >> 4) + ((l >> 2) & 3);
-      const int64_t cell = (int64_t)__shfl(page, b) * a.KV + kh;
-      const int tok = ((p + 16 * ((l >> 2) & 3)) & (a.ps - 1)) + (l & 3);
-      const uint8_t* at = a.k + cell * cell_bytes + tok * D + 16 * h;
+    const int b0 = ((p - p0) >> 4) & 63, b = b0 + h;
+    const float ks = __shfl(cur.ks, b) * qmul, vs = __shfl(cur.vs, b) * vinv;
+    const int next_page = ((p - p0) & (kChunk - 1)) >= kChunk - 256 ? next.page : cur.page;
+    f32x4 s[4];
 #pragma unroll
-      for (int t = 0; t < 4; ++t)
+    for (int t = 0; t < 4; ++t) {
+      s[t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int j = 0; j < D / 64; ++j)
-          kw[t * (D / 64) + j] = *reinterpret_cast<const u32x4*>(at + 4 * t * D + 64 * j);
-    };
-    auto load_v = [&](int p) {
-      const int b = ((p - c0) >> 4) + h;
-      const int64_t cell = (int64_t)__shfl(page, b) * a.KV + kh;
-      const int blk = ((p + 16 * h) & (a.ps - 1)) >> 4;
-      const uint8_t* at = a.v + cell * cell_bytes + (blk * D + c) * 16;
-#pragma unroll
-      for (int d = 0; d < DT; ++d) vw[d] = *reinterpret_cast<const u32x4*>(at + 256 * d);
-    };
-    int p = c0 + 64 * wave;
-    if (p < c1) {
-      load_k(p);
-      load_v(p);
+      for (int j = 0; j < D / 64; ++j) {
+        const u32x4 w = kw[t * (D / 64) + j];
+        s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes8<FP8>(w[0], w[1]), q.v[2 * j], s[t], 0, 0, 0);
+        s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes8<FP8>(w[2], w[3]), q.v[2 * j + 1], s[t], 0, 0, 0);
+      }
     }
-    for (; p < c1; p += 256) {
-      const int b = ((p - c0) >> 4) + h;
-      const float ks = __shfl(bks, b) * qmul, vs = __shfl(bvs, b) * vinv;
-      f32x4 s[4];
+    const bool more = p + 256 < p1;
+    if (more) load_k(next_page, p + 256);
+    const bool masked = p < safe_lo || p + 64 > safe_hi || p + 64 > p1 || ((cur.absent >> b0) & 15) != 0;
+    float x[16];
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        s[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int t = 0; t < 4; ++t)
 #pragma unroll
-        for (int j = 0; j < D / 64; ++j) {
-          const u32x4 w = kw[t * (D / 64) + j];
-          s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes8<FP8>(w[0], w[1]), q.v[2 * j], s[t], 0, 0, 0);
-          s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes8<FP8>(w[2], w[3]), q.v[2 * j + 1], s[t], 0, 0, 0);
-        }
-      }
-      const bool more = p + 256 < c1;
-      if (more) load_k(p + 256);
-      const bool masked = p < safe_lo || p + 64 > safe_hi || p + 64 > c1 || ((absent >> ((p - c0) >> 4)) & 15) != 0;
-      float x[16];
+      for (int e = 0; e < 4; ++e) x[4 * t + e] = s[t][e] * ks;
+    if (masked) {
+      const bool gone = __shfl(cur.page, b) < 0;
+      const int at = p + 16 * h;
 #pragma unroll
-      for (int t = 0; t < 4; ++t)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x[4 * t + e] = s[t][e] * ks;
-      if (masked) {
-        const bool gone = (absent >> b) & 1;
-        const int at = p + 16 * h;
-#pragma unroll
-        for (int e = 0; e < 16; ++e) x[e] = !gone && at + e >= lo && at + e < min(hi, c1) ? x[e] : -INFINITY;
-      }
-      float mx = x[0];
-#pragma unroll
-      for (int e = 1; e < 16; ++e) mx = fmaxf(mx, x[e]);
-      mx = max_over_h(mx);
-      const float nm = fmaxf(m, mx);
-      if (__any(nm > m)) {
-        const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - nm);
-        sum *= f;
-#pragma unroll
-        for (int d = 0; d < DT; ++d) acc[d] *= f;
-        m = nm;
-      }
-      const float base = m == -INFINITY ? 0.f : m;
-      f16x8 pw[2];
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const float ex = __builtin_amdgcn_exp2f(x[e] - base);
-        sum += ex;
-        float w = ex * vs;
-        if (masked) w = x[e] == -INFINITY ? 0.f : w;
-        pw[e >> 3][e & 7] = (f16)w;
-      }
-      if (FP8 && masked) {
-        // codes of tokens that no row sees may be NaN
-        const int at = p + 16 * h;
-        const u32x4 keep = byte_mask(first_seen - at, ((absent >> b) & 1) ? 0 : c1 - at);
-#pragma unroll
-        for (int d = 0; d < DT; ++d) vw[d] &= keep;
-      }
-#pragma unroll
-      for (int d = 0; d < DT; ++d) {
-        acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes8<FP8>(vw[d][0], vw[d][1]), pw[0], acc[d], 0, 0, 0);
-        acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes8<FP8>(vw[d][2], vw[d][3]), pw[1], acc[d], 0, 0, 0);
-      }
-      if (more) load_v(p + 256);
+      for (int e = 0; e < 16; ++e) x[e] = !gone && at + e >= lo && at + e < min(hi, p1) ? x[e] : -INFINITY;
     }
+    float mx = x[0];
+#pragma unroll
+    for (int e = 1; e < 16; ++e) mx = fmaxf(mx, x[e]);
+    mx = max_over_h(mx);
+    const float nm = fmaxf(m, mx);
+    if (__any(nm > m)) {
+      const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - nm);
+      sum *= f;
+#pragma unroll
+      for (int d = 0; d < DT; ++d) acc[d] *= f;
+      m = nm;
+    }
+    const float base = m == -INFINITY ? 0.f : m;
+    f16x8 pw[2];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const float ex = __builtin_amdgcn_exp2f(x[e] - base);
+      sum += ex;
+      float w = ex * vs;
+      if (masked) w = x[e] == -INFINITY ? 0.f : w;
+      pw[e >> 3][e & 7] = (f16)w;
+    }
+    if (FP8 && masked) {
+      // codes of tokens that no row sees may be NaN
+      const int at = p + 16 * h;
+      const u32x4 keep = byte_mask(first_seen - at, __shfl(cur.page, b) < 0 ? 0 : p1 - at);
+#pragma unroll
+      for (int d = 0; d < DT; ++d) vw[d] &= keep;
+    }
+#pragma unroll
+    for (int d = 0; d < DT; ++d) {
+      acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes8<FP8>(vw[d][0], vw[d][1]), pw[0], acc[d], 0, 0, 0);
+      acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes8<FP8>(vw[d][2], vw[d][3]), pw[1], acc[d], 0, 0, 0);
+    }
+    if (more) load_v(next_page, p + 256);
   }
 
   // the four waves' results, joined in their order
@@ -372,38 +399,52 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(AttnArgs a) {
   }
   __syncthreads();
   if (!s_last) return;
-  om = -INFINITY, ol = 0.f;
+  // All threads: D / 4 of them a row, rows x G groups of splits, joined through LDS.
+  constexpr int kRowThreads = D / 4, kRowSlots = 256 / kRowThreads;
+  const int slot = tid / kRowThreads, dim = 4 * (tid % kRowThreads);
+  const int n_rows = min(rows, 16);
+  const int groups = n_rows >= kRowSlots ? 1 : kRowSlots / n_rows;  // groups of splits a row
+  for (int r0 = 0; r0 < n_rows; r0 += kRowSlots) {
+    const int left = min(n_rows - r0, kRowSlots);
+    const int jr = slot % left, grp = slot / left;
+    const bool on = grp < groups;
+    float jm = -INFINITY, jl = 0.f;
+    f32x4 jo = {0.f, 0.f, 0.f, 0.f};
+    for (int s0 = on ? grp : splits; s0 < splits; s0 += 8 * groups) {
+      float ms[8], ls[8];
+      f32x4 v[8];
 #pragma unroll
-  for (int x = 0; x < kPer; ++x) o[x] = 0.f;
-  const int jrow = mine ? orow : 0;
-  for (int s0 = 0; s0 < splits; s0 += 8) {
-    float ms[8], ls[8];
-    f32x4 v[8][kPer / 4];
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const int off = (min(s0 + k, splits - 1) * tile_rows + jrow) * kRec * 4;
-      ms[k] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rp, off + 4 * D, 0, kSc1));
-      ls[k] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rp, off + 4 * D + 4, 0, kSc1));
-#pragma unroll
-      for (int x = 0; x < kPer; x += 4)
-        v[k][x / 4] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rp, off + 4 * (od + x), 0, kSc1));
-    }
-    __builtin_amdgcn_sched_barrier(0);  // the loads stay together, ahead of their uses
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const bool use = s0 + k < splits && !(ms[k] == -INFINITY && ls[k] == 0.f);
-      const float nm = use ? fmaxf(om, ms[k]) : om;
-      const float fo = om == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(om - nm);
-      const float fn = use ? __builtin_amdgcn_exp2f(ms[k] - nm) : 0.f;
-      if (use) {
-        ol = fmaf(ol, fo, ls[k] * fn);
-#pragma unroll
-        for (int x = 0; x < kPer; ++x) o[x] = fmaf(o[x], fo, v[k][x / 4][x % 4] * fn);
-        om = nm;
+      for (int k = 0; k < 8; ++k) {
+        const int off = (min(s0 + k * groups, splits - 1) * tile_rows + r0 + jr) * kRec * 4;
+        ms[k] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rp, off + 4 * D, 0, kSc1));
+        ls[k] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rp, off + 4 * D + 4, 0, kSc1));
+        v[k] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rp, off + 4 * dim, 0, kSc1));
       }
+      __builtin_amdgcn_sched_barrier(0);  // the loads stay together, ahead of their uses
+#pragma unroll
+      for (int k = 0; k < 8; ++k) join(jm, jl, jo, ms[k], ls[k], v[k], s0 + k * groups < splits);
+    }
+    __syncthreads();
+    float* mine_f = &s_acc[0][0][0] + slot * (D + 2);
+    *reinterpret_cast<float2*>(mine_f) = float2{jm, jl};
+#pragma unroll
+    for (int x = 0; x < 4; ++x) mine_f[2 + dim + x] = jo[x];
+    __syncthreads();
+    if (slot < left) {
+      jm = -INFINITY, jl = 0.f, jo = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int g = 0; g < groups; ++g) {
+        const float* f = &s_acc[0][0][0] + (slot + g * left) * (D + 2);
+        join(jm, jl, jo, f[0], f[1], f32x4{f[2 + dim], f[3 + dim], f[4 + dim], f[5 + dim]}, true);
+      }
+      const float inv = jl > 0.f ? 1.f / jl : (jl != jl ? jl : 0.f);
+      const int row1 = rt * 16 + r0 + slot;
+      typedef T T4 __attribute__((ext_vector_type(4)));
+      T4 y;
+#pragma unroll
+      for (int x = 0; x < 4; ++x) y[x] = (T)(jo[x] * inv);
+      *reinterpret_cast<T4*>((T*)a.out + ((int64_t)(start + row1 / G) * a.H + kh * G + row1 % G) * D + dim) = y;
     }
   }
-  store(ol > 0.f ? 1.f / ol : (ol != ol ? ol : 0.f));
   if (tid == 0) __hip_atomic_store(&a.counters[item], 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
