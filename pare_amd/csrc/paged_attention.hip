@@ -4,6 +4,8 @@
 // p <= L - n + i (and p > L - n + i - window):
 //   o = sum_p e_p (vs_p v_p) / sum_p e_p,   e_p = exp(scale q . (ks_p k_p) - max)
 // with the codes k_p, v_p and their pages' scales. A query that sees nothing gives 0.
+#include <type_traits>
+
 #include "paged.h"
 #include "pmi_common.h"
 #include "pmi_launch.h"
@@ -147,8 +149,6 @@ constexpr float kPBias = 16384.f;  // probabilities are held in fp16 times this
 // Scales: a lane's 16 tokens share theirs, so ks multiplies the scores and vs the
 // probabilities, in fp32, before these become fp16: times vs / (largest vs of the range)
 // and 2^14, so that they use fp16's range from the top.
-// Sixteen-token blocks of a range are looked up 64 at a time, a lane a block.
-constexpr int kChunk = 1024;  // tokens per look-up
 constexpr int64_t kFewWgs = 1024;
 
 template <typename T, int D, bool FP8>
@@ -162,9 +162,22 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(AttnArgs a) {
   const int sp = blockIdx.x, kh = blockIdx.y % a.KV, rt = blockIdx.y / a.KV;
   const int r = blockIdx.z;
   const int G = a.H / a.KV;
-  const int start = a.q_starts ? a.q_starts[r] : r;
-  int n = a.q_starts ? a.q_starts[r + 1] - start : 1;
-  const int len = min(min(max(a.kv_lens[r], 0), a.max_kv), a.width * a.ps);
+  // What does not hang on another load is loaded first: lengths, and the pages of a range that
+  // begins at a multiple of `per`.
+  const int32_t* table = a.tables + (int64_t)r * a.stride;
+  auto look_up = [&](int p) { return table[min((p + 16 * h) >> a.ps_log, a.width - 1)]; };
+  int early0 = -1, early1 = -1;
+  if (!a.window && a.width > 0) {
+    early0 = look_up(sp * a.per + 64 * wave);
+    early1 = look_up(sp * a.per + 64 * wave + 256);
+  }
+  const int len0 = a.kv_lens[r];
+  int start = r, n = 1;
+  if (a.q_starts) {
+    start = a.q_starts[r];
+    n = a.q_starts[r + 1] - start;
+  }
+  const int len = min(min(max(len0, 0), a.max_kv), a.width * a.ps);
   // the limits of queries are set by what the request has, also past max_q
   const int shift = len - n;
   n = min(n, a.max_q);
@@ -196,40 +209,19 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(AttnArgs a) {
 #pragma unroll
   for (int d = 0; d < DT; ++d) acc[d] = f32x4{0.f, 0.f, 0.f, 0.f};
   float m = -INFINITY, sum = 0.f, vref = 0.f;
-  const int32_t* table = a.tables + (int64_t)r * a.stride;
   const int64_t cell_bytes = (int64_t)a.ps * D;
 
-  // The blocks of a chunk: lane l holds the page and the scales of block l. Pages are
-  // looked up two chunks ahead and scales one, so that no tile waits for a look-up.
-  auto look_up = [&](int c0) {
-    const int bp = c0 + 16 * l;
-    return bp < p1 ? table[bp >> a.ps_log] : -1;
-  };
-  struct Blocks {
-    int page;  // -1: outside the cache, or past the range
-    float ks, vs;
-    // Of all blocks, the same in every lane: only shifted by uniform amounts. A 64-bit shift by
-    // a vector register that is the last of the wave's allocation has given wrong lanes here
-    // (v_lshlrev_b64 with its amount in v127 of 128).
-    uint64_t absent;
-  };
-  auto blocks_of = [&](int entry) {
-    const bool there = (unsigned)entry < a.n_pages;
-    Blocks x = {there ? entry : -1, 0.f, 0.f, ~__ballot(there)};
-    if (there) {
-      const int64_t cell = (int64_t)x.page * a.KV + kh;
-      x.ks = a.k_scale[cell];
-      x.vs = a.v_scale[cell];
-    }
-    return x;
-  };
+  // Look-ups run ahead: a tile's entry of the table (of the lane's 16 tokens, block h) is loaded
+  // two tiles before it, its scales and keys one, its values half a tile. Every load of the main
+  // loop is issued on every pass, at a place inside the cache (page 0 for entries outside it, which
+  // are masked): behind a branch the compiler can no longer tell how many are younger than the
+  // one it waits for, and waits for all of them.
   u32x4 kw[D / 16], vw[DT];
-  // pages are read where they are there, page 0 of the cache elsewhere (and masked)
+  auto valid = [&](int entry, int p) { return p + 16 * h < p1 && (unsigned)entry < a.n_pages ? entry : -1; };
   auto load_k = [&](int page, int p) {
-    const int b = (((p - p0) >> 4) & 63) + ((l >> 2) & 3);
-    const int64_t cell = (int64_t)max(__shfl(page, b), 0) * a.KV + kh;
-    const int tok = ((p + 16 * ((l >> 2) & 3)) & (a.ps - 1)) + (l & 3);
-    const uint8_t* at = a.k + cell * cell_bytes + tok * D + 16 * h;
+    const int b = (l >> 2) & 3;  // the block of the lane's row
+    const int64_t cell = (int64_t)max(__shfl(page, 16 * b), 0) * a.KV + kh;
+    const uint8_t* at = a.k + cell * cell_bytes + (((p + 16 * b) & (a.ps - 1)) + (l & 3)) * D + 16 * h;
 #pragma unroll
     for (int t = 0; t < 4; ++t)
 #pragma unroll
@@ -237,42 +229,23 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(AttnArgs a) {
         kw[t * (D / 64) + j] = *reinterpret_cast<const u32x4*>(at + 4 * t * D + 64 * j);
   };
   auto load_v = [&](int page, int p) {
-    const int b = (((p - p0) >> 4) & 63) + h;
-    const int64_t cell = (int64_t)max(__shfl(page, b), 0) * a.KV + kh;
-    const int blk = ((p + 16 * h) & (a.ps - 1)) >> 4;
-    const uint8_t* at = a.v + cell * cell_bytes + (blk * D + c) * 16;
+    const int64_t cell = (int64_t)max(page, 0) * a.KV + kh;
+    const uint8_t* at = a.v + cell * cell_bytes + ((((p + 16 * h) & (a.ps - 1)) >> 4) * D + c) * 16;
 #pragma unroll
     for (int d = 0; d < DT; ++d) vw[d] = *reinterpret_cast<const u32x4*>(at + 256 * d);
   };
   int p = p0 + 64 * wave;
-  int entry1 = look_up(p0 + kChunk);
-  Blocks cur = blocks_of(look_up(p0)), next = cur;
-  float vinv = 0.f;
-  if (p < p1) {
-    load_k(cur.page, p);
-    load_v(cur.page, p);
-  }
-  for (; p < p1; p += 256) {
-    if (((p - p0) & (kChunk - 1)) < 256) {  // this wave's first tile of a chunk
-      if (p - p0 >= kChunk) cur = next;
-      const int c0 = (p - p0) / kChunk * kChunk + p0;
-      next = blocks_of(entry1);
-      entry1 = look_up(c0 + 2 * kChunk);
-      float top = cur.vs < INFINITY ? cur.vs : 0.f;
-#pragma unroll
-      for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
-      const float now = fmaxf(vref, top);
-      if (now > vref && vref > 0.f) {
-        const float f = vref / now;
-#pragma unroll
-        for (int d = 0; d < DT; ++d) acc[d] *= f;
-      }
-      vref = now;
-      vinv = vref > 0.f ? kPBias / vref : 0.f;
-    }
-    const int b0 = ((p - p0) >> 4) & 63, b = b0 + h;
-    const float ks = __shfl(cur.ks, b) * qmul, vs = __shfl(cur.vs, b) * vinv;
-    const int next_page = ((p - p0) & (kChunk - 1)) >= kChunk - 256 ? next.page : cur.page;
+  int page = -1, entry = -1;
+  float bks = 0.f, bvs = 0.f;  // scales of the lane's block
+  auto load_scales = [&](int pg) {
+    const int64_t cell = (int64_t)max(pg, 0) * a.KV + kh;
+    bks = a.k_scale[cell];
+    bvs = a.v_scale[cell];
+  };
+  auto tile = [&](auto last) {
+    constexpr bool kLast = decltype(last)::value;
+    const bool gone = page < 0;
+    const float ks = gone ? 0.f : bks * qmul, tvs = gone ? 0.f : bvs;
     f32x4 s[4];
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
@@ -284,17 +257,28 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(AttnArgs a) {
         s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes8<FP8>(w[2], w[3]), q.v[2 * j + 1], s[t], 0, 0, 0);
       }
     }
-    const bool more = p + 256 < p1;
-    if (more) load_k(next_page, p + 256);
-    const bool masked = p < safe_lo || p + 64 > safe_hi || p + 64 > p1 || ((cur.absent >> b0) & 15) != 0;
+    int next_page = -1;
+    if constexpr (!kLast) {
+      next_page = valid(entry, p + 256);
+      load_scales(next_page);
+      entry = look_up(p + 512);
+      load_k(next_page, p + 256);
+    }
+    // the largest value scale so far is the unit of acc
+    const float top = fmaxf(vref, max_over_h(tvs < INFINITY ? tvs : 0.f));
+    if (__any(top > vref)) {
+      const float f = vref > 0.f ? vref / top : 1.f;
+#pragma unroll
+      for (int d = 0; d < DT; ++d) acc[d] *= f;
+      vref = top;
+    }
+    const float vs = vref > 0.f ? tvs * (kPBias / vref) : 0.f;
+    const bool masked = p < safe_lo || p + 64 > safe_hi || p + 64 > p1 || __any(gone);
+    const int at = p + 16 * h;
     float x[16];
 #pragma unroll
-    for (int t = 0; t < 4; ++t)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) x[4 * t + e] = s[t][e] * ks;
+    for (int e = 0; e < 16; ++e) x[e] = s[e >> 2][e & 3] * ks;
     if (masked) {
-      const bool gone = __shfl(cur.page, b) < 0;
-      const int at = p + 16 * h;
 #pragma unroll
       for (int e = 0; e < 16; ++e) x[e] = !gone && at + e >= lo && at + e < min(hi, p1) ? x[e] : -INFINITY;
     }
@@ -322,8 +306,7 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(AttnArgs a) {
     }
     if (FP8 && masked) {
       // codes of tokens that no row sees may be NaN
-      const int at = p + 16 * h;
-      const u32x4 keep = byte_mask(first_seen - at, __shfl(cur.page, b) < 0 ? 0 : p1 - at);
+      const u32x4 keep = byte_mask(first_seen - at, gone ? 0 : p1 - at);
 #pragma unroll
       for (int d = 0; d < DT; ++d) vw[d] &= keep;
     }
@@ -332,7 +315,19 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(AttnArgs a) {
       acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes8<FP8>(vw[d][0], vw[d][1]), pw[0], acc[d], 0, 0, 0);
       acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes8<FP8>(vw[d][2], vw[d][3]), pw[1], acc[d], 0, 0, 0);
     }
-    if (more) load_v(next_page, p + 256);
+    if constexpr (!kLast) {
+      load_v(next_page, p + 256);
+      page = next_page;
+    }
+  };
+  if (p < p1) {
+    page = valid(a.window ? look_up(p) : early0, p);
+    entry = a.window ? look_up(p + 256) : early1;
+    load_scales(page);
+    load_k(page, p);
+    load_v(page, p);
+    for (; p + 256 < p1; p += 256) tile(std::false_type{});
+    tile(std::true_type{});
   }
 
   // the four waves' results, joined in their order
