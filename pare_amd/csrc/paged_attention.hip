@@ -26,11 +26,36 @@ struct AttnArgs {
   int64_t stride, q_token, q_head, n_pages;
   int T, R, width, H, KV, ps, ps_log, window;
   float scale;
-  // split over the keys: `per` positions a workgroup, at most S of them
-  int per, S, row_tiles, max_q, max_kv;
-  int* counters;
+  int max_q, max_kv;
+  int few_rows;   // requests of up to so many query rows (tokens x heads of a KV head) are `few`
+  int* counters;  // one per workgroup
   float* part;
 };
+
+// What a request's queries see, from its row of kv_lens and q_starts.
+struct Request {
+  int start, n;       // its queries (none: nothing to do)
+  int len, shift;     // its keys; query i sees positions up to shift + i
+  int first_seen;     // the first position that its first query sees
+  int lo, hi;         // positions that any of its queries sees: [lo, hi), lo a multiple of 16
+};
+PMI_DEV Request request(const AttnArgs& a, int r) {
+  const int len0 = a.kv_lens[r];
+  Request q;
+  q.start = r, q.n = 1;
+  if (a.q_starts) {
+    q.start = a.q_starts[r];
+    q.n = a.q_starts[r + 1] - q.start;
+  }
+  q.len = min(min(max(len0, 0), a.max_kv), a.width * a.ps);
+  q.shift = q.len - q.n;  // (also of the queries past max_q)
+  q.n = min(q.n, a.max_q);
+  if (q.n < 0 || q.start < 0 || (int64_t)q.start + q.n > a.T) q.n = 0;
+  q.first_seen = a.window ? max(0, q.shift + 1 - a.window) : 0;
+  q.lo = q.first_seen & ~15;
+  q.hi = a.n_pages ? max(q.lo, min(q.len, q.shift + q.n)) : q.lo;
+  return q;
+}
 
 // ---- operands from codes ----------------------------------------------------------
 // Eight codes (two words) as fp16, exact: e4m3 by the conversion, int8 c as 1152 + c
@@ -138,18 +163,29 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kPBias = 16384.f;  // probabilities are held in fp16 times this
 
 // ---- few query rows ------------------------------------------------------------------
-// Up to 16 query rows (tokens x heads of one KV head) per workgroup against a range of
-// keys: bound by the bytes of the codes. Four waves take the range's 64-token tiles in
-// turn. All operands come straight from memory to registers:
+// Requests of few query rows (tokens x heads of one KV head): bound by the bytes of the
+// codes. An item is 16 rows of one KV head of a request against the request's keys, in
+// tiles of 64 tokens. The tiles of all items, in order, are dealt evenly to a fixed number
+// of workgroups (two per CU, four with heads of 64): lengths differ from request to
+// request, and with a part of each request per workgroup the longest decided
+// (64 requests of 2048 to 8191 keys, 8 KV heads of 128: 142 us that way).
+//
+// Four waves take the tiles of a workgroup's part of an item in turn. All operands come
+// straight from memory to registers:
 //   S^T = K q^T: 16x16x32 fp16 products, rows = tokens. Row m of product t is token
 //     16 (m / 4) + 4 t + m % 4 of the tile, so that a lane's results of the four products
 //     are 16 consecutive tokens, 16 h .. 16 h + 15 (h = lane / 16), all of one page;
 //   O^T = V^T P^T: a lane's operand of P is then what it holds, and that of V its 16-byte
 //     piece of the page's block (one dimension, 16 tokens).
 // Scales: a lane's 16 tokens share theirs, so ks multiplies the scores and vs the
-// probabilities, in fp32, before these become fp16: times vs / (largest vs of the range)
-// and 2^14, so that they use fp16's range from the top.
-constexpr int64_t kFewWgs = 1024;
+// probabilities, in fp32, before these become fp16: times vs / (largest vs so far) and
+// 2^14, so that they use fp16's range from the top.
+//
+// An item that several workgroups share is joined by the last of them to arrive, in
+// order. A workgroup shares at most two items: the one it begins in (record 2 w) and the one
+// it ends in (record 2 w + 1), and only the latter can begin in it, so the
+// workgroup in which an item begins lends it its counter.
+constexpr int kMinShare = 4;  // tiles per workgroup, at least
 
 template <typename T, int D, bool FP8>
 __global__ __launch_bounds__(256, 2) void attention_few_kernel(AttnArgs a) {
@@ -159,30 +195,51 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(AttnArgs a) {
   __shared__ int s_last;
   const int tid = threadIdx.x, l = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c = l & 15, h = l >> 4;
-  const int sp = blockIdx.x, kh = blockIdx.y % a.KV, rt = blockIdx.y / a.KV;
-  const int r = blockIdx.z;
   const int G = a.H / a.KV;
-  // What does not hang on another load is loaded first: lengths, and the pages of a range that
-  // begins at a multiple of `per`.
+
+  // The tiles of all requests, and where this workgroup begins. Every wave works it out for
+  // itself, a lane a run of requests: no barrier, and one round of loads up to 64 requests.
+  // (The host sees to it that the sum is below 2^31.)
+  auto tiles_of = [&](const Request& rq) { return max(1, (rq.hi - rq.lo + 63) >> 6); };
+  auto items_of = [&](const Request& rq) { return rq.n * G > a.few_rows ? 0 : (rq.n * G + 15) / 16 * a.KV; };
+  const int run = (a.R + 63) >> 6, r_lane = run * l;
+  int in_lane = 0;
+  for (int x = r_lane; x < min(a.R, r_lane + run); ++x) {
+    const Request rq = request(a, x);
+    in_lane += tiles_of(rq) * items_of(rq);
+  }
+  int upto = in_lane;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int u = __shfl_up(upto, o);
+    if (l >= o) upto += u;
+  }
+  const int total = __builtin_amdgcn_readlane(upto, 63);
+  const int share = max(kMinShare, (int)(((uint32_t)total + gridDim.x - 1) / gridDim.x));
+  if ((int64_t)share * blockIdx.x >= total) return;
+  int g = share * blockIdx.x;
+  const int g_end = min((int64_t)g + share, (int64_t)total);
+  const int lane0 = __builtin_ctzll(__ballot(upto > g));
+  int r = run * lane0;
+  int off = g - (__builtin_amdgcn_readlane(upto, lane0) - __builtin_amdgcn_readlane(in_lane, lane0));  // tiles of r before g
+  while (g < g_end && r < a.R) {
+  const Request rq = request(a, r);
+  const int row_tiles = (rq.n * G + 15) / 16, nt = tiles_of(rq);
+  const int all = nt * items_of(rq);
+  if (off >= all) {
+    off -= all, ++r;
+    continue;
+  }
+  const int item = off / nt, tile0 = off - item * nt;
+  const int n_tiles = min(g_end - g, nt - tile0);
+  const int kh = item / row_tiles, rt = item - kh * row_tiles;
+  const int item_g = g - tile0;  // the item's first tile of all
+  g += n_tiles, off += n_tiles;
+
   const int32_t* table = a.tables + (int64_t)r * a.stride;
   auto look_up = [&](int p) { return table[min((p + 16 * h) >> a.ps_log, a.width - 1)]; };
-  int early0 = -1, early1 = -1;
-  if (!a.window && a.width > 0) {
-    early0 = look_up(sp * a.per + 64 * wave);
-    early1 = look_up(sp * a.per + 64 * wave + 256);
-  }
-  const int len0 = a.kv_lens[r];
-  int start = r, n = 1;
-  if (a.q_starts) {
-    start = a.q_starts[r];
-    n = a.q_starts[r + 1] - start;
-  }
-  const int len = min(min(max(len0, 0), a.max_kv), a.width * a.ps);
-  // the limits of queries are set by what the request has, also past max_q
-  const int shift = len - n;
-  n = min(n, a.max_q);
-  const int rows = n * G - rt * 16;  // of this tile and the ones behind it
-  if (rows <= 0 || start < 0 || (int64_t)start + n > a.T) return;
+  const int start = rq.start, len = rq.len, shift = rq.shift;
+  const int rows = rq.n * G - rt * 16;  // of this tile of rows and the ones behind it
   const int row = rt * 16 + c;
   const bool live = c < rows;
   const int i = row / G;
@@ -190,12 +247,8 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(AttnArgs a) {
   const int hi = live ? max(0, min(len, shift + i + 1)) : 0;
   const int lo = a.window ? max(0, shift + i + 1 - a.window) : 0;
   const int i_first = rt * 16 / G, i_last = (rt * 16 + min(rows, 16) - 1) / G;
-  const int all_hi = a.n_pages ? max(0, min(len, shift + i_last + 1)) : 0;
-  const int first_seen = a.window ? max(0, shift + i_first + 1 - a.window) : 0, all_lo = first_seen & ~15;
-  const int range = max(0, all_hi - all_lo);
-  const int splits = max(1, (range + a.per - 1) / a.per);
-  if (sp >= splits) return;
-  const int p0 = all_lo + sp * a.per, p1 = min(all_hi, p0 + a.per);
+  const int first_seen = rq.first_seen;
+  const int p0 = rq.lo + 64 * tile0, p1 = min(rq.hi, p0 + 64 * n_tiles);
   // tiles inside of [safe_lo, safe_hi) need no mask
   const int safe_hi = max(0, min(len, shift + i_first + 1));
   const int safe_lo = a.window ? max(0, shift + i_last + 1 - a.window) : 0;
@@ -321,8 +374,8 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(AttnArgs a) {
     }
   };
   if (p < p1) {
-    page = valid(a.window ? look_up(p) : early0, p);
-    entry = a.window ? look_up(p + 256) : early1;
+    page = valid(look_up(p), p);
+    entry = look_up(p + 256);
     load_scales(page);
     load_k(page, p);
     load_v(page, p);
@@ -362,19 +415,20 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(AttnArgs a) {
     for (int x = 0; x < kPer; ++x) y[x] = (T)(o[x] * inv);
     if (mine) *reinterpret_cast<Tv*>(dst) = y;
   };
-  if (splits == 1) {
+  if (n_tiles == nt) {
     store(ol > 0.f ? 1.f / ol : (ol != ol ? ol : 0.f));
-    return;
+    __syncthreads();  // s_acc is read
+    continue;
   }
 
-  // Partial rows to the workspace; the last workgroup of the item to arrive joins them in
-  // split order. Stores and loads are coherent across the XCDs' L2 caches (sc1).
+  // Partial rows to the workspace. Stores and loads are coherent across the XCDs' L2 caches
+  // (sc1).
   constexpr int kSc1 = 16, kRec = D + 4;  // floats of a row: values, max, sum
-  const int item = (r * a.row_tiles + rt) * a.KV + kh;
-  const int tile_rows = min(16, a.max_q * G);
-  float* base = a.part + (int64_t)item * a.S * tile_rows * kRec;
-  const __amdgpu_buffer_rsrc_t rp = rsrc(base, (int64_t)a.S * tile_rows * kRec * 4);
-  const int rec = (sp * tile_rows + orow) * kRec * 4;
+  const int first_wg = item_g / share, parts = (item_g + nt - 1) / share - first_wg + 1;
+  const __amdgpu_buffer_rsrc_t rp = rsrc(a.part + (int64_t)first_wg * 32 * kRec, (int64_t)parts * 32 * kRec * 4);
+  // record of part s: the first one's second, the others' first
+  auto record = [&](int s, int rr) { return ((s ? 2 * s : 1) * 16 + rr) * kRec * 4; };
+  const int rec = record((int)blockIdx.x - first_wg, orow);
   if (mine) {
 #pragma unroll
     for (int x = 0; x < kPer; x += 4)
@@ -389,12 +443,13 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(AttnArgs a) {
   __builtin_amdgcn_s_waitcnt(0);
   __syncthreads();
   if (tid == 0) {
-    const int old = __hip_atomic_fetch_add(&a.counters[item], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    s_last = old == splits - 1;
+    const int old = __hip_atomic_fetch_add(&a.counters[first_wg], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    s_last = old == parts - 1;
   }
   __syncthreads();
-  if (!s_last) return;
+  if (!s_last) continue;
   // All threads: D / 4 of them a row, rows x G groups of splits, joined through LDS.
+  constexpr int kFly = 16;  // parts in flight
   constexpr int kRowThreads = D / 4, kRowSlots = 256 / kRowThreads;
   const int slot = tid / kRowThreads, dim = 4 * (tid % kRowThreads);
   const int n_rows = min(rows, 16);
@@ -405,19 +460,19 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(AttnArgs a) {
     const bool on = grp < groups;
     float jm = -INFINITY, jl = 0.f;
     f32x4 jo = {0.f, 0.f, 0.f, 0.f};
-    for (int s0 = on ? grp : splits; s0 < splits; s0 += 8 * groups) {
-      float ms[8], ls[8];
-      f32x4 v[8];
+    for (int s0 = on ? grp : parts; s0 < parts; s0 += kFly * groups) {
+      float ms[kFly], ls[kFly];
+      f32x4 v[kFly];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const int off = (min(s0 + k * groups, splits - 1) * tile_rows + r0 + jr) * kRec * 4;
-        ms[k] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rp, off + 4 * D, 0, kSc1));
-        ls[k] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rp, off + 4 * D + 4, 0, kSc1));
-        v[k] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rp, off + 4 * dim, 0, kSc1));
+      for (int k = 0; k < kFly; ++k) {
+        const int at = record(min(s0 + k * groups, parts - 1), r0 + jr);
+        ms[k] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rp, at + 4 * D, 0, kSc1));
+        ls[k] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rp, at + 4 * D + 4, 0, kSc1));
+        v[k] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rp, at + 4 * dim, 0, kSc1));
       }
       __builtin_amdgcn_sched_barrier(0);  // the loads stay together, ahead of their uses
 #pragma unroll
-      for (int k = 0; k < 8; ++k) join(jm, jl, jo, ms[k], ls[k], v[k], s0 + k * groups < splits);
+      for (int k = 0; k < kFly; ++k) join(jm, jl, jo, ms[k], ls[k], v[k], s0 + k * groups < parts);
     }
     __syncthreads();
     float* mine_f = &s_acc[0][0][0] + slot * (D + 2);
@@ -440,46 +495,27 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(AttnArgs a) {
       *reinterpret_cast<T4*>((T*)a.out + ((int64_t)(start + row1 / G) * a.H + kh * G + row1 % G) * D + dim) = y;
     }
   }
-  if (tid == 0) __hip_atomic_store(&a.counters[item], 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  if (tid == 0) __hip_atomic_store(&a.counters[first_wg], 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  __syncthreads();  // s_acc is read
+  }
 }
 
 template <typename T, int D>
-hipError_t few(const AttnArgs& a, bool fp8, hipStream_t stream) {
-  const dim3 grid((unsigned)a.S, (unsigned)(a.KV * a.row_tiles), (unsigned)a.R);
+hipError_t few(const AttnArgs& a, bool fp8, int wgs, hipStream_t stream) {
   if (fp8)
-    hipLaunchKernelGGL((attention_few_kernel<T, D, true>), grid, dim3(256), 0, stream, a);
+    hipLaunchKernelGGL((attention_few_kernel<T, D, true>), dim3(wgs), dim3(256), 0, stream, a);
   else
-    hipLaunchKernelGGL((attention_few_kernel<T, D, false>), grid, dim3(256), 0, stream, a);
+    hipLaunchKernelGGL((attention_few_kernel<T, D, false>), dim3(wgs), dim3(256), 0, stream, a);
   return hipGetLastError();
 }
 
-struct FewPlan {
-  int row_tiles, per, S;
-  size_t part;
-};
-FewPlan few_plan(const PagedAttention& p, const PagedCache& c) {
-  FewPlan f;
-  const int64_t G = p.H / c.KV;
-  f.row_tiles = (int)((p.max_q * G + 15) / 16);
-  const int64_t range = p.window ? (p.max_kv < p.window + p.max_q + 15 ? p.max_kv : p.window + p.max_q + 15) : p.max_kv;
-  const int64_t items = p.R * c.KV * f.row_tiles;
-  // Up to kFewWgs workgroups where the range allows it, 256 tokens (a tile a wave) each or more.
-  int64_t S = items > (int64_t)kWsCounterBytes / 4 ? 1 : kFewWgs / items;
-  if (S < 1) S = 1;
-  f.per = (int)(((range + S - 1) / S + 255) / 256 * 256);
-  if (f.per < 256) f.per = 256;
-  f.S = (int)((range + f.per - 1) / f.per);
-  if (f.S < 1) f.S = 1;
-  const int64_t rows = p.max_q * G < 16 ? p.max_q * G : 16;
-  f.part = f.S > 1 ? (size_t)(items * f.S * rows * (c.D + 4) * 4) : 0;
-  return f;
-}
+// Workgroups of the few-row kernel: what the CUs hold at once.
+int few_wgs(int64_t D) { return device_cu_count() * (D == 64 ? 4 : 2); }
 
 }  // namespace
 
 size_t paged_attention_ws_bytes(const PagedAttention& p, const PagedCache& c) {
-  const FewPlan f = few_plan(p, c);
-  return f.part ? kWsCounterBytes + f.part : 0;
+  return kWsCounterBytes + (size_t)few_wgs(c.D) * 32 * (c.D + 4) * 4;
 }
 
 hipError_t launch_paged_attention(const PagedAttention& p, const PagedCache& c, void* workspace, size_t ws_bytes,
@@ -487,12 +523,13 @@ hipError_t launch_paged_attention(const PagedAttention& p, const PagedCache& c, 
   AttnArgs a = {p.q, p.out, (const uint8_t*)c.k, (const uint8_t*)c.v, c.k_scale, c.v_scale, p.tables, p.kv_lens,
                 p.q_starts, p.stride, p.q_token, p.q_head, c.pages, (int)p.T, (int)p.R, (int)p.width, (int)p.H,
                 (int)c.KV, (int)c.ps, __builtin_ctz((unsigned)c.ps), (int)p.window, p.scale};
-  const FewPlan f = few_plan(p, c);
-  a.per = f.per, a.S = f.S, a.row_tiles = f.row_tiles, a.max_q = (int)p.max_q, a.max_kv = (int)p.max_kv;
+  a.max_q = (int)p.max_q, a.max_kv = (int)p.max_kv;
+  a.few_rows = 0x7fffffff;
   a.counters = (int*)workspace;
   a.part = (float*)((char*)workspace + kWsCounterBytes);
-  if (p.bf16) return c.D == 64 ? few<__bf16, 64>(a, c.fp8, stream) : few<__bf16, 128>(a, c.fp8, stream);
-  return c.D == 64 ? few<f16, 64>(a, c.fp8, stream) : few<f16, 128>(a, c.fp8, stream);
+  const int wgs = few_wgs(c.D);
+  if (p.bf16) return c.D == 64 ? few<__bf16, 64>(a, c.fp8, wgs, stream) : few<__bf16, 128>(a, c.fp8, wgs, stream);
+  return c.D == 64 ? few<f16, 64>(a, c.fp8, wgs, stream) : few<f16, 128>(a, c.fp8, wgs, stream);
 }
 
 }  // namespace pmi
