@@ -190,7 +190,7 @@ constexpr int kMinShare = 4;  // tiles per workgroup, at least
 template <typename T, int D, bool FP8>
 __global__ __launch_bounds__(256, 2) void attention_few_kernel(AttnArgs a) {
   constexpr int DT = D / 16;  // 16-dimension tiles of the output
-  __shared__ float s_acc[4][16][D];
+  __shared__ __attribute__((aligned(16))) float s_acc[4][16][D + 4];  // rows 16 bytes apart in the banks
   __shared__ float s_m[4][16], s_l[4][16];
   __shared__ int s_last;
   const int tid = threadIdx.x, l = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -202,18 +202,27 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(AttnArgs a) {
   // (The host sees to it that the sum is below 2^31.)
   auto tiles_of = [&](const Request& rq) { return max(1, (rq.hi - rq.lo + 63) >> 6); };
   auto items_of = [&](const Request& rq) { return rq.n * G > a.few_rows ? 0 : (rq.n * G + 15) / 16 * a.KV; };
+  auto up = [](int nt) { return (nt + kMinShare - 1) / kMinShare * kMinShare; };
   const int run = (a.R + 63) >> 6, r_lane = run * l;
-  int in_lane = 0;
+  int in_lane = 0, in_lane_up = 0;
   for (int x = r_lane; x < min(a.R, r_lane + run); ++x) {
     const Request rq = request(a, x);
     in_lane += tiles_of(rq) * items_of(rq);
+    in_lane_up += up(tiles_of(rq)) * items_of(rq);
   }
-  int upto = in_lane;
+  auto scan = [&](int v) {
 #pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int u = __shfl_up(upto, o);
-    if (l >= o) upto += u;
-  }
+    for (int o = 1; o < 64; o <<= 1) {
+      const int u = __shfl_up(v, o);
+      if (l >= o) v += u;
+    }
+    return v;
+  };
+  // Few tiles: items are cut every kMinShare tiles, so that no workgroup has parts of two.
+  int upto = scan(in_lane_up);
+  const bool cut = __builtin_amdgcn_readlane(upto, 63) <= kMinShare * (int)gridDim.x;
+  if (!cut) upto = scan(in_lane);
+  in_lane = cut ? in_lane_up : in_lane;
   const int total = __builtin_amdgcn_readlane(upto, 63);
   const int share = max(kMinShare, (int)(((uint32_t)total + gridDim.x - 1) / gridDim.x));
   if ((int64_t)share * blockIdx.x >= total) return;
@@ -225,16 +234,17 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(AttnArgs a) {
   while (g < g_end && r < a.R) {
   const Request rq = request(a, r);
   const int row_tiles = (rq.n * G + 15) / 16, nt = tiles_of(rq);
-  const int all = nt * items_of(rq);
+  const int span = cut ? up(nt) : nt;  // what an item takes of the order
+  const int all = span * items_of(rq);
   if (off >= all) {
     off -= all, ++r;
     continue;
   }
-  const int item = off / nt, tile0 = off - item * nt;
-  const int n_tiles = min(g_end - g, nt - tile0);
+  const int item = off / span, tile0 = off - item * span;
+  const int n_tiles = min(g_end - g, nt - tile0), n_span = min(g_end - g, span - tile0);
   const int kh = item / row_tiles, rt = item - kh * row_tiles;
   const int item_g = g - tile0;  // the item's first tile of all
-  g += n_tiles, off += n_tiles;
+  g += n_span, off += n_span;
 
   const int32_t* table = a.tables + (int64_t)r * a.stride;
   auto look_up = [&](int p) { return table[min((p + 16 * h) >> a.ps_log, a.width - 1)]; };
@@ -387,26 +397,34 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(AttnArgs a) {
   sum = sum_over_h(sum);
   const float unit = vref * (1.f / kPBias);
 #pragma unroll
-  for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4*>(&s_acc[wave][c][16 * d + 4 * h]) = acc[d] * unit;
+  for (int d = 0; d < DT; ++d)
+    if (live) *reinterpret_cast<f32x4*>(&s_acc[wave][c][16 * d + 4 * h]) = acc[d] * unit;
   if (h == 0) s_m[wave][c] = m, s_l[wave][c] = sum;
   __syncthreads();
   constexpr int kPer = D / 16;  // dimensions per thread: 16 threads a row
   const int orow = tid >> 4, od = (tid & 15) * kPer;
+  const bool mine = orow < rows;
   float om = -INFINITY, ol = 0.f, o[kPer];
 #pragma unroll
-  for (int w = 0; w < 4; ++w) om = fmaxf(om, s_m[w][orow]);
-#pragma unroll
   for (int x = 0; x < kPer; ++x) o[x] = 0.f;
+  if (mine) {
+    float mw[4];
 #pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    const float f = s_m[w][orow] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(s_m[w][orow] - om);
-    ol = fmaf(s_l[w][orow], f, ol);
-    // (a wave without a key it sees holds zeros, or NaN of a page that shows them)
+    for (int w = 0; w < 4; ++w) mw[w] = s_m[w][orow], om = fmaxf(om, mw[w]);
 #pragma unroll
-    for (int x = 0; x < kPer; ++x) o[x] = f == 0.f ? o[x] : fmaf(s_acc[w][orow][od + x], f, o[x]);
+    for (int w = 0; w < 4; ++w) {
+      // a wave that saw no key holds zeros; the sum of one whose scores are all NaN is NaN
+      const float f = mw[w] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mw[w] - om);
+      ol = fmaf(s_l[w][orow], f, ol);
+#pragma unroll
+      for (int x = 0; x < kPer; x += 4) {
+        const f32x4 v = *reinterpret_cast<const f32x4*>(&s_acc[w][orow][od + x]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[x + e] = fmaf(v[e], f, o[x + e]);
+      }
+    }
   }
   const int grow = rt * 16 + orow;
-  const bool mine = orow < rows;
   T* dst = (T*)a.out + ((int64_t)(start + grow / G) * a.H + kh * G + grow % G) * D + od;
   auto store = [&](float inv) {
     typedef T Tv __attribute__((ext_vector_type(kPer)));
@@ -449,7 +467,6 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(AttnArgs a) {
   __syncthreads();
   if (!s_last) continue;
   // All threads: D / 4 of them a row, rows x G groups of splits, joined through LDS.
-  constexpr int kFly = 16;  // parts in flight
   constexpr int kRowThreads = D / 4, kRowSlots = 256 / kRowThreads;
   const int slot = tid / kRowThreads, dim = 4 * (tid % kRowThreads);
   const int n_rows = min(rows, 16);
@@ -460,7 +477,8 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(AttnArgs a) {
     const bool on = grp < groups;
     float jm = -INFINITY, jl = 0.f;
     f32x4 jo = {0.f, 0.f, 0.f, 0.f};
-    for (int s0 = on ? grp : parts; s0 < parts; s0 += kFly * groups) {
+    auto batch = [&](auto fly, int s0) {
+      constexpr int kFly = decltype(fly)::value;
       float ms[kFly], ls[kFly];
       f32x4 v[kFly];
 #pragma unroll
@@ -471,8 +489,27 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(AttnArgs a) {
         v[k] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rp, at + 4 * dim, 0, kSc1));
       }
       __builtin_amdgcn_sched_barrier(0);  // the loads stay together, ahead of their uses
+      float nm = jm;
 #pragma unroll
-      for (int k = 0; k < kFly; ++k) join(jm, jl, jo, ms[k], ls[k], v[k], s0 + k * groups < parts);
+      for (int k = 0; k < kFly; ++k) nm = fmaxf(nm, s0 + k * groups < parts ? ms[k] : -INFINITY);
+      const float f = jm == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(jm - nm);
+      jl *= f, jo *= f;
+#pragma unroll
+      for (int k = 0; k < kFly; ++k) {
+        // (a part that saw no key: weight 0; its sum may be NaN, see above)
+        const bool use = s0 + k * groups < parts;
+        const float w = use && ms[k] != -INFINITY ? __builtin_amdgcn_exp2f(ms[k] - nm) : 0.f;
+        jl = fmaf(use ? ls[k] : 0.f, w, jl);
+#pragma unroll
+        for (int x = 0; x < 4; ++x) jo[x] = fmaf(use ? v[k][x] : 0.f, w, jo[x]);
+      }
+      jm = nm;
+    };
+    if (on) {
+      if (parts <= 4 * groups)
+        batch(std::integral_constant<int, 4>{}, grp);
+      else
+        for (int s0 = grp; s0 < parts; s0 += 16 * groups) batch(std::integral_constant<int, 16>{}, s0);
     }
     __syncthreads();
     float* mine_f = &s_acc[0][0][0] + slot * (D + 2);
