@@ -1463,7 +1463,7 @@ size_t pmi_paged_attention_workspace_bytes(int64_t T, int64_t R, int64_t H, int6
   if (T <= 0 || R <= 0 || H <= 0 || KV <= 0 || H % KV != 0 || D <= 0 || max_q <= 0 || max_kv <= 0) return 0;
   if (T >= most || R >= most || H > 65535 || D > 65535 || max_q >= most || max_kv >= most || window < 0) return 0;
   pmi::PagedAttention p = {};
-  p.T = T, p.R = R, p.H = H, p.max_q = max_q, p.max_kv = max_kv, p.window = window;
+  p.T = T, p.R = R, p.H = H, p.max_q = max_q < T ? max_q : T, p.max_kv = max_kv, p.window = window;
   pmi::PagedCache c = {};
   c.KV = KV, c.D = D;
   return pmi::paged_attention_ws_bytes(p, c);
@@ -1489,9 +1489,10 @@ int pmi_paged_attention(const void* q, int dtype, int64_t q_stride, int64_t q_he
     return fail(PMI_ERR_UNSUPPORTED, "%s: at most 64 query heads per KV head (got %lld)", fn, (long long)(H / KV));
   if (q_stride % 8 != 0 || q_head_stride % 8 != 0)
     return fail(PMI_ERR_INVALID, "%s: the strides of q must be multiples of 8 elements", fn);
+  if (max_q > T) max_q = T;
   if (T == 0 || R == 0 || max_q == 0) return ok();
   if (T >= (1ll << 31) / H || R >= (1ll << 31) / KV || width > (1ll << 30) / page_size || max_kv >= (1ll << 31) ||
-      max_q >= (1ll << 31) / (H / KV) || window >= (1ll << 31))
+      window >= (1ll << 31))
     return fail(PMI_ERR_UNSUPPORTED, "%s: too large", fn);
   if (!q || !out || !kv_lens || (width && !tables)) return fail(PMI_ERR_INVALID, "%s: null buffer", fn);
   if (!aligned(q, 16) || !aligned(out, 16))

@@ -27,6 +27,7 @@ struct AttnArgs {
   int T, R, width, H, KV, ps, ps_log, window;
   float scale;
   int max_q, max_kv;
+  int splits, per;  // many rows: ranges of keys, and tokens in one
   int few_rows;   // requests of up to so many query rows (tokens x heads of a KV head) are `few`
   int* counters;  // one per workgroup
   float* part;
@@ -92,6 +93,16 @@ PMI_DEV u32x4 byte_mask(int first, int last) {
   return m;
 }
 
+// 2^e <= m < 2^(e + 1) as `up`, and its inverse; 1 for zero, subnormal and infinite m.
+struct PowerOfTwo {
+  float up, down;
+};
+PMI_DEV PowerOfTwo power_below(float m) {
+  const uint32_t e = __builtin_bit_cast(uint32_t, m) >> 23;
+  if (e < 1 || e > 253) return {1.f, 1.f};
+  return {__builtin_bit_cast(float, e << 23), __builtin_bit_cast(float, (254u - e) << 23)};
+}
+
 // A row of q as fp16 that the products take exactly: bf16 rows are scaled by a power of two
 // to a largest value in [1, 2) (what falls under 2^-24 of it is lost to fp16's range, and
 // is 2^-16 of bf16's own rounding of the largest). mul takes the power back.
@@ -124,15 +135,12 @@ PMI_DEV void load_query(QueryRow<T, D>& q, const T* row, bool live, int h) {
       for (int e = 0; e < 8; ++e) m = fmaxf(m, fabsf((float)raw[i][e]));
     m = fmaxf(m, __shfl_xor(m, 16));
     m = fmaxf(m, __shfl_xor(m, 32));
-    // 2^-exponent as bits; rows of zeros (or subnormals), infinities keep 1
-    const uint32_t e = __builtin_bit_cast(uint32_t, m) >> 23;
-    const bool ok = e >= 1 && e <= 253;
-    const float down = ok ? __builtin_bit_cast(float, (254u - e) << 23) : 1.f;
-    q.mul = ok ? __builtin_bit_cast(float, e << 23) : 1.f;
+    const PowerOfTwo w = power_below(m);
+    q.mul = w.up;
 #pragma unroll
     for (int i = 0; i < D / 32; ++i)
 #pragma unroll
-      for (int x = 0; x < 8; ++x) q.v[i][x] = (f16)((float)raw[i][x] * down);
+      for (int x = 0; x < 8; ++x) q.v[i][x] = (f16)((float)raw[i][x] * w.down);
   } else {
 #pragma unroll
     for (int i = 0; i < D / 32; ++i) q.v[i] = __builtin_bit_cast(f16x8, raw[i]);
@@ -546,13 +554,412 @@ hipError_t few(const AttnArgs& a, bool fp8, int wgs, hipStream_t stream) {
   return hipGetLastError();
 }
 
+// ---- many query rows -----------------------------------------------------------------
+// Requests with more query rows: bound by the matrix cores and the softmax beside them. A
+// workgroup takes 128 query rows (32 a wave, tokens x heads of one KV head, so that the heads
+// share the keys) against tiles of 64 keys. The tile's codes become fp16 once, on their way
+// from registers to LDS (two slots), and serve the four waves:
+//   S^T = K q^T, 32x32x16 products, rows = tokens: row m of product u is token 32 u + 16 (m / 16) +
+//     8 (m / 4 % 2) + 4 (m / 8 % 2) + m % 4, so that eight of a lane's results are eight
+//     consecutive tokens, its operand of P;
+//   O^T = V^T P^T from V^T in LDS, rows = dimensions.
+// A block of 16 tokens, and with it a page's scales, is the same for all lanes. In LDS,
+// 16-byte chunk x of row y lies at x ^ (y % 16) (K) and x ^ (y % 8) (V^T): reads of
+// consecutive rows fall in different banks.
+// Where the rows give fewer workgroups than the CUs hold, the keys are split as well
+// (`splits` ranges of `per` tokens), and the last range to arrive joins them.
+constexpr int kRows = 128;
+
+template <typename T, int D, bool FP8>
+__global__ __launch_bounds__(256, 2) void attention_rows_kernel(AttnArgs a) {
+  constexpr int KP = D / 64;       // 16-byte pieces of K, and of V, per thread and tile
+  constexpr int kSlot = 64 * D * 2;  // bytes of K (or V) of a tile as fp16
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];  // [2 slots][K, V]
+  __shared__ int s_last;
+  const int tid = threadIdx.x, l = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int c = l & 31, h = l >> 5;
+  const int G = a.H / a.KV;
+
+  // which rows: the row tiles of all requests in order, each request's last ones (with the most
+  // keys) first, the KV heads innermost (an XCD then keeps few heads' keys in its L2)
+  auto tiles_of = [&](int r) {
+    const Request rq = request(a, r);
+    return rq.n * G > a.few_rows ? (rq.n * G + kRows - 1) / kRows : 0;
+  };
+  const int kh = blockIdx.x % a.KV, rest = blockIdx.x / a.KV;
+  const int sp = rest % a.splits, index = rest / a.splits;
+  const int run = (a.R + 63) >> 6, r_lane = run * l;
+  int in_lane = 0;
+  for (int x = r_lane; x < min(a.R, r_lane + run); ++x) in_lane += tiles_of(x);
+  int upto = in_lane;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int u = __shfl_up(upto, o);
+    if (l >= o) upto += u;
+  }
+  if (index >= __builtin_amdgcn_readlane(upto, 63)) return;
+  const int lane0 = __builtin_ctzll(__ballot(upto > index));
+  int r = run * lane0;
+  int at_tile = index - (__builtin_amdgcn_readlane(upto, lane0) - __builtin_amdgcn_readlane(in_lane, lane0));
+  int count = tiles_of(r);
+  while (at_tile >= count) {
+    at_tile -= count;
+    if (++r >= a.R) return;
+    count = tiles_of(r);
+  }
+  const int rt = count - 1 - at_tile;
+  const Request rq = request(a, r);
+  const int start = rq.start, len = rq.len, shift = rq.shift;
+  const int rows = min(kRows, rq.n * G - rt * kRows);
+  const int row = rt * kRows + wave * 32 + c;
+  const bool live = wave * 32 + c < rows;
+  const int i = row / G;
+  const int hi = live ? max(0, min(len, shift + i + 1)) : 0;
+  const int lo = a.window ? max(0, shift + i + 1 - a.window) : 0;
+  const int i_first = rt * kRows / G, i_last = (rt * kRows + rows - 1) / G;
+  const int first_seen = a.window ? max(0, shift + i_first + 1 - a.window) : 0, all_lo = first_seen & ~15;
+  const int all_hi = a.n_pages ? max(all_lo, min(len, shift + i_last + 1)) : all_lo;
+  const int parts = max(1, (all_hi - all_lo + a.per - 1) / a.per);
+  if (sp >= parts) return;
+  const int p0 = all_lo + sp * a.per, p1 = min(all_hi, p0 + a.per);
+  const int safe_hi = max(0, min(len, shift + i_first + 1));
+  const int safe_lo = a.window ? max(0, shift + i_last + 1 - a.window) : 0;
+
+  // the wave's query rows: step s holds dimensions 16 s + 8 h .. + 7
+  f16x8 qv[D / 16];
+  // (the sign of the scale goes into q: block maxima need a factor that is not negative)
+  float qmul = fmaxf(fabsf(a.scale) * kLog2e, 1e-18f);
+  {
+    typedef T T8 __attribute__((ext_vector_type(8)));
+    const T* qr = (const T*)a.q + (int64_t)(start + (live ? i : i_first)) * a.q_token +
+                  (int64_t)(kh * G + (live ? row - i * G : 0)) * a.q_head;
+    T8 raw[D / 16];
+#pragma unroll
+    for (int s = 0; s < D / 16; ++s) raw[s] = *reinterpret_cast<const T8*>(qr + 16 * s + 8 * h);
+    if constexpr (__is_same(T, f16)) {
+#pragma unroll
+      for (int s = 0; s < D / 16; ++s) qv[s] = a.scale < 0.f ? -raw[s] : raw[s];
+    } else {
+      float m = 0.f;
+#pragma unroll
+      for (int s = 0; s < D / 16; ++s)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) m = fmaxf(m, fabsf((float)raw[s][e]));
+      m = fmaxf(m, __shfl_xor(m, 32));
+      PowerOfTwo w = power_below(m);
+      qmul *= w.up;
+      if (a.scale < 0.f) w.down = -w.down;
+#pragma unroll
+      for (int s = 0; s < D / 16; ++s)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) qv[s][e] = (f16)((float)raw[s][e] * w.down);
+    }
+  }
+
+  typedef float f32x16 __attribute__((ext_vector_type(16)));
+  f32x16 acc[D / 32];
+#pragma unroll
+  for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) acc[d][e] = 0.f;
+  float m = -INFINITY, sum = 0.f, vref = 0.f, vinv = 0.f;
+  const int32_t* table = a.tables + (int64_t)r * a.stride;
+  const int64_t cell_bytes = (int64_t)a.ps * D;
+
+  // the four blocks of the tile at p: their pages (-1: not there) and scales
+  struct Blocks {
+    int page[4];
+    float ks[4], vs[4];
+    bool bad;  // one of them is not finite
+  };
+  auto look_up = [&](int p, int* entry) {
+#pragma unroll
+    for (int b = 0; b < 4; ++b) entry[b] = table[min((p + 16 * b) >> a.ps_log, a.width - 1)];
+  };
+  auto blocks_of = [&](int p, const int* entry) {
+    Blocks x;
+    x.bad = false;
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+      const bool there = p + 16 * b < p1 && (unsigned)entry[b] < a.n_pages;
+      x.page[b] = there ? entry[b] : -1;
+      const int64_t cell = (int64_t)(there ? entry[b] : 0) * a.KV + kh;
+      const float ks = a.k_scale[cell], vs = a.v_scale[cell];
+      x.ks[b] = there ? (ks < 1e-18f ? 1e-18f : ks) : 1e-18f;
+      x.vs[b] = there ? vs : 0.f;
+      x.bad |= !(x.ks[b] < INFINITY) || !(x.vs[b] < INFINITY);
+    }
+    return x;
+  };
+  auto pick = [](const int* v, int b) {
+    const int lo2 = b & 1 ? v[1] : v[0], hi2 = b & 1 ? v[3] : v[2];
+    return b & 2 ? hi2 : lo2;
+  };
+  u32x4 kw[KP], vw[KP];
+  auto load_tile = [&](int p, const Blocks& x) {
+#pragma unroll
+    for (int k = 0; k < KP; ++k) {
+      const int idx = tid + 256 * k;
+      const int krow = idx / (D / 16), kpiece = idx % (D / 16);
+      const int64_t kc = (int64_t)max(pick(x.page, krow >> 4), 0) * a.KV + kh;
+      kw[k] = *reinterpret_cast<const u32x4*>(a.k + kc * cell_bytes + ((p + krow) & (a.ps - 1)) * D + 16 * kpiece);
+      const int vblk = idx / D, vd = idx % D;
+      const int64_t vc = (int64_t)max(pick(x.page, vblk), 0) * a.KV + kh;
+      vw[k] = *reinterpret_cast<const u32x4*>(a.v + vc * cell_bytes + ((((p + 16 * vblk) & (a.ps - 1)) >> 4) * D + vd) * 16);
+    }
+  };
+  auto store_tile = [&](int p, const Blocks& x, int slot) {
+    uint8_t* kb = lds + slot * 2 * kSlot;
+    uint8_t* vb = kb + kSlot;
+    // codes of tokens that no row sees may be NaN (e4m3)
+    const bool edge = FP8 && (p < first_seen || p + 64 > p1 || (x.page[0] | x.page[1] | x.page[2] | x.page[3]) < 0);
+#pragma unroll
+    for (int k = 0; k < KP; ++k) {
+      const int idx = tid + 256 * k;
+      const int krow = idx / (D / 16), kpiece = idx % (D / 16);
+      const f16x8 k0 = codes8<FP8>(kw[k][0], kw[k][1]), k1 = codes8<FP8>(kw[k][2], kw[k][3]);
+      *reinterpret_cast<f16x8*>(kb + krow * D * 2 + (((2 * kpiece) ^ (krow & (D / 8 - 1))) << 4)) = k0;
+      *reinterpret_cast<f16x8*>(kb + krow * D * 2 + (((2 * kpiece + 1) ^ (krow & (D / 8 - 1))) << 4)) = k1;
+      const int vblk = idx / D, vd = idx % D;
+      if (edge) vw[k] &= byte_mask(first_seen - p - 16 * vblk, pick(x.page, vblk) < 0 ? 0 : p1 - p - 16 * vblk);
+      const f16x8 v0 = codes8<FP8>(vw[k][0], vw[k][1]), v1 = codes8<FP8>(vw[k][2], vw[k][3]);
+      *reinterpret_cast<f16x8*>(vb + vd * 128 + (((2 * vblk) ^ (vd & 7)) << 4)) = v0;
+      *reinterpret_cast<f16x8*>(vb + vd * 128 + (((2 * vblk + 1) ^ (vd & 7)) << 4)) = v1;
+    }
+  };
+
+  if (p0 < p1) {
+    int entry[4];
+    look_up(p0, entry);
+    Blocks cur = blocks_of(p0, entry);
+    load_tile(p0, cur);
+    look_up(p0 + 64, entry);
+    Blocks next = blocks_of(p0 + 64, entry);
+    store_tile(p0, cur, 0);
+    load_tile(p0 + 64, next);
+    look_up(p0 + 128, entry);
+    int slot = 0;
+    for (int p = p0; p < p1; p += 64, slot ^= 1) {
+      __syncthreads();  // the slot is written; the other one is read
+      Blocks after = next;
+      if (p + 64 < p1) {
+        store_tile(p + 64, next, slot ^ 1);
+        after = blocks_of(p + 128, entry);
+        load_tile(p + 128, after);
+        look_up(p + 192, entry);
+      }
+      const uint8_t* kb = lds + slot * 2 * kSlot;
+      const uint8_t* vb = kb + kSlot;
+      f32x16 s[2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[u][e] = 0.f;
+        const int krow = 32 * u + 16 * (c >> 4) + 8 * ((c >> 2) & 1) + 4 * ((c >> 3) & 1) + (c & 3);
+#pragma unroll
+        for (int x = 0; x < D / 16; ++x) {
+          const f16x8 k8 = *reinterpret_cast<const f16x8*>(kb + krow * D * 2 + (((2 * x + h) ^ (krow & (D / 8 - 1))) << 4));
+          s[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k8, qv[x], s[u], 0, 0, 0);
+        }
+      }
+      // the largest value scale so far is the unit of acc
+      float top = vref;
+#pragma unroll
+      for (int b = 0; b < 4; ++b) top = fmaxf(top, cur.vs[b] < INFINITY ? cur.vs[b] : 0.f);
+      if (top > vref) {
+        const float f = vref > 0.f ? vref / top : 1.f;
+#pragma unroll
+        for (int d = 0; d < D / 32; ++d) acc[d] *= f;
+        vref = top;
+        vinv = kPBias / vref;
+      }
+      // result 16 u + 4 j + e: token 32 u + 16 (j / 2) + 8 h + 4 (j % 2) + e, block 2 u + j / 2.
+      // Hidden tokens get -inf, which stays one through the scales (at least 1e-18).
+      if (p < safe_lo || p + 64 > safe_hi || p + 64 > p1 || (cur.page[0] | cur.page[1] | cur.page[2] | cur.page[3]) < 0) {
+        const int from = lo - p - 8 * h, to = min(hi, p1) - p - 8 * h;
+#pragma unroll
+        for (int y = 0; y < 32; ++y) {
+          const int at = 16 * (y >> 3) + (y & 7);
+          s[y >> 4][y & 15] = at >= from && at < (cur.page[y >> 3] >= 0 ? to : 0) ? s[y >> 4][y & 15] : -INFINITY;
+        }
+      }
+      if (cur.bad) {
+        // a page that holds an infinity or NaN: what sees it becomes NaN
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+          if (cur.ks[b] < INFINITY && cur.vs[b] < INFINITY) continue;
+          cur.ks[b] = 1e-18f, cur.vs[b] = 0.f;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float t = s[b >> 1][8 * (b & 1) + e];
+            s[b >> 1][8 * (b & 1) + e] = t == -INFINITY ? t : __builtin_nanf("");
+          }
+        }
+      }
+      float mx = -INFINITY;
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        float t = s[b >> 1][8 * (b & 1)];
+#pragma unroll
+        for (int e = 1; e < 8; ++e) t = fmaxf(t, s[b >> 1][8 * (b & 1) + e]);
+        mx = fmaxf(mx, t * (cur.ks[b] * qmul));
+      }
+      mx = fmaxf(mx, __shfl_xor(mx, 32));
+      const float nm = fmaxf(m, mx);
+      if (__any(nm > m)) {
+        const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - nm);
+        sum *= f;
+#pragma unroll
+        for (int d = 0; d < D / 32; ++d) acc[d] *= f;
+        m = nm;
+      }
+      const float base = m == -INFINITY ? 0.f : m;
+      f16x8 pw[4];
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        const float k1 = cur.ks[b] * qmul, vs = cur.vs[b] * vinv;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float ex = __builtin_amdgcn_exp2f(fmaf(s[b >> 1][8 * (b & 1) + e], k1, -base));
+          sum += ex;
+          pw[b][e] = (f16)(ex * vs);
+        }
+      }
+#pragma unroll
+      for (int d = 0; d < D / 32; ++d) {
+        const int vrow = 32 * d + c;
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+          const f16x8 v8 = *reinterpret_cast<const f16x8*>(vb + vrow * 128 + (((2 * b + h) ^ (vrow & 7)) << 4));
+          acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v8, pw[b], acc[d], 0, 0, 0);
+        }
+      }
+      cur = next;
+      next = after;
+    }
+  }
+
+  // result 4 j + e of tile d: dimension 32 d + 8 j + 4 h + e
+  sum += __shfl_xor(sum, 32);
+  const float unit = vref * (1.f / kPBias);
+  typedef T T4 __attribute__((ext_vector_type(4)));
+  T* dst = (T*)a.out + ((int64_t)(start + i) * a.H + kh * G + row - i * G) * D + 4 * h;
+  if (parts == 1) {
+    const float inv = sum > 0.f ? unit / sum : (sum != sum ? sum : 0.f);
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        T4 y;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] = (T)(acc[d][4 * j + e] * inv);
+        if (live) *reinterpret_cast<T4*>(dst + 32 * d + 8 * j) = y;
+      }
+    return;
+  }
+
+  // partial rows, as in the kernel above: values, max, sum
+  constexpr int kSc1 = 16, kRec = D + 4;
+  const int item = index * a.KV + kh;
+  const __amdgpu_buffer_rsrc_t rp = rsrc(a.part + (int64_t)item * a.splits * kRows * kRec, (int64_t)parts * kRows * kRec * 4);
+  const int rrow = wave * 32 + c;
+  if (live) {
+    const int rec = (sp * kRows + rrow) * kRec * 4;
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        f32x4 y;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] = acc[d][4 * j + e] * unit;
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, y), rp, rec + 4 * (32 * d + 8 * j + 4 * h), 0, kSc1);
+      }
+    if (h == 0) {
+      __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, m), rp, rec + 4 * D, 0, kSc1);
+      __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, sum), rp, rec + 4 * D + 4, 0, kSc1);
+    }
+  }
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0);
+  __syncthreads();
+  if (tid == 0) {
+    const int old = __hip_atomic_fetch_add(&a.counters[item], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    s_last = old == parts - 1;
+  }
+  __syncthreads();
+  if (!s_last) return;
+  constexpr int kRowThreads = D / 4;
+  for (int y = tid / kRowThreads; y < rows; y += 256 / kRowThreads) {
+    const int dim = 4 * (tid % kRowThreads);
+    float jm = -INFINITY, jl = 0.f;
+    f32x4 jo = {0.f, 0.f, 0.f, 0.f};
+    for (int s0 = 0; s0 < parts; s0 += 4) {
+      float ms[4], ls[4];
+      f32x4 v[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int at = (min(s0 + k, parts - 1) * kRows + y) * kRec * 4;
+        ms[k] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rp, at + 4 * D, 0, kSc1));
+        ls[k] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rp, at + 4 * D + 4, 0, kSc1));
+        v[k] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rp, at + 4 * dim, 0, kSc1));
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) join(jm, jl, jo, ms[k], ls[k], v[k], s0 + k < parts);
+    }
+    const float inv = jl > 0.f ? 1.f / jl : (jl != jl ? jl : 0.f);
+    const int grow = rt * kRows + y;
+    T4 o;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = (T)(jo[e] * inv);
+    *reinterpret_cast<T4*>((T*)a.out + ((int64_t)(start + grow / G) * a.H + kh * G + grow % G) * D + dim) = o;
+  }
+  if (tid == 0) __hip_atomic_store(&a.counters[item], 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+template <typename T, int D>
+hipError_t many(const AttnArgs& a, bool fp8, int64_t wgs, hipStream_t stream) {
+  constexpr int kLds = 2 * 2 * 64 * D * 2;
+  if (fp8)
+    hipLaunchKernelGGL((attention_rows_kernel<T, D, true>), dim3((unsigned)wgs), dim3(256), kLds, stream, a);
+  else
+    hipLaunchKernelGGL((attention_rows_kernel<T, D, false>), dim3((unsigned)wgs), dim3(256), kLds, stream, a);
+  return hipGetLastError();
+}
+
 // Workgroups of the few-row kernel: what the CUs hold at once.
 int few_wgs(int64_t D) { return device_cu_count() * (D == 64 ? 4 : 2); }
+constexpr int kFewRows = 64;
+
+struct ManyPlan {
+  int64_t items;  // at most: row tiles of all requests x KV heads
+  int splits, per;
+  size_t part;
+};
+ManyPlan many_plan(const PagedAttention& p, const PagedCache& c) {
+  ManyPlan f = {};
+  const int64_t G = p.H / c.KV;
+  if (p.max_q * G <= kFewRows) return f;
+  // row tiles: every request's last one may be partly filled, and has more than kFewRows rows
+  const int64_t most = p.T * G / (kFewRows + 1) < p.R ? p.T * G / (kFewRows + 1) : p.R;
+  f.items = (p.T * G / kRows + most) * c.KV;
+  const int64_t range = p.window && p.window + p.max_q + 15 < p.max_kv ? p.window + p.max_q + 15 : p.max_kv;
+  // two workgroups a CU; a range of at least eight tiles, as its join costs about two
+  int64_t S = f.items > 0 ? 2 * device_cu_count() / f.items : 1;
+  if (S > range / 512) S = range / 512;
+  if (S < 1 || f.items > (int64_t)kWsCounterBytes / 4) S = 1;
+  f.per = (int)(((range + S - 1) / S + 63) / 64 * 64);
+  if (f.per < 64) f.per = 64;
+  f.splits = (int)((range + f.per - 1) / f.per);
+  if (f.splits < 1) f.splits = 1;
+  f.part = f.splits > 1 ? (size_t)(f.items * f.splits * kRows * (c.D + 4) * 4) : 0;
+  return f;
+}
 
 }  // namespace
 
 size_t paged_attention_ws_bytes(const PagedAttention& p, const PagedCache& c) {
-  return kWsCounterBytes + (size_t)few_wgs(c.D) * 32 * (c.D + 4) * 4;
+  const size_t few = (size_t)few_wgs(c.D) * 32 * (c.D + 4) * 4, many = many_plan(p, c).part;
+  return kWsCounterBytes + (few > many ? few : many);
 }
 
 hipError_t launch_paged_attention(const PagedAttention& p, const PagedCache& c, void* workspace, size_t ws_bytes,
@@ -561,12 +968,26 @@ hipError_t launch_paged_attention(const PagedAttention& p, const PagedCache& c, 
                 p.q_starts, p.stride, p.q_token, p.q_head, c.pages, (int)p.T, (int)p.R, (int)p.width, (int)p.H,
                 (int)c.KV, (int)c.ps, __builtin_ctz((unsigned)c.ps), (int)p.window, p.scale};
   a.max_q = (int)p.max_q, a.max_kv = (int)p.max_kv;
-  a.few_rows = 0x7fffffff;
+  a.few_rows = kFewRows;
   a.counters = (int*)workspace;
   a.part = (float*)((char*)workspace + kWsCounterBytes);
+  const ManyPlan f = many_plan(p, c);
   const int wgs = few_wgs(c.D);
-  if (p.bf16) return c.D == 64 ? few<__bf16, 64>(a, c.fp8, wgs, stream) : few<__bf16, 128>(a, c.fp8, wgs, stream);
-  return c.D == 64 ? few<f16, 64>(a, c.fp8, wgs, stream) : few<f16, 128>(a, c.fp8, wgs, stream);
+  hipError_t e = hipSuccess;
+  // Any batch of several requests may have some of few rows; a lone one stays with many.
+  if (f.items > 0 && p.R == 1) {
+    a.few_rows = 0;
+  } else {
+    if (p.bf16)
+      e = c.D == 64 ? few<__bf16, 64>(a, c.fp8, wgs, stream) : few<__bf16, 128>(a, c.fp8, wgs, stream);
+    else
+      e = c.D == 64 ? few<f16, 64>(a, c.fp8, wgs, stream) : few<f16, 128>(a, c.fp8, wgs, stream);
+  }
+  if (e != hipSuccess || f.items == 0) return e;
+  a.splits = f.splits, a.per = f.per;
+  const int64_t n = f.items * f.splits;
+  if (p.bf16) return c.D == 64 ? many<__bf16, 64>(a, c.fp8, n, stream) : many<__bf16, 128>(a, c.fp8, n, stream);
+  return c.D == 64 ? many<f16, 64>(a, c.fp8, n, stream) : many<f16, 128>(a, c.fp8, n, stream);
 }
 
 }  // namespace pmi

@@ -87,7 +87,7 @@ def test_append_refuses(change):
                                     dict(H=6, KV=4), dict(H=65, KV=1), dict(stride=513), dict(head=4), dict(T=-1),
                                     dict(R=-1), dict(width=5), dict(max_q=-1), dict(max_kv=-1), dict(window=-1),
                                     dict(starts=None), dict(T=1 << 40), dict(width=1 << 40, tstride=1 << 40),
-                                    dict(max_kv=1 << 40), dict(max_q=1 << 40), dict(q=None), dict(q=P8 + 8),
+                                    dict(max_kv=1 << 40), dict(q=None), dict(q=P8 + 8),
                                     dict(out=None), dict(lens=None), dict(tables=None), dict(k=None),
                                     dict(window=1 << 40), dict(R=1 << 40)])
 def test_attention_refuses(change):
