@@ -168,7 +168,12 @@ PMI_DEV void join(float& m, float& l, f32x4& o, float pm, float pl, f32x4 po, bo
 }
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kPBias = 16384.f;  // probabilities are held in fp16 times this
+// Probabilities are held in fp16 times kPBias. The reference that the scores are taken off is not
+// raised to a new maximum before this is 2^kSlack times what it was (and the unit of the values'
+// scales not before they have doubled): raising it rescales all sums, and some row of a tile has a
+// new maximum more often than not. 2^8 2^6 2 < 65504, and what is lost under fp16's range is
+// below 2^-25 / 2^8 of the largest probability.
+constexpr float kPBias = 256.f, kSlack = 6.f;
 
 // ---- few query rows ------------------------------------------------------------------
 // Requests of few query rows (tokens x heads of one KV head): bound by the bytes of the
@@ -335,9 +340,9 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(AttnArgs a) {
       entry = look_up(p + 512);
       load_k(next_page, p + 256);
     }
-    // the largest value scale so far is the unit of acc
+    // the unit of acc: the largest value scale so far, or half of it
     const float top = fmaxf(vref, max_over_h(tvs < INFINITY ? tvs : 0.f));
-    if (__any(top > vref)) {
+    if (__any(top > 2.f * vref)) {
       const float f = vref > 0.f ? vref / top : 1.f;
 #pragma unroll
       for (int d = 0; d < DT; ++d) acc[d] *= f;
@@ -358,7 +363,7 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(AttnArgs a) {
     for (int e = 1; e < 16; ++e) mx = fmaxf(mx, x[e]);
     mx = max_over_h(mx);
     const float nm = fmaxf(m, mx);
-    if (__any(nm > m)) {
+    if (__any(nm > m + kSlack)) {
       const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - nm);
       sum *= f;
 #pragma unroll
@@ -695,17 +700,19 @@ __global__ __launch_bounds__(256, 2) void attention_rows_kernel(AttnArgs a) {
     const int lo2 = b & 1 ? v[1] : v[0], hi2 = b & 1 ? v[3] : v[2];
     return b & 2 ? hi2 : lo2;
   };
+  // A wave's 64 pieces of 16 bytes (piece tid + 256 k of the tile, token-major for K, dimension-major
+  // in a block for V) are all of one block, so that addresses are the same but for a constant.
   u32x4 kw[KP], vw[KP];
+  auto block_of = [&](int k) { return (64 * wave + 256 * k) / D; };
   auto load_tile = [&](int p, const Blocks& x) {
 #pragma unroll
     for (int k = 0; k < KP; ++k) {
-      const int idx = tid + 256 * k;
-      const int krow = idx / (D / 16), kpiece = idx % (D / 16);
-      const int64_t kc = (int64_t)max(pick(x.page, krow >> 4), 0) * a.KV + kh;
-      kw[k] = *reinterpret_cast<const u32x4*>(a.k + kc * cell_bytes + ((p + krow) & (a.ps - 1)) * D + 16 * kpiece);
-      const int vblk = idx / D, vd = idx % D;
-      const int64_t vc = (int64_t)max(pick(x.page, vblk), 0) * a.KV + kh;
-      vw[k] = *reinterpret_cast<const u32x4*>(a.v + vc * cell_bytes + ((((p + 16 * vblk) & (a.ps - 1)) >> 4) * D + vd) * 16);
+      const int idx = tid + 256 * k, b = block_of(k);
+      const int64_t cell = (int64_t)max(pick(x.page, b), 0) * a.KV + kh;
+      const int tok = (p + 16 * b) & (a.ps - 1);
+      const int64_t at = cell * cell_bytes + tok * D;  // of both: a block of v is 16 tokens of D bytes
+      kw[k] = *reinterpret_cast<const u32x4*>(a.k + at + (uint32_t)(16 * (idx % D)));
+      vw[k] = *reinterpret_cast<const u32x4*>(a.v + at + (uint32_t)(16 * (idx % D)));
     }
   };
   auto store_tile = [&](int p, const Blocks& x, int slot) {
@@ -720,7 +727,7 @@ __global__ __launch_bounds__(256, 2) void attention_rows_kernel(AttnArgs a) {
       const f16x8 k0 = codes8<FP8>(kw[k][0], kw[k][1]), k1 = codes8<FP8>(kw[k][2], kw[k][3]);
       *reinterpret_cast<f16x8*>(kb + krow * D * 2 + (((2 * kpiece) ^ (krow & (D / 8 - 1))) << 4)) = k0;
       *reinterpret_cast<f16x8*>(kb + krow * D * 2 + (((2 * kpiece + 1) ^ (krow & (D / 8 - 1))) << 4)) = k1;
-      const int vblk = idx / D, vd = idx % D;
+      const int vblk = block_of(k), vd = idx % D;
       if (edge) vw[k] &= byte_mask(first_seen - p - 16 * vblk, pick(x.page, vblk) < 0 ? 0 : p1 - p - 16 * vblk);
       const f16x8 v0 = codes8<FP8>(vw[k][0], vw[k][1]), v1 = codes8<FP8>(vw[k][2], vw[k][3]);
       *reinterpret_cast<f16x8*>(vb + vd * 128 + (((2 * vblk) ^ (vd & 7)) << 4)) = v0;
@@ -762,11 +769,11 @@ __global__ __launch_bounds__(256, 2) void attention_rows_kernel(AttnArgs a) {
           s[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k8, qv[x], s[u], 0, 0, 0);
         }
       }
-      // the largest value scale so far is the unit of acc
+      // the unit of acc: the largest value scale so far, or half of it
       float top = vref;
 #pragma unroll
       for (int b = 0; b < 4; ++b) top = fmaxf(top, cur.vs[b] < INFINITY ? cur.vs[b] : 0.f);
-      if (top > vref) {
+      if (top > 2.f * vref) {
         const float f = vref > 0.f ? vref / top : 1.f;
 #pragma unroll
         for (int d = 0; d < D / 32; ++d) acc[d] *= f;
@@ -806,7 +813,7 @@ __global__ __launch_bounds__(256, 2) void attention_rows_kernel(AttnArgs a) {
       }
       mx = fmaxf(mx, __shfl_xor(mx, 32));
       const float nm = fmaxf(m, mx);
-      if (__any(nm > m)) {
+      if (__any(nm > m + kSlack)) {
         const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - nm);
         sum *= f;
 #pragma unroll
