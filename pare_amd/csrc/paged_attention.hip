@@ -748,15 +748,14 @@ __global__ __launch_bounds__(256, 2) void attention_rows_kernel(AttnArgs a) {
     int slot = 0;
     for (int p = p0; p < p1; p += 64, slot ^= 1) {
       __syncthreads();  // the slot is written; the other one is read
-      Blocks after = next;
-      if (p + 64 < p1) {
-        store_tile(p + 64, next, slot ^ 1);
-        after = blocks_of(p + 128, entry);
-        load_tile(p + 128, after);
-        look_up(p + 192, entry);
-      }
+      // (past the range: page 0 of the cache, never used)
+      store_tile(p + 64, next, slot ^ 1);
+      const Blocks after = blocks_of(p + 128, entry);
+      load_tile(p + 128, after);
+      look_up(p + 192, entry);
       const uint8_t* kb = lds + slot * 2 * kSlot;
       const uint8_t* vb = kb + kSlot;
+      __builtin_amdgcn_s_setprio(1);  // products ahead of the other wave's softmax
       f32x16 s[2];
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
@@ -769,6 +768,7 @@ __global__ __launch_bounds__(256, 2) void attention_rows_kernel(AttnArgs a) {
           s[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k8, qv[x], s[u], 0, 0, 0);
         }
       }
+      __builtin_amdgcn_s_setprio(0);
       // the unit of acc: the largest value scale so far, or half of it
       float top = vref;
 #pragma unroll
@@ -821,24 +821,21 @@ __global__ __launch_bounds__(256, 2) void attention_rows_kernel(AttnArgs a) {
         m = nm;
       }
       const float base = m == -INFINITY ? 0.f : m;
-      f16x8 pw[4];
 #pragma unroll
       for (int b = 0; b < 4; ++b) {
         const float k1 = cur.ks[b] * qmul, vs = cur.vs[b] * vinv;
+        f16x8 pw;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const float ex = __builtin_amdgcn_exp2f(fmaf(s[b >> 1][8 * (b & 1) + e], k1, -base));
           sum += ex;
-          pw[b][e] = (f16)(ex * vs);
+          pw[e] = (f16)(ex * vs);
         }
-      }
 #pragma unroll
-      for (int d = 0; d < D / 32; ++d) {
-        const int vrow = 32 * d + c;
-#pragma unroll
-        for (int b = 0; b < 4; ++b) {
+        for (int d = 0; d < D / 32; ++d) {
+          const int vrow = 32 * d + c;
           const f16x8 v8 = *reinterpret_cast<const f16x8*>(vb + vrow * 128 + (((2 * b + h) ^ (vrow & 7)) << 4));
-          acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v8, pw[b], acc[d], 0, 0, 0);
+          acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v8, pw, acc[d], 0, 0, 0);
         }
       }
       cur = next;
