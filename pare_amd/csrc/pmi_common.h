@@ -153,6 +153,30 @@ PMI_DEV void copy_to_lds(__amdgpu_buffer_rsrc_t r, void* lds, int voff, int soff
 #endif
 }
 
+// Buffer descriptor in SGPRs (untyped dwords, no swizzle) for the copies of dma16.
+PMI_DEV u32x4 descriptor(const void* p, uint32_t bytes) {
+  const uint64_t a = (uint64_t)p;
+  u32x4 d = {(uint32_t)a, (uint32_t)(a >> 32) & 0xFFFFu, bytes, 0x00020000u};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) d[i] = __builtin_amdgcn_readfirstlane(d[i]);
+  return d;
+}
+
+// 16 bytes per lane from a buffer to LDS address base + 16 * lane, from inline asm: the
+// compiler, which cannot tell two LDS slots apart, would drain copies made with the builtin
+// before every read of the other slot. base is uniform. No register but m0 is written, which
+// is reserved (a clobber list may not name it): the compiler sets it right ahead of each of
+// its own uses, so it is for kernels that have none. The caller waits with wait_vmcnt<0>.
+PMI_DEV void dma16(u32x4 r, uint32_t base, int voff, int soff) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(base),
+               "v"(voff), "s"(r), "s"(__builtin_amdgcn_readfirstlane(soff))
+               : "memory");
+#else
+  (void)r, (void)base, (void)voff, (void)soff;
+#endif
+}
+
 // Workgroup barrier without the fence of __syncthreads(): that fence counts
 // in-flight buffer->LDS copies as pending LDS stores and would drain the whole
 // ring at every step. Callers order memory themselves (vmcnt waits before,

@@ -100,29 +100,7 @@ struct Shape {
   static_assert(kGroup <= 80 * 1024, "two groups fit the LDS of a CU");
 };
 
-// Buffer descriptor in SGPRs (untyped dwords, no swizzle) for the copies
-// below.
-PMI_DEV u32x4 descriptor(const void* p, uint32_t bytes) {
-  const uint64_t a = (uint64_t)p;
-  u32x4 d = {(uint32_t)a, (uint32_t)(a >> 32) & 0xFFFFu, bytes, 0x00020000u};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) d[i] = __builtin_amdgcn_readfirstlane(d[i]);
-  return d;
-}
-
-// 16 (or 4) bytes per lane from a buffer to LDS address base + 16 (4) * lane.
-// base is uniform. No register but m0 is written, which is reserved (a clobber list
-// may not name it): the compiler sets it right ahead of each of its own uses, and
-// has none in this kernel. The caller waits with wait_vmcnt<0>.
-PMI_DEV void dma16(u32x4 r, uint32_t base, int voff, int soff) {
-#if defined(__HIP_DEVICE_COMPILE__)
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(base),
-               "v"(voff), "s"(r), "s"(__builtin_amdgcn_readfirstlane(soff))
-               : "memory");
-#else
-  (void)r, (void)base, (void)voff, (void)soff;
-#endif
-}
+// 4 bytes per lane, as dma16 copies 16.
 PMI_DEV void dma4(u32x4 r, uint32_t base, int voff, int soff) {
 #if defined(__HIP_DEVICE_COMPILE__)
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, %3 offen lds" ::"s"(base),

@@ -4,10 +4,12 @@
 //   code = round(x * 127 / amax),  scale = amax / 127     (per row of K values)
 //   y[m, n] = sx[m] sw[n] sum_k cx[m, k] cw[n, k] (+ bias[n])
 //
-// The sum is exact in int32 (K <= 131072: 127^2 K < 2^31); the scales are applied
-// in fp32 and y is rounded once. The reference only simulates this (its
-// quantize_inputs path rounds the activations and multiplies in floating point,
-// pare/layers/linear.py:120-138).
+// The sum is exact in int32 (K <= 131072: 127^2 K < 2^31), so neither the order of the
+// products nor a split of K changes a bit; the scales are applied in fp32 and y is
+// rounded once. The reference only simulates this (its quantize_inputs path rounds the
+// activations and multiplies in floating point, pare/layers/linear.py:120-138).
+#include <atomic>
+
 #include "pmi_common.h"
 #include "pmi_launch.h"
 #include "w8a8.h"
@@ -15,16 +17,51 @@
 namespace pmi {
 namespace {
 
-// Codes of a row, zeros from K to ld. One workgroup per row.
+typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
+typedef int32_t i32x16 __attribute__((ext_vector_type(16)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
+template <typename T>
+using vec8 = T __attribute__((ext_vector_type(8)));
+
+// ---- quantisation of rows ----------------------------------------------------------
+
+template <typename T>
+PMI_DEV uint32_t abs_max8(const T* p, int n, bool wide, vec8<T>& v) {
+  if (wide) {
+    v = *reinterpret_cast<const vec8<T>*>(p);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = e < n ? p[e] : (T)0.f;
+  }
+  uint32_t m = 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) m = max(m, __builtin_bit_cast(uint32_t, (float)v[e]) & 0x7fffffffu);
+  return m;
+}
+
+// Codes of a row, zeros from K to ld. One workgroup of 256 threads per row, eight values a
+// thread and step; the first kKeep steps (rows up to 8192) stay in registers between the
+// maximum and the codes. |x| is compared as bits, where infinities and NaN are the largest.
 template <typename T>
 __global__ __launch_bounds__(256) void quantize_rows_kernel(const T* __restrict__ x, int64_t x_ld,
                                                             int8_t* __restrict__ codes, float* __restrict__ scales,
-                                                            int K, int ld) {
+                                                            int K, int ld, int wide) {
+  constexpr int kKeep = 4;
   __shared__ uint32_t red[4];
   const int tid = threadIdx.x;
   const T* row = x + (int64_t)blockIdx.x * x_ld;
+  vec8<T> keep[kKeep];
   uint32_t m = 0;
-  for (int k = tid; k < K; k += 256) m = max(m, __builtin_bit_cast(uint32_t, (float)row[k]) & 0x7fffffffu);
+#pragma unroll
+  for (int i = 0; i < kKeep; ++i) {
+    const int k = 8 * (tid + 256 * i);
+    if (k < K) m = max(m, abs_max8(row + k, K - k, wide && k + 8 <= K, keep[i]));
+  }
+  for (int k = 8 * (tid + 256 * kKeep); k < K; k += 2048) {
+    vec8<T> v;
+    m = max(m, abs_max8(row + k, K - k, wide && k + 8 <= K, v));
+  }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, o));
   if ((tid & 63) == 0) red[tid >> 6] = m;
@@ -34,35 +71,299 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(const T* __restrict_
   const float inv = amax > 0.f ? 127.f / amax : 0.f;
   if (tid == 0) scales[blockIdx.x] = amax * (1.f / 127.f);
   int8_t* out = codes + (int64_t)blockIdx.x * ld;
-  for (int k = tid; k < ld; k += 256)
-    out[k] = k < K ? (int8_t)(int)fminf(fmaxf(rintf((float)row[k] * inv), -127.f), 127.f) : (int8_t)0;
+  auto put = [&](int k, const vec8<T>& v) {
+    u32x2 w = {0, 0};
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int q = (int)fminf(fmaxf(rintf((float)v[e] * inv), -127.f), 127.f);
+      w[e >> 2] |= (uint32_t)(q & 255) << (8 * (e & 3));
+    }
+    *reinterpret_cast<u32x2*>(out + k) = w;
+  };
+#pragma unroll
+  for (int i = 0; i < kKeep; ++i) {
+    const int k = 8 * (tid + 256 * i);
+    if (k < K) put(k, keep[i]);
+  }
+  for (int k = 8 * (tid + 256 * kKeep); k < K; k += 2048) {
+    vec8<T> v;
+    abs_max8(row + k, K - k, wide && k + 8 <= K, v);
+    put(k, v);
+  }
+  // (K <= 8 (tid + ..) < ld: at most one thread, the columns between K rounded up to 8 and to 16)
+  const int tail = (K + 7) / 8 * 8;
+  if (tid == 0 && tail < ld) *reinterpret_cast<u32x2*>(out + tail) = u32x2{0, 0};
 }
 
+// y of eight neighbouring columns n .. n + 7 of row m from their sums.
 template <typename T>
-__global__ __launch_bounds__(256) void w8a8_kernel(const int8_t* __restrict__ x, const float* __restrict__ sx,
-                                                   const int8_t* __restrict__ w, const float* __restrict__ sw,
-                                                   const T* __restrict__ bias, T* __restrict__ y, int M, int N,
-                                                   int ld) {
-  const int n = blockIdx.x * 16 + (threadIdx.x >> 4), m = blockIdx.y * 16 + (threadIdx.x & 15);
-  if (n >= N || m >= M) return;
-  const u32x4* xr = reinterpret_cast<const u32x4*>(x + (int64_t)m * ld);
-  const u32x4* wr = reinterpret_cast<const u32x4*>(w + (int64_t)n * ld);
-  int s = 0;
-  for (int k = 0; k < ld / 16; ++k) {
-    const u32x4 a = xr[k], b = wr[k];
+PMI_DEV void store_row8(T* __restrict__ y, const int* sums, const float* sw, const float* bias, float sx, int m, int n,
+                        int N, bool wide) {
+  vec8<T> o;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) s = __builtin_amdgcn_sdot4((int)a[e], (int)b[e], s, false);
+  for (int e = 0; e < 8; ++e) o[e] = (T)((float)sums[e] * sx * sw[e] + bias[e]);
+  T* at = y + (int64_t)m * N + n;
+  if (wide && n + 8 <= N) {
+    *reinterpret_cast<vec8<T>*>(at) = o;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (n + e < N) at[e] = o[e];
   }
-  float v = (float)s * sx[m] * sw[n];
-  if (bias) v += (float)bias[n];
-  y[(int64_t)m * N + n] = (T)v;
+}
+
+// ---- many rows ---------------------------------------------------------------------
+// BN weight rows x BM activation rows per workgroup of WN x WM waves, in steps of 128
+// columns. Both operands' rows go from memory straight to LDS (two slots, one barrier a step; the
+// copies of the next step fly while this one is multiplied); 16-byte chunk c of row r lies at
+// chunk c ^ (r % 8), so that reads of eight consecutive rows fall in different banks. Products
+// 32x32x32: the weights are the rows of the result, so that a wave reads (BN / WN + BM / WM) x
+// 32 bytes for BN / WN x BM / WM / 1024 of them. Columns past ld and rows past the end are copied
+// as zeros (from past the descriptor's end). The sums go through LDS, 32 activation rows at a
+// time, to be written 16 bytes a lane.
+template <typename T, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(64 * WM * WN) void w8a8_tiles_kernel(W8A8 p, int grid_m, int grid_n, int chunk) {
+  constexpr int NW = WM * WN, TM = BM / WM / 32, TN = BN / WN / 32;
+  constexpr int kSlot = (BM + BN) * 128;
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+  const int tid = threadIdx.x, l = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave % WM, wn = wave / WM;
+  const int c = l & 31, h = l >> 5;
+  // Workgroup 8 k + x runs on XCD x and takes tile x chunk + k of the list: blocks of eight tiles of
+  // activation rows, columns of weights inside, so that an XCD's tiles share rows of both.
+  const int tile = (blockIdx.x % 8) * chunk + blockIdx.x / 8;
+  if ((int)blockIdx.x / 8 >= chunk || tile >= grid_m * grid_n) return;
+  const int band = tile / (8 * grid_n), in_band = tile - band * 8 * grid_n;
+  const int band_rows = min(8, grid_m - 8 * band);
+  const int m0 = (8 * band + in_band % band_rows) * BM, n0 = in_band / band_rows * BN;
+  const int M = (int)p.M, N = (int)p.N, ld = (int)p.ld;
+  const int rows_m = min(BM, M - m0), rows_n = min(BN, N - n0);
+  const u32x4 dx = descriptor(p.x + (int64_t)m0 * ld, (uint32_t)rows_m * ld);
+  const u32x4 dw = descriptor(p.w + (int64_t)n0 * ld, (uint32_t)rows_n * ld);
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
+
+  // a copy: eight rows of 128 bytes, lane 8 r + c chunk c ^ r of row r
+  const int crow = l >> 3, ccol = 16 * ((l & 7) ^ (l >> 3));
+  auto copy = [&](int kt, int slot) {
+    const int k = 128 * kt + ccol;
+    const int at = k < ld ? crow * ld + ccol : 0x7ffffff0;  // past the end: zeros
+#pragma unroll
+    for (int i = 0; i < BN / 8 / NW; ++i) {
+      const int r = 8 * (wave + NW * i);
+      dma16(dw, lds0 + slot * kSlot + r * 128, k < ld ? at + r * ld : at, 128 * kt);
+    }
+#pragma unroll
+    for (int i = 0; i < BM / 8 / NW; ++i) {
+      const int r = 8 * (wave + NW * i);
+      dma16(dx, lds0 + slot * kSlot + BN * 128 + r * 128, k < ld ? at + r * ld : at, 128 * kt);
+    }
+  };
+
+  i32x16 acc[TN][TM];
+#pragma unroll
+  for (int i = 0; i < TN; ++i)
+#pragma unroll
+    for (int j = 0; j < TM; ++j)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[i][j][e] = 0;
+
+  const int steps = (ld + 127) / 128;
+  copy(0, 0);
+  for (int kt = 0; kt < steps; ++kt) {
+    wait_vmcnt_lgkm0<0>();  // this wave's copies have arrived, its reads of the other slot are done
+    barrier_only();
+    const int slot = kt & 1;
+    if (kt + 1 < steps) copy(kt + 1, slot ^ 1);
+    const uint8_t* wb = lds + slot * kSlot + (wn * (BN / WN) + c) * 128;
+    const uint8_t* xb = lds + slot * kSlot + BN * 128 + (wm * (BM / WM) + c) * 128;
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) {
+      const int at = 16 * ((2 * ks + h) ^ (c & 7));
+      i32x4 wv[TN], xv[TM];
+#pragma unroll
+      for (int i = 0; i < TN; ++i) wv[i] = *reinterpret_cast<const i32x4*>(wb + 32 * 128 * i + at);
+#pragma unroll
+      for (int j = 0; j < TM; ++j) xv[j] = *reinterpret_cast<const i32x4*>(xb + 32 * 128 * j + at);
+#pragma unroll
+      for (int i = 0; i < TN; ++i)
+#pragma unroll
+        for (int j = 0; j < TM; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(wv[i], xv[j], acc[i][j], 0, 0, 0);
+    }
+  }
+  wait_lgkm0();
+  barrier_only();  // every wave has read the last step: the slots are free
+
+  // result 4 e + f of tile (i, j): weight row 32 i + 8 e + 4 h + f, activation row 32 j + c
+  constexpr int kRow = BN / WN + 4;  // words of a row of sums, rows 16 bytes apart in the banks
+  constexpr int kLanes = BN / WN / 8, kStep = 64 / kLanes;  // lanes a row, rows a step
+  int* buf = reinterpret_cast<int*>(lds) + wave * 32 * kRow;
+  const int n = n0 + wn * (BN / WN) + 8 * (l % kLanes);
+  float sw[8], bias[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    sw[e] = n + e < N ? p.sw[n + e] : 0.f;
+    bias[e] = p.bias && n + e < N ? (float)((const T*)p.bias)[n + e] : 0.f;
+  }
+  const bool wide = N % 8 == 0 && (uintptr_t)p.y % (8 * sizeof(T)) == 0;
+#pragma unroll
+  for (int j = 0; j < TM; ++j) {
+#pragma unroll
+    for (int i = 0; i < TN; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        *reinterpret_cast<i32x4*>(buf + c * kRow + 32 * i + 8 * e + 4 * h) =
+            i32x4{acc[i][j][4 * e], acc[i][j][4 * e + 1], acc[i][j][4 * e + 2], acc[i][j][4 * e + 3]};
+    // (one wave's own rows: ordered by its LDS counter alone)
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+    for (int s = 0; s < 32; s += kStep) {
+      const int r = s + l / kLanes, m = m0 + wm * (BM / WM) + 32 * j + r;
+      const int* at = buf + r * kRow + 8 * (l % kLanes);
+      int sums[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sums[e] = at[e];
+      if (m < M && n < N) store_row8((T*)p.y, sums, sw, bias, p.sx[m], m, n, N, wide);
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  }
+}
+
+template <typename T, int BM, int BN, int WM, int WN>
+hipError_t tiles(const W8A8& p, hipStream_t stream) {
+  constexpr int kWaves = WM * WN, kOut = kWaves * 32 * (BN / WN + 4) * 4, kIn = 2 * (BM + BN) * 128;
+  constexpr int kLds = kOut > kIn ? kOut : kIn;
+  static_assert(kLds <= 160 * 1024, "LDS of a CU");
+  static std::atomic<uint64_t> allowed{0};
+  int dev = 0;
+  if (hipError_t e = hipGetDevice(&dev); e != hipSuccess) return e;
+  const uint64_t bit = 1ull << (dev & 63);
+  const void* fn = reinterpret_cast<const void*>(&w8a8_tiles_kernel<T, BM, BN, WM, WN>);
+  if (!(allowed.load() & bit)) {
+    if (hipError_t e = hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024); e != hipSuccess)
+      return e;
+    allowed.fetch_or(bit);
+  }
+  const int gm = (int)((p.M + BM - 1) / BM), gn = (int)((p.N + BN - 1) / BN);
+  const int chunk = (int)(((int64_t)gm * gn + 7) / 8);
+  hipLaunchKernelGGL((w8a8_tiles_kernel<T, BM, BN, WM, WN>), dim3((unsigned)chunk * 8), dim3(64 * kWaves), kLds, stream, p,
+                     gm, gn, chunk);
+  return hipGetLastError();
+}
+
+// ---- few rows ----------------------------------------------------------------------
+// Up to 64 activation rows: bound by the bytes of the weights. A workgroup takes 16 NT weight
+// rows, its eight waves the steps of 64 columns in turn; both operands come straight from memory
+// to registers (the activations from L2), 16x16x64 products, the weights the rows of the
+// result. The waves' sums are added through LDS.
+template <typename T, int MT, int NT>
+__global__ __launch_bounds__(512, 2) void w8a8_few_kernel(W8A8 p) {
+  constexpr int kFly = 8 / (MT + NT) < 1 ? 1 : 8 / (MT + NT);  // steps in flight ahead
+  __shared__ __attribute__((aligned(16))) int sums[16 * MT][16 * NT + 4];
+  const int tid = threadIdx.x, l = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int c = l & 15, h = l >> 4;
+  const int n0 = blockIdx.x * 16 * NT;
+  const int M = (int)p.M, N = (int)p.N, ld = (int)p.ld;
+  for (int i = tid; i < 16 * MT * (16 * NT + 4); i += 512) (&sums[0][0])[i] = 0;
+  // rows past the end read the last one, and are not stored
+  const int8_t* wrow[NT];
+  const int8_t* xrow[MT];
+#pragma unroll
+  for (int i = 0; i < NT; ++i) wrow[i] = p.w + (int64_t)min(n0 + 16 * i + c, N - 1) * ld;
+#pragma unroll
+  for (int j = 0; j < MT; ++j) xrow[j] = p.x + (int64_t)min(16 * j + c, M - 1) * ld;
+  i32x4 acc[NT][MT];
+#pragma unroll
+  for (int i = 0; i < NT; ++i)
+#pragma unroll
+    for (int j = 0; j < MT; ++j) acc[i][j] = i32x4{0, 0, 0, 0};
+  const i32x4 zero = {0, 0, 0, 0};
+  const int full = ld / 64;  // whole steps
+  i32x4 wv[kFly][NT], xv[kFly][MT];
+  auto load = [&](int f, int s) {  // step s, or (past the end) the first again
+    const int k = 64 * (s < full ? s : 0) + 16 * h;
+#pragma unroll
+    for (int i = 0; i < NT; ++i) wv[f][i] = __builtin_nontemporal_load(reinterpret_cast<const i32x4*>(wrow[i] + k));
+#pragma unroll
+    for (int j = 0; j < MT; ++j) xv[f][j] = *reinterpret_cast<const i32x4*>(xrow[j] + k);
+  };
+  auto multiply = [&](int f) {
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+      for (int j = 0; j < MT; ++j)
+        acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wv[f][i], xv[f][j], acc[i][j], 0, 0, 0);
+  };
+  if (wave < full) {
+    int s = wave;
+#pragma unroll
+    for (int f = 0; f < kFly; ++f) load(f, s + 8 * f);
+    for (; s + 8 * kFly < full; s += 8 * kFly) {
+#pragma unroll
+      for (int f = 0; f < kFly; ++f) {
+        multiply(f);
+        load(f, s + 8 * (f + kFly));
+      }
+    }
+#pragma unroll
+    for (int f = 0; f < kFly; ++f)
+      if (s + 8 * f < full) multiply(f);
+  }
+  if (wave == full % 8 && ld % 64) {  // the columns behind the last whole step: 16, 32 or 48
+    const int k = 64 * full + 16 * h;
+#pragma unroll
+    for (int i = 0; i < NT; ++i) wv[0][i] = k < ld ? *reinterpret_cast<const i32x4*>(wrow[i] + k) : zero;
+#pragma unroll
+    for (int j = 0; j < MT; ++j) xv[0][j] = k < ld ? *reinterpret_cast<const i32x4*>(xrow[j] + k) : zero;
+    multiply(0);
+  }
+  __syncthreads();  // sums are cleared
+  // result e of tile (i, j): weight row 16 i + 4 h + e, activation row 16 j + c
+#pragma unroll
+  for (int i = 0; i < NT; ++i)
+#pragma unroll
+    for (int j = 0; j < MT; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) atomicAdd(&sums[16 * j + c][16 * i + 4 * h + e], acc[i][j][e]);
+  __syncthreads();
+  const bool wide = N % 8 == 0 && (uintptr_t)p.y % (8 * sizeof(T)) == 0;
+  for (int u = tid; u < M * 2 * NT; u += 512) {
+    const int m = u / (2 * NT), n = n0 + 8 * (u % (2 * NT));
+    if (n >= N) continue;
+    float sw[8], bias[8];
+    int v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      v[e] = sums[m][n - n0 + e];
+      sw[e] = n + e < N ? p.sw[n + e] : 0.f;
+      bias[e] = p.bias && n + e < N ? (float)((const T*)p.bias)[n + e] : 0.f;
+    }
+    store_row8((T*)p.y, v, sw, bias, p.sx[m], m, n, N, wide);
+  }
+}
+
+template <typename T, int MT>
+hipError_t few(const W8A8& p, hipStream_t stream) {
+  const int64_t cus = device_cu_count();
+  // 64 weight rows a workgroup where that still gives every CU two of them
+  const dim3 block(512);
+  if (p.N >= 128 * cus)
+    hipLaunchKernelGGL((w8a8_few_kernel<T, MT, 4>), dim3((unsigned)((p.N + 63) / 64)), block, 0, stream, p);
+  else if (p.N >= 64 * cus)
+    hipLaunchKernelGGL((w8a8_few_kernel<T, MT, 2>), dim3((unsigned)((p.N + 31) / 32)), block, 0, stream, p);
+  else
+    hipLaunchKernelGGL((w8a8_few_kernel<T, MT, 1>), dim3((unsigned)((p.N + 15) / 16)), block, 0, stream, p);
+  return hipGetLastError();
 }
 
 template <typename T>
 hipError_t product(const W8A8& p, hipStream_t stream) {
-  hipLaunchKernelGGL(w8a8_kernel<T>, dim3((unsigned)((p.N + 15) / 16), (unsigned)((p.M + 15) / 16)), dim3(256), 0,
-                     stream, p.x, p.sx, p.w, p.sw, (const T*)p.bias, (T*)p.y, (int)p.M, (int)p.N, (int)p.ld);
-  return hipGetLastError();
+  if (p.M <= 16) return few<T, 1>(p, stream);
+  if (p.M <= 32) return few<T, 2>(p, stream);
+  if (p.M <= 64) return few<T, 4>(p, stream);
+  // 256 x 256 tiles where they fill the CUs, else 128 x 128
+  const int64_t big = ((p.M + 255) / 256) * ((p.N + 255) / 256);
+  if (big >= device_cu_count()) return tiles<T, 256, 256, 4, 2>(p, stream);
+  return tiles<T, 128, 128, 2, 2>(p, stream);
 }
 
 }  // namespace
@@ -70,15 +371,17 @@ hipError_t product(const W8A8& p, hipStream_t stream) {
 hipError_t launch_quantize_rows(const void* x, int x_dtype, int64_t x_ld, int8_t* codes, float* scales, int64_t M,
                                 int64_t K, int64_t ld, hipStream_t stream) {
   const dim3 grid((unsigned)M), block(256);
+  const int size = x_dtype == 2 ? 4 : 2;
+  const int wide = (uintptr_t)x % (8 * size) == 0 && x_ld % 8 == 0;
   if (x_dtype == 0)
     hipLaunchKernelGGL(quantize_rows_kernel<f16>, grid, block, 0, stream, (const f16*)x, x_ld, codes, scales, (int)K,
-                       (int)ld);
+                       (int)ld, wide);
   else if (x_dtype == 1)
     hipLaunchKernelGGL(quantize_rows_kernel<__bf16>, grid, block, 0, stream, (const __bf16*)x, x_ld, codes, scales,
-                       (int)K, (int)ld);
+                       (int)K, (int)ld, wide);
   else
     hipLaunchKernelGGL(quantize_rows_kernel<float>, grid, block, 0, stream, (const float*)x, x_ld, codes, scales,
-                       (int)K, (int)ld);
+                       (int)K, (int)ld, wide);
   return hipGetLastError();
 }
 
