@@ -252,12 +252,12 @@ hipError_t tiles(const W8A8& p, hipStream_t stream) {
 
 // ---- few rows ----------------------------------------------------------------------
 // Up to 64 activation rows: bound by the bytes of the weights. A workgroup takes 16 NT weight
-// rows, its eight waves the steps of 64 columns in turn; both operands come straight from memory
+// rows, its eight waves the steps of 128 columns in turn; both operands come straight from memory
 // to registers (the activations from L2), 16x16x64 products, the weights the rows of the
 // result. The waves' sums are added through LDS.
 template <typename T, int MT, int NT>
 __global__ __launch_bounds__(512, 2) void w8a8_few_kernel(W8A8 p) {
-  constexpr int kFly = 8 / (MT + NT) < 1 ? 1 : 8 / (MT + NT);  // steps in flight ahead
+  constexpr int kFly = 10 / (MT + NT) < 1 ? 1 : 10 / (MT + NT);  // steps in flight
   __shared__ __attribute__((aligned(16))) int sums[16 * MT][16 * NT + 4];
   const int tid = threadIdx.x, l = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c = l & 15, h = l >> 4;
@@ -276,22 +276,30 @@ __global__ __launch_bounds__(512, 2) void w8a8_few_kernel(W8A8 p) {
   for (int i = 0; i < NT; ++i)
 #pragma unroll
     for (int j = 0; j < MT; ++j) acc[i][j] = i32x4{0, 0, 0, 0};
+  // a step: 128 columns, a lane's 32 h .. 32 h + 31 of a row (whole lines of 128 bytes a row)
   const i32x4 zero = {0, 0, 0, 0};
-  const int full = ld / 64;  // whole steps
-  i32x4 wv[kFly][NT], xv[kFly][MT];
+  const int full = ld / 128;  // whole steps
+  i32x4 wv[kFly][NT][2], xv[kFly][MT][2];
   auto load = [&](int f, int s) {  // step s, or (past the end) the first again
-    const int k = 64 * (s < full ? s : 0) + 16 * h;
-#pragma unroll
-    for (int i = 0; i < NT; ++i) wv[f][i] = __builtin_nontemporal_load(reinterpret_cast<const i32x4*>(wrow[i] + k));
-#pragma unroll
-    for (int j = 0; j < MT; ++j) xv[f][j] = *reinterpret_cast<const i32x4*>(xrow[j] + k);
-  };
-  auto multiply = [&](int f) {
+    const int k = 128 * (s < full ? s : 0) + 32 * h;
 #pragma unroll
     for (int i = 0; i < NT; ++i)
 #pragma unroll
-      for (int j = 0; j < MT; ++j)
-        acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wv[f][i], xv[f][j], acc[i][j], 0, 0, 0);
+      for (int q = 0; q < 2; ++q)
+        wv[f][i][q] = __builtin_nontemporal_load(reinterpret_cast<const i32x4*>(wrow[i] + k + 16 * q));
+#pragma unroll
+    for (int j = 0; j < MT; ++j)
+#pragma unroll
+      for (int q = 0; q < 2; ++q) xv[f][j][q] = *reinterpret_cast<const i32x4*>(xrow[j] + k + 16 * q);
+  };
+  auto multiply = [&](int f) {
+#pragma unroll
+    for (int q = 0; q < 2; ++q)
+#pragma unroll
+      for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int j = 0; j < MT; ++j)
+          acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wv[f][i][q], xv[f][j][q], acc[i][j], 0, 0, 0);
   };
   if (wave < full) {
     int s = wave;
@@ -308,12 +316,15 @@ __global__ __launch_bounds__(512, 2) void w8a8_few_kernel(W8A8 p) {
     for (int f = 0; f < kFly; ++f)
       if (s + 8 * f < full) multiply(f);
   }
-  if (wave == full % 8 && ld % 64) {  // the columns behind the last whole step: 16, 32 or 48
-    const int k = 64 * full + 16 * h;
+  if (wave == full % 8 && ld % 128) {  // the columns behind the last whole step: a multiple of 16
 #pragma unroll
-    for (int i = 0; i < NT; ++i) wv[0][i] = k < ld ? *reinterpret_cast<const i32x4*>(wrow[i] + k) : zero;
+    for (int q = 0; q < 2; ++q) {
+      const int k = 128 * full + 32 * h + 16 * q;
 #pragma unroll
-    for (int j = 0; j < MT; ++j) xv[0][j] = k < ld ? *reinterpret_cast<const i32x4*>(xrow[j] + k) : zero;
+      for (int i = 0; i < NT; ++i) wv[0][i][q] = k < ld ? *reinterpret_cast<const i32x4*>(wrow[i] + k) : zero;
+#pragma unroll
+      for (int j = 0; j < MT; ++j) xv[0][j][q] = k < ld ? *reinterpret_cast<const i32x4*>(xrow[j] + k) : zero;
+    }
     multiply(0);
   }
   __syncthreads();  // sums are cleared
@@ -343,12 +354,16 @@ __global__ __launch_bounds__(512, 2) void w8a8_few_kernel(W8A8 p) {
 
 template <typename T, int MT>
 hipError_t few(const W8A8& p, hipStream_t stream) {
+  // More weight rows a workgroup read the activations less often (a quarter of them with 64), as
+  // long as there are workgroups for the CUs. M x N x K, 16 / 32 / 64 weight rows (us with the
+  // quantisation): 1 x 128256 x 4096 120 / 124 / 95, 8 x 14336 x 4096 22.8 / 23.4 / 19.4, 64 x 28672 x 4096
+  // 72 / 54 / 48, 17 x 6144 x 4096 20.0 / 14.3 / 19.2, 1 x 4096 x 4096 10.1 / 13.1 / 16.5, 64 x 4096 x 14336
+  // 42 / 50 / 69.
   const int64_t cus = device_cu_count();
-  // 64 weight rows a workgroup where that still gives every CU two of them
   const dim3 block(512);
-  if (p.N >= 128 * cus)
+  if (p.N >= 48 * cus)
     hipLaunchKernelGGL((w8a8_few_kernel<T, MT, 4>), dim3((unsigned)((p.N + 63) / 64)), block, 0, stream, p);
-  else if (p.N >= 64 * cus)
+  else if (p.N >= 20 * cus)
     hipLaunchKernelGGL((w8a8_few_kernel<T, MT, 2>), dim3((unsigned)((p.N + 31) / 32)), block, 0, stream, p);
   else
     hipLaunchKernelGGL((w8a8_few_kernel<T, MT, 1>), dim3((unsigned)((p.N + 15) / 16)), block, 0, stream, p);
@@ -359,6 +374,7 @@ template <typename T>
 hipError_t product(const W8A8& p, hipStream_t stream) {
   if (p.M <= 16) return few<T, 1>(p, stream);
   if (p.M <= 32) return few<T, 2>(p, stream);
+  if (p.M <= 48) return few<T, 3>(p, stream);
   if (p.M <= 64) return few<T, 4>(p, stream);
   // 256 x 256 tiles where they fill the CUs, else 128 x 128
   const int64_t big = ((p.M + 255) / 256) * ((p.N + 255) / 256);
