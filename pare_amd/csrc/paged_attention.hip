@@ -569,8 +569,8 @@ hipError_t few(const AttnArgs& a, bool fp8, int wgs, hipStream_t stream) {
 //     consecutive tokens, its operand of P;
 //   O^T = V^T P^T from V^T in LDS, rows = dimensions.
 // A block of 16 tokens, and with it a page's scales, is the same for all lanes. In LDS,
-// 16-byte chunk x of row y lies at x ^ (y % 16) (K) and x ^ (y % 8) (V^T): reads of
-// consecutive rows fall in different banks.
+// 16-byte chunk x of row y lies at x ^ (y % 16) (K of heads of 128) or x ^ (y / 2 % 8) (K of heads
+// of 64, and V^T): reads of 16 consecutive rows fall in different banks.
 // Where the rows give fewer workgroups than the CUs hold, the keys are split as well
 // (`splits` ranges of `per` tokens), and the last range to arrive joins them.
 constexpr int kRows = 128;
@@ -715,6 +715,8 @@ __global__ __launch_bounds__(256, 2) void attention_rows_kernel(AttnArgs a) {
       vw[k] = *reinterpret_cast<const u32x4*>(a.v + at + (uint32_t)(16 * (idx % D)));
     }
   };
+  // 16 consecutive rows in different banks: one row fills the 64 banks (D = 128), or two do
+  auto swizzle = [](int krow) { return D == 128 ? krow & 15 : (krow >> 1) & 7; };
   auto store_tile = [&](int p, const Blocks& x, int slot) {
     uint8_t* kb = lds + slot * 2 * kSlot;
     uint8_t* vb = kb + kSlot;
@@ -725,13 +727,13 @@ __global__ __launch_bounds__(256, 2) void attention_rows_kernel(AttnArgs a) {
       const int idx = tid + 256 * k;
       const int krow = idx / (D / 16), kpiece = idx % (D / 16);
       const f16x8 k0 = codes8<FP8>(kw[k][0], kw[k][1]), k1 = codes8<FP8>(kw[k][2], kw[k][3]);
-      *reinterpret_cast<f16x8*>(kb + krow * D * 2 + (((2 * kpiece) ^ (krow & (D / 8 - 1))) << 4)) = k0;
-      *reinterpret_cast<f16x8*>(kb + krow * D * 2 + (((2 * kpiece + 1) ^ (krow & (D / 8 - 1))) << 4)) = k1;
+      *reinterpret_cast<f16x8*>(kb + krow * D * 2 + (((2 * kpiece) ^ swizzle(krow)) << 4)) = k0;
+      *reinterpret_cast<f16x8*>(kb + krow * D * 2 + (((2 * kpiece + 1) ^ swizzle(krow)) << 4)) = k1;
       const int vblk = block_of(k), vd = idx % D;
       if (edge) vw[k] &= byte_mask(first_seen - p - 16 * vblk, pick(x.page, vblk) < 0 ? 0 : p1 - p - 16 * vblk);
       const f16x8 v0 = codes8<FP8>(vw[k][0], vw[k][1]), v1 = codes8<FP8>(vw[k][2], vw[k][3]);
-      *reinterpret_cast<f16x8*>(vb + vd * 128 + (((2 * vblk) ^ (vd & 7)) << 4)) = v0;
-      *reinterpret_cast<f16x8*>(vb + vd * 128 + (((2 * vblk + 1) ^ (vd & 7)) << 4)) = v1;
+      *reinterpret_cast<f16x8*>(vb + vd * 128 + (((2 * vblk) ^ ((vd >> 1) & 7)) << 4)) = v0;
+      *reinterpret_cast<f16x8*>(vb + vd * 128 + (((2 * vblk + 1) ^ ((vd >> 1) & 7)) << 4)) = v1;
     }
   };
 
@@ -764,7 +766,7 @@ __global__ __launch_bounds__(256, 2) void attention_rows_kernel(AttnArgs a) {
         const int krow = 32 * u + 16 * (c >> 4) + 8 * ((c >> 2) & 1) + 4 * ((c >> 3) & 1) + (c & 3);
 #pragma unroll
         for (int x = 0; x < D / 16; ++x) {
-          const f16x8 k8 = *reinterpret_cast<const f16x8*>(kb + krow * D * 2 + (((2 * x + h) ^ (krow & (D / 8 - 1))) << 4));
+          const f16x8 k8 = *reinterpret_cast<const f16x8*>(kb + krow * D * 2 + (((2 * x + h) ^ swizzle(krow)) << 4));
           s[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k8, qv[x], s[u], 0, 0, 0);
         }
       }
@@ -834,7 +836,7 @@ __global__ __launch_bounds__(256, 2) void attention_rows_kernel(AttnArgs a) {
 #pragma unroll
         for (int d = 0; d < D / 32; ++d) {
           const int vrow = 32 * d + c;
-          const f16x8 v8 = *reinterpret_cast<const f16x8*>(vb + vrow * 128 + (((2 * b + h) ^ (vrow & 7)) << 4));
+          const f16x8 v8 = *reinterpret_cast<const f16x8*>(vb + vrow * 128 + (((2 * b + h) ^ ((vrow >> 1) & 7)) << 4));
           acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v8, pw, acc[d], 0, 0, 0);
         }
       }

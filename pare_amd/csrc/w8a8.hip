@@ -116,7 +116,8 @@ PMI_DEV void store_row8(T* __restrict__ y, const int* sums, const float* sw, con
 // BN weight rows x BM activation rows per workgroup of WN x WM waves, in steps of 128
 // columns. Both operands' rows go from memory straight to LDS (two slots, one barrier a step; the
 // copies of the next step fly while this one is multiplied); 16-byte chunk c of row r lies at
-// chunk c ^ (r % 8), so that reads of eight consecutive rows fall in different banks. Products
+// chunk c ^ (r / 2 % 8), so that reads of 16 consecutive rows (two rows fill the 64 banks) do not
+// meet in one. Products
 // 32x32x32: the weights are the rows of the result, so that a wave reads (BN / WN + BM / WM) x
 // 32 bytes for BN / WN x BM / WM / 1024 of them. Columns past ld and rows past the end are copied
 // as zeros (from past the descriptor's end). The sums go through LDS, 32 activation rows at a
@@ -142,8 +143,8 @@ __global__ __launch_bounds__(64 * WM * WN) void w8a8_tiles_kernel(W8A8 p, int gr
   const u32x4 dw = descriptor(p.w + (int64_t)n0 * ld, (uint32_t)rows_n * ld);
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
 
-  // a copy: eight rows of 128 bytes, lane 8 r + c chunk c ^ r of row r
-  const int crow = l >> 3, ccol = 16 * ((l & 7) ^ (l >> 3));
+  // a copy: eight rows of 128 bytes, from row 8 (wave + NW i) on (NW is even)
+  const int crow = l >> 3, ccol = 16 * ((l & 7) ^ ((crow >> 1) + 4 * (wave & 1)));
   auto copy = [&](int kt, int slot) {
     const int k = 128 * kt + ccol;
     const int at = k < ld ? crow * ld + ccol : 0x7ffffff0;  // past the end: zeros
@@ -178,7 +179,7 @@ __global__ __launch_bounds__(64 * WM * WN) void w8a8_tiles_kernel(W8A8 p, int gr
     const uint8_t* xb = lds + slot * kSlot + BN * 128 + (wm * (BM / WM) + c) * 128;
 #pragma unroll
     for (int ks = 0; ks < 4; ++ks) {
-      const int at = 16 * ((2 * ks + h) ^ (c & 7));
+      const int at = 16 * ((2 * ks + h) ^ ((c >> 1) & 7));
       i32x4 wv[TN], xv[TM];
 #pragma unroll
       for (int i = 0; i < TN; ++i) wv[i] = *reinterpret_cast<const i32x4*>(wb + 32 * 128 * i + at);
