@@ -122,6 +122,11 @@ PMI_DEV void store_row8(T* __restrict__ y, const int* sums, const float* sw, con
 // 32 bytes for BN / WN x BM / WM / 1024 of them. Columns past ld and rows past the end are copied
 // as zeros (from past the descriptor's end). The sums go through LDS, 32 activation rows at a
 // time, to be written 16 bytes a lane.
+//
+// What bounds it (4099 x 28672 x 4096, 500 us with 13 of quantisation, 1.9e15 operations a second): the
+// products alone take about 290 us, the copies hold them up by some 120 and the stores of y, which
+// nothing overlaps as one workgroup fills a CU's LDS, by 70 (measured with each left out). Four
+// slots of 64 columns, three steps ahead: 545 us, twice the requests to L2 for half a line each.
 template <typename T, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(64 * WM * WN) void w8a8_tiles_kernel(W8A8 p, int grid_m, int grid_n, int chunk) {
   constexpr int NW = WM * WN, TM = BM / WM / 32, TN = BN / WN / 32;
@@ -145,19 +150,18 @@ __global__ __launch_bounds__(64 * WM * WN) void w8a8_tiles_kernel(W8A8 p, int gr
 
   // a copy: eight rows of 128 bytes, from row 8 (wave + NW i) on (NW is even)
   const int crow = l >> 3, ccol = 16 * ((l & 7) ^ ((crow >> 1) + 4 * (wave & 1)));
+  int at_row[BN / 8 / NW > BM / 8 / NW ? BN / 8 / NW : BM / 8 / NW];
+#pragma unroll
+  for (int i = 0; i < (int)(sizeof(at_row) / sizeof(int)); ++i) at_row[i] = (8 * (wave + NW * i) + crow) * ld + ccol;
   auto copy = [&](int kt, int slot) {
-    const int k = 128 * kt + ccol;
-    const int at = k < ld ? crow * ld + ccol : 0x7ffffff0;  // past the end: zeros
+    const uint32_t to = lds0 + slot * kSlot + wave * 1024;
+    // past the end of the rows (the last step): past the end of all, zeros
+    const bool out = 128 * kt + ccol >= ld;
 #pragma unroll
-    for (int i = 0; i < BN / 8 / NW; ++i) {
-      const int r = 8 * (wave + NW * i);
-      dma16(dw, lds0 + slot * kSlot + r * 128, k < ld ? at + r * ld : at, 128 * kt);
-    }
+    for (int i = 0; i < BN / 8 / NW; ++i) dma16(dw, to + i * NW * 1024, out ? 0x7ffffff0 : at_row[i], 128 * kt);
 #pragma unroll
-    for (int i = 0; i < BM / 8 / NW; ++i) {
-      const int r = 8 * (wave + NW * i);
-      dma16(dx, lds0 + slot * kSlot + BN * 128 + r * 128, k < ld ? at + r * ld : at, 128 * kt);
-    }
+    for (int i = 0; i < BM / 8 / NW; ++i)
+      dma16(dx, to + BN * 128 + i * NW * 1024, out ? 0x7ffffff0 : at_row[i], 128 * kt);
   };
 
   i32x16 acc[TN][TM];
@@ -379,7 +383,7 @@ hipError_t product(const W8A8& p, hipStream_t stream) {
   if (p.M <= 64) return few<T, 4>(p, stream);
   // 256 x 256 tiles where they fill the CUs, else 128 x 128
   const int64_t big = ((p.M + 255) / 256) * ((p.N + 255) / 256);
-  if (big >= device_cu_count()) return tiles<T, 256, 256, 4, 2>(p, stream);
+  if (big >= device_cu_count()) return tiles<T, 256, 256, 2, 4>(p, stream);
   return tiles<T, 128, 128, 2, 2>(p, stream);
 }
 
