@@ -589,6 +589,7 @@ PMI_API int pmi_silu_mul_f16(const void* gate_up, void* out, int64_t rows, int64
  *   q_starts int32 [R + 1]  where each request's new tokens begin (at most total)
  *   kv_lens_out int32 [R]   the lengths with the new tokens; may be kv_lens
  *   first int32 [R]         the position of its first new token, -1 if refused
+ *   fresh int32 [R + 1]     how many pages the requests before each one took
  *   positions, slots int32 [total]  of every new token: its position, and
  *                           page * page_size + offset (-1 and position 0 for refused
  *                           ones and from q_starts[R] on)
@@ -597,8 +598,8 @@ PMI_API int pmi_silu_mul_f16(const void* gate_up, void* out, int64_t rows, int64
 PMI_API int pmi_extend_block_tables(int32_t* tables, int64_t table_stride, const int32_t* kv_lens,
                                     const int32_t* new_lens, const int32_t* free_pages,
                                     const int32_t* pool, int32_t* q_starts, int32_t* kv_lens_out,
-                                    int32_t* first, int32_t* positions, int32_t* slots,
-                                    int32_t* pool_out, int64_t R, int64_t width, int64_t ring,
+                                    int32_t* first, int32_t* fresh, int32_t* positions,
+                                    int32_t* slots, int32_t* pool_out, int64_t R, int64_t width, int64_t ring,
                                     int64_t page_size, int64_t total, void* stream);
 
 /* The pages of every request r with done[r] != 0 (u8 [R]) go to the end of the ring

@@ -18,6 +18,7 @@ struct PagedTables {
   int32_t* q_starts;          // [R + 1]
   int32_t* kv_lens_out;       // [R], may be kv_lens
   int32_t* first;             // [R]
+  int32_t* fresh;             // [R + 1]
   int32_t* positions;         // [total]
   int32_t* slots;             // [total]
   int32_t* pool_out;          // [4], may be pool

@@ -34,13 +34,10 @@ class BatchPlan(NamedTuple):
     q_starts: torch.Tensor   # [R + 1] where each request's new tokens begin
     kv_lens: torch.Tensor    # [R] lengths with the new tokens
     first: torch.Tensor      # [R] position of its first new token, -1 if refused
+    fresh: torch.Tensor      # [R + 1] pages that the requests before each one took
     positions: torch.Tensor  # [total] position of each new token
     slots: torch.Tensor      # [total] page * page_size + offset, -1: not stored
     pool: torch.Tensor       # [4] head and count of the free ring, requests refused, 0
-
-
-def _need(cond: bool, what: str) -> None:
-    assert cond, what
 
 
 def _hip(t: torch.Tensor, fn: str) -> torch.device:
@@ -53,17 +50,17 @@ def _ints(dev: torch.device, n: int | None = None, **tensors: torch.Tensor) -> N
     for name, t in tensors.items():
         if t.device != dev:
             raise RuntimeError(f"{name} is on {t.device}, expected {dev}")
-        _need(t.dtype == torch.int32 and t.dim() == 1 and t.is_contiguous() and (n is None or t.numel() == n),
-              f"{name} must be a contiguous int32 [{'n' if n is None else n}] tensor")
+        assert (t.dtype == torch.int32 and t.dim() == 1 and t.is_contiguous() and (n is None or t.numel() == n)), (
+            f"{name} must be a contiguous int32 [{'n' if n is None else n}] tensor")
 
 
 def _tables(tables: torch.Tensor, dev: torch.device, R: int) -> None:
     if tables.device != dev:
         raise RuntimeError(f"block_tables is on {tables.device}, expected {dev}")
-    _need(tables.dtype == torch.int32 and tables.dim() == 2 and tables.shape[0] == R
-          and (tables.shape[1] <= 1 or tables.stride(1) == 1)
-          and (R <= 1 or tables.stride(0) >= tables.shape[1]),
-          f"block_tables must be an int32 [{R}, width] tensor with contiguous rows")
+    assert (tables.dtype == torch.int32 and tables.dim() == 2 and tables.shape[0] == R
+            and (tables.shape[1] <= 1 or tables.stride(1) == 1)
+            and (R <= 1 or tables.stride(0) >= tables.shape[1])), (
+        f"block_tables must be an int32 [{R}, width] tensor with contiguous rows")
 
 
 def _row_stride(tables: torch.Tensor) -> int:
@@ -73,17 +70,17 @@ def _row_stride(tables: torch.Tensor) -> int:
 def _cache(dev: torch.device, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
            v_scale: torch.Tensor) -> tuple[int, int, int, int, int]:
     """(pages, KV, page_size, D, code) of a cache, after its checks."""
-    _need(k_cache.dim() == 4 and v_cache.dim() == 5, "k_cache must be [pages, KV, page_size, D] and v_cache "
-          "[pages, KV, page_size / 16, D, 16]")
+    assert k_cache.dim() == 4 and v_cache.dim() == 5, (
+        "k_cache must be [pages, KV, page_size, D] and v_cache [pages, KV, page_size / 16, D, 16]")
     pages, KV, ps, D = k_cache.shape
-    _need(tuple(v_cache.shape) == (pages, KV, ps // 16, D, 16) and ps % 16 == 0,
-          f"v_cache must be [{pages}, {KV}, {ps // 16}, {D}, 16], got {tuple(v_cache.shape)}")
-    _need(k_cache.dtype in _CODES and v_cache.dtype == k_cache.dtype,
-          "the caches must both be int8 or both float8_e4m3fn")
-    _need(k_cache.is_contiguous() and v_cache.is_contiguous(), "the caches must be contiguous")
+    assert tuple(v_cache.shape) == (pages, KV, ps // 16, D, 16) and ps % 16 == 0, (
+        f"v_cache must be [{pages}, {KV}, {ps // 16}, {D}, 16], got {tuple(v_cache.shape)}")
+    assert k_cache.dtype in _CODES and v_cache.dtype == k_cache.dtype, (
+        "the caches must both be int8 or both float8_e4m3fn")
+    assert k_cache.is_contiguous() and v_cache.is_contiguous(), "the caches must be contiguous"
     for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
-        _need(t.dtype == torch.float32 and tuple(t.shape) == (pages, KV) and t.is_contiguous(),
-              f"{name} must be a contiguous float32 [{pages}, {KV}] tensor")
+        assert t.dtype == torch.float32 and tuple(t.shape) == (pages, KV) and t.is_contiguous(), (
+            f"{name} must be a contiguous float32 [{pages}, {KV}] tensor")
     for name, t in (("k_cache", k_cache), ("v_cache", v_cache), ("k_scale", k_scale), ("v_scale", v_scale)):
         if t.device != dev:
             raise RuntimeError(f"{name} is on {t.device}, expected {dev}")
@@ -115,10 +112,10 @@ def extend_block_tables(block_tables: torch.Tensor, kv_lens: torch.Tensor, new_l
         _ints(dev, R, kv_lens_out=kv_lens_out)
     if pool_out is not None:
         _ints(dev, 4, pool_out=pool_out)
-    buf = torch.empty(2 * R + 1 + 2 * total + (R if kv_lens_out is None else 0) + (4 if pool_out is None else 0),
+    buf = torch.empty(3 * R + 2 + 2 * total + (R if kv_lens_out is None else 0) + (4 if pool_out is None else 0),
                       dtype=torch.int32, device=dev)
-    cut = [R + 1, R, total, total]
-    q_starts, first, positions, slots, rest = buf.split([*cut, buf.numel() - sum(cut)])
+    cut = [R + 1, R, R + 1, total, total]
+    q_starts, first, fresh, positions, slots, rest = buf.split([*cut, buf.numel() - sum(cut)])
     if kv_lens_out is None:
         kv_lens_out, rest = rest[:R], rest[R:]
     if pool_out is None:
@@ -127,9 +124,9 @@ def extend_block_tables(block_tables: torch.Tensor, kv_lens: torch.Tensor, new_l
         _lib.check(_lib.lib().pmi_extend_block_tables(
             block_tables.data_ptr(), _row_stride(block_tables), kv_lens.data_ptr(), new_lens.data_ptr(),
             free_pages.data_ptr(), pool.data_ptr(), q_starts.data_ptr(), kv_lens_out.data_ptr(), first.data_ptr(),
-            positions.data_ptr(), slots.data_ptr(), pool_out.data_ptr(), R, block_tables.shape[1],
+            fresh.data_ptr(), positions.data_ptr(), slots.data_ptr(), pool_out.data_ptr(), R, block_tables.shape[1],
             free_pages.numel(), page_size, total, _stream_handle(dev)), "pmi_extend_block_tables")
-    return BatchPlan(q_starts, kv_lens_out, first, positions, slots, pool_out)
+    return BatchPlan(q_starts, kv_lens_out, first, fresh, positions, slots, pool_out)
 
 
 def release_block_tables(block_tables: torch.Tensor, kv_lens: torch.Tensor, done: torch.Tensor,
@@ -142,8 +139,9 @@ def release_block_tables(block_tables: torch.Tensor, kv_lens: torch.Tensor, done
     _ints(dev, R, kv_lens=kv_lens)
     _ints(dev, free_pages=free_pages)
     _ints(dev, 4, pool=pool)
-    _need(done.dtype == torch.bool and done.dim() == 1 and done.numel() == R and done.is_contiguous()
-          and done.device == dev, f"done must be a contiguous bool [{R}] tensor on {dev}")
+    assert (done.dtype == torch.bool and done.dim() == 1 and done.numel() == R and done.is_contiguous()
+            and done.device == dev), (
+        f"done must be a contiguous bool [{R}] tensor on {dev}")
     with _DeviceGuard(dev):
         _lib.check(_lib.lib().pmi_release_block_tables(
             block_tables.data_ptr(), _row_stride(block_tables), kv_lens.data_ptr(), done.data_ptr(),
@@ -164,18 +162,19 @@ def rope_append_kv(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, posi
     cache are skipped. An infinity or NaN makes its page and head NaN."""
     dev = _hip(qkv, "rope_append_kv")
     pages, KV, ps, D, code = _cache(dev, k_cache, v_cache, k_scale, v_scale)
-    _need(qkv.dim() == 2 and qkv.dtype in (torch.float16, torch.bfloat16), "qkv must be float16 or bfloat16 "
-          "[T, (H + 2 KV) * D]")
+    assert qkv.dim() == 2 and qkv.dtype in (torch.float16, torch.bfloat16), (
+        "qkv must be float16 or bfloat16 [T, (H + 2 KV) * D]")
     T, width = qkv.shape
     H = width // D - 2 * KV
-    _need(width % D == 0 and H > 0 and H % KV == 0, f"qkv has {width} columns, expected (H + 2 * {KV}) * {D}")
+    assert width % D == 0 and H > 0 and H % KV == 0, (
+        f"qkv has {width} columns, expected (H + 2 * {KV}) * {D}")
     if qkv.stride(1) != 1 or qkv.stride(0) % 8 or qkv.stride(0) < width or qkv.data_ptr() % 16:
         qkv = torch.empty(T, width, dtype=qkv.dtype, device=dev).copy_(qkv)
     _ints(dev, T, positions=positions, slots=slots)
     for name, t in (("cos", cos), ("sin", sin)):
-        _need(t.dtype == torch.float32 and t.dim() == 2 and t.shape[1] == D // 2 and t.is_contiguous()
-              and t.device == dev and t.shape == cos.shape, f"{name} must be a contiguous float32 [L, {D // 2}] "
-              f"tensor on {dev}")
+        assert (t.dtype == torch.float32 and t.dim() == 2 and t.shape[1] == D // 2 and t.is_contiguous()
+                and t.device == dev and t.shape == cos.shape), (
+            f"{name} must be a contiguous float32 [L, {D // 2}] tensor on {dev}")
     q = torch.empty(T, H, D, dtype=qkv.dtype, device=dev)
     with _DeviceGuard(dev):
         _lib.check(_lib.lib().pmi_rope_append_kv(
@@ -193,7 +192,7 @@ def read_kv_pages(pages: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
     dev = _hip(k_cache, "read_kv_pages")
     n_pages, KV, ps, D, code = _cache(dev, k_cache, v_cache, k_scale, v_scale)
     _ints(dev, pages=pages)
-    _need(dtype in _VALUES, "dtype must be float16, bfloat16 or float32")
+    assert dtype in _VALUES, "dtype must be float16, bfloat16 or float32"
     k = torch.empty(pages.numel(), KV, ps, D, dtype=dtype, device=dev)
     v = torch.empty_like(k)
     with _DeviceGuard(dev):
@@ -220,8 +219,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     ``scale`` multiplies q . k."""
     dev = _hip(q, "paged_attention")
     pages, KV, ps, D, code = _cache(dev, k_cache, v_cache, k_scale, v_scale)
-    _need(q.dim() == 3 and q.shape[2] == D and q.dtype in (torch.float16, torch.bfloat16),
-          f"q must be float16 or bfloat16 [T, H, {D}]")
+    assert q.dim() == 3 and q.shape[2] == D and q.dtype in (torch.float16, torch.bfloat16), (
+        f"q must be float16 or bfloat16 [T, H, {D}]")
     T, H = q.shape[0], q.shape[1]
     R = kv_lens.numel()
     _tables(block_tables, dev, R)
@@ -229,20 +228,20 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     if q_starts is not None:
         _ints(dev, R + 1, q_starts=q_starts)
     else:
-        _need(T == R, f"without q_starts there is one query per request: q has {T}, kv_lens {R}")
+        assert T == R, f"without q_starts there is one query per request: q has {T}, kv_lens {R}"
         max_q_len = 1
-    _need(max_q_len >= 0 and window >= 0, "max_q_len and window may not be negative")
+    assert max_q_len >= 0 and window >= 0, "max_q_len and window may not be negative"
     if q.stride(2) != 1 or q.stride(0) % 8 or q.stride(1) % 8 or q.data_ptr() % 16:
         q = torch.empty(T, H, D, dtype=q.dtype, device=dev).copy_(q)
     if out is None:
         out = torch.empty(T, H, D, dtype=q.dtype, device=dev)
     else:
-        _need(out.dtype == q.dtype and tuple(out.shape) == (T, H, D) and out.is_contiguous()
-              and out.device == dev and out.data_ptr() % 16 == 0,
-              f"out must be a contiguous, 16-byte aligned [{T}, {H}, {D}] tensor of q's type")
+        assert (out.dtype == q.dtype and tuple(out.shape) == (T, H, D) and out.is_contiguous()
+                and out.device == dev and out.data_ptr() % 16 == 0), (
+            f"out must be a contiguous, 16-byte aligned [{T}, {H}, {D}] tensor of q's type")
     width = block_tables.shape[1]
     max_kv = width * ps if max_kv_len is None else min(max_kv_len, width * ps)
-    _need(max_kv >= 0, "max_kv_len may not be negative")
+    assert max_kv >= 0, "max_kv_len may not be negative"
     L = _lib.lib()
     with _DeviceGuard(dev):
         stream = _stream_handle(dev)

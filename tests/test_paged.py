@@ -108,7 +108,7 @@ def test_attention_without_its_workspace_is_refused():
                                     dict(total=1 << 31), dict(width=1 << 40, stride=1 << 40), dict(ring=1 << 40),
                                     dict(tables=None), dict(pool=None), dict(slots=None), dict(free=None)])
 def test_tables_refuse(change):
-    a = dict(tables=P8, stride=8, lens=P8, new=P8, free=P8, pool=P8, starts=P8, out=P8, first=P8, positions=P8,
+    a = dict(tables=P8, stride=8, lens=P8, new=P8, free=P8, pool=P8, starts=P8, out=P8, first=P8, fresh=P8, positions=P8,
              slots=P8, pool_out=P8, R=2, width=8, ring=16, ps=16, total=2)
     a.update(change)
     rc = _lib.lib().pmi_extend_block_tables(*a.values(), None)
