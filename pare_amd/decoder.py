@@ -22,6 +22,11 @@ With ``fused_ops`` (the default) the ops around the linears are the library's
 caller-side kernels: residual add + RMSNorm, RoPE + KV-cache write, grouped-
 query decode attention and SiLU-gate multiply, one launch each. With
 ``fused_ops=False`` they are plain PyTorch ops (the check in the tests).
+
+``generate_ragged`` serves prompts of different lengths together: one paged 8-bit
+cache (``PagedKVCache``) in place of the fixed-length fp16 one, the prompts as one
+ragged batch, finished requests' pages given back as they end. ``quantize_head``
+puts the output head, the step's largest product, on 8-bit integers as well.
 """
 
 from __future__ import annotations
@@ -42,7 +47,9 @@ from .kernels import (_stream_handle, gate_up_silu_rows_supported, gate_up_silu_
                       matmul_w4a16_residual, matmul_w4a16_rmsnorm, matmul_w4a16_tiled_rmsnorm,
                       residual_stats_count, tiled_rmsnorm_supported)
 from .pack import sz_group_major, tile_w4a16
+from .int8 import Int8Linear
 from .linear import FusedQuantizedLinear, QuantizedLinear
+from .paged import BatchPlan, PagedKVCache
 from .quant import rtn_quantize
 
 
@@ -319,6 +326,24 @@ class DecoderLayer(nn.Module):
         n2, h = add_rmsnorm(h, self.o(a), self.mlp_norm.weight, cfg.rms_eps)
         return h, self._mlp(n2, B, T)
 
+    def forward_paged(self, h, d, cos_t, sin_t, cache: PagedKVCache, layer: int, plan: BatchPlan,
+                      max_q_len: int, max_kv_len: int):
+        """The layer on the tokens of a ragged batch, h and d [1, T, hidden] as in
+        ``forward_fused``: their keys and values go to layer ``layer`` of the paged
+        cache, in the slots that ``plan`` gives them, and every token attends to its own
+        request's positions up to its own. Returns the new (h, d)."""
+        cfg = self.cfg
+        T = h.shape[1]
+        qkv, h = self._norm_linear(self.qkv.fused, h, d, self.attn_norm.weight)
+        q = cache.append(layer, qkv.reshape(T, -1), cos_t, sin_t, plan)
+        a = cache.attend(layer, q, plan, scale=1.0 / math.sqrt(cfg.head_dim), max_q_len=max_q_len,
+                         max_kv_len=max_kv_len)
+        o = self.o(a.reshape(1, T, cfg.hidden))
+        if T > 1:
+            return self._norm_mlp(h, o, 1, T)
+        gu, h = self._norm_linear(self.gate_up.fused, h, o, self.mlp_norm.weight)
+        return h, self._down(gu, 1, 1)
+
     def _summed_ok(self) -> bool:
         """One-token layers can carry the residual stream as (h, partials): every
         linear on the GEMV with u8 zero points, no act_order, no bias on o and
@@ -507,7 +532,18 @@ class QuantizedDecoder(nn.Module):
         self.norm = RMSNorm(cfg.hidden, cfg.rms_eps, dev)
         self.lm_head = nn.Parameter(
             (torch.randn(cfg.vocab, cfg.hidden, generator=gen, device=dev) * cfg.init_std).half())
+        self.int8_head: Int8Linear | None = None
         self._graphs: dict = {}
+
+    def quantize_head(self) -> None:
+        """The output head in 8-bit integers (``Int8Linear``) from now on, in place of its
+        fp16 weight, which is dropped: half the bytes of the largest product of a step."""
+        if self.int8_head is None:
+            self.int8_head = Int8Linear.from_weight(self.lm_head)
+            self.lm_head = None
+
+    def _head(self, n: torch.Tensor) -> torch.Tensor:
+        return F.linear(n, self.lm_head) if self.int8_head is None else self.int8_head(n)
 
     def rope_tables(self, max_len: int):
         return rope_tables(self.cfg.head_dim, self.cfg.rope_theta, max_len, self.embed.device)
@@ -518,6 +554,12 @@ class QuantizedDecoder(nn.Module):
         return [(torch.zeros(shape, dtype=torch.float16, device=self.embed.device),
                  torch.zeros(shape, dtype=torch.float16, device=self.embed.device))
                 for _ in range(cfg.layers)]
+
+    def new_paged_cache(self, requests: int, max_len: int, *, page_size: int = 64, pages: int | None = None,
+                        dtype: torch.dtype = torch.int8) -> PagedKVCache:
+        """The paged cache of all layers (``pare_amd.PagedKVCache``) for ``forward_paged``."""
+        return PagedKVCache(self.cfg.layers, requests, max_len, self.cfg.kv_heads, self.cfg.head_dim,
+                            self.embed.device, page_size=page_size, pages=pages, dtype=dtype)
 
     def forward_tokens(self, tokens, cos, sin, cache, pos, mask, causal: bool,
                        last_only: bool = False):
@@ -536,13 +578,106 @@ class QuantizedDecoder(nn.Module):
                 x = x[:, -1:].contiguous()
                 d = d[:, -1:].contiguous() if d is not None else None
             n, _ = add_rmsnorm(x, d, self.norm.weight, self.cfg.rms_eps)
-            return F.linear(n, self.lm_head)
+            return self._head(n)
         c, s = cos.index_select(0, pos), sin.index_select(0, pos)
         for layer, (ck, cv) in zip(self.layers, cache):
             x = layer(x, c, s, ck, cv, pos, mask, causal)
         if last_only:
             x = x[:, -1:]
-        return F.linear(self.norm(x), self.lm_head)
+        return self._head(self.norm(x))
+
+    def forward_paged(self, tokens: torch.Tensor, cos, sin, cache: PagedKVCache, plan: BatchPlan, *,
+                      max_q_len: int, max_kv_len: int) -> torch.Tensor:
+        """Logits [R, vocab] of every request's last new token. ``tokens`` [T] are the new
+        tokens of ``plan`` (``cache.extend``), request after request; no request has more
+        than ``max_q_len`` of them or more than ``max_kv_len`` positions with them. The rows
+        of requests without new tokens, and of refused ones, mean nothing."""
+        x, d = F.embedding(tokens, self.embed)[None], None
+        for i, layer in enumerate(self.layers):
+            x, d = layer.forward_paged(x, d, cos, sin, cache, i, plan, max_q_len, max_kv_len)
+        last = (plan.q_starts[1:] - 1).clamp_(min=0)
+        n, _ = add_rmsnorm(x[0].index_select(0, last), d[0].index_select(0, last), self.norm.weight,
+                           self.cfg.rms_eps)
+        return self._head(n)
+
+    @torch.no_grad()
+    def generate_ragged(self, prompts: list[torch.Tensor], n_generate: int, *, eos: int | None = None,
+                        dtype: torch.dtype = torch.int8, page_size: int = 64, use_graph: bool = True):
+        """Greedy decode of prompts of different lengths (1-D, none empty) together over a
+        paged cache of ``dtype`` codes (int8 or float8_e4m3fn): (tokens
+        [len(prompts), n_generate], timings). The prompts are prefilled as one ragged batch;
+        a decode step is one graph replay (or the same ops eagerly). A request that has
+        produced ``eos`` gives its pages back, takes no further part, and the rest of its
+        row is ``eos``."""
+        if not prompts or any(p.dim() != 1 or p.numel() == 0 for p in prompts):
+            raise ValueError("prompts must be 1-D tensors of at least one token")
+        if n_generate < 1:
+            raise ValueError("n_generate must be at least 1")
+        dev, R = self.embed.device, len(prompts)
+        lens = [p.numel() for p in prompts]
+        longest, total = max(lens), sum(lens)
+        L = longest + n_generate
+        cos, sin = self.rope_tables(L)
+        cache = self.new_paged_cache(R, L, page_size=page_size, dtype=dtype)
+        out = torch.empty(R, n_generate, dtype=torch.long, device=dev)
+        tok = torch.zeros(R, 1, dtype=torch.long, device=dev)
+        live = torch.ones(R, dtype=torch.int32, device=dev)
+        packed = torch.zeros(R + 1, dtype=torch.long, device=dev)
+
+        def finish():
+            """Takes the requests that have just produced eos out of the batch."""
+            ended = tok[:, 0] == eos
+            cache.release(ended & (live > 0))
+            live.masked_fill_(ended, 0)
+
+        def step():
+            plan = cache.extend(live, R)
+            inputs = tok[:, 0]
+            if eos is not None:
+                # the live requests' tokens in front, where the plan looks for them
+                packed.scatter_(0, torch.where(live > 0, plan.q_starts[:-1], R).long(), inputs)
+                inputs = packed[:R]
+            logits = self.forward_paged(inputs, cos, sin, cache, plan, max_q_len=1, max_kv_len=L)
+            argmax_into(logits, tok)
+            if eos is not None:
+                tok.masked_fill_((live == 0)[:, None], eos)
+                finish()
+
+        graph = None
+        if use_graph and n_generate > 1:
+            # on a side stream after one eager run of the same step, as in generate
+            s = torch.cuda.Stream(dev)
+            s.wait_stream(torch.cuda.current_stream(dev))
+            with torch.cuda.stream(s):
+                step()
+                graph = torch.cuda.CUDAGraph()
+                with torch.cuda.graph(graph, stream=s):
+                    step()
+            torch.cuda.current_stream(dev).wait_stream(s)
+            cache.reset()
+            live.fill_(1)
+        tokens = torch.cat([p.to(dev) for p in prompts])
+        new_lens = torch.tensor(lens, dtype=torch.int32, device=dev)
+        torch.cuda.synchronize(dev)
+
+        t0 = time.perf_counter()
+        plan = cache.extend(new_lens, total)
+        logits = self.forward_paged(tokens, cos, sin, cache, plan, max_q_len=longest, max_kv_len=longest)
+        argmax_into(logits, tok)
+        if eos is not None:
+            finish()
+        out[:, 0] = tok[:, 0]
+        torch.cuda.synchronize(dev)
+        t1 = time.perf_counter()
+        for i in range(1, n_generate):
+            if graph is not None:
+                graph.replay()
+            else:
+                step()
+            out[:, i] = tok[:, 0]
+        torch.cuda.synchronize(dev)
+        t2 = time.perf_counter()
+        return out, {"prefill_s": t1 - t0, "decode_s": t2 - t1, "elapsed_s": t2 - t0}
 
     @torch.no_grad()
     def generate(self, prompt: torch.Tensor, n_generate: int, use_graph: bool = True):
@@ -611,12 +746,14 @@ class QuantizedDecoder(nn.Module):
 
     def linear_bytes_per_token(self) -> int:
         """INT4 codes + fp32 scale + u8 zero of every QuantizedLinear, plus the
-        fp16 lm_head: the bytes one decode step must stream."""
+        lm_head (fp16, or int8 codes): the bytes one decode step must stream."""
         total = 0
         for m in self.modules():
             if isinstance(m, QuantizedLinear):
                 g = m.scale.numel()
                 total += m.packed_weight.numel() + g * 5
+        if self.int8_head is not None:
+            return total + self.int8_head.weight.numel() + 4 * self.int8_head.scale.numel()
         return total + self.lm_head.numel() * 2
 
 
