@@ -226,7 +226,7 @@ struct AppendArgs {
   int64_t ld;  // elements per row of qkv
   int64_t n_slots;
   int T, H, KV, ps, L;
-  int chunk;   // tokens per workgroup of the cache's part
+  int chunk;   // tokens per workgroup of the cache's part, at most 64
   int cache_wgs;  // its workgroups per head
 };
 
@@ -246,20 +246,35 @@ PMI_DEV void store8(T* p, const float* v) {
   *reinterpret_cast<T8*>(p) = x;
 }
 
+// The angles of pairs d .. d + 7 at a position.
+template <int D>
+PMI_DEV void load_angles(const AppendArgs& a, int d, int pos, float* c, float* s) {
+  const f32x4* cp = reinterpret_cast<const f32x4*>(a.cos_t + (int64_t)pos * (D / 2) + d);
+  const f32x4* sp = reinterpret_cast<const f32x4*>(a.sin_t + (int64_t)pos * (D / 2) + d);
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+    const f32x4 x = cp[q], y = sp[q];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) c[4 * q + e] = x[e], s[4 * q + e] = y[e];
+  }
+}
+PMI_DEV void rotate8(float* lo, float* hi, const float* c, const float* s) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float x1 = lo[e], x2 = hi[e];
+    lo[e] = x1 * c[e] - x2 * s[e];
+    hi[e] = x2 * c[e] + x1 * s[e];
+  }
+}
+
 // Pairs d .. d + 7 of one head's row, rotated: lo and hi are its two halves' parts.
 template <typename T, int D>
 PMI_DEV void rotated8(const AppendArgs& a, const T* row, int d, int pos, float* lo, float* hi) {
+  float c[8], s[8];
   load8(row + d, lo);
   load8(row + d + D / 2, hi);
-  const f32x4* cp = reinterpret_cast<const f32x4*>(a.cos_t + (int64_t)pos * (D / 2) + d);
-  const f32x4* sp = reinterpret_cast<const f32x4*>(a.sin_t + (int64_t)pos * (D / 2) + d);
-  const f32x4 c[2] = {cp[0], cp[1]}, s[2] = {sp[0], sp[1]};
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const float x1 = lo[e], x2 = hi[e], ce = c[e >> 2][e & 3], se = s[e >> 2][e & 3];
-    lo[e] = x1 * ce - x2 * se;
-    hi[e] = x2 * ce + x1 * se;
-  }
+  load_angles<D>(a, d, pos, c, s);
+  rotate8(lo, hi, c, s);
 }
 
 // Four values as codes: x * inv rounded to the nearest code, within +-top.
@@ -297,38 +312,73 @@ PMI_DEV void decode4(uint32_t w, float* v) {
 // that a maximum keeps them and the page's scale shows them.
 PMI_DEV uint32_t abs_bits(float x) { return __builtin_bit_cast(uint32_t, x) & 0x7fffffffu; }
 
+// What of a run stays on the chip between its maximum and its codes: 512 units of 16
+// values, keys in registers (2 units a thread), values in LDS as they came.
+constexpr int kHeldUnits = 2;
+constexpr int kHeldBytes = 256 * kHeldUnits * 16 * 2;
+
 // One run of new tokens, consecutive slots of one page, of one KV head: the larger
 // of the page's scale and what they need; the codes of the tokens before them again
-// where it grew; their own codes. All 256 threads.
+// where it grew; their own codes. All 256 threads. Runs of up to 64 tokens (D 128; 128
+// of D 64) are read once, longer ones again for their codes.
 template <typename T, int D, bool FP8>
-PMI_DEV void append_run(const AppendArgs& a, int t0, int n, int slot, int kh, uint32_t* red) {
+PMI_DEV void append_run(const AppendArgs& a, int t0, int n, int slot, int kh, uint32_t* red, T* held) {
   constexpr float kTop = FP8 ? 448.f : 127.f;
+  constexpr int kHeldRows = 256 * kHeldUnits * 16 / D;
   const int tid = threadIdx.x;
-  const int page = slot / a.ps, first = slot - page * a.ps;
+  const int page = slot / a.ps, first = slot - page * a.ps, units = n * (D / 16);
   const int64_t cell = (int64_t)page * a.KV + kh;
   const T* base = (const T*)a.qkv + (int64_t)(a.H + kh) * D;
   uint8_t* kc = a.k_cache + cell * a.ps * D;
   uint8_t* vc = a.v_cache + cell * a.ps * D;
   uint32_t mk = 0, mv = 0;
-  for (int u = tid; u < n * (D / 16); u += 256) {
-    const int i = u / (D / 16), d = 8 * (u % (D / 16));
-    const int pos = min(max(a.positions[t0 + i], 0), a.L - 1);
-    float lo[8], hi[8];
-    const T* row = base + (int64_t)(t0 + i) * a.ld;
-    rotated8<T, D>(a, row, d, pos, lo, hi);
+  float lo[kHeldUnits][8], hi[kHeldUnits][8];
+  const auto turned = [&](int u, float* l, float* h) {
+    const int i = u / (D / 16), pos = min(max(a.positions[t0 + i], 0), a.L - 1);
+    rotated8<T, D>(a, base + (int64_t)(t0 + i) * a.ld, 8 * (u % (D / 16)), pos, l, h);
+  };
+  const auto largest = [&](uint32_t m, const float* l, const float* h) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) mk = max(mk, max(abs_bits(lo[e]), abs_bits(hi[e])));
-    load8(row + (int64_t)a.KV * D + d, lo);
-    load8(row + (int64_t)a.KV * D + d + D / 2, hi);
+    for (int e = 0; e < 8; ++e) m = max(m, max(abs_bits(l[e]), abs_bits(h[e])));
+    return m;
+  };
+  const auto values = [&](int u) { return base + (int64_t)(t0 + u / (D / 8)) * a.ld + (int64_t)a.KV * D + 8 * (u % (D / 8)); };
+  typedef T T8 __attribute__((ext_vector_type(8)));
+  const auto largest_value = [&](const T8& x) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) mv = max(mv, max(abs_bits(lo[e]), abs_bits(hi[e])));
+    for (int e = 0; e < 8; ++e) mv = max(mv, abs_bits((float)x[e]));
+  };
+  __syncthreads();  // red and held of the previous run are read
+  {
+    T8 x[2 * kHeldUnits];
+#pragma unroll
+    for (int j = 0; j < 2 * kHeldUnits; ++j)
+      if (tid + 256 * j < 2 * units) x[j] = *reinterpret_cast<const T8*>(values(tid + 256 * j));
+#pragma unroll
+    for (int j = 0; j < kHeldUnits; ++j)
+      if (tid + 256 * j < units) turned(tid + 256 * j, lo[j], hi[j]);
+#pragma unroll
+    for (int j = 0; j < 2 * kHeldUnits; ++j)
+      if (tid + 256 * j < 2 * units) {
+        reinterpret_cast<T8*>(held)[tid + 256 * j] = x[j];
+        largest_value(x[j]);
+      }
+#pragma unroll
+    for (int j = 0; j < kHeldUnits; ++j)
+      if (tid + 256 * j < units) mk = largest(mk, lo[j], hi[j]);
+  }
+  for (int u = tid + 512 * kHeldUnits; u < 2 * units; u += 256)
+    largest_value(*reinterpret_cast<const T8*>(values(u)));
+  for (int u = tid + 256 * kHeldUnits; u < units; u += 256) {
+    float l[8], h[8];
+    turned(u, l, h);
+    mk = largest(mk, l, h);
   }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) {
     mk = max(mk, (uint32_t)__shfl_xor((int)mk, o));
     mv = max(mv, (uint32_t)__shfl_xor((int)mv, o));
   }
-  __syncthreads();  // red of the previous run is read
   if ((tid & 63) == 0) red[2 * (tid >> 6)] = mk, red[2 * (tid >> 6) + 1] = mv;
   const float before_k = first ? a.k_scale[cell] : 0.f, before_v = first ? a.v_scale[cell] : 0.f;
   __syncthreads();  // and everybody has the page's scales before they are replaced
@@ -353,80 +403,107 @@ PMI_DEV void append_run(const AppendArgs& a, int t0, int n, int slot, int kh, ui
       *reinterpret_cast<u32x4*>(kc + 16 * u) = w;
     }
   }
-  for (int u = tid; u < n * (D / 16); u += 256) {
-    const int i = u / (D / 16), d = 8 * (u % (D / 16));
-    const int pos = min(max(a.positions[t0 + i], 0), a.L - 1);
-    float lo[8], hi[8];
-    rotated8<T, D>(a, base + (int64_t)(t0 + i) * a.ld, d, pos, lo, hi);
-    uint8_t* dst = kc + (first + i) * D + d;
+  const auto store_key = [&](int u, const float* l, const float* h) {
+    uint8_t* dst = kc + (first + u / (D / 16)) * D + 8 * (u % (D / 16));
     typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-    *reinterpret_cast<u32x2*>(dst) = u32x2{code4<FP8>(lo, inv_k), code4<FP8>(lo + 4, inv_k)};
-    *reinterpret_cast<u32x2*>(dst + D / 2) = u32x2{code4<FP8>(hi, inv_k), code4<FP8>(hi + 4, inv_k)};
+    *reinterpret_cast<u32x2*>(dst) = u32x2{code4<FP8>(l, inv_k), code4<FP8>(l + 4, inv_k)};
+    *reinterpret_cast<u32x2*>(dst + D / 2) = u32x2{code4<FP8>(h, inv_k), code4<FP8>(h + 4, inv_k)};
+  };
+#pragma unroll
+  for (int j = 0; j < kHeldUnits; ++j)
+    if (tid + 256 * j < units) store_key(tid + 256 * j, lo[j], hi[j]);
+  for (int u = tid + 256 * kHeldUnits; u < units; u += 256) {
+    float l[8], h[8];
+    turned(u, l, h);
+    store_key(u, l, h);
   }
   // v: one thread takes the 16 tokens of a block at one dimension
   const float fv = grow_v && first ? before_v / sv : 1.f;
   const int b0 = (grow_v ? 0 : first) / 16, b1 = (first + n + 15) / 16;
   for (int u = tid; u < (b1 - b0) * D; u += 256) {
-    const int b = b0 + u / D, d = u % D;
+    const int b = b0 + u / D, d = u % D;  // b is the same in a whole wave
     u32x4* at = reinterpret_cast<u32x4*>(vc + ((int64_t)b * D + d) * 16);
-    u32x4 w = *at;
+    u32x4 w = {0, 0, 0, 0};
+    if (16 * b < first || 16 * b + 16 > first + n) w = *at;
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       const int j0 = 16 * b + 4 * q;  // token of the page
-      float old[4], fresh[4];
-      decode4<FP8>(w[q], old);
+      float fresh[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int i = j0 + e - first;
-        fresh[e] = i >= 0 && i < n ? (float)base[(int64_t)(t0 + i) * a.ld + (int64_t)a.KV * D + d] : 0.f;
+        fresh[e] = 0.f;
+        if (i >= 0 && i < n)
+          fresh[e] = (float)(i < kHeldRows ? held[i * D + d] : base[(int64_t)(t0 + i) * a.ld + (int64_t)a.KV * D + d]);
       }
-      const uint32_t cold = code4<FP8>(old, fv), cnew = code4<FP8>(fresh, inv_v);
-      uint32_t o = 0;
+      const uint32_t cnew = code4<FP8>(fresh, inv_v);
+      if (j0 >= first && j0 + 4 <= first + n) {
+        w[q] = cnew;
+      } else if (j0 < first + n) {
+        float old[4];
+        decode4<FP8>(w[q], old);
+        const uint32_t cold = grow_v ? code4<FP8>(old, fv) : w[q];
+        uint32_t o = 0;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int j = j0 + e;
-        const uint32_t m = 255u << (8 * e);
-        o |= (j < first ? (grow_v ? cold : w[q]) : j < first + n ? cnew : w[q]) & m;
+        for (int e = 0; e < 4; ++e) {
+          const int j = j0 + e;
+          o |= (j < first ? cold : j < first + n ? cnew : w[q]) & (255u << (8 * e));
+        }
+        w[q] = o;
       }
-      w[q] = o;
     }
     *at = w;
   }
 }
 
 // Grid: (cache_wgs + query workgroups, KV). The first take `chunk` tokens of one KV
-// head each and write the runs that begin among them; the others rotate the queries.
+// head each and write the runs that begin among them; the others rotate the queries, a
+// thread the same dimensions of the KV head's whole group, with one load of their angles.
 template <typename T, int D, bool FP8>
 __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
   __shared__ uint32_t red[8];
   __shared__ int run_end;
+  __shared__ __attribute__((aligned(16))) T held[kHeldBytes / sizeof(T)];
   const int tid = threadIdx.x, kh = blockIdx.y;
   if ((int)blockIdx.x >= a.cache_wgs) {
     const int g = a.H / a.KV;
-    const int64_t u = (int64_t)(blockIdx.x - a.cache_wgs) * 256 + tid;
-    const int d = 8 * (int)(u % (D / 16)), hh = (int)(u / (D / 16) % g);
-    const int64_t t = u / (D / 16) / g;
+    const int64_t u = (int64_t)(blockIdx.x - a.cache_wgs) * 256 + tid, t = u / (D / 16);
+    const int d = 8 * (int)(u % (D / 16));
     if (t >= a.T) return;
-    const int h = kh * g + hh, pos = min(max(a.positions[t], 0), a.L - 1);
-    float lo[8], hi[8];
-    rotated8<T, D>(a, (const T*)a.qkv + t * a.ld + (int64_t)h * D, d, pos, lo, hi);
-    T* dst = (T*)a.q_out + (t * a.H + h) * D + d;
-    store8(dst, lo);
-    store8(dst + D / 2, hi);
+    const int pos = min(max(a.positions[t], 0), a.L - 1);
+    float c[8], s[8];
+    load_angles<D>(a, d, pos, c, s);
+    const T* src = (const T*)a.qkv + t * a.ld + (int64_t)kh * g * D + d;
+    T* dst = (T*)a.q_out + (t * a.H + kh * g) * D + d;
+#pragma unroll 4
+    for (int h = 0; h < g; ++h) {
+      float lo[8], hi[8];
+      load8(src + h * D, lo);
+      load8(src + h * D + D / 2, hi);
+      rotate8(lo, hi, c, s);
+      store8(dst + h * D, lo);
+      store8(dst + h * D + D / 2, hi);
+    }
     return;
   }
-  const int c0 = blockIdx.x * a.chunk, c1 = min(a.T, c0 + a.chunk);
-  for (int t = c0; t < c1; ++t) {  // every thread sees the same slots
-    const int slot = a.slots[t];
-    if (slot < 0 || slot >= a.n_slots) continue;
-    if (t > 0 && slot % a.ps != 0 && a.slots[t - 1] == slot - 1) continue;  // inside a run
+  // every wave looks at the whole chunk: lane l at its token l, and where runs begin
+  const int lane = tid & 63, c0 = blockIdx.x * a.chunk, at = c0 + lane;
+  int mine = -1, before = -1;
+  if (lane < a.chunk && at < a.T) {
+    mine = a.slots[at];
+    if (at > 0) before = a.slots[at - 1];
+  }
+  const bool begins = mine >= 0 && mine < a.n_slots && !(mine % a.ps != 0 && before == mine - 1);
+  for (uint64_t todo = __ballot(begins); todo; todo &= todo - 1) {
+    const int l = __builtin_ctzll(todo), t = c0 + l;
+    const int slot = __builtin_amdgcn_readlane(mine, l);
     const int room = min(a.ps - slot % a.ps, a.T - t);
     __syncthreads();
     if (tid == 0) run_end = room;
     __syncthreads();
     if (tid < room && a.slots[t + tid] != slot + tid) atomicMin(&run_end, tid);
     __syncthreads();
-    append_run<T, D, FP8>(a, t, run_end, slot, kh, red);
+    append_run<T, D, FP8>(a, t, run_end, slot, kh, red, held);
   }
 }
 
@@ -515,7 +592,7 @@ hipError_t launch_append_kv(const PagedCache& c, const void* qkv, int64_t ld, bo
   // Many are mostly runs of whole pages.
   a.chunk = T <= 1024 ? 1 : 16;
   a.cache_wgs = (int)((T + a.chunk - 1) / a.chunk);
-  const int64_t wgs = (T * (H / c.KV) * (c.D / 16) + 255) / 256;
+  const int64_t wgs = (T * (c.D / 16) + 255) / 256;
   return bf16 ? append_t<__bf16>(a, (int)c.D, c.fp8, wgs, stream) : append_t<f16>(a, (int)c.D, c.fp8, wgs, stream);
 }
 
