@@ -22,23 +22,34 @@ def _code_width(K: int) -> int:
     return -(-K // 16) * 16
 
 
+def _rows(x: torch.Tensor, fn: str) -> torch.Tensor:
+    """x after its checks, with contiguous rows."""
+    if not x.is_cuda:
+        raise RuntimeError(f"{fn} requires HIP (cuda) tensors.")
+    assert x.dim() == 2 and x.dtype in _VALUES, (
+        f"x must be a float16, bfloat16 or float32 [M, K] tensor, got {x.dtype} {tuple(x.shape)}")
+    if x.stride(1) != 1 and x.shape[1] > 1 or (x.shape[0] > 1 and x.stride(0) < x.shape[1]):
+        x = x.contiguous()
+    return x
+
+
+def _quantize(x: torch.Tensor, codes: int, scales: int, stream: int) -> None:
+    M, K = x.shape
+    _lib.check(_lib.lib().pmi_quantize_rows(x.data_ptr(), _VALUES[x.dtype], max(x.stride(0), K), codes, scales, M, K,
+                                            stream), "pmi_quantize_rows")
+
+
 def quantize_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """(codes int8 [M, K rounded up to 16], scales fp32 [M]) of x [M, K] (fp16, bf16 or
     fp32): code = round(x * (127 / amax)), scale = amax / 127, amax the row's largest
     |x|; zeros in the codes' last columns past K. A row of zeros has scale 0, one with
     an infinity or NaN such a scale. K <= 131072."""
-    if not x.is_cuda:
-        raise RuntimeError("quantize_rows requires HIP (cuda) tensors.")
-    assert x.dim() == 2 and x.dtype in _VALUES, "x must be a float16, bfloat16 or float32 [M, K] tensor"
+    x = _rows(x, "quantize_rows")
     M, K = x.shape
-    if x.stride(1) != 1 and K > 1 or (M > 1 and x.stride(0) < K):
-        x = x.contiguous()
     codes = torch.empty(M, _code_width(K), dtype=torch.int8, device=x.device)
     scales = torch.empty(M, dtype=torch.float32, device=x.device)
     with _DeviceGuard(x.device):
-        _lib.check(_lib.lib().pmi_quantize_rows(x.data_ptr(), _VALUES[x.dtype], max(x.stride(0), K), codes.data_ptr(),
-                                                scales.data_ptr(), M, K, _stream_handle(x.device)),
-                   "pmi_quantize_rows")
+        _quantize(x, codes.data_ptr(), scales.data_ptr(), _stream_handle(x.device))
     return codes, scales
 
 
@@ -57,6 +68,24 @@ def _check_weight(x: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, bias
     return N
 
 
+def _bias_and_out(bias: torch.Tensor | None, out: torch.Tensor | None, M: int, N: int, dtype: torch.dtype,
+                  dev: torch.device) -> tuple[torch.Tensor | None, torch.Tensor]:
+    if bias is not None:
+        bias = bias.to(dtype).contiguous()
+    if out is None:
+        return bias, torch.empty(M, N, dtype=dtype, device=dev)
+    assert out.dtype == dtype and tuple(out.shape) == (M, N) and out.is_contiguous() and out.device == dev, \
+        f"out must be a contiguous [{M}, {N}] {dtype} tensor on {dev}"
+    return bias, out
+
+
+def _product(codes: int, scales: int, w: torch.Tensor, w_scales: torch.Tensor, bias: torch.Tensor | None,
+             out: torch.Tensor, K: int, stream: int) -> None:
+    _lib.check(_lib.lib().pmi_matmul_w8a8(
+        codes, scales, w.data_ptr(), w_scales.data_ptr(), bias.data_ptr() if bias is not None else None,
+        out.data_ptr(), _VALUES[out.dtype], out.shape[0], out.shape[1], K, stream), "pmi_matmul_w8a8")
+
+
 def matmul_int8(codes: torch.Tensor, scales: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, K: int,
                 dtype: torch.dtype, *, bias: torch.Tensor | None = None,
                 out: torch.Tensor | None = None) -> torch.Tensor:
@@ -73,18 +102,9 @@ def matmul_int8(codes: torch.Tensor, scales: torch.Tensor, w: torch.Tensor, w_sc
         scales.device == codes.device, f"scales must be a contiguous float32 [{M}] tensor on {codes.device}"
     N = _check_weight(codes, w, w_scales, bias, K)
     dev = codes.device
-    if bias is not None:
-        bias = bias.to(dtype).contiguous()
-    if out is None:
-        out = torch.empty(M, N, dtype=dtype, device=dev)
-    else:
-        assert out.dtype == dtype and tuple(out.shape) == (M, N) and out.is_contiguous() and out.device == dev, \
-            f"out must be a contiguous [{M}, {N}] {dtype} tensor on {dev}"
+    bias, out = _bias_and_out(bias, out, M, N, dtype, dev)
     with _DeviceGuard(dev):
-        _lib.check(_lib.lib().pmi_matmul_w8a8(
-            codes.data_ptr(), scales.data_ptr(), w.data_ptr(), w_scales.data_ptr(),
-            bias.data_ptr() if bias is not None else None, out.data_ptr(), _VALUES[dtype], M, N, K,
-            _stream_handle(dev)), "pmi_matmul_w8a8")
+        _product(codes.data_ptr(), scales.data_ptr(), w, w_scales, bias, out, K, _stream_handle(dev))
     return out
 
 
@@ -94,11 +114,19 @@ def matmul_w8a8(x: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, *, bia
     fp32): x is quantised row by row, ``w`` and ``w_scales`` are ``quantize_rows`` of the
     weight [N, K]. RuntimeError when x is not on a HIP device, AssertionError on layout
     violations."""
-    if not x.is_cuda:
-        raise RuntimeError("matmul_w8a8 requires HIP (cuda) tensors.")
-    assert x.dim() == 2, f"x must be 2-D [M, K], got shape {tuple(x.shape)}"
-    codes, scales = quantize_rows(x)
-    return matmul_int8(codes, scales, w, w_scales, x.shape[1], x.dtype, bias=bias, out=out)
+    x = _rows(x, "matmul_w8a8")
+    M, K = x.shape
+    dev = x.device
+    N = _check_weight(x, w, w_scales, bias, K)
+    bias, out = _bias_and_out(bias, out, M, N, x.dtype, dev)
+    codes = M * _code_width(K)
+    scratch = torch.empty(codes + 4 * M, dtype=torch.int8, device=dev)  # the codes, then the scales
+    at = scratch.data_ptr()
+    with _DeviceGuard(dev):
+        stream = _stream_handle(dev)
+        _quantize(x, at, at + codes, stream)
+        _product(at, at + codes, w, w_scales, bias, out, K, stream)
+    return out
 
 
 class Int8Linear(nn.Module):

@@ -25,7 +25,9 @@ from . import _lib
 
 
 def _stream_handle(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    # (without the Stream object of torch.cuda.current_stream: 0.2 us against 1.8 us a call)
+    index = torch.cuda.current_device() if device.index is None else device.index
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
 class _DeviceGuard:

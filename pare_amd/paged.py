@@ -112,14 +112,11 @@ def extend_block_tables(block_tables: torch.Tensor, kv_lens: torch.Tensor, new_l
         _ints(dev, R, kv_lens_out=kv_lens_out)
     if pool_out is not None:
         _ints(dev, 4, pool_out=pool_out)
-    buf = torch.empty(3 * R + 2 + 2 * total + (R if kv_lens_out is None else 0) + (4 if pool_out is None else 0),
-                      dtype=torch.int32, device=dev)
-    cut = [R + 1, R, R + 1, total, total]
-    q_starts, first, fresh, positions, slots, rest = buf.split([*cut, buf.numel() - sum(cut)])
-    if kv_lens_out is None:
-        kv_lens_out, rest = rest[:R], rest[R:]
-    if pool_out is None:
-        pool_out = rest
+    cut = [R + 1, R, R + 1, total, total, R if kv_lens_out is None else 0, 4 if pool_out is None else 0]
+    q_starts, first, fresh, positions, slots, lens, state = torch.empty(
+        sum(cut), dtype=torch.int32, device=dev).split(cut)
+    kv_lens_out = lens if kv_lens_out is None else kv_lens_out
+    pool_out = state if pool_out is None else pool_out
     with _DeviceGuard(dev):
         _lib.check(_lib.lib().pmi_extend_block_tables(
             block_tables.data_ptr(), _row_stride(block_tables), kv_lens.data_ptr(), new_lens.data_ptr(),
