@@ -13,6 +13,7 @@ import numpy as np
 import torch
 
 TOP = {torch.int8: np.float32(127.0), torch.float8_e4m3fn: np.float32(448.0)}
+LARGEST = np.finfo(np.float32).max
 
 
 def extend_tables(tables, kv_lens, new_lens, free_pages, pool, ps, total):
@@ -93,7 +94,8 @@ class Cache:
                     old = self.scales[i][page, h] if at else np.float32(0)
                     want = np.abs(new[:, h]).max() * np.float32(np.float32(1) / top)
                     scale = np.maximum(old, want)
-                    inv = np.float32(1) / scale if scale > 0 else np.float32(0)
+                    with np.errstate(over="ignore"):
+                        inv = np.minimum(np.float32(1) / scale, LARGEST) if scale > 0 else np.float32(0)
                     cells = self.codes[i][page, h]
                     if at and scale > old:
                         cells[:at] = encode(decode(cells[:at], self.dtype) * np.float32(old / scale), self.dtype)
@@ -160,8 +162,8 @@ def attention(q, k, v, tables, kv_lens, q_starts, ps, scale, window=0):
 def quantize_rows(x: np.ndarray):
     """codes int8 [M, K], scales fp32 [M] of fp32 rows, one IEEE operation at a time."""
     amax = np.abs(x).max(1).astype(np.float32)
-    with np.errstate(divide="ignore"):
-        inv = np.where(amax > 0, np.float32(127) / amax, np.float32(0)).astype(np.float32)
+    with np.errstate(divide="ignore", over="ignore"):
+        inv = np.where(amax > 0, np.minimum(np.float32(127) / amax, LARGEST), np.float32(0)).astype(np.float32)
     return np.clip(np.rint(x * inv[:, None]), -127, 127).astype(np.int8), amax * np.float32(np.float32(1) / np.float32(127))
 
 

@@ -173,7 +173,8 @@ constexpr float kLog2e = 1.4426950408889634f;
 // scales not before they have doubled): raising it rescales all sums, and some row of a tile has a
 // new maximum more often than not. 2^8 2^6 2 < 65504, and what is lost under fp16's range is
 // below 2^-25 / 2^8 of the largest probability.
-constexpr float kPBias = 256.f, kSlack = 6.f;
+// The unit begins at kLeastUnit, so that its inverse is finite: values under 2^-24 of it are lost.
+constexpr float kPBias = 256.f, kSlack = 6.f, kLeastUnit = 1e-30f;
 
 // ---- few query rows ------------------------------------------------------------------
 // Requests of few query rows (tokens x heads of one KV head): bound by the bytes of the
@@ -284,7 +285,7 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(AttnArgs a) {
   f32x4 acc[DT];
 #pragma unroll
   for (int d = 0; d < DT; ++d) acc[d] = f32x4{0.f, 0.f, 0.f, 0.f};
-  float m = -INFINITY, sum = 0.f, vref = 0.f;
+  float m = -INFINITY, sum = 0.f, vref = kLeastUnit;
   const int64_t cell_bytes = (int64_t)a.ps * D;
 
   // Look-ups run ahead: a tile's entry of the table (of the lane's 16 tokens, block h) is loaded
@@ -343,12 +344,12 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(AttnArgs a) {
     // the unit of acc: the largest value scale so far, or half of it
     const float top = fmaxf(vref, max_over_h(tvs < INFINITY ? tvs : 0.f));
     if (__any(top > 2.f * vref)) {
-      const float f = vref > 0.f ? vref / top : 1.f;
+      const float f = vref / top;
 #pragma unroll
       for (int d = 0; d < DT; ++d) acc[d] *= f;
       vref = top;
     }
-    const float vs = vref > 0.f ? tvs * (kPBias / vref) : 0.f;
+    const float vs = tvs * (kPBias / vref);
     const bool masked = p < safe_lo || p + 64 > safe_hi || p + 64 > p1 || __any(gone);
     const int at = p + 16 * h;
     float x[16];
@@ -667,7 +668,7 @@ __global__ __launch_bounds__(256, 2) void attention_rows_kernel(AttnArgs a) {
   for (int d = 0; d < D / 32; ++d)
 #pragma unroll
     for (int e = 0; e < 16; ++e) acc[d][e] = 0.f;
-  float m = -INFINITY, sum = 0.f, vref = 0.f, vinv = 0.f;
+  float m = -INFINITY, sum = 0.f, vref = kLeastUnit, vinv = kPBias / kLeastUnit;
   const int32_t* table = a.tables + (int64_t)r * a.stride;
   const int64_t cell_bytes = (int64_t)a.ps * D;
 
@@ -776,7 +777,7 @@ __global__ __launch_bounds__(256, 2) void attention_rows_kernel(AttnArgs a) {
 #pragma unroll
       for (int b = 0; b < 4; ++b) top = fmaxf(top, cur.vs[b] < INFINITY ? cur.vs[b] : 0.f);
       if (top > 2.f * vref) {
-        const float f = vref > 0.f ? vref / top : 1.f;
+        const float f = vref / top;
 #pragma unroll
         for (int d = 0; d < D / 32; ++d) acc[d] *= f;
         vref = top;

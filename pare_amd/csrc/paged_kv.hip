@@ -11,6 +11,8 @@
 //
 // None of these has a counterpart in the reference, whose decode is HuggingFace's
 // cache (pare/eval/throughput.py:84-126 times HF generate).
+#include <cfloat>
+
 #include "paged.h"
 #include "pmi_common.h"
 #include "pmi_launch.h"
@@ -387,7 +389,8 @@ PMI_DEV void append_run(const AppendArgs& a, int t0, int n, int slot, int kh, ui
   const float want_k = __builtin_bit_cast(float, mk) * (1.f / kTop), want_v = __builtin_bit_cast(float, mv) * (1.f / kTop);
   const bool grow_k = abs_bits(want_k) > abs_bits(before_k), grow_v = abs_bits(want_v) > abs_bits(before_v);
   const float sk = grow_k ? want_k : before_k, sv = grow_v ? want_v : before_v;
-  const float inv_k = sk > 0.f ? 1.f / sk : 0.f, inv_v = sv > 0.f ? 1.f / sv : 0.f;
+  // (finite, also for subnormal scales)
+  const float inv_k = sk > 0.f ? fminf(1.f / sk, FLT_MAX) : 0.f, inv_v = sv > 0.f ? fminf(1.f / sv, FLT_MAX) : 0.f;
   if (tid == 0) a.k_scale[cell] = sk, a.v_scale[cell] = sv;
 
   if (first && grow_k) {

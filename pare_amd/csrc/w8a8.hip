@@ -8,6 +8,7 @@
 // products nor a split of K changes a bit; the scales are applied in fp32 and y is
 // rounded once. The reference only simulates this (its quantize_inputs path rounds the
 // activations and multiplies in floating point, pare/layers/linear.py:120-138).
+#include <cfloat>
 #include <atomic>
 
 #include "pmi_common.h"
@@ -68,7 +69,7 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(const T* __restrict_
   __syncthreads();
   m = max(max(red[0], red[1]), max(red[2], red[3]));
   const float amax = __builtin_bit_cast(float, m);
-  const float inv = amax > 0.f ? 127.f / amax : 0.f;
+  const float inv = amax > 0.f ? fminf(127.f / amax, FLT_MAX) : 0.f;  // (finite for the smallest rows too)
   if (tid == 0) scales[blockIdx.x] = amax * (1.f / 127.f);
   int8_t* out = codes + (int64_t)blockIdx.x * ld;
   auto put = [&](int k, const vec8<T>& v) {

@@ -81,6 +81,19 @@ def test_quantize_rows_equals_the_oracle_bit_for_bit(dtype, M, K):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_quantize_the_smallest_rows(dtype):
+    """Rows whose scale has no finite inverse, zeros among them."""
+    x = (torch.randn(5, 40, generator=torch.Generator().manual_seed(2)) * 1e-38).to(dtype)
+    x[:, 3:9] = 0
+    codes, scales = P.quantize_rows(x.to(DEV))
+    want, want_scales = S.quantize_rows(x.float().numpy())
+    np.testing.assert_array_equal(scales.cpu().numpy(), want_scales)
+    np.testing.assert_array_equal(codes[:, :40].cpu().numpy(), want)
+    assert (want[:, 3:9] == 0).all()
+
+
+@gpu
 def test_rows_with_infinities_and_nan_are_not_finite():
     x = torch.ones(4, 64, dtype=torch.float16, device=DEV)
     x[1, 3], x[2, 60] = float("nan"), float("-inf")

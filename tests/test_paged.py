@@ -546,6 +546,42 @@ def test_attention_of_peaked_and_large_scores(new):
 
 
 @gpu
+@pytest.mark.parametrize("code", CODES)
+def test_append_of_the_smallest_values(code):
+    """Values whose scale has no finite inverse in fp32: still codes of the right sign and
+    no larger than they should be, so off by at most themselves, top / FLT_MAX."""
+    g = torch.Generator().manual_seed(1)
+    qkv = (torch.randn(20, 3 * 64, generator=g) * 1e-38).to(torch.bfloat16)
+    qkv[3:6] = 0
+    cos, sin = _rope(20, 64)
+    c = P.PagedKVCache(1, 1, 20, 1, 64, DEV, page_size=16, dtype=code)
+    plan = c.extend(_ints([20]), 20)
+    c.append(0, qkv.to(DEV), torch.from_numpy(cos).to(DEV), torch.from_numpy(sin).to(DEV), plan)
+    want = S.Cache(2, 1, 16, 64, code)
+    want.append(qkv.float().numpy(), cos, sin, np.arange(20), np.arange(20), 1)
+    _check_cache(want, c.k[0], c.v[0], c.k_scale[0], c.v_scale[0])
+    _, v = P.read_kv_pages(c.block_tables[0], c.k[0], c.v[0], c.k_scale[0], c.v_scale[0], dtype=torch.float32)
+    got = v.reshape(-1, 64)[:20].cpu().double()
+    err = (got - qkv[:, 128:].double()).abs()
+    assert err.max() <= (127 if code == torch.int8 else 448) / np.finfo(np.float32).max
+
+
+@gpu
+@pytest.mark.parametrize("new", [1, 40])
+@pytest.mark.parametrize("code", CODES)
+def test_attention_of_the_smallest_value_scales(code, new):
+    """Value scales of 1e-38 and zero beside ordinary ones, seen by one request each."""
+    lens = [40, 200, 130]
+    c, tables, starts, q = _attention_case(code, torch.bfloat16, 8, 2, 64, 16, lens, [new] * 3)
+    c.scales[1][tables[0, :3]] = 1e-38
+    c.scales[1][tables[1, 1::2]] = 1e-38
+    c.scales[1][tables[2, :8]] = 0
+    got = _run(c, tables, lens, starts, q)
+    _check(got, *_oracle(c, tables, lens, starts, q), torch.bfloat16)
+    assert got[:new].abs().max() <= 1e-38 * (127 if code == torch.int8 else 448) * 1.01
+
+
+@gpu
 def test_shared_pages_and_bounds_that_are_too_large():
     """Two requests with a common prefix's pages, limits far above what is there."""
     lens, new = [100, 101], [1, 1]
