@@ -334,13 +334,14 @@ __global__ __launch_bounds__(512, 2) void w8a8_few_kernel(W8A8 p) {
     multiply(0);
   }
   __syncthreads();  // sums are cleared
-  // result e of tile (i, j): weight row 16 i + 4 h + e, activation row 16 j + c
+  // result e of tile (i, j): weight row 16 i + 4 h + e, activation row 16 j + c; kept at 16 i + 4 e + h
+  // of the row, so that the 64 lanes of an addition are in 64 banks
 #pragma unroll
   for (int i = 0; i < NT; ++i)
 #pragma unroll
     for (int j = 0; j < MT; ++j)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) atomicAdd(&sums[16 * j + c][16 * i + 4 * h + e], acc[i][j][e]);
+      for (int e = 0; e < 4; ++e) atomicAdd(&sums[16 * j + c][16 * i + 4 * e + h], acc[i][j][e]);
   __syncthreads();
   const bool wide = N % 8 == 0 && (uintptr_t)p.y % (8 * sizeof(T)) == 0;
   for (int u = tid; u < M * 2 * NT; u += 512) {
@@ -350,7 +351,7 @@ __global__ __launch_bounds__(512, 2) void w8a8_few_kernel(W8A8 p) {
     int v[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      v[e] = sums[m][n - n0 + e];
+      v[e] = sums[m][((n - n0) & ~15) + 4 * (e & 3) + ((n - n0) >> 2 & 3) + (e >> 2)];
       sw[e] = n + e < N ? p.sw[n + e] : 0.f;
       bias[e] = p.bias && n + e < N ? (float)((const T*)p.bias)[n + e] : 0.f;
     }
