@@ -681,6 +681,17 @@ PMI_API int pmi_matmul_w8a8(const int8_t* x, const float* x_scales, const int8_t
                             const float* w_scales, const void* bias, void* y, int y_dtype,
                             int64_t M, int64_t N, int64_t K, void* stream);
 
+/* pmi_quantize_rows and pmi_matmul_w8a8 in one call, the same bit for bit: x [M, K], bias
+ * and y of dtype, x's rows x_stride elements apart. Few rows and channels (up to 4 rows of
+ * 4096 columns, 2 of 8192 or 1 of 16384, by 64 channels a CU) are one launch. y may be x. scratch: device memory of
+ * pmi_matmul_w8a8_scratch_bytes() bytes, 16-byte aligned, for the codes; calls that may
+ * run concurrently must not share it. */
+PMI_API int pmi_matmul_w8a8_rows(const void* x, int dtype, int64_t x_stride, const int8_t* w,
+                                 const float* w_scales, const void* bias, void* y, int64_t M,
+                                 int64_t N, int64_t K, void* scratch, size_t scratch_bytes,
+                                 void* stream);
+PMI_API size_t pmi_matmul_w8a8_scratch_bytes(int64_t M, int64_t K);
+
 /* ---- Measurement hook ------------------------------------------------------
  * Reads `bytes` (a multiple of 16) of device memory at `buf` once, with at most
  * `grid` workgroups of 8 waves (the GEMV's workgroup shape) each streaming one

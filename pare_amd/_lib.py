@@ -101,6 +101,8 @@ SIGNATURES = {
     "pmi_paged_attention_workspace_bytes": (ctypes.c_size_t, [_i64] * 8),
     "pmi_quantize_rows": (_i, [_vp, _i, _i64, _vp, _vp, _i64, _i64, _vp]),
     "pmi_matmul_w8a8": (_i, [*[_vp] * 6, _i, _i64, _i64, _i64, _vp]),
+    "pmi_matmul_w8a8_rows": (_i, [_vp, _i, _i64, *[_vp] * 4, *[_i64] * 3, _vp, ctypes.c_size_t, _vp]),
+    "pmi_matmul_w8a8_scratch_bytes": (ctypes.c_size_t, [_i64, _i64]),
     "pmi_read_probe": (_i, [_vp, _i64, _i64, _vp, _vp]),
     "pmi_silu_mul_f16": (_i, [_vp, _vp, _i64, _i64, _vp]),
 }

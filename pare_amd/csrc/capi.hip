@@ -1541,4 +1541,31 @@ int pmi_matmul_w8a8(const int8_t* x, const float* x_scales, const int8_t* w, con
   return from_hip(pmi::launch_w8a8(p, (hipStream_t)stream), fn);
 }
 
+size_t pmi_matmul_w8a8_scratch_bytes(int64_t M, int64_t K) {
+  if (M < 0 || K <= 0 || M >= (1ll << 24) || K > pmi::kW8A8MaxK) return 0;
+  return (size_t)M * ((K + 15) / 16 * 16 + 4);
+}
+
+int pmi_matmul_w8a8_rows(const void* x, int dtype, int64_t x_stride, const int8_t* w, const float* w_scales,
+                         const void* bias, void* y, int64_t M, int64_t N, int64_t K, void* scratch,
+                         size_t scratch_bytes, void* stream) {
+  const char* fn = "pmi_matmul_w8a8_rows";
+  if (dtype != PMI_F16 && dtype != PMI_BF16 && dtype != PMI_F32)
+    return fail(PMI_ERR_INVALID, "%s: dtype must be PMI_F16, PMI_BF16 or PMI_F32 (got %d)", fn, dtype);
+  if (int rc = check_w8a8(M, N, K, fn)) return rc;
+  if (x_stride < K) return fail(PMI_ERR_INVALID, "%s: x_stride=%lld is less than K", fn, (long long)x_stride);
+  if (x_stride >= (1ll << 36)) return fail(PMI_ERR_UNSUPPORTED, "%s: x_stride must be below 2^36", fn);
+  if (M == 0 || N == 0) return ok();
+  if (!x || !w || !w_scales || !y || !scratch) return fail(PMI_ERR_INVALID, "%s: null buffer", fn);
+  const size_t size = dtype == PMI_F32 ? 4 : 2;
+  if (!aligned(x, size) || !aligned(w, 16) || !aligned(y, size) || !aligned(bias, size) || !aligned(scratch, 16))
+    return fail(PMI_ERR_INVALID, "%s: w and scratch must be 16-byte aligned, x, y and bias multiples of their type", fn);
+  if (scratch_bytes < pmi_matmul_w8a8_scratch_bytes(M, K))
+    return fail(PMI_ERR_INVALID, "%s: needs a scratch of %zu bytes", fn, pmi_matmul_w8a8_scratch_bytes(M, K));
+  const int64_t ld = (K + 15) / 16 * 16;
+  int8_t* codes = (int8_t*)scratch;
+  const pmi::W8A8 p = {codes, (const float*)(codes + M * ld), w, w_scales, bias, y, M, N, ld, dtype};
+  return from_hip(pmi::launch_w8a8_rows(p, x, x_stride, K, (hipStream_t)stream), fn);
+}
+
 }  // extern "C"

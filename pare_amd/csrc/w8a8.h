@@ -24,5 +24,8 @@ struct W8A8 {
   int dtype;        // of y: PMI_F16, PMI_BF16 or PMI_F32
 };
 hipError_t launch_w8a8(const W8A8& p, hipStream_t stream);
+// The same of x [M, K] of y's type, row stride x_ld, which becomes codes first: p.x and
+// p.sx are where they may be kept.
+hipError_t launch_w8a8_rows(const W8A8& p, const void* x, int64_t x_ld, int64_t K, hipStream_t stream);
 
 }  // namespace pmi

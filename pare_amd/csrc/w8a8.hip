@@ -18,6 +18,13 @@
 namespace pmi {
 namespace {
 
+// Rows [M, K] that are not codes yet, of y's type.
+struct W8A8Rows {
+  const void* x;
+  int64_t ld;
+  int K, wide;  // wide: eight values may be read at once
+};
+
 typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
 typedef int32_t i32x16 __attribute__((ext_vector_type(16)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
@@ -40,6 +47,19 @@ PMI_DEV uint32_t abs_max8(const T* p, int n, bool wide, vec8<T>& v) {
   for (int e = 0; e < 8; ++e) m = max(m, __builtin_bit_cast(uint32_t, (float)v[e]) & 0x7fffffffu);
   return m;
 }
+
+template <typename T>
+PMI_DEV u32x2 codes_of8(const vec8<T>& v, float inv) {
+  u32x2 w = {0, 0};
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const int q = (int)fminf(fmaxf(rintf((float)v[e] * inv), -127.f), 127.f);
+    w[e >> 2] |= (uint32_t)(q & 255) << (8 * (e & 3));
+  }
+  return w;
+}
+// 127 / amax, finite for the smallest rows too; 0 of a row of zeros.
+PMI_DEV float inverse_of(float amax) { return amax > 0.f ? fminf(127.f / amax, FLT_MAX) : 0.f; }
 
 // Codes of a row, zeros from K to ld. One workgroup of 256 threads per row, eight values a
 // thread and step; the first kKeep steps (rows up to 8192) stay in registers between the
@@ -69,18 +89,10 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(const T* __restrict_
   __syncthreads();
   m = max(max(red[0], red[1]), max(red[2], red[3]));
   const float amax = __builtin_bit_cast(float, m);
-  const float inv = amax > 0.f ? fminf(127.f / amax, FLT_MAX) : 0.f;  // (finite for the smallest rows too)
+  const float inv = inverse_of(amax);
   if (tid == 0) scales[blockIdx.x] = amax * (1.f / 127.f);
   int8_t* out = codes + (int64_t)blockIdx.x * ld;
-  auto put = [&](int k, const vec8<T>& v) {
-    u32x2 w = {0, 0};
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int q = (int)fminf(fmaxf(rintf((float)v[e] * inv), -127.f), 127.f);
-      w[e >> 2] |= (uint32_t)(q & 255) << (8 * (e & 3));
-    }
-    *reinterpret_cast<u32x2*>(out + k) = w;
-  };
+  auto put = [&](int k, const vec8<T>& v) { *reinterpret_cast<u32x2*>(out + k) = codes_of8<T>(v, inv); };
 #pragma unroll
   for (int i = 0; i < kKeep; ++i) {
     const int k = 8 * (tid + 256 * i);
@@ -261,9 +273,17 @@ hipError_t tiles(const W8A8& p, hipStream_t stream) {
 // rows, its eight waves the steps of 128 columns in turn; both operands come straight from memory
 // to registers (the activations from L2), 16x16x64 products, the weights the rows of the
 // result. The waves' sums are added through LDS.
-template <typename T, int MT, int NT>
-__global__ __launch_bounds__(512, 2) void w8a8_few_kernel(W8A8 p) {
+//
+// ROWS: up to 4 rows (4 pieces of 4096 values) that are not codes yet. Every workgroup quantises
+// them for itself into LDS, behind its first loads of weights: a launch less, and the codes
+// are not read from L2.
+constexpr int kPieces = 4;
+template <typename T, int MT, int NT, bool ROWS>
+__global__ __launch_bounds__(512, 2) void w8a8_few_kernel(W8A8 p, W8A8Rows rows) {
   constexpr int kFly = 10 / (MT + NT) < 1 ? 1 : 10 / (MT + NT);  // steps in flight
+  __shared__ __attribute__((aligned(16))) int8_t codes[ROWS ? kPieces * (4096 + 128) : 16];
+  __shared__ uint32_t red[ROWS ? kPieces * 8 : 1];
+  __shared__ float row_scale[kPieces];
   __shared__ __attribute__((aligned(16))) int sums[16 * MT][16 * NT + 4];
   const int tid = threadIdx.x, l = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c = l & 15, h = l >> 4;
@@ -276,7 +296,9 @@ __global__ __launch_bounds__(512, 2) void w8a8_few_kernel(W8A8 p) {
 #pragma unroll
   for (int i = 0; i < NT; ++i) wrow[i] = p.w + (int64_t)min(n0 + 16 * i + c, N - 1) * ld;
 #pragma unroll
-  for (int j = 0; j < MT; ++j) xrow[j] = p.x + (int64_t)min(16 * j + c, M - 1) * ld;
+  for (int j = 0; j < MT; ++j) xrow[j] = ROWS ? nullptr : p.x + (int64_t)min(16 * j + c, M - 1) * ld;
+  // pieces of a row, and its stride in LDS (rows half the banks apart)
+  const int per_row = (ld + 4095) / 4096, x_row = 4096 * per_row + 128;
   i32x4 acc[NT][MT];
 #pragma unroll
   for (int i = 0; i < NT; ++i)
@@ -285,7 +307,7 @@ __global__ __launch_bounds__(512, 2) void w8a8_few_kernel(W8A8 p) {
   // a step: 128 columns, a lane's 32 h .. 32 h + 31 of a row (whole lines of 128 bytes a row)
   const i32x4 zero = {0, 0, 0, 0};
   const int full = ld / 128;  // whole steps
-  i32x4 wv[kFly][NT][2], xv[kFly][MT][2];
+  i32x4 wv[kFly][NT][2], xv[ROWS ? 1 : kFly][MT][2];
   auto load = [&](int f, int s) {  // step s, or (past the end) the first again
     const int k = 128 * (s < full ? s : 0) + 32 * h;
 #pragma unroll
@@ -293,34 +315,77 @@ __global__ __launch_bounds__(512, 2) void w8a8_few_kernel(W8A8 p) {
 #pragma unroll
       for (int q = 0; q < 2; ++q)
         wv[f][i][q] = __builtin_nontemporal_load(reinterpret_cast<const i32x4*>(wrow[i] + k + 16 * q));
+    if constexpr (!ROWS) {
 #pragma unroll
-    for (int j = 0; j < MT; ++j)
+      for (int j = 0; j < MT; ++j)
 #pragma unroll
-      for (int q = 0; q < 2; ++q) xv[f][j][q] = *reinterpret_cast<const i32x4*>(xrow[j] + k + 16 * q);
+        for (int q = 0; q < 2; ++q) xv[f][j][q] = *reinterpret_cast<const i32x4*>(xrow[j] + k + 16 * q);
+    }
   };
-  auto multiply = [&](int f) {
+  auto multiply = [&](int f, int s) {
+    const int g = ROWS ? 0 : f;
+    if constexpr (ROWS) {
+#pragma unroll
+      for (int q = 0; q < 2; ++q)
+        xv[0][0][q] = *reinterpret_cast<const i32x4*>(codes + min(c, M - 1) * x_row + 128 * s + 32 * h + 16 * q);
+    }
 #pragma unroll
     for (int q = 0; q < 2; ++q)
 #pragma unroll
       for (int i = 0; i < NT; ++i)
 #pragma unroll
         for (int j = 0; j < MT; ++j)
-          acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wv[f][i][q], xv[f][j][q], acc[i][j], 0, 0, 0);
+          acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wv[f][i][q], xv[g][j][q], acc[i][j], 0, 0, 0);
   };
+  if constexpr (ROWS) {
+    static_assert(MT == 1, "up to 4 rows");
+    vec8<T> v[kPieces];
+    uint32_t m[kPieces];
+#pragma unroll
+    for (int j = 0; j < kPieces; ++j) {
+      const int row = j / per_row, k = 4096 * (j - row * per_row) + 8 * tid;
+      v[j] = {};
+      m[j] = 0;
+      if (row < M && k < rows.K)
+        m[j] = abs_max8((const T*)rows.x + row * rows.ld + k, rows.K - k, rows.wide && k + 8 <= rows.K, v[j]);
+    }
+#pragma unroll
+    for (int f = 0; f < kFly; ++f) load(f, wave + 8 * f);
+#pragma unroll
+    for (int j = 0; j < kPieces; ++j) {
+#pragma unroll
+      for (int o = 32; o > 0; o >>= 1) m[j] = max(m[j], (uint32_t)__shfl_xor((int)m[j], o));
+      if (l == 0) red[8 * j + wave] = m[j];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < kPieces; ++j) {
+      const int row = j / per_row, piece = j - row * per_row;
+      if (row >= M) continue;
+      uint32_t top = 0;
+      for (int i = 8 * row * per_row; i < 8 * (row + 1) * per_row; ++i) top = max(top, red[i]);
+      const float amax = __builtin_bit_cast(float, top);
+      if (tid == 0) row_scale[row] = amax * (1.f / 127.f);
+      *reinterpret_cast<u32x2*>(codes + row * x_row + 4096 * piece + 8 * tid) = codes_of8<T>(v[j], inverse_of(amax));
+    }
+    __syncthreads();
+  }
   if (wave < full) {
     int s = wave;
+    if constexpr (!ROWS) {
 #pragma unroll
-    for (int f = 0; f < kFly; ++f) load(f, s + 8 * f);
+      for (int f = 0; f < kFly; ++f) load(f, s + 8 * f);
+    }
     for (; s + 8 * kFly < full; s += 8 * kFly) {
 #pragma unroll
       for (int f = 0; f < kFly; ++f) {
-        multiply(f);
+        multiply(f, s + 8 * f);
         load(f, s + 8 * (f + kFly));
       }
     }
 #pragma unroll
     for (int f = 0; f < kFly; ++f)
-      if (s + 8 * f < full) multiply(f);
+      if (s + 8 * f < full) multiply(f, s + 8 * f);
   }
   if (wave == full % 8 && ld % 128) {  // the columns behind the last whole step: a multiple of 16
 #pragma unroll
@@ -328,10 +393,12 @@ __global__ __launch_bounds__(512, 2) void w8a8_few_kernel(W8A8 p) {
       const int k = 128 * full + 32 * h + 16 * q;
 #pragma unroll
       for (int i = 0; i < NT; ++i) wv[0][i][q] = k < ld ? *reinterpret_cast<const i32x4*>(wrow[i] + k) : zero;
+      if constexpr (!ROWS) {
 #pragma unroll
-      for (int j = 0; j < MT; ++j) xv[0][j][q] = k < ld ? *reinterpret_cast<const i32x4*>(xrow[j] + k) : zero;
+        for (int j = 0; j < MT; ++j) xv[0][j][q] = k < ld ? *reinterpret_cast<const i32x4*>(xrow[j] + k) : zero;
+      }
     }
-    multiply(0);
+    multiply(0, full);
   }
   __syncthreads();  // sums are cleared
   // result e of tile (i, j): weight row 16 i + 4 h + e, activation row 16 j + c; kept at 16 i + 4 e + h
@@ -355,12 +422,12 @@ __global__ __launch_bounds__(512, 2) void w8a8_few_kernel(W8A8 p) {
       sw[e] = n + e < N ? p.sw[n + e] : 0.f;
       bias[e] = p.bias && n + e < N ? (float)((const T*)p.bias)[n + e] : 0.f;
     }
-    store_row8((T*)p.y, v, sw, bias, p.sx[m], m, n, N, wide);
+    store_row8((T*)p.y, v, sw, bias, ROWS ? row_scale[m] : p.sx[m], m, n, N, wide);
   }
 }
 
-template <typename T, int MT>
-hipError_t few(const W8A8& p, hipStream_t stream) {
+template <typename T, int MT, bool ROWS = false>
+hipError_t few(const W8A8& p, hipStream_t stream, const W8A8Rows& rows = {}) {
   // More weight rows a workgroup read the activations less often (a quarter of them with 64), as
   // long as there are workgroups for the CUs. M x N x K, 16 / 32 / 64 weight rows (us with the
   // quantisation): 1 x 128256 x 4096 120 / 124 / 95, 8 x 14336 x 4096 22.8 / 23.4 / 19.4, 64 x 28672 x 4096
@@ -369,11 +436,11 @@ hipError_t few(const W8A8& p, hipStream_t stream) {
   const int64_t cus = device_cu_count();
   const dim3 block(512);
   if (p.N >= 48 * cus)
-    hipLaunchKernelGGL((w8a8_few_kernel<T, MT, 4>), dim3((unsigned)((p.N + 63) / 64)), block, 0, stream, p);
+    hipLaunchKernelGGL((w8a8_few_kernel<T, MT, 4, ROWS>), dim3((unsigned)((p.N + 63) / 64)), block, 0, stream, p, rows);
   else if (p.N >= 20 * cus)
-    hipLaunchKernelGGL((w8a8_few_kernel<T, MT, 2>), dim3((unsigned)((p.N + 31) / 32)), block, 0, stream, p);
+    hipLaunchKernelGGL((w8a8_few_kernel<T, MT, 2, ROWS>), dim3((unsigned)((p.N + 31) / 32)), block, 0, stream, p, rows);
   else
-    hipLaunchKernelGGL((w8a8_few_kernel<T, MT, 1>), dim3((unsigned)((p.N + 15) / 16)), block, 0, stream, p);
+    hipLaunchKernelGGL((w8a8_few_kernel<T, MT, 1, ROWS>), dim3((unsigned)((p.N + 15) / 16)), block, 0, stream, p, rows);
   return hipGetLastError();
 }
 
@@ -406,6 +473,27 @@ hipError_t launch_quantize_rows(const void* x, int x_dtype, int64_t x_ld, int8_t
     hipLaunchKernelGGL(quantize_rows_kernel<float>, grid, block, 0, stream, (const float*)x, x_ld, codes, scales,
                        (int)K, (int)ld, wide);
   return hipGetLastError();
+}
+
+hipError_t launch_w8a8_rows(const W8A8& p, const void* x, int64_t x_ld, int64_t K, hipStream_t stream) {
+  // One launch for up to 4 rows while a CU has at most one workgroup, which quantise them again
+  // (M x N x K in one launch / two, us, in a graph: 1 x 4096 x 4096 7.7 / 9.9, 4 x 4096 x 4096 10.0 /
+  // 10.5, 1 x 14336 x 4096 17.1 / 18.9, 1 x 4096 x 14336 19.9 / 19.2, 4 x 28672 x 4096 30.7 / 30.2,
+  // 1 x 128256 x 4096 107 / 97; a call from the host 5 us less), from 1024 columns on, so that every
+  // wave has a step to load, and unless y is written over the x that other workgroups still read.
+  const int size = p.dtype == 2 ? 4 : 2;
+  const uintptr_t x0 = (uintptr_t)x, x1 = x0 + ((p.M - 1) * x_ld + K) * size, y0 = (uintptr_t)p.y, y1 = y0 + p.M * p.N * size;
+  if (p.N <= 64 * (int64_t)device_cu_count() && p.M * ((p.ld + 4095) / 4096) <= kPieces && p.ld >= 1024 && (x1 <= y0 || y1 <= x0)) {
+    const W8A8Rows rows = {x, x_ld, (int)K, (uintptr_t)x % (8 * size) == 0 && x_ld % 8 == 0};
+    if (p.dtype == 0) return few<f16, 1, true>(p, stream, rows);
+    if (p.dtype == 1) return few<__bf16, 1, true>(p, stream, rows);
+    return few<float, 1, true>(p, stream, rows);
+  }
+  if (hipError_t e = launch_quantize_rows(x, p.dtype, x_ld, const_cast<int8_t*>(p.x), const_cast<float*>(p.sx), p.M, K,
+                                          p.ld, stream);
+      e != hipSuccess)
+    return e;
+  return launch_w8a8(p, stream);
 }
 
 hipError_t launch_w8a8(const W8A8& p, hipStream_t stream) {

@@ -33,12 +33,6 @@ def _rows(x: torch.Tensor, fn: str) -> torch.Tensor:
     return x
 
 
-def _quantize(x: torch.Tensor, codes: int, scales: int, stream: int) -> None:
-    M, K = x.shape
-    _lib.check(_lib.lib().pmi_quantize_rows(x.data_ptr(), _VALUES[x.dtype], max(x.stride(0), K), codes, scales, M, K,
-                                            stream), "pmi_quantize_rows")
-
-
 def quantize_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """(codes int8 [M, K rounded up to 16], scales fp32 [M]) of x [M, K] (fp16, bf16 or
     fp32): code = round(x * (127 / amax)), scale = amax / 127, amax the row's largest
@@ -49,7 +43,9 @@ def quantize_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     codes = torch.empty(M, _code_width(K), dtype=torch.int8, device=x.device)
     scales = torch.empty(M, dtype=torch.float32, device=x.device)
     with _DeviceGuard(x.device):
-        _quantize(x, codes.data_ptr(), scales.data_ptr(), _stream_handle(x.device))
+        _lib.check(_lib.lib().pmi_quantize_rows(x.data_ptr(), _VALUES[x.dtype], max(x.stride(0), K), codes.data_ptr(),
+                                                scales.data_ptr(), M, K, _stream_handle(x.device)),
+                   "pmi_quantize_rows")
     return codes, scales
 
 
@@ -79,13 +75,6 @@ def _bias_and_out(bias: torch.Tensor | None, out: torch.Tensor | None, M: int, N
     return bias, out
 
 
-def _product(codes: int, scales: int, w: torch.Tensor, w_scales: torch.Tensor, bias: torch.Tensor | None,
-             out: torch.Tensor, K: int, stream: int) -> None:
-    _lib.check(_lib.lib().pmi_matmul_w8a8(
-        codes, scales, w.data_ptr(), w_scales.data_ptr(), bias.data_ptr() if bias is not None else None,
-        out.data_ptr(), _VALUES[out.dtype], out.shape[0], out.shape[1], K, stream), "pmi_matmul_w8a8")
-
-
 def matmul_int8(codes: torch.Tensor, scales: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, K: int,
                 dtype: torch.dtype, *, bias: torch.Tensor | None = None,
                 out: torch.Tensor | None = None) -> torch.Tensor:
@@ -104,7 +93,10 @@ def matmul_int8(codes: torch.Tensor, scales: torch.Tensor, w: torch.Tensor, w_sc
     dev = codes.device
     bias, out = _bias_and_out(bias, out, M, N, dtype, dev)
     with _DeviceGuard(dev):
-        _product(codes.data_ptr(), scales.data_ptr(), w, w_scales, bias, out, K, _stream_handle(dev))
+        _lib.check(_lib.lib().pmi_matmul_w8a8(
+            codes.data_ptr(), scales.data_ptr(), w.data_ptr(), w_scales.data_ptr(),
+            bias.data_ptr() if bias is not None else None, out.data_ptr(), _VALUES[dtype], M, N, K,
+            _stream_handle(dev)), "pmi_matmul_w8a8")
     return out
 
 
@@ -119,13 +111,12 @@ def matmul_w8a8(x: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, *, bia
     dev = x.device
     N = _check_weight(x, w, w_scales, bias, K)
     bias, out = _bias_and_out(bias, out, M, N, x.dtype, dev)
-    codes = M * _code_width(K)
-    scratch = torch.empty(codes + 4 * M, dtype=torch.int8, device=dev)  # the codes, then the scales
-    at = scratch.data_ptr()
+    scratch = torch.empty(M * (_code_width(K) + 4), dtype=torch.int8, device=dev)
     with _DeviceGuard(dev):
-        stream = _stream_handle(dev)
-        _quantize(x, at, at + codes, stream)
-        _product(at, at + codes, w, w_scales, bias, out, K, stream)
+        _lib.check(_lib.lib().pmi_matmul_w8a8_rows(
+            x.data_ptr(), _VALUES[x.dtype], max(x.stride(0), K), w.data_ptr(), w_scales.data_ptr(),
+            bias.data_ptr() if bias is not None else None, out.data_ptr(), M, N, K, scratch.data_ptr(),
+            scratch.numel(), _stream_handle(dev)), "pmi_matmul_w8a8_rows")
     return out
 
 

@@ -35,6 +35,17 @@ def test_matmul_refuses(change):
     assert _lib.lib().pmi_matmul_w8a8(*a.values(), None) < 0 and "pmi_matmul_w8a8" in _lib.last_error()
 
 
+@pytest.mark.parametrize("change", [dict(dtype=_lib.PMI_I8), dict(stride=15), dict(stride=1 << 40), dict(M=-1),
+                                    dict(N=-1), dict(K=0), dict(K=131073), dict(x=None), dict(x=P8 + 1),
+                                    dict(w=P8 + 4), dict(sw=None), dict(y=None), dict(y=P8 + 1), dict(bias=P8 + 1),
+                                    dict(N=1 << 24), dict(scratch=None), dict(scratch=P8 + 4), dict(bytes=39)])
+def test_matmul_rows_refuses(change):
+    a = dict(x=P8, dtype=_lib.PMI_F16, stride=16, w=P8, sw=P8, bias=None, y=P8, M=2, N=3, K=16, scratch=P8, bytes=40)
+    a.update(change)
+    assert _lib.lib().pmi_matmul_w8a8_rows(*a.values(), None) < 0 and "pmi_matmul_w8a8_rows" in _lib.last_error()
+    assert _lib.lib().pmi_matmul_w8a8_scratch_bytes(2, 16) == 40
+
+
 def test_empty_calls_and_cpu_tensors():
     L = _lib.lib()
     assert L.pmi_quantize_rows(None, _lib.PMI_F16, 16, None, None, 0, 16, None) == _lib.PMI_OK
@@ -78,6 +89,38 @@ def test_quantize_rows_equals_the_oracle_bit_for_bit(dtype, M, K):
     assert torch.equal(again, codes) and torch.equal(s2, scales)
     turned = x.to(DEV).t().contiguous().t()
     assert torch.equal(P.quantize_rows(turned)[0], codes)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("M,N,K", [(1, 5000, 4096), (1, 20000, 2048), (1, 130, 16384), (1, 130, 16385), (2, 12500, 8190), (3, 77, 4090),
+                                   (4, 5200, 4096), (4, 300, 1024), (4, 300, 1009), (4, 300, 1000), (5, 300, 2048),
+                                   (1, 40, 12289)])
+def test_matmul_of_few_rows_is_the_two_calls(dtype, M, N, K):
+    """Rows quantised inside the product or before it: the same bits, also in place of x, from
+    strided and unaligned rows, and with rows of zeros, infinities and NaN."""
+    g = torch.Generator().manual_seed(M * N + K)
+    x = torch.randn(M, K + 3, generator=g).to(dtype).to(DEV)
+    w, sw = P.quantize_rows(torch.randn(N, K, generator=g).to(DEV))
+    bias = torch.randn(N, generator=g).to(dtype).to(DEV)
+
+    def check(x):
+        want = P.matmul_int8(*P.quantize_rows(x), w, sw, K, dtype, bias=bias)
+        got = P.matmul_w8a8(x, w, sw, bias=bias)
+        assert torch.equal(got.view(torch.uint8), want.view(torch.uint8))
+
+    for first in (0, 1, 3):
+        check(x[:, first:first + K])
+    x[0, 5] = float("inf")
+    x[-1, K - 1] = float("nan")
+    check(x[:, :K])
+    x[0] = 0
+    check(x[:, :K])
+    if N >= K:
+        square = P.quantize_rows(torch.randn(K, K, generator=g).to(DEV))
+        y = x[:, :K].contiguous()
+        want = P.matmul_w8a8(y.clone(), *square)
+        assert torch.equal(P.matmul_w8a8(y, *square, out=y).view(torch.uint8), want.view(torch.uint8))
 
 
 @gpu
