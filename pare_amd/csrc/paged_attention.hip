@@ -949,7 +949,8 @@ ManyPlan many_plan(const PagedAttention& p, const PagedCache& c) {
   // row tiles: every request's last one may be partly filled, and has more than kFewRows rows
   const int64_t most = p.T * G / (kFewRows + 1) < p.R ? p.T * G / (kFewRows + 1) : p.R;
   f.items = (p.T * G / kRows + most) * c.KV;
-  const int64_t range = p.window && p.window + p.max_q + 15 < p.max_kv ? p.window + p.max_q + 15 : p.max_kv;
+  // what a row tile sees: up to the window behind each of its queries, from a multiple of 16 on
+  const int64_t seen = p.window + (kRows + G - 2) / G + 15, range = p.window && seen < p.max_kv ? seen : p.max_kv;
   // two workgroups a CU; a range of at least eight tiles, as its join costs about two
   int64_t S = f.items > 0 ? 2 * device_cu_count() / f.items : 1;
   if (S > range / 512) S = range / 512;
