@@ -156,6 +156,16 @@ PMI_DEV float sum_over_h(float v) {
   return v + __shfl_xor(v, 32);
 }
 
+// The largest of each four neighbouring lanes.
+PMI_DEV float max_of_4(float v) {
+  const auto from = [](float x, auto ctrl) {
+    const int i = __builtin_bit_cast(int, x);
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(i, i, decltype(ctrl)::value, 0xf, 0xf, true));
+  };
+  v = fmaxf(v, from(v, std::integral_constant<int, 0xb1>{}));         // quad_perm 1, 0, 3, 2
+  return fmaxf(v, from(v, std::integral_constant<int, 0x4e>{}));      // quad_perm 2, 3, 0, 1
+}
+
 // (m, l, o) joined with another part of the same row; a part that saw no key is left out.
 PMI_DEV void join(float& m, float& l, f32x4& o, float pm, float pl, f32x4 po, bool use) {
   use = use && !(pm == -INFINITY && pl == 0.f);
@@ -672,34 +682,21 @@ __global__ __launch_bounds__(256, 2) void attention_rows_kernel(AttnArgs a) {
   const int32_t* table = a.tables + (int64_t)r * a.stride;
   const int64_t cell_bytes = (int64_t)a.ps * D;
 
-  // the four blocks of the tile at p: their pages (-1: not there) and scales
+  // The four blocks of the tile at p, block b in the lanes with l % 4 = b, so that their pages and
+  // scales are one instruction each (as scalars they were a sixth of the issued ones).
   struct Blocks {
-    int page[4];
-    float ks[4], vs[4];
-    bool bad;  // one of them is not finite
+    int page;  // -1: not there
+    float ks, vs;
   };
-  auto look_up = [&](int p, int* entry) {
-#pragma unroll
-    for (int b = 0; b < 4; ++b) entry[b] = table[min((p + 16 * b) >> a.ps_log, a.width - 1)];
+  const int lane_token = 16 * (l & 3);
+  auto look_up = [&](int p) { return table[min((p + lane_token) >> a.ps_log, a.width - 1)]; };
+  auto blocks_of = [&](int p, int entry) {
+    const bool there = p + lane_token < p1 && (unsigned)entry < a.n_pages;
+    const int64_t cell = (int64_t)(there ? entry : 0) * a.KV + kh;
+    return Blocks{there ? entry : -1, a.k_scale[cell], a.v_scale[cell]};
   };
-  auto blocks_of = [&](int p, const int* entry) {
-    Blocks x;
-    x.bad = false;
-#pragma unroll
-    for (int b = 0; b < 4; ++b) {
-      const bool there = p + 16 * b < p1 && (unsigned)entry[b] < a.n_pages;
-      x.page[b] = there ? entry[b] : -1;
-      const int64_t cell = (int64_t)(there ? entry[b] : 0) * a.KV + kh;
-      const float ks = a.k_scale[cell], vs = a.v_scale[cell];
-      x.ks[b] = there ? (ks < 1e-18f ? 1e-18f : ks) : 1e-18f;
-      x.vs[b] = there ? vs : 0.f;
-      x.bad |= !(x.ks[b] < INFINITY) || !(x.vs[b] < INFINITY);
-    }
-    return x;
-  };
-  auto pick = [](const int* v, int b) {
-    const int lo2 = b & 1 ? v[1] : v[0], hi2 = b & 1 ? v[3] : v[2];
-    return b & 2 ? hi2 : lo2;
+  auto of_block = [](float v, int b) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), b));
   };
   // A wave's 64 pieces of 16 bytes (piece tid + 256 k of the tile, token-major for K, dimension-major
   // in a block for V) are all of one block, so that addresses are the same but for a constant.
@@ -709,7 +706,7 @@ __global__ __launch_bounds__(256, 2) void attention_rows_kernel(AttnArgs a) {
 #pragma unroll
     for (int k = 0; k < KP; ++k) {
       const int idx = tid + 256 * k, b = block_of(k);
-      const int64_t cell = (int64_t)max(pick(x.page, b), 0) * a.KV + kh;
+      const int64_t cell = (int64_t)max(__builtin_amdgcn_readlane(x.page, b), 0) * a.KV + kh;
       const int tok = (p + 16 * b) & (a.ps - 1);
       const int64_t at = cell * cell_bytes + tok * D;  // of both: a block of v is 16 tokens of D bytes
       kw[k] = *reinterpret_cast<const u32x4*>(a.k + at + (uint32_t)(16 * (idx % D)));
@@ -722,7 +719,7 @@ __global__ __launch_bounds__(256, 2) void attention_rows_kernel(AttnArgs a) {
     uint8_t* kb = lds + slot * 2 * kSlot;
     uint8_t* vb = kb + kSlot;
     // codes of tokens that no row sees may be NaN (e4m3)
-    const bool edge = FP8 && (p < first_seen || p + 64 > p1 || (x.page[0] | x.page[1] | x.page[2] | x.page[3]) < 0);
+    const bool edge = FP8 && (p < first_seen || p + 64 > p1 || __any(x.page < 0));
 #pragma unroll
     for (int k = 0; k < KP; ++k) {
       const int idx = tid + 256 * k;
@@ -731,7 +728,8 @@ __global__ __launch_bounds__(256, 2) void attention_rows_kernel(AttnArgs a) {
       *reinterpret_cast<f16x8*>(kb + krow * D * 2 + (((2 * kpiece) ^ swizzle(krow)) << 4)) = k0;
       *reinterpret_cast<f16x8*>(kb + krow * D * 2 + (((2 * kpiece + 1) ^ swizzle(krow)) << 4)) = k1;
       const int vblk = block_of(k), vd = idx % D;
-      if (edge) vw[k] &= byte_mask(first_seen - p - 16 * vblk, pick(x.page, vblk) < 0 ? 0 : p1 - p - 16 * vblk);
+      if (edge) vw[k] &= byte_mask(first_seen - p - 16 * vblk,
+                                     __builtin_amdgcn_readlane(x.page, vblk) < 0 ? 0 : p1 - p - 16 * vblk);
       const f16x8 v0 = codes8<FP8>(vw[k][0], vw[k][1]), v1 = codes8<FP8>(vw[k][2], vw[k][3]);
       *reinterpret_cast<f16x8*>(vb + vd * 128 + (((2 * vblk) ^ ((vd >> 1) & 7)) << 4)) = v0;
       *reinterpret_cast<f16x8*>(vb + vd * 128 + (((2 * vblk + 1) ^ ((vd >> 1) & 7)) << 4)) = v1;
@@ -739,15 +737,12 @@ __global__ __launch_bounds__(256, 2) void attention_rows_kernel(AttnArgs a) {
   };
 
   if (p0 < p1) {
-    int entry[4];
-    look_up(p0, entry);
-    Blocks cur = blocks_of(p0, entry);
+    Blocks cur = blocks_of(p0, look_up(p0));
     load_tile(p0, cur);
-    look_up(p0 + 64, entry);
-    Blocks next = blocks_of(p0 + 64, entry);
+    Blocks next = blocks_of(p0 + 64, look_up(p0 + 64));
     store_tile(p0, cur, 0);
     load_tile(p0 + 64, next);
-    look_up(p0 + 128, entry);
+    int entry = look_up(p0 + 128);
     int slot = 0;
     for (int p = p0; p < p1; p += 64, slot ^= 1) {
       __syncthreads();  // the slot is written; the other one is read
@@ -755,28 +750,30 @@ __global__ __launch_bounds__(256, 2) void attention_rows_kernel(AttnArgs a) {
       store_tile(p + 64, next, slot ^ 1);
       const Blocks after = blocks_of(p + 128, entry);
       load_tile(p + 128, after);
-      look_up(p + 192, entry);
+      entry = look_up(p + 192);
       const uint8_t* kb = lds + slot * 2 * kSlot;
       const uint8_t* vb = kb + kSlot;
       __builtin_amdgcn_s_setprio(1);  // products ahead of the other wave's softmax
       f32x16 s[2];
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
+      for (int u = 0; u < 2; ++u)
 #pragma unroll
         for (int e = 0; e < 16; ++e) s[u][e] = 0.f;
-        const int krow = 32 * u + 16 * (c >> 4) + 8 * ((c >> 2) & 1) + 4 * ((c >> 3) & 1) + (c & 3);
 #pragma unroll
-        for (int x = 0; x < D / 16; ++x) {
+      for (int x = 0; x < D / 16; ++x)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int krow = 32 * u + 16 * (c >> 4) + 8 * ((c >> 2) & 1) + 4 * ((c >> 3) & 1) + (c & 3);
           const f16x8 k8 = *reinterpret_cast<const f16x8*>(kb + krow * D * 2 + (((2 * x + h) ^ swizzle(krow)) << 4));
           s[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k8, qv[x], s[u], 0, 0, 0);
         }
-      }
       __builtin_amdgcn_s_setprio(0);
+      const bool gone = cur.page < 0;
+      float ks = gone || cur.ks < 1e-18f ? 1e-18f : cur.ks, vs = gone ? 0.f : cur.vs;
+      const bool bad = !(ks < INFINITY) || !(vs < INFINITY);
       // the unit of acc: the largest value scale so far, or half of it
-      float top = vref;
-#pragma unroll
-      for (int b = 0; b < 4; ++b) top = fmaxf(top, cur.vs[b] < INFINITY ? cur.vs[b] : 0.f);
-      if (top > 2.f * vref) {
+      const float top = fmaxf(vref, max_of_4(vs < INFINITY ? vs : 0.f));
+      if (__any(top > 2.f * vref)) {
         const float f = vref / top;
 #pragma unroll
         for (int d = 0; d < D / 32; ++d) acc[d] *= f;
@@ -785,34 +782,37 @@ __global__ __launch_bounds__(256, 2) void attention_rows_kernel(AttnArgs a) {
       }
       // result 16 u + 4 j + e: token 32 u + 16 (j / 2) + 8 h + 4 (j % 2) + e, block 2 u + j / 2.
       // Hidden tokens get -inf, which stays one through the scales (at least 1e-18).
-      if (p < safe_lo || p + 64 > safe_hi || p + 64 > p1 || (cur.page[0] | cur.page[1] | cur.page[2] | cur.page[3]) < 0) {
+      if (p < safe_lo || p + 64 > safe_hi || p + 64 > p1 || __any(gone)) {
         const int from = lo - p - 8 * h, to = min(hi, p1) - p - 8 * h;
 #pragma unroll
         for (int y = 0; y < 32; ++y) {
           const int at = 16 * (y >> 3) + (y & 7);
-          s[y >> 4][y & 15] = at >= from && at < (cur.page[y >> 3] >= 0 ? to : 0) ? s[y >> 4][y & 15] : -INFINITY;
+          const int end = __builtin_amdgcn_readlane(cur.page, y >> 3) >= 0 ? to : 0;
+          s[y >> 4][y & 15] = at >= from && at < end ? s[y >> 4][y & 15] : -INFINITY;
         }
       }
-      if (cur.bad) {
+      if (const uint64_t which = __ballot(bad)) {
         // a page that holds an infinity or NaN: what sees it becomes NaN
+        if (bad) ks = 1e-18f, vs = 0.f;
 #pragma unroll
-        for (int b = 0; b < 4; ++b) {
-          if (cur.ks[b] < INFINITY && cur.vs[b] < INFINITY) continue;
-          cur.ks[b] = 1e-18f, cur.vs[b] = 0.f;
+        for (int b = 0; b < 4; ++b)
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
             const float t = s[b >> 1][8 * (b & 1) + e];
-            s[b >> 1][8 * (b & 1) + e] = t == -INFINITY ? t : __builtin_nanf("");
+            s[b >> 1][8 * (b & 1) + e] = t == -INFINITY || !(which >> b & 1) ? t : __builtin_nanf("");
           }
-        }
       }
+      const float vsv = vs * vinv;
+      float k1[4], v1[4];
+#pragma unroll
+      for (int b = 0; b < 4; ++b) k1[b] = of_block(ks, b) * qmul, v1[b] = of_block(vsv, b);
       float mx = -INFINITY;
 #pragma unroll
       for (int b = 0; b < 4; ++b) {
         float t = s[b >> 1][8 * (b & 1)];
 #pragma unroll
         for (int e = 1; e < 8; ++e) t = fmaxf(t, s[b >> 1][8 * (b & 1) + e]);
-        mx = fmaxf(mx, t * (cur.ks[b] * qmul));
+        mx = fmaxf(mx, t * k1[b]);
       }
       mx = fmaxf(mx, __shfl_xor(mx, 32));
       const float nm = fmaxf(m, mx);
@@ -826,13 +826,12 @@ __global__ __launch_bounds__(256, 2) void attention_rows_kernel(AttnArgs a) {
       const float base = m == -INFINITY ? 0.f : m;
 #pragma unroll
       for (int b = 0; b < 4; ++b) {
-        const float k1 = cur.ks[b] * qmul, vs = cur.vs[b] * vinv;
         f16x8 pw;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const float ex = __builtin_amdgcn_exp2f(fmaf(s[b >> 1][8 * (b & 1) + e], k1, -base));
+          const float ex = __builtin_amdgcn_exp2f(fmaf(s[b >> 1][8 * (b & 1) + e], k1[b], -base));
           sum += ex;
-          pw[e] = (f16)(ex * vs);
+          pw[e] = (f16)(ex * v1[b]);
         }
 #pragma unroll
         for (int d = 0; d < D / 32; ++d) {
