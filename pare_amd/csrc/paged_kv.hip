@@ -92,7 +92,8 @@ PMI_DEV void token_slot(const TablesArgs& a, int t, int r, int start, int first,
 }
 
 // One workgroup: the per-request sums and, for few tokens, the fresh pages and slots as
-// well. need_r = ceil((len + new) / ps) - ceil(len / ps); a request is granted where its
+// well. Bound by the chain of loads, two scans and the look-ups (128 requests of one token: 5 us,
+// 6.6 in a graph with its launch), not by its bytes; the sums are 64-bit. need_r = ceil((len + new) / ps) - ceil(len / ps); a request is granted where its
 // table row is wide enough and the sum of the needs up to it is within the pool, so the
 // granted ones that need pages are the first of them in order.
 // Everything is read before anything is written: kv_lens_out may be kv_lens,
@@ -459,6 +460,11 @@ PMI_DEV void append_run(const AppendArgs& a, int t0, int n, int slot, int kh, ui
   }
 }
 
+// Bound by the bytes of qkv and of the rotated q for many tokens (prompts of 6000 tokens, 28 / 4
+// heads of 128, bf16, pages of 32 of e4m3: 20 us for 105 MB), by the chain slots, values, maximum, codes for few (64 tokens, 32 / 8 heads,
+// pages of 64: 8 us). A run is read once: its keys wait for the maximum in registers, its
+// values in LDS, from where a thread takes the 16 tokens of one dimension (6000 tokens: 33 us with a
+// second read, a loop over the slots and the angles loaded for every head).
 // Grid: (cache_wgs + query workgroups, KV). The first take `chunk` tokens of one KV
 // head each and write the runs that begin among them; the others rotate the queries, a
 // thread the same dimensions of the KV head's whole group, with one load of their angles.
@@ -512,6 +518,10 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
 
 // ---- whole pages as values --------------------------------------------------------
 
+// One workgroup per page and head; a thread takes 16 codes of a key, or four dimensions of a
+// block of V, whose tokens are then four values a store (6.7 us with one dimension a thread, 6.0 so:
+// 188 pages of 32 tokens, 4 heads of 128, bf16, 19 MB with the codes). Bound by the launch and the
+// chain page, scale, codes, values, then by the bytes of the values.
 template <typename T, bool FP8>
 __global__ __launch_bounds__(256) void read_pages_kernel(const int32_t* __restrict__ pages,
                                                          const uint8_t* __restrict__ k_cache,
@@ -526,23 +536,38 @@ __global__ __launch_bounds__(256) void read_pages_kernel(const int32_t* __restri
   const int64_t out = (int64_t)blockIdx.x * ps * D;
   const float sk = ok ? k_scale[cell] : 0.f, sv = ok ? v_scale[cell] : 0.f;
   const int units = ps * D / 16;  // 16 codes
-  for (int u = threadIdx.x; u < 2 * units; u += 256) {
-    const bool value = u >= units;
-    const int w16 = value ? u - units : u;
-    u32x4 w = {0, 0, 0, 0};
-    if (ok) w = *reinterpret_cast<const u32x4*>((value ? v_cache : k_cache) + (cell * ps * D + 16 * (int64_t)w16));
-    float v[16];
+  const u32x4* k_codes = reinterpret_cast<const u32x4*>(k_cache + cell * ps * D);
+  const u32x4* v_codes = reinterpret_cast<const u32x4*>(v_cache + cell * ps * D);
+  const u32x4 none = {0, 0, 0, 0};
+  for (int u = threadIdx.x; u < units + units / 4; u += 256) {
+    if (u < units) {
+      const u32x4 w = ok ? k_codes[u] : none;
+      float v[16];
 #pragma unroll
-    for (int q = 0; q < 4; ++q) decode4<FP8>(w[q], v + 4 * q);
-    if (!value) {
+      for (int q = 0; q < 4; ++q) decode4<FP8>(w[q], v + 4 * q);
 #pragma unroll
       for (int e = 0; e < 16; ++e) v[e] = ok ? v[e] * sk : 0.f;
-      store8(k_out + out + 16 * w16, v);
-      store8(k_out + out + 16 * w16 + 8, v + 8);
-    } else {
-      const int b = w16 / D, d = w16 - b * D;
+      store8(k_out + out + 16 * u, v);
+      store8(k_out + out + 16 * u + 8, v + 8);
+      continue;
+    }
+    const int b = 4 * (u - units) / D, d = 4 * (u - units) - b * D;
+    u32x4 w[4];
 #pragma unroll
-      for (int e = 0; e < 16; ++e) v_out[out + (int64_t)(16 * b + e) * D + d] = (T)(ok ? v[e] * sv : 0.f);
+    for (int j = 0; j < 4; ++j) w[j] = ok ? v_codes[b * D + d + j] : none;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {  // four tokens of four dimensions
+      float v[4][4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) decode4<FP8>(w[j][q], v[j]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        typedef T T4 __attribute__((ext_vector_type(4)));
+        T4 y;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) y[j] = (T)(ok ? v[j][e] * sv : 0.f);
+        *reinterpret_cast<T4*>(v_out + out + (int64_t)(16 * b + 4 * q + e) * D + d) = y;
+      }
     }
   }
 }
