@@ -13,7 +13,7 @@ import torch
 import torch.nn as nn
 
 from . import _lib
-from .kernels import _DeviceGuard, _stream_handle
+from .kernels import _DeviceGuard, _raw_stream
 
 _VALUES = {torch.float16: _lib.PMI_F16, torch.bfloat16: _lib.PMI_BF16, torch.float32: _lib.PMI_F32}
 
@@ -44,7 +44,7 @@ def quantize_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     scales = torch.empty(M, dtype=torch.float32, device=x.device)
     with _DeviceGuard(x.device):
         _lib.check(_lib.lib().pmi_quantize_rows(x.data_ptr(), _VALUES[x.dtype], max(x.stride(0), K), codes.data_ptr(),
-                                                scales.data_ptr(), M, K, _stream_handle(x.device)),
+                                                scales.data_ptr(), M, K, _raw_stream(x.device)),
                    "pmi_quantize_rows")
     return codes, scales
 
@@ -96,7 +96,7 @@ def matmul_int8(codes: torch.Tensor, scales: torch.Tensor, w: torch.Tensor, w_sc
         _lib.check(_lib.lib().pmi_matmul_w8a8(
             codes.data_ptr(), scales.data_ptr(), w.data_ptr(), w_scales.data_ptr(),
             bias.data_ptr() if bias is not None else None, out.data_ptr(), _VALUES[dtype], M, N, K,
-            _stream_handle(dev)), "pmi_matmul_w8a8")
+            _raw_stream(dev)), "pmi_matmul_w8a8")
     return out
 
 
@@ -116,7 +116,7 @@ def matmul_w8a8(x: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, *, bia
         _lib.check(_lib.lib().pmi_matmul_w8a8_rows(
             x.data_ptr(), _VALUES[x.dtype], max(x.stride(0), K), w.data_ptr(), w_scales.data_ptr(),
             bias.data_ptr() if bias is not None else None, out.data_ptr(), M, N, K, scratch.data_ptr(),
-            scratch.numel(), _stream_handle(dev)), "pmi_matmul_w8a8_rows")
+            scratch.numel(), _raw_stream(dev)), "pmi_matmul_w8a8_rows")
     return out
 
 

@@ -25,9 +25,12 @@ from . import _lib
 
 
 def _stream_handle(device: torch.device) -> int:
-    # (without the Stream object of torch.cuda.current_stream: 0.2 us against 1.8 us a call)
-    index = torch.cuda.current_device() if device.index is None else device.index
-    return torch._C._cuda_getCurrentRawStream(index)
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+def _raw_stream(device: torch.device) -> int:
+    """``_stream_handle`` without the Stream object: 0.2 us against 1.8 us a call."""
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if device.index is None else device.index)
 
 
 class _DeviceGuard:

@@ -22,7 +22,7 @@ from typing import NamedTuple
 import torch
 
 from . import _lib
-from .kernels import _DeviceGuard, _stream_handle, _workspace
+from .kernels import _DeviceGuard, _raw_stream, _workspace
 
 _CODES = {torch.int8: _lib.PMI_I8, torch.float8_e4m3fn: _lib.PMI_F8}
 _VALUES = {torch.float16: _lib.PMI_F16, torch.bfloat16: _lib.PMI_BF16, torch.float32: _lib.PMI_F32}
@@ -122,7 +122,7 @@ def extend_block_tables(block_tables: torch.Tensor, kv_lens: torch.Tensor, new_l
             block_tables.data_ptr(), _row_stride(block_tables), kv_lens.data_ptr(), new_lens.data_ptr(),
             free_pages.data_ptr(), pool.data_ptr(), q_starts.data_ptr(), kv_lens_out.data_ptr(), first.data_ptr(),
             fresh.data_ptr(), positions.data_ptr(), slots.data_ptr(), pool_out.data_ptr(), R, block_tables.shape[1],
-            free_pages.numel(), page_size, total, _stream_handle(dev)), "pmi_extend_block_tables")
+            free_pages.numel(), page_size, total, _raw_stream(dev)), "pmi_extend_block_tables")
     return BatchPlan(q_starts, kv_lens_out, first, fresh, positions, slots, pool_out)
 
 
@@ -143,7 +143,7 @@ def release_block_tables(block_tables: torch.Tensor, kv_lens: torch.Tensor, done
         _lib.check(_lib.lib().pmi_release_block_tables(
             block_tables.data_ptr(), _row_stride(block_tables), kv_lens.data_ptr(), done.data_ptr(),
             free_pages.data_ptr(), pool.data_ptr(), R, block_tables.shape[1], free_pages.numel(), page_size,
-            _stream_handle(dev)), "pmi_release_block_tables")
+            _raw_stream(dev)), "pmi_release_block_tables")
 
 
 def rope_append_kv(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, positions: torch.Tensor,
@@ -178,7 +178,7 @@ def rope_append_kv(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, posi
             qkv.data_ptr(), _VALUES[qkv.dtype], max(qkv.stride(0), width), cos.data_ptr(), sin.data_ptr(),
             cos.shape[0], positions.data_ptr(), slots.data_ptr(), q.data_ptr(), k_cache.data_ptr(),
             v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), code, pages, ps, T, H, KV, D,
-            _stream_handle(dev)), "pmi_rope_append_kv")
+            _raw_stream(dev)), "pmi_rope_append_kv")
     return q
 
 
@@ -195,7 +195,7 @@ def read_kv_pages(pages: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
     with _DeviceGuard(dev):
         _lib.check(_lib.lib().pmi_read_kv_pages(
             pages.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), code,
-            n_pages, ps, k.data_ptr(), v.data_ptr(), _VALUES[dtype], pages.numel(), KV, D, _stream_handle(dev)),
+            n_pages, ps, k.data_ptr(), v.data_ptr(), _VALUES[dtype], pages.numel(), KV, D, _raw_stream(dev)),
             "pmi_read_kv_pages")
     return k, v
 
@@ -241,7 +241,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     assert max_kv >= 0, "max_kv_len may not be negative"
     L = _lib.lib()
     with _DeviceGuard(dev):
-        stream = _stream_handle(dev)
+        stream = _raw_stream(dev)
         max_q = min(max_q_len, T)
         nbytes = L.pmi_paged_attention_workspace_bytes(T, R, H, KV, D, max_q, max_kv, window)
         ws = _workspace(dev, stream, nbytes)
