@@ -210,6 +210,14 @@ constexpr float kPBias = 256.f, kSlack = 6.f, kLeastUnit = 1e-30f;
 // it ends in (record 2 w + 1), and only the latter can begin in it, so the
 // workgroup in which an item begins lends it its counter.
 constexpr int kMinShare = 4;  // tiles per workgroup, at least
+// Few tiles: items are cut every so many tiles instead, a part a workgroup, so that none has parts
+// of two. The smallest cut whose parts are at most half the workgroups is taken with heads of 128,
+// or else at most all of them: one workgroup a CU, whose waves have some tiles each, beats two of
+// half the tiles and twice the parts to join (8 requests of 4000 keys, 8 KV heads: 18.3 us, 19.6 with
+// two a CU, 22.3 dealt evenly; 1 of 32000: 21.2, dealt evenly 26.7; 24 of 1000: 15.4 and 20.3; with
+// heads of 64 a half as many took 14.5 us instead of 13.3).
+constexpr int kCuts = 6;
+constexpr int cut_of(int k) { return k < 4 ? 4 * (k + 1) : k == 4 ? 24 : 32; }
 
 template <typename T, int D, bool FP8>
 __global__ __launch_bounds__(256, 2) void attention_few_kernel(AttnArgs a) {
@@ -226,13 +234,14 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(AttnArgs a) {
   // (The host sees to it that the sum is below 2^31.)
   auto tiles_of = [&](const Request& rq) { return max(1, (rq.hi - rq.lo + 63) >> 6); };
   auto items_of = [&](const Request& rq) { return rq.n * G > a.few_rows ? 0 : (rq.n * G + 15) / 16 * a.KV; };
-  auto up = [](int nt) { return (nt + kMinShare - 1) / kMinShare * kMinShare; };
   const int run = (a.R + 63) >> 6, r_lane = run * l;
-  int in_lane = 0, in_lane_up = 0;
+  int in_lane = 0, parts_lane[kCuts] = {};  // tiles, and parts of cut_of(k) tiles
   for (int x = r_lane; x < min(a.R, r_lane + run); ++x) {
     const Request rq = request(a, x);
-    in_lane += tiles_of(rq) * items_of(rq);
-    in_lane_up += up(tiles_of(rq)) * items_of(rq);
+    const int nt = tiles_of(rq), items = items_of(rq);
+    in_lane += nt * items;
+#pragma unroll
+    for (int k = 0; k < kCuts; ++k) parts_lane[k] += (nt + cut_of(k) - 1) / cut_of(k) * items;
   }
   auto scan = [&](int v) {
 #pragma unroll
@@ -242,13 +251,32 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(AttnArgs a) {
     }
     return v;
   };
-  // Few tiles: items are cut every kMinShare tiles, so that no workgroup has parts of two.
-  int upto = scan(in_lane_up);
-  const bool cut = __builtin_amdgcn_readlane(upto, 63) <= kMinShare * (int)gridDim.x;
-  if (!cut) upto = scan(in_lane);
-  in_lane = cut ? in_lane_up : in_lane;
+  constexpr int kHalf = D == 128 ? 1 : 0;
+  // (a call of few tiles takes the first cut, and no other chain of shuffles than its scan)
+  int cut = cut_of(0), upto = scan(cut * parts_lane[0]);
+  if (__builtin_amdgcn_readlane(upto, 63) > cut * (int)(gridDim.x >> kHalf)) {
+    // the parts of all, two counts a word (a lane's 1023, or more, are too many)
+    uint32_t parts_all[kCuts / 2];
+#pragma unroll
+    for (int j = 0; j < kCuts / 2; ++j) {
+      parts_all[j] = (uint32_t)min(parts_lane[2 * j], 1023) | (uint32_t)min(parts_lane[2 * j + 1], 1023) << 16;
+#pragma unroll
+      for (int o = 32; o > 0; o >>= 1) parts_all[j] += __shfl_xor(parts_all[j], o);
+      parts_all[j] = __builtin_amdgcn_readfirstlane(parts_all[j]);
+    }
+    cut = 0;
+#pragma unroll
+    for (int half = kHalf; half >= 0; --half)
+#pragma unroll
+      for (int k = 0; k < kCuts; ++k)
+        if (!cut && (parts_all[k / 2] >> (16 * (k & 1)) & 0xffff) <= min(gridDim.x >> half, 1022u))
+          cut = cut_of(k), in_lane = cut_of(k) * parts_lane[k];
+    upto = scan(in_lane);
+  } else {
+    in_lane = cut * parts_lane[0];
+  }
   const int total = __builtin_amdgcn_readlane(upto, 63);
-  const int share = max(kMinShare, (int)(((uint32_t)total + gridDim.x - 1) / gridDim.x));
+  const int share = cut ? cut : max(kMinShare, (int)(((uint32_t)total + gridDim.x - 1) / gridDim.x));
   if ((int64_t)share * blockIdx.x >= total) return;
   int g = share * blockIdx.x;
   const int g_end = min((int64_t)g + share, (int64_t)total);
@@ -258,7 +286,7 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(AttnArgs a) {
   while (g < g_end && r < a.R) {
   const Request rq = request(a, r);
   const int row_tiles = (rq.n * G + 15) / 16, nt = tiles_of(rq);
-  const int span = cut ? up(nt) : nt;  // what an item takes of the order
+  const int span = cut ? (nt + cut - 1) / cut * cut : nt;  // what an item takes of the order
   const int all = span * items_of(rq);
   if (off >= all) {
     off -= all, ++r;

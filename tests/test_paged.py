@@ -420,6 +420,32 @@ def test_decode_attention_of_long_contexts(lens):
 
 
 @gpu
+@pytest.mark.parametrize("KV,D,lens", [(64, 64, [40000]), (64, 64, [33000]), (64, 64, [3000, 200, 9000]), (32, 128, [16000]),
+                                       (16, 128, [64, 65, 4000] * 4), (2, 128, [8200] * 7), (1, 64, [70000, 1]),
+                                       (8, 128, [500] * 130), (2, 64, [129] * 1100), (16, 128, [9000])])
+def test_decode_attention_at_every_cut(KV, D, lens):
+    """Numbers of tiles on both sides of every way to deal them out (pages used many times)."""
+    rng = np.random.default_rng(len(lens) * KV)
+    c = S.Cache(5, KV, 256, D, CODES[0])
+    c.fill(rng)
+    tables = rng.integers(0, 5, (len(lens), -(-max(lens) // 256))).astype(np.int32)
+    starts = np.arange(len(lens) + 1).astype(np.int32)
+    q = torch.from_numpy(rng.standard_normal((len(lens), KV, D))).half()
+    few = sorted({0, 1, len(lens) // 2, len(lens) - 1} & set(range(len(lens))))  # (the oracle is slow)
+    got = _run(c, tables, lens, starts, q)
+    want = _oracle(c, tables[few], [lens[i] for i in few], np.arange(len(few) + 1), q[few])
+    _check(got[few], *want, torch.float16)
+    again = _run(c, tables, lens, starts, q)
+    assert torch.equal(got, again)
+    # the requests that the oracle skipped: the same keys one by one
+    for i in range(0, len(lens), max(1, len(lens) // 8)):
+        alone = _run(c, tables[i:i + 1], lens[i:i + 1], starts[:2], q[i:i + 1])
+        err = (got[i].double() - alone[0].double()).abs().cpu().numpy()
+        weight = np.abs(c.values(1)).max()
+        assert (err <= 2 * _tolerance(alone[0].double().cpu().numpy(), weight, torch.float16)).all()
+
+
+@gpu
 @pytest.mark.parametrize("window", [1, 16, 63, 64, 65, 300, 5000])
 def test_windows(window):
     lens = [1, 64, 130, 700, 0, 2000]
