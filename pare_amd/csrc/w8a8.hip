@@ -8,8 +8,9 @@
 // products nor a split of K changes a bit; the scales are applied in fp32 and y is
 // rounded once. The reference only simulates this (its quantize_inputs path rounds the
 // activations and multiplies in floating point, pare/layers/linear.py:120-138).
-#include <cfloat>
+#include <algorithm>
 #include <atomic>
+#include <cfloat>
 
 #include "pmi_common.h"
 #include "pmi_launch.h"
@@ -134,13 +135,16 @@ PMI_DEV void store_row8(T* __restrict__ y, const int* sums, const float* sw, con
 // meet in one. Products
 // 32x32x32: the weights are the rows of the result, so that a wave reads (BN / WN + BM / WM) x
 // 32 bytes for BN / WN x BM / WM / 1024 of them. Columns past ld and rows past the end are copied
-// as zeros (from past the descriptor's end). The sums go through LDS, 32 activation rows at a
-// time, to be written 16 bytes a lane.
+// as zeros (from past the descriptor's end). The sums go through LDS (the second slot), 32
+// activation rows at a time, to be written 16 bytes a lane. A workgroup stays for several tiles: the
+// next one's first copies fly into the first slot meanwhile (4099 x 28672 x 4096: 490 us, a workgroup a
+// tile 515; 4096 rows 453 and 473; 2000 x 6144 x 4096 65.5 and 68.3).
 //
-// What bounds it (4099 x 28672 x 4096, 500 us with 13 of quantisation, 1.9e15 operations a second): the
-// products alone take about 290 us, the copies hold them up by some 120 and the stores of y, which
-// nothing overlaps as one workgroup fills a CU's LDS, by 70 (measured with each left out). Four
-// slots of 64 columns, three steps ahead: 545 us, twice the requests to L2 for half a line each.
+// What bounds it (4099 x 28672 x 4096 with 13 us of quantisation, 1.96e15 operations a second, 2.12e15 with
+// 4096 rows, which fill their tiles): the products alone take about 290 us, the copies hold them up
+// by some 120, the stores of y by 70 before they met the next tile's copies (measured with each
+// left out). Four slots of 64 columns, three steps ahead: 545 us, twice the requests to L2 for
+// half a line each.
 template <typename T, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(64 * WM * WN) void w8a8_tiles_kernel(W8A8 p, int grid_m, int grid_n, int chunk) {
   constexpr int NW = WM * WN, TM = BM / WM / 32, TN = BN / WN / 32;
@@ -149,17 +153,24 @@ __global__ __launch_bounds__(64 * WM * WN) void w8a8_tiles_kernel(W8A8 p, int gr
   const int tid = threadIdx.x, l = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave % WM, wn = wave / WM;
   const int c = l & 31, h = l >> 5;
-  // Workgroup 8 k + x runs on XCD x and takes tile x chunk + k of the list: blocks of eight tiles of
-  // activation rows, columns of weights inside, so that an XCD's tiles share rows of both.
-  const int tile = (blockIdx.x % 8) * chunk + blockIdx.x / 8;
-  if ((int)blockIdx.x / 8 >= chunk || tile >= grid_m * grid_n) return;
-  const int band = tile / (8 * grid_n), in_band = tile - band * 8 * grid_n;
-  const int band_rows = min(8, grid_m - 8 * band);
-  const int m0 = (8 * band + in_band % band_rows) * BM, n0 = in_band / band_rows * BN;
+  // Workgroup 8 k + x runs on XCD x and takes tiles x chunk + k, + gridDim / 8 and so on of the list:
+  // blocks of eight tiles of activation rows, columns of weights inside, so that an XCD's tiles share
+  // rows of both.
+  const int tiles = min(chunk, grid_m * grid_n - (int)(blockIdx.x % 8) * chunk);  // of this XCD
   const int M = (int)p.M, N = (int)p.N, ld = (int)p.ld;
-  const int rows_m = min(BM, M - m0), rows_n = min(BN, N - n0);
-  const u32x4 dx = descriptor(p.x + (int64_t)m0 * ld, (uint32_t)rows_m * ld);
-  const u32x4 dw = descriptor(p.w + (int64_t)n0 * ld, (uint32_t)rows_n * ld);
+  int m0, n0;
+  u32x4 dx, dw;
+  auto find = [&](int k) {
+    const int tile = (blockIdx.x % 8) * chunk + k;
+    const int band = tile / (8 * grid_n), in_band = tile - band * 8 * grid_n;
+    const int band_rows = min(8, grid_m - 8 * band);
+    m0 = (8 * band + in_band % band_rows) * BM, n0 = in_band / band_rows * BN;
+    dx = descriptor(p.x + (int64_t)m0 * ld, (uint32_t)min(BM, M - m0) * ld);
+    dw = descriptor(p.w + (int64_t)n0 * ld, (uint32_t)min(BN, N - n0) * ld);
+  };
+  int mine = blockIdx.x / 8;
+  if (mine >= tiles) return;
+  find(mine);
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
 
   // a copy: eight rows of 128 bytes, from row 8 (wave + NW i) on (NW is even)
@@ -178,79 +189,96 @@ __global__ __launch_bounds__(64 * WM * WN) void w8a8_tiles_kernel(W8A8 p, int gr
       dma16(dx, to + BN * 128 + i * NW * 1024, out ? 0x7ffffff0 : at_row[i], 128 * kt);
   };
 
-  i32x16 acc[TN][TM];
-#pragma unroll
-  for (int i = 0; i < TN; ++i)
-#pragma unroll
-    for (int j = 0; j < TM; ++j)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) acc[i][j][e] = 0;
-
   const int steps = (ld + 127) / 128;
-  copy(0, 0);
-  for (int kt = 0; kt < steps; ++kt) {
-    wait_vmcnt_lgkm0<0>();  // this wave's copies have arrived, its reads of the other slot are done
-    barrier_only();
-    const int slot = kt & 1;
-    if (kt + 1 < steps) copy(kt + 1, slot ^ 1);
-    const uint8_t* wb = lds + slot * kSlot + (wn * (BN / WN) + c) * 128;
-    const uint8_t* xb = lds + slot * kSlot + BN * 128 + (wm * (BM / WM) + c) * 128;
-#pragma unroll
-    for (int ks = 0; ks < 4; ++ks) {
-      const int at = 16 * ((2 * ks + h) ^ ((c >> 1) & 7));
-      i32x4 wv[TN], xv[TM];
-#pragma unroll
-      for (int i = 0; i < TN; ++i) wv[i] = *reinterpret_cast<const i32x4*>(wb + 32 * 128 * i + at);
-#pragma unroll
-      for (int j = 0; j < TM; ++j) xv[j] = *reinterpret_cast<const i32x4*>(xb + 32 * 128 * j + at);
-#pragma unroll
-      for (int i = 0; i < TN; ++i)
-#pragma unroll
-        for (int j = 0; j < TM; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(wv[i], xv[j], acc[i][j], 0, 0, 0);
-    }
-  }
-  wait_lgkm0();
-  barrier_only();  // every wave has read the last step: the slots are free
-
-  // result 4 e + f of tile (i, j): weight row 32 i + 8 e + 4 h + f, activation row 32 j + c
   constexpr int kRow = BN / WN + 4;  // words of a row of sums, rows 16 bytes apart in the banks
   constexpr int kLanes = BN / WN / 8, kStep = 64 / kLanes;  // lanes a row, rows a step
-  int* buf = reinterpret_cast<int*>(lds) + wave * 32 * kRow;
-  const int n = n0 + wn * (BN / WN) + 8 * (l % kLanes);
-  float sw[8], bias[8];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    sw[e] = n + e < N ? p.sw[n + e] : 0.f;
-    bias[e] = p.bias && n + e < N ? (float)((const T*)p.bias)[n + e] : 0.f;
-  }
+  int* buf = reinterpret_cast<int*>(lds + kSlot) + wave * 32 * kRow;
   const bool wide = N % 8 == 0 && (uintptr_t)p.y % (8 * sizeof(T)) == 0;
+  copy(0, 0);
+  while (true) {
+    // the tile's scales, before any product: the loads of the end would wait for the next tile's copies
+    const int n = n0 + wn * (BN / WN) + 8 * (l % kLanes), m_first = m0 + wm * (BM / WM) + l / kLanes;
+    float sw[8], bias[8], sx[TM * 32 / kStep];
 #pragma unroll
-  for (int j = 0; j < TM; ++j) {
+    for (int e = 0; e < 8; ++e) {
+      sw[e] = n + e < N ? p.sw[n + e] : 0.f;
+      bias[e] = p.bias && n + e < N ? (float)((const T*)p.bias)[n + e] : 0.f;
+    }
+#pragma unroll
+    for (int r = 0; r < TM * 32 / kStep; ++r) sx[r] = p.sx[min(m_first + kStep * r, M - 1)];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) asm volatile("" : "+v"(sw[e]), "+v"(bias[e]));
+#pragma unroll
+    for (int r = 0; r < TM * 32 / kStep; ++r) asm volatile("" : "+v"(sx[r]));
+
+    i32x16 acc[TN][TM];
 #pragma unroll
     for (int i = 0; i < TN; ++i)
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        *reinterpret_cast<i32x4*>(buf + c * kRow + 32 * i + 8 * e + 4 * h) =
-            i32x4{acc[i][j][4 * e], acc[i][j][4 * e + 1], acc[i][j][4 * e + 2], acc[i][j][4 * e + 3]};
-    // (one wave's own rows: ordered by its LDS counter alone)
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      for (int j = 0; j < TM; ++j)
 #pragma unroll
-    for (int s = 0; s < 32; s += kStep) {
-      const int r = s + l / kLanes, m = m0 + wm * (BM / WM) + 32 * j + r;
-      const int* at = buf + r * kRow + 8 * (l % kLanes);
-      int sums[8];
+        for (int e = 0; e < 16; ++e) acc[i][j][e] = 0;
+    for (int kt = 0; kt < steps; ++kt) {
+      wait_vmcnt_lgkm0<0>();  // this wave's copies have arrived, its reads of the other slot are done
+      barrier_only();
+      const int slot = kt & 1;
+      if (kt + 1 < steps) copy(kt + 1, slot ^ 1);
+      const uint8_t* wb = lds + slot * kSlot + (wn * (BN / WN) + c) * 128;
+      const uint8_t* xb = lds + slot * kSlot + BN * 128 + (wm * (BM / WM) + c) * 128;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) sums[e] = at[e];
-      if (m < M && n < N) store_row8((T*)p.y, sums, sw, bias, p.sx[m], m, n, N, wide);
+      for (int ks = 0; ks < 4; ++ks) {
+        const int at = 16 * ((2 * ks + h) ^ ((c >> 1) & 7));
+        i32x4 wv[TN], xv[TM];
+#pragma unroll
+        for (int i = 0; i < TN; ++i) wv[i] = *reinterpret_cast<const i32x4*>(wb + 32 * 128 * i + at);
+#pragma unroll
+        for (int j = 0; j < TM; ++j) xv[j] = *reinterpret_cast<const i32x4*>(xb + 32 * 128 * j + at);
+#pragma unroll
+        for (int i = 0; i < TN; ++i)
+#pragma unroll
+          for (int j = 0; j < TM; ++j)
+            acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(wv[i], xv[j], acc[i][j], 0, 0, 0);
+      }
     }
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    wait_lgkm0();
+    barrier_only();  // every wave has read the last step: the slots are free
+    // the next tile's first copies, to the first slot, while this one's sums go through the second
+    mine += gridDim.x / 8;
+    const bool more = mine < tiles;
+    if (more) {
+      find(mine);
+      copy(0, 0);
+    }
+
+    // result 4 e + f of tile (i, j): weight row 32 i + 8 e + 4 h + f, activation row 32 j + c
+#pragma unroll
+    for (int j = 0; j < TM; ++j) {
+#pragma unroll
+      for (int i = 0; i < TN; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          *reinterpret_cast<i32x4*>(buf + c * kRow + 32 * i + 8 * e + 4 * h) =
+              i32x4{acc[i][j][4 * e], acc[i][j][4 * e + 1], acc[i][j][4 * e + 2], acc[i][j][4 * e + 3]};
+      // (one wave's own rows: ordered by its LDS counter alone)
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+      for (int s = 0; s < 32; s += kStep) {
+        const int m = m_first + 32 * j + s;
+        const i32x4* at = reinterpret_cast<const i32x4*>(buf + (s + l / kLanes) * kRow + 8 * (l % kLanes));
+        const i32x4 lo = at[0], hi = at[1];
+        const int sums[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+        if (m < M && n < N) store_row8((T*)p.y, sums, sw, bias, sx[(32 * j + s) / kStep], m, n, N, wide);
+      }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    }
+    if (!more) return;
   }
 }
 
 template <typename T, int BM, int BN, int WM, int WN>
 hipError_t tiles(const W8A8& p, hipStream_t stream) {
-  constexpr int kWaves = WM * WN, kOut = kWaves * 32 * (BN / WN + 4) * 4, kIn = 2 * (BM + BN) * 128;
-  constexpr int kLds = kOut > kIn ? kOut : kIn;
+  constexpr int kWaves = WM * WN, kOut = kWaves * 32 * (BN / WN + 4) * 4, kSlot = (BM + BN) * 128;
+  constexpr int kLds = kSlot + (kOut > kSlot ? kOut : kSlot), kPerCu = 160 * 1024 / kLds;
   static_assert(kLds <= 160 * 1024, "LDS of a CU");
   static std::atomic<uint64_t> allowed{0};
   int dev = 0;
@@ -264,8 +292,9 @@ hipError_t tiles(const W8A8& p, hipStream_t stream) {
   }
   const int gm = (int)((p.M + BM - 1) / BM), gn = (int)((p.N + BN - 1) / BN);
   const int chunk = (int)(((int64_t)gm * gn + 7) / 8);
-  hipLaunchKernelGGL((w8a8_tiles_kernel<T, BM, BN, WM, WN>), dim3((unsigned)chunk * 8), dim3(64 * kWaves), kLds, stream, p,
-                     gm, gn, chunk);
+  const int per_xcd = device_cu_count() * kPerCu / 8;  // workgroups that the CUs hold
+  hipLaunchKernelGGL((w8a8_tiles_kernel<T, BM, BN, WM, WN>), dim3((unsigned)std::min(chunk, std::max(per_xcd, 1)) * 8),
+                     dim3(64 * kWaves), kLds, stream, p, gm, gn, chunk);
   return hipGetLastError();
 }
 
