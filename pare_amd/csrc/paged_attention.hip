@@ -29,8 +29,9 @@ struct AttnArgs {
   int max_q, max_kv;
   int splits, per;  // many rows: ranges of keys, and tokens in one
   int few_rows;   // requests of up to so many query rows (tokens x heads of a KV head) are `few`
-  int* counters;  // one per workgroup
-  float* part;
+  int few_wgs;    // workgroups of the few-row part
+  int* counters;  // one of each of them, and behind them one of each item of many rows
+  float *few_part, *many_part;
 };
 
 // What a request's queries see, from its row of kv_lens and q_starts.
@@ -219,12 +220,21 @@ constexpr int kMinShare = 4;  // tiles per workgroup, at least
 constexpr int kCuts = 6;
 constexpr int cut_of(int k) { return k < 4 ? 4 * (k + 1) : k == 4 ? 24 : 32; }
 
+template <int D>
+struct FewLds {
+  float acc[4][16][D + 4];  // rows 16 bytes apart in the banks
+  float m[4][16], l[4][16];
+  int last;
+};
+
 template <typename T, int D, bool FP8>
-__global__ __launch_bounds__(256, 2) void attention_few_kernel(AttnArgs a) {
+PMI_DEV void few_rows(const AttnArgs& a, FewLds<D>& lds, int wg) {
   constexpr int DT = D / 16;  // 16-dimension tiles of the output
-  __shared__ __attribute__((aligned(16))) float s_acc[4][16][D + 4];  // rows 16 bytes apart in the banks
-  __shared__ float s_m[4][16], s_l[4][16];
-  __shared__ int s_last;
+  float(&s_acc)[4][16][D + 4] = lds.acc;
+  float(&s_m)[4][16] = lds.m;
+  float(&s_l)[4][16] = lds.l;
+  int& s_last = lds.last;
+  const int wgs = a.few_wgs;
   const int tid = threadIdx.x, l = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c = l & 15, h = l >> 4;
   const int G = a.H / a.KV;
@@ -254,7 +264,7 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(AttnArgs a) {
   constexpr int kHalf = D == 128 ? 1 : 0;
   // (a call of few tiles takes the first cut, and no other chain of shuffles than its scan)
   int cut = cut_of(0), upto = scan(cut * parts_lane[0]);
-  if (__builtin_amdgcn_readlane(upto, 63) > cut * (int)(gridDim.x >> kHalf)) {
+  if (__builtin_amdgcn_readlane(upto, 63) > cut * (wgs >> kHalf)) {
     // the parts of all, two counts a word (a lane's 1023, or more, are too many)
     uint32_t parts_all[kCuts / 2];
 #pragma unroll
@@ -269,16 +279,16 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(AttnArgs a) {
     for (int half = kHalf; half >= 0; --half)
 #pragma unroll
       for (int k = 0; k < kCuts; ++k)
-        if (!cut && (parts_all[k / 2] >> (16 * (k & 1)) & 0xffff) <= min(gridDim.x >> half, 1022u))
+        if (!cut && (parts_all[k / 2] >> (16 * (k & 1)) & 0xffff) <= (uint32_t)min(wgs >> half, 1022))
           cut = cut_of(k), in_lane = cut_of(k) * parts_lane[k];
     upto = scan(in_lane);
   } else {
     in_lane = cut * parts_lane[0];
   }
   const int total = __builtin_amdgcn_readlane(upto, 63);
-  const int share = cut ? cut : max(kMinShare, (int)(((uint32_t)total + gridDim.x - 1) / gridDim.x));
-  if ((int64_t)share * blockIdx.x >= total) return;
-  int g = share * blockIdx.x;
+  const int share = cut ? cut : max(kMinShare, (int)(((uint32_t)total + wgs - 1) / wgs));
+  if ((int64_t)share * wg >= total) return;
+  int g = share * wg;
   const int g_end = min((int64_t)g + share, (int64_t)total);
   const int lane0 = __builtin_ctzll(__ballot(upto > g));
   int r = run * lane0;
@@ -495,10 +505,10 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(AttnArgs a) {
   // (sc1).
   constexpr int kSc1 = 16, kRec = D + 4;  // floats of a row: values, max, sum
   const int first_wg = item_g / share, parts = (item_g + nt - 1) / share - first_wg + 1;
-  const __amdgpu_buffer_rsrc_t rp = rsrc(a.part + (int64_t)first_wg * 32 * kRec, (int64_t)parts * 32 * kRec * 4);
+  const __amdgpu_buffer_rsrc_t rp = rsrc(a.few_part + (int64_t)first_wg * 32 * kRec, (int64_t)parts * 32 * kRec * 4);
   // record of part s: the first one's second, the others' first
   auto record = [&](int s, int rr) { return ((s ? 2 * s : 1) * 16 + rr) * kRec * 4; };
-  const int rec = record((int)blockIdx.x - first_wg, orow);
+  const int rec = record(wg - first_wg, orow);
   if (mine) {
 #pragma unroll
     for (int x = 0; x < kPer; x += 4)
@@ -589,12 +599,18 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(AttnArgs a) {
   }
 }
 
+template <typename T, int D, bool FP8>
+__global__ __launch_bounds__(256, 2) void attention_few_kernel(AttnArgs a) {
+  __shared__ __attribute__((aligned(16))) FewLds<D> lds;
+  few_rows<T, D, FP8>(a, lds, blockIdx.x);
+}
+
 template <typename T, int D>
-hipError_t few(const AttnArgs& a, bool fp8, int wgs, hipStream_t stream) {
+hipError_t few(const AttnArgs& a, bool fp8, hipStream_t stream) {
   if (fp8)
-    hipLaunchKernelGGL((attention_few_kernel<T, D, true>), dim3(wgs), dim3(256), 0, stream, a);
+    hipLaunchKernelGGL((attention_few_kernel<T, D, true>), dim3(a.few_wgs), dim3(256), 0, stream, a);
   else
-    hipLaunchKernelGGL((attention_few_kernel<T, D, false>), dim3(wgs), dim3(256), 0, stream, a);
+    hipLaunchKernelGGL((attention_few_kernel<T, D, false>), dim3(a.few_wgs), dim3(256), 0, stream, a);
   return hipGetLastError();
 }
 
@@ -620,11 +636,9 @@ hipError_t few(const AttnArgs& a, bool fp8, int wgs, hipStream_t stream) {
 constexpr int kRows = 128;
 
 template <typename T, int D, bool FP8>
-__global__ __launch_bounds__(256, 2) void attention_rows_kernel(AttnArgs a) {
+PMI_DEV void many_rows(const AttnArgs& a, uint8_t* lds, int& s_last, int wg) {
   constexpr int KP = D / 64;       // 16-byte pieces of K, and of V, per thread and tile
   constexpr int kSlot = 64 * D * 2;  // bytes of K (or V) of a tile as fp16
-  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];  // [2 slots][K, V]
-  __shared__ int s_last;
   const int tid = threadIdx.x, l = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c = l & 31, h = l >> 5;
   const int G = a.H / a.KV;
@@ -635,7 +649,7 @@ __global__ __launch_bounds__(256, 2) void attention_rows_kernel(AttnArgs a) {
     const Request rq = request(a, r);
     return rq.n * G > a.few_rows ? (rq.n * G + kRows - 1) / kRows : 0;
   };
-  const int kh = blockIdx.x % a.KV, rest = blockIdx.x / a.KV;
+  const int kh = wg % a.KV, rest = wg / a.KV;
   const int sp = rest % a.splits, index = rest / a.splits;
   const int run = (a.R + 63) >> 6, r_lane = run * l;
   int in_lane = 0;
@@ -901,7 +915,7 @@ __global__ __launch_bounds__(256, 2) void attention_rows_kernel(AttnArgs a) {
   // partial rows, as in the kernel above: values, max, sum
   constexpr int kSc1 = 16, kRec = D + 4;
   const int item = index * a.KV + kh;
-  const __amdgpu_buffer_rsrc_t rp = rsrc(a.part + (int64_t)item * a.splits * kRows * kRec, (int64_t)parts * kRows * kRec * 4);
+  const __amdgpu_buffer_rsrc_t rp = rsrc(a.many_part + (int64_t)item * a.splits * kRows * kRec, (int64_t)parts * kRows * kRec * 4);
   const int rrow = wave * 32 + c;
   if (live) {
     const int rec = (sp * kRows + rrow) * kRec * 4;
@@ -923,7 +937,7 @@ __global__ __launch_bounds__(256, 2) void attention_rows_kernel(AttnArgs a) {
   __builtin_amdgcn_s_waitcnt(0);
   __syncthreads();
   if (tid == 0) {
-    const int old = __hip_atomic_fetch_add(&a.counters[item], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    const int old = __hip_atomic_fetch_add(&a.counters[a.few_wgs + item], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     s_last = old == parts - 1;
   }
   __syncthreads();
@@ -953,7 +967,22 @@ __global__ __launch_bounds__(256, 2) void attention_rows_kernel(AttnArgs a) {
     for (int e = 0; e < 4; ++e) o[e] = (T)(jo[e] * inv);
     *reinterpret_cast<T4*>((T*)a.out + ((int64_t)(start + grow / G) * a.H + kh * G + grow % G) * D + dim) = o;
   }
-  if (tid == 0) __hip_atomic_store(&a.counters[item], 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  if (tid == 0) __hip_atomic_store(&a.counters[a.few_wgs + item], 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// The requests of few rows first, then those of many, in one launch, so that the end of the one
+// fills with the other (32 / 8 heads of 128: 8 single tokens of 2000 keys and a prompt of 2048 71 us, in
+// two launches 81; 32 of 3000 and a chunk of 512 behind 1000 77 and 84; two prompts of 300, where the
+// first find nothing to do, 17.4 and 18.6).
+template <typename T, int D, bool FP8>
+__global__ __launch_bounds__(256, 2) void attention_rows_kernel(AttnArgs a) {
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];  // [2 slots][K, V]
+  __shared__ int s_last;
+  static_assert(sizeof(FewLds<D>) <= 2 * 2 * 64 * D * 2, "fits the slots");
+  if ((int)blockIdx.x < a.few_wgs)
+    few_rows<T, D, FP8>(a, *reinterpret_cast<FewLds<D>*>(lds), blockIdx.x);
+  else
+    many_rows<T, D, FP8>(a, lds, s_last, blockIdx.x - a.few_wgs);
 }
 
 template <typename T, int D>
@@ -987,7 +1016,7 @@ ManyPlan many_plan(const PagedAttention& p, const PagedCache& c) {
   // two workgroups a CU; a range of at least eight tiles, as its join costs about two
   int64_t S = f.items > 0 ? 2 * device_cu_count() / f.items : 1;
   if (S > range / 512) S = range / 512;
-  if (S < 1 || f.items > (int64_t)kWsCounterBytes / 4) S = 1;
+  if (S < 1 || f.items > (int64_t)kWsCounterBytes / 4 - few_wgs(c.D)) S = 1;
   f.per = (int)(((range + S - 1) / S + 63) / 64 * 64);
   if (f.per < 64) f.per = 64;
   f.splits = (int)((range + f.per - 1) / f.per);
@@ -998,9 +1027,10 @@ ManyPlan many_plan(const PagedAttention& p, const PagedCache& c) {
 
 }  // namespace
 
+size_t few_part_bytes(int64_t D) { return (size_t)few_wgs(D) * 32 * (D + 4) * 4; }
+
 size_t paged_attention_ws_bytes(const PagedAttention& p, const PagedCache& c) {
-  const size_t few = (size_t)few_wgs(c.D) * 32 * (c.D + 4) * 4, many = many_plan(p, c).part;
-  return kWsCounterBytes + (few > many ? few : many);
+  return kWsCounterBytes + few_part_bytes(c.D) + many_plan(p, c).part;
 }
 
 hipError_t launch_paged_attention(const PagedAttention& p, const PagedCache& c, void* workspace, size_t ws_bytes,
@@ -1011,22 +1041,18 @@ hipError_t launch_paged_attention(const PagedAttention& p, const PagedCache& c, 
   a.max_q = (int)p.max_q, a.max_kv = (int)p.max_kv;
   a.few_rows = kFewRows;
   a.counters = (int*)workspace;
-  a.part = (float*)((char*)workspace + kWsCounterBytes);
+  a.few_part = (float*)((char*)workspace + kWsCounterBytes);
+  a.many_part = (float*)((char*)a.few_part + few_part_bytes(c.D));
+  a.few_wgs = few_wgs(c.D);
   const ManyPlan f = many_plan(p, c);
-  const int wgs = few_wgs(c.D);
-  hipError_t e = hipSuccess;
-  // Any batch of several requests may have some of few rows; a lone one stays with many.
-  if (f.items > 0 && p.R == 1) {
-    a.few_rows = 0;
-  } else {
-    if (p.bf16)
-      e = c.D == 64 ? few<__bf16, 64>(a, c.fp8, wgs, stream) : few<__bf16, 128>(a, c.fp8, wgs, stream);
-    else
-      e = c.D == 64 ? few<f16, 64>(a, c.fp8, wgs, stream) : few<f16, 128>(a, c.fp8, wgs, stream);
+  if (f.items == 0) {
+    if (p.bf16) return c.D == 64 ? few<__bf16, 64>(a, c.fp8, stream) : few<__bf16, 128>(a, c.fp8, stream);
+    return c.D == 64 ? few<f16, 64>(a, c.fp8, stream) : few<f16, 128>(a, c.fp8, stream);
   }
-  if (e != hipSuccess || f.items == 0) return e;
+  // Any batch of several requests may have some of few rows; a lone one stays with many.
+  if (p.R == 1) a.few_rows = 0, a.few_wgs = 0;
   a.splits = f.splits, a.per = f.per;
-  const int64_t n = f.items * f.splits;
+  const int64_t n = a.few_wgs + f.items * f.splits;
   if (p.bf16) return c.D == 64 ? many<__bf16, 64>(a, c.fp8, n, stream) : many<__bf16, 128>(a, c.fp8, n, stream);
   return c.D == 64 ? many<f16, 64>(a, c.fp8, n, stream) : many<f16, 128>(a, c.fp8, n, stream);
 }

@@ -486,6 +486,21 @@ def test_longer_prompts_and_several_tokens(new, lens):
 
 
 @gpu
+@pytest.mark.parametrize("H,KV,D", [(8, 2, 128), (8, 1, 64)])
+def test_prompts_among_single_tokens(H, KV, D):
+    """Requests of few and of many query rows in one call, both in parts that are joined, many
+    times over: no part of the one reaches the other's."""
+    lens = [3000, 700, 1, 5000, 2500, 64, 1300, 900]
+    new = [1, 200, 1, 1, 150, 8, 17, 1]
+    c, tables, starts, q = _attention_case(CODES[0], torch.float16, H, KV, D, 64, lens, new)
+    want = _oracle(c, tables, lens, starts, q)
+    first = _run(c, tables, lens, starts, q)
+    _check(first, *want, torch.float16)
+    for _ in range(50):
+        assert torch.equal(_run(c, tables, lens, starts, q), first)
+
+
+@gpu
 def test_attention_takes_strided_queries_and_leaves_rows_behind_the_last():
     lens, new = [70, 9], [5, 2]
     c, tables, starts, q = _attention_case(CODES[0], torch.float16, 4, 2, 64, 16, lens, new)
