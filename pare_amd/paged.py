@@ -202,8 +202,8 @@ def read_kv_pages(pages: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
 
 def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
                     v_scale: torch.Tensor, block_tables: torch.Tensor, kv_lens: torch.Tensor,
-                    q_starts: torch.Tensor | None = None, *, scale: float, window: int = 0, max_q_len: int = 1,
-                    max_kv_len: int | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+                    q_starts: torch.Tensor | None = None, *, scale: float, window: int = 0,
+                    max_q_len: int | None = None, max_kv_len: int | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
     """Attention [T, H, D] of the queries ``q`` [T, H, D] (fp16 or bf16, any token and head
     strides) over the cache.
 
@@ -212,7 +212,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     sees positions up to ``kv_lens[r] - n + i``, with ``window`` > 0 the last ``window`` of
     those. A query that sees nothing gives zeros; rows behind the last request's are
     left as they were (``out``) or undefined. ``max_q_len`` and ``max_kv_len`` bound what
-    a request has (default: the table's width); tighter bounds make the call faster.
+    a request has (default: all of q, the table's width): tighter bounds make the call
+    faster, and queries and keys past them are left out.
     ``scale`` multiplies q . k."""
     dev = _hip(q, "paged_attention")
     pages, KV, ps, D, code = _cache(dev, k_cache, v_cache, k_scale, v_scale)
@@ -227,7 +228,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     else:
         assert T == R, f"without q_starts there is one query per request: q has {T}, kv_lens {R}"
         max_q_len = 1
-    assert max_q_len >= 0 and window >= 0, "max_q_len and window may not be negative"
+    max_q = T if max_q_len is None else min(max_q_len, T)
+    assert max_q >= 0 and window >= 0, "max_q_len and window may not be negative"
     if q.stride(2) != 1 or q.stride(0) % 8 or q.stride(1) % 8 or q.data_ptr() % 16:
         q = torch.empty(T, H, D, dtype=q.dtype, device=dev).copy_(q)
     if out is None:
@@ -242,7 +244,6 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     L = _lib.lib()
     with _DeviceGuard(dev):
         stream = _raw_stream(dev)
-        max_q = min(max_q_len, T)
         nbytes = L.pmi_paged_attention_workspace_bytes(T, R, H, KV, D, max_q, max_kv, window)
         ws = _workspace(dev, stream, nbytes)
         _lib.check(L.pmi_paged_attention(
@@ -267,6 +268,12 @@ class PagedKVCache:
                  page_size: int = 64, pages: int | None = None, dtype: torch.dtype = torch.int8) -> None:
         if dtype not in _CODES:
             raise ValueError("the cache holds int8 or float8_e4m3fn codes")
+        if page_size not in (16, 32, 64, 128, 256):
+            raise ValueError(f"page_size must be 16, 32, 64, 128 or 256, got {page_size}")
+        if head_dim not in (64, 128):
+            raise ValueError(f"head_dim must be 64 or 128, got {head_dim}")
+        if min(layers, requests, max_len, kv_heads) < 1 or (pages is not None and pages < 1):
+            raise ValueError("layers, requests, max_len, kv_heads and pages must be positive")
         dev = torch.device(device)
         width = -(-max_len // page_size)
         pages = requests * width if pages is None else pages
@@ -303,7 +310,7 @@ class PagedKVCache:
                               self.k_scale[layer], self.v_scale[layer])
 
     def attend(self, layer: int, q: torch.Tensor, plan: BatchPlan, *, scale: float, window: int = 0,
-               max_q_len: int = 1, max_kv_len: int | None = None) -> torch.Tensor:
+               max_q_len: int | None = None, max_kv_len: int | None = None) -> torch.Tensor:
         return paged_attention(q, self.k[layer], self.v[layer], self.k_scale[layer], self.v_scale[layer],
                                self.block_tables, plan.kv_lens, plan.q_starts, scale=scale, window=window,
                                max_q_len=max_q_len, max_kv_len=max_kv_len)

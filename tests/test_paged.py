@@ -145,6 +145,11 @@ def test_cpu_tensors_raise():
         P.extend_block_tables(i[None], i, i, i, torch.zeros(4, dtype=torch.int32), 16, 1)
     with pytest.raises(ValueError):
         P.PagedKVCache(1, 1, 16, 1, 64, "cpu", dtype=torch.float16)
+    for args, kw in (((1, 1, 16, 1, 80, "cpu"), {}), ((1, 1, 16, 1, 64, "cpu"), dict(page_size=24)),
+                     ((1, 1, 16, 1, 64, "cpu"), dict(page_size=512)), ((1, 0, 16, 1, 64, "cpu"), {}),
+                     ((1, 1, 0, 1, 64, "cpu"), {}), ((1, 1, 16, 1, 64, "cpu"), dict(pages=0))):
+        with pytest.raises(ValueError):
+            P.PagedKVCache(*args, **kw)
 
 
 # --- block tables --------------------------------------------------------------------
@@ -633,8 +638,21 @@ def test_shared_pages_and_bounds_that_are_too_large():
         _check(_run(c, tables, lens, starts, q, **kw), *want, torch.float16)
     k, v, ks, vs = c.tensors(DEV)
     got = P.paged_attention(q.to(DEV), k, v, ks, vs, torch.from_numpy(tables).to(DEV), _ints(lens),
+                            torch.from_numpy(starts).to(DEV), scale=1 / 128 ** 0.5)
+    _check(got, *want, torch.float16)
+    got = P.paged_attention(q.to(DEV), k, v, ks, vs, torch.from_numpy(tables).to(DEV), _ints(lens),
                             torch.from_numpy(starts).to(DEV), scale=1 / 128 ** 0.5, max_q_len=1000)
     _check(got, *want, torch.float16)
+
+
+@gpu
+def test_without_bounds_everything_is_attended_to():
+    lens, new = [100, 300, 7], [60, 1, 7]
+    c, tables, starts, q = _attention_case(CODES[0], torch.float16, 4, 2, 128, 64, lens, new)
+    k, v, ks, vs = c.tensors(DEV)
+    got = P.paged_attention(q.to(DEV), k, v, ks, vs, torch.from_numpy(tables).to(DEV), _ints(lens),
+                            torch.from_numpy(starts).to(DEV), scale=1 / 128 ** 0.5)
+    _check(got, *_oracle(c, tables, lens, starts, q), torch.float16)
 
 
 @gpu
