@@ -203,7 +203,8 @@ def read_kv_pages(pages: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
 def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
                     v_scale: torch.Tensor, block_tables: torch.Tensor, kv_lens: torch.Tensor,
                     q_starts: torch.Tensor | None = None, *, scale: float, window: int = 0,
-                    max_q_len: int | None = None, max_kv_len: int | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+                    max_q_len: int | None = None, max_kv_len: int | None = None,
+                    out: torch.Tensor | None = None) -> torch.Tensor:
     """Attention [T, H, D] of the queries ``q`` [T, H, D] (fp16 or bf16, any token and head
     strides) over the cache.
 
@@ -272,8 +273,8 @@ class PagedKVCache:
             raise ValueError(f"page_size must be 16, 32, 64, 128 or 256, got {page_size}")
         if head_dim not in (64, 128):
             raise ValueError(f"head_dim must be 64 or 128, got {head_dim}")
-        if min(layers, requests, max_len, kv_heads) < 1 or (pages is not None and pages < 1):
-            raise ValueError("layers, requests, max_len, kv_heads and pages must be positive")
+        if layers < 0 or min(requests, max_len, kv_heads) < 1 or (pages is not None and pages < 1):
+            raise ValueError("requests, max_len, kv_heads and pages must be positive, layers not negative")
         dev = torch.device(device)
         width = -(-max_len // page_size)
         pages = requests * width if pages is None else pages
