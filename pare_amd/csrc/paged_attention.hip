@@ -4,6 +4,7 @@
 // p <= L - n + i (and p > L - n + i - window):
 //   o = sum_p e_p (vs_p v_p) / sum_p e_p,   e_p = exp(scale q . (ks_p k_p) - max)
 // with the codes k_p, v_p and their pages' scales. A query that sees nothing gives 0.
+#include <cfloat>
 #include <type_traits>
 
 #include "paged.h"
@@ -691,7 +692,7 @@ PMI_DEV void many_rows(const AttnArgs& a, uint8_t* lds, int& s_last, int wg) {
   // the wave's query rows: step s holds dimensions 16 s + 8 h .. + 7
   f16x8 qv[D / 16];
   // (the sign of the scale goes into q: block maxima need a factor that is not negative)
-  float qmul = fmaxf(fabsf(a.scale) * kLog2e, 1e-18f);
+  float qmul = fabsf(a.scale) * kLog2e;
   {
     typedef T T8 __attribute__((ext_vector_type(8)));
     const T* qr = (const T*)a.q + (int64_t)(start + (live ? i : i_first)) * a.q_token +
@@ -811,7 +812,7 @@ PMI_DEV void many_rows(const AttnArgs& a, uint8_t* lds, int& s_last, int wg) {
         }
       __builtin_amdgcn_s_setprio(0);
       const bool gone = cur.page < 0;
-      float ks = gone || cur.ks < 1e-18f ? 1e-18f : cur.ks, vs = gone ? 0.f : cur.vs;
+      float ks = gone ? 0.f : cur.ks, vs = gone ? 0.f : cur.vs;
       const bool bad = !(ks < INFINITY) || !(vs < INFINITY);
       // the unit of acc: the largest value scale so far, or half of it
       const float top = fmaxf(vref, max_of_4(vs < INFINITY ? vs : 0.f));
@@ -823,7 +824,7 @@ PMI_DEV void many_rows(const AttnArgs& a, uint8_t* lds, int& s_last, int wg) {
         vinv = kPBias / vref;
       }
       // result 16 u + 4 j + e: token 32 u + 16 (j / 2) + 8 h + 4 (j % 2) + e, block 2 u + j / 2.
-      // Hidden tokens get -inf, which stays one through the scales (at least 1e-18).
+      // Hidden tokens get -inf, which stays one through the factors k1 (at least FLT_MIN).
       if (p < safe_lo || p + 64 > safe_hi || p + 64 > p1 || __any(gone)) {
         const int from = lo - p - 8 * h, to = min(hi, p1) - p - 8 * h;
 #pragma unroll
@@ -835,7 +836,7 @@ PMI_DEV void many_rows(const AttnArgs& a, uint8_t* lds, int& s_last, int wg) {
       }
       if (const uint64_t which = __ballot(bad)) {
         // a page that holds an infinity or NaN: what sees it becomes NaN
-        if (bad) ks = 1e-18f, vs = 0.f;
+        if (bad) ks = 0.f, vs = 0.f;
 #pragma unroll
         for (int b = 0; b < 4; ++b)
 #pragma unroll
@@ -845,9 +846,11 @@ PMI_DEV void many_rows(const AttnArgs& a, uint8_t* lds, int& s_last, int wg) {
           }
       }
       const float vsv = vs * vinv;
+      // (FLT_MIN after all factors, the query's power of two among them; the sums are below 2^33, so what
+      // it raises is a score of 0 all the same)
       float k1[4], v1[4];
 #pragma unroll
-      for (int b = 0; b < 4; ++b) k1[b] = of_block(ks, b) * qmul, v1[b] = of_block(vsv, b);
+      for (int b = 0; b < 4; ++b) k1[b] = fmaxf(of_block(ks, b) * qmul, FLT_MIN), v1[b] = of_block(vsv, b);
       float mx = -INFINITY;
 #pragma unroll
       for (int b = 0; b < 4; ++b) {

@@ -675,3 +675,31 @@ def test_python_checks():
         P.extend_block_tables(t, lens, lens.long(), lens, _ints([0, 0, 0, 0]), 16, 1)
     with pytest.raises(_lib.PmiError):
         P.extend_block_tables(t, lens, lens, lens, _ints([0, 0, 0, 0]), 24, 1)
+
+
+# --- extremes ----------------------------------------------------------------------------
+
+def _check_finite(got, o, weight, dtype):
+    """``_check``, and nothing is NaN where the definition is not."""
+    assert got.isfinite().all(), f"{(~got.isfinite()).sum().item()} of {got.numel()} not finite"
+    _check(got, o, weight, dtype)
+
+
+@gpu
+@pytest.mark.parametrize("new", [1, 40])
+@pytest.mark.parametrize("size,keys", [(1e-24, 1), (1e-27, 1), (1e-37, 1), (1e20, 1e-20)])
+def test_attention_of_small_queries_and_small_keys(size, keys, new):
+    """bf16 queries whose products with the keys' scales leave fp32's range on one side, over
+    partial last tiles and pages of zero keys: finite, and right, in both forms."""
+    lens, ps = [200, 513, 70], 32
+    c, tables, starts, q = _attention_case(CODES[0], torch.bfloat16, 4, 1, 128, ps, lens, [new] * 3, spread=2 * size)
+    c.scales[0] *= np.float32(keys)
+    for page in (tables[0, 1], tables[1, 7], tables[1, 16]):
+        c.codes[0][page] = 0
+        c.scales[0][page] = 0
+    _check_finite(_run(c, tables, lens, starts, q), *_oracle(c, tables, lens, starts, q), torch.bfloat16)
+    k, v, ks, vs = c.tensors(DEV)
+    flat = P.paged_attention(q.to(DEV), k, v, ks, vs, torch.from_numpy(tables).to(DEV), _ints(lens),
+                             torch.from_numpy(starts).to(DEV), scale=0.0, max_q_len=new)
+    _check_finite(flat, *S.attention(np.zeros(q.shape), c.values(0), c.values(1), tables, lens, starts, ps, 0.0),
+           torch.bfloat16)
