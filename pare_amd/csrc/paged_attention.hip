@@ -95,19 +95,20 @@ PMI_DEV u32x4 byte_mask(int first, int last) {
   return m;
 }
 
-// 2^e <= m < 2^(e + 1) as `up`, and its inverse; 1 for zero, subnormal and infinite m.
+// 2^e <= m < 2^(e + 1) as `up`, and its inverse, both finite and normal: e from -126 (also
+// of zero and subnormal m) to 113 (also of larger, infinite and NaN m).
 struct PowerOfTwo {
   float up, down;
 };
 PMI_DEV PowerOfTwo power_below(float m) {
-  const uint32_t e = __builtin_bit_cast(uint32_t, m) >> 23;
-  if (e < 1 || e > 253) return {1.f, 1.f};
+  const uint32_t e = min(max(__builtin_bit_cast(uint32_t, m) >> 23, 1u), 240u);
   return {__builtin_bit_cast(float, e << 23), __builtin_bit_cast(float, (254u - e) << 23)};
 }
 
 // A row of q as fp16 that the products take exactly: bf16 rows are scaled by a power of two
 // to a largest value in [1, 2) (what falls under 2^-24 of it is lost to fp16's range, and
-// is 2^-16 of bf16's own rounding of the largest). mul takes the power back.
+// is 2^-16 of bf16's own rounding of the largest), at most 2^15 of rows from 2^114 on, so that
+// the power times the scale stays finite. mul takes the power back.
 template <typename T, int D>
 struct QueryRow {
   f16x8 v[D / 32];

@@ -703,3 +703,18 @@ def test_attention_of_small_queries_and_small_keys(size, keys, new):
                              torch.from_numpy(starts).to(DEV), scale=0.0, max_q_len=new)
     _check_finite(flat, *S.attention(np.zeros(q.shape), c.values(0), c.values(1), tables, lens, starts, ps, 0.0),
            torch.bfloat16)
+
+
+@gpu
+@pytest.mark.parametrize("new", [1, 40])
+@pytest.mark.parametrize("size,keys", [(0.9e38, 1e-38), (2e-39, 1e38)])
+def test_attention_of_queries_at_the_ends_of_bf16(size, keys, new):
+    """Queries of up to the largest bf16 and subnormal ones, with keys that make ordinary
+    scores of them."""
+    lens = [200, 513, 70]
+    c, tables, starts, q = _attention_case(CODES[0], torch.bfloat16, 4, 1, 128, 32, lens, [new] * 3, spread=1.0)
+    q = (q.double() * size).clamp(-3.3e38, 3.3e38).to(torch.bfloat16)
+    largest = q.abs().float().amax(-1)
+    assert largest.isfinite().all() and (largest.max() > 2.0 ** 127 if size > 1 else largest.max() < 2.0 ** -126)
+    c.scales[0] *= np.float32(keys)
+    _check_finite(_run(c, tables, lens, starts, q), *_oracle(c, tables, lens, starts, q), torch.bfloat16)
