@@ -1502,9 +1502,9 @@ int pmi_paged_attention(const void* q, int dtype, int64_t q_stride, int64_t q_he
   const pmi::PagedCache c = {const_cast<void*>(k_cache), const_cast<void*>(v_cache), const_cast<float*>(k_scale),
                              const_cast<float*>(v_scale), n_pages, KV, page_size, D, code_dtype == PMI_F8};
   if (p.max_kv > width * page_size) p.max_kv = width * page_size;
-  // the kernel counts tiles of 64 keys x 16 query rows in 32 bits
-  if ((double)R * (double)KV * (double)(max_q * (H / KV) / 16 + 1) * (double)(p.max_kv / 64 + 5) >= 2147483648.0)
-    return fail(PMI_ERR_UNSUPPORTED, "%s: too many tiles (R KV max_q H / KV max_kv): give tighter max_q and max_kv", fn);
+  if (!pmi::paged_attention_tiles_fit(p, c))
+    return fail(PMI_ERR_UNSUPPORTED, "%s: too many tiles of 64 keys for 32 bits (R KV max_kv): give a tighter max_kv "
+                "or fewer requests", fn);
   const size_t need = pmi_paged_attention_workspace_bytes(T, R, H, KV, D, max_q, p.max_kv, window);
   if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 256)))
     return fail(PMI_ERR_INVALID, "%s: needs a 256-byte aligned workspace of %zu bytes", fn, need);

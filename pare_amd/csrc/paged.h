@@ -59,7 +59,9 @@ struct PagedAttention {
   float scale;
   bool bf16;
 };
-// Bytes after the counters of the workspace for calls of these limits (0: none needed).
+// Whether the count of tiles that the requests of few query rows may have fits 32 bits.
+bool paged_attention_tiles_fit(const PagedAttention& p, const PagedCache& c);
+// Bytes of the workspace, its counters included, for calls of these limits.
 size_t paged_attention_ws_bytes(const PagedAttention& p, const PagedCache& c);
 hipError_t launch_paged_attention(const PagedAttention& p, const PagedCache& c, void* workspace, size_t ws_bytes,
                                   hipStream_t stream);

@@ -1033,6 +1033,13 @@ ManyPlan many_plan(const PagedAttention& p, const PagedCache& c) {
 
 size_t few_part_bytes(int64_t D) { return (size_t)few_wgs(D) * 32 * (D + 4) * 4; }
 
+bool paged_attention_tiles_fit(const PagedAttention& p, const PagedCache& c) {
+  // of every request the rows of one of few rows, in tiles of 16; keys in tiles of 64, one more for a
+  // range that begins inside a tile, and up to four for its last cut
+  const int64_t rows = p.max_q * (p.H / c.KV), row_tiles = ((rows < kFewRows ? rows : kFewRows) + 15) / 16;
+  return (double)p.R * (double)c.KV * (double)row_tiles * (double)(p.max_kv / 64 + 5) < 2147483648.0;
+}
+
 size_t paged_attention_ws_bytes(const PagedAttention& p, const PagedCache& c) {
   return kWsCounterBytes + few_part_bytes(c.D) + many_plan(p, c).part;
 }

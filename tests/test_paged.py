@@ -718,3 +718,33 @@ def test_attention_of_queries_at_the_ends_of_bf16(size, keys, new):
     assert largest.isfinite().all() and (largest.max() > 2.0 ** 127 if size > 1 else largest.max() < 2.0 ** -126)
     c.scales[0] *= np.float32(keys)
     _check_finite(_run(c, tables, lens, starts, q), *_oracle(c, tables, lens, starts, q), torch.bfloat16)
+
+
+def test_attention_accepts_one_long_request_among_many():
+    """The count of tiles that must fit 32 bits is that of the requests of few query rows: a
+    long prompt, or a chunk, among many requests is not refused (but for the workspace that
+    is missing here), nor are loose bounds; a count that does not fit is."""
+    L = _lib.lib()
+    for kw in (dict(T=16384, R=256, max_q=8192, max_kv=32768, width=512), dict(T=8192, R=64, max_q=8192,
+                                                                               max_kv=131072, width=2048),
+               dict(T=34000, R=64, max_q=32768, max_kv=32768, width=512), dict(T=4096, R=4096, max_q=1, max_kv=131072,
+                                                                               width=2048)):
+        rc = L.pmi_paged_attention(*_attention_args(H=32, KV=8, ps=64, stride=4096, pages=1 << 16, ws=None,
+                                                    tstride=kw["width"], **kw))
+        assert rc == _lib.PMI_ERR_INVALID and "workspace" in _lib.last_error(), (kw, _lib.last_error())
+    rc = L.pmi_paged_attention(*_attention_args(H=32, KV=8, ps=256, stride=4096, T=65536, R=4096, max_q=16, ws=None,
+                                                max_kv=1 << 22, width=1 << 14, tstride=1 << 14))
+    assert rc == _lib.PMI_ERR_UNSUPPORTED and "tiles" in _lib.last_error()
+
+
+@gpu
+def test_attention_with_bounds_far_above_a_ragged_batch():
+    """A prompt and many single tokens without bounds, tables for half a million tokens."""
+    lens, new = [200] + [20 + i for i in range(63)], [200] + [1] * 63
+    c, tables, starts, q = _attention_case(CODES[0], torch.float16, 16, 2, 64, 64, lens, new, width=8400)
+    k, v, ks, vs = c.tensors(DEV)
+    rows = torch.zeros(6000, 16, 64, dtype=torch.float16, device=DEV)
+    rows[:263] = q.to(DEV)
+    got = P.paged_attention(rows, k, v, ks, vs, torch.from_numpy(tables).to(DEV), _ints(lens),
+                            torch.from_numpy(starts).to(DEV), scale=1 / 8)
+    _check_finite(got[:263], *_oracle(c, tables, lens, starts, q), torch.float16)
