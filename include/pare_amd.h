@@ -632,7 +632,7 @@ PMI_API int pmi_rope_append_kv(const void* qkv, int dtype, int64_t qkv_stride, c
 /* Whole pages as values: k_out, v_out [n, KV, page_size, D] of out_dtype (PMI_F16,
  * PMI_BF16 or PMI_F32, 16-byte aligned) of pages[i] (int32 [n]); zeros for a page
  * number outside the cache. Tokens that nothing was written to read as whatever
- * their bytes stand for. */
+ * their bytes stand for. n KV < 2^24. */
 PMI_API int pmi_read_kv_pages(const int32_t* pages, const void* k_cache, const void* v_cache,
                               const float* k_scale, const float* v_scale, int code_dtype,
                               int64_t n_pages, int64_t page_size, void* k_out, void* v_out,

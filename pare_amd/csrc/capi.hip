@@ -1429,7 +1429,9 @@ int pmi_rope_append_kv(const void* qkv, int dtype, int64_t qkv_stride, const flo
     return fail(PMI_ERR_INVALID, "%s: need T >= 0, L > 0 and qkv_stride >= (H + 2 KV) D, a multiple of 8 "
                 "(T=%lld L=%lld stride=%lld)", fn, (long long)T, (long long)L, (long long)qkv_stride);
   if (T == 0) return ok();
-  if (T >= (1ll << 31) || L >= (1ll << 31) || T * (H / KV) * (D / 16) >= (1ll << 36))
+  // (a launch holds fewer than 2^24 workgroups of 256 threads: one for every 8 tokens here, and one for
+  // every 256 units of D / 16 a token)
+  if (T >= (1ll << 31) || L >= (1ll << 31) || T / 8 + 1 + T * (D / 16) / 256 + 1 >= (1ll << 24))
     return fail(PMI_ERR_UNSUPPORTED, "%s: too many tokens", fn);
   if (!qkv || !cos_t || !sin_t || !positions || !slots || !q_out) return fail(PMI_ERR_INVALID, "%s: null buffer", fn);
   for (const void* p : {qkv, (const void*)cos_t, (const void*)sin_t, (const void*)q_out})
@@ -1448,7 +1450,7 @@ int pmi_read_kv_pages(const int32_t* pages, const void* k_cache, const void* v_c
     return fail(PMI_ERR_INVALID, "%s: out_dtype must be PMI_F16, PMI_BF16 or PMI_F32 (got %d)", fn, out_dtype);
   if (n < 0) return fail(PMI_ERR_INVALID, "%s: need n >= 0", fn);
   if (n == 0) return ok();
-  if (n >= (1ll << 31) / KV) return fail(PMI_ERR_UNSUPPORTED, "%s: too many pages", fn);
+  if (n >= (1ll << 24) / KV) return fail(PMI_ERR_UNSUPPORTED, "%s: too many pages", fn);
   if (!pages || !k_out || !v_out) return fail(PMI_ERR_INVALID, "%s: null buffer", fn);
   if (!aligned(k_out, 16) || !aligned(v_out, 16))
     return fail(PMI_ERR_INVALID, "%s: k_out and v_out must be 16-byte aligned", fn);
@@ -1502,6 +1504,8 @@ int pmi_paged_attention(const void* q, int dtype, int64_t q_stride, int64_t q_he
   const pmi::PagedCache c = {const_cast<void*>(k_cache), const_cast<void*>(v_cache), const_cast<float*>(k_scale),
                              const_cast<float*>(v_scale), n_pages, KV, page_size, D, code_dtype == PMI_F8};
   if (p.max_kv > width * page_size) p.max_kv = width * page_size;
+  if (!pmi::paged_attention_launch_fits(p, c))
+    return fail(PMI_ERR_UNSUPPORTED, "%s: too many query rows for one launch (T H)", fn);
   if (!pmi::paged_attention_tiles_fit(p, c))
     return fail(PMI_ERR_UNSUPPORTED, "%s: too many tiles of 64 keys for 32 bits (R KV max_kv): give a tighter max_kv "
                 "or fewer requests", fn);

@@ -61,6 +61,8 @@ struct PagedAttention {
 };
 // Whether the count of tiles that the requests of few query rows may have fits 32 bits.
 bool paged_attention_tiles_fit(const PagedAttention& p, const PagedCache& c);
+// Whether its workgroups fit a launch.
+bool paged_attention_launch_fits(const PagedAttention& p, const PagedCache& c);
 // Bytes of the workspace, its counters included, for calls of these limits.
 size_t paged_attention_ws_bytes(const PagedAttention& p, const PagedCache& c);
 hipError_t launch_paged_attention(const PagedAttention& p, const PagedCache& c, void* workspace, size_t ws_bytes,

@@ -1040,6 +1040,11 @@ bool paged_attention_tiles_fit(const PagedAttention& p, const PagedCache& c) {
   return (double)p.R * (double)c.KV * (double)row_tiles * (double)(p.max_kv / 64 + 5) < 2147483648.0;
 }
 
+bool paged_attention_launch_fits(const PagedAttention& p, const PagedCache& c) {
+  const ManyPlan f = many_plan(p, c);
+  return few_wgs(c.D) + f.items * f.splits < (1ll << 24);  // of 256 threads: 2^32
+}
+
 size_t paged_attention_ws_bytes(const PagedAttention& p, const PagedCache& c) {
   return kWsCounterBytes + few_part_bytes(c.D) + many_plan(p, c).part;
 }

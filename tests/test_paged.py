@@ -748,3 +748,15 @@ def test_attention_with_bounds_far_above_a_ragged_batch():
     got = P.paged_attention(rows, k, v, ks, vs, torch.from_numpy(tables).to(DEV), _ints(lens),
                             torch.from_numpy(starts).to(DEV), scale=1 / 8)
     _check_finite(got[:263], *_oracle(c, tables, lens, starts, q), torch.float16)
+
+
+def test_launches_past_32_bits_are_refused():
+    """Grids of 2^32 threads or more (whose sizes a launch counts in 32 bits)."""
+    L = _lib.lib()
+    n = 1 << 24
+    assert L.pmi_read_kv_pages(P8, P8, P8, P8, P8, _lib.PMI_I8, 4, 16, P8, P8, _lib.PMI_F16, n // 4, 4, 64,
+                               None) == _lib.PMI_ERR_UNSUPPORTED
+    assert L.pmi_rope_append_kv(*_append_args(T=1 << 27, D=128, H=1, KV=1, stride=384)) == _lib.PMI_ERR_UNSUPPORTED
+    rc = L.pmi_paged_attention(*_attention_args(H=2, KV=2, D=64, T=1 << 29, R=1 << 23, max_q=65, stride=128, head=64,
+                                                max_kv=64, width=4))
+    assert rc == _lib.PMI_ERR_UNSUPPORTED, rc
