@@ -312,7 +312,7 @@ PMI_DEV void decode4(uint32_t w, float* v) {
 }
 
 // |x| as bits: ordered as the values are, with infinities and NaN above them, so
-// that a maximum keeps them and the page's scale shows them.
+// that a maximum keeps them and the page's scale shows them (as NaN).
 PMI_DEV uint32_t abs_bits(float x) { return __builtin_bit_cast(uint32_t, x) & 0x7fffffffu; }
 
 // What of a run stays on the chip between its maximum and its codes: 512 units of 16
@@ -389,7 +389,10 @@ PMI_DEV void append_run(const AppendArgs& a, int t0, int n, int slot, int kh, ui
   for (int w = 0; w < 4; ++w) mk = max(mk, red[2 * w]), mv = max(mv, red[2 * w + 1]);
   const float want_k = __builtin_bit_cast(float, mk) * (1.f / kTop), want_v = __builtin_bit_cast(float, mv) * (1.f / kTop);
   const bool grow_k = abs_bits(want_k) > abs_bits(before_k), grow_v = abs_bits(want_v) > abs_bits(before_v);
-  const float sk = grow_k ? want_k : before_k, sv = grow_v ? want_v : before_v;
+  // An infinity becomes NaN too: its page's codes times an infinite scale would be NaN, an infinity
+  // of either sign or (a code of 0 written later) NaN again.
+  const auto or_nan = [](float s) { return s < INFINITY ? s : __builtin_nanf(""); };
+  const float sk = or_nan(grow_k ? want_k : before_k), sv = or_nan(grow_v ? want_v : before_v);
   // (finite, also for subnormal scales)
   const float inv_k = sk > 0.f ? fminf(1.f / sk, FLT_MAX) : 0.f, inv_v = sv > 0.f ? fminf(1.f / sv, FLT_MAX) : 0.f;
   if (tid == 0) a.k_scale[cell] = sk, a.v_scale[cell] = sv;

@@ -760,3 +760,40 @@ def test_launches_past_32_bits_are_refused():
     rc = L.pmi_paged_attention(*_attention_args(H=2, KV=2, D=64, T=1 << 29, R=1 << 23, max_q=65, stride=128, head=64,
                                                 max_kv=64, width=4))
     assert rc == _lib.PMI_ERR_UNSUPPORTED, rc
+
+
+@gpu
+@pytest.mark.parametrize("code", CODES)
+@pytest.mark.parametrize("bad", [float("inf"), float("-inf"), float("nan")])
+def test_a_page_with_an_infinity_reads_as_nan(bad, code):
+    """An infinite or NaN key or value makes its page and head NaN, as they are read and for
+    every query that sees them; nothing else changes."""
+    H, KV, D, ps, T = 4, 2, 64, 16, 40
+    g = torch.Generator(device=DEV).manual_seed(2)
+    qkv = torch.randn(T, (H + 2 * KV) * D, generator=g, device=DEV).half()
+    cos, sin = (torch.from_numpy(t).to(DEV) for t in _rope(48, D))
+    for col, which in ((H * D + 5, 0), ((H + KV) * D + 5, 1)):
+        caches = []
+        for value in (1.0, bad):
+            c = P.PagedKVCache(1, 1, 48, KV, D, DEV, page_size=ps, dtype=code)
+            x = qkv.clone()
+            x[20, col] = value  # second page, head 0
+            q = c.append(0, x, cos, sin, c.extend(_ints([T]), T))
+            caches.append(c)
+        page = caches[1].block_tables[0]
+        read = P.read_kv_pages(page, caches[1].k[0], caches[1].v[0], caches[1].k_scale[0], caches[1].v_scale[0])
+        clean = P.read_kv_pages(page, caches[0].k[0], caches[0].v[0], caches[0].k_scale[0], caches[0].v_scale[0])
+        assert read[which][1, 0].isnan().all()
+        read[which][1, 0] = clean[which][1, 0]
+        assert torch.equal(read[0], clean[0]) and torch.equal(read[1], clean[1])
+        for queries in (q, -q, q[-1:], -q[-1:]):
+            n = len(queries)
+            want, got = (P.paged_attention(queries, c.k[0], c.v[0], c.k_scale[0], c.v_scale[0], c.block_tables,
+                                           c.kv_lens, _ints([0, n]), scale=0.125) for c in caches)
+            sees = torch.arange(T - n, T, device=DEV) >= 16
+            assert got[sees][:, :2].isnan().all()
+            # (the largest value scale of a tile is the unit that probabilities are rounded in, of rows
+            # that do not see its page too: both are within _tolerance of the same)
+            assert torch.equal(got[:, 2:], want[:, 2:])
+            a, b = (t[~sees].double().cpu().numpy() for t in (got, want))
+            assert (np.abs(a - b) <= 2 * _tolerance(b, clean[1].abs().max().item(), torch.float16)).all()
