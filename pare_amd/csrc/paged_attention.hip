@@ -372,7 +372,9 @@ PMI_DEV void few_rows(const AttnArgs& a, FewLds<D>& lds, int wg) {
   auto tile = [&](auto last) {
     constexpr bool kLast = decltype(last)::value;
     const bool gone = page < 0;
-    const float ks = gone ? 0.f : bks * qmul, tvs = gone ? 0.f : bvs;
+    // (a page that holds an infinity or NaN: what sees it becomes NaN, not an infinity by its codes' signs)
+    const bool bad = !(bks < INFINITY) || !(bvs < INFINITY);
+    const float ks = gone ? 0.f : bad ? __builtin_nanf("") : bks * qmul, tvs = gone ? 0.f : bvs;
     f32x4 s[4];
 #pragma unroll
     for (int t = 0; t < 4; ++t) {

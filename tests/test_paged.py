@@ -797,3 +797,26 @@ def test_a_page_with_an_infinity_reads_as_nan(bad, code):
             assert torch.equal(got[:, 2:], want[:, 2:])
             a, b = (t[~sees].double().cpu().numpy() for t in (got, want))
             assert (np.abs(a - b) <= 2 * _tolerance(b, clean[1].abs().max().item(), torch.float16)).all()
+
+
+@gpu
+@pytest.mark.parametrize("new", [1, 40])
+@pytest.mark.parametrize("code", CODES)
+@pytest.mark.parametrize("which", [0, 1])
+@pytest.mark.parametrize("bad", [np.inf, np.nan])
+def test_attention_over_a_scale_that_is_not_finite(bad, which, code, new):
+    """What sees a page whose scale is infinite or NaN is NaN in every dimension, whatever its
+    codes and the query's sign; other requests and heads are as without it."""
+    lens = [100, 130, 64]
+    c, tables, starts, q = _attention_case(code, torch.float16, 8, 2, 64, 32, lens, [new] * 3)
+    clean = _run(c, tables, lens, starts, q)
+    page = tables[1, 1]  # positions 32 to 63 of request 1
+    c.codes[which][page, 0] = 0x81 if code == torch.int8 else 0xFE  # the most negative code: no 0 * inf
+    c.scales[which][page, 0] = bad
+    for sign in (1, -1):
+        got = _run(c, tables, lens, starts, sign * q)
+        a, b = int(starts[1]), int(starts[2])
+        assert got[a:b, :4].isnan().all()
+        if sign == 1:
+            assert torch.equal(got[a:b, 4:], clean[a:b, 4:])
+            assert torch.equal(got[:a], clean[:a]) and torch.equal(got[b:], clean[b:])
