@@ -42,6 +42,9 @@ struct Request {
   int first_seen;     // the first position that its first query sees
   int lo, hi;         // positions that any of its queries sees: [lo, hi), lo a multiple of 16
 };
+// The first position that a query sees whose last is `last` (negative ones see nothing, and a
+// large window less them would leave the integers).
+PMI_DEV int first_position(const AttnArgs& a, int last) { return a.window && last >= a.window ? last + 1 - a.window : 0; }
 PMI_DEV Request request(const AttnArgs& a, int r) {
   const int len0 = a.kv_lens[r];
   Request q;
@@ -54,7 +57,7 @@ PMI_DEV Request request(const AttnArgs& a, int r) {
   q.shift = q.len - q.n;  // (also of the queries past max_q)
   q.n = min(q.n, a.max_q);
   if (q.n < 0 || q.start < 0 || (int64_t)q.start + q.n > a.T) q.n = 0;
-  q.first_seen = a.window ? max(0, q.shift + 1 - a.window) : 0;
+  q.first_seen = first_position(a, q.shift);
   q.lo = q.first_seen & ~15;
   q.hi = a.n_pages ? max(q.lo, min(q.len, q.shift + q.n)) : q.lo;
   return q;
@@ -319,13 +322,13 @@ PMI_DEV void few_rows(const AttnArgs& a, FewLds<D>& lds, int wg) {
   const int i = row / G;
   // positions that this column's query sees: [lo, hi)
   const int hi = live ? max(0, min(len, shift + i + 1)) : 0;
-  const int lo = a.window ? max(0, shift + i + 1 - a.window) : 0;
+  const int lo = first_position(a, shift + i);
   const int i_first = rt * 16 / G, i_last = (rt * 16 + min(rows, 16) - 1) / G;
   const int first_seen = rq.first_seen;
   const int p0 = rq.lo + 64 * tile0, p1 = min(rq.hi, p0 + 64 * n_tiles);
   // tiles inside of [safe_lo, safe_hi) need no mask
   const int safe_hi = max(0, min(len, shift + i_first + 1));
-  const int safe_lo = a.window ? max(0, shift + i_last + 1 - a.window) : 0;
+  const int safe_lo = first_position(a, shift + i_last);
 
   QueryRow<T, D> q;
   load_query<T, D>(q, (const T*)a.q + (int64_t)(start + (live ? i : 0)) * a.q_token +
@@ -682,15 +685,15 @@ PMI_DEV void many_rows(const AttnArgs& a, uint8_t* lds, int& s_last, int wg) {
   const bool live = wave * 32 + c < rows;
   const int i = row / G;
   const int hi = live ? max(0, min(len, shift + i + 1)) : 0;
-  const int lo = a.window ? max(0, shift + i + 1 - a.window) : 0;
+  const int lo = first_position(a, shift + i);
   const int i_first = rt * kRows / G, i_last = (rt * kRows + rows - 1) / G;
-  const int first_seen = a.window ? max(0, shift + i_first + 1 - a.window) : 0, all_lo = first_seen & ~15;
+  const int first_seen = first_position(a, shift + i_first), all_lo = first_seen & ~15;
   const int all_hi = a.n_pages ? max(all_lo, min(len, shift + i_last + 1)) : all_lo;
   const int parts = max(1, (all_hi - all_lo + a.per - 1) / a.per);
   if (sp >= parts) return;
   const int p0 = all_lo + sp * a.per, p1 = min(all_hi, p0 + a.per);
   const int safe_hi = max(0, min(len, shift + i_first + 1));
-  const int safe_lo = a.window ? max(0, shift + i_last + 1 - a.window) : 0;
+  const int safe_lo = first_position(a, shift + i_last);
 
   // the wave's query rows: step s holds dimensions 16 s + 8 h .. + 7
   f16x8 qv[D / 16];

@@ -820,3 +820,14 @@ def test_attention_over_a_scale_that_is_not_finite(bad, which, code, new):
         if sign == 1:
             assert torch.equal(got[a:b, 4:], clean[a:b, 4:])
             assert torch.equal(got[:a], clean[:a]) and torch.equal(got[b:], clean[b:])
+
+
+@gpu
+@pytest.mark.parametrize("new,lens", [([9, 3], [5, 100]), ([40, 70], [30, 300])])
+def test_the_largest_window_hides_nothing(new, lens):
+    """Windows up to the largest int, also where there are more queries than keys."""
+    c, tables, starts, q = _attention_case(CODES[0], torch.float16, 4, 1, 64, 16, lens, new)
+    want = _run(c, tables, lens, starts, q)
+    assert want[-1].isfinite().all() and (want[-1] != 0).any()
+    for window in (2 ** 31 - 1, 2 ** 31 - 2, 2 ** 30, 10 ** 6):
+        assert torch.equal(_run(c, tables, lens, starts, q, window=window), want), window
