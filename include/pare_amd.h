@@ -601,6 +601,15 @@ PMI_API int pmi_extend_block_tables(int32_t* tables, int64_t table_stride, const
                                     int32_t* first, int32_t* fresh, int32_t* positions,
                                     int32_t* slots, int32_t* pool_out, int64_t R, int64_t width, int64_t ring,
                                     int64_t page_size, int64_t total, void* stream);
+/* The same, where a request that would grow past max_len tokens (>= 0) is refused as well:
+ * the rows of its tables may hold more, and the RoPE tables less. */
+PMI_API int pmi_extend_block_tables_upto(int32_t* tables, int64_t table_stride, const int32_t* kv_lens,
+                                         const int32_t* new_lens, const int32_t* free_pages,
+                                         const int32_t* pool, int32_t* q_starts, int32_t* kv_lens_out,
+                                         int32_t* first, int32_t* fresh, int32_t* positions,
+                                         int32_t* slots, int32_t* pool_out, int64_t R, int64_t width,
+                                         int64_t ring, int64_t page_size, int64_t max_len, int64_t total,
+                                         void* stream);
 
 /* The pages of every request r with done[r] != 0 (u8 [R]) go to the end of the ring
  * of free pages, in request order, and kv_lens[r] becomes 0. The tables stay. */

@@ -93,6 +93,7 @@ SIGNATURES = {
     "pmi_argmax_f16": (_i, [_vp, _i64, _i64, _vp, _i64, _vp, ctypes.c_size_t, _vp]),
     "pmi_argmax_workspace_bytes": (ctypes.c_size_t, [_i64, _i64]),
     "pmi_extend_block_tables": (_i, [_vp, _i64, *[_vp] * 11, *[_i64] * 5, _vp]),
+    "pmi_extend_block_tables_upto": (_i, [_vp, _i64, *[_vp] * 11, *[_i64] * 6, _vp]),
     "pmi_release_block_tables": (_i, [_vp, _i64, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp]),
     "pmi_rope_append_kv": (_i, [_vp, _i, _i64, _vp, _vp, _i64, *[_vp] * 7, _i, *[_i64] * 6, _vp]),
     "pmi_read_kv_pages": (_i, [*[_vp] * 5, _i, _i64, _i64, _vp, _vp, _i, _i64, _i64, _i64, _vp]),

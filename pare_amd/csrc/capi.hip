@@ -1394,15 +1394,26 @@ int pmi_extend_block_tables(int32_t* tables, int64_t table_stride, const int32_t
                             int32_t* q_starts, int32_t* kv_lens_out, int32_t* first, int32_t* fresh,
                             int32_t* positions, int32_t* slots, int32_t* pool_out, int64_t R, int64_t width, int64_t ring,
                             int64_t page_size, int64_t total, void* stream) {
+  return pmi_extend_block_tables_upto(tables, table_stride, kv_lens, new_lens, free_pages, pool, q_starts, kv_lens_out,
+                                      first, fresh, positions, slots, pool_out, R, width, ring, page_size, INT32_MAX,
+                                      total, stream);
+}
+
+int pmi_extend_block_tables_upto(int32_t* tables, int64_t table_stride, const int32_t* kv_lens,
+                                 const int32_t* new_lens, const int32_t* free_pages, const int32_t* pool,
+                                 int32_t* q_starts, int32_t* kv_lens_out, int32_t* first, int32_t* fresh,
+                                 int32_t* positions, int32_t* slots, int32_t* pool_out, int64_t R, int64_t width,
+                                 int64_t ring, int64_t page_size, int64_t max_len, int64_t total, void* stream) {
   const char* fn = "pmi_extend_block_tables";
   if (int rc = check_tables(R, width, table_stride, ring, page_size, fn)) return rc;
+  if (max_len < 0) return fail(PMI_ERR_INVALID, "%s: max_len=%lld may not be negative", fn, (long long)max_len);
   if (total < 0 || total >= (1ll << 31))
     return fail(PMI_ERR_INVALID, "%s: total=%lld must be in [0, 2^31)", fn, (long long)total);
   if (!pool || !q_starts || !fresh || !pool_out || (R && (!tables || !kv_lens || !new_lens || !kv_lens_out || !first)) ||
       (ring && !free_pages) || (total && (!positions || !slots)))
     return fail(PMI_ERR_INVALID, "%s: null buffer", fn);
   const pmi::PagedTables t = {tables, table_stride, kv_lens, new_lens, free_pages, pool, q_starts, kv_lens_out,
-                              first, fresh, positions, slots, pool_out, R, width, ring, page_size, total};
+                              first, fresh, positions, slots, pool_out, R, width, ring, page_size, total, max_len};
   return from_hip(pmi::launch_extend_tables(t, (hipStream_t)stream), fn);
 }
 

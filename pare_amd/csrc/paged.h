@@ -23,6 +23,7 @@ struct PagedTables {
   int32_t* slots;             // [total]
   int32_t* pool_out;          // [4], may be pool
   int64_t R, width, ring, ps, total;
+  int64_t max_len;  // no request grows past so many tokens
 };
 hipError_t launch_extend_tables(const PagedTables& t, hipStream_t stream);
 hipError_t launch_release_tables(const int32_t* tables, int64_t stride, int32_t* kv_lens, const uint8_t* done,

@@ -69,6 +69,7 @@ struct TablesArgs {
   int32_t* slots;
   int32_t* pool_out;
   int R, width, ring, ps, total;
+  int64_t max_len;
 };
 
 // Fresh page i of all (of request r, whose first is fresh page `base`) into its row.
@@ -93,9 +94,10 @@ PMI_DEV void token_slot(const TablesArgs& a, int t, int r, int start, int first,
 
 // One workgroup: the per-request sums and, for few tokens, the fresh pages and slots as
 // well. Bound by the chain of loads, two scans and the look-ups (128 requests of one token: 5 us,
-// 6.6 in a graph with its launch), not by its bytes; the sums are 64-bit. need_r = ceil((len + new) / ps) - ceil(len / ps); a request is granted where its
-// table row is wide enough and the sum of the needs up to it is within the pool, so the
-// granted ones that need pages are the first of them in order.
+// 6.6 in a graph with its launch), not by its bytes; the sums are 64-bit.
+// need_r = ceil((len + new) / ps) - ceil(len / ps); a request is granted where its table row is wide
+// enough, it stays within max_len and the sum of the needs up to it is within the pool, so the granted ones
+// that need pages are the first of them in order.
 // Everything is read before anything is written: kv_lens_out may be kv_lens,
 // pool_out may be pool.
 __global__ __launch_bounds__(1024) void extend_tables_kernel(TablesArgs a, int fill) {
@@ -119,7 +121,7 @@ __global__ __launch_bounds__(1024) void extend_tables_kernel(TablesArgs a, int f
       len = max(a.kv_lens[r], 0);
       fresh = max(a.new_lens[r], 0);
       const int64_t want = ((int64_t)len + fresh + a.ps - 1) / a.ps, held = ((int64_t)len + a.ps - 1) / a.ps;
-      fits = want <= a.width;
+      fits = want <= a.width && (int64_t)len + fresh <= a.max_len;
       need = fits ? want - held : 0;
     }
     Pair s = wg_scan(Pair{(int64_t)fresh, need}, wave_sums);
@@ -581,7 +583,7 @@ hipError_t launch_extend_tables(const PagedTables& t, hipStream_t stream) {
   TablesArgs a = {t.tables,    t.stride,      t.kv_lens, t.new_lens, t.free_pages, t.pool,
                   t.q_starts,  t.kv_lens_out, t.first,   t.fresh,    t.positions,  t.slots,
                   t.pool_out,
-                  (int)t.R,    (int)t.width,  (int)t.ring, (int)t.ps, (int)t.total};
+                  (int)t.R,    (int)t.width,  (int)t.ring, (int)t.ps, (int)t.total, t.max_len};
   // One workgroup looks up 1024 tokens at a time; past a few rounds a grid is quicker (700
   // requests of 16-token pages, 270000 tokens: 23 + 5 us with the pages in the one workgroup).
   const bool fill = t.total <= 4096;

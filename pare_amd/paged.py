@@ -89,8 +89,8 @@ def _cache(dev: torch.device, k_cache: torch.Tensor, v_cache: torch.Tensor, k_sc
 
 def extend_block_tables(block_tables: torch.Tensor, kv_lens: torch.Tensor, new_lens: torch.Tensor,
                         free_pages: torch.Tensor, pool: torch.Tensor, page_size: int, total: int, *,
-                        kv_lens_out: torch.Tensor | None = None,
-                        pool_out: torch.Tensor | None = None) -> BatchPlan:
+                        kv_lens_out: torch.Tensor | None = None, pool_out: torch.Tensor | None = None,
+                        max_len: int | None = None) -> BatchPlan:
     """Pages, slots and positions of a step in which request r gets ``new_lens[r]``
     more tokens, in one or two launches and without the host knowing the lengths.
 
@@ -99,9 +99,10 @@ def extend_block_tables(block_tables: torch.Tensor, kv_lens: torch.Tensor, new_l
     pages whose first entry and count are ``pool[0]`` and ``pool[1]`` (int32 [4];
     ``pool[2]`` counts refused requests), ``total`` the number of new tokens of all
     requests (fewer in fact: the rest get slot -1). A request whose table row is too
-    short, or that needs pages when the needs up to it exceed the pool, is refused:
-    it keeps its length and its tokens get slot -1. ``kv_lens_out`` and ``pool_out`` may
-    be ``kv_lens`` and ``pool``: the step is then taken in place."""
+    short, that would be longer than ``max_len``, or that needs pages when the needs up to
+    it exceed the pool, is refused: it keeps its length and its tokens get slot -1.
+    ``kv_lens_out`` and ``pool_out`` may be ``kv_lens`` and ``pool``: the step is then taken
+    in place."""
     dev = _hip(block_tables, "extend_block_tables")
     R = block_tables.shape[0]
     _tables(block_tables, dev, R)
@@ -112,17 +113,19 @@ def extend_block_tables(block_tables: torch.Tensor, kv_lens: torch.Tensor, new_l
         _ints(dev, R, kv_lens_out=kv_lens_out)
     if pool_out is not None:
         _ints(dev, 4, pool_out=pool_out)
+    assert max_len is None or max_len >= 0, "max_len may not be negative"
     cut = [R + 1, R, R + 1, total, total, R if kv_lens_out is None else 0, 4 if pool_out is None else 0]
     q_starts, first, fresh, positions, slots, lens, state = torch.empty(
         sum(cut), dtype=torch.int32, device=dev).split(cut)
     kv_lens_out = lens if kv_lens_out is None else kv_lens_out
     pool_out = state if pool_out is None else pool_out
     with _DeviceGuard(dev):
-        _lib.check(_lib.lib().pmi_extend_block_tables(
+        _lib.check(_lib.lib().pmi_extend_block_tables_upto(
             block_tables.data_ptr(), _row_stride(block_tables), kv_lens.data_ptr(), new_lens.data_ptr(),
             free_pages.data_ptr(), pool.data_ptr(), q_starts.data_ptr(), kv_lens_out.data_ptr(), first.data_ptr(),
             fresh.data_ptr(), positions.data_ptr(), slots.data_ptr(), pool_out.data_ptr(), R, block_tables.shape[1],
-            free_pages.numel(), page_size, total, _raw_stream(dev)), "pmi_extend_block_tables")
+            free_pages.numel(), page_size, (1 << 31) - 1 if max_len is None else max_len, total, _raw_stream(dev)),
+            "pmi_extend_block_tables")
     return BatchPlan(q_starts, kv_lens_out, first, fresh, positions, slots, pool_out)
 
 
@@ -152,7 +155,8 @@ def rope_append_kv(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, posi
     """Rotated q [T, H, D] of the fused rows ``qkv`` [T, (H + 2 KV) * D] (fp16 or bf16);
     the rotated k and the v of token t are quantised into slot ``slots[t]``.
 
-    ``cos``, ``sin`` fp32 [L, D/2], indexed by ``positions`` int32 [T]. Tokens with
+    ``cos``, ``sin`` fp32 [L, D/2], indexed by ``positions`` int32 [T] (one outside the
+    table takes its first or last row). Tokens with
     consecutive slots of one page form a run, and a page may be in one run only (as
     ``extend_block_tables`` makes them). A run raises its page's scale to what its values
     need; the page's older codes are rounded again to the new scale. Slots outside the
@@ -261,7 +265,8 @@ class PagedKVCache:
     """The paged 8-bit cache of a model's layers, with one block table for all of them.
 
     ``requests`` rows of up to ``max_len`` tokens share ``pages`` pages (default: enough
-    for all of them at full length). ``extend`` makes room for a step's new tokens,
+    for all of them at full length). ``extend`` makes room for a step's new tokens (never
+    past ``max_len``, so RoPE tables of as many positions do),
     ``append`` writes them layer by layer, ``attend`` reads, ``release`` gives a finished
     request's pages back. ``pool[2]`` counts requests that ``extend`` refused."""
 
@@ -278,7 +283,7 @@ class PagedKVCache:
         dev = torch.device(device)
         width = -(-max_len // page_size)
         pages = requests * width if pages is None else pages
-        self.page_size = page_size
+        self.page_size, self.max_len = page_size, max_len
         shape = (pages, kv_heads, page_size, head_dim)
         self.k = [torch.zeros(shape, dtype=torch.uint8, device=dev).view(dtype) for _ in range(layers)]
         self.v = [torch.zeros(pages, kv_heads, page_size // 16, head_dim, 16, dtype=torch.uint8,
@@ -300,7 +305,8 @@ class PagedKVCache:
     def extend(self, new_lens: torch.Tensor, total: int) -> BatchPlan:
         """``extend_block_tables`` in place."""
         return extend_block_tables(self.block_tables, self.kv_lens, new_lens, self.free_pages, self.pool,
-                                   self.page_size, total, kv_lens_out=self.kv_lens, pool_out=self.pool)
+                                   self.page_size, total, kv_lens_out=self.kv_lens, pool_out=self.pool,
+                                   max_len=self.max_len)
 
     def release(self, done: torch.Tensor) -> None:
         release_block_tables(self.block_tables, self.kv_lens, done, self.free_pages, self.pool, self.page_size)

@@ -831,3 +831,33 @@ def test_the_largest_window_hides_nothing(new, lens):
     assert want[-1].isfinite().all() and (want[-1] != 0).any()
     for window in (2 ** 31 - 1, 2 ** 31 - 2, 2 ** 30, 10 ** 6):
         assert torch.equal(_run(c, tables, lens, starts, q, window=window), want), window
+
+
+@gpu
+def test_requests_stop_at_max_len():
+    """A request may not grow past ``max_len``, also where its last page has room."""
+    c = P.PagedKVCache(1, 3, 100, 1, 64, DEV, page_size=64)
+    plan = c.extend(_ints([100, 90, 0]), 190)
+    assert c.kv_lens.tolist() == [100, 90, 0] and (plan.slots >= 0).all()
+    plan = c.extend(_ints([1, 10, 101]), 112)
+    assert plan.kv_lens.tolist() == [100, 100, 0] and c.pool[2].item() == 2
+    assert plan.first.tolist() == [-1, 90, -1]
+    slots = plan.slots.tolist()
+    assert slots[0] == -1 and min(slots[1:11]) >= 0 and slots[11:] == [-1] * 101
+    plan = c.extend(_ints([0, 1, 100]), 101)
+    assert c.kv_lens.tolist() == [100, 100, 100] and c.pool.tolist()[1:3] == [0, 3]
+    assert plan.slots.tolist()[0] == -1 and plan.positions.tolist()[1:] == list(range(100))
+    # the function itself: no limit but the row, or the one that is given
+    t, lens, free, pool = _ints([[0, -1]]), _ints([5]), _ints([0, 1, 2]), _ints([1, 2, 0, 0])
+    for limit, want in ((None, 32), (32, 32), (31, 5)):
+        plan = P.extend_block_tables(t.clone(), lens, _ints([27]), free, pool, 16, 27, max_len=limit)
+        assert plan.kv_lens.tolist() == [want] and plan.pool[2].item() == int(want == 5)
+    with pytest.raises(AssertionError):
+        P.extend_block_tables(t, lens, _ints([1]), free, pool, 16, 1, max_len=-1)
+
+
+def test_a_negative_max_len_is_refused():
+    a = dict(tables=P8, stride=8, lens=P8, new=P8, free=P8, pool=P8, starts=P8, out=P8, first=P8, fresh=P8, positions=P8,
+             slots=P8, pool_out=P8, R=2, width=8, ring=16, ps=16, max_len=-1, total=2)
+    assert _lib.lib().pmi_extend_block_tables_upto(*a.values(), None) == _lib.PMI_ERR_INVALID
+    assert "max_len" in _lib.last_error()
