@@ -300,7 +300,8 @@ class PagedKVCache:
         pages = self.free_pages.numel()
         self.kv_lens.zero_()
         torch.arange(pages, out=self.free_pages)
-        self.pool.copy_(torch.tensor([0, pages, 0, 0], dtype=torch.int32))
+        self.pool.zero_()
+        self.pool[1:2].fill_(pages)  # (from the host's memory it would wait for the device)
 
     def extend(self, new_lens: torch.Tensor, total: int) -> BatchPlan:
         """``extend_block_tables`` in place."""

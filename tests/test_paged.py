@@ -861,3 +861,44 @@ def test_a_negative_max_len_is_refused():
              slots=P8, pool_out=P8, R=2, width=8, ring=16, ps=16, max_len=-1, total=2)
     assert _lib.lib().pmi_extend_block_tables_upto(*a.values(), None) == _lib.PMI_ERR_INVALID
     assert "max_len" in _lib.last_error()
+
+
+@gpu
+def test_no_call_waits_for_the_device():
+    """Every call of a cache, under torch's check for synchronising ones, and captured."""
+    KV, D, T = 1, 64, 20
+    c = P.PagedKVCache(1, 2, 64, KV, D, DEV, page_size=16)
+    cos, sin = (torch.from_numpy(t).to(DEV) for t in _rope(64, D))
+    qkv = torch.randn(T, 3 * D, device=DEV).half()
+    new, done = _ints([13, 7]), torch.tensor([True, False], device=DEV)
+
+    def step():
+        c.reset()
+        plan = c.extend(new, T)
+        o = c.attend(0, c.append(0, qkv, cos, sin, plan), plan, scale=0.125, max_q_len=13)
+        P.read_kv_pages(c.free_pages, c.k[0], c.v[0], c.k_scale[0], c.v_scale[0])
+        c.release(done)
+        return o
+
+    step()
+    torch.cuda.synchronize()
+    mode = torch.cuda.get_sync_debug_mode()
+    torch.cuda.set_sync_debug_mode("error")
+    try:
+        want = step()
+    finally:
+        torch.cuda.set_sync_debug_mode(mode)
+    lens, pool, free = c.kv_lens.tolist(), c.pool.tolist(), c.free_pages.tolist()
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=s):
+            got = step()
+    torch.cuda.current_stream().wait_stream(s)
+    for _ in range(3):
+        c.extend(_ints([30, 30]), 60)  # something for reset to undo
+        graph.replay()
+        assert torch.equal(got, want)
+        assert (c.kv_lens.tolist(), c.pool.tolist(), c.free_pages.tolist()) == (lens, pool, free)
