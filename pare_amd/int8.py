@@ -123,7 +123,8 @@ def matmul_w8a8(x: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, *, bia
 class Int8Linear(nn.Module):
     """A linear layer in 8-bit integers: weights quantised once per output channel,
     activations per token at every call. Buffers ``weight`` int8 [out, in rounded up to
-    16], ``scale`` fp32 [out]; ``bias`` optional. Runs on the HIP device only."""
+    16], ``scale`` fp32 [out], which both keep their types when the module is converted
+    (``half()``, ``to(dtype)``); ``bias`` optional. Runs on the HIP device only."""
 
     def __init__(self, weight: torch.Tensor, scale: torch.Tensor, in_features: int,
                  bias: torch.Tensor | None = None) -> None:
@@ -137,6 +138,15 @@ class Int8Linear(nn.Module):
         self.register_buffer("weight", weight.contiguous())
         self.register_buffer("scale", scale.float())
         self.bias = nn.Parameter(bias.detach().clone()) if bias is not None else None
+
+    def _apply(self, fn, recurse=True):
+        # conversions of a model's floating-point tensors reach the scale as well: fp16 would round it,
+        # and lose what lies under 2^-24
+        scale = self.scale
+        super()._apply(fn, recurse)
+        if self.scale.dtype != torch.float32:
+            self.scale = scale.to(self.scale.device)
+        return self
 
     @classmethod
     def from_weight(cls, weight: torch.Tensor, bias: torch.Tensor | None = None) -> "Int8Linear":

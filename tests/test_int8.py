@@ -246,3 +246,30 @@ def test_int8_linear(bias):
     assert torch.equal(again(x), y)
     cpu = P.Int8Linear.from_weight(lin.weight.detach().cpu())
     assert cpu.weight.device.type == "cpu" and torch.equal(cpu.weight, q.weight.cpu())
+
+
+def _codes(N, K, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    return torch.randint(-127, 128, (N, -(-K // 16) * 16), generator=g, dtype=torch.int8), torch.rand(N, generator=g) * 1e-5
+
+
+def test_scales_stay_fp32_when_the_module_changes_type():
+    """``half()`` and ``to(dtype)`` of a model convert the bias; the scales, which fp16 would
+    round or lose, and the codes stay."""
+    for convert in (lambda m: m.half(), lambda m: m.to(torch.bfloat16), lambda m: m.double(),
+                    lambda m: nn.Sequential(m).half()[0]):
+        codes, scale = _codes(5, 32)
+        m = convert(P.Int8Linear(codes, scale, 32, torch.ones(5)))
+        assert m.scale.dtype == torch.float32 and torch.equal(m.scale, scale)
+        assert m.weight.dtype == torch.int8 and torch.equal(m.weight, codes)
+        assert m.bias.dtype != torch.float32
+        assert m.state_dict()["scale"].dtype == torch.float32
+
+
+@gpu
+def test_a_converted_module_gives_the_same():
+    lin = nn.Linear(256, 40).half().to(DEV)
+    m = P.Int8Linear.from_linear(lin)
+    x = _rows(3, 256, torch.float16, 1).to(DEV)
+    want = m(x)
+    assert torch.equal(m.half()(x), want) and torch.equal(nn.Sequential(m).to(torch.float16)(x), want)
