@@ -543,7 +543,7 @@ class QuantizedDecoder(nn.Module):
             self.lm_head = None
 
     def _head(self, n: torch.Tensor) -> torch.Tensor:
-        return F.linear(n, self.lm_head) if self.int8_head is None else self.int8_head(n)
+        return F.linear(n, self.lm_head) if self.int8_head is None else self.int8_head(n.detach())
 
     def rope_tables(self, max_len: int):
         return rope_tables(self.cfg.head_dim, self.cfg.rope_theta, max_len, self.embed.device)

@@ -124,7 +124,8 @@ class Int8Linear(nn.Module):
     """A linear layer in 8-bit integers: weights quantised once per output channel,
     activations per token at every call. Buffers ``weight`` int8 [out, in rounded up to
     16], ``scale`` fp32 [out], which both keep their types when the module is converted
-    (``half()``, ``to(dtype)``); ``bias`` optional. Runs on the HIP device only."""
+    (``half()``, ``to(dtype)``); ``bias`` optional. Runs on the HIP device only, and forward only: the
+    bias takes no gradient, and an input that needs one is refused."""
 
     def __init__(self, weight: torch.Tensor, scale: torch.Tensor, in_features: int,
                  bias: torch.Tensor | None = None) -> None:
@@ -137,7 +138,7 @@ class Int8Linear(nn.Module):
         self.out_features = weight.shape[0]
         self.register_buffer("weight", weight.contiguous())
         self.register_buffer("scale", scale.float())
-        self.bias = nn.Parameter(bias.detach().clone()) if bias is not None else None
+        self.bias = nn.Parameter(bias.detach().clone(), requires_grad=False) if bias is not None else None
 
     def _apply(self, fn, recurse=True):
         # conversions of a model's floating-point tensors reach the scale as well: fp16 would round it,
@@ -165,8 +166,10 @@ class Int8Linear(nn.Module):
         if not x.is_cuda:
             raise RuntimeError("pare_amd.Int8Linear runs on the HIP device only (no CPU fallback); move the module "
                                "and input to cuda")
-        y = matmul_w8a8(x.reshape(-1, self.in_features), self.weight, self.scale,
-                        bias=None if self.bias is None else self.bias.detach())
+        if x.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError("pare_amd.Int8Linear has no backward pass: detach the input or call it under no_grad, "
+                               "its gradient would be left out")
+        y = matmul_w8a8(x.reshape(-1, self.in_features), self.weight, self.scale, bias=self.bias)
         return y.reshape(*x.shape[:-1], self.out_features)
 
     def extra_repr(self) -> str:

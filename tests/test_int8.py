@@ -273,3 +273,23 @@ def test_a_converted_module_gives_the_same():
     x = _rows(3, 256, torch.float16, 1).to(DEV)
     want = m(x)
     assert torch.equal(m.half()(x), want) and torch.equal(nn.Sequential(m).to(torch.float16)(x), want)
+
+
+def test_the_bias_is_no_leaf_to_train():
+    """The product has no backward pass, so no optimizer is offered the bias."""
+    codes, scale = _codes(5, 32)
+    m = P.Int8Linear(codes, scale, 32, torch.ones(5))
+    assert not any(p.requires_grad for p in m.parameters())
+
+
+@gpu
+def test_an_input_that_needs_a_gradient_is_refused():
+    m = P.Int8Linear.from_linear(nn.Linear(64, 8).to(DEV))
+    x = torch.randn(2, 64, device=DEV, requires_grad=True)
+    with pytest.raises(RuntimeError, match="gradient"):
+        m(x)
+    with torch.no_grad():
+        y = m(x)
+    assert torch.equal(m(x.detach()), y)
+    with torch.inference_mode():
+        assert torch.equal(m(x), y)

@@ -288,3 +288,16 @@ def test_int8_output_head():
     assert torch.equal(out, again)
     prompt = torch.stack(_prompts([12, 12]))
     assert torch.equal(model.generate(prompt, 6)[0], model.generate(prompt, 6, use_graph=False)[0])
+
+
+def test_the_unfused_decoder_runs_with_an_int8_head_outside_no_grad():
+    """Its plain ops record a graph up to the head, which has no backward pass."""
+    model = QuantizedDecoder(SMALL, DEV, seed=7, fused_ops=False)
+    model.quantize_head()
+    cos, sin = model.rope_tables(8)
+    tokens = torch.arange(8, device=DEV)[None]
+    args = (tokens, cos, sin, model.new_cache(1, 8), torch.arange(8, device=DEV), None, True)
+    with torch.no_grad():
+        want = model.forward_tokens(*args)
+    got = model.forward_tokens(*args)
+    assert not got.requires_grad and torch.equal(got, want)
