@@ -19,6 +19,10 @@ Differences from the reference, all additive:
     buffers on a device.
   - act_order layers keep their ``<layer>.g_idx`` tensor (int32 [in]); the
     metadata records ``has_g_idx``.
+  - ``Int8Linear`` layers (8-bit integer products) are recorded under
+    ``int8_layers`` (``{name: {in_features, out_features, has_bias}}``) and come back
+    as such; the reference's loader would put their codes into a float weight, so
+    ``save_quantized`` warns.
   - ``save_quantized(..., kernel_layout=True)`` also stores each layer's
     derived kernel-layout weight as ``<layer>.packed_weight_kernel`` and
     records ``kernel_layout_version``; a loader with the same version takes it
@@ -36,6 +40,7 @@ import torch
 import torch.nn as nn
 
 from .config import QuantConfig
+from .int8 import Int8Linear
 from .linear import QuantizedLinear
 
 PARE_CONFIG_FILE = "pare_config.json"
@@ -53,8 +58,12 @@ def save_quantized(model: nn.Module, path, kernel_layout: bool = False) -> None:
     path = Path(path)
     path.mkdir(parents=True, exist_ok=True)
     layers: dict[str, dict] = {}
+    int8: dict[str, dict] = {}
     extra: dict[str, torch.Tensor] = {}
     for name, m in model.named_modules():
+        if isinstance(m, Int8Linear):
+            int8[name] = {"in_features": m.in_features, "out_features": m.out_features,
+                          "has_bias": m.bias is not None}
         if isinstance(m, QuantizedLinear):
             layers[name] = {
                 "bits": m.config.bits,
@@ -77,7 +86,10 @@ def save_quantized(model: nn.Module, path, kernel_layout: bool = False) -> None:
         warnings.warn(f"save_quantized: {len(act_order)} act_order layer(s) (first: {act_order[0]}) "
                       "carry g_idx; the reference's load_quantized ignores it and would "
                       "dequantize them with contiguous groups", stacklevel=2)
-    if not layers:
+    if int8:
+        warnings.warn(f"save_quantized: {len(int8)} 8-bit layer(s) (first: {next(iter(int8))}) that the "
+                      "reference's load_quantized does not know", stacklevel=2)
+    if not layers and not int8:
         raise ValueError("save_quantized: the model holds no QuantizedLinear layer to save "
                          "(quantize it before saving)")
     # one copy per storage (tied weights, pare/model/io.py:92-107)
@@ -91,6 +103,8 @@ def save_quantized(model: nn.Module, path, kernel_layout: bool = False) -> None:
             tensors[k] = v
     save_file(tensors, str(path / TENSORS_FILE))
     meta = {"pare_version": "pare_amd", "quantized_layers": layers}
+    if int8:
+        meta["int8_layers"] = int8
     if kernel_layout:
         meta["kernel_layout_version"] = KERNEL_LAYOUT_VERSION
     (path / PARE_CONFIG_FILE).write_text(json.dumps(meta, indent=2))
@@ -103,9 +117,9 @@ def replace_module(root: nn.Module, dotted: str, new: nn.Module) -> None:
 
 
 def load_quantized(model: nn.Module, path, use_kernel: bool = True, device=None) -> nn.Module:
-    """Rebuilds the QuantizedLinear layers of ``path`` in ``model`` and loads
-    the other tensors (pare/model/io.py:130-196). INT4 layers only: this
-    package implements the INT4 kernel path."""
+    """Rebuilds the QuantizedLinear and Int8Linear layers of ``path`` in ``model`` and
+    loads the other tensors (pare/model/io.py:130-196). Of the reference's layers INT4
+    only: this package implements the INT4 kernel path."""
     from safetensors.torch import load_file
 
     path = Path(path)
@@ -130,7 +144,12 @@ def load_quantized(model: nn.Module, path, use_kernel: bool = True, device=None)
         if stored_layout and w_k is not None and ql.packed_weight.is_cuda:
             ql.adopt_kernel_layout(w_k)
         replace_module(model, name, ql)
-    prefixes = tuple(n + "." for n in layers)
+    int8: dict[str, dict] = meta.get("int8_layers", {})
+    for name, lm in int8.items():
+        pre = name + "."
+        replace_module(model, name, Int8Linear(tensors[pre + "weight"], tensors[pre + "scale"], lm["in_features"],
+                                               tensors.get(pre + "bias")))
+    prefixes = tuple(n + "." for n in [*layers, *int8])
     rest = {k: v for k, v in tensors.items() if not k.startswith(prefixes)}
     model.load_state_dict(rest, strict=False)
     return model

@@ -293,3 +293,41 @@ def test_an_input_that_needs_a_gradient_is_refused():
     assert torch.equal(m(x.detach()), y)
     with torch.inference_mode():
         assert torch.equal(m(x), y)
+
+
+def test_models_with_int8_layers_are_saved_and_loaded(tmp_path):
+    """``save_quantized`` and ``load_quantized`` of a model that holds both kinds of layer: the
+    codes come back as codes, not as the float weight of what stood there."""
+    config = P.QuantConfig(bits=4, scheme="rtn", group_size=32)
+    g = torch.Generator().manual_seed(0)
+
+    def four(n, k):
+        return P.QuantizedLinear(torch.randint(0, 256, (n, k // 2), generator=g, dtype=torch.uint8),
+                                 torch.rand(n, k // 32, 1, generator=g), torch.full((n, k // 32, 1), 8.0), config, None, k, n)
+
+    def eight(n, k, bias):
+        return P.Int8Linear(*_codes(n, k, n), k, torch.randn(n, generator=g) if bias else None)
+
+    model = nn.ModuleDict({"a": four(64, 64), "b": eight(48, 64, True), "c": nn.ModuleDict({"d": eight(32, 40, False)}),
+                           "e": nn.Linear(8, 8)})
+    with pytest.warns(UserWarning, match="8-bit"):
+        P.save_quantized(model, tmp_path)
+    for other in (nn.ModuleDict({"a": nn.Linear(64, 64), "b": nn.Linear(64, 48),
+                                 "c": nn.ModuleDict({"d": nn.Linear(40, 32, bias=False)}), "e": nn.Linear(8, 8)}),
+                  nn.ModuleDict({"a": four(64, 64), "b": eight(48, 64, True),
+                                 "c": nn.ModuleDict({"d": eight(32, 40, False)}), "e": nn.Linear(8, 8)})):
+        got = P.load_quantized(other, tmp_path)
+        assert isinstance(got["b"], P.Int8Linear) and isinstance(got["c"]["d"], P.Int8Linear)
+        assert got["c"]["d"].in_features == 40 and got["c"]["d"].out_features == 32 and got["c"]["d"].bias is None
+        assert isinstance(got["a"], P.QuantizedLinear) and isinstance(got["e"], nn.Linear)
+        have, want = got.state_dict(), model.state_dict()
+        assert have.keys() == want.keys()
+        assert all(have[n].dtype == want[n].dtype and torch.equal(have[n], want[n]) for n in want)
+    # 8-bit layers alone
+    alone = nn.ModuleDict({"b": eight(48, 64, True)})
+    with pytest.warns(UserWarning, match="8-bit"):
+        P.save_quantized(alone, tmp_path / "alone")
+    got = P.load_quantized(nn.ModuleDict({"b": nn.Linear(64, 48)}), tmp_path / "alone")
+    assert torch.equal(got["b"].weight, alone["b"].weight)
+    with pytest.raises(ValueError):
+        P.save_quantized(nn.Linear(4, 4), tmp_path / "none")
