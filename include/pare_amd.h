@@ -654,8 +654,8 @@ PMI_API int pmi_read_kv_pages(const int32_t* pages, const void* k_cache, const v
  * kv_lens[r] keys, its own among them: query i of n sees positions p <= kv_lens[r] -
  * n + i, and with window > 0 only the last `window` of them. A query that sees
  * nothing gives zeros; rows of out from q_starts[R] on stay as they were.
- * Scales are not negative (as the write leaves them); one that is infinite or NaN
- * makes what sees its page NaN.
+ * The cache's scales are not negative (as the write leaves them); one that is infinite or
+ * NaN makes what sees its page NaN. `scale` is finite.
  * max_q and max_kv bound the queries and keys of a request (of a longer one the
  * queries past max_q stay unwritten, and keys past max_kv unread); H / KV <= 64;
  * width * page_size <= 2^30; R KV (max_kv / 64 + 5) ceil(min(max_q H / KV, 64) / 16) < 2^31.

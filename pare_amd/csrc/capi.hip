@@ -7,6 +7,7 @@
 #include <string.h>
 
 #include <atomic>
+#include <cmath>
 #include <mutex>
 
 #include "paged.h"
@@ -1498,6 +1499,7 @@ int pmi_paged_attention(const void* q, int dtype, int64_t q_stride, int64_t q_he
   if (!q_starts && T != R)
     return fail(PMI_ERR_INVALID, "%s: without q_starts every request has one query (T=%lld R=%lld)", fn, (long long)T,
                 (long long)R);
+  if (!std::isfinite(scale)) return fail(PMI_ERR_INVALID, "%s: scale must be finite", fn);
   if (H / KV > 64)
     return fail(PMI_ERR_UNSUPPORTED, "%s: at most 64 query heads per KV head (got %lld)", fn, (long long)(H / KV));
   if (q_stride % 8 != 0 || q_head_stride % 8 != 0)

@@ -902,3 +902,22 @@ def test_no_call_waits_for_the_device():
         graph.replay()
         assert torch.equal(got, want)
         assert (c.kv_lens.tolist(), c.pool.tolist(), c.free_pages.tolist()) == (lens, pool, free)
+
+
+@pytest.mark.parametrize("scale", [float("nan"), float("inf"), -float("inf"), 1e39])
+def test_a_scale_that_is_not_finite_is_refused(scale):
+    rc = _lib.lib().pmi_paged_attention(*_attention_args(scale=scale))
+    assert rc == _lib.PMI_ERR_INVALID and "scale" in _lib.last_error()
+
+
+@gpu
+@pytest.mark.parametrize("new", [1, 40])
+@pytest.mark.parametrize("scale", [-0.1, 1e-6])
+def test_negative_and_small_scales(scale, new):
+    lens = [200, 65, 330]
+    c, tables, starts, q = _attention_case(CODES[0], torch.bfloat16, 4, 1, 128, 32, lens, [new] * 3)
+    k, v, ks, vs = c.tensors(DEV)
+    got = P.paged_attention(q.to(DEV), k, v, ks, vs, torch.from_numpy(tables).to(DEV), _ints(lens),
+                            torch.from_numpy(starts).to(DEV), scale=scale, max_q_len=new)
+    _check_finite(got, *S.attention(q.double().numpy(), c.values(0), c.values(1), tables, lens, starts, 32, scale),
+                  torch.bfloat16)
