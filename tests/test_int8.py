@@ -331,3 +331,23 @@ def test_models_with_int8_layers_are_saved_and_loaded(tmp_path):
     assert torch.equal(got["b"].weight, alone["b"].weight)
     with pytest.raises(ValueError):
         P.save_quantized(nn.Linear(4, 4), tmp_path / "none")
+
+
+@gpu
+@pytest.mark.parametrize("M,N,K,dtype,bias", [
+    # 256 x 256 tiles, two or three a workgroup, ragged on both sides
+    (300, 70001, 144, torch.bfloat16, True), (1100, 33001, 272, torch.float16, False),
+    (520, 33003, 400, torch.float32, True),
+    # 128 x 128 tiles, two a workgroup
+    (130, 64900, 272, torch.float16, True), (129, 60001, 128, torch.float32, False),
+    # up to 64 rows with 32 and 64 weight rows a workgroup
+    (1, 5200, 1040, torch.float16, True), (6, 5200, 528, torch.bfloat16, False), (16, 12400, 1040, torch.float16, True),
+    (17, 5200, 1040, torch.bfloat16, True), (17, 12401, 528, torch.float16, False), (40, 5201, 528, torch.float32, True),
+    (40, 12400, 1040, torch.bfloat16, False), (64, 5200, 528, torch.float16, True), (64, 12403, 1040, torch.float16, True)])
+def test_matmul_of_every_tile(M, N, K, dtype, bias):
+    """The forms that only wide products take."""
+    x, w, sw, b, want, mag = _case(M, N, K, dtype, bias)
+    y = P.matmul_w8a8(x, w, sw, bias=b)
+    assert y.isfinite().all()
+    _check(y, want, mag, dtype)
+    assert torch.equal(y, P.matmul_w8a8(x, w, sw, bias=b))

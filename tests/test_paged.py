@@ -702,7 +702,7 @@ def test_attention_of_small_queries_and_small_keys(size, keys, new):
     flat = P.paged_attention(q.to(DEV), k, v, ks, vs, torch.from_numpy(tables).to(DEV), _ints(lens),
                              torch.from_numpy(starts).to(DEV), scale=0.0, max_q_len=new)
     _check_finite(flat, *S.attention(np.zeros(q.shape), c.values(0), c.values(1), tables, lens, starts, ps, 0.0),
-           torch.bfloat16)
+                  torch.bfloat16)
 
 
 @gpu
@@ -921,3 +921,89 @@ def test_negative_and_small_scales(scale, new):
                             torch.from_numpy(starts).to(DEV), scale=scale, max_q_len=new)
     _check_finite(got, *S.attention(q.double().numpy(), c.values(0), c.values(1), tables, lens, starts, 32, scale),
                   torch.bfloat16)
+
+
+# --- forms that only larger calls take ----------------------------------------------------
+
+@gpu
+@pytest.mark.parametrize("code,dtype,ps", [(CODES[0], torch.float16, 16), (CODES[1], torch.bfloat16, 128),
+                                           (CODES[1], torch.float16, 32), (CODES[0], torch.bfloat16, 256)])
+def test_append_of_many_tokens_equals_the_oracle(code, dtype, ps):
+    """More than 1024 tokens (several a workgroup, whose runs end in the next ones' tokens):
+    ragged prompts behind contexts, refused requests among them, slots outside the cache."""
+    H, KV, D = 2, 1, 64 if ps == 32 else 128
+    rng = np.random.default_rng(ps)
+    lens, new = [0, 5, ps, 3 * ps - 1, 0, 70], [ps + 3, 403, 1, 299, 333, 517]
+    refused = 4
+    need = [-(-(a + b) // ps) for a, b in zip(lens, new)]
+    pages = sum(need)
+    c = S.Cache(pages, KV, ps, D, code)
+    c.fill(rng)
+    k, v, ks, vs = c.tensors(DEV)
+    order, at, slots, positions = rng.permutation(pages), 0, [], []
+    for r, (a, n) in enumerate(zip(lens, new)):
+        row = order[at:at + need[r]]
+        at += need[r]
+        p = np.arange(a, a + n)
+        positions.append(p)
+        slots.append(np.full(n, -1) if r == refused else row[p // ps] * ps + p % ps)
+        if r == 1:
+            slots[-1][17:19] = pages * ps + 5, -7
+    slots, positions = np.concatenate(slots).astype(np.int32), np.concatenate(positions).astype(np.int32)
+    T = len(slots)
+    assert T > 1024
+    # a run ends where the slots do: the tokens behind the hole begin another one of the same page, which
+    # no caller makes; the page is left out of both
+    hole = int(slots[new[0] + 16]) // ps
+    slots[slots // ps == hole] = -1
+    cos, sin = _rope(1200, D)
+    x = torch.from_numpy(rng.standard_normal((T, (H + 2 * KV) * D)) * (0.2 + 3 * rng.random((T, 1)))).to(dtype)
+    q = P.rope_append_kv(x.to(DEV), torch.from_numpy(cos).to(DEV), torch.from_numpy(sin).to(DEV),
+                         torch.from_numpy(positions).to(DEV), torch.from_numpy(slots).to(DEV), k, v, ks, vs)
+    want = c.append(x.float().numpy(), cos, sin, positions, slots, H)
+    assert torch.equal(q.cpu(), torch.from_numpy(want).to(dtype))
+    _check_cache(c, k, v, ks, vs)
+
+
+@gpu
+@pytest.mark.parametrize("window", [1100, 2500])
+@pytest.mark.parametrize("D,code", [(64, CODES[1]), (128, CODES[0])])
+def test_windows_over_several_ranges_of_keys(D, code, window):
+    """Many query rows whose window is cut into ranges that are joined."""
+    lens, new = [6000, 1300, 3011], [200, 40, 17]
+    c, tables, starts, q = _attention_case(code, torch.float16, 8, 2, D, 64, lens, new)
+    _check_finite(_run(c, tables, lens, starts, q, window=window),
+                  *_oracle(c, tables, lens, starts, q, window), torch.float16)
+    alone = _run(c, tables[:1], lens[:1], starts[:2], q[:200], window=window)
+    _check_finite(alone, *_oracle(c, tables[:1], lens[:1], starts[:2], q[:200], window), torch.float16)
+
+
+@gpu
+def test_a_cache_past_32_bits_of_bytes():
+    """The last pages of a cache of 5 GiB each for keys and values: written, read, attended to
+    by a prompt and by a single token."""
+    H, KV, D, ps, pages = 4, 4, 128, 256, 40960
+    k = torch.zeros(pages, KV, ps, D, dtype=torch.int8, device=DEV)
+    v = torch.zeros(pages, KV, ps // 16, D, 16, dtype=torch.int8, device=DEV)
+    ks, vs = torch.zeros(pages, KV, device=DEV), torch.zeros(pages, KV, device=DEV)
+    T, rows = 300, [pages - 1, pages - 2]
+    c = S.Cache(2, KV, ps, D, torch.int8)  # the same two pages alone
+    rng = np.random.default_rng(0)
+    x = torch.from_numpy(rng.standard_normal((T, (H + 2 * KV) * D))).half()
+    cos, sin = _rope(T, D)
+    p = np.arange(T)
+    want = c.append(x.float().numpy(), cos, sin, p, p, H)
+    slots = np.array(rows)[p // ps] * ps + p % ps
+    q = P.rope_append_kv(x.to(DEV), torch.from_numpy(cos).to(DEV), torch.from_numpy(sin).to(DEV),
+                         _ints(p.tolist()), _ints(slots.tolist()), k, v, ks, vs)
+    assert torch.equal(q.cpu(), torch.from_numpy(want).half())
+    at = torch.tensor(rows, device=DEV)
+    _check_cache(c, k[at], v[at], ks[at], vs[at])
+    rk, rv = P.read_kv_pages(_ints(rows), k, v, ks, vs, dtype=torch.float32)
+    for got, i in ((rk, 0), (rv, 1)):
+        assert torch.equal(got.cpu(), torch.from_numpy(S.decode(c.codes[i], c.dtype) * c.scales[i][..., None, None]))
+    tables = np.array([[0, 1]], np.int32)
+    for n in (1, T):
+        starts = np.array([0, n], np.int32)
+        got = P.paged_attention(q[-n:], k, v, ks, vs, _ints([rows]), _ints([T]), _ints([0, n]), scale=1 / 128 ** 0.5)
+        _check_finite(got, *_oracle(c, tables, [T], starts, q[-n:].cpu()), torch.float16)
