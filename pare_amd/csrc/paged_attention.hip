@@ -184,13 +184,37 @@ PMI_DEV void join(float& m, float& l, f32x4& o, float pm, float pl, f32x4 po, bo
 }
 
 constexpr float kLog2e = 1.4426950408889634f;
-// Probabilities are held in fp16 times kPBias. The reference that the scores are taken off is not
-// raised to a new maximum before this is 2^kSlack times what it was (and the unit of the values'
-// scales not before they have doubled): raising it rescales all sums, and some row of a tile has a
-// new maximum more often than not. 2^8 2^6 2 < 65504, and what is lost under fp16's range is
-// below 2^-25 / 2^8 of the largest probability.
-// The unit begins at kLeastUnit, so that its inverse is finite: values under 2^-24 of it are lost.
-constexpr float kPBias = 256.f, kSlack = 6.f, kLeastUnit = 1e-30f;
+// Probabilities, times their page's value scale, are held in fp16: as 2^kPBias of the largest of
+// them that the row has seen (2^weight), so that neither a page of large values without weight nor
+// one that the row does not see pushes the others out of fp16's range. Neither that reference nor
+// the one that the scores are taken off (2^max) is raised before it has grown 2^kSlack-fold: raising one
+// rescales all sums, and some row of a tile has a new maximum more often than not. 2^8 2^6 < 65504, and
+// what is lost under fp16's range is below 2^-25 / 2^8 of the largest product.
+// weight is at least max + kLeastWeight, so that their quotient is finite: values under 2^-24 of
+// 2^kLeastWeight are lost.
+constexpr float kPBias = 8.f, kSlack = 6.f, kLeastWeight = -100.f;
+
+// The two references of a row, and what they make of the values' scales. All -inf: nothing seen.
+struct Row {
+  float max = -INFINITY, weight = -INFINITY;
+  float gain = 0.f;  // 2^(max - weight + kPBias)
+};
+// Raises them; what the row's sum and its accumulators have to be multiplied with.
+struct Rescale {
+  float sum, acc;
+};
+PMI_DEV Rescale raise(Row& r, float max, float weight) {
+  weight = fmaxf(fmaxf(r.weight, weight), max + kLeastWeight);
+  const Rescale f = {r.max == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(r.max - max),
+                     r.weight == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(r.weight - weight)};
+  r.max = max, r.weight = weight;
+  r.gain = max == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(max - weight + kPBias);
+  return f;
+}
+// What the accumulators count in.
+PMI_DEV float unit_of(const Row& r) { return r.max == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(r.weight - r.max - kPBias); }
+// A finite scale's share of a probability (weights under 2^-126 have none, whatever their values).
+PMI_DEV float share_of(float scale, const Row& r) { return fminf(scale * r.gain, FLT_MAX); }
 
 // ---- few query rows ------------------------------------------------------------------
 // Requests of few query rows (tokens x heads of one KV head): bound by the bytes of the
@@ -208,8 +232,7 @@ constexpr float kPBias = 256.f, kSlack = 6.f, kLeastUnit = 1e-30f;
 //   O^T = V^T P^T: a lane's operand of P is then what it holds, and that of V its 16-byte
 //     piece of the page's block (one dimension, 16 tokens).
 // Scales: a lane's 16 tokens share theirs, so ks multiplies the scores and vs the
-// probabilities, in fp32, before these become fp16: times vs / (largest vs so far) and
-// 2^14, so that they use fp16's range from the top.
+// probabilities, in fp32, before these become fp16.
 //
 // An item that several workgroups share is joined by the last of them to arrive, in
 // order. A workgroup shares at most two items: the one it begins in (record 2 w) and the one
@@ -338,7 +361,8 @@ PMI_DEV void few_rows(const AttnArgs& a, FewLds<D>& lds, int wg) {
   f32x4 acc[DT];
 #pragma unroll
   for (int d = 0; d < DT; ++d) acc[d] = f32x4{0.f, 0.f, 0.f, 0.f};
-  float m = -INFINITY, sum = 0.f, vref = kLeastUnit;
+  Row ref;
+  float sum = 0.f;
   const int64_t cell_bytes = (int64_t)a.ps * D;
 
   // Look-ups run ahead: a tile's entry of the table (of the lane's 16 tokens, block h) is loaded
@@ -396,15 +420,6 @@ PMI_DEV void few_rows(const AttnArgs& a, FewLds<D>& lds, int wg) {
       entry = look_up(p + 512);
       load_k(next_page, p + 256);
     }
-    // the unit of acc: the largest value scale so far, or half of it
-    const float top = fmaxf(vref, max_over_h(tvs < INFINITY ? tvs : 0.f));
-    if (__any(top > 2.f * vref)) {
-      const float f = vref / top;
-#pragma unroll
-      for (int d = 0; d < DT; ++d) acc[d] *= f;
-      vref = top;
-    }
-    const float vs = tvs * (kPBias / vref);
     const bool masked = p < safe_lo || p + 64 > safe_hi || p + 64 > p1 || __any(gone);
     const int at = p + 16 * h;
     float x[16];
@@ -417,16 +432,16 @@ PMI_DEV void few_rows(const AttnArgs& a, FewLds<D>& lds, int wg) {
     float mx = x[0];
 #pragma unroll
     for (int e = 1; e < 16; ++e) mx = fmaxf(mx, x[e]);
+    const float most = max_over_h(mx + __builtin_amdgcn_logf(tvs < INFINITY ? tvs : 0.f));
     mx = max_over_h(mx);
-    const float nm = fmaxf(m, mx);
-    if (__any(nm > m + kSlack)) {
-      const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - nm);
-      sum *= f;
+    const float nm = fmaxf(ref.max, mx);
+    if (__any(nm > ref.max + kSlack || most > ref.weight + kSlack)) {
+      const Rescale f = raise(ref, nm, most);
+      sum *= f.sum;
 #pragma unroll
-      for (int d = 0; d < DT; ++d) acc[d] *= f;
-      m = nm;
+      for (int d = 0; d < DT; ++d) acc[d] *= f.acc;
     }
-    const float base = m == -INFINITY ? 0.f : m;
+    const float vs = share_of(tvs, ref), base = ref.max == -INFINITY ? 0.f : ref.max;
     f16x8 pw[2];
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
@@ -464,11 +479,11 @@ PMI_DEV void few_rows(const AttnArgs& a, FewLds<D>& lds, int wg) {
 
   // the four waves' results, joined in their order
   sum = sum_over_h(sum);
-  const float unit = vref * (1.f / kPBias);
+  const float unit = unit_of(ref);
 #pragma unroll
   for (int d = 0; d < DT; ++d)
     if (live) *reinterpret_cast<f32x4*>(&s_acc[wave][c][16 * d + 4 * h]) = acc[d] * unit;
-  if (h == 0) s_m[wave][c] = m, s_l[wave][c] = sum;
+  if (h == 0) s_m[wave][c] = ref.max, s_l[wave][c] = sum;
   __syncthreads();
   constexpr int kPer = D / 16;  // dimensions per thread: 16 threads a row
   const int orow = tid >> 4, od = (tid & 15) * kPer;
@@ -732,7 +747,8 @@ PMI_DEV void many_rows(const AttnArgs& a, uint8_t* lds, int& s_last, int wg) {
   for (int d = 0; d < D / 32; ++d)
 #pragma unroll
     for (int e = 0; e < 16; ++e) acc[d][e] = 0.f;
-  float m = -INFINITY, sum = 0.f, vref = kLeastUnit, vinv = kPBias / kLeastUnit;
+  Row ref;
+  float sum = 0.f;
   const int32_t* table = a.tables + (int64_t)r * a.stride;
   const int64_t cell_bytes = (int64_t)a.ps * D;
 
@@ -820,15 +836,6 @@ PMI_DEV void many_rows(const AttnArgs& a, uint8_t* lds, int& s_last, int wg) {
       const bool gone = cur.page < 0;
       float ks = gone ? 0.f : cur.ks, vs = gone ? 0.f : cur.vs;
       const bool bad = !(ks < INFINITY) || !(vs < INFINITY);
-      // the unit of acc: the largest value scale so far, or half of it
-      const float top = fmaxf(vref, max_of_4(vs < INFINITY ? vs : 0.f));
-      if (__any(top > 2.f * vref)) {
-        const float f = vref / top;
-#pragma unroll
-        for (int d = 0; d < D / 32; ++d) acc[d] *= f;
-        vref = top;
-        vinv = kPBias / vref;
-      }
       // result 16 u + 4 j + e: token 32 u + 16 (j / 2) + 8 h + 4 (j % 2) + e, block 2 u + j / 2.
       // Hidden tokens get -inf, which stays one through the factors k1 (at least FLT_MIN).
       if (p < safe_lo || p + 64 > safe_hi || p + 64 > p1 || __any(gone)) {
@@ -851,12 +858,12 @@ PMI_DEV void many_rows(const AttnArgs& a, uint8_t* lds, int& s_last, int wg) {
             s[b >> 1][8 * (b & 1) + e] = t == -INFINITY || !(which >> b & 1) ? t : __builtin_nanf("");
           }
       }
-      const float vsv = vs * vinv;
+      const float vlog = __builtin_amdgcn_logf(vs);
       // (FLT_MIN after all factors, the query's power of two among them; the sums are below 2^33, so what
       // it raises is a score of 0 all the same)
-      float k1[4], v1[4];
+      float k1[4];
 #pragma unroll
-      for (int b = 0; b < 4; ++b) k1[b] = fmaxf(of_block(ks, b) * qmul, FLT_MIN), v1[b] = of_block(vsv, b);
+      for (int b = 0; b < 4; ++b) k1[b] = fmaxf(of_block(ks, b) * qmul, FLT_MIN);
       float mx = -INFINITY;
 #pragma unroll
       for (int b = 0; b < 4; ++b) {
@@ -866,13 +873,22 @@ PMI_DEV void many_rows(const AttnArgs& a, uint8_t* lds, int& s_last, int wg) {
         mx = fmaxf(mx, t * k1[b]);
       }
       mx = fmaxf(mx, __shfl_xor(mx, 32));
-      const float nm = fmaxf(m, mx);
-      if (__any(nm > m + kSlack)) {
-        const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - nm);
-        sum *= f;
+      const float nm = fmaxf(ref.max, mx);
+      // (the largest product of the tile is at most the one of its largest score and its largest scale)
+      if (__any(nm > ref.max + kSlack || mx + max_of_4(vlog) > ref.weight + kSlack)) {
+        float most = -INFINITY;
 #pragma unroll
-        for (int d = 0; d < D / 32; ++d) acc[d] *= f;
-        m = nm;
+        for (int b = 0; b < 4; ++b) {
+          float t = s[b >> 1][8 * (b & 1)];
+#pragma unroll
+          for (int e = 1; e < 8; ++e) t = fmaxf(t, s[b >> 1][8 * (b & 1) + e]);
+          most = fmaxf(most, fmaf(t, k1[b], of_block(vlog, b)));
+        }
+        most = fmaxf(most, __shfl_xor(most, 32));
+        const Rescale f = raise(ref, nm, most);
+        sum *= f.sum;
+#pragma unroll
+        for (int d = 0; d < D / 32; ++d) acc[d] *= f.acc;
       }
       // The next tile to its slot (past the range: page 0 of the cache, never used), among the
       // exponentials: at the top of the loop this took 114.9 us instead of 112.1.
@@ -880,15 +896,16 @@ PMI_DEV void many_rows(const AttnArgs& a, uint8_t* lds, int& s_last, int wg) {
       const Blocks after = blocks_of(p + 128, entry);
       load_tile(p + 128, after);
       entry = look_up(p + 192);
-      const float base = m == -INFINITY ? 0.f : m;
+      const float base = ref.max == -INFINITY ? 0.f : ref.max;
 #pragma unroll
       for (int b = 0; b < 4; ++b) {
+        const float v1 = share_of(of_block(vs, b), ref);
         f16x8 pw;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const float ex = __builtin_amdgcn_exp2f(fmaf(s[b >> 1][8 * (b & 1) + e], k1[b], -base));
           sum += ex;
-          pw[e] = (f16)(ex * v1[b]);
+          pw[e] = (f16)(ex * v1);
         }
 #pragma unroll
         for (int d = 0; d < D / 32; ++d) {
@@ -904,7 +921,7 @@ PMI_DEV void many_rows(const AttnArgs& a, uint8_t* lds, int& s_last, int wg) {
 
   // result 4 j + e of tile d: dimension 32 d + 8 j + 4 h + e
   sum += __shfl_xor(sum, 32);
-  const float unit = vref * (1.f / kPBias);
+  const float unit = unit_of(ref);
   typedef T T4 __attribute__((ext_vector_type(4)));
   T* dst = (T*)a.out + ((int64_t)(start + i) * a.H + kh * G + row - i * G) * D + 4 * h;
   if (parts == 1) {
@@ -938,7 +955,7 @@ PMI_DEV void many_rows(const AttnArgs& a, uint8_t* lds, int& s_last, int wg) {
         __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, y), rp, rec + 4 * (32 * d + 8 * j + 4 * h), 0, kSc1);
       }
     if (h == 0) {
-      __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, m), rp, rec + 4 * D, 0, kSc1);
+      __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, ref.max), rp, rec + 4 * D, 0, kSc1);
       __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, sum), rp, rec + 4 * D + 4, 0, kSc1);
     }
   }

@@ -1007,3 +1007,36 @@ def test_a_cache_past_32_bits_of_bytes():
         starts = np.array([0, n], np.int32)
         got = P.paged_attention(q[-n:], k, v, ks, vs, _ints([rows]), _ints([T]), _ints([0, n]), scale=1 / 128 ** 0.5)
         _check_finite(got, *_oracle(c, tables, [T], starts, q[-n:].cpu()), torch.float16)
+
+
+@gpu
+@pytest.mark.parametrize("new", [1, 40])
+@pytest.mark.parametrize("where", ["first", "middle", "last"])
+@pytest.mark.parametrize("power,low", [(20, 130), (40, 130), (70, 130), (20, 10), (70, 40), (100, 10)])
+def test_pages_of_much_larger_values(power, low, where, new):
+    """A page whose values are 2^power times the others', with scores lower by about `low` (no
+    weight at all, or some of the output, or all of it), or which only the last queries see."""
+    lens, ps = [300, 64, 1000], 16
+    c, tables, starts, q = _attention_case(CODES[0], torch.bfloat16, 4, 1, 128, ps, lens, [new] * 3, spread=1.0)
+    q[..., 0] = 4.0
+    for r, n in enumerate(lens):
+        page = tables[r, {"first": 0, "middle": n // ps // 2, "last": (n - 1) // ps}[where]]
+        c.scales[1][page] *= np.float32(2.0 ** power)
+        if where != "last" or new == 1:
+            c.codes[0][page, :, :, 0] = 0x81
+            c.scales[0][page] = low * 128 ** 0.5 / (4 * 127)
+            c.codes[0][page, :, :, 1:] = 0
+    got = _run(c, tables, lens, starts, q)
+    o, weight = _oracle(c, tables, lens, starts, q)
+    # fp16 holds products of probabilities and scales as 2^8 of the largest and in steps of 2^-24: each is off
+    # by up to 2^-33 of that, up to 1000 of them with codes up to 127 by 2^-16, where a page of the
+    # largest products has codes of 0 (2^-15 of what half a code of it stands for)
+    for r in range(3):
+        big = int(np.argmax([c.scales[1][p, 0] for p in tables[r, :-(-lens[r] // ps)]]))
+        ones = np.zeros_like(c.values(1))
+        ones[tables[r, big]] = c.scales[1][tables[r, big], 0]
+        rows = slice(int(starts[r]), int(starts[r + 1]))
+        weight[rows] += S.attention(q[rows].double().numpy(), c.values(0), ones, tables[r:r + 1], lens[r:r + 1],
+                                    np.array([0, new]), ps, 1 / 128 ** 0.5)[0] * 2.0 ** -5
+    # (2^-16 of it is 2^-5 of what _tolerance takes from the weight, 2^-11)
+    _check_finite(got, o, weight, torch.bfloat16)
