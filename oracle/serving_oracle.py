@@ -131,20 +131,21 @@ def token_major(v_cache: torch.Tensor) -> np.ndarray:
     return np.ascontiguousarray(v.swapaxes(3, 4)).reshape(p, kv, 16 * b, d)
 
 
-def attention(q, k, v, tables, kv_lens, q_starts, ps, scale, window=0):
+def attention(q, k, v, tables, kv_lens, q_starts, ps, scale, window=0, max_kv=None):
     """(o, weight) in 64 bits: q [T, H, D] and the values k, v [pages, KV, ps, D]; weight =
-    sum p |v|, what a relative error of the probabilities moves o by. Rows behind the
-    last request are NaN."""
+    sum p |v|, what a relative error of the probabilities moves o by. Of a request of
+    more keys than max_kv, or than its row of tables holds, the first ones. Rows behind
+    the last request are NaN."""
     T, H, D = q.shape
     pages, KV = k.shape[:2]
     out, weight = np.full((T, H, D), np.nan), np.full((T, H, D), np.nan)
     for r, length in enumerate(kv_lens):
         a, b = q_starts[r], q_starts[r + 1]
-        length = min(max(length, 0), tables.shape[1] * ps)
-        n = b - a
+        length, n = max(length, 0), b - a
+        bound = tables.shape[1] * ps if max_kv is None else min(max_kv, tables.shape[1] * ps)
         for i in range(n):
             last = length - n + i
-            p = np.arange(max(0, last - window + 1) if window else 0, last + 1)
+            p = np.arange(max(0, last - window + 1) if window else 0, min(last + 1, bound))
             page = tables[r, p // ps] if len(p) else np.zeros(0, int)
             p, page = p[(page >= 0) & (page < pages)], page[(page >= 0) & (page < pages)]
             for h in range(H):

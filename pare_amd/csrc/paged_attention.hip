@@ -38,7 +38,7 @@ struct AttnArgs {
 // What a request's queries see, from its row of kv_lens and q_starts.
 struct Request {
   int start, n;       // its queries (none: nothing to do)
-  int len, shift;     // its keys; query i sees positions up to shift + i
+  int len, shift;     // its keys, of those within the bounds; query i sees positions up to shift + i
   int first_seen;     // the first position that its first query sees
   int lo, hi;         // positions that any of its queries sees: [lo, hi), lo a multiple of 16
 };
@@ -54,10 +54,10 @@ PMI_DEV Request request(const AttnArgs& a, int r) {
     q.n = a.q_starts[r + 1] - q.start;
   }
   q.len = min(min(max(len0, 0), a.max_kv), a.width * a.ps);
-  q.shift = q.len - q.n;  // (also of the queries past max_q)
+  q.shift = max(len0, 0) - q.n;  // (with the keys past the bounds and the queries past max_q)
   q.n = min(q.n, a.max_q);
   if (q.n < 0 || q.start < 0 || (int64_t)q.start + q.n > a.T) q.n = 0;
-  q.first_seen = first_position(a, q.shift);
+  q.first_seen = min(first_position(a, q.shift), q.len);
   q.lo = q.first_seen & ~15;
   q.hi = a.n_pages ? max(q.lo, min(q.len, q.shift + q.n)) : q.lo;
   return q;
@@ -702,7 +702,7 @@ PMI_DEV void many_rows(const AttnArgs& a, uint8_t* lds, int& s_last, int wg) {
   const int hi = live ? max(0, min(len, shift + i + 1)) : 0;
   const int lo = first_position(a, shift + i);
   const int i_first = rt * kRows / G, i_last = (rt * kRows + rows - 1) / G;
-  const int first_seen = first_position(a, shift + i_first), all_lo = first_seen & ~15;
+  const int first_seen = min(first_position(a, shift + i_first), len), all_lo = first_seen & ~15;
   const int all_hi = a.n_pages ? max(all_lo, min(len, shift + i_last + 1)) : all_lo;
   const int parts = max(1, (all_hi - all_lo + a.per - 1) / a.per);
   if (sp >= parts) return;

@@ -1040,3 +1040,20 @@ def test_pages_of_much_larger_values(power, low, where, new):
                                     np.array([0, new]), ps, 1 / 128 ** 0.5)[0] * 2.0 ** -5
     # (2^-16 of it is 2^-5 of what _tolerance takes from the weight, 2^-11)
     _check_finite(got, o, weight, torch.bfloat16)
+
+
+@gpu
+@pytest.mark.parametrize("new", [1, 40])
+@pytest.mark.parametrize("window", [0, 30])
+def test_keys_past_the_bound_are_left_out(window, new):
+    """A request of more keys than ``max_kv_len``, or than its table's row holds: its queries
+    see what they see of the first ones, from where they stand."""
+    lens, ps = [100, 300, 64], 32
+    c, tables, starts, q = _attention_case(CODES[0], torch.float16, 8, 2, 64, ps, lens, [new] * 3)
+    for bound in (50, 64, 80, 288):
+        want = S.attention(q.double().numpy(), c.values(0), c.values(1), tables, lens, starts, ps, 1 / 8, window,
+                           bound)
+        _check_finite(_run(c, tables, lens, starts, q, window=window, max_kv_len=bound), *want, torch.float16)
+        if bound % ps == 0:  # and by rows of so many pages
+            short = np.ascontiguousarray(tables[:, :bound // ps])
+            _check_finite(_run(c, short, lens, starts, q, window=window), *want, torch.float16)
