@@ -583,8 +583,8 @@ PMI_API int pmi_silu_mul_f16(const void* gate_up, void* out, int64_t rows, int64
  * next ones of free_pages, a ring of `ring` page numbers (the cache's n_pages)
  * whose first free entry and number of free entries are pool[0] and pool[1] (int32
  * [4]; pool[2] counts refused requests). In request order, a request whose row is
- * too short, or that needs pages when the needs up to it exceed pool[1], is refused:
- * it keeps its length and its tokens get slot -1.
+ * too short, or whose new tokens pass total, or that needs pages when the needs up
+ * to it exceed pool[1], is refused: it keeps its length and its tokens get slot -1.
  * Writes the fresh entries of tables, and
  *   q_starts int32 [R + 1]  where each request's new tokens begin (at most total)
  *   kv_lens_out int32 [R]   the lengths with the new tokens; may be kv_lens

@@ -21,14 +21,15 @@ def extend_tables(tables, kv_lens, new_lens, free_pages, pool, ps, total):
     tables = [list(row) for row in tables]
     ring, width = len(free_pages), len(tables[0]) if tables else 0
     head, count, refused = pool[0], pool[1], pool[2]
-    starts, lens, first, positions, slots, asked, taken = [0], [], [], [], [], 0, 0
+    starts, lens, first, positions, slots, asked, taken, tokens = [0], [], [], [], [], 0, 0, 0
     for r, (length, new) in enumerate(zip(kv_lens, new_lens)):
         length, new = max(length, 0), max(new, 0)
         held, want = -(-length // ps), -(-(length + new) // ps)
         ok = want <= width
         need = want - held if ok else 0
         asked += need
-        ok = ok and (need == 0 or asked <= count)
+        tokens += new
+        ok = ok and (need == 0 or asked <= count) and (new == 0 or tokens <= total)
         if ok:
             for i in range(need):
                 tables[r][held + i] = free_pages[(head + taken + i) % ring]

@@ -96,8 +96,8 @@ PMI_DEV void token_slot(const TablesArgs& a, int t, int r, int start, int first,
 // well. Bound by the chain of loads, two scans and the look-ups (128 requests of one token: 5 us,
 // 6.6 in a graph with its launch), not by its bytes; the sums are 64-bit.
 // need_r = ceil((len + new) / ps) - ceil(len / ps); a request is granted where its table row is wide
-// enough, it stays within max_len and the sum of the needs up to it is within the pool, so the granted ones
-// that need pages are the first of them in order.
+// enough, it stays within max_len and the sums up to it, of needs and of new tokens, are within the pool and
+// the total, so the granted ones that need pages are the first of them in order.
 // Everything is read before anything is written: kv_lens_out may be kv_lens,
 // pool_out may be pool.
 __global__ __launch_bounds__(1024) void extend_tables_kernel(TablesArgs a, int fill) {
@@ -127,7 +127,7 @@ __global__ __launch_bounds__(1024) void extend_tables_kernel(TablesArgs a, int f
     Pair s = wg_scan(Pair{(int64_t)fresh, need}, wave_sums);
     s.a += base.a, s.b += base.b;
     if (r < a.R) {
-      const bool granted = fits && (need == 0 || s.b <= count);
+      const bool granted = fits && (need == 0 || s.b <= count) && (fresh == 0 || s.a <= a.total);
       ends[r] = (int)min(s.a, (int64_t)a.total);
       pages[r] = (int)min(s.b, (int64_t)INT32_MAX);
       old_len[r] = granted ? len : -1;

@@ -99,8 +99,9 @@ def extend_block_tables(block_tables: torch.Tensor, kv_lens: torch.Tensor, new_l
     pages whose first entry and count are ``pool[0]`` and ``pool[1]`` (int32 [4];
     ``pool[2]`` counts refused requests), ``total`` the number of new tokens of all
     requests (fewer in fact: the rest get slot -1). A request whose table row is too
-    short, that would be longer than ``max_len``, or that needs pages when the needs up to
-    it exceed the pool, is refused: it keeps its length and its tokens get slot -1.
+    short, that would be longer than ``max_len``, whose tokens pass ``total``, or that needs
+    pages when the needs up to it exceed the pool, is refused: it keeps its length and its
+    tokens get slot -1.
     ``kv_lens_out`` and ``pool_out`` may be ``kv_lens`` and ``pool``: the step is then taken
     in place."""
     dev = _hip(block_tables, "extend_block_tables")

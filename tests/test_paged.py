@@ -1057,3 +1057,36 @@ def test_keys_past_the_bound_are_left_out(window, new):
         if bound % ps == 0:  # and by rows of so many pages
             short = np.ascontiguousarray(tables[:, :bound // ps])
             _check_finite(_run(c, short, lens, starts, q, window=window), *want, torch.float16)
+
+
+@gpu
+def test_tokens_past_the_total_are_refused_with_their_request():
+    """More new tokens than ``total`` says: the requests whose tokens have no place in the plan
+    keep their lengths, so that no key is counted that was never written."""
+    for R, total, ps in ((4, 25, 16), (4, 5000, 16)):
+        new = [total - 5, 3, 4, 0]
+        c = P.PagedKVCache(0, R, 2 * total, 1, 64, DEV, page_size=ps)
+        plan = c.extend(_ints(new), total)
+        assert plan.kv_lens.tolist() == [total - 5, 3, 0, 0]
+        assert plan.q_starts.tolist() == [0, total - 5, total - 2, total, total]
+        assert plan.slots.tolist()[total - 2:] == [-1, -1] and min(plan.slots.tolist()[:total - 2]) >= 0
+        taken = -(-(total - 5) // ps) + 1
+        pages = c.free_pages.numel()
+        assert c.pool.tolist() == [taken, pages - taken, 1, 0] and plan.first.tolist() == [0, 0, -1, 0]
+        plan = c.extend(_ints([0, 0, 4, 1]), 5)
+        assert plan.kv_lens.tolist() == [total - 5, 3, 4, 1] and min(plan.slots.tolist()) >= 0
+
+
+@gpu
+@pytest.mark.parametrize("R,ps,longest,newest,short", [(70, 16, 200, 90, 100), (300, 64, 1000, 90, 7000), (5, 32, 10, 4, 1)])
+def test_extend_with_a_total_that_is_too_small(R, ps, longest, newest, short):
+    rng = random.Random(R)
+    tables, lens, new, free, pool = _random_tables(rng, R, ps, longest, newest, 3)
+    total = max(0, sum(new) - short)
+    want = S.extend_tables(tables, lens, new, free, pool, ps, total)
+    t = _ints(tables)
+    plan = P.extend_block_tables(t, _ints(lens), _ints(new), _ints(free), _ints(pool), ps, total)
+    got = (t, plan.q_starts, plan.kv_lens, plan.first, plan.positions, plan.slots, plan.pool)
+    assert want[6][2] > pool[2]
+    for name, g, w in zip(("tables", "q_starts", "kv_lens", "first", "positions", "slots", "pool"), got, want):
+        assert g.tolist() == w, name
