@@ -638,8 +638,8 @@ hipError_t few(const AttnArgs& a, bool fp8, hipStream_t stream) {
 
 // ---- many query rows -----------------------------------------------------------------
 // Requests with more query rows: bound by the softmax's vector instructions, 11 a score,
-// beside the matrix cores (prompts of 345 to 2048 tokens, 32 / 8 heads of 128, int8: 112 us, 570
-// TFLOP/s; chunks of 198 to 500 tokens in a window of 4096, 16 / 2 heads of 64, e4m3: 52 us, 310
+// beside the matrix cores (prompts of 345 to 2048 tokens, 32 / 8 heads of 128, int8: 110 us, 580
+// TFLOP/s; chunks of 198 to 500 tokens in a window of 4096, 16 / 2 heads of 64, e4m3: 50 us, 320
 // TFLOP/s, the same rate of scores; counters: 32 % of a wave's cycles issue vector
 // instructions, two waves a SIMD). Scores multiplied a tile ahead of the softmax cost more in
 // copies than they hid (126 us for the prompts), three workgroups a CU too (59 us for the chunks). A
@@ -997,9 +997,9 @@ PMI_DEV void many_rows(const AttnArgs& a, uint8_t* lds, int& s_last, int wg) {
 }
 
 // The requests of few rows first, then those of many, in one launch, so that the end of the one
-// fills with the other (32 / 8 heads of 128: 8 single tokens of 2000 keys and a prompt of 2048 71 us, in
-// two launches 81; 32 of 3000 and a chunk of 512 behind 1000 77 and 84; two prompts of 300, where the
-// first find nothing to do, 17.4 and 18.6).
+// fills with the other (32 / 8 heads of 128: 8 single tokens of 2000 keys and a prompt of 2048 72 us, in
+// two launches 81; 32 of 3000 and a chunk of 512 behind 1000 79 and 84; two prompts of 300, where the
+// first find nothing to do, 17.6 and 18.6).
 template <typename T, int D, bool FP8>
 __global__ __launch_bounds__(256, 2) void attention_rows_kernel(AttnArgs a) {
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];  // [2 slots][K, V]
@@ -1021,8 +1021,19 @@ hipError_t many(const AttnArgs& a, bool fp8, int64_t wgs, hipStream_t stream) {
   return hipGetLastError();
 }
 
-// Workgroups of the few-row kernel: what the CUs hold at once.
+// Workgroups of the few-row part: what the CUs hold at once of its own kernel (with heads of 64 half
+// as many of the joint one, the others follow).
 int few_wgs(int64_t D) { return device_cu_count() * (D == 64 ? 4 : 2); }
+// Query rows of a KV head up to which a request is one of few. From 17 on its codes are read and
+// converted by two to four items, where the other form has one row tile; but that one shares its keys among
+// fewer workgroups. us, few / many rows, KV heads x D, requests x keys each (int8, fp16):
+//   rows                     16          32          48          64
+//   8 x 128,  1 x  4000   13 /  24    14 /  28    17 /  31    17 /  34
+//   8 x 128,  8 x  4000   20 /  36    28 /  41    41 /  49    48 /  53
+//   8 x 128, 64 x  4000   96 / 170   181 / 177   263 / 191   346 / 181
+//   8 x 128, 16 x 32000  190 / 396   304 / 403   524 / 435   621 / 434
+//   8 x  64, 16 x 32000  116 / 291   158 / 293   247 / 322   307 / 324
+// 64 is best while the requests do not fill the CUs; 32 would be where many of 33 to 64 rows do.
 constexpr int kFewRows = 64;
 
 struct ManyPlan {

@@ -465,7 +465,8 @@ hipError_t few(const W8A8& p, hipStream_t stream, const W8A8Rows& rows = {}) {
   // long as there are workgroups for the CUs. M x N x K, 16 / 32 / 64 weight rows (us with the
   // quantisation): 1 x 128256 x 4096 120 / 124 / 95, 8 x 14336 x 4096 22.8 / 23.4 / 19.4, 64 x 28672 x 4096
   // 72 / 54 / 48, 17 x 6144 x 4096 20.0 / 14.3 / 19.2, 1 x 4096 x 4096 10.1 / 13.1 / 16.5, 64 x 4096 x 14336
-  // 42 / 50 / 69.
+  // 42 / 50 / 69; the products alone where the rule is not the best: 1 x 6144 x 4096 9.0 / 10.2 / 12.9, 8 x 18944
+  // x 3584 23.7 / 22.1 / 24.7, 64 x 18944 x 3584 49 / 33 / 37.
   const int64_t cus = device_cu_count();
   const dim3 block(512);
   if (p.N >= 48 * cus)
@@ -483,7 +484,10 @@ hipError_t product(const W8A8& p, hipStream_t stream) {
   if (p.M <= 32) return few<T, 2>(p, stream);
   if (p.M <= 48) return few<T, 3>(p, stream);
   if (p.M <= 64) return few<T, 4>(p, stream);
-  // 256 x 256 tiles where they fill the CUs, else 128 x 128
+  // 256 x 256 tiles where they fill the CUs, else 128 x 128 (the products alone, us, 256 / 128: 4096 x 4096 x
+  // 4096 65 / 74, 256 x 128256 x 4096 157 / 184, 1024 x 4096 x 4096, 64 big tiles, 47 / 27; near the border
+  // 300 x 28672 x 4096, 224 of them half filled, 55 / 54, 2000 x 6144 x 4096, 192, 55 / 58, 1024 x 14336 x
+  // 4096, 224, 59 / 69; half filled, 128 x 128256 x 4096, 148 / 135)
   const int64_t big = ((p.M + 255) / 256) * ((p.N + 255) / 256);
   if (big >= device_cu_count()) return tiles<T, 256, 256, 2, 4>(p, stream);
   return tiles<T, 128, 128, 2, 2>(p, stream);
