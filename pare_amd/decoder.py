@@ -537,7 +537,8 @@ class QuantizedDecoder(nn.Module):
 
     def quantize_head(self) -> None:
         """The output head in 8-bit integers (``Int8Linear``) from now on, in place of its
-        fp16 weight, which is dropped: half the bytes of the largest product of a step."""
+        fp16 weight, which is dropped: half the bytes of the largest product of a step. A
+        state dict taken afterwards loads into a decoder whose head is quantised too."""
         if self.int8_head is None:
             self.int8_head = Int8Linear.from_weight(self.lm_head)
             self.lm_head = None

@@ -301,3 +301,19 @@ def test_the_unfused_decoder_runs_with_an_int8_head_outside_no_grad():
         want = model.forward_tokens(*args)
     got = model.forward_tokens(*args)
     assert not got.requires_grad and torch.equal(got, want)
+
+
+def test_a_decoder_with_an_int8_head_is_saved_and_loaded(tmp_path):
+    model = QuantizedDecoder(SMALL, DEV, seed=7)
+    model.quantize_head()
+    prompts = _prompts([12, 3])
+    want = model.generate_ragged(prompts, 6)[0]
+    other = QuantizedDecoder(SMALL, DEV, seed=8)
+    assert not torch.equal(other.generate_ragged(prompts, 6)[0], want)
+    other.quantize_head()
+    other.load_state_dict(model.state_dict())
+    assert torch.equal(other.generate_ragged(prompts, 6)[0], want)
+    with pytest.warns(UserWarning, match="8-bit"):
+        P.save_quantized(model, tmp_path)
+    third = P.load_quantized(QuantizedDecoder(SMALL, DEV, seed=9), tmp_path, device=DEV)
+    assert torch.equal(third.generate_ragged(prompts, 6)[0], want)
