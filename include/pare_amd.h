@@ -658,7 +658,8 @@ PMI_API int pmi_read_kv_pages(const int32_t* pages, const void* k_cache, const v
  * NaN makes what sees its page NaN. `scale` is finite.
  * max_q and max_kv bound the queries and keys of a request (of a longer one the
  * queries past max_q stay unwritten, and keys past max_kv unread); H / KV <= 64;
- * width * page_size <= 2^30; R KV (max_kv / 64 + 5) ceil(min(max_q H / KV, 64) / 16) < 2^31.
+ * width * page_size <= 2^30; with at most so many keys as max_kv,
+ * R KV (max_kv / 64 + 5) ceil(min(max_q H / KV, 64) / 16) < 2^31.
  * workspace: device scratch of pmi_paged_attention_workspace_bytes() bytes for
  * the same sizes, 256-byte aligned, its first 64 KiB zero before its first use
  * (every call leaves them zero). Calls that may run concurrently must not share it. */

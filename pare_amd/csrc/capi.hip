@@ -1477,7 +1477,8 @@ size_t pmi_paged_attention_workspace_bytes(int64_t T, int64_t R, int64_t H, int6
   if (T <= 0 || R <= 0 || H <= 0 || KV <= 0 || H % KV != 0 || D <= 0 || max_q <= 0 || max_kv <= 0) return 0;
   if (T >= most || R >= most || H > 65535 || D > 65535 || max_q >= most || max_kv >= most || window < 0) return 0;
   pmi::PagedAttention p = {};
-  p.T = T, p.R = R, p.H = H, p.max_q = max_q < T ? max_q : T, p.max_kv = max_kv, p.window = window;
+  p.T = T, p.R = R, p.H = H, p.max_q = max_q < T ? max_q : T, p.window = window;
+  p.max_kv = max_kv < pmi::kPagedMaxKeys ? max_kv : pmi::kPagedMaxKeys;
   pmi::PagedCache c = {};
   c.KV = KV, c.D = D;
   return pmi::paged_attention_ws_bytes(p, c);
@@ -1506,7 +1507,7 @@ int pmi_paged_attention(const void* q, int dtype, int64_t q_stride, int64_t q_he
     return fail(PMI_ERR_INVALID, "%s: the strides of q must be multiples of 8 elements", fn);
   if (max_q > T) max_q = T;
   if (T == 0 || R == 0 || max_q == 0) return ok();
-  if (T >= (1ll << 31) / H || R >= (1ll << 31) / KV || width > (1ll << 30) / page_size || max_kv >= (1ll << 31) ||
+  if (T >= (1ll << 31) / H || R >= (1ll << 31) / KV || width > pmi::kPagedMaxKeys / page_size || max_kv >= (1ll << 31) ||
       window >= (1ll << 31))
     return fail(PMI_ERR_UNSUPPORTED, "%s: too large", fn);
   if (!q || !out || !kv_lens || (width && !tables)) return fail(PMI_ERR_INVALID, "%s: null buffer", fn);
@@ -1516,7 +1517,8 @@ int pmi_paged_attention(const void* q, int dtype, int64_t q_stride, int64_t q_he
                            max_q, max_kv, window, scale, dtype == PMI_BF16};
   const pmi::PagedCache c = {const_cast<void*>(k_cache), const_cast<void*>(v_cache), const_cast<float*>(k_scale),
                              const_cast<float*>(v_scale), n_pages, KV, page_size, D, code_dtype == PMI_F8};
-  if (p.max_kv > width * page_size) p.max_kv = width * page_size;
+  // (not cut to the table's width: the ranges of keys have to be those that the workspace was asked for)
+  if (p.max_kv > pmi::kPagedMaxKeys) p.max_kv = pmi::kPagedMaxKeys;
   if (!pmi::paged_attention_launch_fits(p, c))
     return fail(PMI_ERR_UNSUPPORTED, "%s: too many query rows for one launch (T H)", fn);
   if (!pmi::paged_attention_tiles_fit(p, c))

@@ -46,6 +46,8 @@ hipError_t launch_append_kv(const PagedCache& c, const void* qkv, int64_t ld, bo
 hipError_t launch_read_pages(const PagedCache& c, const int32_t* pages, int out_dtype, void* k, void* v, int64_t n,
                              hipStream_t stream);
 
+constexpr int64_t kPagedMaxKeys = 1ll << 30;  // of a request: width * page_size
+
 struct PagedAttention {
   const void* q;  // [T, H, D], element strides below
   int64_t q_token, q_head;

@@ -1070,7 +1070,8 @@ bool paged_attention_tiles_fit(const PagedAttention& p, const PagedCache& c) {
   // of every request the rows of one of few rows, in tiles of 16; keys in tiles of 64, one more for a
   // range that begins inside a tile, and up to four for its last cut
   const int64_t rows = p.max_q * (p.H / c.KV), row_tiles = ((rows < kFewRows ? rows : kFewRows) + 15) / 16;
-  return (double)p.R * (double)c.KV * (double)row_tiles * (double)(p.max_kv / 64 + 5) < 2147483648.0;
+  const int64_t keys = p.width * c.ps < p.max_kv ? p.width * c.ps : p.max_kv;
+  return (double)p.R * (double)c.KV * (double)row_tiles * (double)(keys / 64 + 5) < 2147483648.0;
 }
 
 bool paged_attention_launch_fits(const PagedAttention& p, const PagedCache& c) {

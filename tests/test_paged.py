@@ -1090,3 +1090,18 @@ def test_extend_with_a_total_that_is_too_small(R, ps, longest, newest, short):
     assert want[6][2] > pool[2]
     for name, g, w in zip(("tables", "q_starts", "kv_lens", "first", "positions", "slots", "pool"), got, want):
         assert g.tolist() == w, name
+
+
+def test_the_workspace_of_a_bound_past_the_table_is_enough():
+    """What the query asks for a bound is what the call takes with it, whatever the table's
+    width: more keys may take fewer ranges, and so less workspace."""
+    L = _lib.lib()
+    sizes = dict(T=300, R=1, H=4, KV=1, D=128, max_q=300)
+    need = {n: L.pmi_paged_attention_workspace_bytes(*sizes.values(), n, 0) for n in (42432, 42433, 1 << 30, (1 << 31) - 1)}
+    assert need[42433] < need[42432] and need[1 << 30] == need[(1 << 31) - 1]
+    for max_kv in need:
+        args = dict(**sizes, ps=64, width=663, tstride=663, max_kv=max_kv)  # 42432 tokens
+        rc = L.pmi_paged_attention(*_attention_args(**args, ws=None))
+        assert rc == _lib.PMI_ERR_INVALID and f" {need[max_kv]} bytes" in _lib.last_error()
+    many = L.pmi_paged_attention_workspace_bytes(100000, 8, 32, 8, 128, 100000, (1 << 31) - 1, 0)
+    assert many == L.pmi_paged_attention_workspace_bytes(100000, 8, 32, 8, 128, 100000, 1 << 30, 0) < 1 << 30
