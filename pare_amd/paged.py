@@ -73,6 +73,7 @@ def _cache(dev: torch.device, k_cache: torch.Tensor, v_cache: torch.Tensor, k_sc
     assert k_cache.dim() == 4 and v_cache.dim() == 5, (
         "k_cache must be [pages, KV, page_size, D] and v_cache [pages, KV, page_size / 16, D, 16]")
     pages, KV, ps, D = k_cache.shape
+    assert KV > 0 and D > 0, "the caches must hold at least one head"
     assert tuple(v_cache.shape) == (pages, KV, ps // 16, D, 16) and ps % 16 == 0, (
         f"v_cache must be [{pages}, {KV}, {ps // 16}, {D}, 16], got {tuple(v_cache.shape)}")
     assert k_cache.dtype in _CODES and v_cache.dtype == k_cache.dtype, (

@@ -1105,3 +1105,14 @@ def test_the_workspace_of_a_bound_past_the_table_is_enough():
         assert rc == _lib.PMI_ERR_INVALID and f" {need[max_kv]} bytes" in _lib.last_error()
     many = L.pmi_paged_attention_workspace_bytes(100000, 8, 32, 8, 128, 100000, (1 << 31) - 1, 0)
     assert many == L.pmi_paged_attention_workspace_bytes(100000, 8, 32, 8, 128, 100000, 1 << 30, 0) < 1 << 30
+
+
+@gpu
+def test_a_cache_without_heads_is_refused():
+    k, v = torch.zeros(2, 0, 16, 64, dtype=torch.int8, device=DEV), torch.zeros(2, 0, 1, 64, 16, dtype=torch.int8, device=DEV)
+    s, i, angles = torch.zeros(2, 0, device=DEV), _ints([0]), torch.zeros(1, 32, device=DEV)
+    qkv = torch.zeros(1, 192, dtype=torch.float16, device=DEV)
+    for call in (lambda: P.rope_append_kv(qkv, angles, angles, i, i, k, v, s, s), lambda: P.read_kv_pages(i, k, v, s, s),
+                 lambda: P.paged_attention(qkv.view(1, 3, 64), k, v, s, s, i[None], i, scale=1.0)):
+        with pytest.raises(AssertionError, match="head"):
+            call()
