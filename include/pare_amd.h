@@ -675,6 +675,125 @@ PMI_API size_t pmi_paged_attention_workspace_bytes(int64_t T, int64_t R, int64_t
                                                    int64_t D, int64_t max_q, int64_t max_kv,
                                                    int64_t window);
 
+/* pmi_paged_attention of requests of which some share their first pages: run_starts int32
+ * [R + 1] and run_lens int32 [R] as pmi_shared_prefixes gives them for the same tables, lengths and
+ * queries. The result is the same but for roundings: a run's shared keys are read once for the queries of
+ * all its members, where no request has more than 64 query rows (max_q H / KV) and there is no
+ * window. workspace: pmi_paged_attention_shared_workspace_bytes() bytes, otherwise as above. */
+PMI_API int pmi_paged_attention_shared(const void* q, int dtype, int64_t q_stride,
+                                       int64_t q_head_stride, const void* k_cache,
+                                       const void* v_cache, const float* k_scale,
+                                       const float* v_scale, int code_dtype, int64_t n_pages,
+                                       int64_t page_size, const int32_t* tables,
+                                       int64_t table_stride, const int32_t* kv_lens,
+                                       const int32_t* q_starts, const int32_t* run_starts,
+                                       const int32_t* run_lens, void* out, int64_t T, int64_t R,
+                                       int64_t width, int64_t H, int64_t KV, int64_t D,
+                                       int64_t max_q, int64_t max_kv, int64_t window, float scale,
+                                       void* workspace, size_t workspace_bytes, void* stream);
+PMI_API size_t pmi_paged_attention_shared_workspace_bytes(int64_t T, int64_t R, int64_t H,
+                                                          int64_t KV, int64_t D, int64_t max_q,
+                                                          int64_t max_kv, int64_t window);
+
+/* Requests that begin as forks of others. shares int32 [ring] counts the owners of a page
+ * beyond the first (0: of fresh and of free ones), parents int32 [R] names for each request
+ * the one whose tokens it begins with (none: outside 0 .. R - 1, or itself) and lengths int32 [R]
+ * (nullable: all) how many of them; a request's parent is what it was before the call. With n tokens
+ * the n / page_size whole pages are shared; if any are left, the page that holds them
+ * is to be copied: a page from the ring becomes the fork's, and (src[r], dst[r]) int32 [R]
+ * say what to copy where (-1, -1: nothing). Refused, and counted in pool[2]: a request that holds
+ * tokens already, and one that needs a page when the needs up to it exceed the pool. scratch:
+ * device memory of 4 R bytes. A page with several owners is whole, so that no token is
+ * written to it. */
+PMI_API int pmi_fork_block_tables(int32_t* tables, int64_t table_stride, int32_t* kv_lens,
+                                  const int32_t* parents, const int32_t* lengths,
+                                  const int32_t* free_pages, int32_t* pool, int32_t* shares,
+                                  int32_t* src, int32_t* dst, int32_t* scratch, int64_t R,
+                                  int64_t width, int64_t ring, int64_t page_size, void* stream);
+
+/* pmi_release_block_tables where pages may have several owners: one that a request with
+ * done[r] holds loses an owner, and goes to the end of the ring when none is left, in the order of
+ * the pages' numbers. scratch: device memory of pmi_release_shared_scratch_bytes() bytes. */
+PMI_API int pmi_release_shared_block_tables(const int32_t* tables, int64_t table_stride,
+                                            int32_t* kv_lens, const uint8_t* done,
+                                            int32_t* free_pages, int32_t* pool, int32_t* shares,
+                                            int64_t R, int64_t width, int64_t ring,
+                                            int64_t page_size, void* scratch, size_t scratch_bytes,
+                                            void* stream);
+PMI_API size_t pmi_release_shared_scratch_bytes(int64_t ring);
+
+/* The live pages (those in the tables of the requests' kv_lens) become pages 0 .. n - 1: those
+ * from n on, in order, take the places of the free ones before it, in order. The tables,
+ * shares (nullable: no page has two owners) and the ring (n, n + 1, .., pages - 1 free, in that
+ * order) are rewritten; moves[0] (int32) is how many pages have to be copied, src[i] to dst[i]
+ * (int32 [ring / 2], -1 behind the last), which no two copies have in common. scratch: device
+ * memory of pmi_compact_scratch_bytes() bytes. */
+PMI_API int pmi_compact_block_tables(int32_t* tables, int64_t table_stride, const int32_t* kv_lens,
+                                     int32_t* free_pages, int32_t* pool, int32_t* shares,
+                                     int32_t* src, int32_t* dst, int32_t* moves, int64_t R,
+                                     int64_t width, int64_t ring, int64_t page_size, void* scratch,
+                                     size_t scratch_bytes, void* stream);
+PMI_API size_t pmi_compact_scratch_bytes(int64_t ring);
+
+/* Page src[i] to page dst[i], codes and scales, of all layers, for i < n, or where `count`
+ * is given (int32, on the device) for i < min(n, count[0]). Pairs with a page that the cache does not
+ * have are left out; no page may be dst twice, or src and dst. k_caches .. v_scales:
+ * host arrays of `layers` device pointers, caches as above of the same sizes. */
+PMI_API int pmi_copy_kv_pages(const int32_t* src, const int32_t* dst, const int32_t* count,
+                              int64_t n, void* const* k_caches, void* const* v_caches,
+                              float* const* k_scales, float* const* v_scales, int64_t layers,
+                              int64_t n_pages, int64_t page_size, int64_t KV, int64_t D,
+                              void* stream);
+
+/* Runs of neighbouring requests whose first pages are the same: a request with new tokens
+ * (q_starts int32 [R + 1] counts them; null: one each; kv_lens int32 [R] with them) begins a run
+ * if fewer than least_pages (>= 1) of its first pages, whole and before its new tokens, are those
+ * of the request with new tokens before it. starts int32 [R + 1]: the requests with
+ * which runs begin, R behind the last; lens int32 [R]: how many positions the members of the
+ * request's run share, 0 for a run of one. workspace: device scratch of
+ * pmi_shared_prefixes_workspace_bytes() bytes, as for pmi_paged_attention. */
+PMI_API int pmi_shared_prefixes(const int32_t* tables, int64_t table_stride,
+                                const int32_t* kv_lens, const int32_t* q_starts, int32_t* starts,
+                                int32_t* lens, int64_t R, int64_t width, int64_t page_size,
+                                int64_t least_pages, void* workspace, size_t workspace_bytes,
+                                void* stream);
+PMI_API size_t pmi_shared_prefixes_workspace_bytes(int64_t R);
+
+/* Logits before a token is chosen. x [R, V] (PMI_F16, PMI_BF16 or PMI_F32, rows `stride` elements
+ * apart) to out of the same type (rows out_stride apart; may be x), in fp32, rounded once:
+ *   x > 0 ? x / repetition[r] : x * repetition[r]       for tokens in the row's history
+ *   x - frequency[r] * c - presence[r]                  for those c > 0 times in it behind the prompt
+ *   x + the row's biases of the token                   (added up in their order first)
+ *   -inf                                                for tokens without a bit in the row's mask
+ * history int32 [R, L] (nullable), of which history_lens[r] (int32 [R], nullable: L) tokens count,
+ * the first prompt_lens[r] (nullable: 0) of them as the prompt; repetition, presence and
+ * frequency fp32 [R], each nullable. bias_ids int32 and bias fp32 [R, n_bias]. Tokens outside
+ * 0 .. V - 1 are skipped in both. allowed int32 [masks, words] (nullable): bit t % 32 of word t / 32 allows
+ * token t; row r has mask allowed_rows[r] (int32 [R]; null: mask r), or none if there is no such one. */
+PMI_API int pmi_process_logits(const void* logits, int dtype, int64_t stride,
+                               const int32_t* history, int64_t history_stride, int64_t L,
+                               const int32_t* history_lens, const int32_t* prompt_lens,
+                               const float* repetition, const float* presence,
+                               const float* frequency, const int32_t* bias_ids, const float* bias,
+                               int64_t n_bias, const int32_t* allowed, int64_t masks, int64_t words,
+                               const int32_t* allowed_rows, void* out, int64_t out_stride,
+                               int64_t R, int64_t V, void* stream);
+
+/* The largest of each row of what pmi_process_logits gives, without writing it: its token to
+ * tokens[r * token_stride] (int64), the lowest of several, NaN the largest of all, 0 for a row
+ * whose mask allows nothing. R <= 16384. workspace: device scratch of
+ * pmi_greedy_tokens_workspace_bytes() bytes, as for pmi_paged_attention. */
+PMI_API int pmi_greedy_tokens(const void* logits, int dtype, int64_t stride,
+                              const int32_t* history, int64_t history_stride, int64_t L,
+                              const int32_t* history_lens, const int32_t* prompt_lens,
+                              const float* repetition, const float* presence,
+                              const float* frequency, const int32_t* bias_ids, const float* bias,
+                              int64_t n_bias, const int32_t* allowed, int64_t masks, int64_t words,
+                              const int32_t* allowed_rows, int64_t* tokens, int64_t token_stride,
+                              int64_t R, int64_t V, void* workspace, size_t workspace_bytes,
+                              void* stream);
+PMI_API size_t pmi_greedy_tokens_workspace_bytes(int64_t R, int64_t V, int dtype);
+
 /* Rows of x [M, K] (PMI_F16, PMI_BF16 or PMI_F32, rows x_stride elements apart) as
  * 8-bit integers: codes int8 [M, ld] = round(x * (127 / amax)), zeros from column K
  * to ld = K rounded up to 16, and scales fp32 [M] = amax / 127, amax the largest |x| of the

@@ -100,6 +100,22 @@ SIGNATURES = {
     "pmi_paged_attention": (_i, [_vp, _i, _i64, _i64, *[_vp] * 4, _i, _i64, _i64, _vp, _i64, _vp, _vp, _vp,
                                  *[_i64] * 9, ctypes.c_float, _vp, ctypes.c_size_t, _vp]),
     "pmi_paged_attention_workspace_bytes": (ctypes.c_size_t, [_i64] * 8),
+    "pmi_paged_attention_shared": (_i, [_vp, _i, _i64, _i64, *[_vp] * 4, _i, _i64, _i64, _vp, _i64, *[_vp] * 5,
+                                        *[_i64] * 9, ctypes.c_float, _vp, ctypes.c_size_t, _vp]),
+    "pmi_paged_attention_shared_workspace_bytes": (ctypes.c_size_t, [_i64] * 8),
+    "pmi_fork_block_tables": (_i, [_vp, _i64, *[_vp] * 9, *[_i64] * 4, _vp]),
+    "pmi_release_shared_block_tables": (_i, [_vp, _i64, *[_vp] * 5, *[_i64] * 4, _vp, ctypes.c_size_t, _vp]),
+    "pmi_release_shared_scratch_bytes": (ctypes.c_size_t, [_i64]),
+    "pmi_compact_block_tables": (_i, [_vp, _i64, *[_vp] * 7, *[_i64] * 4, _vp, ctypes.c_size_t, _vp]),
+    "pmi_compact_scratch_bytes": (ctypes.c_size_t, [_i64]),
+    "pmi_copy_kv_pages": (_i, [_vp, _vp, _vp, _i64, *[_vp] * 4, *[_i64] * 5, _vp]),
+    "pmi_shared_prefixes": (_i, [_vp, _i64, *[_vp] * 4, *[_i64] * 4, _vp, ctypes.c_size_t, _vp]),
+    "pmi_shared_prefixes_workspace_bytes": (ctypes.c_size_t, [_i64]),
+    "pmi_process_logits": (_i, [_vp, _i, _i64, _vp, _i64, _i64, *[_vp] * 7, _i64, _vp, _i64, _i64, _vp, _vp, _i64,
+                                _i64, _i64, _vp]),
+    "pmi_greedy_tokens": (_i, [_vp, _i, _i64, _vp, _i64, _i64, *[_vp] * 7, _i64, _vp, _i64, _i64, _vp, _vp, _i64,
+                               _i64, _i64, _vp, ctypes.c_size_t, _vp]),
+    "pmi_greedy_tokens_workspace_bytes": (ctypes.c_size_t, [_i64, _i64, _i]),
     "pmi_quantize_rows": (_i, [_vp, _i, _i64, _vp, _vp, _i64, _i64, _vp]),
     "pmi_matmul_w8a8": (_i, [*[_vp] * 6, _i, _i64, _i64, _i64, _vp]),
     "pmi_matmul_w8a8_rows": (_i, [_vp, _i, _i64, *[_vp] * 4, *[_i64] * 3, _vp, ctypes.c_size_t, _vp]),

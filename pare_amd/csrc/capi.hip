@@ -10,6 +10,7 @@
 #include <cmath>
 #include <mutex>
 
+#include "logits.h"
 #include "paged.h"
 #include "pmi_launch.h"
 #include "w8a8.h"
@@ -123,6 +124,29 @@ int check_cache(const void* k, const void* v, const float* ks, const float* vs, 
   if (pages && (!k || !v || !ks || !vs)) return fail(PMI_ERR_INVALID, "%s: null cache buffer", fn);
   if (!aligned(k, 16) || !aligned(v, 16))
     return fail(PMI_ERR_INVALID, "%s: the caches must be 16-byte aligned", fn);
+  return PMI_OK;
+}
+
+int check_logits(const pmi::Logits& f, const char* fn) {
+  if (f.dtype != PMI_F16 && f.dtype != PMI_BF16 && f.dtype != PMI_F32)
+    return fail(PMI_ERR_INVALID, "%s: dtype must be PMI_F16, PMI_BF16 or PMI_F32 (got %d)", fn, f.dtype);
+  if (f.R < 0 || f.V < 0 || f.stride < f.V || f.L < 0 || f.history_stride < f.L || f.n_bias < 0 || f.masks < 0)
+    return fail(PMI_ERR_INVALID, "%s: R, V, L, n_bias and masks may not be negative, rows not overlap", fn);
+  if (f.V >= (1ll << 30) || f.L >= (1ll << 31) || f.n_bias >= (1ll << 30) || f.masks >= (1ll << 31) ||
+      pmi::logits_workgroups(f.R < (1ll << 31) ? f.R : 1ll << 31, f.V, f.dtype) >= (1ll << 24))
+    return fail(PMI_ERR_UNSUPPORTED, "%s: too large (R=%lld V=%lld)", fn, (long long)f.R, (long long)f.V);
+  if (f.R == 0 || f.V == 0) return PMI_OK;
+  if (!f.x) return fail(PMI_ERR_INVALID, "%s: null buffer", fn);
+  if (f.n_bias && (!f.bias_ids || !f.bias))
+    return fail(PMI_ERR_INVALID, "%s: biases need both their tokens and their values", fn);
+  if (f.allowed && f.words < (f.V + 31) / 32)
+    return fail(PMI_ERR_INVALID, "%s: a mask of %lld words is too short for %lld tokens", fn, (long long)f.words,
+                (long long)f.V);
+  if (f.allowed && !f.allowed_rows && f.masks < f.R)
+    return fail(PMI_ERR_INVALID, "%s: without allowed_rows every row has its mask (R=%lld masks=%lld)", fn,
+                (long long)f.R, (long long)f.masks);
+  const size_t size = f.dtype == PMI_F32 ? 4 : 2;
+  if (!aligned(f.x, size)) return fail(PMI_ERR_INVALID, "%s: logits are not aligned to their type", fn);
   return PMI_OK;
 }
 
@@ -1471,8 +1495,10 @@ int pmi_read_kv_pages(const int32_t* pages, const void* k_cache, const void* v_c
   return from_hip(pmi::launch_read_pages(c, pages, out_dtype, k_out, v_out, n, (hipStream_t)stream), fn);
 }
 
-size_t pmi_paged_attention_workspace_bytes(int64_t T, int64_t R, int64_t H, int64_t KV, int64_t D, int64_t max_q,
-                                           int64_t max_kv, int64_t window) {
+namespace {
+
+size_t attention_ws_bytes(int64_t T, int64_t R, int64_t H, int64_t KV, int64_t D, int64_t max_q, int64_t max_kv,
+                          int64_t window, bool runs) {
   const int64_t most = 1ll << 31;
   if (T <= 0 || R <= 0 || H <= 0 || KV <= 0 || H % KV != 0 || D <= 0 || max_q <= 0 || max_kv <= 0) return 0;
   if (T >= most || R >= most || H > 65535 || D > 65535 || max_q >= most || max_kv >= most || window < 0) return 0;
@@ -1481,16 +1507,29 @@ size_t pmi_paged_attention_workspace_bytes(int64_t T, int64_t R, int64_t H, int6
   p.max_kv = max_kv < pmi::kPagedMaxKeys ? max_kv : pmi::kPagedMaxKeys;
   pmi::PagedCache c = {};
   c.KV = KV, c.D = D;
-  return pmi::paged_attention_ws_bytes(p, c);
+  return runs && pmi::paged_attention_shares(p, c) ? pmi::paged_shared_ws_bytes(p, c) : pmi::paged_attention_ws_bytes(p, c);
 }
 
-int pmi_paged_attention(const void* q, int dtype, int64_t q_stride, int64_t q_head_stride, const void* k_cache,
+}  // namespace
+
+size_t pmi_paged_attention_workspace_bytes(int64_t T, int64_t R, int64_t H, int64_t KV, int64_t D, int64_t max_q,
+                                           int64_t max_kv, int64_t window) {
+  return attention_ws_bytes(T, R, H, KV, D, max_q, max_kv, window, false);
+}
+
+size_t pmi_paged_attention_shared_workspace_bytes(int64_t T, int64_t R, int64_t H, int64_t KV, int64_t D,
+                                                  int64_t max_q, int64_t max_kv, int64_t window) {
+  return attention_ws_bytes(T, R, H, KV, D, max_q, max_kv, window, true);
+}
+
+namespace {
+
+int paged_attention(const char* fn, const int32_t* run_starts, const int32_t* run_lens, const void* q, int dtype, int64_t q_stride, int64_t q_head_stride, const void* k_cache,
                         const void* v_cache, const float* k_scale, const float* v_scale, int code_dtype,
                         int64_t n_pages, int64_t page_size, const int32_t* tables, int64_t table_stride,
                         const int32_t* kv_lens, const int32_t* q_starts, void* out, int64_t T, int64_t R,
                         int64_t width, int64_t H, int64_t KV, int64_t D, int64_t max_q, int64_t max_kv,
                         int64_t window, float scale, void* workspace, size_t workspace_bytes, void* stream) {
-  const char* fn = "pmi_paged_attention";
   if (int rc = check_cache(k_cache, v_cache, k_scale, v_scale, code_dtype, n_pages, page_size, H, KV, D, fn)) return rc;
   if (dtype != PMI_F16 && dtype != PMI_BF16)
     return fail(PMI_ERR_INVALID, "%s: dtype must be PMI_F16 or PMI_BF16 (got %d)", fn, dtype);
@@ -1514,20 +1553,199 @@ int pmi_paged_attention(const void* q, int dtype, int64_t q_stride, int64_t q_he
   if (!aligned(q, 16) || !aligned(out, 16))
     return fail(PMI_ERR_INVALID, "%s: q and out must be 16-byte aligned", fn);
   pmi::PagedAttention p = {q, q_stride, q_head_stride, out, tables, table_stride, kv_lens, q_starts, T, R, width, H,
-                           max_q, max_kv, window, scale, dtype == PMI_BF16};
+                           max_q, max_kv, window, scale, dtype == PMI_BF16, run_starts, run_lens};
   const pmi::PagedCache c = {const_cast<void*>(k_cache), const_cast<void*>(v_cache), const_cast<float*>(k_scale),
                              const_cast<float*>(v_scale), n_pages, KV, page_size, D, code_dtype == PMI_F8};
   // (not cut to the table's width: the ranges of keys have to be those that the workspace was asked for)
   if (p.max_kv > pmi::kPagedMaxKeys) p.max_kv = pmi::kPagedMaxKeys;
-  if (!pmi::paged_attention_launch_fits(p, c))
+  const bool shares = run_starts && pmi::paged_attention_shares(p, c);
+  if (!(shares ? pmi::paged_shared_launch_fits(p, c) : pmi::paged_attention_launch_fits(p, c)))
     return fail(PMI_ERR_UNSUPPORTED, "%s: too many query rows for one launch (T H)", fn);
-  if (!pmi::paged_attention_tiles_fit(p, c))
+  pmi::PagedAttention whole = p;  // (a run has the queries of all its members)
+  if (shares) whole.max_q = T;
+  if (!pmi::paged_attention_tiles_fit(whole, c))
     return fail(PMI_ERR_UNSUPPORTED, "%s: too many tiles of 64 keys for 32 bits (R KV max_kv): give a tighter max_kv "
                 "or fewer requests", fn);
-  const size_t need = pmi_paged_attention_workspace_bytes(T, R, H, KV, D, max_q, p.max_kv, window);
+  const size_t need = attention_ws_bytes(T, R, H, KV, D, max_q, p.max_kv, window, run_starts != nullptr);
   if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 256)))
     return fail(PMI_ERR_INVALID, "%s: needs a 256-byte aligned workspace of %zu bytes", fn, need);
+  if (shares) return from_hip(pmi::launch_paged_shared(p, c, workspace, (hipStream_t)stream), fn);
   return from_hip(pmi::launch_paged_attention(p, c, workspace, workspace_bytes, (hipStream_t)stream), fn);
+}
+
+}  // namespace
+
+int pmi_paged_attention(const void* q, int dtype, int64_t q_stride, int64_t q_head_stride, const void* k_cache,
+                        const void* v_cache, const float* k_scale, const float* v_scale, int code_dtype,
+                        int64_t n_pages, int64_t page_size, const int32_t* tables, int64_t table_stride,
+                        const int32_t* kv_lens, const int32_t* q_starts, void* out, int64_t T, int64_t R,
+                        int64_t width, int64_t H, int64_t KV, int64_t D, int64_t max_q, int64_t max_kv,
+                        int64_t window, float scale, void* workspace, size_t workspace_bytes, void* stream) {
+  return paged_attention("pmi_paged_attention", nullptr, nullptr, q, dtype, q_stride, q_head_stride, k_cache, v_cache, k_scale, v_scale, code_dtype,
+                         n_pages, page_size, tables, table_stride, kv_lens, q_starts, out, T, R, width, H, KV, D, max_q, max_kv,
+                         window, scale, workspace, workspace_bytes, stream);
+}
+
+int pmi_paged_attention_shared(const void* q, int dtype, int64_t q_stride, int64_t q_head_stride, const void* k_cache,
+                        const void* v_cache, const float* k_scale, const float* v_scale, int code_dtype,
+                        int64_t n_pages, int64_t page_size, const int32_t* tables, int64_t table_stride,
+                        const int32_t* kv_lens, const int32_t* q_starts, const int32_t* run_starts, const int32_t* run_lens, void* out, int64_t T, int64_t R,
+                        int64_t width, int64_t H, int64_t KV, int64_t D, int64_t max_q, int64_t max_kv,
+                        int64_t window, float scale, void* workspace, size_t workspace_bytes, void* stream) {
+  const char* fn = "pmi_paged_attention_shared";
+  if (R > 0 && (!run_starts || !run_lens)) return fail(PMI_ERR_INVALID, "%s: null buffer", fn);
+  return paged_attention(fn, run_starts, run_lens, q, dtype, q_stride, q_head_stride, k_cache, v_cache, k_scale, v_scale, code_dtype,
+                         n_pages, page_size, tables, table_stride, kv_lens, q_starts, out, T, R, width, H, KV, D, max_q, max_kv,
+                         window, scale, workspace, workspace_bytes, stream);
+}
+
+int pmi_fork_block_tables(int32_t* tables, int64_t table_stride, int32_t* kv_lens, const int32_t* parents,
+                          const int32_t* lengths, const int32_t* free_pages, int32_t* pool, int32_t* shares,
+                          int32_t* src, int32_t* dst, int32_t* scratch, int64_t R, int64_t width, int64_t ring,
+                          int64_t page_size, void* stream) {
+  const char* fn = "pmi_fork_block_tables";
+  if (int rc = check_tables(R, width, table_stride, ring, page_size, fn)) return rc;
+  if (R == 0) return ok();
+  if (!kv_lens || !parents || !pool || !src || !dst || !scratch || (width && !tables) || (ring && (!free_pages || !shares)))
+    return fail(PMI_ERR_INVALID, "%s: null buffer", fn);
+  const pmi::PagedFork f = {tables, table_stride, kv_lens, parents, lengths, free_pages, pool, shares, src, dst,
+                            scratch, R, width, ring, page_size};
+  return from_hip(pmi::launch_fork_tables(f, (hipStream_t)stream), fn);
+}
+
+size_t pmi_release_shared_scratch_bytes(int64_t ring) {
+  return ring <= 0 || ring >= (1ll << 31) ? 0 : (size_t)(pmi::page_chunks(ring) + 2) * 4;
+}
+
+int pmi_release_shared_block_tables(const int32_t* tables, int64_t table_stride, int32_t* kv_lens, const uint8_t* done,
+                                    int32_t* free_pages, int32_t* pool, int32_t* shares, int64_t R, int64_t width,
+                                    int64_t ring, int64_t page_size, void* scratch, size_t scratch_bytes,
+                                    void* stream) {
+  const char* fn = "pmi_release_shared_block_tables";
+  if (int rc = check_tables(R, width, table_stride, ring, page_size, fn)) return rc;
+  if (R == 0 || ring == 0) return ok();
+  if (!kv_lens || !done || !free_pages || !pool || !shares || (width && !tables))
+    return fail(PMI_ERR_INVALID, "%s: null buffer", fn);
+  if (!scratch || scratch_bytes < pmi_release_shared_scratch_bytes(ring) || !aligned(scratch, 4))
+    return fail(PMI_ERR_INVALID, "%s: needs a scratch of %zu bytes", fn, pmi_release_shared_scratch_bytes(ring));
+  const pmi::PagedRelease f = {tables, table_stride, kv_lens, done, free_pages, pool, shares, (int32_t*)scratch,
+                               R, width, ring, page_size};
+  return from_hip(pmi::launch_release_shared(f, (hipStream_t)stream), fn);
+}
+
+size_t pmi_compact_scratch_bytes(int64_t ring) {
+  return ring <= 0 || ring >= (1ll << 31) ? 0 : (size_t)(2 * ring + pmi::page_chunks(ring)) * 4;
+}
+
+int pmi_compact_block_tables(int32_t* tables, int64_t table_stride, const int32_t* kv_lens, int32_t* free_pages,
+                             int32_t* pool, int32_t* shares, int32_t* src, int32_t* dst, int32_t* moves, int64_t R,
+                             int64_t width, int64_t ring, int64_t page_size, void* scratch, size_t scratch_bytes,
+                             void* stream) {
+  const char* fn = "pmi_compact_block_tables";
+  if (int rc = check_tables(R, width, table_stride, ring, page_size, fn)) return rc;
+  if (ring == 0) return ok();
+  if (!free_pages || !pool || !moves || (ring > 1 && (!src || !dst)) || (R && (!kv_lens || (width && !tables))))
+    return fail(PMI_ERR_INVALID, "%s: null buffer", fn);
+  if (!scratch || scratch_bytes < pmi_compact_scratch_bytes(ring) || !aligned(scratch, 4))
+    return fail(PMI_ERR_INVALID, "%s: needs a scratch of %zu bytes", fn, pmi_compact_scratch_bytes(ring));
+  int32_t* s = (int32_t*)scratch;
+  const pmi::PagedCompact f = {tables, table_stride, kv_lens, free_pages, pool, shares, src, dst, moves, s, s + ring,
+                               s + 2 * ring, R, width, ring, page_size};
+  return from_hip(pmi::launch_compact_tables(f, (hipStream_t)stream), fn);
+}
+
+int pmi_copy_kv_pages(const int32_t* src, const int32_t* dst, const int32_t* count, int64_t n, void* const* k_caches,
+                      void* const* v_caches, float* const* k_scales, float* const* v_scales, int64_t layers,
+                      int64_t n_pages, int64_t page_size, int64_t KV, int64_t D, void* stream) {
+  const char* fn = "pmi_copy_kv_pages";
+  if (n < 0 || layers < 0 || n >= (1ll << 31))
+    return fail(PMI_ERR_INVALID, "%s: need n, layers >= 0 (n=%lld layers=%lld)", fn, (long long)n, (long long)layers);
+  if (layers && (!k_caches || !v_caches || !k_scales || !v_scales)) return fail(PMI_ERR_INVALID, "%s: null buffer", fn);
+  for (int64_t i = 0; i < (layers ? layers : 1); ++i)
+    if (int rc = layers ? check_cache(k_caches[i], v_caches[i], k_scales[i], v_scales[i], PMI_I8, n_pages, page_size,
+                                      KV, KV, D, fn)
+                        : check_cache(nullptr, nullptr, nullptr, nullptr, PMI_I8, 0, page_size, KV, KV, D, fn))
+      return rc;
+  if (n == 0 || layers == 0 || n_pages == 0) return ok();
+  if (!src || !dst) return fail(PMI_ERR_INVALID, "%s: null buffer", fn);
+  for (int64_t first = 0; first < layers; first += pmi::kCopyLayers) {
+    pmi::PagedCopy f = {};
+    f.layers = layers - first < pmi::kCopyLayers ? layers - first : pmi::kCopyLayers;
+    for (int64_t i = 0; i < f.layers; ++i)
+      f.k[i] = k_caches[first + i], f.v[i] = v_caches[first + i], f.k_scale[i] = k_scales[first + i],
+      f.v_scale[i] = v_scales[first + i];
+    f.src = src, f.dst = dst, f.count = count;
+    f.n = n, f.pages = n_pages, f.KV = KV, f.page_bytes = KV * page_size * D;
+    if (int rc = from_hip(pmi::launch_copy_pages(f, (hipStream_t)stream), fn)) return rc;
+  }
+  return ok();
+}
+
+size_t pmi_shared_prefixes_workspace_bytes(int64_t R) {
+  return R <= 0 || R > pmi::kTablesMaxRequests ? 0 : pmi::kWsCounterBytes + (size_t)R * 4;
+}
+
+int pmi_shared_prefixes(const int32_t* tables, int64_t table_stride, const int32_t* kv_lens, const int32_t* q_starts,
+                        int32_t* starts, int32_t* lens, int64_t R, int64_t width, int64_t page_size,
+                        int64_t least_pages, void* workspace, size_t workspace_bytes, void* stream) {
+  const char* fn = "pmi_shared_prefixes";
+  if (int rc = check_tables(R, width, table_stride, 0, page_size, fn)) return rc;
+  if (least_pages < 1 || least_pages >= (1ll << 31))
+    return fail(PMI_ERR_INVALID, "%s: least_pages=%lld must be positive", fn, (long long)least_pages);
+  if (R == 0) return ok();
+  if (!kv_lens || !starts || !lens || (width && !tables)) return fail(PMI_ERR_INVALID, "%s: null buffer", fn);
+  const size_t need = pmi_shared_prefixes_workspace_bytes(R);
+  if (!workspace || workspace_bytes < need || !aligned(workspace, 256))
+    return fail(PMI_ERR_INVALID, "%s: needs a 256-byte aligned workspace of %zu bytes", fn, need);
+  const pmi::PagedRuns f = {tables, table_stride, kv_lens, q_starts, starts, lens, (int32_t*)workspace,
+                            (int32_t*)((char*)workspace + pmi::kWsCounterBytes), R, width, page_size, least_pages};
+  return from_hip(pmi::launch_shared_runs(f, (hipStream_t)stream), fn);
+}
+
+int pmi_process_logits(const void* logits, int dtype, int64_t stride, const int32_t* history, int64_t history_stride,
+                       int64_t L, const int32_t* history_lens, const int32_t* prompt_lens, const float* repetition,
+                       const float* presence, const float* frequency, const int32_t* bias_ids, const float* bias,
+                       int64_t n_bias, const int32_t* allowed, int64_t masks, int64_t words,
+                       const int32_t* allowed_rows, void* out, int64_t out_stride, int64_t R, int64_t V,
+                       void* stream) {
+  const char* fn = "pmi_process_logits";
+  const pmi::Logits f = {logits, stride, history, history_stride, L, history_lens, prompt_lens, repetition, presence,
+                         frequency, bias_ids, bias, n_bias, (const uint32_t*)allowed, masks, words, allowed_rows, R, V,
+                         dtype};
+  if (int rc = check_logits(f, fn)) return rc;
+  if (out_stride < V) return fail(PMI_ERR_INVALID, "%s: rows of out may not overlap", fn);
+  if (R == 0 || V == 0) return ok();
+  if (!out || !aligned(out, dtype == PMI_F32 ? 4 : 2))
+    return fail(PMI_ERR_INVALID, "%s: out is null or not aligned to its type", fn);
+  return from_hip(pmi::launch_process_logits(f, out, out_stride, (hipStream_t)stream), fn);
+}
+
+size_t pmi_greedy_tokens_workspace_bytes(int64_t R, int64_t V, int dtype) {
+  if (R <= 0 || R > pmi::kGreedyMaxRows || V <= 0 || V >= (1ll << 30)) return 0;
+  return pmi::greedy_ws_bytes(R, V, dtype);
+}
+
+int pmi_greedy_tokens(const void* logits, int dtype, int64_t stride, const int32_t* history, int64_t history_stride,
+                      int64_t L, const int32_t* history_lens, const int32_t* prompt_lens, const float* repetition,
+                      const float* presence, const float* frequency, const int32_t* bias_ids, const float* bias,
+                      int64_t n_bias, const int32_t* allowed, int64_t masks, int64_t words,
+                      const int32_t* allowed_rows, int64_t* tokens, int64_t token_stride, int64_t R, int64_t V,
+                      void* workspace, size_t workspace_bytes, void* stream) {
+  const char* fn = "pmi_greedy_tokens";
+  const pmi::Logits f = {logits, stride, history, history_stride, L, history_lens, prompt_lens, repetition, presence,
+                         frequency, bias_ids, bias, n_bias, (const uint32_t*)allowed, masks, words, allowed_rows, R, V,
+                         dtype};
+  if (int rc = check_logits(f, fn)) return rc;
+  if (R == 0) return ok();
+  if (V == 0) return fail(PMI_ERR_INVALID, "%s: a row of no tokens has no largest one", fn);
+  if (R > pmi::kGreedyMaxRows)
+    return fail(PMI_ERR_UNSUPPORTED, "%s: at most %lld rows (got %lld)", fn, (long long)pmi::kGreedyMaxRows,
+                (long long)R);
+  if (!tokens || token_stride < 1) return fail(PMI_ERR_INVALID, "%s: null tokens, or a stride below 1", fn);
+  const size_t need = pmi_greedy_tokens_workspace_bytes(R, V, dtype);
+  if (!workspace || workspace_bytes < need || !aligned(workspace, 256))
+    return fail(PMI_ERR_INVALID, "%s: needs a 256-byte aligned workspace of %zu bytes", fn, need);
+  return from_hip(pmi::launch_greedy_tokens(f, tokens, token_stride, workspace, (hipStream_t)stream), fn);
 }
 
 int pmi_quantize_rows(const void* x, int x_dtype, int64_t x_stride, int8_t* codes, float* scales, int64_t M,

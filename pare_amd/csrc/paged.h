@@ -30,6 +30,81 @@ hipError_t launch_release_tables(const int32_t* tables, int64_t stride, int32_t*
                                  int32_t* free_pages, int32_t* pool, int64_t R, int64_t width, int64_t ring,
                                  int64_t ps, hipStream_t stream);
 
+// Requests r that begin as forks of request parents[r] (none: not 0 .. R - 1, or r itself).
+struct PagedFork {
+  int32_t* tables;
+  int64_t stride;
+  int32_t* kv_lens;
+  const int32_t* parents;
+  const int32_t* lengths;  // tokens to begin with, or null: all of the parent's
+  const int32_t* free_pages;
+  int32_t* pool;
+  int32_t* shares;  // [ring] a page's owners beyond the first
+  int32_t* src;     // [R] the page to be copied for r and where to, or -1
+  int32_t* dst;
+  int32_t* from;  // [R] scratch
+  int64_t R, width, ring, ps;
+};
+hipError_t launch_fork_tables(const PagedFork& f, hipStream_t stream);
+
+struct PagedRelease {
+  const int32_t* tables;
+  int64_t stride;
+  int32_t* kv_lens;
+  const uint8_t* done;
+  int32_t* free_pages;
+  int32_t* pool;
+  int32_t* shares;
+  int32_t* counts;  // scratch [page_chunks(ring) + 2]
+  int64_t R, width, ring, ps;
+};
+int64_t page_chunks(int64_t ring);
+hipError_t launch_release_shared(const PagedRelease& f, hipStream_t stream);
+
+struct PagedCompact {
+  int32_t* tables;
+  int64_t stride;
+  const int32_t* kv_lens;
+  int32_t* free_pages;
+  int32_t* pool;
+  int32_t* shares;  // or null
+  int32_t* src;     // [ring / 2]
+  int32_t* dst;
+  int32_t* moves;   // [1] how many of them
+  int32_t* live;    // scratch: [ring], [ring], [page_chunks(ring)]
+  int32_t* to;
+  int32_t* counts;
+  int64_t R, width, ring, ps;
+};
+hipError_t launch_compact_tables(const PagedCompact& f, hipStream_t stream);
+
+constexpr int kCopyLayers = 64;  // of a launch
+struct PagedCopy {
+  void* k[kCopyLayers];
+  void* v[kCopyLayers];
+  float* k_scale[kCopyLayers];
+  float* v_scale[kCopyLayers];
+  const int32_t* src;
+  const int32_t* dst;
+  const int32_t* count;  // entries of them, or null: n
+  int64_t n, layers, pages, KV, page_bytes;
+};
+hipError_t launch_copy_pages(const PagedCopy& f, hipStream_t stream);
+
+// Runs of requests whose first pages are the same.
+struct PagedRuns {
+  const int32_t* tables;
+  int64_t stride;
+  const int32_t* kv_lens;
+  const int32_t* q_starts;  // null: one query a request
+  int32_t* starts;          // [R + 1]
+  int32_t* lens;            // [R]
+  int32_t* counter;         // 0, and 0 again afterwards
+  int32_t* common;          // scratch [R]
+  int64_t R, width, ps, least_pages;
+};
+hipError_t launch_shared_runs(const PagedRuns& f, hipStream_t stream);
+
 struct PagedCache {
   void* k;  // [pages, KV, ps, D] codes
   void* v;  // [pages, KV, ps / 16, D, 16] codes
@@ -61,6 +136,8 @@ struct PagedAttention {
   int64_t window;  // 0: none
   float scale;
   bool bf16;
+  const int32_t* run_starts;  // [R + 1] and [R]: runs of requests that share their first pages, or null
+  const int32_t* run_lens;
 };
 // Whether the count of tiles that the requests of few query rows may have fits 32 bits.
 bool paged_attention_tiles_fit(const PagedAttention& p, const PagedCache& c);
@@ -70,5 +147,12 @@ bool paged_attention_launch_fits(const PagedAttention& p, const PagedCache& c);
 size_t paged_attention_ws_bytes(const PagedAttention& p, const PagedCache& c);
 hipError_t launch_paged_attention(const PagedAttention& p, const PagedCache& c, void* workspace, size_t ws_bytes,
                                   hipStream_t stream);
+
+// Whether a call with runs reads what a run shares once for all of it.
+bool paged_attention_shares(const PagedAttention& p, const PagedCache& c);
+// The same of such a call, two launches.
+bool paged_shared_launch_fits(const PagedAttention& p, const PagedCache& c);
+size_t paged_shared_ws_bytes(const PagedAttention& p, const PagedCache& c);
+hipError_t launch_paged_shared(const PagedAttention& p, const PagedCache& c, void* workspace, hipStream_t stream);
 
 }  // namespace pmi

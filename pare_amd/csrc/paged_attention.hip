@@ -33,10 +33,23 @@ struct AttnArgs {
   int few_wgs;    // workgroups of the few-row part
   int* counters;  // one of each of them, and behind them one of each item of many rows
   float *few_part, *many_part;
+  // runs of requests with the same first pages (kShared, kOwn)
+  const int32_t* run_starts;
+  const int32_t* run_lens;
+  int many_wgs;   // kShared: workgroups that the ranges of keys are made for
+  float* shared;  // the shared part of every query: [T, H, D + 4] values, max, sum
 };
+
+// What a launch computes. kAll: whole rows. Where requests share their first pages these are
+// read once for all of a run, in two launches: kShared takes a run as a request whose queries are
+// those of all its members and whose keys are the shared ones, which all of its queries see, and
+// leaves values, maximum and sum of each row; kOwn takes the requests with the keys behind
+// those, and joins the two.
+enum Part { kAll, kShared, kOwn };
 
 // What a request's queries see, from its row of kv_lens and q_starts.
 struct Request {
+  int row;            // of the tables
   int start, n;       // its queries (none: nothing to do)
   int len, shift;     // its keys, of those within the bounds; query i sees positions up to shift + i
   int first_seen;     // the first position that its first query sees
@@ -45,9 +58,36 @@ struct Request {
 // The first position that a query sees whose last is `last` (negative ones see nothing, and a
 // large window less them would leave the integers).
 PMI_DEV int first_position(const AttnArgs& a, int last) { return a.window && last >= a.window ? last + 1 - a.window : 0; }
+// Positions that request r shares with its run, in whole pages.
+PMI_DEV int shared_len(const AttnArgs& a, int r) {
+  return min(max(a.run_lens[r], 0), a.width * a.ps) & ~(a.ps - 1);
+}
+// The same, or 0 where one of its own queries (from position `shift` on) lies among them.
+PMI_DEV int shared_before(const AttnArgs& a, int r, int shift) {
+  const int len = shared_len(a, r);
+  return shift + 1 > len ? len : 0;
+}
+template <Part PART>
 PMI_DEV Request request(const AttnArgs& a, int r) {
-  const int len0 = a.kv_lens[r];
   Request q;
+  if constexpr (PART == kShared) {
+    const int first = a.run_starts[r], last = a.run_starts[r + 1];
+    const bool run = first >= 0 && first < last && last <= a.R;
+    q.row = run ? first : 0;
+    q.start = run ? first : 0, q.n = run ? last - first : 0;
+    if (run && a.q_starts) {
+      q.start = a.q_starts[first];
+      q.n = a.q_starts[last] - q.start;
+    }
+    q.len = run ? min(shared_len(a, first), a.max_kv) : 0;
+    q.shift = q.len;  // (all queries see all of them)
+    if (q.len == 0 || q.n < 0 || q.start < 0 || (int64_t)q.start + q.n > a.T) q.n = 0;
+    q.first_seen = q.lo = 0;
+    q.hi = a.n_pages ? q.len : 0;
+    return q;
+  }
+  const int len0 = a.kv_lens[r];
+  q.row = r;
   q.start = r, q.n = 1;
   if (a.q_starts) {
     q.start = a.q_starts[r];
@@ -57,7 +97,7 @@ PMI_DEV Request request(const AttnArgs& a, int r) {
   q.shift = max(len0, 0) - q.n;  // (with the keys past the bounds and the queries past max_q)
   q.n = min(q.n, a.max_q);
   if (q.n < 0 || q.start < 0 || (int64_t)q.start + q.n > a.T) q.n = 0;
-  q.first_seen = min(first_position(a, q.shift), q.len);
+  q.first_seen = min(PART == kOwn ? shared_before(a, r, q.shift) : first_position(a, q.shift), q.len);
   q.lo = q.first_seen & ~15;
   q.hi = a.n_pages ? max(q.lo, min(q.len, q.shift + q.n)) : q.lo;
   return q;
@@ -255,7 +295,7 @@ struct FewLds {
   int last;
 };
 
-template <typename T, int D, bool FP8>
+template <typename T, int D, bool FP8, Part PART>
 PMI_DEV void few_rows(const AttnArgs& a, FewLds<D>& lds, int wg) {
   constexpr int DT = D / 16;  // 16-dimension tiles of the output
   float(&s_acc)[4][16][D + 4] = lds.acc;
@@ -275,7 +315,7 @@ PMI_DEV void few_rows(const AttnArgs& a, FewLds<D>& lds, int wg) {
   const int run = (a.R + 63) >> 6, r_lane = run * l;
   int in_lane = 0, parts_lane[kCuts] = {};  // tiles, and parts of cut_of(k) tiles
   for (int x = r_lane; x < min(a.R, r_lane + run); ++x) {
-    const Request rq = request(a, x);
+    const Request rq = request<PART>(a, x);
     const int nt = tiles_of(rq), items = items_of(rq);
     in_lane += nt * items;
 #pragma unroll
@@ -322,7 +362,7 @@ PMI_DEV void few_rows(const AttnArgs& a, FewLds<D>& lds, int wg) {
   int r = run * lane0;
   int off = g - (__builtin_amdgcn_readlane(upto, lane0) - __builtin_amdgcn_readlane(in_lane, lane0));  // tiles of r before g
   while (g < g_end && r < a.R) {
-  const Request rq = request(a, r);
+  const Request rq = request<PART>(a, r);
   const int row_tiles = (rq.n * G + 15) / 16, nt = tiles_of(rq);
   const int span = cut ? (nt + cut - 1) / cut * cut : nt;  // what an item takes of the order
   const int all = span * items_of(rq);
@@ -336,7 +376,7 @@ PMI_DEV void few_rows(const AttnArgs& a, FewLds<D>& lds, int wg) {
   const int item_g = g - tile0;  // the item's first tile of all
   g += n_span, off += n_span;
 
-  const int32_t* table = a.tables + (int64_t)r * a.stride;
+  const int32_t* table = a.tables + (int64_t)rq.row * a.stride;
   auto look_up = [&](int p) { return table[min((p + 16 * h) >> a.ps_log, a.width - 1)]; };
   const int start = rq.start, len = rq.len, shift = rq.shift;
   const int rows = rq.n * G - rt * 16;  // of this tile of rows and the ones behind it
@@ -345,13 +385,13 @@ PMI_DEV void few_rows(const AttnArgs& a, FewLds<D>& lds, int wg) {
   const int i = row / G;
   // positions that this column's query sees: [lo, hi)
   const int hi = live ? max(0, min(len, shift + i + 1)) : 0;
-  const int lo = first_position(a, shift + i);
+  const int lo = PART == kAll ? first_position(a, shift + i) : rq.first_seen;
   const int i_first = rt * 16 / G, i_last = (rt * 16 + min(rows, 16) - 1) / G;
   const int first_seen = rq.first_seen;
   const int p0 = rq.lo + 64 * tile0, p1 = min(rq.hi, p0 + 64 * n_tiles);
   // tiles inside of [safe_lo, safe_hi) need no mask
   const int safe_hi = max(0, min(len, shift + i_first + 1));
-  const int safe_lo = first_position(a, shift + i_last);
+  const int safe_lo = PART == kAll ? first_position(a, shift + i_last) : first_seen;
 
   QueryRow<T, D> q;
   load_query<T, D>(q, (const T*)a.q + (int64_t)(start + (live ? i : 0)) * a.q_token +
@@ -509,8 +549,38 @@ PMI_DEV void few_rows(const AttnArgs& a, FewLds<D>& lds, int wg) {
     }
   }
   const int grow = rt * 16 + orow;
-  T* dst = (T*)a.out + ((int64_t)(start + grow / G) * a.H + kh * G + grow % G) * D + od;
-  auto store = [&](float inv) {
+  const int64_t out_row = (int64_t)(start + grow / G) * a.H + kh * G + grow % G;
+  T* dst = (T*)a.out + out_row * D + od;
+  // the shared part of a row: `dims` of its values from dimension d on
+  auto keep_shared = [&](int64_t row, int d, auto dims, const float* v, float m, float l) {
+    float* rec = a.shared + row * (D + 4);
+#pragma unroll
+    for (int x = 0; x < decltype(dims)::value; x += 4)
+      *reinterpret_cast<f32x4*>(rec + d + x) = f32x4{v[x], v[x + 1], v[x + 2], v[x + 3]};
+    if (d == 0) *reinterpret_cast<float2*>(rec + D) = float2{m, l};
+  };
+  auto join_shared = [&](int64_t row, int d, auto dims, float* v, float& m, float& l) {
+    const float* rec = a.shared + row * (D + 4);
+    const float m0 = m, l0 = l;
+#pragma unroll
+    for (int x = 0; x < decltype(dims)::value; x += 4) {
+      f32x4 o4 = {v[x], v[x + 1], v[x + 2], v[x + 3]};
+      m = m0, l = l0;
+      join(m, l, o4, rec[D], rec[D + 1], *reinterpret_cast<const f32x4*>(rec + d + x), true);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[x + e] = o4[e];
+    }
+  };
+  auto store = [&]() {
+    using Per = std::integral_constant<int, kPer>;
+    if constexpr (PART == kShared) {
+      if (mine) keep_shared(out_row, od, Per{}, o, om, ol);
+      return;
+    }
+    if constexpr (PART == kOwn) {
+      if (mine && first_seen > 0) join_shared(out_row, od, Per{}, o, om, ol);
+    }
+    const float inv = ol > 0.f ? 1.f / ol : (ol != ol ? ol : 0.f);
     typedef T Tv __attribute__((ext_vector_type(kPer)));
     Tv y;
 #pragma unroll
@@ -518,7 +588,7 @@ PMI_DEV void few_rows(const AttnArgs& a, FewLds<D>& lds, int wg) {
     if (mine) *reinterpret_cast<Tv*>(dst) = y;
   };
   if (n_tiles == nt) {
-    store(ol > 0.f ? 1.f / ol : (ol != ol ? ol : 0.f));
+    store();
     __syncthreads();  // s_acc is read
     continue;
   }
@@ -607,13 +677,24 @@ PMI_DEV void few_rows(const AttnArgs& a, FewLds<D>& lds, int wg) {
         const float* f = &s_acc[0][0][0] + (slot + g * left) * (D + 2);
         join(jm, jl, jo, f[0], f[1], f32x4{f[2 + dim], f[3 + dim], f[4 + dim], f[5 + dim]}, true);
       }
-      const float inv = jl > 0.f ? 1.f / jl : (jl != jl ? jl : 0.f);
       const int row1 = rt * 16 + r0 + slot;
+      const int64_t out1 = (int64_t)(start + row1 / G) * a.H + kh * G + row1 % G;
+      using Four = std::integral_constant<int, 4>;
+      if constexpr (PART != kAll) {
+        float v[4] = {jo[0], jo[1], jo[2], jo[3]};
+        if constexpr (PART == kShared) {
+          keep_shared(out1, dim, Four{}, v, jm, jl);
+          continue;
+        }
+        if (first_seen > 0) join_shared(out1, dim, Four{}, v, jm, jl);
+        jo = f32x4{v[0], v[1], v[2], v[3]};
+      }
+      const float inv = jl > 0.f ? 1.f / jl : (jl != jl ? jl : 0.f);
       typedef T T4 __attribute__((ext_vector_type(4)));
       T4 y;
 #pragma unroll
       for (int x = 0; x < 4; ++x) y[x] = (T)(jo[x] * inv);
-      *reinterpret_cast<T4*>((T*)a.out + ((int64_t)(start + row1 / G) * a.H + kh * G + row1 % G) * D + dim) = y;
+      *reinterpret_cast<T4*>((T*)a.out + out1 * D + dim) = y;
     }
   }
   if (tid == 0) __hip_atomic_store(&a.counters[first_wg], 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -621,18 +702,18 @@ PMI_DEV void few_rows(const AttnArgs& a, FewLds<D>& lds, int wg) {
   }
 }
 
-template <typename T, int D, bool FP8>
+template <typename T, int D, bool FP8, Part PART>
 __global__ __launch_bounds__(256, 2) void attention_few_kernel(AttnArgs a) {
   __shared__ __attribute__((aligned(16))) FewLds<D> lds;
-  few_rows<T, D, FP8>(a, lds, blockIdx.x);
+  few_rows<T, D, FP8, PART>(a, lds, blockIdx.x);
 }
 
-template <typename T, int D>
+template <typename T, int D, Part PART>
 hipError_t few(const AttnArgs& a, bool fp8, hipStream_t stream) {
   if (fp8)
-    hipLaunchKernelGGL((attention_few_kernel<T, D, true>), dim3(a.few_wgs), dim3(256), 0, stream, a);
+    hipLaunchKernelGGL((attention_few_kernel<T, D, true, PART>), dim3(a.few_wgs), dim3(256), 0, stream, a);
   else
-    hipLaunchKernelGGL((attention_few_kernel<T, D, false>), dim3(a.few_wgs), dim3(256), 0, stream, a);
+    hipLaunchKernelGGL((attention_few_kernel<T, D, false, PART>), dim3(a.few_wgs), dim3(256), 0, stream, a);
   return hipGetLastError();
 }
 
@@ -657,7 +738,7 @@ hipError_t few(const AttnArgs& a, bool fp8, hipStream_t stream) {
 // (`splits` ranges of `per` tokens), and the last range to arrive joins them.
 constexpr int kRows = 128;
 
-template <typename T, int D, bool FP8>
+template <typename T, int D, bool FP8, Part PART>
 PMI_DEV void many_rows(const AttnArgs& a, uint8_t* lds, int& s_last, int wg) {
   constexpr int KP = D / 64;       // 16-byte pieces of K, and of V, per thread and tile
   constexpr int kSlot = 64 * D * 2;  // bytes of K (or V) of a tile as fp16
@@ -668,11 +749,10 @@ PMI_DEV void many_rows(const AttnArgs& a, uint8_t* lds, int& s_last, int wg) {
   // which rows: the row tiles of all requests in order, each request's last ones (with the most
   // keys) first, the KV heads innermost (an XCD then keeps few heads' keys in its L2)
   auto tiles_of = [&](int r) {
-    const Request rq = request(a, r);
+    const Request rq = request<PART>(a, r);
     return rq.n * G > a.few_rows ? (rq.n * G + kRows - 1) / kRows : 0;
   };
   const int kh = wg % a.KV, rest = wg / a.KV;
-  const int sp = rest % a.splits, index = rest / a.splits;
   const int run = (a.R + 63) >> 6, r_lane = run * l;
   int in_lane = 0;
   for (int x = r_lane; x < min(a.R, r_lane + run); ++x) in_lane += tiles_of(x);
@@ -682,7 +762,12 @@ PMI_DEV void many_rows(const AttnArgs& a, uint8_t* lds, int& s_last, int wg) {
     const int u = __shfl_up(upto, o);
     if (l >= o) upto += u;
   }
-  if (index >= __builtin_amdgcn_readlane(upto, 63)) return;
+  const int all_tiles = __builtin_amdgcn_readlane(upto, 63);
+  // (the host does not know how many runs there are, nor what they share)
+  int splits = a.splits;
+  if constexpr (PART == kShared) splits = all_tiles > 0 ? max(1, a.many_wgs / (all_tiles * a.KV)) : 1;
+  const int sp = rest % splits, index = rest / splits;
+  if (index >= all_tiles) return;
   const int lane0 = __builtin_ctzll(__ballot(upto > index));
   int r = run * lane0;
   int at_tile = index - (__builtin_amdgcn_readlane(upto, lane0) - __builtin_amdgcn_readlane(in_lane, lane0));
@@ -693,22 +778,25 @@ PMI_DEV void many_rows(const AttnArgs& a, uint8_t* lds, int& s_last, int wg) {
     count = tiles_of(r);
   }
   const int rt = count - 1 - at_tile;
-  const Request rq = request(a, r);
+  const Request rq = request<PART>(a, r);
   const int start = rq.start, len = rq.len, shift = rq.shift;
   const int rows = min(kRows, rq.n * G - rt * kRows);
   const int row = rt * kRows + wave * 32 + c;
   const bool live = wave * 32 + c < rows;
   const int i = row / G;
   const int hi = live ? max(0, min(len, shift + i + 1)) : 0;
-  const int lo = first_position(a, shift + i);
+  const int lo = PART == kAll ? first_position(a, shift + i) : rq.first_seen;
   const int i_first = rt * kRows / G, i_last = (rt * kRows + rows - 1) / G;
-  const int first_seen = min(first_position(a, shift + i_first), len), all_lo = first_seen & ~15;
+  const int first_seen = PART == kAll ? min(first_position(a, shift + i_first), len) : rq.first_seen;
+  const int all_lo = first_seen & ~15;
   const int all_hi = a.n_pages ? max(all_lo, min(len, shift + i_last + 1)) : all_lo;
-  const int parts = max(1, (all_hi - all_lo + a.per - 1) / a.per);
+  // a range of at least eight tiles, as its join costs about two
+  const int per = PART == kShared ? max(512, ((len + splits - 1) / splits + 63) & ~63) : a.per;
+  const int parts = max(1, (all_hi - all_lo + per - 1) / per);
   if (sp >= parts) return;
-  const int p0 = all_lo + sp * a.per, p1 = min(all_hi, p0 + a.per);
+  const int p0 = all_lo + sp * per, p1 = min(all_hi, p0 + per);
   const int safe_hi = max(0, min(len, shift + i_first + 1));
-  const int safe_lo = first_position(a, shift + i_last);
+  const int safe_lo = PART == kAll ? first_position(a, shift + i_last) : first_seen;
 
   // the wave's query rows: step s holds dimensions 16 s + 8 h .. + 7
   f16x8 qv[D / 16];
@@ -749,7 +837,7 @@ PMI_DEV void many_rows(const AttnArgs& a, uint8_t* lds, int& s_last, int wg) {
     for (int e = 0; e < 16; ++e) acc[d][e] = 0.f;
   Row ref;
   float sum = 0.f;
-  const int32_t* table = a.tables + (int64_t)r * a.stride;
+  const int32_t* table = a.tables + (int64_t)rq.row * a.stride;
   const int64_t cell_bytes = (int64_t)a.ps * D;
 
   // The four blocks of the tile at p, block b in the lanes with l % 4 = b, so that their pages and
@@ -923,7 +1011,43 @@ PMI_DEV void many_rows(const AttnArgs& a, uint8_t* lds, int& s_last, int wg) {
   sum += __shfl_xor(sum, 32);
   const float unit = unit_of(ref);
   typedef T T4 __attribute__((ext_vector_type(4)));
-  T* dst = (T*)a.out + ((int64_t)(start + i) * a.H + kh * G + row - i * G) * D + 4 * h;
+  const int64_t out_row = (int64_t)(start + i) * a.H + kh * G + row - i * G;
+  T* dst = (T*)a.out + out_row * D + 4 * h;
+  if (PART == kShared && parts == 1) {
+    float* rec = a.shared + out_row * (D + 4);
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        f32x4 y;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] = acc[d][4 * j + e] * unit;
+        if (live) *reinterpret_cast<f32x4*>(rec + 32 * d + 8 * j + 4 * h) = y;
+      }
+    if (live && h == 0) *reinterpret_cast<float2*>(rec + D) = float2{ref.max, sum};
+    return;
+  }
+  if (PART == kOwn && parts == 1 && first_seen > 0) {
+    const float* rec = a.shared + out_row * (D + 4);
+    const float pm = live ? rec[D] : 0.f, pl = live ? rec[D + 1] : 0.f;
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float m = ref.max, l = sum;
+        f32x4 y;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] = acc[d][4 * j + e] * unit;
+        if (!live) continue;
+        join(m, l, y, pm, pl, *reinterpret_cast<const f32x4*>(rec + 32 * d + 8 * j + 4 * h), true);
+        const float inv = l > 0.f ? 1.f / l : (l != l ? l : 0.f);
+        T4 o;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = (T)(y[e] * inv);
+        *reinterpret_cast<T4*>(dst + 32 * d + 8 * j) = o;
+      }
+    return;
+  }
   if (parts == 1) {
     const float inv = sum > 0.f ? unit / sum : (sum != sum ? sum : 0.f);
 #pragma unroll
@@ -941,7 +1065,7 @@ PMI_DEV void many_rows(const AttnArgs& a, uint8_t* lds, int& s_last, int wg) {
   // partial rows, as in the kernel above: values, max, sum
   constexpr int kSc1 = 16, kRec = D + 4;
   const int item = index * a.KV + kh;
-  const __amdgpu_buffer_rsrc_t rp = rsrc(a.many_part + (int64_t)item * a.splits * kRows * kRec, (int64_t)parts * kRows * kRec * 4);
+  const __amdgpu_buffer_rsrc_t rp = rsrc(a.many_part + (int64_t)item * splits * kRows * kRec, (int64_t)parts * kRows * kRec * 4);
   const int rrow = wave * 32 + c;
   if (live) {
     const int rec = (sp * kRows + rrow) * kRec * 4;
@@ -986,12 +1110,23 @@ PMI_DEV void many_rows(const AttnArgs& a, uint8_t* lds, int& s_last, int wg) {
 #pragma unroll
       for (int k = 0; k < 4; ++k) join(jm, jl, jo, ms[k], ls[k], v[k], s0 + k < parts);
     }
-    const float inv = jl > 0.f ? 1.f / jl : (jl != jl ? jl : 0.f);
     const int grow = rt * kRows + y;
+    const int64_t out1 = (int64_t)(start + grow / G) * a.H + kh * G + grow % G;
+    if constexpr (PART == kShared) {
+      float* rec = a.shared + out1 * (D + 4);
+      *reinterpret_cast<f32x4*>(rec + dim) = jo;
+      if (dim == 0) *reinterpret_cast<float2*>(rec + D) = float2{jm, jl};
+      continue;
+    }
+    if (PART == kOwn && first_seen > 0) {
+      const float* rec = a.shared + out1 * (D + 4);
+      join(jm, jl, jo, rec[D], rec[D + 1], *reinterpret_cast<const f32x4*>(rec + dim), true);
+    }
+    const float inv = jl > 0.f ? 1.f / jl : (jl != jl ? jl : 0.f);
     T4 o;
 #pragma unroll
     for (int e = 0; e < 4; ++e) o[e] = (T)(jo[e] * inv);
-    *reinterpret_cast<T4*>((T*)a.out + ((int64_t)(start + grow / G) * a.H + kh * G + grow % G) * D + dim) = o;
+    *reinterpret_cast<T4*>((T*)a.out + out1 * D + dim) = o;
   }
   if (tid == 0) __hip_atomic_store(&a.counters[a.few_wgs + item], 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
@@ -1000,24 +1135,24 @@ PMI_DEV void many_rows(const AttnArgs& a, uint8_t* lds, int& s_last, int wg) {
 // fills with the other (32 / 8 heads of 128: 8 single tokens of 2000 keys and a prompt of 2048 72 us, in
 // two launches 81; 32 of 3000 and a chunk of 512 behind 1000 79 and 84; two prompts of 300, where the
 // first find nothing to do, 17.6 and 18.6).
-template <typename T, int D, bool FP8>
+template <typename T, int D, bool FP8, Part PART>
 __global__ __launch_bounds__(256, 2) void attention_rows_kernel(AttnArgs a) {
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];  // [2 slots][K, V]
   __shared__ int s_last;
   static_assert(sizeof(FewLds<D>) <= 2 * 2 * 64 * D * 2, "fits the slots");
   if ((int)blockIdx.x < a.few_wgs)
-    few_rows<T, D, FP8>(a, *reinterpret_cast<FewLds<D>*>(lds), blockIdx.x);
+    few_rows<T, D, FP8, PART>(a, *reinterpret_cast<FewLds<D>*>(lds), blockIdx.x);
   else
-    many_rows<T, D, FP8>(a, lds, s_last, blockIdx.x - a.few_wgs);
+    many_rows<T, D, FP8, PART>(a, lds, s_last, blockIdx.x - a.few_wgs);
 }
 
-template <typename T, int D>
+template <typename T, int D, Part PART>
 hipError_t many(const AttnArgs& a, bool fp8, int64_t wgs, hipStream_t stream) {
   constexpr int kLds = 2 * 2 * 64 * D * 2;
   if (fp8)
-    hipLaunchKernelGGL((attention_rows_kernel<T, D, true>), dim3((unsigned)wgs), dim3(256), kLds, stream, a);
+    hipLaunchKernelGGL((attention_rows_kernel<T, D, true, PART>), dim3((unsigned)wgs), dim3(256), kLds, stream, a);
   else
-    hipLaunchKernelGGL((attention_rows_kernel<T, D, false>), dim3((unsigned)wgs), dim3(256), kLds, stream, a);
+    hipLaunchKernelGGL((attention_rows_kernel<T, D, false, PART>), dim3((unsigned)wgs), dim3(256), kLds, stream, a);
   return hipGetLastError();
 }
 
@@ -1083,8 +1218,10 @@ size_t paged_attention_ws_bytes(const PagedAttention& p, const PagedCache& c) {
   return kWsCounterBytes + few_part_bytes(c.D) + many_plan(p, c).part;
 }
 
-hipError_t launch_paged_attention(const PagedAttention& p, const PagedCache& c, void* workspace, size_t ws_bytes,
-                                  hipStream_t stream) {
+namespace {
+
+// The arguments that all parts of a call have in common.
+AttnArgs attention_args(const PagedAttention& p, const PagedCache& c, void* workspace) {
   AttnArgs a = {p.q, p.out, (const uint8_t*)c.k, (const uint8_t*)c.v, c.k_scale, c.v_scale, p.tables, p.kv_lens,
                 p.q_starts, p.stride, p.q_token, p.q_head, c.pages, (int)p.T, (int)p.R, (int)p.width, (int)p.H,
                 (int)c.KV, (int)c.ps, __builtin_ctz((unsigned)c.ps), (int)p.window, p.scale};
@@ -1094,17 +1231,68 @@ hipError_t launch_paged_attention(const PagedAttention& p, const PagedCache& c, 
   a.few_part = (float*)((char*)workspace + kWsCounterBytes);
   a.many_part = (float*)((char*)a.few_part + few_part_bytes(c.D));
   a.few_wgs = few_wgs(c.D);
-  const ManyPlan f = many_plan(p, c);
-  if (f.items == 0) {
-    if (p.bf16) return c.D == 64 ? few<__bf16, 64>(a, c.fp8, stream) : few<__bf16, 128>(a, c.fp8, stream);
-    return c.D == 64 ? few<f16, 64>(a, c.fp8, stream) : few<f16, 128>(a, c.fp8, stream);
+  a.run_starts = p.run_starts, a.run_lens = p.run_lens;
+  return a;
+}
+
+// Requests of few rows alone (n = 0), or n workgroups of both.
+template <Part PART>
+hipError_t launch_part(const AttnArgs& a, const PagedAttention& p, const PagedCache& c, int64_t n, hipStream_t stream) {
+  if (n == 0) {
+    if (p.bf16) return c.D == 64 ? few<__bf16, 64, PART>(a, c.fp8, stream) : few<__bf16, 128, PART>(a, c.fp8, stream);
+    return c.D == 64 ? few<f16, 64, PART>(a, c.fp8, stream) : few<f16, 128, PART>(a, c.fp8, stream);
   }
+  if (p.bf16)
+    return c.D == 64 ? many<__bf16, 64, PART>(a, c.fp8, n, stream) : many<__bf16, 128, PART>(a, c.fp8, n, stream);
+  return c.D == 64 ? many<f16, 64, PART>(a, c.fp8, n, stream) : many<f16, 128, PART>(a, c.fp8, n, stream);
+}
+
+// Row tiles of all runs x KV heads, at most: those of many rows, of which each has at least kFewRows + 1.
+int64_t shared_items(const PagedAttention& p, const PagedCache& c) {
+  const int64_t G = p.H / c.KV, rows = p.T * G;
+  if (rows <= kFewRows) return 0;
+  const int64_t runs = rows / (kFewRows + 1) < p.R ? rows / (kFewRows + 1) : p.R;
+  return (rows / kRows + runs) * c.KV;
+}
+int64_t shared_part_bytes(const PagedAttention& p, const PagedCache& c) {
+  return shared_items(p, c) ? (int64_t)2 * device_cu_count() * kRows * (c.D + 4) * 4 : 0;
+}
+
+}  // namespace
+
+bool paged_attention_shares(const PagedAttention& p, const PagedCache& c) {
+  return p.R > 1 && p.T < (1ll << 30) && p.window == 0 && p.max_q * (p.H / c.KV) <= kFewRows;
+}
+
+bool paged_shared_launch_fits(const PagedAttention& p, const PagedCache& c) {
+  return few_wgs(c.D) + shared_items(p, c) + 2 * device_cu_count() < (1ll << 24);
+}
+
+size_t paged_shared_ws_bytes(const PagedAttention& p, const PagedCache& c) {
+  return kWsCounterBytes + few_part_bytes(c.D) + (size_t)shared_part_bytes(p, c) + (size_t)(p.T * p.H * (c.D + 4) * 4);
+}
+
+hipError_t launch_paged_shared(const PagedAttention& p, const PagedCache& c, void* workspace, hipStream_t stream) {
+  AttnArgs a = attention_args(p, c, workspace);
+  a.shared = (float*)((char*)a.many_part + shared_part_bytes(p, c));
+  const int64_t items = shared_items(p, c);
+  a.many_wgs = 2 * device_cu_count();
+  const int64_t wgs = items > a.many_wgs ? items : a.many_wgs;
+  a.max_q = (int)p.T;
+  if (hipError_t e = launch_part<kShared>(a, p, c, items ? a.few_wgs + wgs : 0, stream); e != hipSuccess) return e;
+  a.max_q = (int)p.max_q;
+  return launch_part<kOwn>(a, p, c, 0, stream);
+}
+
+hipError_t launch_paged_attention(const PagedAttention& p, const PagedCache& c, void* workspace, size_t ws_bytes,
+                                  hipStream_t stream) {
+  AttnArgs a = attention_args(p, c, workspace);
+  const ManyPlan f = many_plan(p, c);
+  if (f.items == 0) return launch_part<kAll>(a, p, c, 0, stream);
   // Any batch of several requests may have some of few rows; a lone one stays with many.
   if (p.R == 1) a.few_rows = 0, a.few_wgs = 0;
   a.splits = f.splits, a.per = f.per;
-  const int64_t n = a.few_wgs + f.items * f.splits;
-  if (p.bf16) return c.D == 64 ? many<__bf16, 64>(a, c.fp8, n, stream) : many<__bf16, 128>(a, c.fp8, n, stream);
-  return c.D == 64 ? many<f16, 64>(a, c.fp8, n, stream) : many<f16, 128>(a, c.fp8, n, stream);
+  return launch_part<kAll>(a, p, c, a.few_wgs + f.items * f.splits, stream);
 }
 
 }  // namespace pmi

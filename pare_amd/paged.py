@@ -7,6 +7,13 @@ RoPE (``rope_append_kv``), attention of one or many new tokens per request
 (``paged_attention``) and the read of whole pages (``read_kv_pages``).
 ``PagedKVCache`` holds the buffers of a model's layers and makes these calls.
 
+Requests may own pages together (``shares``, int32 [pages], counts a page's owners beyond
+the first): ``fork_block_tables`` lets a request begin with another one's tokens,
+``release_block_tables`` gives back what nobody else owns, ``compact_block_tables`` moves the
+live pages to the cache's front, ``copy_kv_pages`` copies what both say. ``shared_prefixes``
+finds the requests of a step whose first pages are the same, and ``paged_attention`` then
+reads those once for all of them.
+
 The cache: codes int8 or float8_e4m3fn, code * scale = value,
   k_cache [pages, KV, page_size, D], v_cache [pages, KV, page_size / 16, D, 16]
   (token 16 b + j of a page at [b, :, j]), k_scale and v_scale fp32 [pages, KV].
@@ -17,7 +24,8 @@ reference serves through HuggingFace's cache (pare/eval/throughput.py:84-126).
 
 from __future__ import annotations
 
-from typing import NamedTuple
+import ctypes
+from typing import NamedTuple, Sequence
 
 import torch
 
@@ -38,6 +46,22 @@ class BatchPlan(NamedTuple):
     positions: torch.Tensor  # [total] position of each new token
     slots: torch.Tensor      # [total] page * page_size + offset, -1: not stored
     pool: torch.Tensor       # [4] head and count of the free ring, requests refused, 0
+
+
+class PageMoves(NamedTuple):
+    """Pages to be copied: ``src[i]`` to ``dst[i]`` (int32 [n], -1: none), of the first
+    ``count[0]`` (int32 [1], on the device) if there is one."""
+
+    src: torch.Tensor
+    dst: torch.Tensor
+    count: torch.Tensor | None
+
+
+class SharedPrefixes(NamedTuple):
+    """Runs of neighbouring requests that begin with the same pages (``shared_prefixes``)."""
+
+    starts: torch.Tensor  # int32 [R + 1] the first request of each run, R behind the last
+    lens: torch.Tensor    # int32 [R] positions that the members of a request's run share
 
 
 def _hip(t: torch.Tensor, fn: str) -> torch.device:
@@ -132,9 +156,12 @@ def extend_block_tables(block_tables: torch.Tensor, kv_lens: torch.Tensor, new_l
 
 
 def release_block_tables(block_tables: torch.Tensor, kv_lens: torch.Tensor, done: torch.Tensor,
-                         free_pages: torch.Tensor, pool: torch.Tensor, page_size: int) -> None:
+                         free_pages: torch.Tensor, pool: torch.Tensor, page_size: int, *,
+                         shares: torch.Tensor | None = None) -> None:
     """Gives the pages of the requests with ``done[r]`` (bool [R]) back to the ring of
-    free pages, in request order, and sets their ``kv_lens`` to 0."""
+    free pages, in request order, and sets their ``kv_lens`` to 0. With ``shares`` (int32
+    [pages]) a page loses an owner for each of them, and goes back when it has none left,
+    in the order of the pages' numbers."""
     dev = _hip(block_tables, "release_block_tables")
     R = block_tables.shape[0]
     _tables(block_tables, dev, R)
@@ -144,11 +171,144 @@ def release_block_tables(block_tables: torch.Tensor, kv_lens: torch.Tensor, done
     assert (done.dtype == torch.bool and done.dim() == 1 and done.numel() == R and done.is_contiguous()
             and done.device == dev), (
         f"done must be a contiguous bool [{R}] tensor on {dev}")
+    if shares is not None:
+        _ints(dev, free_pages.numel(), shares=shares)
+        L = _lib.lib()
+        nbytes = L.pmi_release_shared_scratch_bytes(free_pages.numel())
+        scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        with _DeviceGuard(dev):
+            _lib.check(L.pmi_release_shared_block_tables(
+                block_tables.data_ptr(), _row_stride(block_tables), kv_lens.data_ptr(), done.data_ptr(),
+                free_pages.data_ptr(), pool.data_ptr(), shares.data_ptr(), R, block_tables.shape[1],
+                free_pages.numel(), page_size, scratch.data_ptr(), nbytes, _raw_stream(dev)),
+                "pmi_release_shared_block_tables")
+        return
     with _DeviceGuard(dev):
         _lib.check(_lib.lib().pmi_release_block_tables(
             block_tables.data_ptr(), _row_stride(block_tables), kv_lens.data_ptr(), done.data_ptr(),
             free_pages.data_ptr(), pool.data_ptr(), R, block_tables.shape[1], free_pages.numel(), page_size,
             _raw_stream(dev)), "pmi_release_block_tables")
+
+
+def fork_block_tables(block_tables: torch.Tensor, kv_lens: torch.Tensor, parents: torch.Tensor,
+                      free_pages: torch.Tensor, pool: torch.Tensor, shares: torch.Tensor, page_size: int, *,
+                      lengths: torch.Tensor | None = None) -> PageMoves:
+    """Request r begins with the first ``lengths[r]`` (int32 [R]; None, or more than there are: all)
+    tokens of request ``parents[r]`` (int32 [R]; itself, or none of 0 .. R - 1: nothing
+    happens), in place and without the host knowing any length.
+
+    Their whole pages are owned by both from now on (``shares`` int32 [pages] counts a page's
+    owners beyond the first); a last page that they do not fill is copied to a page from the ring:
+    the returned moves ([R]) are for ``copy_kv_pages``, on the same stream. A parent is what it was
+    before the call. Refused, and counted in ``pool[2]``, is a request that holds tokens, or that
+    needs a page when the needs up to it exceed the pool."""
+    dev = _hip(block_tables, "fork_block_tables")
+    R, width = block_tables.shape[0], block_tables.shape[1] if block_tables.dim() == 2 else 0
+    _tables(block_tables, dev, R)
+    _ints(dev, R, kv_lens=kv_lens, parents=parents)
+    _ints(dev, free_pages=free_pages)
+    _ints(dev, free_pages.numel(), shares=shares)
+    _ints(dev, 4, pool=pool)
+    if lengths is not None:
+        _ints(dev, R, lengths=lengths)
+    src, dst, scratch = torch.empty(3, R, dtype=torch.int32, device=dev)
+    with _DeviceGuard(dev):
+        _lib.check(_lib.lib().pmi_fork_block_tables(
+            block_tables.data_ptr(), _row_stride(block_tables), kv_lens.data_ptr(), parents.data_ptr(),
+            lengths.data_ptr() if lengths is not None else None, free_pages.data_ptr(), pool.data_ptr(),
+            shares.data_ptr(), src.data_ptr(), dst.data_ptr(), scratch.data_ptr(), R, width, free_pages.numel(),
+            page_size, _raw_stream(dev)), "pmi_fork_block_tables")
+    return PageMoves(src, dst, None)
+
+
+def compact_block_tables(block_tables: torch.Tensor, kv_lens: torch.Tensor, free_pages: torch.Tensor,
+                         pool: torch.Tensor, shares: torch.Tensor | None, page_size: int) -> PageMoves:
+    """Makes the n pages that the requests hold (by ``kv_lens`` and ``block_tables``) pages
+    0 .. n - 1, in place: those from n on, in order, take the places of the free ones before it, in order.
+    Pages n, n + 1, .. are the ring's free ones afterwards, in that order, also pages that
+    neither a request nor the ring held. The returned moves ([pages / 2], as many as ``count``
+    says) are for ``copy_kv_pages``, on the same stream. ``shares``: as in ``fork_block_tables``, or
+    None."""
+    dev = _hip(block_tables, "compact_block_tables")
+    R, width = block_tables.shape[0], block_tables.shape[1] if block_tables.dim() == 2 else 0
+    _tables(block_tables, dev, R)
+    _ints(dev, R, kv_lens=kv_lens)
+    _ints(dev, free_pages=free_pages)
+    pages = free_pages.numel()
+    _ints(dev, 4, pool=pool)
+    if shares is not None:
+        _ints(dev, pages, shares=shares)
+    L = _lib.lib()
+    nbytes = L.pmi_compact_scratch_bytes(pages)
+    src, dst, count, scratch = torch.empty(2 * (pages // 2) + 1 + nbytes // 4, dtype=torch.int32, device=dev).split(
+        [pages // 2, pages // 2, 1, nbytes // 4])
+    with _DeviceGuard(dev):
+        if pages == 0:
+            count.zero_()
+        _lib.check(L.pmi_compact_block_tables(
+            block_tables.data_ptr(), _row_stride(block_tables), kv_lens.data_ptr(), free_pages.data_ptr(),
+            pool.data_ptr(), shares.data_ptr() if shares is not None else None, src.data_ptr(), dst.data_ptr(),
+            count.data_ptr(), R, width, pages, page_size, scratch.data_ptr(), nbytes, _raw_stream(dev)),
+            "pmi_compact_block_tables")
+    return PageMoves(src, dst, count)
+
+
+def copy_kv_pages(moves: PageMoves, k_caches: Sequence[torch.Tensor], v_caches: Sequence[torch.Tensor],
+                  k_scales: Sequence[torch.Tensor], v_scales: Sequence[torch.Tensor]) -> None:
+    """Copies the pages of ``moves``, codes and scales, in the caches of all layers (sequences of as
+    many tensors each, all of the same sizes and type), in one launch per 64 layers. Pairs
+    with a page that the cache does not have are left out; no page may be copied to twice, or be copied
+    from and to."""
+    n = len(k_caches)
+    assert len(v_caches) == n and len(k_scales) == n and len(v_scales) == n, (
+        "the caches and scales must be sequences of one tensor a layer")
+    dev = _hip(moves.src, "copy_kv_pages")
+    _ints(dev, moves.src.numel(), src=moves.src, dst=moves.dst)
+    if moves.count is not None:
+        _ints(dev, 1, count=moves.count)
+    if n == 0:
+        return
+    sizes = None
+    for layer in zip(k_caches, v_caches, k_scales, v_scales):
+        mine = _cache(dev, *layer)
+        assert sizes is None or mine == sizes, "the caches of all layers must have the same sizes and type"
+        sizes = mine
+    pages, KV, ps, D, _ = sizes
+    pointers = [(ctypes.c_void_p * n)(*[t.data_ptr() for t in ts]) for ts in (k_caches, v_caches, k_scales, v_scales)]
+    with _DeviceGuard(dev):
+        _lib.check(_lib.lib().pmi_copy_kv_pages(
+            moves.src.data_ptr(), moves.dst.data_ptr(), moves.count.data_ptr() if moves.count is not None else None,
+            moves.src.numel(), *pointers, n, pages, ps, KV, D, _raw_stream(dev)), "pmi_copy_kv_pages")
+
+
+def shared_prefixes(block_tables: torch.Tensor, kv_lens: torch.Tensor, q_starts: torch.Tensor | None,
+                    page_size: int, *, least: int = 256) -> SharedPrefixes:
+    """Which neighbouring requests of a step begin with the same pages, for ``paged_attention``.
+
+    ``kv_lens`` int32 [R] with the new tokens that ``q_starts`` int32 [R + 1] counts (None: one
+    each). A request joins the run of the request with new tokens before it if at least
+    ``least`` positions of theirs, in whole pages before their new tokens, lie in the same pages;
+    the members of a run share what all of them have in common."""
+    dev = _hip(block_tables, "shared_prefixes")
+    R, width = block_tables.shape[0], block_tables.shape[1] if block_tables.dim() == 2 else 0
+    _tables(block_tables, dev, R)
+    _ints(dev, R, kv_lens=kv_lens)
+    if q_starts is not None:
+        _ints(dev, R + 1, q_starts=q_starts)
+    assert least >= 1, "least must be at least one position"
+    starts, lens = torch.empty(2 * R + 1, dtype=torch.int32, device=dev).split([R + 1, R])
+    L = _lib.lib()
+    with _DeviceGuard(dev):
+        stream = _raw_stream(dev)
+        if R == 0:
+            starts.zero_()
+        ws = _workspace(dev, stream, L.pmi_shared_prefixes_workspace_bytes(R))
+        _lib.check(L.pmi_shared_prefixes(
+            block_tables.data_ptr(), _row_stride(block_tables), kv_lens.data_ptr(),
+            q_starts.data_ptr() if q_starts is not None else None, starts.data_ptr(), lens.data_ptr(), R, width,
+            page_size, -(-least // max(page_size, 1)), ws.data_ptr() if ws is not None else None,
+            ws.numel() if ws is not None else 0, stream), "pmi_shared_prefixes")
+    return SharedPrefixes(starts, lens)
 
 
 def rope_append_kv(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, positions: torch.Tensor,
@@ -210,7 +370,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
                     v_scale: torch.Tensor, block_tables: torch.Tensor, kv_lens: torch.Tensor,
                     q_starts: torch.Tensor | None = None, *, scale: float, window: int = 0,
                     max_q_len: int | None = None, max_kv_len: int | None = None,
-                    out: torch.Tensor | None = None) -> torch.Tensor:
+                    out: torch.Tensor | None = None, shared: SharedPrefixes | None = None) -> torch.Tensor:
     """Attention [T, H, D] of the queries ``q`` [T, H, D] (fp16 or bf16, any token and head
     strides) over the cache.
 
@@ -221,7 +381,11 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     left as they were (``out``) or undefined. ``max_q_len`` and ``max_kv_len`` bound what
     a request has (default: all of q, the table's width): tighter bounds make the call
     faster, and queries and keys past them are left out.
-    ``scale`` multiplies q . k."""
+    ``scale`` multiplies q . k.
+
+    ``shared``: what ``shared_prefixes`` says of the same tables, lengths and queries. The result
+    is the same but for roundings; keys that a run of requests shares are read once for all of it,
+    where no request has more than 64 query rows (``max_q_len`` H / KV) and there is no window."""
     dev = _hip(q, "paged_attention")
     pages, KV, ps, D, code = _cache(dev, k_cache, v_cache, k_scale, v_scale)
     assert q.dim() == 3 and q.shape[2] == D and q.dtype in (torch.float16, torch.bfloat16), (
@@ -249,6 +413,21 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     max_kv = width * ps if max_kv_len is None else min(max_kv_len, width * ps)
     assert max_kv >= 0, "max_kv_len may not be negative"
     L = _lib.lib()
+    if shared is not None:
+        _ints(dev, R + 1, starts=shared.starts)
+        _ints(dev, R, lens=shared.lens)
+        with _DeviceGuard(dev):
+            stream = _raw_stream(dev)
+            ws = _workspace(dev, stream, L.pmi_paged_attention_shared_workspace_bytes(T, R, H, KV, D, max_q, max_kv,
+                                                                                      window))
+            _lib.check(L.pmi_paged_attention_shared(
+                q.data_ptr(), _VALUES[q.dtype], q.stride(0), q.stride(1), k_cache.data_ptr(), v_cache.data_ptr(),
+                k_scale.data_ptr(), v_scale.data_ptr(), code, pages, ps, block_tables.data_ptr(),
+                _row_stride(block_tables), kv_lens.data_ptr(), q_starts.data_ptr() if q_starts is not None else None,
+                shared.starts.data_ptr(), shared.lens.data_ptr(), out.data_ptr(), T, R, width, H, KV, D, max_q,
+                max_kv, window, scale, ws.data_ptr() if ws is not None else None,
+                ws.numel() if ws is not None else 0, stream), "pmi_paged_attention_shared")
+        return out
     with _DeviceGuard(dev):
         stream = _raw_stream(dev)
         nbytes = L.pmi_paged_attention_workspace_bytes(T, R, H, KV, D, max_q, max_kv, window)
@@ -270,10 +449,15 @@ class PagedKVCache:
     for all of them at full length). ``extend`` makes room for a step's new tokens (never
     past ``max_len``, so RoPE tables of as many positions do),
     ``append`` writes them layer by layer, ``attend`` reads, ``release`` gives a finished
-    request's pages back. ``pool[2]`` counts requests that ``extend`` refused."""
+    request's pages back. ``pool[2]`` counts requests that ``extend`` and ``fork`` refused.
+
+    With ``sharing`` requests may begin as forks of others (``fork``), whose whole pages they then
+    own together; ``shared_prefixes`` tells ``attend`` which those are. ``compact`` moves the
+    live pages to the front, ``resize`` changes how many pages there are."""
 
     def __init__(self, layers: int, requests: int, max_len: int, kv_heads: int, head_dim: int, device, *,
-                 page_size: int = 64, pages: int | None = None, dtype: torch.dtype = torch.int8) -> None:
+                 page_size: int = 64, pages: int | None = None, dtype: torch.dtype = torch.int8,
+                 sharing: bool = False) -> None:
         if dtype not in _CODES:
             raise ValueError("the cache holds int8 or float8_e4m3fn codes")
         if page_size not in (16, 32, 64, 128, 256):
@@ -296,11 +480,14 @@ class PagedKVCache:
         self.kv_lens = torch.zeros(requests, dtype=torch.int32, device=dev)
         self.free_pages = torch.arange(pages, dtype=torch.int32, device=dev)
         self.pool = torch.tensor([0, pages, 0, 0], dtype=torch.int32, device=dev)
+        self.shares = torch.zeros(pages, dtype=torch.int32, device=dev) if sharing else None
 
     def reset(self) -> None:
         """An empty cache: every page free."""
         pages = self.free_pages.numel()
         self.kv_lens.zero_()
+        if self.shares is not None:
+            self.shares.zero_()
         torch.arange(pages, out=self.free_pages)
         self.pool.zero_()
         self.pool[1:2].fill_(pages)  # (from the host's memory it would wait for the device)
@@ -312,7 +499,50 @@ class PagedKVCache:
                                    max_len=self.max_len)
 
     def release(self, done: torch.Tensor) -> None:
-        release_block_tables(self.block_tables, self.kv_lens, done, self.free_pages, self.pool, self.page_size)
+        release_block_tables(self.block_tables, self.kv_lens, done, self.free_pages, self.pool, self.page_size,
+                             shares=self.shares)
+
+    def fork(self, parents: torch.Tensor, lengths: torch.Tensor | None = None) -> None:
+        """``fork_block_tables`` in place, with the copies of all layers."""
+        if self.shares is None:
+            raise RuntimeError("fork needs a cache made with sharing=True")
+        self._copy(fork_block_tables(self.block_tables, self.kv_lens, parents, self.free_pages, self.pool, self.shares,
+                                     self.page_size, lengths=lengths))
+
+    def compact(self) -> None:
+        """``compact_block_tables`` in place, with the copies of all layers."""
+        self._copy(compact_block_tables(self.block_tables, self.kv_lens, self.free_pages, self.pool, self.shares,
+                                        self.page_size))
+
+    def _copy(self, moves: PageMoves) -> None:
+        copy_kv_pages(moves, self.k, self.v, self.k_scale, self.v_scale)
+
+    def resize(self, pages: int) -> None:
+        """A cache of ``pages`` pages with the same requests, after ``compact``. The buffers are new
+        ones (a graph captured before writes to the old ones), and the call waits for the device."""
+        if pages < 1:
+            raise ValueError("pages must be positive")
+        self.compact()
+        old, dev = self.free_pages.numel(), self.free_pages.device
+        live = old - int(self.pool[1])
+        if pages < live:
+            raise ValueError(f"the requests hold {live} pages, more than {pages}")
+        for buffers in (self.k, self.v, self.k_scale, self.v_scale):
+            for i, t in enumerate(buffers):
+                raw = t.view(torch.uint8) if t.dtype != torch.float32 else t
+                new = torch.zeros(pages, *t.shape[1:], dtype=raw.dtype, device=dev)
+                new[:live] = raw[:live]
+                buffers[i] = new.view(t.dtype)
+        if self.shares is not None:
+            shares = torch.zeros(pages, dtype=torch.int32, device=dev)
+            shares[:live] = self.shares[:live]
+            self.shares = shares
+        self.free_pages = ((torch.arange(pages, device=dev) + live) % pages).to(torch.int32)
+        self.pool[1:2].fill_(pages - live)
+
+    def shared_prefixes(self, plan: BatchPlan, least: int = 256) -> SharedPrefixes:
+        """Which of the plan's requests begin with the same pages, for ``attend``: once a step."""
+        return shared_prefixes(self.block_tables, plan.kv_lens, plan.q_starts, self.page_size, least=least)
 
     def append(self, layer: int, qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
                plan: BatchPlan) -> torch.Tensor:
@@ -320,7 +550,8 @@ class PagedKVCache:
                               self.k_scale[layer], self.v_scale[layer])
 
     def attend(self, layer: int, q: torch.Tensor, plan: BatchPlan, *, scale: float, window: int = 0,
-               max_q_len: int | None = None, max_kv_len: int | None = None) -> torch.Tensor:
+               max_q_len: int | None = None, max_kv_len: int | None = None,
+               shared: SharedPrefixes | None = None) -> torch.Tensor:
         return paged_attention(q, self.k[layer], self.v[layer], self.k_scale[layer], self.v_scale[layer],
                                self.block_tables, plan.kv_lens, plan.q_starts, scale=scale, window=window,
-                               max_q_len=max_q_len, max_kv_len=max_kv_len)
+                               max_q_len=max_q_len, max_kv_len=max_kv_len, shared=shared)
