@@ -1561,8 +1561,8 @@ int paged_attention(const char* fn, const int32_t* run_starts, const int32_t* ru
   const bool shares = run_starts && pmi::paged_attention_shares(p, c);
   if (!(shares ? pmi::paged_shared_launch_fits(p, c) : pmi::paged_attention_launch_fits(p, c)))
     return fail(PMI_ERR_UNSUPPORTED, "%s: too many query rows for one launch (T H)", fn);
-  pmi::PagedAttention whole = p;  // (a run has the queries of all its members)
-  if (shares) whole.max_q = T;
+  pmi::PagedAttention whole = p;  // (a run is one more request, with the queries of all its members)
+  if (shares) whole.max_q = T, whole.R = 2 * R;
   if (!pmi::paged_attention_tiles_fit(whole, c))
     return fail(PMI_ERR_UNSUPPORTED, "%s: too many tiles of 64 keys for 32 bits (R KV max_kv): give a tighter max_kv "
                 "or fewer requests", fn);

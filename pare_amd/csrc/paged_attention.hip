@@ -33,23 +33,29 @@ struct AttnArgs {
   int few_wgs;    // workgroups of the few-row part
   int* counters;  // one of each of them, and behind them one of each item of many rows
   float *few_part, *many_part;
-  // runs of requests with the same first pages (kShared, kOwn)
+  // runs of requests with the same first pages (kParts)
   const int32_t* run_starts;
   const int32_t* run_lens;
-  int many_wgs;   // kShared: workgroups that the ranges of keys are made for
-  float* shared;  // the shared part of every query: [T, H, D + 4] values, max, sum
+  int run_rows;       // runs of up to so many query rows are `few`
+  int many_wgs;       // workgroups that the ranges of a run's keys are made for
+  // Parts of rows, D + 4 floats each (values, max, sum): of the ranges of runs of many rows, in
+  // tiles of kRows; of runs of few rows [T, H]; of the keys behind what is shared [T, H].
+  float *parts_many, *parts_few, *parts_own;
+  int2* where;        // [T, H] a row's first shared part (its offset from parts_many in records), and how many
+  int part_records;   // that parts_many and parts_few hold
 };
 
-// What a launch computes. kAll: whole rows. Where requests share their first pages these are
-// read once for all of a run, in two launches: kShared takes a run as a request whose queries are
-// those of all its members and whose keys are the shared ones, which all of its queries see, and
-// leaves values, maximum and sum of each row; kOwn takes the requests with the keys behind
-// those, and joins the two.
-enum Part { kAll, kShared, kOwn };
+// What a launch computes: whole rows; or, where requests share their first pages, parts of
+// rows. A run is then a request whose queries are those of all its members and whose keys are the
+// shared ones, which all of its queries see; each member has the keys behind them for itself. All
+// parts are of one launch, and a second one joins them (join_parts_kernel). Numbers 0 .. R - 1 are
+// the requests, R .. 2 R - 1 the runs.
+enum Mode { kWhole, kParts };
 
 // What a request's queries see, from its row of kv_lens and q_starts.
 struct Request {
   int row;            // of the tables
+  bool run;
   int start, n;       // its queries (none: nothing to do)
   int len, shift;     // its keys, of those within the bounds; query i sees positions up to shift + i
   int first_seen;     // the first position that its first query sees
@@ -67,10 +73,12 @@ PMI_DEV int shared_before(const AttnArgs& a, int r, int shift) {
   const int len = shared_len(a, r);
   return shift + 1 > len ? len : 0;
 }
-template <Part PART>
+template <Mode MODE>
 PMI_DEV Request request(const AttnArgs& a, int r) {
   Request q;
-  if constexpr (PART == kShared) {
+  q.run = MODE == kParts && r >= a.R;
+  if (q.run) {
+    r -= a.R;
     const int first = a.run_starts[r], last = a.run_starts[r + 1];
     const bool run = first >= 0 && first < last && last <= a.R;
     q.row = run ? first : 0;
@@ -97,7 +105,7 @@ PMI_DEV Request request(const AttnArgs& a, int r) {
   q.shift = max(len0, 0) - q.n;  // (with the keys past the bounds and the queries past max_q)
   q.n = min(q.n, a.max_q);
   if (q.n < 0 || q.start < 0 || (int64_t)q.start + q.n > a.T) q.n = 0;
-  q.first_seen = min(PART == kOwn ? shared_before(a, r, q.shift) : first_position(a, q.shift), q.len);
+  q.first_seen = min(MODE == kParts ? shared_before(a, r, q.shift) : first_position(a, q.shift), q.len);
   q.lo = q.first_seen & ~15;
   q.hi = a.n_pages ? max(q.lo, min(q.len, q.shift + q.n)) : q.lo;
   return q;
@@ -295,7 +303,7 @@ struct FewLds {
   int last;
 };
 
-template <typename T, int D, bool FP8, Part PART>
+template <typename T, int D, bool FP8, Mode MODE>
 PMI_DEV void few_rows(const AttnArgs& a, FewLds<D>& lds, int wg) {
   constexpr int DT = D / 16;  // 16-dimension tiles of the output
   float(&s_acc)[4][16][D + 4] = lds.acc;
@@ -311,11 +319,14 @@ PMI_DEV void few_rows(const AttnArgs& a, FewLds<D>& lds, int wg) {
   // itself, a lane a run of requests: no barrier, and one round of loads up to 64 requests.
   // (The host sees to it that the sum is below 2^31.)
   auto tiles_of = [&](const Request& rq) { return max(1, (rq.hi - rq.lo + 63) >> 6); };
-  auto items_of = [&](const Request& rq) { return rq.n * G > a.few_rows ? 0 : (rq.n * G + 15) / 16 * a.KV; };
-  const int run = (a.R + 63) >> 6, r_lane = run * l;
+  auto items_of = [&](const Request& rq) {
+    return rq.n * G > (rq.run ? a.run_rows : a.few_rows) ? 0 : (rq.n * G + 15) / 16 * a.KV;
+  };
+  const int requests = MODE == kWhole ? a.R : 2 * a.R;
+  const int run = (requests + 63) >> 6, r_lane = run * l;
   int in_lane = 0, parts_lane[kCuts] = {};  // tiles, and parts of cut_of(k) tiles
-  for (int x = r_lane; x < min(a.R, r_lane + run); ++x) {
-    const Request rq = request<PART>(a, x);
+  for (int x = r_lane; x < min(requests, r_lane + run); ++x) {
+    const Request rq = request<MODE>(a, x);
     const int nt = tiles_of(rq), items = items_of(rq);
     in_lane += nt * items;
 #pragma unroll
@@ -361,8 +372,8 @@ PMI_DEV void few_rows(const AttnArgs& a, FewLds<D>& lds, int wg) {
   const int lane0 = __builtin_ctzll(__ballot(upto > g));
   int r = run * lane0;
   int off = g - (__builtin_amdgcn_readlane(upto, lane0) - __builtin_amdgcn_readlane(in_lane, lane0));  // tiles of r before g
-  while (g < g_end && r < a.R) {
-  const Request rq = request<PART>(a, r);
+  while (g < g_end && r < requests) {
+  const Request rq = request<MODE>(a, r);
   const int row_tiles = (rq.n * G + 15) / 16, nt = tiles_of(rq);
   const int span = cut ? (nt + cut - 1) / cut * cut : nt;  // what an item takes of the order
   const int all = span * items_of(rq);
@@ -385,13 +396,13 @@ PMI_DEV void few_rows(const AttnArgs& a, FewLds<D>& lds, int wg) {
   const int i = row / G;
   // positions that this column's query sees: [lo, hi)
   const int hi = live ? max(0, min(len, shift + i + 1)) : 0;
-  const int lo = PART == kAll ? first_position(a, shift + i) : rq.first_seen;
+  const int lo = MODE == kWhole ? first_position(a, shift + i) : rq.first_seen;
   const int i_first = rt * 16 / G, i_last = (rt * 16 + min(rows, 16) - 1) / G;
   const int first_seen = rq.first_seen;
   const int p0 = rq.lo + 64 * tile0, p1 = min(rq.hi, p0 + 64 * n_tiles);
   // tiles inside of [safe_lo, safe_hi) need no mask
   const int safe_hi = max(0, min(len, shift + i_first + 1));
-  const int safe_lo = PART == kAll ? first_position(a, shift + i_last) : first_seen;
+  const int safe_lo = MODE == kWhole ? first_position(a, shift + i_last) : first_seen;
 
   QueryRow<T, D> q;
   load_query<T, D>(q, (const T*)a.q + (int64_t)(start + (live ? i : 0)) * a.q_token +
@@ -551,34 +562,21 @@ PMI_DEV void few_rows(const AttnArgs& a, FewLds<D>& lds, int wg) {
   const int grow = rt * 16 + orow;
   const int64_t out_row = (int64_t)(start + grow / G) * a.H + kh * G + grow % G;
   T* dst = (T*)a.out + out_row * D + od;
-  // the shared part of a row: `dims` of its values from dimension d on
-  auto keep_shared = [&](int64_t row, int d, auto dims, const float* v, float m, float l) {
-    float* rec = a.shared + row * (D + 4);
+  // a row that is a part: its values from dimension d on
+  const bool is_part = MODE == kParts && (rq.run || first_seen > 0);
+  auto keep_part = [&](int64_t at, int d, const auto& v, int n, float m, float l) {
+    float* rec = (rq.run ? a.parts_few : a.parts_own) + at * (D + 4);
 #pragma unroll
-    for (int x = 0; x < decltype(dims)::value; x += 4)
-      *reinterpret_cast<f32x4*>(rec + d + x) = f32x4{v[x], v[x + 1], v[x + 2], v[x + 3]};
-    if (d == 0) *reinterpret_cast<float2*>(rec + D) = float2{m, l};
-  };
-  auto join_shared = [&](int64_t row, int d, auto dims, float* v, float& m, float& l) {
-    const float* rec = a.shared + row * (D + 4);
-    const float m0 = m, l0 = l;
-#pragma unroll
-    for (int x = 0; x < decltype(dims)::value; x += 4) {
-      f32x4 o4 = {v[x], v[x + 1], v[x + 2], v[x + 3]};
-      m = m0, l = l0;
-      join(m, l, o4, rec[D], rec[D + 1], *reinterpret_cast<const f32x4*>(rec + d + x), true);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) v[x + e] = o4[e];
+    for (int x = 0; x < n; x += 4) *reinterpret_cast<f32x4*>(rec + d + x) = f32x4{v[x], v[x + 1], v[x + 2], v[x + 3]};
+    if (d == 0) {
+      *reinterpret_cast<float2*>(rec + D) = float2{m, l};
+      if (rq.run) a.where[at] = int2{(int)((a.parts_few - a.parts_many) / (D + 4) + at), 1};
     }
   };
   auto store = [&]() {
-    using Per = std::integral_constant<int, kPer>;
-    if constexpr (PART == kShared) {
-      if (mine) keep_shared(out_row, od, Per{}, o, om, ol);
+    if (is_part) {
+      if (mine) keep_part(out_row, od, o, kPer, om, ol);
       return;
-    }
-    if constexpr (PART == kOwn) {
-      if (mine && first_seen > 0) join_shared(out_row, od, Per{}, o, om, ol);
     }
     const float inv = ol > 0.f ? 1.f / ol : (ol != ol ? ol : 0.f);
     typedef T Tv __attribute__((ext_vector_type(kPer)));
@@ -679,15 +677,9 @@ PMI_DEV void few_rows(const AttnArgs& a, FewLds<D>& lds, int wg) {
       }
       const int row1 = rt * 16 + r0 + slot;
       const int64_t out1 = (int64_t)(start + row1 / G) * a.H + kh * G + row1 % G;
-      using Four = std::integral_constant<int, 4>;
-      if constexpr (PART != kAll) {
-        float v[4] = {jo[0], jo[1], jo[2], jo[3]};
-        if constexpr (PART == kShared) {
-          keep_shared(out1, dim, Four{}, v, jm, jl);
-          continue;
-        }
-        if (first_seen > 0) join_shared(out1, dim, Four{}, v, jm, jl);
-        jo = f32x4{v[0], v[1], v[2], v[3]};
+      if (is_part) {
+        keep_part(out1, dim, jo, 4, jm, jl);
+        continue;
       }
       const float inv = jl > 0.f ? 1.f / jl : (jl != jl ? jl : 0.f);
       typedef T T4 __attribute__((ext_vector_type(4)));
@@ -702,18 +694,18 @@ PMI_DEV void few_rows(const AttnArgs& a, FewLds<D>& lds, int wg) {
   }
 }
 
-template <typename T, int D, bool FP8, Part PART>
+template <typename T, int D, bool FP8, Mode MODE>
 __global__ __launch_bounds__(256, 2) void attention_few_kernel(AttnArgs a) {
   __shared__ __attribute__((aligned(16))) FewLds<D> lds;
-  few_rows<T, D, FP8, PART>(a, lds, blockIdx.x);
+  few_rows<T, D, FP8, MODE>(a, lds, blockIdx.x);
 }
 
-template <typename T, int D, Part PART>
+template <typename T, int D, Mode MODE>
 hipError_t few(const AttnArgs& a, bool fp8, hipStream_t stream) {
   if (fp8)
-    hipLaunchKernelGGL((attention_few_kernel<T, D, true, PART>), dim3(a.few_wgs), dim3(256), 0, stream, a);
+    hipLaunchKernelGGL((attention_few_kernel<T, D, true, MODE>), dim3(a.few_wgs), dim3(256), 0, stream, a);
   else
-    hipLaunchKernelGGL((attention_few_kernel<T, D, false, PART>), dim3(a.few_wgs), dim3(256), 0, stream, a);
+    hipLaunchKernelGGL((attention_few_kernel<T, D, false, MODE>), dim3(a.few_wgs), dim3(256), 0, stream, a);
   return hipGetLastError();
 }
 
@@ -737,8 +729,9 @@ hipError_t few(const AttnArgs& a, bool fp8, hipStream_t stream) {
 // Where the rows give fewer workgroups than the CUs hold, the keys are split as well
 // (`splits` ranges of `per` tokens), and the last range to arrive joins them.
 constexpr int kRows = 128;
+constexpr int kLeastRange = 256;  // keys of a run's range, at least
 
-template <typename T, int D, bool FP8, Part PART>
+template <typename T, int D, bool FP8, Mode MODE>
 PMI_DEV void many_rows(const AttnArgs& a, uint8_t* lds, int& s_last, int wg) {
   constexpr int KP = D / 64;       // 16-byte pieces of K, and of V, per thread and tile
   constexpr int kSlot = 64 * D * 2;  // bytes of K (or V) of a tile as fp16
@@ -748,9 +741,10 @@ PMI_DEV void many_rows(const AttnArgs& a, uint8_t* lds, int& s_last, int wg) {
 
   // which rows: the row tiles of all requests in order, each request's last ones (with the most
   // keys) first, the KV heads innermost (an XCD then keeps few heads' keys in its L2)
+  const int first_request = MODE == kWhole ? 0 : a.R;
   auto tiles_of = [&](int r) {
-    const Request rq = request<PART>(a, r);
-    return rq.n * G > a.few_rows ? (rq.n * G + kRows - 1) / kRows : 0;
+    const Request rq = request<MODE>(a, first_request + r);
+    return rq.n * G > (MODE == kWhole ? a.few_rows : a.run_rows) ? (rq.n * G + kRows - 1) / kRows : 0;
   };
   const int kh = wg % a.KV, rest = wg / a.KV;
   const int run = (a.R + 63) >> 6, r_lane = run * l;
@@ -765,7 +759,7 @@ PMI_DEV void many_rows(const AttnArgs& a, uint8_t* lds, int& s_last, int wg) {
   const int all_tiles = __builtin_amdgcn_readlane(upto, 63);
   // (the host does not know how many runs there are, nor what they share)
   int splits = a.splits;
-  if constexpr (PART == kShared) splits = all_tiles > 0 ? max(1, a.many_wgs / (all_tiles * a.KV)) : 1;
+  if constexpr (MODE == kParts) splits = all_tiles > 0 ? max(1, a.many_wgs / (all_tiles * a.KV)) : 1;
   const int sp = rest % splits, index = rest / splits;
   if (index >= all_tiles) return;
   const int lane0 = __builtin_ctzll(__ballot(upto > index));
@@ -778,25 +772,24 @@ PMI_DEV void many_rows(const AttnArgs& a, uint8_t* lds, int& s_last, int wg) {
     count = tiles_of(r);
   }
   const int rt = count - 1 - at_tile;
-  const Request rq = request<PART>(a, r);
+  const Request rq = request<MODE>(a, first_request + r);
   const int start = rq.start, len = rq.len, shift = rq.shift;
   const int rows = min(kRows, rq.n * G - rt * kRows);
   const int row = rt * kRows + wave * 32 + c;
   const bool live = wave * 32 + c < rows;
   const int i = row / G;
   const int hi = live ? max(0, min(len, shift + i + 1)) : 0;
-  const int lo = PART == kAll ? first_position(a, shift + i) : rq.first_seen;
+  const int lo = MODE == kWhole ? first_position(a, shift + i) : rq.first_seen;
   const int i_first = rt * kRows / G, i_last = (rt * kRows + rows - 1) / G;
-  const int first_seen = PART == kAll ? min(first_position(a, shift + i_first), len) : rq.first_seen;
+  const int first_seen = MODE == kWhole ? min(first_position(a, shift + i_first), len) : rq.first_seen;
   const int all_lo = first_seen & ~15;
   const int all_hi = a.n_pages ? max(all_lo, min(len, shift + i_last + 1)) : all_lo;
-  // a range of at least eight tiles, as its join costs about two
-  const int per = PART == kShared ? max(512, ((len + splits - 1) / splits + 63) & ~63) : a.per;
+  const int per = MODE == kParts ? max(kLeastRange, ((len + splits - 1) / splits + 63) & ~63) : a.per;
   const int parts = max(1, (all_hi - all_lo + per - 1) / per);
   if (sp >= parts) return;
   const int p0 = all_lo + sp * per, p1 = min(all_hi, p0 + per);
   const int safe_hi = max(0, min(len, shift + i_first + 1));
-  const int safe_lo = PART == kAll ? first_position(a, shift + i_last) : first_seen;
+  const int safe_lo = MODE == kWhole ? first_position(a, shift + i_last) : first_seen;
 
   // the wave's query rows: step s holds dimensions 16 s + 8 h .. + 7
   f16x8 qv[D / 16];
@@ -1013,8 +1006,9 @@ PMI_DEV void many_rows(const AttnArgs& a, uint8_t* lds, int& s_last, int wg) {
   typedef T T4 __attribute__((ext_vector_type(4)));
   const int64_t out_row = (int64_t)(start + i) * a.H + kh * G + row - i * G;
   T* dst = (T*)a.out + out_row * D + 4 * h;
-  if (PART == kShared && parts == 1) {
-    float* rec = a.shared + out_row * (D + 4);
+  if constexpr (MODE == kParts) {
+    const int64_t at = ((int64_t)(index * a.KV + kh) * splits + sp) * kRows + wave * 32 + c;
+    float* rec = a.parts_many + at * (D + 4);
 #pragma unroll
     for (int d = 0; d < D / 32; ++d)
 #pragma unroll
@@ -1025,27 +1019,7 @@ PMI_DEV void many_rows(const AttnArgs& a, uint8_t* lds, int& s_last, int wg) {
         if (live) *reinterpret_cast<f32x4*>(rec + 32 * d + 8 * j + 4 * h) = y;
       }
     if (live && h == 0) *reinterpret_cast<float2*>(rec + D) = float2{ref.max, sum};
-    return;
-  }
-  if (PART == kOwn && parts == 1 && first_seen > 0) {
-    const float* rec = a.shared + out_row * (D + 4);
-    const float pm = live ? rec[D] : 0.f, pl = live ? rec[D + 1] : 0.f;
-#pragma unroll
-    for (int d = 0; d < D / 32; ++d)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        float m = ref.max, l = sum;
-        f32x4 y;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) y[e] = acc[d][4 * j + e] * unit;
-        if (!live) continue;
-        join(m, l, y, pm, pl, *reinterpret_cast<const f32x4*>(rec + 32 * d + 8 * j + 4 * h), true);
-        const float inv = l > 0.f ? 1.f / l : (l != l ? l : 0.f);
-        T4 o;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] = (T)(y[e] * inv);
-        *reinterpret_cast<T4*>(dst + 32 * d + 8 * j) = o;
-      }
+    if (live && h == 0 && sp == 0) a.where[out_row] = int2{(int)at, parts};
     return;
   }
   if (parts == 1) {
@@ -1112,16 +1086,6 @@ PMI_DEV void many_rows(const AttnArgs& a, uint8_t* lds, int& s_last, int wg) {
     }
     const int grow = rt * kRows + y;
     const int64_t out1 = (int64_t)(start + grow / G) * a.H + kh * G + grow % G;
-    if constexpr (PART == kShared) {
-      float* rec = a.shared + out1 * (D + 4);
-      *reinterpret_cast<f32x4*>(rec + dim) = jo;
-      if (dim == 0) *reinterpret_cast<float2*>(rec + D) = float2{jm, jl};
-      continue;
-    }
-    if (PART == kOwn && first_seen > 0) {
-      const float* rec = a.shared + out1 * (D + 4);
-      join(jm, jl, jo, rec[D], rec[D + 1], *reinterpret_cast<const f32x4*>(rec + dim), true);
-    }
     const float inv = jl > 0.f ? 1.f / jl : (jl != jl ? jl : 0.f);
     T4 o;
 #pragma unroll
@@ -1135,25 +1099,73 @@ PMI_DEV void many_rows(const AttnArgs& a, uint8_t* lds, int& s_last, int wg) {
 // fills with the other (32 / 8 heads of 128: 8 single tokens of 2000 keys and a prompt of 2048 72 us, in
 // two launches 81; 32 of 3000 and a chunk of 512 behind 1000 79 and 84; two prompts of 300, where the
 // first find nothing to do, 17.6 and 18.6).
-template <typename T, int D, bool FP8, Part PART>
+template <typename T, int D, bool FP8, Mode MODE>
 __global__ __launch_bounds__(256, 2) void attention_rows_kernel(AttnArgs a) {
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];  // [2 slots][K, V]
   __shared__ int s_last;
   static_assert(sizeof(FewLds<D>) <= 2 * 2 * 64 * D * 2, "fits the slots");
+  // (of parts the runs' are the longest: they begin first)
+  if constexpr (MODE == kParts) {
+    const int many = (int)gridDim.x - a.few_wgs;
+    if ((int)blockIdx.x < many)
+      many_rows<T, D, FP8, MODE>(a, lds, s_last, blockIdx.x);
+    else
+      few_rows<T, D, FP8, MODE>(a, *reinterpret_cast<FewLds<D>*>(lds), blockIdx.x - many);
+    return;
+  }
   if ((int)blockIdx.x < a.few_wgs)
-    few_rows<T, D, FP8, PART>(a, *reinterpret_cast<FewLds<D>*>(lds), blockIdx.x);
+    few_rows<T, D, FP8, MODE>(a, *reinterpret_cast<FewLds<D>*>(lds), blockIdx.x);
   else
-    many_rows<T, D, FP8, PART>(a, lds, s_last, blockIdx.x - a.few_wgs);
+    many_rows<T, D, FP8, MODE>(a, lds, s_last, blockIdx.x - a.few_wgs);
 }
 
-template <typename T, int D, Part PART>
+template <typename T, int D, Mode MODE>
 hipError_t many(const AttnArgs& a, bool fp8, int64_t wgs, hipStream_t stream) {
   constexpr int kLds = 2 * 2 * 64 * D * 2;
   if (fp8)
-    hipLaunchKernelGGL((attention_rows_kernel<T, D, true, PART>), dim3((unsigned)wgs), dim3(256), kLds, stream, a);
+    hipLaunchKernelGGL((attention_rows_kernel<T, D, true, MODE>), dim3((unsigned)wgs), dim3(256), kLds, stream, a);
   else
-    hipLaunchKernelGGL((attention_rows_kernel<T, D, false, PART>), dim3((unsigned)wgs), dim3(256), kLds, stream, a);
+    hipLaunchKernelGGL((attention_rows_kernel<T, D, false, MODE>), dim3((unsigned)wgs), dim3(256), kLds, stream, a);
   return hipGetLastError();
+}
+
+// The parts of the rows that share keys: a workgroup the rows of a request and KV head, D / 4 threads a
+// row, its own part first and the shared ones in order.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void join_parts_kernel(AttnArgs a) {
+  constexpr int kRowThreads = D / 4, kFly = 8;
+  const int r = blockIdx.x, kh = blockIdx.y, G = a.H / a.KV;
+  const Request rq = request<kParts>(a, r);
+  if (rq.n <= 0 || rq.first_seen <= 0) return;
+  const int dim = 4 * (threadIdx.x % kRowThreads);
+  for (int row = threadIdx.x / kRowThreads; row < rq.n * G; row += 256 / kRowThreads) {
+    const int64_t out_row = (int64_t)(rq.start + row / G) * a.H + kh * G + row % G;
+    const float* own = a.parts_own + out_row * (D + 4);
+    float m = own[D], l = own[D + 1];
+    f32x4 o = *reinterpret_cast<const f32x4*>(own + dim);
+    int2 at = a.where[out_row];
+    // (nobody wrote it if the runs are not this batch's)
+    if (at.x < 0 || at.y < 0 || (int64_t)at.x + (int64_t)kRows * (at.y - 1) >= a.part_records) at = int2{0, 0};
+    const float* rec = a.parts_many + (int64_t)at.x * (D + 4);
+    for (int s0 = 0; s0 < at.y; s0 += kFly) {
+      float2 ml[kFly];
+      f32x4 v[kFly];
+#pragma unroll
+      for (int k = 0; k < kFly; ++k) {
+        const float* p = rec + (int64_t)min(s0 + k, at.y - 1) * kRows * (D + 4);
+        ml[k] = *reinterpret_cast<const float2*>(p + D);
+        v[k] = *reinterpret_cast<const f32x4*>(p + dim);
+      }
+#pragma unroll
+      for (int k = 0; k < kFly; ++k) join(m, l, o, ml[k].x, ml[k].y, v[k], s0 + k < at.y);
+    }
+    const float inv = l > 0.f ? 1.f / l : (l != l ? l : 0.f);
+    typedef T T4 __attribute__((ext_vector_type(4)));
+    T4 y;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y[e] = (T)(o[e] * inv);
+    *reinterpret_cast<T4*>((T*)a.out + out_row * D + dim) = y;
+  }
 }
 
 // Workgroups of the few-row part: what the CUs hold at once of its own kernel (with heads of 64 half
@@ -1236,27 +1248,33 @@ AttnArgs attention_args(const PagedAttention& p, const PagedCache& c, void* work
 }
 
 // Requests of few rows alone (n = 0), or n workgroups of both.
-template <Part PART>
-hipError_t launch_part(const AttnArgs& a, const PagedAttention& p, const PagedCache& c, int64_t n, hipStream_t stream) {
+template <Mode MODE>
+hipError_t launch_mode(const AttnArgs& a, const PagedAttention& p, const PagedCache& c, int64_t n, hipStream_t stream) {
   if (n == 0) {
-    if (p.bf16) return c.D == 64 ? few<__bf16, 64, PART>(a, c.fp8, stream) : few<__bf16, 128, PART>(a, c.fp8, stream);
-    return c.D == 64 ? few<f16, 64, PART>(a, c.fp8, stream) : few<f16, 128, PART>(a, c.fp8, stream);
+    if (p.bf16) return c.D == 64 ? few<__bf16, 64, MODE>(a, c.fp8, stream) : few<__bf16, 128, MODE>(a, c.fp8, stream);
+    return c.D == 64 ? few<f16, 64, MODE>(a, c.fp8, stream) : few<f16, 128, MODE>(a, c.fp8, stream);
   }
   if (p.bf16)
-    return c.D == 64 ? many<__bf16, 64, PART>(a, c.fp8, n, stream) : many<__bf16, 128, PART>(a, c.fp8, n, stream);
-  return c.D == 64 ? many<f16, 64, PART>(a, c.fp8, n, stream) : many<f16, 128, PART>(a, c.fp8, n, stream);
+    return c.D == 64 ? many<__bf16, 64, MODE>(a, c.fp8, n, stream) : many<__bf16, 128, MODE>(a, c.fp8, n, stream);
+  return c.D == 64 ? many<f16, 64, MODE>(a, c.fp8, n, stream) : many<f16, 128, MODE>(a, c.fp8, n, stream);
 }
 
-// Row tiles of all runs x KV heads, at most: those of many rows, of which each has at least kFewRows + 1.
-int64_t shared_items(const PagedAttention& p, const PagedCache& c) {
+// Query rows up to which a run is one of few.
+constexpr int kRunRows = 32;
+
+// Row tiles of all runs of many rows x KV heads, at most.
+int64_t run_items(const PagedAttention& p, const PagedCache& c) {
   const int64_t G = p.H / c.KV, rows = p.T * G;
-  if (rows <= kFewRows) return 0;
-  const int64_t runs = rows / (kFewRows + 1) < p.R ? rows / (kFewRows + 1) : p.R;
+  if (rows <= kRunRows) return 0;
+  const int64_t runs = rows / (kRunRows + 1) < p.R ? rows / (kRunRows + 1) : p.R;
   return (rows / kRows + runs) * c.KV;
 }
-int64_t shared_part_bytes(const PagedAttention& p, const PagedCache& c) {
-  return shared_items(p, c) ? (int64_t)2 * device_cu_count() * kRows * (c.D + 4) * 4 : 0;
+// Workgroups of runs of many rows: those that the CUs hold, as ranges of keys, or one for each row tile.
+int64_t run_wgs(const PagedAttention& p, const PagedCache& c) {
+  const int64_t items = run_items(p, c), held = 2 * device_cu_count();
+  return items == 0 ? 0 : items > held ? items : held;
 }
+size_t part_bytes(int64_t rows, int64_t D) { return (size_t)(rows * (D + 4) * 4); }
 
 }  // namespace
 
@@ -1265,34 +1283,51 @@ bool paged_attention_shares(const PagedAttention& p, const PagedCache& c) {
 }
 
 bool paged_shared_launch_fits(const PagedAttention& p, const PagedCache& c) {
-  return few_wgs(c.D) + shared_items(p, c) + 2 * device_cu_count() < (1ll << 24);
+  // (parts are counted in 32 bits, and requests and runs together)
+  return few_wgs(c.D) + run_wgs(p, c) < (1ll << 23) && p.R < (1ll << 29) && p.R * c.KV < (1ll << 24) &&
+         run_wgs(p, c) * kRows + 2 * p.T * p.H < (1ll << 31);
 }
 
 size_t paged_shared_ws_bytes(const PagedAttention& p, const PagedCache& c) {
-  return kWsCounterBytes + few_part_bytes(c.D) + (size_t)shared_part_bytes(p, c) + (size_t)(p.T * p.H * (c.D + 4) * 4);
+  return kWsCounterBytes + few_part_bytes(c.D) + part_bytes(run_wgs(p, c) * kRows + 2 * p.T * p.H, c.D) +
+         (size_t)(p.T * p.H * 8);
 }
 
 hipError_t launch_paged_shared(const PagedAttention& p, const PagedCache& c, void* workspace, hipStream_t stream) {
   AttnArgs a = attention_args(p, c, workspace);
-  a.shared = (float*)((char*)a.many_part + shared_part_bytes(p, c));
-  const int64_t items = shared_items(p, c);
+  const int64_t wgs = run_wgs(p, c), rows = p.T * p.H;
+  a.parts_many = a.many_part;
+  a.parts_few = a.parts_many + wgs * kRows * (c.D + 4);
+  a.parts_own = a.parts_few + rows * (c.D + 4);
+  a.where = (int2*)(a.parts_own + rows * (c.D + 4));
+  a.part_records = (int)(wgs * kRows + rows);
+  a.run_rows = kRunRows;
   a.many_wgs = 2 * device_cu_count();
-  const int64_t wgs = items > a.many_wgs ? items : a.many_wgs;
-  a.max_q = (int)p.T;
-  if (hipError_t e = launch_part<kShared>(a, p, c, items ? a.few_wgs + wgs : 0, stream); e != hipSuccess) return e;
-  a.max_q = (int)p.max_q;
-  return launch_part<kOwn>(a, p, c, 0, stream);
+  if (hipError_t e = launch_mode<kParts>(a, p, c, wgs ? a.few_wgs + wgs : 0, stream); e != hipSuccess) return e;
+  const dim3 grid((unsigned)p.R, (unsigned)c.KV), block(256);
+  if (p.bf16) {
+    if (c.D == 64)
+      hipLaunchKernelGGL((join_parts_kernel<__bf16, 64>), grid, block, 0, stream, a);
+    else
+      hipLaunchKernelGGL((join_parts_kernel<__bf16, 128>), grid, block, 0, stream, a);
+  } else {
+    if (c.D == 64)
+      hipLaunchKernelGGL((join_parts_kernel<f16, 64>), grid, block, 0, stream, a);
+    else
+      hipLaunchKernelGGL((join_parts_kernel<f16, 128>), grid, block, 0, stream, a);
+  }
+  return hipGetLastError();
 }
 
 hipError_t launch_paged_attention(const PagedAttention& p, const PagedCache& c, void* workspace, size_t ws_bytes,
                                   hipStream_t stream) {
   AttnArgs a = attention_args(p, c, workspace);
   const ManyPlan f = many_plan(p, c);
-  if (f.items == 0) return launch_part<kAll>(a, p, c, 0, stream);
+  if (f.items == 0) return launch_mode<kWhole>(a, p, c, 0, stream);
   // Any batch of several requests may have some of few rows; a lone one stays with many.
   if (p.R == 1) a.few_rows = 0, a.few_wgs = 0;
   a.splits = f.splits, a.per = f.per;
-  return launch_part<kAll>(a, p, c, a.few_wgs + f.items * f.splits, stream);
+  return launch_mode<kWhole>(a, p, c, a.few_wgs + f.items * f.splits, stream);
 }
 
 }  // namespace pmi

@@ -514,6 +514,10 @@ def test_runs_of_another_batch_stay_inside_the_buffers():
         out = torch.full((3, 4, 64), 7.0, dtype=torch.float16, device=DEV)
         got = _run(case, shared=P.SharedPrefixes(_ints(starts), _ints(lens)), out=out)[0]
         _check(got, case, torch.float16)
+    # positions that are said to be shared, of no run: those requests' rows mean nothing, the others' are right
+    for starts in ([3, 3, 3, 3], [2, 3, 3, 3], [0, 1, 3, 3], [1, 0, 9, 9]):
+        got = _run(case, shared=P.SharedPrefixes(_ints(starts), _ints([144, 144, 0])))[0]
+        assert torch.equal(got[2], right[2])
 
 
 @gpu
