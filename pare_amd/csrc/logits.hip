@@ -20,46 +20,52 @@ struct Frame {  // what 16 bytes hold
   typedef T Vec __attribute__((ext_vector_type(16 / sizeof(T))));
 };
 
-// A value above another one, or the same earlier in the row; NaN is the largest, as argmax has it.
-PMI_DEV bool better(float v, int i, float b, int bi) {
-  if (bi < 0) return i >= 0;
-  if (i < 0) return false;
-  if (v != v) return b == b || i < bi;
-  if (b != b) return false;
-  return v > b || (v == b && i < bi);
+// Values as integers in their order, NaN above all of them and both zeros the same; a value and its token
+// as one, where the lower token is the larger of two equal values.
+PMI_DEV uint32_t ordered(float v) {
+  const uint32_t u = __builtin_bit_cast(uint32_t, v + 0.f);
+  return v != v ? ~0u : u ^ ((uint32_t)((int)u >> 31) | 0x80000000u);
 }
-
-PMI_DEV void better_of_wave(float& v, int& i) {
+PMI_DEV uint64_t keyed(uint32_t value, int token) { return (uint64_t)value << 32 | (uint32_t)~token; }
+PMI_DEV int token_of(uint64_t key) { return ~(int)(uint32_t)key; }
+PMI_DEV uint64_t largest_of_wave(uint64_t key) {
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) {
-    const float ov = __shfl_xor(v, o);
-    const int oi = __shfl_xor(i, o);
-    if (better(ov, oi, v, i)) v = ov, i = oi;
+    const uint64_t other = __shfl_xor(key, o);
+    key = other > key ? other : key;
   }
+  return key;
 }
 
-constexpr int kThreads = 256;
-constexpr int kSlice = 4096;  // tokens of a workgroup
-constexpr int kNoBias = 0x7fffffff;
+// Tokens of a workgroup, its threads, and how LDS holds what its tokens count and their biases' entries:
+// in 16 bits while the history is shorter than 2^15 tokens (bit 15 is for the prompt's) and there are
+// fewer entries than 2^16 - 1, else in 32.
+template <int SLICE, int THREADS, typename C>
+struct Form {
+  static constexpr int kSlice = SLICE, kThreads = THREADS;
+  typedef C Count;
+  static constexpr uint32_t kPrompt = 1u << (8 * sizeof(C) - 1), kNoBias = (C)~(C)0;
+};
 
-// A workgroup takes kSlice tokens of a row, in frames of 16 bytes that are aligned in memory (a row
+// A workgroup takes a slice of a row, in frames of 16 bytes that are aligned in memory (a row
 // of odd size begins inside one). What the slice's tokens count in the history is made in LDS from all
-// of the row's history, so that no list of a row's distinct tokens is needed; bit 31 is for
-// the prompt's. Of a token's biases LDS holds the first entry; whether any token has two is known
-// as well, and only then the others are looked for.
+// of the row's history, so that no list of a row's distinct tokens is needed. Of a token's biases LDS holds one
+// entry; if any token has two, the entries are gone through in their order for each that has one.
 // WRITE: the logits to `out`; else the largest of them, the slices' joined by the last to arrive.
-template <typename T, bool WRITE>
-__global__ __launch_bounds__(kThreads) void logits_kernel(Logits f, T* out, int64_t out_stride,
-                                                          int64_t* __restrict__ tokens, int64_t token_stride,
-                                                          int* __restrict__ counters, float* __restrict__ part,
-                                                          int slices) {
-  constexpr int E = Frame<T>::kSize, kFrames = kSlice / E / kThreads;  // frames of a thread
+template <typename T, bool WRITE, typename F>
+__global__ __launch_bounds__(F::kThreads) void logits_kernel(Logits f, T* out, int64_t out_stride,
+                                                             int64_t* __restrict__ tokens, int64_t token_stride,
+                                                             int* __restrict__ counters,
+                                                             uint64_t* __restrict__ part, int slices) {
+  constexpr int E = Frame<T>::kSize, kSlice = F::kSlice, kThreads = F::kThreads;
+  constexpr int kFrames = kSlice / E / kThreads;  // frames of a thread
   typedef typename Frame<T>::Vec Vec;
-  __shared__ __attribute__((aligned(16))) uint32_t counts[kSlice];
-  __shared__ __attribute__((aligned(16))) int biases[kSlice];
+  typedef typename F::Count C;
+  typedef C CVec __attribute__((ext_vector_type(E)));
+  __shared__ __attribute__((aligned(16))) C counts[kSlice];
+  __shared__ __attribute__((aligned(16))) C biases[kSlice];
   __shared__ int twice, s_last;
-  __shared__ float best_s[kThreads / 64];
-  __shared__ int at_s[kThreads / 64];
+  __shared__ uint64_t best_s[kThreads / 64];
   const int tid = threadIdx.x;
   const int r = blockIdx.x / slices, slice = blockIdx.x - r * slices;
   const int V = (int)f.V;
@@ -97,77 +103,89 @@ __global__ __launch_bounds__(kThreads) void logits_kernel(Logits f, T* out, int6
   const int n_bias = (int)f.n_bias;
   float rho = 1.f, alpha = 0.f, beta = 0.f;
   if (penalties || biased) {
-    for (int i = tid; i < kSlice / 4; i += kThreads) {
+    constexpr int kWords = kSlice * (int)sizeof(C) / 16;
+    for (int i = tid; i < kWords; i += kThreads) {
       reinterpret_cast<u32x4*>(counts)[i] = u32x4{0, 0, 0, 0};
-      reinterpret_cast<u32x4*>(biases)[i] = u32x4{kNoBias, kNoBias, kNoBias, kNoBias};
+      reinterpret_cast<u32x4*>(biases)[i] = u32x4{~0u, ~0u, ~0u, ~0u};
     }
     if (tid == 0) twice = 0;
-    __syncthreads();
-    const auto of_slice = [&](int t) { return t >= 0 && t < V && t >= s0 && t < s0 + kSlice; };
+    const auto of_slice = [&](int t) {
+      return (uint32_t)t < (uint32_t)V && (uint32_t)t - (uint32_t)s0 < (uint32_t)kSlice;
+    };
+    const int32_t* past = f.history + r * f.history_stride;
+    const int n = !penalties ? 0 : (int)(f.history_lens ? min((int64_t)max(f.history_lens[r], 0), f.L) : f.L);
+    const int prompt = penalties && f.prompt_lens ? f.prompt_lens[r] : 0;
     if (penalties) {
       if (f.repetition) rho = f.repetition[r];
       if (f.presence) alpha = f.presence[r];
       if (f.frequency) beta = f.frequency[r];
-      const int32_t* past = f.history + r * f.history_stride;
-      const int n = (int)(f.history_lens ? min((int64_t)max(f.history_lens[r], 0), f.L) : f.L);
-      const int prompt = f.prompt_lens ? f.prompt_lens[r] : 0;
-      for (int i = tid; i < n; i += kThreads) {
-        const int t = past[i];
-        if (!of_slice(t)) continue;
-        if (i < prompt)
-          atomicOr(&counts[t - s0], 0x80000000u);
+    }
+    __syncthreads();
+    constexpr int kFly = 8;  // tokens in flight a thread
+    for (int i0 = tid; i0 < n; i0 += kThreads * kFly) {
+      int t[kFly];
+#pragma unroll
+      for (int k = 0; k < kFly; ++k) t[k] = i0 + kThreads * k < n ? past[i0 + kThreads * k] : -1;
+#pragma unroll
+      for (int k = 0; k < kFly; ++k) {
+        if (!of_slice(t[k])) continue;
+        constexpr uint32_t kPer = 4 / sizeof(C);  // counts of a word
+        const uint32_t at = t[k] - s0, up = 8 * sizeof(C) * (at % kPer);
+        uint32_t* word = reinterpret_cast<uint32_t*>(counts) + at / kPer;
+        if (i0 + kThreads * k < prompt)
+          atomicOr(word, F::kPrompt << up);
         else
-          atomicAdd(&counts[t - s0], 1u);
+          atomicAdd(word, 1u << up);
       }
     }
     if (biased) {
       for (int i = tid; i < n_bias; i += kThreads)
-        if (of_slice(ids[i])) atomicMin(&biases[ids[i] - s0], i);
+        if (of_slice(ids[i])) biases[ids[i] - s0] = (C)i;  // (whichever comes last)
       __syncthreads();
       for (int i = tid; i < n_bias; i += kThreads)
-        if (of_slice(ids[i]) && biases[ids[i] - s0] != i) twice = 1;
+        if (of_slice(ids[i]) && biases[ids[i] - s0] != (C)i) twice = 1;
     }
     __syncthreads();
   }
 
   T* to = WRITE ? out + r * out_stride : nullptr;
   const bool wide = WRITE && (int)((uintptr_t)to % 16 / sizeof(T)) == shift;
-  float best = 0.f;
-  int best_at = -1;
+  uint32_t best = 0;  // below every value's
+  int best_at = 0;
 #pragma unroll
   for (int k = 0; k < kFrames; ++k) {
     const int in = E * (tid + kThreads * k), t = s0 + in;
     if (t >= V || t + E <= 0) continue;
     if (penalties || biased) {
+      const CVec c = *reinterpret_cast<const CVec*>(counts + in), b = *reinterpret_cast<const CVec*>(biases + in);
 #pragma unroll
-      for (int q = 0; q < E / 4; ++q) {
-        const u32x4 c = *reinterpret_cast<const u32x4*>(counts + in + 4 * q);
-        const u32x4 b = *reinterpret_cast<const u32x4*>(biases + in + 4 * q);
-        if (!(c[0] | c[1] | c[2] | c[3]) && (b[0] & b[1] & b[2] & b[3]) == (uint32_t)kNoBias) continue;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float v = (float)x[k][4 * q + e];
-          if (c[e]) {
-            v = v > 0.f ? v / rho : v * rho;
-            const uint32_t n = c[e] & 0x7fffffffu;
-            if (n) v = v - beta * (float)n - alpha;
-          }
-          if (b[e] != (uint32_t)kNoBias) {
-            float sum = values[b[e]];
-            if (twice)
-              for (int i = (int)b[e] + 1; i < n_bias; ++i)
-                if (ids[i] == t + 4 * q + e) sum += values[i];
-            v += sum;
-          }
-          x[k][4 * q + e] = (T)v;
+      for (int e = 0; e < E; ++e) {
+        if (c[e] == 0 && b[e] == (C)F::kNoBias) continue;
+        float v = (float)x[k][e];
+        if (c[e]) {
+          v = v > 0.f ? v / rho : v * rho;
+          const uint32_t n = c[e] & (F::kPrompt - 1);
+          if (n) v = v - beta * (float)n - alpha;
         }
+        if (b[e] != (C)F::kNoBias) {
+          float sum = values[b[e]];
+          if (twice) {
+            bool any = false;
+            for (int i = 0; i < n_bias; ++i)
+              if (ids[i] == t + e) sum = any ? sum + values[i] : values[i], any = true;
+          }
+          v += sum;
+        }
+        x[k][e] = (T)v;
       }
     }
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       if (!(bits[k] >> e & 1)) x[k][e] = (T)-INFINITY;
-      if (!WRITE && t + e >= 0 && t + e < V && better((float)x[k][e], t + e, best, best_at))
-        best = (float)x[k][e], best_at = t + e;
+      if constexpr (!WRITE) {
+        const uint32_t value = t + e >= 0 && t + e < V ? ordered((float)x[k][e]) : 0;
+        if (value > best) best = value, best_at = t + e;
+      }
     }
     if constexpr (WRITE) {
       if (wide && t >= 0 && t + E <= V) {
@@ -180,21 +198,18 @@ __global__ __launch_bounds__(kThreads) void logits_kernel(Logits f, T* out, int6
     }
   }
   if constexpr (!WRITE) {
-    better_of_wave(best, best_at);
-    if ((tid & 63) == 0) best_s[tid >> 6] = best, at_s[tid >> 6] = best_at;
+    uint64_t key = largest_of_wave(keyed(best, best_at));
+    if ((tid & 63) == 0) best_s[tid >> 6] = key;
     __syncthreads();
     if (tid == 0) {
 #pragma unroll
-      for (int w = 1; w < kThreads / 64; ++w)
-        if (better(best_s[w], at_s[w], best, best_at)) best = best_s[w], best_at = at_s[w];
+      for (int w = 1; w < kThreads / 64; ++w) key = best_s[w] > key ? best_s[w] : key;
       if (slices == 1) {
-        tokens[r * token_stride] = max(best_at, 0);
+        tokens[r * token_stride] = token_of(key);
         s_last = 0;
       } else {
         // coherent across the XCDs' L2 caches
-        float* at = part + 2 * ((int64_t)r * slices + slice);
-        __hip_atomic_store(at, best, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        __hip_atomic_store(reinterpret_cast<int*>(at + 1), best_at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __hip_atomic_store(&part[(int64_t)r * slices + slice], key, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         asm volatile("" ::: "memory");
         __builtin_amdgcn_s_waitcnt(0);
         asm volatile("" ::: "memory");
@@ -203,49 +218,65 @@ __global__ __launch_bounds__(kThreads) void logits_kernel(Logits f, T* out, int6
     }
     __syncthreads();
     if (!s_last || tid >= 64) return;
-    best = 0.f, best_at = -1;
+    key = 0;
     for (int i = tid; i < slices; i += 64) {
-      float* at = part + 2 * ((int64_t)r * slices + i);
-      const float v = __hip_atomic_load(at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      const int vi = __hip_atomic_load(reinterpret_cast<int*>(at + 1), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      if (better(v, vi, best, best_at)) best = v, best_at = vi;
+      const uint64_t other = __hip_atomic_load(&part[(int64_t)r * slices + i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      key = other > key ? other : key;
     }
-    better_of_wave(best, best_at);
+    key = largest_of_wave(key);
     if (tid == 0) {
-      tokens[r * token_stride] = max(best_at, 0);
+      tokens[r * token_stride] = token_of(key);
       __hip_atomic_store(&counters[r], 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
   }
 }
 
-// Slices of a row; one that begins inside a frame may need one more.
-int64_t slices_of(int64_t V, int64_t size) { return (V + 16 / size - 1 + kSlice - 1) / kSlice; }
+// Tokens of a workgroup: the history is gone through once for each slice of a row, so that slices are large
+// where the rows are workgroups enough.
+typedef Form<4096, 256, uint16_t> Small;
+typedef Form<16384, 1024, uint16_t> Large;
+typedef Form<8192, 512, uint32_t> Wide;
+
 int64_t size_of(int dtype) { return dtype == 2 ? 4 : 2; }
+// Slices of a row (one that begins inside a frame may need one more).
+int64_t slices_of(int64_t V, int64_t size, bool aligned, int slice) {
+  return (V + (aligned ? 0 : 16 / size - 1) + slice - 1) / slice;
+}
+
+template <typename T, bool WRITE, typename F>
+hipError_t launch_form(const Logits& f, void* out, int64_t out_stride, int64_t* tokens, int64_t token_stride, void* ws,
+                       hipStream_t stream) {
+  const bool aligned = (uintptr_t)f.x % 16 == 0 && f.stride * sizeof(T) % 16 == 0;
+  const int slices = (int)slices_of(f.V, sizeof(T), aligned, F::kSlice);
+  hipLaunchKernelGGL((logits_kernel<T, WRITE, F>), dim3((unsigned)(f.R * slices)), dim3(F::kThreads), 0, stream, f,
+                     (T*)out, out_stride, tokens, token_stride, (int*)ws,
+                     WRITE ? nullptr : (uint64_t*)((char*)ws + kWsCounterBytes), slices);
+  return hipGetLastError();
+}
+
+template <typename T, bool WRITE>
+hipError_t launch_t(const Logits& f, void* out, int64_t out_stride, int64_t* tokens, int64_t token_stride, void* ws,
+                    hipStream_t stream) {
+  if (f.L >= 1 << 15 || f.n_bias >= (1 << 16) - 1)
+    return launch_form<T, WRITE, Wide>(f, out, out_stride, tokens, token_stride, ws, stream);
+  if (f.R * ((f.V + Large::kSlice - 1) / Large::kSlice) >= device_cu_count())
+    return launch_form<T, WRITE, Large>(f, out, out_stride, tokens, token_stride, ws, stream);
+  return launch_form<T, WRITE, Small>(f, out, out_stride, tokens, token_stride, ws, stream);
+}
 
 template <bool WRITE>
 hipError_t launch(const Logits& f, void* out, int64_t out_stride, int64_t* tokens, int64_t token_stride, void* ws,
                   hipStream_t stream) {
-  const int64_t size = size_of(f.dtype);
-  const bool aligned = (uintptr_t)f.x % 16 == 0 && f.stride * size % 16 == 0;
-  const int slices = (int)(aligned ? (f.V + kSlice - 1) / kSlice : slices_of(f.V, size));
-  const dim3 grid((unsigned)(f.R * slices)), block(kThreads);
-  int* counters = (int*)ws;
-  float* part = WRITE ? nullptr : (float*)((char*)ws + kWsCounterBytes);
-  if (f.dtype == 0)
-    hipLaunchKernelGGL((logits_kernel<f16, WRITE>), grid, block, 0, stream, f, (f16*)out, out_stride, tokens,
-                       token_stride, counters, part, slices);
-  else if (f.dtype == 1)
-    hipLaunchKernelGGL((logits_kernel<__bf16, WRITE>), grid, block, 0, stream, f, (__bf16*)out, out_stride, tokens,
-                       token_stride, counters, part, slices);
-  else
-    hipLaunchKernelGGL((logits_kernel<float, WRITE>), grid, block, 0, stream, f, (float*)out, out_stride, tokens,
-                       token_stride, counters, part, slices);
-  return hipGetLastError();
+  if (f.dtype == 0) return launch_t<f16, WRITE>(f, out, out_stride, tokens, token_stride, ws, stream);
+  if (f.dtype == 1) return launch_t<__bf16, WRITE>(f, out, out_stride, tokens, token_stride, ws, stream);
+  return launch_t<float, WRITE>(f, out, out_stride, tokens, token_stride, ws, stream);
 }
 
 }  // namespace
 
-int64_t logits_workgroups(int64_t R, int64_t V, int dtype) { return R * slices_of(V, size_of(dtype)); }
+int64_t logits_workgroups(int64_t R, int64_t V, int dtype) {
+  return R * slices_of(V, size_of(dtype), false, Small::kSlice);
+}
 
 hipError_t launch_process_logits(const Logits& f, void* out, int64_t out_stride, hipStream_t stream) {
   return launch<true>(f, out, out_stride, nullptr, 0, nullptr, stream);
