@@ -177,6 +177,8 @@ def host():
         ext.bind(*(ctypes.cast(getattr(handle, fn), ctypes.c_void_p).value for fn in (
             "pmi_matmul_w4a16", "pmi_matmul_kernel_choice", "pmi_matmul_best_workspace_bytes",
             "pmi_matmul_route")))
+        ext.bind_serving(*(ctypes.cast(getattr(handle, fn), ctypes.c_void_p).value for fn in (
+            "pmi_process_logits", "pmi_greedy_tokens", "pmi_greedy_tokens_workspace_bytes", "pmi_copy_kv_pages")))
         _host = ext
     return _host
 

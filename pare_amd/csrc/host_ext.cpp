@@ -1,19 +1,25 @@
-// Host path of a matmul call (CPython extension): the checks, the output
-// allocation and the pmi_matmul_w4a16 call that pare_amd.kernels and
-// pare_amd.linear otherwise make from Python. Calls at decode sizes take 3-15 us
-// on the GPU, and the Python path issued one every 20 us (QuantizedLinear at one
-// row); this one every 7.
+// Host path of calls that the host would bound (CPython extension): the checks, the output
+// allocation and the library call that pare_amd otherwise makes from Python.
+//   matmul: pmi_matmul_w4a16, of pare_amd.kernels and pare_amd.linear. Calls at decode sizes take
+//     3-15 us on the GPU, and the Python path issued one every 20 us (QuantizedLinear at one
+//     row); this one every 7.
+//   logits: pmi_process_logits and pmi_greedy_tokens, of pare_amd.logits, with up to eleven tensors to
+//     check (one row: 6 us on the GPU; a call every 12.4 us from Python, every 5.0 from here).
+//   copy_pages: pmi_copy_kv_pages, of pare_amd.paged, with four tensors a layer (32 layers: 9 us on the GPU;
+//     a call every 57 us from Python, every 6.4 from here).
 //
 // Only plain calls are taken: dense tensors of the expected types on the current
-// device. For everything else, and where the library refuses, matmul() returns
+// device. For everything else, and where the library refuses, they return
 // None and the caller's general path runs, with its own conversions and errors.
 // Nothing is kept between calls, and no HIP header is needed: the library's entry
 // points arrive as addresses, the stream as its handle.
 #include <ATen/ATen.h>
 #include <ATen/TensorSubclassLikeUtils.h>
+#include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <optional>
+#include <vector>
 
 namespace py = pybind11;
 
@@ -26,6 +32,21 @@ using ChoiceFn = int (*)(int64_t, int64_t, int64_t, int64_t, int);
 using WorkspaceFn = size_t (*)(int64_t, int64_t, int64_t, int64_t, int);
 using RouteFn = int (*)(int64_t, int64_t, int64_t, int64_t, int, int, size_t);
 
+using ProcessFn = int (*)(const void*, int, int64_t, const int32_t*, int64_t, int64_t, const int32_t*, const int32_t*,
+                          const float*, const float*, const float*, const int32_t*, const float*, int64_t,
+                          const int32_t*, int64_t, int64_t, const int32_t*, void*, int64_t, int64_t, int64_t, void*);
+using GreedyFn = int (*)(const void*, int, int64_t, const int32_t*, int64_t, int64_t, const int32_t*, const int32_t*,
+                         const float*, const float*, const float*, const int32_t*, const float*, int64_t,
+                         const int32_t*, int64_t, int64_t, const int32_t*, int64_t*, int64_t, int64_t, int64_t, void*,
+                         size_t, void*);
+using GreedyWorkspaceFn = size_t (*)(int64_t, int64_t, int);
+using CopyFn = int (*)(const int32_t*, const int32_t*, const int32_t*, int64_t, void* const*, void* const*,
+                       float* const*, float* const*, int64_t, int64_t, int64_t, int64_t, int64_t, void*);
+
+ProcessFn g_process = nullptr;
+GreedyFn g_greedy = nullptr;
+GreedyWorkspaceFn g_greedy_workspace = nullptr;
+CopyFn g_copy = nullptr;
 MatmulFn g_matmul = nullptr;
 ChoiceFn g_choice = nullptr;
 WorkspaceFn g_workspace = nullptr;
@@ -39,6 +60,13 @@ void bind(uintptr_t matmul, uintptr_t choice, uintptr_t workspace, uintptr_t rou
   g_choice = reinterpret_cast<ChoiceFn>(choice);
   g_workspace = reinterpret_cast<WorkspaceFn>(workspace);
   g_route = reinterpret_cast<RouteFn>(route);
+}
+
+void bind_serving(uintptr_t process, uintptr_t greedy, uintptr_t greedy_workspace, uintptr_t copy) {
+  g_process = reinterpret_cast<ProcessFn>(process);
+  g_greedy = reinterpret_cast<GreedyFn>(greedy);
+  g_greedy_workspace = reinterpret_cast<GreedyWorkspaceFn>(greedy_workspace);
+  g_copy = reinterpret_cast<CopyFn>(copy);
 }
 
 bool plain(const at::Tensor& t) {
@@ -129,9 +157,154 @@ py::object matmul(const at::Tensor& x, const at::Tensor& w, const at::Tensor& sc
   return rc == 0 ? py::cast(y) : py::none();
 }
 
+using Maybe = std::optional<at::Tensor>;
+
+// No tensor, or a buffer of these sizes.
+bool none_or(const Maybe& t, const at::Device& dev, at::ScalarType dtype, at::IntArrayRef sizes) {
+  return !t || (plain(*t) && t->device() == dev && t->scalar_type() == dtype && t->sizes() == sizes && t->is_contiguous());
+}
+
+// Rows of a 2-D tensor that are contiguous and do not overlap; their stride.
+bool rows(const at::Tensor& t, int64_t& stride) {
+  stride = t.stride(0) > t.size(1) ? t.stride(0) : t.size(1);
+  return (t.size(1) <= 1 || t.stride(1) == 1) && (t.size(0) <= 1 || t.stride(0) >= t.size(1));
+}
+
+// The processed logits, or with `greedy` their tokens: the arguments of pare_amd.process_logits and
+// pare_amd.greedy_tokens in their order.
+py::object logits(bool greedy, const at::Tensor& x, const Maybe& history, const Maybe& history_lens,
+                  const Maybe& prompt_lens, const Maybe& repetition, const Maybe& presence, const Maybe& frequency,
+                  const Maybe& bias_ids, const Maybe& bias, const Maybe& allowed, const Maybe& allowed_rows,
+                  const Maybe& out, int64_t device, uintptr_t stream, const py::function& workspace_fn) {
+  if (!g_process || !plain(x) || x.dim() != 2) return py::none();
+  const at::Device dev = x.device();
+  const at::ScalarType type = x.scalar_type();
+  const int64_t R = x.size(0), V = x.size(1);
+  if (dev.index() != device || R == 0 || V == 0 ||
+      (type != at::kHalf && type != at::kBFloat16 && type != at::kFloat))
+    return py::none();
+  const int code = type == at::kHalf ? 0 : type == at::kBFloat16 ? 1 : 2;
+  int64_t stride, history_stride = 0, L = 0, n_bias = 0, masks = 0, words = 0;
+  if (!rows(x, stride)) return py::none();
+  if (history) {
+    if (!plain(*history) || history->device() != dev || history->scalar_type() != at::kInt || history->dim() != 2 ||
+        history->size(0) != R || !rows(*history, history_stride))
+      return py::none();
+    L = history->size(1);
+  } else if (history_lens || prompt_lens || repetition || presence || frequency) {
+    return py::none();
+  }
+  for (const Maybe* t : {&history_lens, &prompt_lens})
+    if (!none_or(*t, dev, at::kInt, {R})) return py::none();
+  for (const Maybe* t : {&repetition, &presence, &frequency})
+    if (!none_or(*t, dev, at::kFloat, {R})) return py::none();
+  if (bias_ids.has_value() != bias.has_value()) return py::none();
+  if (bias_ids) {
+    if (bias_ids->dim() != 2) return py::none();
+    n_bias = bias_ids->size(1);
+    if (!none_or(bias_ids, dev, at::kInt, {R, n_bias}) || !none_or(bias, dev, at::kFloat, {R, n_bias}))
+      return py::none();
+  }
+  if (allowed) {
+    if (allowed->dim() != 2) return py::none();
+    masks = allowed->size(0), words = (V + 31) / 32;
+    if (!none_or(allowed, dev, at::kInt, {masks, words}) || (!allowed_rows && masks != R)) return py::none();
+  }
+  if (!none_or(allowed_rows, dev, at::kInt, {R}) || (allowed_rows && !allowed)) return py::none();
+  at::Tensor y, ws;
+  int64_t out_stride = greedy ? 1 : V;
+  if (out) {
+    y = *out;
+    if (!plain(y) || y.device() != dev) return py::none();
+    if (greedy) {
+      if (y.scalar_type() != at::kLong || y.dim() < 1 || y.size(0) != R || y.numel() != R) return py::none();
+      out_stride = R > 1 ? y.stride(0) : 1;
+    } else if (y.scalar_type() != type || y.sizes() != x.sizes() || !rows(y, out_stride)) {
+      return py::none();
+    }
+  }
+  const size_t need = greedy ? g_greedy_workspace(R, V, code) : 0;
+  if (need) {
+    ws = workspace_fn(need).cast<at::Tensor>();
+    if (!plain(ws) || ws.device() != dev) return py::none();
+  }
+  std::optional<py::gil_scoped_release> unlocked(std::in_place);
+  if (!out) {
+    const at::TensorOptions options = at::TensorOptions().device(dev);
+    y = greedy ? at::empty({R}, options.dtype(at::kLong)) : at::empty({R, V}, options.dtype(type));
+  }
+  const auto call = [&](auto fn, auto... rest) {
+    return fn(x.const_data_ptr(), code, stride, ptr<int32_t>(history), history_stride, L, ptr<int32_t>(history_lens),
+              ptr<int32_t>(prompt_lens), ptr<float>(repetition), ptr<float>(presence), ptr<float>(frequency),
+              ptr<int32_t>(bias_ids), ptr<float>(bias), n_bias, ptr<int32_t>(allowed), masks, words,
+              ptr<int32_t>(allowed_rows), rest..., reinterpret_cast<void*>(stream));
+  };
+  const int rc = greedy ? call(g_greedy, static_cast<int64_t*>(y.mutable_data_ptr()), out_stride, R, V,
+                               need ? ws.mutable_data_ptr() : nullptr, need ? (size_t)ws.numel() : (size_t)0)
+                        : call(g_process, y.mutable_data_ptr(), out_stride, R, V);
+  unlocked.reset();
+  return rc == 0 ? py::cast(y) : py::none();
+}
+
+// The layers' buffers of one kind: a sequence of tensors of the same sizes and type, or one tensor with the
+// layers first. `first` is the first layer's.
+bool layers(const py::object& all, const at::Device& dev, std::vector<void*>& at_layers, at::Tensor& first) {
+  if (THPVariable_Check(all.ptr())) {
+    const at::Tensor& t = THPVariable_Unpack(all.ptr());
+    if (!plain(t) || t.device() != dev || t.dim() < 1 || t.size(0) == 0 || !t.is_contiguous()) return false;
+    first = t.select(0, 0);
+    for (int64_t i = 0; i < t.size(0); ++i)
+      at_layers.push_back(static_cast<char*>(t.mutable_data_ptr()) + i * first.numel() * t.element_size());
+    return true;
+  }
+  if (!PyList_Check(all.ptr()) && !PyTuple_Check(all.ptr())) return false;
+  PyObject** items = PySequence_Fast_ITEMS(all.ptr());
+  for (Py_ssize_t i = 0; i < PySequence_Fast_GET_SIZE(all.ptr()); ++i) {
+    if (!THPVariable_Check(items[i])) return false;
+    const at::Tensor& t = THPVariable_Unpack(items[i]);
+    if (i == 0) first = t;
+    if (!plain(t) || t.device() != dev || t.scalar_type() != first.scalar_type() || t.sizes() != first.sizes() ||
+        !t.is_contiguous())
+      return false;
+    at_layers.push_back(t.mutable_data_ptr());
+  }
+  return !at_layers.empty();
+}
+
+// pare_amd.copy_kv_pages: whether it was done.
+bool copy_pages(const at::Tensor& src, const at::Tensor& dst, const Maybe& count, const py::object& k_caches,
+                const py::object& v_caches, const py::object& k_scales, const py::object& v_scales, int64_t device,
+                uintptr_t stream) {
+  if (!g_copy || !plain(src)) return false;
+  const at::Device dev = src.device();
+  const int64_t n = src.numel();
+  if (dev.index() != device || !none_or(src, dev, at::kInt, {n}) || !none_or(dst, dev, at::kInt, {n}) ||
+      !none_or(count, dev, at::kInt, {1}))
+    return false;
+  std::vector<void*> kp, vp, ksp, vsp;
+  at::Tensor k, v, ks, vs;
+  if (!layers(k_caches, dev, kp, k) || !layers(v_caches, dev, vp, v) || !layers(k_scales, dev, ksp, ks) ||
+      !layers(v_scales, dev, vsp, vs) || vp.size() != kp.size() || ksp.size() != kp.size() || vsp.size() != kp.size())
+    return false;
+  if (k.dim() != 4 || (k.scalar_type() != at::kChar && k.scalar_type() != at::kFloat8_e4m3fn) ||
+      v.scalar_type() != k.scalar_type() || ks.scalar_type() != at::kFloat || vs.scalar_type() != at::kFloat)
+    return false;
+  const int64_t pages = k.size(0), KV = k.size(1), ps = k.size(2), D = k.size(3);
+  if (KV == 0 || ps % 16 || v.sizes() != at::IntArrayRef{pages, KV, ps / 16, D, 16} ||
+      ks.sizes() != at::IntArrayRef{pages, KV} || vs.sizes() != ks.sizes())
+    return false;
+  py::gil_scoped_release unlocked;
+  return g_copy(src.const_data_ptr<int32_t>(), dst.const_data_ptr<int32_t>(), ptr<int32_t>(count), n, kp.data(),
+                vp.data(), reinterpret_cast<float* const*>(ksp.data()), reinterpret_cast<float* const*>(vsp.data()),
+                (int64_t)kp.size(), pages, ps, KV, D, reinterpret_cast<void*>(stream)) == 0;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_host, m) {
   m.def("bind", &bind);
+  m.def("bind_serving", &bind_serving);
+  m.def("logits", &logits);
+  m.def("copy_pages", &copy_pages);
   m.def("matmul", &matmul);
 }

@@ -79,6 +79,17 @@ def _arguments(fn, logits, history, history_lens, prompt_lens, repetition, prese
             n_bias, at(allowed), masks, words, at(allowed_rows)]
 
 
+def _host(greedy, logits, *rest):
+    """The call through the host extension, or None where it is not a plain one: the general path then
+    takes it."""
+    if not logits.is_cuda:
+        return None
+    dev = torch._C._cuda_getDevice()
+    stream = torch._C._cuda_getCurrentRawStream(dev)
+    return _lib.host().logits(greedy, logits, *rest, dev, stream,
+                              lambda nbytes: _workspace(logits.device, stream, nbytes))
+
+
 def process_logits(logits: torch.Tensor, *, history: torch.Tensor | None = None,
                    history_lens: torch.Tensor | None = None, prompt_lens: torch.Tensor | None = None,
                    repetition: torch.Tensor | None = None, presence: torch.Tensor | None = None,
@@ -99,6 +110,10 @@ def process_logits(logits: torch.Tensor, *, history: torch.Tensor | None = None,
 
     The penalties are fp32 [R], each optional. Tokens outside 0 .. V - 1 are skipped (-1: none).
     Rounded once. ``out`` may be ``logits``."""
+    y = _host(False, logits, history, history_lens, prompt_lens, repetition, presence, frequency, bias_ids, bias,
+              allowed, allowed_rows, out)
+    if y is not None:
+        return y if out is None else out
     args = _arguments("process_logits", logits, history, history_lens, prompt_lens, repetition, presence, frequency,
                       bias_ids, bias, allowed, allowed_rows)
     R, V = logits.shape
@@ -126,6 +141,10 @@ def greedy_tokens(logits: torch.Tensor, *, history: torch.Tensor | None = None,
     arguments, without writing those: the lowest token of equal ones, NaN above all numbers, token 0
     where the mask allows nothing. ``out``: int64 with R elements at a constant stride (such as a [R, 1]
     buffer of tokens). At most 16384 rows."""
+    y = _host(True, logits, history, history_lens, prompt_lens, repetition, presence, frequency, bias_ids, bias,
+              allowed, allowed_rows, out)
+    if y is not None:
+        return y if out is None else out
     args = _arguments("greedy_tokens", logits, history, history_lens, prompt_lens, repetition, presence, frequency,
                       bias_ids, bias, allowed, allowed_rows)
     R, V = logits.shape

@@ -253,12 +253,19 @@ def compact_block_tables(block_tables: torch.Tensor, kv_lens: torch.Tensor, free
     return PageMoves(src, dst, count)
 
 
-def copy_kv_pages(moves: PageMoves, k_caches: Sequence[torch.Tensor], v_caches: Sequence[torch.Tensor],
-                  k_scales: Sequence[torch.Tensor], v_scales: Sequence[torch.Tensor]) -> None:
+def copy_kv_pages(moves: PageMoves, k_caches: Sequence[torch.Tensor] | torch.Tensor,
+                  v_caches: Sequence[torch.Tensor] | torch.Tensor, k_scales: Sequence[torch.Tensor] | torch.Tensor,
+                  v_scales: Sequence[torch.Tensor] | torch.Tensor) -> None:
     """Copies the pages of ``moves``, codes and scales, in the caches of all layers (sequences of as
-    many tensors each, all of the same sizes and type), in one launch per 64 layers. Pairs
-    with a page that the cache does not have are left out; no page may be copied to twice, or be copied
-    from and to."""
+    many tensors each, all of the same sizes and type, or tensors with the layers first), in one
+    launch per 64 layers. Pairs with a page that the cache does not have are left out; no page may be
+    copied to twice, or be copied from and to."""
+    _hip(moves.src, "copy_kv_pages")
+    dev = torch._C._cuda_getDevice()
+    if _lib.host().copy_pages(*moves, k_caches, v_caches, k_scales, v_scales, dev,
+                              torch._C._cuda_getCurrentRawStream(dev)):
+        return
+    k_caches, v_caches, k_scales, v_scales = (list(t) for t in (k_caches, v_caches, k_scales, v_scales))
     n = len(k_caches)
     assert len(v_caches) == n and len(k_scales) == n and len(v_scales) == n, (
         "the caches and scales must be sequences of one tensor a layer")

@@ -313,6 +313,14 @@ def test_copy(layers, pages, KV, ps, D, code):
                         want[b] = o.view(torch.uint8)[a]
                 assert torch.equal(t.view(torch.uint8), want)
     P.copy_kv_pages(P.PageMoves(_ints(src), _ints(dst), None), [], [], [], [])
+    # the layers in one tensor each
+    whole = [torch.stack([t.view(torch.uint8) for t in group]).view(group[0].dtype) for group in (k, v, *s)]
+    moves = P.PageMoves(_ints([1, 0]), _ints([3, 2]), None)
+    P.copy_kv_pages(moves, *whole)
+    P.copy_kv_pages(moves, tuple(k), v, *s)
+    for t, group in zip(whole, (k, v, *s)):
+        assert torch.equal(t.view(torch.uint8), torch.stack([x.view(torch.uint8) for x in group]))
+        assert torch.equal(t.view(torch.uint8)[:, 3], t.view(torch.uint8)[:, 1])
     with pytest.raises(AssertionError):
         P.copy_kv_pages(P.PageMoves(_ints(src), _ints(dst), None), k, v, s[0], s[1][:-1])
     with pytest.raises(AssertionError):
