@@ -469,7 +469,7 @@ def run(s):
                 free = free.clone()
                 P.release_block_tables(tables, lens, s["done"], free, pool, s["page"], shares=shares)
                 moves = P.compact_block_tables(tables, lens, free, pool, shares, s["page"])
-            P.copy_kv_pages(moves, list(s["k"]), list(s["v"]), list(s["ks"]), list(s["vs"]))
+            P.copy_kv_pages(moves, s["k"], s["v"], s["ks"], s["vs"])
             out = {"tables": tables, "kv_lens": lens, "pool": pool, "shares": shares, "src": moves.src,
                    "dst": moves.dst, **_codes(s)}
             return out if s["op"] == "fork" else {**out, "free": free}
