@@ -675,18 +675,17 @@ PMI_API size_t pmi_paged_attention_workspace_bytes(int64_t T, int64_t R, int64_t
                                                    int64_t D, int64_t max_q, int64_t max_kv,
                                                    int64_t window);
 
-/* pmi_paged_attention of requests of which some share their first pages: run_starts int32
- * [R + 1] and run_lens int32 [R] as pmi_shared_prefixes gives them for the same tables, lengths and
- * queries. The result is the same but for roundings: a run's shared keys are read once for the queries of
- * all its members, where no request has more than 64 query rows (max_q H / KV) and there is no
- * window. workspace: pmi_paged_attention_shared_workspace_bytes() bytes, otherwise as above. */
+/* pmi_paged_attention of requests of which some share their first pages: runs and run_lens are
+ * what pmi_shared_prefixes gives as runs and lens for the same tables, lengths and queries. The result is the same but for roundings: a run's shared keys are read once for the queries of
+ * all its members, where that pays by the bounds (no request of more than 32 query rows, max_q H / KV;
+ * 2^27 bytes of keys and values of all requests, max_kv of at least 2048; no window). workspace: pmi_paged_attention_shared_workspace_bytes() bytes, otherwise as above. */
 PMI_API int pmi_paged_attention_shared(const void* q, int dtype, int64_t q_stride,
                                        int64_t q_head_stride, const void* k_cache,
                                        const void* v_cache, const float* k_scale,
                                        const float* v_scale, int code_dtype, int64_t n_pages,
                                        int64_t page_size, const int32_t* tables,
                                        int64_t table_stride, const int32_t* kv_lens,
-                                       const int32_t* q_starts, const int32_t* run_starts,
+                                       const int32_t* q_starts, const int32_t* runs,
                                        const int32_t* run_lens, void* out, int64_t T, int64_t R,
                                        int64_t width, int64_t H, int64_t KV, int64_t D,
                                        int64_t max_q, int64_t max_kv, int64_t window, float scale,
@@ -750,13 +749,15 @@ PMI_API int pmi_copy_kv_pages(const int32_t* src, const int32_t* dst, const int3
  * if fewer than least_pages (>= 1) of its first pages, whole and before its new tokens, are those
  * of the request with new tokens before it. starts int32 [R + 1]: the requests with
  * which runs begin, R behind the last; lens int32 [R]: how many positions the members of the
- * request's run share, 0 for a run of one. workspace: device scratch of
+ * request's run share, 0 for a run of one; runs int32 [R, 4] (16-byte aligned): of each run of
+ * several requests the first one, its first query, the queries of all and the positions shared,
+ * zeros elsewhere. workspace: device scratch of
  * pmi_shared_prefixes_workspace_bytes() bytes, as for pmi_paged_attention. */
 PMI_API int pmi_shared_prefixes(const int32_t* tables, int64_t table_stride,
                                 const int32_t* kv_lens, const int32_t* q_starts, int32_t* starts,
-                                int32_t* lens, int64_t R, int64_t width, int64_t page_size,
-                                int64_t least_pages, void* workspace, size_t workspace_bytes,
-                                void* stream);
+                                int32_t* lens, int32_t* runs, int64_t R, int64_t width,
+                                int64_t page_size, int64_t least_pages, void* workspace,
+                                size_t workspace_bytes, void* stream);
 PMI_API size_t pmi_shared_prefixes_workspace_bytes(int64_t R);
 
 /* Logits before a token is chosen. x [R, V] (PMI_F16, PMI_BF16 or PMI_F32, rows `stride` elements

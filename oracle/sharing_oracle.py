@@ -80,7 +80,7 @@ def compact(tables, kv_lens, pool, shares, ps):
 
 
 def runs(tables, kv_lens, q_starts, ps, least):
-    """(starts [R + 1], lens [R])."""
+    """(starts [R + 1], lens [R], runs [R][4])."""
     R = len(kv_lens)
     groups, last = [], None
     for r in range(R):
@@ -101,7 +101,13 @@ def runs(tables, kv_lens, q_starts, ps, least):
     for first, members in groups:
         for r in [first] + [m for m, _ in members] if members else []:
             lens[r] = ps * min(c for _, c in members)
-    return [g[0] for g in groups] + [R] * (R + 1 - len(groups)), lens
+    starts = [g[0] for g in groups] + [R] * (R + 1 - len(groups))
+    rows = [[0] * 4 for _ in range(R)]
+    for i, (first, members) in enumerate(groups):
+        if members:
+            a, b = (first, starts[i + 1]) if q_starts is None else (q_starts[first], q_starts[starts[i + 1]])
+            rows[i] = [first, a, b - a, lens[first]]
+    return starts, lens, rows
 
 
 def logits(x, history, history_lens, prompt_lens, repetition, presence, frequency, bias_ids, bias, allowed, rows):

@@ -109,7 +109,7 @@ SIGNATURES = {
     "pmi_compact_block_tables": (_i, [_vp, _i64, *[_vp] * 7, *[_i64] * 4, _vp, ctypes.c_size_t, _vp]),
     "pmi_compact_scratch_bytes": (ctypes.c_size_t, [_i64]),
     "pmi_copy_kv_pages": (_i, [_vp, _vp, _vp, _i64, *[_vp] * 4, *[_i64] * 5, _vp]),
-    "pmi_shared_prefixes": (_i, [_vp, _i64, *[_vp] * 4, *[_i64] * 4, _vp, ctypes.c_size_t, _vp]),
+    "pmi_shared_prefixes": (_i, [_vp, _i64, *[_vp] * 5, *[_i64] * 4, _vp, ctypes.c_size_t, _vp]),
     "pmi_shared_prefixes_workspace_bytes": (ctypes.c_size_t, [_i64]),
     "pmi_process_logits": (_i, [_vp, _i, _i64, _vp, _i64, _i64, *[_vp] * 7, _i64, _vp, _i64, _i64, _vp, _vp, _i64,
                                 _i64, _i64, _vp]),
@@ -177,6 +177,10 @@ def host():
         ext.bind(*(ctypes.cast(getattr(handle, fn), ctypes.c_void_p).value for fn in (
             "pmi_matmul_w4a16", "pmi_matmul_kernel_choice", "pmi_matmul_best_workspace_bytes",
             "pmi_matmul_route")))
+        ext.bind_tables(*(ctypes.cast(getattr(handle, fn), ctypes.c_void_p).value for fn in (
+            "pmi_fork_block_tables", "pmi_release_shared_block_tables", "pmi_release_shared_scratch_bytes",
+            "pmi_compact_block_tables", "pmi_compact_scratch_bytes", "pmi_shared_prefixes",
+            "pmi_shared_prefixes_workspace_bytes")))
         ext.bind_serving(*(ctypes.cast(getattr(handle, fn), ctypes.c_void_p).value for fn in (
             "pmi_process_logits", "pmi_greedy_tokens", "pmi_greedy_tokens_workspace_bytes", "pmi_copy_kv_pages")))
         _host = ext

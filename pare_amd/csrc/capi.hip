@@ -1524,7 +1524,8 @@ size_t pmi_paged_attention_shared_workspace_bytes(int64_t T, int64_t R, int64_t 
 
 namespace {
 
-int paged_attention(const char* fn, const int32_t* run_starts, const int32_t* run_lens, const void* q, int dtype, int64_t q_stride, int64_t q_head_stride, const void* k_cache,
+int paged_attention(const char* fn, const int32_t* runs, const int32_t* run_lens, const void* q, int dtype,
+                    int64_t q_stride, int64_t q_head_stride, const void* k_cache,
                         const void* v_cache, const float* k_scale, const float* v_scale, int code_dtype,
                         int64_t n_pages, int64_t page_size, const int32_t* tables, int64_t table_stride,
                         const int32_t* kv_lens, const int32_t* q_starts, void* out, int64_t T, int64_t R,
@@ -1553,12 +1554,12 @@ int paged_attention(const char* fn, const int32_t* run_starts, const int32_t* ru
   if (!aligned(q, 16) || !aligned(out, 16))
     return fail(PMI_ERR_INVALID, "%s: q and out must be 16-byte aligned", fn);
   pmi::PagedAttention p = {q, q_stride, q_head_stride, out, tables, table_stride, kv_lens, q_starts, T, R, width, H,
-                           max_q, max_kv, window, scale, dtype == PMI_BF16, run_starts, run_lens};
+                           max_q, max_kv, window, scale, dtype == PMI_BF16, runs, run_lens};
   const pmi::PagedCache c = {const_cast<void*>(k_cache), const_cast<void*>(v_cache), const_cast<float*>(k_scale),
                              const_cast<float*>(v_scale), n_pages, KV, page_size, D, code_dtype == PMI_F8};
   // (not cut to the table's width: the ranges of keys have to be those that the workspace was asked for)
   if (p.max_kv > pmi::kPagedMaxKeys) p.max_kv = pmi::kPagedMaxKeys;
-  const bool shares = run_starts && pmi::paged_attention_shares(p, c);
+  const bool shares = runs && pmi::paged_attention_shares(p, c);
   if (!(shares ? pmi::paged_shared_launch_fits(p, c) : pmi::paged_attention_launch_fits(p, c)))
     return fail(PMI_ERR_UNSUPPORTED, "%s: too many query rows for one launch (T H)", fn);
   pmi::PagedAttention whole = p;  // (a run is one more request, with the queries of all its members)
@@ -1566,7 +1567,7 @@ int paged_attention(const char* fn, const int32_t* run_starts, const int32_t* ru
   if (!pmi::paged_attention_tiles_fit(whole, c))
     return fail(PMI_ERR_UNSUPPORTED, "%s: too many tiles of 64 keys for 32 bits (R KV max_kv): give a tighter max_kv "
                 "or fewer requests", fn);
-  const size_t need = attention_ws_bytes(T, R, H, KV, D, max_q, p.max_kv, window, run_starts != nullptr);
+  const size_t need = attention_ws_bytes(T, R, H, KV, D, max_q, p.max_kv, window, runs != nullptr);
   if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 256)))
     return fail(PMI_ERR_INVALID, "%s: needs a 256-byte aligned workspace of %zu bytes", fn, need);
   if (shares) return from_hip(pmi::launch_paged_shared(p, c, workspace, (hipStream_t)stream), fn);
@@ -1589,12 +1590,12 @@ int pmi_paged_attention(const void* q, int dtype, int64_t q_stride, int64_t q_he
 int pmi_paged_attention_shared(const void* q, int dtype, int64_t q_stride, int64_t q_head_stride, const void* k_cache,
                         const void* v_cache, const float* k_scale, const float* v_scale, int code_dtype,
                         int64_t n_pages, int64_t page_size, const int32_t* tables, int64_t table_stride,
-                        const int32_t* kv_lens, const int32_t* q_starts, const int32_t* run_starts, const int32_t* run_lens, void* out, int64_t T, int64_t R,
+                        const int32_t* kv_lens, const int32_t* q_starts, const int32_t* runs, const int32_t* run_lens, void* out, int64_t T, int64_t R,
                         int64_t width, int64_t H, int64_t KV, int64_t D, int64_t max_q, int64_t max_kv,
                         int64_t window, float scale, void* workspace, size_t workspace_bytes, void* stream) {
   const char* fn = "pmi_paged_attention_shared";
-  if (R > 0 && (!run_starts || !run_lens)) return fail(PMI_ERR_INVALID, "%s: null buffer", fn);
-  return paged_attention(fn, run_starts, run_lens, q, dtype, q_stride, q_head_stride, k_cache, v_cache, k_scale, v_scale, code_dtype,
+  if (R > 0 && (!runs || !run_lens || !aligned(runs, 16))) return fail(PMI_ERR_INVALID, "%s: null buffer", fn);
+  return paged_attention(fn, runs, run_lens, q, dtype, q_stride, q_head_stride, k_cache, v_cache, k_scale, v_scale, code_dtype,
                          n_pages, page_size, tables, table_stride, kv_lens, q_starts, out, T, R, width, H, KV, D, max_q, max_kv,
                          window, scale, workspace, workspace_bytes, stream);
 }
@@ -1686,18 +1687,19 @@ size_t pmi_shared_prefixes_workspace_bytes(int64_t R) {
 }
 
 int pmi_shared_prefixes(const int32_t* tables, int64_t table_stride, const int32_t* kv_lens, const int32_t* q_starts,
-                        int32_t* starts, int32_t* lens, int64_t R, int64_t width, int64_t page_size,
-                        int64_t least_pages, void* workspace, size_t workspace_bytes, void* stream) {
+                        int32_t* starts, int32_t* lens, int32_t* runs, int64_t R, int64_t width,
+                        int64_t page_size, int64_t least_pages, void* workspace, size_t workspace_bytes, void* stream) {
   const char* fn = "pmi_shared_prefixes";
   if (int rc = check_tables(R, width, table_stride, 0, page_size, fn)) return rc;
   if (least_pages < 1 || least_pages >= (1ll << 31))
     return fail(PMI_ERR_INVALID, "%s: least_pages=%lld must be positive", fn, (long long)least_pages);
   if (R == 0) return ok();
-  if (!kv_lens || !starts || !lens || (width && !tables)) return fail(PMI_ERR_INVALID, "%s: null buffer", fn);
+  if (!kv_lens || !starts || !lens || !runs || !aligned(runs, 16) || (width && !tables))
+    return fail(PMI_ERR_INVALID, "%s: null buffer", fn);
   const size_t need = pmi_shared_prefixes_workspace_bytes(R);
   if (!workspace || workspace_bytes < need || !aligned(workspace, 256))
     return fail(PMI_ERR_INVALID, "%s: needs a 256-byte aligned workspace of %zu bytes", fn, need);
-  const pmi::PagedRuns f = {tables, table_stride, kv_lens, q_starts, starts, lens, (int32_t*)workspace,
+  const pmi::PagedRuns f = {tables, table_stride, kv_lens, q_starts, starts, lens, runs, (int32_t*)workspace,
                             (int32_t*)((char*)workspace + pmi::kWsCounterBytes), R, width, page_size, least_pages};
   return from_hip(pmi::launch_shared_runs(f, (hipStream_t)stream), fn);
 }

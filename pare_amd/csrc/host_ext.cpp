@@ -5,6 +5,8 @@
 //     row); this one every 7.
 //   logits: pmi_process_logits and pmi_greedy_tokens, of pare_amd.logits, with up to eleven tensors to
 //     check (one row: 6 us on the GPU; a call every 12.4 us from Python, every 5.0 from here).
+//   fork_tables, release_tables, compact_tables, shared_prefixes: the entry points of pare_amd.paged for pages of
+//     several requests (3-5 us on the GPU; a call every 10 to 20 us from Python, every 4.3 to 6.2 from here).
 //   copy_pages: pmi_copy_kv_pages, of pare_amd.paged, with four tensors a layer (32 layers: 9 us on the GPU;
 //     a call every 57 us from Python, every 6.4 from here).
 //
@@ -43,6 +45,21 @@ using GreedyWorkspaceFn = size_t (*)(int64_t, int64_t, int);
 using CopyFn = int (*)(const int32_t*, const int32_t*, const int32_t*, int64_t, void* const*, void* const*,
                        float* const*, float* const*, int64_t, int64_t, int64_t, int64_t, int64_t, void*);
 
+using ForkFn = int (*)(int32_t*, int64_t, int32_t*, const int32_t*, const int32_t*, const int32_t*, int32_t*, int32_t*,
+                       int32_t*, int32_t*, int32_t*, int64_t, int64_t, int64_t, int64_t, void*);
+using ReleaseFn = int (*)(const int32_t*, int64_t, int32_t*, const uint8_t*, int32_t*, int32_t*, int32_t*, int64_t,
+                          int64_t, int64_t, int64_t, void*, size_t, void*);
+using CompactFn = int (*)(int32_t*, int64_t, const int32_t*, int32_t*, int32_t*, int32_t*, int32_t*, int32_t*, int32_t*,
+                          int64_t, int64_t, int64_t, int64_t, void*, size_t, void*);
+using RunsFn = int (*)(const int32_t*, int64_t, const int32_t*, const int32_t*, int32_t*, int32_t*, int32_t*, int64_t,
+                       int64_t, int64_t, int64_t, void*, size_t, void*);
+using BytesFn = size_t (*)(int64_t);
+
+ForkFn g_fork = nullptr;
+ReleaseFn g_release = nullptr;
+CompactFn g_compact = nullptr;
+RunsFn g_runs = nullptr;
+BytesFn g_release_bytes = nullptr, g_compact_bytes = nullptr, g_runs_bytes = nullptr;
 ProcessFn g_process = nullptr;
 GreedyFn g_greedy = nullptr;
 GreedyWorkspaceFn g_greedy_workspace = nullptr;
@@ -60,6 +77,17 @@ void bind(uintptr_t matmul, uintptr_t choice, uintptr_t workspace, uintptr_t rou
   g_choice = reinterpret_cast<ChoiceFn>(choice);
   g_workspace = reinterpret_cast<WorkspaceFn>(workspace);
   g_route = reinterpret_cast<RouteFn>(route);
+}
+
+void bind_tables(uintptr_t fork, uintptr_t release, uintptr_t release_bytes, uintptr_t compact, uintptr_t compact_bytes,
+                 uintptr_t runs, uintptr_t runs_bytes) {
+  g_fork = reinterpret_cast<ForkFn>(fork);
+  g_release = reinterpret_cast<ReleaseFn>(release);
+  g_release_bytes = reinterpret_cast<BytesFn>(release_bytes);
+  g_compact = reinterpret_cast<CompactFn>(compact);
+  g_compact_bytes = reinterpret_cast<BytesFn>(compact_bytes);
+  g_runs = reinterpret_cast<RunsFn>(runs);
+  g_runs_bytes = reinterpret_cast<BytesFn>(runs_bytes);
 }
 
 void bind_serving(uintptr_t process, uintptr_t greedy, uintptr_t greedy_workspace, uintptr_t copy) {
@@ -246,6 +274,102 @@ py::object logits(bool greedy, const at::Tensor& x, const Maybe& history, const 
   return rc == 0 ? py::cast(y) : py::none();
 }
 
+// Block tables, and the sizes that go with them.
+struct Tables {
+  at::Device dev = at::kCPU;
+  int64_t R, width, stride;
+  int32_t* at;
+  bool of(const at::Tensor& t, int64_t device) {
+    if (!plain(t) || t.dim() != 2 || t.scalar_type() != at::kInt || t.device().index() != device || !rows(t, stride))
+      return false;
+    dev = t.device(), R = t.size(0), width = t.size(1), at = t.mutable_data_ptr<int32_t>();
+    return R > 0;
+  }
+  bool ints(const Maybe& t, int64_t n) const { return none_or(t, dev, at::kInt, {n}); }
+  bool pool_of(const at::Tensor& free, const at::Tensor& pool, const Maybe& shares) const {
+    return free.dim() == 1 && ints(free, free.size(0)) && ints(pool, 4) && ints(shares, free.size(0));
+  }
+};
+int32_t* out(const Maybe& t) { return t ? t->mutable_data_ptr<int32_t>() : nullptr; }
+
+// pare_amd.fork_block_tables: (src, dst).
+py::object fork_tables(const at::Tensor& tables, const at::Tensor& kv_lens, const at::Tensor& parents,
+                       const at::Tensor& free, const at::Tensor& pool, const at::Tensor& shares, const Maybe& lengths,
+                       int64_t ps, int64_t device, uintptr_t stream) {
+  Tables t;
+  if (!g_fork || !t.of(tables, device) || !t.ints(kv_lens, t.R) || !t.ints(parents, t.R) || !t.ints(lengths, t.R) ||
+      !t.pool_of(free, pool, shares))
+    return py::none();
+  const at::Tensor all = at::empty({3, t.R}, at::TensorOptions().dtype(at::kInt).device(t.dev));
+  int32_t* p = all.mutable_data_ptr<int32_t>();
+  int rc;
+  {
+    py::gil_scoped_release unlocked;
+    rc = g_fork(t.at, t.stride, out(kv_lens), ptr<int32_t>(parents), ptr<int32_t>(lengths), ptr<int32_t>(free),
+                out(pool), out(shares), p, p + t.R, p + 2 * t.R, t.R, t.width, free.size(0), ps,
+                reinterpret_cast<void*>(stream));
+  }
+  return rc == 0 ? py::object(py::make_tuple(all.select(0, 0), all.select(0, 1))) : py::none();
+}
+
+// pare_amd.release_block_tables with shares: whether it was done.
+bool release_tables(const at::Tensor& tables, const at::Tensor& kv_lens, const at::Tensor& done, const at::Tensor& free,
+                    const at::Tensor& pool, const at::Tensor& shares, int64_t ps, int64_t device, uintptr_t stream) {
+  Tables t;
+  if (!g_release || !t.of(tables, device) || !t.ints(kv_lens, t.R) || !none_or(done, t.dev, at::kBool, {t.R}) ||
+      !t.pool_of(free, pool, shares))
+    return false;
+  const size_t bytes = g_release_bytes(free.size(0));
+  const at::Tensor scratch = at::empty({(int64_t)bytes}, at::TensorOptions().dtype(at::kByte).device(t.dev));
+  py::gil_scoped_release unlocked;
+  return g_release(t.at, t.stride, out(kv_lens), reinterpret_cast<const uint8_t*>(done.const_data_ptr()), out(free),
+                   out(pool), out(shares), t.R, t.width, free.size(0), ps, scratch.mutable_data_ptr(), bytes,
+                   reinterpret_cast<void*>(stream)) == 0;
+}
+
+// pare_amd.compact_block_tables: (src, dst, count).
+py::object compact_tables(const at::Tensor& tables, const at::Tensor& kv_lens, const at::Tensor& free,
+                          const at::Tensor& pool, const Maybe& shares, int64_t ps, int64_t device, uintptr_t stream) {
+  Tables t;
+  if (!g_compact || !t.of(tables, device) || !t.ints(kv_lens, t.R) || !t.pool_of(free, pool, shares)) return py::none();
+  const int64_t pages = free.size(0), half = pages / 2;
+  if (pages == 0) return py::none();
+  const size_t bytes = g_compact_bytes(pages);
+  const at::Tensor all =
+      at::empty({2 * half + 1 + (int64_t)(bytes / 4)}, at::TensorOptions().dtype(at::kInt).device(t.dev));
+  int32_t* p = all.mutable_data_ptr<int32_t>();
+  int rc;
+  {
+    py::gil_scoped_release unlocked;
+    rc = g_compact(t.at, t.stride, ptr<int32_t>(kv_lens), out(free), out(pool), out(shares), p, p + half, p + 2 * half,
+                   t.R, t.width, pages, ps, p + 2 * half + 1, bytes, reinterpret_cast<void*>(stream));
+  }
+  if (rc != 0) return py::none();
+  return py::make_tuple(all.narrow(0, 0, half), all.narrow(0, half, half), all.narrow(0, 2 * half, 1));
+}
+
+// pare_amd.shared_prefixes: (starts, lens, runs).
+py::object shared_prefixes(const at::Tensor& tables, const at::Tensor& kv_lens, const Maybe& q_starts, int64_t ps,
+                           int64_t least_pages, int64_t device, uintptr_t stream, const py::function& workspace_fn) {
+  Tables t;
+  if (!g_runs || !t.of(tables, device) || !t.ints(kv_lens, t.R) || !t.ints(q_starts, t.R + 1)) return py::none();
+  const size_t need = g_runs_bytes(t.R);
+  if (!need) return py::none();
+  const at::Tensor ws = workspace_fn(need).cast<at::Tensor>();
+  if (!plain(ws) || ws.device() != t.dev) return py::none();
+  const at::Tensor all = at::empty({6 * t.R + 1}, at::TensorOptions().dtype(at::kInt).device(t.dev));
+  int32_t* p = all.mutable_data_ptr<int32_t>() + 4 * t.R;
+  int rc;
+  {
+    py::gil_scoped_release unlocked;
+    rc = g_runs(t.at, t.stride, ptr<int32_t>(kv_lens), ptr<int32_t>(q_starts), p, p + t.R + 1, p - 4 * t.R, t.R, t.width,
+                ps, least_pages, ws.mutable_data_ptr(), (size_t)ws.numel(), reinterpret_cast<void*>(stream));
+  }
+  if (rc != 0) return py::none();
+  return py::make_tuple(all.narrow(0, 4 * t.R, t.R + 1), all.narrow(0, 5 * t.R + 1, t.R),
+                        all.narrow(0, 0, 4 * t.R).view({t.R, 4}));
+}
+
 // The layers' buffers of one kind: a sequence of tensors of the same sizes and type, or one tensor with the
 // layers first. `first` is the first layer's.
 bool layers(const py::object& all, const at::Device& dev, std::vector<void*>& at_layers, at::Tensor& first) {
@@ -304,7 +428,12 @@ bool copy_pages(const at::Tensor& src, const at::Tensor& dst, const Maybe& count
 PYBIND11_MODULE(_host, m) {
   m.def("bind", &bind);
   m.def("bind_serving", &bind_serving);
+  m.def("bind_tables", &bind_tables);
   m.def("logits", &logits);
+  m.def("fork_tables", &fork_tables);
+  m.def("release_tables", &release_tables);
+  m.def("compact_tables", &compact_tables);
+  m.def("shared_prefixes", &shared_prefixes);
   m.def("copy_pages", &copy_pages);
   m.def("matmul", &matmul);
 }

@@ -99,6 +99,7 @@ struct PagedRuns {
   const int32_t* q_starts;  // null: one query a request
   int32_t* starts;          // [R + 1]
   int32_t* lens;            // [R]
+  int32_t* runs;            // [R, 4] of each: first request, first query, queries, positions shared; 0 behind the last
   int32_t* counter;         // 0, and 0 again afterwards
   int32_t* common;          // scratch [R]
   int64_t R, width, ps, least_pages;
@@ -136,8 +137,8 @@ struct PagedAttention {
   int64_t window;  // 0: none
   float scale;
   bool bf16;
-  const int32_t* run_starts;  // [R + 1] and [R]: runs of requests that share their first pages, or null
-  const int32_t* run_lens;
+  const int32_t* runs;      // [R, 4] runs of requests that share their first pages (PagedRuns), or null
+  const int32_t* run_lens;  // [R]
 };
 // Whether the count of tiles that the requests of few query rows may have fits 32 bits.
 bool paged_attention_tiles_fit(const PagedAttention& p, const PagedCache& c);

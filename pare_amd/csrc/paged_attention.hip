@@ -34,22 +34,23 @@ struct AttnArgs {
   int* counters;  // one of each of them, and behind them one of each item of many rows
   float *few_part, *many_part;
   // runs of requests with the same first pages (kParts)
-  const int32_t* run_starts;
-  const int32_t* run_lens;
+  const int4* runs;         // [R] first request, first query, queries, keys; no queries: none
+  const int32_t* run_lens;  // [R] positions that a request shares
   int run_rows;       // runs of up to so many query rows are `few`
   int many_wgs;       // workgroups that the ranges of a run's keys are made for
   // Parts of rows, D + 4 floats each (values, max, sum): of the ranges of runs of many rows, in
   // tiles of kRows; of runs of few rows [T, H]; of the keys behind what is shared [T, H].
   float *parts_many, *parts_few, *parts_own;
-  int2* where;        // [T, H] a row's first shared part (its offset from parts_many in records), and how many
+  int2* where;        // [T, H] a row's first shared part (its offset from parts_many in records), and 2 n of n
+                      // parts that lie kRows records apart, 2 n + 1 of n that lie kRows / 2 apart
   int part_records;   // that parts_many and parts_few hold
 };
 
 // What a launch computes: whole rows; or, where requests share their first pages, parts of
 // rows. A run is then a request whose queries are those of all its members and whose keys are the
 // shared ones, which all of its queries see; each member has the keys behind them for itself. All
-// parts are of one launch, and a second one joins them (join_parts_kernel). Numbers 0 .. R - 1 are
-// the requests, R .. 2 R - 1 the runs.
+// parts are of one launch, and a second one joins them (join_parts_kernel). Numbers 2 r are
+// the requests, 2 r + 1 the runs.
 enum Mode { kWhole, kParts };
 
 // What a request's queries see, from its row of kv_lens and q_starts.
@@ -64,32 +65,21 @@ struct Request {
 // The first position that a query sees whose last is `last` (negative ones see nothing, and a
 // large window less them would leave the integers).
 PMI_DEV int first_position(const AttnArgs& a, int last) { return a.window && last >= a.window ? last + 1 - a.window : 0; }
-// Positions that request r shares with its run, in whole pages.
-PMI_DEV int shared_len(const AttnArgs& a, int r) {
-  return min(max(a.run_lens[r], 0), a.width * a.ps) & ~(a.ps - 1);
-}
-// The same, or 0 where one of its own queries (from position `shift` on) lies among them.
-PMI_DEV int shared_before(const AttnArgs& a, int r, int shift) {
-  const int len = shared_len(a, r);
-  return shift + 1 > len ? len : 0;
-}
+// Positions that are shared, in whole pages.
+PMI_DEV int shared_len(const AttnArgs& a, int len) { return min(max(len, 0), a.width * a.ps) & ~(a.ps - 1); }
 template <Mode MODE>
 PMI_DEV Request request(const AttnArgs& a, int r) {
   Request q;
-  q.run = MODE == kParts && r >= a.R;
+  q.run = MODE == kParts && (r & 1);
+  if constexpr (MODE == kParts) r >>= 1;
   if (q.run) {
-    r -= a.R;
-    const int first = a.run_starts[r], last = a.run_starts[r + 1];
-    const bool run = first >= 0 && first < last && last <= a.R;
-    q.row = run ? first : 0;
-    q.start = run ? first : 0, q.n = run ? last - first : 0;
-    if (run && a.q_starts) {
-      q.start = a.q_starts[first];
-      q.n = a.q_starts[last] - q.start;
-    }
-    q.len = run ? min(shared_len(a, first), a.max_kv) : 0;
+    const int4 run = a.runs[r];
+    const bool there = run.x >= 0 && run.x < a.R && run.y >= 0 && run.z > 0 && (int64_t)run.y + run.z <= a.T;
+    q.row = there ? run.x : 0;
+    q.start = there ? run.y : 0;
+    q.len = there ? min(shared_len(a, run.w), a.max_kv) : 0;
+    q.n = q.len ? run.z : 0;
     q.shift = q.len;  // (all queries see all of them)
-    if (q.len == 0 || q.n < 0 || q.start < 0 || (int64_t)q.start + q.n > a.T) q.n = 0;
     q.first_seen = q.lo = 0;
     q.hi = a.n_pages ? q.len : 0;
     return q;
@@ -105,7 +95,12 @@ PMI_DEV Request request(const AttnArgs& a, int r) {
   q.shift = max(len0, 0) - q.n;  // (with the keys past the bounds and the queries past max_q)
   q.n = min(q.n, a.max_q);
   if (q.n < 0 || q.start < 0 || (int64_t)q.start + q.n > a.T) q.n = 0;
-  q.first_seen = min(MODE == kParts ? shared_before(a, r, q.shift) : first_position(a, q.shift), q.len);
+  if constexpr (MODE == kParts) {
+    const int len = shared_len(a, a.run_lens[r]);
+    q.first_seen = q.shift + 1 > len ? min(len, q.len) : 0;  // (none of its own queries may lie among them)
+  } else {
+    q.first_seen = min(first_position(a, q.shift), q.len);
+  }
   q.lo = q.first_seen & ~15;
   q.hi = a.n_pages ? max(q.lo, min(q.len, q.shift + q.n)) : q.lo;
   return q;
@@ -322,15 +317,21 @@ PMI_DEV void few_rows(const AttnArgs& a, FewLds<D>& lds, int wg) {
   auto items_of = [&](const Request& rq) {
     return rq.n * G > (rq.run ? a.run_rows : a.few_rows) ? 0 : (rq.n * G + 15) / 16 * a.KV;
   };
-  const int requests = MODE == kWhole ? a.R : 2 * a.R;
-  const int run = (requests + 63) >> 6, r_lane = run * l;
+  constexpr int kOf = MODE == kWhole ? 1 : 2;  // numbers of a request
+  const int requests = kOf * a.R;
+  const int run = kOf * ((a.R + 63) >> 6), r_lane = run * l;
   int in_lane = 0, parts_lane[kCuts] = {};  // tiles, and parts of cut_of(k) tiles
-  for (int x = r_lane; x < min(requests, r_lane + run); ++x) {
-    const Request rq = request<MODE>(a, x);
-    const int nt = tiles_of(rq), items = items_of(rq);
-    in_lane += nt * items;
+  for (int x = r_lane; x < min(requests, r_lane + run); x += kOf) {
+    Request rq[kOf];
 #pragma unroll
-    for (int k = 0; k < kCuts; ++k) parts_lane[k] += (nt + cut_of(k) - 1) / cut_of(k) * items;
+    for (int i = 0; i < kOf; ++i) rq[i] = request<MODE>(a, x + i);
+#pragma unroll
+    for (int i = 0; i < kOf; ++i) {
+      const int nt = tiles_of(rq[i]), items = items_of(rq[i]);
+      in_lane += nt * items;
+#pragma unroll
+      for (int k = 0; k < kCuts; ++k) parts_lane[k] += (nt + cut_of(k) - 1) / cut_of(k) * items;
+    }
   }
   auto scan = [&](int v) {
 #pragma unroll
@@ -570,7 +571,7 @@ PMI_DEV void few_rows(const AttnArgs& a, FewLds<D>& lds, int wg) {
     for (int x = 0; x < n; x += 4) *reinterpret_cast<f32x4*>(rec + d + x) = f32x4{v[x], v[x + 1], v[x + 2], v[x + 3]};
     if (d == 0) {
       *reinterpret_cast<float2*>(rec + D) = float2{m, l};
-      if (rq.run) a.where[at] = int2{(int)((a.parts_few - a.parts_many) / (D + 4) + at), 1};
+      if (rq.run) a.where[at] = int2{(int)((a.parts_few - a.parts_many) / (D + 4) + at), 2};
     }
   };
   auto store = [&]() {
@@ -729,21 +730,27 @@ hipError_t few(const AttnArgs& a, bool fp8, hipStream_t stream) {
 // Where the rows give fewer workgroups than the CUs hold, the keys are split as well
 // (`splits` ranges of `per` tokens), and the last range to arrive joins them.
 constexpr int kRows = 128;
-constexpr int kLeastRange = 256;  // keys of a run's range, at least
+// Keys of a run's range, at least (us, 64 requests of 8192 shared keys, 256 / 512 / 768 / 1024: 49 / 42 / 45 / 52; 16 of 8000
+// 31 / 28 / 30 / 34): every range is 68 KB of parts.
+constexpr int kLeastRange = 512;
+
+// HALVES (kParts): 2 for runs of up to half as many rows: two waves take the first 32 keys of each
+// tile, two the last, as parts of their own. Nothing waits for the ranges: their parts are joined by
+// another launch (joined by the last range of an item, 16 x 128 rows of 16 ranges took 81 us, so 36).
+template <typename T, int D, bool FP8, Mode MODE, int HALVES>
+PMI_DEV void many_tile(const AttnArgs& a, uint8_t* lds, int& s_last, const Request& rq, int rt, int kh, int index,
+                       int sp, int splits);
 
 template <typename T, int D, bool FP8, Mode MODE>
 PMI_DEV void many_rows(const AttnArgs& a, uint8_t* lds, int& s_last, int wg) {
-  constexpr int KP = D / 64;       // 16-byte pieces of K, and of V, per thread and tile
-  constexpr int kSlot = 64 * D * 2;  // bytes of K (or V) of a tile as fp16
-  const int tid = threadIdx.x, l = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int c = l & 31, h = l >> 5;
+  const int l = threadIdx.x & 63;
   const int G = a.H / a.KV;
 
   // which rows: the row tiles of all requests in order, each request's last ones (with the most
   // keys) first, the KV heads innermost (an XCD then keeps few heads' keys in its L2)
-  const int first_request = MODE == kWhole ? 0 : a.R;
+  const auto number = [](int r) { return MODE == kWhole ? r : 2 * r + 1; };
   auto tiles_of = [&](int r) {
-    const Request rq = request<MODE>(a, first_request + r);
+    const Request rq = request<MODE>(a, number(r));
     return rq.n * G > (MODE == kWhole ? a.few_rows : a.run_rows) ? (rq.n * G + kRows - 1) / kRows : 0;
   };
   const int kh = wg % a.KV, rest = wg / a.KV;
@@ -772,15 +779,32 @@ PMI_DEV void many_rows(const AttnArgs& a, uint8_t* lds, int& s_last, int wg) {
     count = tiles_of(r);
   }
   const int rt = count - 1 - at_tile;
-  const Request rq = request<MODE>(a, first_request + r);
+  const Request rq = request<MODE>(a, number(r));
+  if (MODE == kParts && rq.n * G <= kRows / 2)
+    many_tile<T, D, FP8, MODE, MODE == kParts ? 2 : 1>(a, lds, s_last, rq, rt, kh, index, sp, splits);
+  else
+    many_tile<T, D, FP8, MODE, 1>(a, lds, s_last, rq, rt, kh, index, sp, splits);
+}
+
+template <typename T, int D, bool FP8, Mode MODE, int HALVES>
+PMI_DEV void many_tile(const AttnArgs& a, uint8_t* lds, int& s_last, const Request& rq, int rt, int kh, int index,
+                       int sp, int splits) {
+  constexpr int KP = D / 64;       // 16-byte pieces of K, and of V, per thread and tile
+  constexpr int kSlot = 64 * D * 2;  // bytes of K (or V) of a tile as fp16
+  constexpr int U = 2 / HALVES;    // of the tile's two halves, those of a wave
+  constexpr int kTileRows = kRows / HALVES;
+  const int tid = threadIdx.x, l = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int c = l & 31, h = l >> 5;
+  const int G = a.H / a.KV;
+  const int row_wave = HALVES == 1 ? wave : wave & 1, half = HALVES == 1 ? 0 : wave >> 1;
   const int start = rq.start, len = rq.len, shift = rq.shift;
-  const int rows = min(kRows, rq.n * G - rt * kRows);
-  const int row = rt * kRows + wave * 32 + c;
-  const bool live = wave * 32 + c < rows;
+  const int rows = min(kTileRows, rq.n * G - rt * kTileRows);
+  const int row = rt * kTileRows + row_wave * 32 + c;
+  const bool live = row_wave * 32 + c < rows;
   const int i = row / G;
   const int hi = live ? max(0, min(len, shift + i + 1)) : 0;
   const int lo = MODE == kWhole ? first_position(a, shift + i) : rq.first_seen;
-  const int i_first = rt * kRows / G, i_last = (rt * kRows + rows - 1) / G;
+  const int i_first = rt * kTileRows / G, i_last = (rt * kTileRows + rows - 1) / G;
   const int first_seen = MODE == kWhole ? min(first_position(a, shift + i_first), len) : rq.first_seen;
   const int all_lo = first_seen & ~15;
   const int all_hi = a.n_pages ? max(all_lo, min(len, shift + i_last + 1)) : all_lo;
@@ -900,16 +924,16 @@ PMI_DEV void many_rows(const AttnArgs& a, uint8_t* lds, int& s_last, int wg) {
       const uint8_t* kb = lds + slot * 2 * kSlot;
       const uint8_t* vb = kb + kSlot;
       __builtin_amdgcn_s_setprio(1);  // products ahead of the other wave's softmax
-      f32x16 s[2];
+      f32x16 s[U];
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
+      for (int u = 0; u < U; ++u)
 #pragma unroll
         for (int e = 0; e < 16; ++e) s[u][e] = 0.f;
 #pragma unroll
       for (int x = 0; x < D / 16; ++x)
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const int krow = 32 * u + 16 * (c >> 4) + 8 * ((c >> 2) & 1) + 4 * ((c >> 3) & 1) + (c & 3);
+        for (int u = 0; u < U; ++u) {
+          const int krow = 32 * (u + half) + 16 * (c >> 4) + 8 * ((c >> 2) & 1) + 4 * ((c >> 3) & 1) + (c & 3);
           const f16x8 k8 = *reinterpret_cast<const f16x8*>(kb + krow * D * 2 + (((2 * x + h) ^ swizzle(krow)) << 4));
           s[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k8, qv[x], s[u], 0, 0, 0);
         }
@@ -920,11 +944,11 @@ PMI_DEV void many_rows(const AttnArgs& a, uint8_t* lds, int& s_last, int wg) {
       // result 16 u + 4 j + e: token 32 u + 16 (j / 2) + 8 h + 4 (j % 2) + e, block 2 u + j / 2.
       // Hidden tokens get -inf, which stays one through the factors k1 (at least FLT_MIN).
       if (p < safe_lo || p + 64 > safe_hi || p + 64 > p1 || __any(gone)) {
-        const int from = lo - p - 8 * h, to = min(hi, p1) - p - 8 * h;
+        const int from = lo - p - 8 * h - 32 * half, to = min(hi, p1) - p - 8 * h - 32 * half;
 #pragma unroll
-        for (int y = 0; y < 32; ++y) {
+        for (int y = 0; y < 16 * U; ++y) {
           const int at = 16 * (y >> 3) + (y & 7);
-          const int end = __builtin_amdgcn_readlane(cur.page, y >> 3) >= 0 ? to : 0;
+          const int end = __builtin_amdgcn_readlane(cur.page, 2 * half + (y >> 3)) >= 0 ? to : 0;
           s[y >> 4][y & 15] = at >= from && at < end ? s[y >> 4][y & 15] : -INFINITY;
         }
       }
@@ -932,22 +956,22 @@ PMI_DEV void many_rows(const AttnArgs& a, uint8_t* lds, int& s_last, int wg) {
         // a page that holds an infinity or NaN: what sees it becomes NaN
         if (bad) ks = 0.f, vs = 0.f;
 #pragma unroll
-        for (int b = 0; b < 4; ++b)
+        for (int b = 0; b < 2 * U; ++b)
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
             const float t = s[b >> 1][8 * (b & 1) + e];
-            s[b >> 1][8 * (b & 1) + e] = t == -INFINITY || !(which >> b & 1) ? t : __builtin_nanf("");
+            s[b >> 1][8 * (b & 1) + e] = t == -INFINITY || !(which >> (2 * half + b) & 1) ? t : __builtin_nanf("");
           }
       }
       const float vlog = __builtin_amdgcn_logf(vs);
       // (FLT_MIN after all factors, the query's power of two among them; the sums are below 2^33, so what
       // it raises is a score of 0 all the same)
-      float k1[4];
+      float k1[2 * U];
 #pragma unroll
-      for (int b = 0; b < 4; ++b) k1[b] = fmaxf(of_block(ks, b) * qmul, FLT_MIN);
+      for (int b = 0; b < 2 * U; ++b) k1[b] = fmaxf(of_block(ks, 2 * half + b) * qmul, FLT_MIN);
       float mx = -INFINITY;
 #pragma unroll
-      for (int b = 0; b < 4; ++b) {
+      for (int b = 0; b < 2 * U; ++b) {
         float t = s[b >> 1][8 * (b & 1)];
 #pragma unroll
         for (int e = 1; e < 8; ++e) t = fmaxf(t, s[b >> 1][8 * (b & 1) + e]);
@@ -959,11 +983,11 @@ PMI_DEV void many_rows(const AttnArgs& a, uint8_t* lds, int& s_last, int wg) {
       if (__any(nm > ref.max + kSlack || mx + max_of_4(vlog) > ref.weight + kSlack)) {
         float most = -INFINITY;
 #pragma unroll
-        for (int b = 0; b < 4; ++b) {
+        for (int b = 0; b < 2 * U; ++b) {
           float t = s[b >> 1][8 * (b & 1)];
 #pragma unroll
           for (int e = 1; e < 8; ++e) t = fmaxf(t, s[b >> 1][8 * (b & 1) + e]);
-          most = fmaxf(most, fmaf(t, k1[b], of_block(vlog, b)));
+          most = fmaxf(most, fmaf(t, k1[b], of_block(vlog, 2 * half + b)));
         }
         most = fmaxf(most, __shfl_xor(most, 32));
         const Rescale f = raise(ref, nm, most);
@@ -979,8 +1003,8 @@ PMI_DEV void many_rows(const AttnArgs& a, uint8_t* lds, int& s_last, int wg) {
       entry = look_up(p + 192);
       const float base = ref.max == -INFINITY ? 0.f : ref.max;
 #pragma unroll
-      for (int b = 0; b < 4; ++b) {
-        const float v1 = share_of(of_block(vs, b), ref);
+      for (int b = 0; b < 2 * U; ++b) {
+        const float v1 = share_of(of_block(vs, 2 * half + b), ref);
         f16x8 pw;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
@@ -991,7 +1015,7 @@ PMI_DEV void many_rows(const AttnArgs& a, uint8_t* lds, int& s_last, int wg) {
 #pragma unroll
         for (int d = 0; d < D / 32; ++d) {
           const int vrow = 32 * d + c;
-          const f16x8 v8 = *reinterpret_cast<const f16x8*>(vb + vrow * 128 + (((2 * b + h) ^ ((vrow >> 1) & 7)) << 4));
+          const f16x8 v8 = *reinterpret_cast<const f16x8*>(vb + vrow * 128 + (((2 * b + 4 * half + h) ^ ((vrow >> 1) & 7)) << 4));
           acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v8, pw, acc[d], 0, 0, 0);
         }
       }
@@ -1008,6 +1032,7 @@ PMI_DEV void many_rows(const AttnArgs& a, uint8_t* lds, int& s_last, int wg) {
   T* dst = (T*)a.out + out_row * D + 4 * h;
   if constexpr (MODE == kParts) {
     const int64_t at = ((int64_t)(index * a.KV + kh) * splits + sp) * kRows + wave * 32 + c;
+    static_assert(HALVES <= 2, "the second half's records lie behind the first's");
     float* rec = a.parts_many + at * (D + 4);
 #pragma unroll
     for (int d = 0; d < D / 32; ++d)
@@ -1019,7 +1044,7 @@ PMI_DEV void many_rows(const AttnArgs& a, uint8_t* lds, int& s_last, int wg) {
         if (live) *reinterpret_cast<f32x4*>(rec + 32 * d + 8 * j + 4 * h) = y;
       }
     if (live && h == 0) *reinterpret_cast<float2*>(rec + D) = float2{ref.max, sum};
-    if (live && h == 0 && sp == 0) a.where[out_row] = int2{(int)at, parts};
+    if (live && h == 0 && sp == 0 && half == 0) a.where[out_row] = int2{(int)at, 2 * HALVES * parts + HALVES - 1};
     return;
   }
   if (parts == 1) {
@@ -1129,36 +1154,54 @@ hipError_t many(const AttnArgs& a, bool fp8, int64_t wgs, hipStream_t stream) {
   return hipGetLastError();
 }
 
-// The parts of the rows that share keys: a workgroup the rows of a request and KV head, D / 4 threads a
-// row, its own part first and the shared ones in order.
+// The parts of the rows that share keys. D / 4 threads a row and four groups of them, which take every
+// fourth shared part, the first its own as well; the groups are joined in LDS, in order. Bound by its
+// chain of loads (lengths, where, parts). Workgroup (r, KV head, z) takes every gridDim.z-th of the head's
+// rows of request r, some at a time.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void join_parts_kernel(AttnArgs a) {
-  constexpr int kRowThreads = D / 4, kFly = 8;
+  constexpr int kRowThreads = D / 4, kGroups = 4, kFly = 8, kSlots = 256 / kRowThreads / kGroups;
+  __shared__ __attribute__((aligned(16))) float s_o[kSlots][kGroups][D];
+  __shared__ float2 s_ml[kSlots][kGroups];
   const int r = blockIdx.x, kh = blockIdx.y, G = a.H / a.KV;
-  const Request rq = request<kParts>(a, r);
+  const Request rq = request<kParts>(a, 2 * r);
   if (rq.n <= 0 || rq.first_seen <= 0) return;
-  const int dim = 4 * (threadIdx.x % kRowThreads);
-  for (int row = threadIdx.x / kRowThreads; row < rq.n * G; row += 256 / kRowThreads) {
+  const int dim = 4 * (threadIdx.x % kRowThreads), group = threadIdx.x / kRowThreads % kGroups;
+  const int slot = threadIdx.x / kRowThreads / kGroups;
+  for (int row0 = blockIdx.z * kSlots; row0 < rq.n * G; row0 += gridDim.z * kSlots) {
+    const int row = min(row0 + slot, rq.n * G - 1);
     const int64_t out_row = (int64_t)(rq.start + row / G) * a.H + kh * G + row % G;
     const float* own = a.parts_own + out_row * (D + 4);
-    float m = own[D], l = own[D + 1];
-    f32x4 o = *reinterpret_cast<const f32x4*>(own + dim);
-    int2 at = a.where[out_row];
+    const bool first = group == 0;
+    float m = first ? own[D] : -INFINITY, l = first ? own[D + 1] : 0.f;
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    if (first) o = *reinterpret_cast<const f32x4*>(own + dim);
+    const int2 at = a.where[out_row];
+    const int apart = at.y & 1 ? kRows / 2 : kRows;
     // (nobody wrote it if the runs are not this batch's)
-    if (at.x < 0 || at.y < 0 || (int64_t)at.x + (int64_t)kRows * (at.y - 1) >= a.part_records) at = int2{0, 0};
+    const bool there = at.x >= 0 && at.y >= 2 && (int64_t)at.x + (int64_t)apart * ((at.y >> 1) - 1) < a.part_records;
+    const int n = there ? at.y >> 1 : 0;
     const float* rec = a.parts_many + (int64_t)at.x * (D + 4);
-    for (int s0 = 0; s0 < at.y; s0 += kFly) {
+    for (int s0 = group; s0 < n; s0 += kFly * kGroups) {
       float2 ml[kFly];
       f32x4 v[kFly];
 #pragma unroll
       for (int k = 0; k < kFly; ++k) {
-        const float* p = rec + (int64_t)min(s0 + k, at.y - 1) * kRows * (D + 4);
+        const float* p = rec + (int64_t)min(s0 + kGroups * k, n - 1) * apart * (D + 4);
         ml[k] = *reinterpret_cast<const float2*>(p + D);
         v[k] = *reinterpret_cast<const f32x4*>(p + dim);
       }
 #pragma unroll
-      for (int k = 0; k < kFly; ++k) join(m, l, o, ml[k].x, ml[k].y, v[k], s0 + k < at.y);
+      for (int k = 0; k < kFly; ++k) join(m, l, o, ml[k].x, ml[k].y, v[k], s0 + kGroups * k < n);
     }
+    __syncthreads();  // the previous rows are read
+    *reinterpret_cast<f32x4*>(&s_o[slot][group][dim]) = o;
+    if (dim == 0) s_ml[slot][group] = float2{m, l};
+    __syncthreads();
+    if (!first || row0 + slot >= rq.n * G) continue;
+#pragma unroll
+    for (int g = 1; g < kGroups; ++g)
+      join(m, l, o, s_ml[slot][g].x, s_ml[slot][g].y, *reinterpret_cast<const f32x4*>(&s_o[slot][g][dim]), true);
     const float inv = l > 0.f ? 1.f / l : (l != l ? l : 0.f);
     typedef T T4 __attribute__((ext_vector_type(4)));
     T4 y;
@@ -1243,7 +1286,7 @@ AttnArgs attention_args(const PagedAttention& p, const PagedCache& c, void* work
   a.few_part = (float*)((char*)workspace + kWsCounterBytes);
   a.many_part = (float*)((char*)a.few_part + few_part_bytes(c.D));
   a.few_wgs = few_wgs(c.D);
-  a.run_starts = p.run_starts, a.run_lens = p.run_lens;
+  a.runs = (const int4*)p.runs, a.run_lens = p.run_lens;
   return a;
 }
 
@@ -1259,8 +1302,9 @@ hipError_t launch_mode(const AttnArgs& a, const PagedAttention& p, const PagedCa
   return c.D == 64 ? many<f16, 64, MODE>(a, c.fp8, n, stream) : many<f16, 128, MODE>(a, c.fp8, n, stream);
 }
 
-// Query rows up to which a run is one of few.
-constexpr int kRunRows = 32;
+// Query rows up to which a run is one of few: those read its codes once for every 16 rows (us with 16 / 32, 64
+// requests of 8 families, 4000 / 16000 keys each: 39 / 69, 65 / 155; 8 of one, 8000: 22.0 / 25.1).
+constexpr int kRunRows = 16;
 
 // Row tiles of all runs of many rows x KV heads, at most.
 int64_t run_items(const PagedAttention& p, const PagedCache& c) {
@@ -1278,13 +1322,26 @@ size_t part_bytes(int64_t rows, int64_t D) { return (size_t)(rows * (D + 4) * 4)
 
 }  // namespace
 
+// Parts pay where what is read per request without them is much. us, in parts / whole (32 / 8 heads of 128
+// unless said, int8, one token each; `families` of equal share, 300 more keys each; without the 6 of
+// finding the runs):
+//   16 requests, 1 family, 1000 / 2000 / 4000 keys   20.8 / 14.2   21.1 / 18.4   23.0 / 25.6
+//   64 requests, 1 family, 1000 / 2000 / 8000         32.5 / 21.8   34.4 / 39.1   40.1 / 101
+//   64 requests, 8 families, 1000 / 2000 / 16000      29.8 / 21.4   31.4 / 40.9   65 / 218
+//   64 of 4 KV heads of 64, 1 family, 4000 / 8000     26.4 / 22.8   29.0 / 42.7
+//   8 requests, 1 family, 4000 / 8000                 20.6 / 18.4   22.0 / 25.6
+// Many rows a request make better use of keys by themselves: 7 tokens each of 32 (28 rows), 4000 keys, 45.6 /
+// 52.1; 16 of 64 (64 rows), 2000 keys, 121 / 80.
+constexpr int kShareRows = 32;
+constexpr int64_t kShareKeys = 2048, kShareBytes = 1ll << 27;
 bool paged_attention_shares(const PagedAttention& p, const PagedCache& c) {
-  return p.R > 1 && p.T < (1ll << 30) && p.window == 0 && p.max_q * (p.H / c.KV) <= kFewRows;
+  return p.R > 1 && p.T < (1ll << 30) && p.window == 0 && p.max_q * (p.H / c.KV) <= kShareRows &&
+         p.max_kv >= kShareKeys && p.R * c.KV * 2 * c.D >= (kShareBytes + p.max_kv - 1) / p.max_kv;
 }
 
 bool paged_shared_launch_fits(const PagedAttention& p, const PagedCache& c) {
   // (parts are counted in 32 bits, and requests and runs together)
-  return few_wgs(c.D) + run_wgs(p, c) < (1ll << 23) && p.R < (1ll << 29) && p.R * c.KV < (1ll << 24) &&
+  return few_wgs(c.D) + run_wgs(p, c) < (1ll << 23) && p.R < (1ll << 29) && p.R * c.KV < (1ll << 21) &&
          run_wgs(p, c) * kRows + 2 * p.T * p.H < (1ll << 31);
 }
 
@@ -1304,7 +1361,9 @@ hipError_t launch_paged_shared(const PagedAttention& p, const PagedCache& c, voi
   a.run_rows = kRunRows;
   a.many_wgs = 2 * device_cu_count();
   if (hipError_t e = launch_mode<kParts>(a, p, c, wgs ? a.few_wgs + wgs : 0, stream); e != hipSuccess) return e;
-  const dim3 grid((unsigned)p.R, (unsigned)c.KV), block(256);
+  // (of a row's four groups of D / 4 threads each; up to 8 workgroups share a request's rows)
+  const int64_t slots = 64 / (c.D / 4), pieces = (p.max_q * (p.H / c.KV) + slots - 1) / slots;
+  const dim3 grid((unsigned)p.R, (unsigned)c.KV, (unsigned)(pieces < 8 ? pieces : 8)), block(256);
   if (p.bf16) {
     if (c.D == 64)
       hipLaunchKernelGGL((join_parts_kernel<__bf16, 64>), grid, block, 0, stream, a);

@@ -122,6 +122,125 @@ __global__ __launch_bounds__(256) void share_pages_kernel(PagedFork f) {
   for (int j = j0 + threadIdx.x; j < min(full, j0 + kRowEntries); j += 256) share_page(f, r, parent, j);
 }
 
+// ---- caches of few pages, in one workgroup ----------------------------------------------
+
+// Releases and compactions of few table entries and pages are bound by their launches and the chain of
+// loads: one workgroup of 1024 threads then does all, with a bit or a count of each page in LDS (12 requests of 19
+// pages, a cache of 40: SMALL_US; in two and in five launches LARGE_US).
+constexpr int kSmallPages = 16384, kSmallEntries = 4096, kSmallThreads = 1024;
+
+// f(r, j, page) for the entries of all requests that `use(r)` tells to take, eight of a thread in flight.
+template <typename Use, typename F>
+PMI_DEV void each_entry(const int32_t* tables, int64_t stride, const int32_t* kv_lens, int R, int width, int ps, int ring,
+                        Use use, F f) {
+  constexpr int kFly = 8;
+  const int n = R * width;
+  for (int u0 = threadIdx.x; u0 < n; u0 += kSmallThreads * kFly) {
+    int page[kFly], len[kFly];
+#pragma unroll
+    for (int k = 0; k < kFly; ++k) {
+      const int u = min(u0 + kSmallThreads * k, n - 1), r = u / width;
+      page[k] = tables[r * stride + u - r * width];
+      len[k] = use(r) ? kv_lens[r] : 0;
+    }
+#pragma unroll
+    for (int k = 0; k < kFly; ++k) {
+      const int u = u0 + kSmallThreads * k;
+      if (u >= n) break;
+      const int r = u / width, j = u - r * width;
+      if (j < held_pages(len[k], ps, width) && (unsigned)page[k] < (unsigned)ring) f(r, j, page[k]);
+    }
+  }
+}
+
+// Bits of pages, and how many are set before each word of them.
+struct PageBits {
+  uint32_t bit[kSmallPages / 32];
+  int before[kSmallPages / 32];
+  int waves[kSmallThreads / 64];
+  PMI_DEV bool has(int p) const { return bit[p >> 5] >> (p & 31) & 1; }
+  PMI_DEV int rank(int p) const { return before[p >> 5] + __popc(bit[p >> 5] & ((1u << (p & 31)) - 1)); }
+  // The bits are set (by all threads, before): the sums, and how many there are.
+  PMI_DEV int count() {
+    static_assert(kSmallPages / 32 <= kSmallThreads, "a word a thread");
+    const int tid = threadIdx.x;
+    __syncthreads();
+    const int mine = tid < kSmallPages / 32 ? __popc(bit[tid]) : 0;
+    int all;
+    const int upto = wg_sum_upto(mine, waves, all);
+    if (tid < kSmallPages / 32) before[tid] = upto - mine;
+    __syncthreads();
+    return all;
+  }
+};
+
+__global__ __launch_bounds__(kSmallThreads) void release_small_kernel(PagedRelease f) {
+  __shared__ PageBits left;
+  __shared__ uint32_t gone[kSmallPages];  // owners that a page loses
+  const int tid = threadIdx.x, R = (int)f.R, ring = (int)f.ring;
+  const int count = min(max(f.pool[1], 0), ring), head = f.pool[0] >= 0 && f.pool[0] < ring ? f.pool[0] : 0;
+  for (int p = tid; p < ring; p += kSmallThreads) gone[p] = 0;
+  if (tid < kSmallPages / 32) left.bit[tid] = 0;
+  __syncthreads();
+  each_entry(f.tables, f.stride, f.kv_lens, R, (int)f.width, (int)f.ps, ring, [&](int r) { return f.done[r] != 0; },
+             [&](int, int, int page) { atomicAdd(&gone[page], 1u); });
+  __syncthreads();
+  for (int p = tid; p < ring; p += kSmallThreads) {
+    if (!gone[p]) continue;
+    const int owners = f.shares[p] - (int)gone[p];
+    f.shares[p] = max(owners, 0);
+    if (owners < 0) atomicOr(&left.bit[p >> 5], 1u << (p & 31));
+  }
+  const int n = left.count();
+  for (int p = tid; p < ring; p += kSmallThreads) {
+    if (!left.has(p)) continue;
+    // (more than the ring has room for cannot be the pool's)
+    const int at = left.rank(p);
+    if (at < ring - count) f.free_pages[(head + count + at) % ring] = p;
+  }
+  if (tid == 0) f.pool[1] = min(count + n, ring);
+  for (int r = tid; r < R; r += kSmallThreads)
+    if (f.done[r]) f.kv_lens[r] = 0;
+}
+
+__global__ __launch_bounds__(kSmallThreads) void compact_small_kernel(PagedCompact f) {
+  __shared__ PageBits live;
+  __shared__ uint16_t hole[kSmallPages / 2];
+  const int tid = threadIdx.x, R = (int)f.R, ring = (int)f.ring, width = (int)f.width, ps = (int)f.ps;
+  const auto all_rows = [](int) { return true; };
+  if (tid < kSmallPages / 32) live.bit[tid] = 0;
+  __syncthreads();
+  each_entry(f.tables, f.stride, f.kv_lens, R, width, ps, ring, all_rows,
+             [&](int, int, int page) { atomicOr(&live.bit[page >> 5], 1u << (page & 31)); });
+  const int n = live.count();
+  const int below = n < kSmallPages ? live.rank(n) : n, movers = n - below;
+  for (int p = tid; p < ring; p += kSmallThreads) {
+    f.free_pages[p] = p + n < ring ? n + p : n + p - ring;
+    if (!live.has(p) && p < n) hole[p - live.rank(p)] = (uint16_t)p;
+  }
+  for (int i = movers + tid; i < ring / 2; i += kSmallThreads) f.src[i] = -1, f.dst[i] = -1;
+  __syncthreads();
+  for (int p = tid; p < ring; p += kSmallThreads) {
+    const bool there = live.has(p);
+    if (p < n) continue;  // stays, or is written for the page that moves there
+    if (there) {
+      const int i = live.rank(p) - below;
+      f.src[i] = p, f.dst[i] = hole[i];
+      if (f.shares) f.shares[hole[i]] = f.shares[p];
+    }
+    if (f.shares) f.shares[p] = 0;
+  }
+  each_entry(f.tables, f.stride, f.kv_lens, R, width, ps, ring, all_rows, [&](int r, int j, int page) {
+    if (page >= n) f.tables[r * f.stride + j] = hole[live.rank(page) - below];
+  });
+  if (tid == 0) {
+    f.moves[0] = movers;
+    f.pool[0] = 0;
+    f.pool[1] = ring - n;
+    f.pool[3] = 0;
+  }
+}
+
 // ---- pages given back by their last owner --------------------------------------------
 
 constexpr int kChunk = 4096;  // pages of a workgroup of 1024 threads
@@ -348,6 +467,7 @@ PMI_DEV RequestPages request_pages(const PagedRuns& f, int r) {
 __global__ __launch_bounds__(kRunThreads) void shared_runs_kernel(PagedRuns f) {
   __shared__ int waves[kRunThreads / 64];
   __shared__ int common_s[kTablesMaxRequests], run_s[kTablesMaxRequests], least_s[kTablesMaxRequests];
+  __shared__ int first_s[kTablesMaxRequests];
   __shared__ int s_last;
   const int tid = threadIdx.x, l = tid & 63, R = (int)f.R;
   const int r = blockIdx.x * (kRunThreads / 64) + (tid >> 6);
@@ -415,7 +535,7 @@ __global__ __launch_bounds__(kRunThreads) void shared_runs_kernel(PagedRuns f) {
     if (x < R) {
       common_s[x] = c, run_s[x] = run;
       least_s[x] = INT32_MAX;
-      if (begins) f.starts[run] = x;
+      if (begins) f.starts[run] = first_s[run] = x;
     }
   }
   __syncthreads();
@@ -427,6 +547,17 @@ __global__ __launch_bounds__(kRunThreads) void shared_runs_kernel(PagedRuns f) {
     f.lens[x] = pages == INT32_MAX ? 0 : pages * (int)f.ps;
   }
   for (int x = base + tid; x <= R; x += kRunThreads) f.starts[x] = R;
+  // what a run is as one request (base of them; the next one's first request ends it)
+  for (int x = tid; x < R; x += kRunThreads) {
+    int4 run = {0, 0, 0, 0};
+    const int pages = x < base ? least_s[x] : INT32_MAX;
+    if (pages != INT32_MAX) {
+      const int first = first_s[x], last = x + 1 < base ? first_s[x + 1] : R;
+      run = int4{first, f.q_starts ? f.q_starts[first] : first, 0, pages * (int)f.ps};
+      run.z = (f.q_starts ? f.q_starts[last] : last) - run.y;
+    }
+    reinterpret_cast<int4*>(f.runs)[x] = run;
+  }
   if (tid == 0) __hip_atomic_store(f.counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
@@ -445,17 +576,27 @@ hipError_t launch_fork_tables(const PagedFork& f, hipStream_t stream) {
 
 int64_t page_chunks(int64_t ring) { return (ring + kChunk - 1) / kChunk; }
 
+bool small(int64_t R, int64_t width, int64_t ring) { return ring <= kSmallPages && R * width <= kSmallEntries; }
+
 hipError_t launch_release_shared(const PagedRelease& f, hipStream_t stream) {
+  if (small(f.R, f.width, f.ring)) {
+    hipLaunchKernelGGL(release_small_kernel, dim3(1), dim3(kSmallThreads), 0, stream, f);
+    return hipGetLastError();
+  }
   if (f.width > 0)
     hipLaunchKernelGGL(leave_pages_kernel, dim3(row_pieces(f.width), (unsigned)f.R), dim3(256), 0, stream, f);
   const int chunks = (int)page_chunks(f.ring);
-  const bool alone = chunks <= 4;
+  const bool alone = chunks <= 4;  // (no count of them first)
   if (!alone) hipLaunchKernelGGL(count_left_kernel, dim3((unsigned)chunks), dim3(1024), 0, stream, f);
   hipLaunchKernelGGL(collect_left_kernel, dim3(alone ? 1u : (unsigned)chunks), dim3(1024), 0, stream, f, chunks);
   return hipGetLastError();
 }
 
 hipError_t launch_compact_tables(const PagedCompact& f, hipStream_t stream) {
+  if (small(f.R, f.width, f.ring)) {
+    hipLaunchKernelGGL(compact_small_kernel, dim3(1), dim3(kSmallThreads), 0, stream, f);
+    return hipGetLastError();
+  }
   const unsigned chunks = (unsigned)page_chunks(f.ring), pieces = row_pieces(f.width);
   hipLaunchKernelGGL(clear_live_kernel, dim3(chunks), dim3(256), 0, stream, f);
   if (f.R > 0 && pieces > 0)

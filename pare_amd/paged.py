@@ -62,12 +62,20 @@ class SharedPrefixes(NamedTuple):
 
     starts: torch.Tensor  # int32 [R + 1] the first request of each run, R behind the last
     lens: torch.Tensor    # int32 [R] positions that the members of a request's run share
+    runs: torch.Tensor    # int32 [R, 4] first request, first query, queries and positions shared of each, or zeros
 
 
 def _hip(t: torch.Tensor, fn: str) -> torch.device:
     if not t.is_cuda:
         raise RuntimeError(f"{fn} requires HIP (cuda) tensors.")
     return t.device
+
+
+def _here() -> tuple[int, int]:
+    """The current device and its stream, for the calls of the host extension: it takes plain calls on
+    that device, and leaves all others to the path behind it."""
+    here = torch._C._cuda_getDevice()
+    return here, torch._C._cuda_getCurrentRawStream(here)
 
 
 def _ints(dev: torch.device, n: int | None = None, **tensors: torch.Tensor) -> None:
@@ -163,6 +171,9 @@ def release_block_tables(block_tables: torch.Tensor, kv_lens: torch.Tensor, done
     [pages]) a page loses an owner for each of them, and goes back when it has none left,
     in the order of the pages' numbers."""
     dev = _hip(block_tables, "release_block_tables")
+    if shares is not None and _lib.host().release_tables(block_tables, kv_lens, done, free_pages, pool, shares,
+                                                         page_size, *_here()):
+        return
     R = block_tables.shape[0]
     _tables(block_tables, dev, R)
     _ints(dev, R, kv_lens=kv_lens)
@@ -203,6 +214,11 @@ def fork_block_tables(block_tables: torch.Tensor, kv_lens: torch.Tensor, parents
     before the call. Refused, and counted in ``pool[2]``, is a request that holds tokens, or that
     needs a page when the needs up to it exceed the pool."""
     dev = _hip(block_tables, "fork_block_tables")
+    here, stream = _here()
+    moves = _lib.host().fork_tables(block_tables, kv_lens, parents, free_pages, pool, shares, lengths, page_size, here,
+                                    stream)
+    if moves is not None:
+        return PageMoves(*moves, None)
     R, width = block_tables.shape[0], block_tables.shape[1] if block_tables.dim() == 2 else 0
     _tables(block_tables, dev, R)
     _ints(dev, R, kv_lens=kv_lens, parents=parents)
@@ -230,6 +246,9 @@ def compact_block_tables(block_tables: torch.Tensor, kv_lens: torch.Tensor, free
     says) are for ``copy_kv_pages``, on the same stream. ``shares``: as in ``fork_block_tables``, or
     None."""
     dev = _hip(block_tables, "compact_block_tables")
+    moves = _lib.host().compact_tables(block_tables, kv_lens, free_pages, pool, shares, page_size, *_here())
+    if moves is not None:
+        return PageMoves(*moves)
     R, width = block_tables.shape[0], block_tables.shape[1] if block_tables.dim() == 2 else 0
     _tables(block_tables, dev, R)
     _ints(dev, R, kv_lens=kv_lens)
@@ -261,9 +280,7 @@ def copy_kv_pages(moves: PageMoves, k_caches: Sequence[torch.Tensor] | torch.Ten
     launch per 64 layers. Pairs with a page that the cache does not have are left out; no page may be
     copied to twice, or be copied from and to."""
     _hip(moves.src, "copy_kv_pages")
-    dev = torch._C._cuda_getDevice()
-    if _lib.host().copy_pages(*moves, k_caches, v_caches, k_scales, v_scales, dev,
-                              torch._C._cuda_getCurrentRawStream(dev)):
+    if _lib.host().copy_pages(*moves, k_caches, v_caches, k_scales, v_scales, *_here()):
         return
     k_caches, v_caches, k_scales, v_scales = (list(t) for t in (k_caches, v_caches, k_scales, v_scales))
     n = len(k_caches)
@@ -297,13 +314,18 @@ def shared_prefixes(block_tables: torch.Tensor, kv_lens: torch.Tensor, q_starts:
     ``least`` positions of theirs, in whole pages before their new tokens, lie in the same pages;
     the members of a run share what all of them have in common."""
     dev = _hip(block_tables, "shared_prefixes")
+    here, stream = _here()
+    runs = _lib.host().shared_prefixes(block_tables, kv_lens, q_starts, page_size, -(-least // max(page_size, 1)), here,
+                                       stream, lambda nbytes: _workspace(dev, stream, nbytes))
+    if runs is not None:
+        return SharedPrefixes(*runs)
     R, width = block_tables.shape[0], block_tables.shape[1] if block_tables.dim() == 2 else 0
     _tables(block_tables, dev, R)
     _ints(dev, R, kv_lens=kv_lens)
     if q_starts is not None:
         _ints(dev, R + 1, q_starts=q_starts)
     assert least >= 1, "least must be at least one position"
-    starts, lens = torch.empty(2 * R + 1, dtype=torch.int32, device=dev).split([R + 1, R])
+    runs, starts, lens = torch.empty(6 * R + 1, dtype=torch.int32, device=dev).split([4 * R, R + 1, R])
     L = _lib.lib()
     with _DeviceGuard(dev):
         stream = _raw_stream(dev)
@@ -312,10 +334,10 @@ def shared_prefixes(block_tables: torch.Tensor, kv_lens: torch.Tensor, q_starts:
         ws = _workspace(dev, stream, L.pmi_shared_prefixes_workspace_bytes(R))
         _lib.check(L.pmi_shared_prefixes(
             block_tables.data_ptr(), _row_stride(block_tables), kv_lens.data_ptr(),
-            q_starts.data_ptr() if q_starts is not None else None, starts.data_ptr(), lens.data_ptr(), R, width,
-            page_size, -(-least // max(page_size, 1)), ws.data_ptr() if ws is not None else None,
+            q_starts.data_ptr() if q_starts is not None else None, starts.data_ptr(), lens.data_ptr(),
+            runs.data_ptr(), R, width, page_size, -(-least // max(page_size, 1)), ws.data_ptr() if ws is not None else None,
             ws.numel() if ws is not None else 0, stream), "pmi_shared_prefixes")
-    return SharedPrefixes(starts, lens)
+    return SharedPrefixes(starts, lens, runs.view(R, 4))
 
 
 def rope_append_kv(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, positions: torch.Tensor,
@@ -391,8 +413,9 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     ``scale`` multiplies q . k.
 
     ``shared``: what ``shared_prefixes`` says of the same tables, lengths and queries. The result
-    is the same but for roundings; keys that a run of requests shares are read once for all of it,
-    where no request has more than 64 query rows (``max_q_len`` H / KV) and there is no window."""
+    is the same but for roundings; keys that a run of requests shares are read once for all of it
+    where that pays: from 2048 keys (``max_kv_len``) and 2^27 bytes of all requests' keys and values on, up
+    to 32 query rows a request (``max_q_len`` H / KV), without a window."""
     dev = _hip(q, "paged_attention")
     pages, KV, ps, D, code = _cache(dev, k_cache, v_cache, k_scale, v_scale)
     assert q.dim() == 3 and q.shape[2] == D and q.dtype in (torch.float16, torch.bfloat16), (
@@ -421,8 +444,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     assert max_kv >= 0, "max_kv_len may not be negative"
     L = _lib.lib()
     if shared is not None:
-        _ints(dev, R + 1, starts=shared.starts)
         _ints(dev, R, lens=shared.lens)
+        _ints(dev, 4 * R, runs=shared.runs.reshape(-1))
         with _DeviceGuard(dev):
             stream = _raw_stream(dev)
             ws = _workspace(dev, stream, L.pmi_paged_attention_shared_workspace_bytes(T, R, H, KV, D, max_q, max_kv,
@@ -431,7 +454,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
                 q.data_ptr(), _VALUES[q.dtype], q.stride(0), q.stride(1), k_cache.data_ptr(), v_cache.data_ptr(),
                 k_scale.data_ptr(), v_scale.data_ptr(), code, pages, ps, block_tables.data_ptr(),
                 _row_stride(block_tables), kv_lens.data_ptr(), q_starts.data_ptr() if q_starts is not None else None,
-                shared.starts.data_ptr(), shared.lens.data_ptr(), out.data_ptr(), T, R, width, H, KV, D, max_q,
+                shared.runs.data_ptr(), shared.lens.data_ptr(), out.data_ptr(), T, R, width, H, KV, D, max_q,
                 max_kv, window, scale, ws.data_ptr() if ws is not None else None,
                 ws.numel() if ws is not None else 0, stream), "pmi_paged_attention_shared")
         return out

@@ -42,7 +42,7 @@ def test_oracle_by_hand():
     assert tables[2:] == [[0, 2, 1], [3, -1, -1]] and free[:3] == [4, 5, 6] and pool == [0, 6, 1, 0]
     assert (src, dst) == ([4, 7, -1, -1, -1], [0, 3, -1, -1, -1])
     assert O.runs([[1, 2, 3], [1, 2, 4], [1, 2, 3], [5, 2, 3]], [48, 48, 0, 33], None, 16, 32) == \
-        ([0, 3, 4, 4, 4], [32, 32, 0, 0])
+        ([0, 3, 4, 4, 4], [32, 32, 0, 0], [[0, 0, 3, 32]] + [[0] * 4] * 3)
 
 
 def _fork_args(**kw):
@@ -74,7 +74,7 @@ def _copy_args(layers=2, **kw):
 
 
 def _runs_args(**kw):
-    a = dict(t=P8, stride=4, lens=P8, starts=P8, out=P8, shared=P8, R=2, width=4, ps=16, least=1, ws=P8, nbytes=1 << 20)
+    a = dict(t=P8, stride=4, lens=P8, starts=P8, out=P8, shared=P8, runs=P8, R=2, width=4, ps=16, least=1, ws=P8, nbytes=1 << 20)
     a.update(kw)
     return [*a.values(), None]
 
@@ -111,7 +111,7 @@ def test_copy_refuses(change):
 
 
 @pytest.mark.parametrize("change", SIZES + [dict(t=None), dict(lens=None), dict(out=None), dict(shared=None),
-                                            dict(least=0), dict(least=1 << 31), dict(ws=None), dict(ws=P8 + 16),
+                                            dict(runs=None), dict(runs=P8 + 4), dict(least=0), dict(least=1 << 31), dict(ws=None), dict(ws=P8 + 16),
                                             dict(nbytes=100)])
 def test_shared_prefixes_refuses(change):
     assert _lib.lib().pmi_shared_prefixes(*_runs_args(**change)) in BAD
@@ -125,7 +125,7 @@ def _attention_args(**kw):
     return [*a.values(), None]
 
 
-@pytest.mark.parametrize("change", [dict(runs=None), dict(shared=None), dict(dtype=_lib.PMI_F32), dict(D=80), dict(ps=48),
+@pytest.mark.parametrize("change", [dict(runs=None), dict(runs=P8 + 8), dict(shared=None), dict(dtype=_lib.PMI_F32), dict(D=80), dict(ps=48),
                                     dict(H=65), dict(scale=float("nan")), dict(ws=None), dict(ws_bytes=1 << 16),
                                     dict(ws=P8 + 16), dict(lens=None), dict(tables=None), dict(max_q=-1),
                                     dict(T=1 << 25, max_q=64, H=64, KV=64, R=1 << 25, starts=None)])
@@ -242,7 +242,8 @@ def test_fork_of_strange_states():
 @gpu
 @pytest.mark.parametrize("R,ps,longest,parents,children,spare", [(1, 16, 40, 1, 0, 0), (9, 16, 200, 2, 7, 3),
                                                                  (60, 32, 3000, 10, 50, 20), (300, 16, 3000, 40, 200, 9000),
-                                                                 (4096, 16, 100, 2000, 2096, 5)])
+                                                                 (4096, 16, 100, 2000, 2096, 5), (6, 16, 200, 3, 3, 16330),
+                                                                 (6, 16, 200, 3, 3, 16400)])
 def test_release_of_shared_pages(R, ps, longest, parents, children, spare):
     rng = random.Random(R)
     for share in (0.3, 1.0, 0.0):
@@ -262,6 +263,7 @@ def test_release_of_shared_pages(R, ps, longest, parents, children, spare):
 @pytest.mark.parametrize("R,ps,longest,parents,children,spare", [(1, 16, 40, 1, 0, 0), (9, 16, 200, 2, 7, 3),
                                                                  (60, 32, 3000, 10, 50, 900), (300, 16, 3000, 40, 200, 9000),
                                                                  (4096, 16, 100, 2000, 2096, 5), (3, 16, 20, 0, 0, 5000),
+                                                                 (6, 16, 200, 3, 3, 16330), (6, 16, 200, 3, 3, 16400),
                                                                  (2, 256, 100, 1, 0, 0)])
 @pytest.mark.parametrize("shared", [True, False])
 def test_compact(R, ps, longest, parents, children, spare, shared):
@@ -352,7 +354,7 @@ def test_shared_prefixes(R, ps, longest, least):
         starts = None if mode in (0, 2) else np.concatenate([[0], np.cumsum(new)]).tolist()
         got = P.shared_prefixes(_ints(tables).view(R, width), _ints(lens), _ints(starts) if starts else None, ps, least=least)
         want = O.runs(tables, lens, starts, ps, least)
-        assert got.starts.tolist() == want[0] and got.lens.tolist() == want[1]
+        assert got.starts.tolist() == want[0] and got.lens.tolist() == want[1] and got.runs.tolist() == want[2]
     none = P.shared_prefixes(_ints([[1]]).view(1, 1)[:0], _ints([1])[:0], None, 16)
     assert none.starts.tolist() == [0] and none.lens.numel() == 0
 
@@ -362,8 +364,9 @@ def test_shared_prefixes(R, ps, longest, least):
 HALF = {torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}
 
 
-def _case(code, dtype, H, KV, D, ps, runs, seed=0, extra=2):
-    """runs: per run (shared tokens in whole pages, [(tokens behind, new tokens), ..])."""
+def _case(code, dtype, H, KV, D, ps, runs, seed=0, extra=2, share=True):
+    """runs: per run (shared tokens in whole pages, [(tokens behind, new tokens), ..]). The tables are as wide as
+    it takes for the call to read shared pages once (by its bounds: 2048 keys, 2^27 bytes of all requests)."""
     rng = np.random.default_rng(seed)
     lens, new, rows, at = [], [], [], 0
     for pages, members in runs:
@@ -378,7 +381,9 @@ def _case(code, dtype, H, KV, D, ps, runs, seed=0, extra=2):
     c = S.Cache(at + 3, KV, ps, D, code)
     c.fill(rng)
     name = rng.permutation(at + 3)
-    tables = rng.integers(0, at + 3, (len(lens), max(map(len, rows)) + extra)).astype(np.int32)
+    wide = -(-max(2048, (1 << 27) // (len(lens) * KV * 2 * D) + 1) // ps) if share else 0
+    width = max(max(map(len, rows)) + extra, wide)
+    tables = rng.integers(0, at + 3, (len(lens), width)).astype(np.int32)
     for r, row in enumerate(rows):
         tables[r, :len(row)] = name[row]
     starts = np.concatenate([[0], np.cumsum(new)]).astype(np.int32)
@@ -433,7 +438,9 @@ def test_single_tokens_of_shared_pages(code, dtype, H, KV, D, ps):
 
 @gpu
 @pytest.mark.parametrize("H,KV,D,ps,shared,members", [(32, 8, 128, 64, 70, 40), (28, 4, 128, 128, 9, 70),
-                                                      (16, 2, 64, 16, 500, 33), (4, 4, 64, 16, 129, 300)])
+                                                      (16, 2, 64, 16, 500, 33), (4, 4, 64, 16, 129, 300),
+                                                      (8, 2, 128, 64, 41, 11), (32, 2, 64, 16, 300, 3),
+                                                      (8, 2, 128, 64, 33, 4)])
 def test_long_prefixes_in_several_ranges(H, KV, D, ps, shared, members):
     code, dtype = (CODES[0], torch.float16) if H == 32 else (CODES[1], torch.bfloat16)
     case = _case(code, dtype, H, KV, D, ps, [(shared, [(i % 7 * 20, 1) for i in range(members)]), (3, [(9, 1), (0, 1)])])
@@ -482,16 +489,18 @@ def test_finished_requests_in_the_middle_and_rows_behind_the_last():
 
 
 @gpu
-@pytest.mark.parametrize("max_kv", [0, 5, 64, 100, 150, 152, 160, 170])
+@pytest.mark.parametrize("max_kv", [0, 5, 64, 150, 2048, 2099, 2304, 2310, 2400])
 def test_keys_past_the_bound_are_left_out(max_kv):
     """A bound inside of the shared pages, at their end and behind it."""
-    case = _case(CODES[0], torch.float16, 8, 2, 64, 16, [(9, [(i, 1) for i in range(30)])])
+    case = _case(CODES[0], torch.float16, 8, 8, 64, 256, [(9, [(i, 1) for i in range(65)])])
     _check(_run(case, max_kv_len=max_kv)[0], case, torch.float16, max_kv=max_kv)
 
 
 @gpu
 def test_calls_that_do_not_share():
-    """A window, requests of many rows, one request: the same values as without runs, bit for bit."""
+    """A window, requests of many rows, one request, few bytes: the same values as without runs, bit for bit."""
+    case = _case(CODES[0], torch.float16, 8, 1, 64, 16, [(9, [(3, 1), (5, 1), (0, 1)])], share=False)
+    assert torch.equal(_run(case)[0], _run(case, shared=None)[0])
     case = _case(CODES[0], torch.float16, 8, 1, 64, 16, [(9, [(3, 9), (5, 1), (0, 4)])])
     assert torch.equal(_run(case)[0], _run(case, shared=None)[0])       # 72 rows
     case = _case(CODES[0], torch.float16, 8, 1, 64, 16, [(9, [(3, 1), (5, 1), (0, 1)])])
@@ -511,21 +520,25 @@ def test_requests_that_share_nothing_are_as_without_runs():
 
 @gpu
 def test_runs_of_another_batch_stay_inside_the_buffers():
-    """Starts and lengths that no batch has lead nowhere else: what is read and written is this
+    """Runs and lengths that no batch has lead nowhere else: what is read and written is this
     call's (requests whose members' rows are right have right results)."""
     case = _case(CODES[0], torch.float16, 4, 2, 64, 16, [(9, [(3, 1), (20, 1)]), (0, [(50, 1)])])
-    good = P.SharedPrefixes(_ints([0, 2, 3, 3]), _ints([144, 144, 0]))
-    right = _run(case, shared=good)[0]
-    assert torch.equal(right, _run(case)[0])
-    for starts, lens in (([-5, 2, 3, 3], [0, 0, 0]), ([7, 9, -1, 2], [0, 0, 0]), ([3, 2, 1, 0], [0, 0, 0]),
-                         ([0, 2, 3, 3], [-8, -8, 1 << 30])):
-        out = torch.full((3, 4, 64), 7.0, dtype=torch.float16, device=DEV)
-        got = _run(case, shared=P.SharedPrefixes(_ints(starts), _ints(lens)), out=out)[0]
-        _check(got, case, torch.float16)
-    # positions that are said to be shared, of no run: those requests' rows mean nothing, the others' are right
-    for starts in ([3, 3, 3, 3], [2, 3, 3, 3], [0, 1, 3, 3], [1, 0, 9, 9]):
-        got = _run(case, shared=P.SharedPrefixes(_ints(starts), _ints([144, 144, 0])))[0]
-        assert torch.equal(got[2], right[2])
+    def runs(lens, *rows):
+        return P.SharedPrefixes(_ints([0] * 4), _ints(lens), _ints(list(rows) + [[0] * 4] * (3 - len(rows))))
+
+    right, found = _run(case)
+    assert found.runs.tolist() == [[0, 0, 2, 144], [0] * 4, [0] * 4]
+    assert torch.equal(_run(case, shared=runs([144, 144, 0], [0, 0, 2, 144]))[0], right)
+    big = (1 << 31) - 1
+    strange = ([-5, 0, 2, 144], [3, 0, 2, 144], [0, -1, 2, 144], [0, 0, 4, 144], [0, 3, 1, 144], [0, 1, big, 144],
+               [big, big, big, big], [0, 0, -2, 144], [0, 0, 2, -9], [2, 2, 1, big])
+    for lens in ([0, 0, 0], [-8, -8, 1 << 30]):
+        for row in strange:
+            out = torch.full((3, 4, 64), 7.0, dtype=torch.float16, device=DEV)
+            _check(_run(case, shared=runs(lens, row), out=out)[0], case, torch.float16)
+    # positions that are said to be shared, of no such run: those requests' rows mean nothing, the others' are right
+    for row in strange + ([2, 2, 1, 48], [1, 1, 1, 144]):
+        assert torch.equal(_run(case, shared=runs([144, 144, 0], row))[0][2], right[2])
 
 
 @gpu
@@ -608,7 +621,7 @@ def test_shared_attention_captured():
 
     def step():
         runs = P.shared_prefixes(t, n, None, 32, least=64)
-        return P.paged_attention(x, k, v, ks, vs, t, n, scale=0.1, max_kv_len=1000, shared=runs)
+        return P.paged_attention(x, k, v, ks, vs, t, n, scale=0.1, shared=runs)
 
     step()
     s = torch.cuda.Stream()
@@ -635,12 +648,13 @@ def test_shared_attention_captured():
 @gpu
 def test_python_checks():
     case = _case(CODES[0], torch.float16, 4, 2, 64, 16, [(9, [(3, 1), (20, 1)])])
-    for starts, lens in ((_ints([0, 2]), _ints([0, 0])), (_ints([0, 2, 2]), _ints([0])),
-                         (_ints([0, 2, 2]).long(), _ints([0, 0]))):
+    starts = _ints([0, 2, 2])
+    for lens, runs in ((_ints([0]), _ints([[0] * 4] * 2)), (_ints([0, 0]), _ints([[0] * 4])),
+                       (_ints([0, 0]), _ints([[0] * 4] * 2).long()), (_ints([0, 0]).long(), _ints([[0] * 4] * 2))):
         with pytest.raises(AssertionError):
-            _run(case, shared=P.SharedPrefixes(starts, lens))
+            _run(case, shared=P.SharedPrefixes(starts, lens, runs))
     with pytest.raises(RuntimeError):
-        _run(case, shared=P.SharedPrefixes(_ints([0, 2, 2]).cpu(), _ints([0, 0])))
+        _run(case, shared=P.SharedPrefixes(starts, _ints([0, 0]), _ints([[0] * 4] * 2).cpu()))
     t = _ints([[1, 2], [3, 4]]).view(2, 2)
     two, four, free = _ints([0, 0]), _ints([0, 5, 0, 0]), _ints([0] * 5)
     for bad in (lambda: P.fork_block_tables(t, two, two.long(), free, four, free, 16),
