@@ -21,7 +21,7 @@ from .gptq import HessianAccumulator, gptq_quantize, quantize_linear_gptq
 from .int8 import Int8Linear, matmul_int8, matmul_w8a8, quantize_rows
 from .kernels import kernel_available, kernel_choice, matmul_w4a16, matmul_w4a16_bf16, triton_available
 from .linear import FusedQuantizedLinear, QuantizedLinear
-from .logits import greedy_tokens, process_logits
+from .logits import LogitRules, greedy_tokens, process_logits
 from .model_io import load_quantized, save_quantized
 from .pack import (dequantize_int4, perm_from_g_idx, perm_u16, repack_int4_for_kernel, sz_group_major,
                    tile_w4a16, tiled_supported, zeros_to_u8)
@@ -39,7 +39,7 @@ __all__ = [
     "load_quantized", "rtn_quantize", "save_quantized", "sz_group_major", "tile_w4a16",
     "BatchPlan", "Int8Linear", "PagedKVCache", "extend_block_tables", "matmul_int8", "matmul_w8a8",
     "paged_attention", "quantize_rows", "read_kv_pages", "release_block_tables", "rope_append_kv",
-    "PageMoves", "SharedPrefixes", "compact_block_tables", "copy_kv_pages", "fork_block_tables", "greedy_tokens",
+    "LogitRules", "PageMoves", "SharedPrefixes", "compact_block_tables", "copy_kv_pages", "fork_block_tables", "greedy_tokens",
     "process_logits", "shared_prefixes",
     "tiled_supported", "triton_available", "zeros_to_u8",
 ]

@@ -25,7 +25,9 @@ query decode attention and SiLU-gate multiply, one launch each. With
 
 ``generate_ragged`` serves prompts of different lengths together: one paged 8-bit
 cache (``PagedKVCache``) in place of the fixed-length fp16 one, the prompts as one
-ragged batch, finished requests' pages given back as they end. ``quantize_head``
+ragged batch, finished requests' pages given back as they end. Prompts with a common
+``prefix`` begin as forks of one request, whose pages they own together and attend to once for
+all; ``rules`` are penalties, biases and masks of the tokens to choose from. ``quantize_head``
 puts the output head, the step's largest product, on 8-bit integers as well.
 """
 
@@ -49,7 +51,8 @@ from .kernels import (_stream_handle, gate_up_silu_rows_supported, gate_up_silu_
 from .pack import sz_group_major, tile_w4a16
 from .int8 import Int8Linear
 from .linear import FusedQuantizedLinear, QuantizedLinear
-from .paged import BatchPlan, PagedKVCache
+from .logits import LogitRules, greedy_tokens
+from .paged import BatchPlan, PagedKVCache, SharedPrefixes
 from .quant import rtn_quantize
 
 
@@ -327,17 +330,18 @@ class DecoderLayer(nn.Module):
         return h, self._mlp(n2, B, T)
 
     def forward_paged(self, h, d, cos_t, sin_t, cache: PagedKVCache, layer: int, plan: BatchPlan,
-                      max_q_len: int, max_kv_len: int):
+                      max_q_len: int, max_kv_len: int, shared: SharedPrefixes | None = None):
         """The layer on the tokens of a ragged batch, h and d [1, T, hidden] as in
         ``forward_fused``: their keys and values go to layer ``layer`` of the paged
         cache, in the slots that ``plan`` gives them, and every token attends to its own
-        request's positions up to its own. Returns the new (h, d)."""
+        request's positions up to its own (those that ``shared`` says are shared, once for
+        all). Returns the new (h, d)."""
         cfg = self.cfg
         T = h.shape[1]
         qkv, h = self._norm_linear(self.qkv.fused, h, d, self.attn_norm.weight)
         q = cache.append(layer, qkv.reshape(T, -1), cos_t, sin_t, plan)
         a = cache.attend(layer, q, plan, scale=1.0 / math.sqrt(cfg.head_dim), max_q_len=max_q_len,
-                         max_kv_len=max_kv_len)
+                         max_kv_len=max_kv_len, shared=shared)
         o = self.o(a.reshape(1, T, cfg.hidden))
         if T > 1:
             return self._norm_mlp(h, o, 1, T)
@@ -557,10 +561,10 @@ class QuantizedDecoder(nn.Module):
                 for _ in range(cfg.layers)]
 
     def new_paged_cache(self, requests: int, max_len: int, *, page_size: int = 64, pages: int | None = None,
-                        dtype: torch.dtype = torch.int8) -> PagedKVCache:
+                        dtype: torch.dtype = torch.int8, sharing: bool = False) -> PagedKVCache:
         """The paged cache of all layers (``pare_amd.PagedKVCache``) for ``forward_paged``."""
         return PagedKVCache(self.cfg.layers, requests, max_len, self.cfg.kv_heads, self.cfg.head_dim,
-                            self.embed.device, page_size=page_size, pages=pages, dtype=dtype)
+                            self.embed.device, page_size=page_size, pages=pages, dtype=dtype, sharing=sharing)
 
     def forward_tokens(self, tokens, cos, sin, cache, pos, mask, causal: bool,
                        last_only: bool = False):
@@ -588,14 +592,19 @@ class QuantizedDecoder(nn.Module):
         return self._head(self.norm(x))
 
     def forward_paged(self, tokens: torch.Tensor, cos, sin, cache: PagedKVCache, plan: BatchPlan, *,
-                      max_q_len: int, max_kv_len: int) -> torch.Tensor:
+                      max_q_len: int, max_kv_len: int, shared: SharedPrefixes | None = None,
+                      head: bool = True) -> torch.Tensor | None:
         """Logits [R, vocab] of every request's last new token. ``tokens`` [T] are the new
         tokens of ``plan`` (``cache.extend``), request after request; no request has more
         than ``max_q_len`` of them or more than ``max_kv_len`` positions with them. The rows
-        of requests without new tokens, and of refused ones, mean nothing."""
+        of requests without new tokens, and of refused ones, mean nothing. ``shared``: what
+        ``cache.shared_prefixes`` says of the plan. Without ``head`` the cache is filled, and
+        nothing returned."""
         x, d = F.embedding(tokens, self.embed)[None], None
         for i, layer in enumerate(self.layers):
-            x, d = layer.forward_paged(x, d, cos, sin, cache, i, plan, max_q_len, max_kv_len)
+            x, d = layer.forward_paged(x, d, cos, sin, cache, i, plan, max_q_len, max_kv_len, shared)
+        if not head:
+            return None
         last = (plan.q_starts[1:] - 1).clamp_(min=0)
         n, _ = add_rmsnorm(x[0].index_select(0, last), d[0].index_select(0, last), self.norm.weight,
                            self.cfg.rms_eps)
@@ -603,27 +612,57 @@ class QuantizedDecoder(nn.Module):
 
     @torch.no_grad()
     def generate_ragged(self, prompts: list[torch.Tensor], n_generate: int, *, eos: int | None = None,
-                        dtype: torch.dtype = torch.int8, page_size: int = 64, use_graph: bool = True):
+                        dtype: torch.dtype = torch.int8, page_size: int = 64, use_graph: bool = True,
+                        prefix: torch.Tensor | None = None, rules: LogitRules | None = None):
         """Greedy decode of prompts of different lengths (1-D, none empty) together over a
         paged cache of ``dtype`` codes (int8 or float8_e4m3fn): (tokens
         [len(prompts), n_generate], timings). The prompts are prefilled as one ragged batch;
         a decode step is one graph replay (or the same ops eagerly). A request that has
         produced ``eos`` gives its pages back, takes no further part, and the rest of its
-        row is ``eos``."""
+        row is ``eos``.
+
+        ``prefix`` (1-D) stands before every prompt: it is prefilled once, and the requests
+        begin as forks of it. With ``rules`` (of one row a prompt) the tokens are those of
+        ``greedy_tokens``, each request's history its prefix, prompt and answer, of which only
+        the answer counts for presence and frequency."""
         if not prompts or any(p.dim() != 1 or p.numel() == 0 for p in prompts):
             raise ValueError("prompts must be 1-D tensors of at least one token")
         if n_generate < 1:
             raise ValueError("n_generate must be at least 1")
+        if prefix is not None and (prefix.dim() != 1 or prefix.numel() == 0):
+            raise ValueError("prefix must be a 1-D tensor of at least one token")
         dev, R = self.embed.device, len(prompts)
         lens = [p.numel() for p in prompts]
+        before = 0 if prefix is None else prefix.numel()
         longest, total = max(lens), sum(lens)
-        L = longest + n_generate
+        L = before + longest + n_generate
         cos, sin = self.rope_tables(L)
-        cache = self.new_paged_cache(R, L, page_size=page_size, dtype=dtype)
+        cache = self.new_paged_cache(R, L, page_size=page_size, dtype=dtype, sharing=prefix is not None)
         out = torch.empty(R, n_generate, dtype=torch.long, device=dev)
         tok = torch.zeros(R, 1, dtype=torch.long, device=dev)
         live = torch.ones(R, dtype=torch.int32, device=dev)
         packed = torch.zeros(R + 1, dtype=torch.long, device=dev)
+        if rules is not None:
+            whole = [p if prefix is None else torch.cat([prefix.to(p.device), p]) for p in prompts]
+            history = torch.zeros(R, L + 1, dtype=torch.int32, device=dev)
+            for r, p in enumerate(whole):
+                history[r, :p.numel()] = p.to(dev, torch.int32)
+            prompt_lens = torch.tensor([p.numel() for p in whole], dtype=torch.int32, device=dev)
+            history_lens = prompt_lens.clone()
+
+        def choose(logits):
+            """The next token of every request to ``tok``."""
+            if rules is None:
+                argmax_into(logits, tok)
+                return
+            greedy_tokens(logits, history=history, history_lens=history_lens, prompt_lens=prompt_lens, out=tok,
+                          **rules._asdict())
+            # (a finished request's length stays where it was)
+            history.scatter_(1, history_lens[:, None].long(), tok.to(torch.int32))
+            history_lens.add_(live)
+
+        def runs(plan):
+            return cache.shared_prefixes(plan) if prefix is not None else None
 
         def finish():
             """Takes the requests that have just produced eos out of the batch."""
@@ -638,8 +677,8 @@ class QuantizedDecoder(nn.Module):
                 # the live requests' tokens in front, where the plan looks for them
                 packed.scatter_(0, torch.where(live > 0, plan.q_starts[:-1], R).long(), inputs)
                 inputs = packed[:R]
-            logits = self.forward_paged(inputs, cos, sin, cache, plan, max_q_len=1, max_kv_len=L)
-            argmax_into(logits, tok)
+            logits = self.forward_paged(inputs, cos, sin, cache, plan, max_q_len=1, max_kv_len=L, shared=runs(plan))
+            choose(logits)
             if eos is not None:
                 tok.masked_fill_((live == 0)[:, None], eos)
                 finish()
@@ -657,14 +696,23 @@ class QuantizedDecoder(nn.Module):
             torch.cuda.current_stream(dev).wait_stream(s)
             cache.reset()
             live.fill_(1)
+            if rules is not None:
+                history_lens.copy_(prompt_lens)
         tokens = torch.cat([p.to(dev) for p in prompts])
         new_lens = torch.tensor(lens, dtype=torch.int32, device=dev)
+        first = torch.arange(R, dtype=torch.int32, device=dev)
         torch.cuda.synchronize(dev)
 
         t0 = time.perf_counter()
+        if prefix is not None:
+            # in request 0, of which all others are forks
+            plan = cache.extend((first == 0).int() * before, before)
+            self.forward_paged(prefix.to(dev), cos, sin, cache, plan, max_q_len=before, max_kv_len=before, head=False)
+            cache.fork(torch.zeros_like(first))
         plan = cache.extend(new_lens, total)
-        logits = self.forward_paged(tokens, cos, sin, cache, plan, max_q_len=longest, max_kv_len=longest)
-        argmax_into(logits, tok)
+        logits = self.forward_paged(tokens, cos, sin, cache, plan, max_q_len=longest, max_kv_len=before + longest,
+                                    shared=runs(plan))
+        choose(logits)
         if eos is not None:
             finish()
         out[:, 0] = tok[:, 0]

@@ -9,12 +9,26 @@ no counterpart: its decode is HuggingFace's greedy generate (pare/eval/throughpu
 
 from __future__ import annotations
 
+from typing import NamedTuple
+
 import torch
 
 from . import _lib
 from .kernels import _DeviceGuard, _raw_stream, _workspace
 
 _VALUES = {torch.float16: _lib.PMI_F16, torch.bfloat16: _lib.PMI_BF16, torch.float32: _lib.PMI_F32}
+
+
+class LogitRules(NamedTuple):
+    """What the rows of a batch have beside their histories, as ``process_logits`` takes it."""
+
+    repetition: torch.Tensor | None = None    # fp32 [R] each
+    presence: torch.Tensor | None = None
+    frequency: torch.Tensor | None = None
+    bias_ids: torch.Tensor | None = None      # int32 and fp32 [R, n]
+    bias: torch.Tensor | None = None
+    allowed: torch.Tensor | None = None       # int32 [masks, ceil(V / 32)]
+    allowed_rows: torch.Tensor | None = None  # int32 [R]
 
 
 def _tensor(name: str, t: torch.Tensor, dev: torch.device, dtype: torch.dtype, shape: tuple) -> None:
