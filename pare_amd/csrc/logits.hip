@@ -93,8 +93,7 @@ __global__ __launch_bounds__(F::kThreads) void logits_kernel(Logits f, T* out, i
     bits[k] = 0xffffffffu;
     if (mask && t + E > 0 && t < V) {  // bit e: token t + e (any for those that the row does not have)
       const int at = max(t, 0), word = at >> 5;
-      const uint64_t two = mask[word] | (uint64_t)mask[min(word + 1, (V - 1) >> 5)] << 32;
-      bits[k] = (uint32_t)(two >> (at & 31)) << (at - t);
+      bits[k] = __builtin_amdgcn_alignbit(mask[min(word + 1, (V - 1) >> 5)], mask[word], at & 31) << (at - t);
     }
   }
 
