@@ -1177,7 +1177,10 @@ __global__ __launch_bounds__(256) void join_parts_kernel(AttnArgs a) {
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
     if (first) o = *reinterpret_cast<const f32x4*>(own + dim);
     const int2 at = a.where[out_row];
-    const int apart = at.y & 1 ? kRows / 2 : kRows;
+    int apart = at.y & 1 ? kRows / 2 : kRows;
+    // (as a power of two the compiler would shift by it, 64 bits by an amount of a lane's own, which has given
+    // wrong lanes on this hardware)
+    asm("" : "+v"(apart));
     // (nobody wrote it if the runs are not this batch's)
     const bool there = at.x >= 0 && at.y >= 2 && (int64_t)at.x + (int64_t)apart * ((at.y >> 1) - 1) < a.part_records;
     const int n = there ? at.y >> 1 : 0;
