@@ -321,16 +321,19 @@ PMI_DEV void few_rows(const AttnArgs& a, FewLds<D>& lds, int wg) {
   const int requests = kOf * a.R;
   const int run = kOf * ((a.R + 63) >> 6), r_lane = run * l;
   int in_lane = 0, parts_lane[kCuts] = {};  // tiles, and parts of cut_of(k) tiles
+  auto count = [&](const Request& rq) {
+    const int nt = tiles_of(rq), items = items_of(rq);
+    in_lane += nt * items;
+#pragma unroll
+    for (int k = 0; k < kCuts; ++k) parts_lane[k] += (nt + cut_of(k) - 1) / cut_of(k) * items;
+  };
   for (int x = r_lane; x < min(requests, r_lane + run); x += kOf) {
-    Request rq[kOf];
-#pragma unroll
-    for (int i = 0; i < kOf; ++i) rq[i] = request<MODE>(a, x + i);
-#pragma unroll
-    for (int i = 0; i < kOf; ++i) {
-      const int nt = tiles_of(rq[i]), items = items_of(rq[i]);
-      in_lane += nt * items;
-#pragma unroll
-      for (int k = 0; k < kCuts; ++k) parts_lane[k] += (nt + cut_of(k) - 1) / cut_of(k) * items;
+    if constexpr (MODE == kWhole) {
+      count(request<MODE>(a, x));
+    } else {
+      const Request own = request<MODE>(a, x), of_run = request<MODE>(a, x + 1);  // (their loads together)
+      count(own);
+      count(of_run);
     }
   }
   auto scan = [&](int v) {
@@ -754,6 +757,8 @@ PMI_DEV void many_rows(const AttnArgs& a, uint8_t* lds, int& s_last, int wg) {
     return rq.n * G > (MODE == kWhole ? a.few_rows : a.run_rows) ? (rq.n * G + kRows - 1) / kRows : 0;
   };
   const int kh = wg % a.KV, rest = wg / a.KV;
+  int splits = a.splits, sp = 0, index = 0;
+  if constexpr (MODE == kWhole) sp = rest % splits, index = rest / splits;
   const int run = (a.R + 63) >> 6, r_lane = run * l;
   int in_lane = 0;
   for (int x = r_lane; x < min(a.R, r_lane + run); ++x) in_lane += tiles_of(x);
@@ -764,10 +769,11 @@ PMI_DEV void many_rows(const AttnArgs& a, uint8_t* lds, int& s_last, int wg) {
     if (l >= o) upto += u;
   }
   const int all_tiles = __builtin_amdgcn_readlane(upto, 63);
-  // (the host does not know how many runs there are, nor what they share)
-  int splits = a.splits;
-  if constexpr (MODE == kParts) splits = all_tiles > 0 ? max(1, a.many_wgs / (all_tiles * a.KV)) : 1;
-  const int sp = rest % splits, index = rest / splits;
+  if constexpr (MODE == kParts) {
+    // (the host does not know how many runs there are, nor what they share)
+    splits = all_tiles > 0 ? max(1, a.many_wgs / (all_tiles * a.KV)) : 1;
+    sp = rest % splits, index = rest / splits;
+  }
   if (index >= all_tiles) return;
   const int lane0 = __builtin_ctzll(__ballot(upto > index));
   int r = run * lane0;
