@@ -1507,7 +1507,11 @@ size_t attention_ws_bytes(int64_t T, int64_t R, int64_t H, int64_t KV, int64_t D
   p.max_kv = max_kv < pmi::kPagedMaxKeys ? max_kv : pmi::kPagedMaxKeys;
   pmi::PagedCache c = {};
   c.KV = KV, c.D = D;
-  return runs && pmi::paged_attention_shares(p, c) ? pmi::paged_shared_ws_bytes(p, c) : pmi::paged_attention_ws_bytes(p, c);
+  // (with runs: of either way, as the table's width has a say in which it is)
+  const size_t whole = pmi::paged_attention_ws_bytes(p, c);
+  if (!runs || !pmi::paged_attention_shares(p, c) || !pmi::paged_shared_launch_fits(p, c)) return whole;
+  const size_t parts = pmi::paged_shared_ws_bytes(p, c);
+  return parts > whole ? parts : whole;
 }
 
 }  // namespace
@@ -1559,12 +1563,13 @@ int paged_attention(const char* fn, const int32_t* runs, const int32_t* run_lens
                              const_cast<float*>(v_scale), n_pages, KV, page_size, D, code_dtype == PMI_F8};
   // (not cut to the table's width: the ranges of keys have to be those that the workspace was asked for)
   if (p.max_kv > pmi::kPagedMaxKeys) p.max_kv = pmi::kPagedMaxKeys;
-  const bool shares = runs && pmi::paged_attention_shares(p, c);
-  if (!(shares ? pmi::paged_shared_launch_fits(p, c) : pmi::paged_attention_launch_fits(p, c)))
+  pmi::PagedAttention with_runs = p;  // (a run is one more request, with the queries of all its members)
+  with_runs.max_q = T, with_runs.R = 2 * R;
+  const bool shares = runs && pmi::paged_attention_shares(p, c) && pmi::paged_shared_launch_fits(p, c) &&
+                      pmi::paged_attention_tiles_fit(with_runs, c);
+  if (!shares && !pmi::paged_attention_launch_fits(p, c))
     return fail(PMI_ERR_UNSUPPORTED, "%s: too many query rows for one launch (T H)", fn);
-  pmi::PagedAttention whole = p;  // (a run is one more request, with the queries of all its members)
-  if (shares) whole.max_q = T, whole.R = 2 * R;
-  if (!pmi::paged_attention_tiles_fit(whole, c))
+  if (!shares && !pmi::paged_attention_tiles_fit(p, c))
     return fail(PMI_ERR_UNSUPPORTED, "%s: too many tiles of 64 keys for 32 bits (R KV max_kv): give a tighter max_kv "
                 "or fewer requests", fn);
   const size_t need = attention_ws_bytes(T, R, H, KV, D, max_q, p.max_kv, window, runs != nullptr);

@@ -38,12 +38,13 @@ struct AttnArgs {
   const int32_t* run_lens;  // [R] positions that a request shares
   int run_rows;       // runs of up to so many query rows are `few`
   int many_wgs;       // workgroups that the ranges of a run's keys are made for
-  // Parts of rows, D + 4 floats each (values, max, sum): of the ranges of runs of many rows, in
-  // tiles of kRows; of runs of few rows [T, H]; of the keys behind what is shared [T, H].
-  float *parts_many, *parts_few, *parts_own;
-  int2* where;        // [T, H] a row's first shared part (its offset from parts_many in records), and 2 n of n
-                      // parts that lie kRows records apart, 2 n + 1 of n that lie kRows / 2 apart
-  int part_records;   // that parts_many and parts_few hold
+  // Parts of rows, D + 4 floats each (values, max, sum): of several ranges of runs of many rows, in
+  // tiles of kRows; of runs in one range or of few rows [2, T, H] (the second for the second half of a
+  // tile's keys); of the keys behind what is shared [T, H].
+  float *parts_many, *parts_one, *parts_own;
+  int2* where;        // [T, H] a row's first shared part (its offset from parts_many in records), and 4 n + a
+                      // of n parts that lie kRows (a = 0), kRows / 2 (1) or T H records (2) apart
+  int part_records;   // that parts_many and parts_one hold
 };
 
 // What a launch computes: whole rows; or, where requests share their first pages, parts of
@@ -569,12 +570,12 @@ PMI_DEV void few_rows(const AttnArgs& a, FewLds<D>& lds, int wg) {
   // a row that is a part: its values from dimension d on
   const bool is_part = MODE == kParts && (rq.run || first_seen > 0);
   auto keep_part = [&](int64_t at, int d, const auto& v, int n, float m, float l) {
-    float* rec = (rq.run ? a.parts_few : a.parts_own) + at * (D + 4);
+    float* rec = (rq.run ? a.parts_one : a.parts_own) + at * (D + 4);
 #pragma unroll
     for (int x = 0; x < n; x += 4) *reinterpret_cast<f32x4*>(rec + d + x) = f32x4{v[x], v[x + 1], v[x + 2], v[x + 3]};
     if (d == 0) {
       *reinterpret_cast<float2*>(rec + D) = float2{m, l};
-      if (rq.run) a.where[at] = int2{(int)((a.parts_few - a.parts_many) / (D + 4) + at), 2};
+      if (rq.run) a.where[at] = int2{(int)((a.parts_one - a.parts_many) / (D + 4) + at), 4};
     }
   };
   auto store = [&]() {
@@ -1037,8 +1038,9 @@ PMI_DEV void many_tile(const AttnArgs& a, uint8_t* lds, int& s_last, const Reque
   const int64_t out_row = (int64_t)(start + i) * a.H + kh * G + row - i * G;
   T* dst = (T*)a.out + out_row * D + 4 * h;
   if constexpr (MODE == kParts) {
-    const int64_t at = ((int64_t)(index * a.KV + kh) * splits + sp) * kRows + wave * 32 + c;
     static_assert(HALVES <= 2, "the second half's records lie behind the first's");
+    const int64_t in_one = (a.parts_one - a.parts_many) / (D + 4) + (int64_t)half * a.T * a.H + out_row;
+    const int64_t at = splits == 1 ? in_one : ((int64_t)(index * a.KV + kh) * splits + sp) * kRows + wave * 32 + c;
     float* rec = a.parts_many + at * (D + 4);
 #pragma unroll
     for (int d = 0; d < D / 32; ++d)
@@ -1050,7 +1052,8 @@ PMI_DEV void many_tile(const AttnArgs& a, uint8_t* lds, int& s_last, const Reque
         if (live) *reinterpret_cast<f32x4*>(rec + 32 * d + 8 * j + 4 * h) = y;
       }
     if (live && h == 0) *reinterpret_cast<float2*>(rec + D) = float2{ref.max, sum};
-    if (live && h == 0 && sp == 0 && half == 0) a.where[out_row] = int2{(int)at, 2 * HALVES * parts + HALVES - 1};
+    if (live && h == 0 && sp == 0 && half == 0)
+      a.where[out_row] = int2{(int)at, 4 * HALVES * parts + (splits == 1 ? 2 : HALVES - 1)};
     return;
   }
   if (parts == 1) {
@@ -1183,13 +1186,13 @@ __global__ __launch_bounds__(256) void join_parts_kernel(AttnArgs a) {
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
     if (first) o = *reinterpret_cast<const f32x4*>(own + dim);
     const int2 at = a.where[out_row];
-    int apart = at.y & 1 ? kRows / 2 : kRows;
+    int apart = at.y & 2 ? a.T * a.H : at.y & 1 ? kRows / 2 : kRows;
     // (as a power of two the compiler would shift by it, 64 bits by an amount of a lane's own, which has given
     // wrong lanes on this hardware)
     asm("" : "+v"(apart));
     // (nobody wrote it if the runs are not this batch's)
-    const bool there = at.x >= 0 && at.y >= 2 && (int64_t)at.x + (int64_t)apart * ((at.y >> 1) - 1) < a.part_records;
-    const int n = there ? at.y >> 1 : 0;
+    const bool there = at.x >= 0 && at.y >= 4 && (int64_t)at.x + (int64_t)apart * ((at.y >> 2) - 1) < a.part_records;
+    const int n = there ? at.y >> 2 : 0;
     const float* rec = a.parts_many + (int64_t)at.x * (D + 4);
     for (int s0 = group; s0 < n; s0 += kFly * kGroups) {
       float2 ml[kFly];
@@ -1327,6 +1330,10 @@ int64_t run_wgs(const PagedAttention& p, const PagedCache& c) {
   const int64_t items = run_items(p, c), held = 2 * device_cu_count();
   return items == 0 ? 0 : items > held ? items : held;
 }
+// Records of their ranges: those are several only where all ranges together are as many as the CUs hold.
+int64_t run_records(const PagedAttention& p, const PagedCache& c) {
+  return run_items(p, c) ? (int64_t)2 * device_cu_count() * kRows : 0;
+}
 size_t part_bytes(int64_t rows, int64_t D) { return (size_t)(rows * (D + 4) * 4); }
 
 }  // namespace
@@ -1351,22 +1358,22 @@ bool paged_attention_shares(const PagedAttention& p, const PagedCache& c) {
 bool paged_shared_launch_fits(const PagedAttention& p, const PagedCache& c) {
   // (parts are counted in 32 bits, and requests and runs together)
   return few_wgs(c.D) + run_wgs(p, c) < (1ll << 23) && p.R < (1ll << 29) && p.R * c.KV < (1ll << 21) &&
-         run_wgs(p, c) * kRows + 2 * p.T * p.H < (1ll << 31);
+         run_records(p, c) + 3 * p.T * p.H < (1ll << 31);
 }
 
 size_t paged_shared_ws_bytes(const PagedAttention& p, const PagedCache& c) {
-  return kWsCounterBytes + few_part_bytes(c.D) + part_bytes(run_wgs(p, c) * kRows + 2 * p.T * p.H, c.D) +
+  return kWsCounterBytes + few_part_bytes(c.D) + part_bytes(run_records(p, c) + 3 * p.T * p.H, c.D) +
          (size_t)(p.T * p.H * 8);
 }
 
 hipError_t launch_paged_shared(const PagedAttention& p, const PagedCache& c, void* workspace, hipStream_t stream) {
   AttnArgs a = attention_args(p, c, workspace);
-  const int64_t wgs = run_wgs(p, c), rows = p.T * p.H;
+  const int64_t wgs = run_wgs(p, c), rows = p.T * p.H, records = run_records(p, c);
   a.parts_many = a.many_part;
-  a.parts_few = a.parts_many + wgs * kRows * (c.D + 4);
-  a.parts_own = a.parts_few + rows * (c.D + 4);
+  a.parts_one = a.parts_many + records * (c.D + 4);
+  a.parts_own = a.parts_one + 2 * rows * (c.D + 4);
   a.where = (int2*)(a.parts_own + rows * (c.D + 4));
-  a.part_records = (int)(wgs * kRows + rows);
+  a.part_records = (int)(records + 2 * rows);
   a.run_rows = kRunRows;
   a.many_wgs = 2 * device_cu_count();
   if (hipError_t e = launch_mode<kParts>(a, p, c, wgs ? a.few_wgs + wgs : 0, stream); e != hipSuccess) return e;

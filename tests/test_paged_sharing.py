@@ -612,6 +612,67 @@ def test_many_requests_and_runs():
 
 
 @gpu
+@pytest.mark.parametrize("H,KV,D,runs,members", [(8, 8, 64, 40, 20), (16, 8, 64, 35, 35), (16, 16, 128, 20, 20)])
+def test_more_runs_than_workgroups(H, KV, D, runs, members):
+    """Runs that fill the CUs unsplit, of up to 64 rows and of more: one part a row, or one a half."""
+    rng = random.Random(runs)
+    case = _case(CODES[0], torch.float16, H, KV, D, 16, [(rng.randint(2, 9), [(rng.randint(0, 20), 1) for _ in range(members)])
+                                                        for _ in range(runs)])
+    got, found = _run(case)
+    assert found.starts.tolist()[:runs + 1] == [members * i for i in range(runs + 1)]
+    c, tables, lens, _, q = case
+    few = sorted(rng.sample(range(len(lens)), 60))
+    _check(got[few], (c, tables[few], [lens[i] for i in few], np.arange(61).astype(np.int32), q[few]), torch.float16)
+    plain = _run(case, shared=None)[0]
+    weight = np.abs(c.values(1)).max()
+    err = (got.double() - plain.double()).abs().cpu().numpy()
+    tol = 2 * HALF[torch.float16] * np.abs(plain.double().cpu().numpy()) + 2 * (2.0 ** -11 + 2.0 ** -12) * weight
+    assert (err <= tol).all() and not torch.equal(got, plain)
+
+
+@gpu
+def test_more_than_the_parts_hold_is_done_without_them():
+    """A call of too many requests x KV heads for parts: as without runs, not refused."""
+    L = _lib.lib()
+    R, KV = 1 << 18, 16
+    args = (R, R, KV, KV, 64, 1, 4096, 0)
+    assert L.pmi_paged_attention_shared_workspace_bytes(*args) == L.pmi_paged_attention_workspace_bytes(*args)
+    assert L.pmi_paged_attention_shared_workspace_bytes(64, 64, 32, 8, 128, 1, 8192, 0) > \
+        L.pmi_paged_attention_workspace_bytes(64, 64, 32, 8, 128, 1, 8192, 0)
+
+
+@gpu
+def test_pages_past_32_bits_of_bytes():
+    """Copies, and shared pages, whose offsets pass 2^32 bytes."""
+    pages, KV, ps, D = 17000, 8, 256, 128
+    k = torch.zeros(pages, KV, ps, D, dtype=torch.int8, device=DEV)
+    v = torch.zeros(pages, KV, ps // 16, D, 16, dtype=torch.int8, device=DEV)
+    ks, vs = torch.full((pages, KV), 0.01, device=DEV), torch.full((pages, KV), 0.01, device=DEV)
+    g = torch.Generator(device=DEV).manual_seed(0)
+    top = pages - 1
+    for t in (k, v):
+        t[top - 8:] = torch.randint(-127, 128, t[top - 8:].shape, generator=g, device=DEV, dtype=torch.int8)
+    P.copy_kv_pages(P.PageMoves(_ints([top, top - 8]), _ints([3, 16500]), None), [k], [v], [ks], [vs])
+    for t in (k, v):
+        assert torch.equal(t[3], t[top]) and torch.equal(t[16500], t[top - 8]) and not t[2].any() and not t[4].any()
+    # 40 requests of eight pages at the end of the cache, and the same ones at its front
+    rows = torch.arange(top - 8, top, dtype=torch.int32, device=DEV)
+    wide = -(-max(2048, (1 << 27) // (40 * KV * 2 * D) + 1) // ps)
+    q = torch.randn(40, 16, D, generator=g, device=DEV).half()
+    out = []
+    for at in (rows, rows - (top - 8) + 8):
+        P.copy_kv_pages(P.PageMoves(rows, at.contiguous(), None), [k], [v], [ks], [vs])
+        tables = torch.zeros(40, max(wide, 9), dtype=torch.int32, device=DEV)
+        tables[:, :8] = at
+        tables[:, 8] = torch.arange(100, 140, device=DEV)
+        lens = torch.full((40,), 8 * ps + 5, dtype=torch.int32, device=DEV)
+        shared = P.shared_prefixes(tables, lens, None, ps)
+        assert shared.lens.tolist() == [8 * ps] * 40
+        out.append(P.paged_attention(q, k, v, ks, vs, tables, lens, scale=0.01, shared=shared))
+    assert torch.equal(*out) and out[0].any()
+
+
+@gpu
 def test_shared_attention_captured():
     """Lengths grow and a request ends between the replays; each equals the eager call."""
     case = _case(CODES[0], torch.float16, 8, 2, 128, 32, [(20, [(1, 1)] * 9), (3, [(0, 1)] * 2)], extra=6)
