@@ -323,6 +323,30 @@ def test_no_call_waits_for_the_device():
 
 
 @gpu
+def test_logits_past_2_31_values():
+    R, V = 16384, 140001
+    x = torch.zeros(R, V, dtype=torch.bfloat16, device=DEV)
+    at = torch.arange(R, device=DEV) * 7 % V
+    x[torch.arange(R, device=DEV), at] = 5
+    h = at.int()[:, None].contiguous()
+    assert torch.equal(P.greedy_tokens(x), at)
+    got = P.greedy_tokens(x, history=h, presence=torch.full((R,), 6.0, device=DEV))
+    assert torch.equal(got, (at == 0).long())
+    P.process_logits(x, history=h, presence=torch.full((R,), 6.0, device=DEV), out=x)
+    assert (x.gather(1, at[:, None]) == -1).all() and int((x != 0).sum()) == R
+
+
+@gpu
+def test_a_gradient_is_refused():
+    x = torch.zeros(2, 64, device=DEV, requires_grad=True)
+    with pytest.raises(RuntimeError, match="backward"):
+        P.process_logits(x)
+    with torch.no_grad():
+        assert not P.process_logits(x).requires_grad
+    assert P.greedy_tokens(x).tolist() == [0, 0]
+
+
+@gpu
 @pytest.mark.parametrize("rows", [1000, 16384])
 def test_many_rows(rows):
     x = torch.randn(rows, 4100, device=DEV)
