@@ -675,10 +675,13 @@ PMI_API size_t pmi_paged_attention_workspace_bytes(int64_t T, int64_t R, int64_t
                                                    int64_t D, int64_t max_q, int64_t max_kv,
                                                    int64_t window);
 
-/* pmi_paged_attention of requests of which some share their first pages: runs and run_lens are
- * what pmi_shared_prefixes gives as runs and lens for the same tables, lengths and queries. The result is the same but for roundings: a run's shared keys are read once for the queries of
- * all its members, where that pays by the bounds (no request of more than 32 query rows, max_q H / KV;
- * 2^27 bytes of keys and values of all requests, max_kv of at least 2048; no window). workspace: pmi_paged_attention_shared_workspace_bytes() bytes, otherwise as above. */
+/* pmi_paged_attention of requests of which some share their first pages: runs and
+ * run_lens are what pmi_shared_prefixes gives as runs and lens for the same tables,
+ * lengths and queries. The result is the same but for roundings: a run's shared keys
+ * are read once for the queries of all its members, where that pays by the bounds (no
+ * request of more than 32 query rows, max_q H / KV; 2^27 bytes of keys and values of
+ * all requests, max_kv of at least 2048; no window). workspace:
+ * pmi_paged_attention_shared_workspace_bytes() bytes, otherwise as above. */
 PMI_API int pmi_paged_attention_shared(const void* q, int dtype, int64_t q_stride,
                                        int64_t q_head_stride, const void* k_cache,
                                        const void* v_cache, const float* k_scale,
@@ -761,7 +764,7 @@ PMI_API int pmi_shared_prefixes(const int32_t* tables, int64_t table_stride,
 PMI_API size_t pmi_shared_prefixes_workspace_bytes(int64_t R);
 
 /* Logits before a token is chosen. x [R, V] (PMI_F16, PMI_BF16 or PMI_F32, rows `stride` elements
- * apart) to out of the same type (rows out_stride apart; may be x), in fp32, rounded once:
+ * apart) to out of the same type (rows out_stride apart; x, or no value of x's), in fp32, rounded once:
  *   x > 0 ? x / repetition[r] : x * repetition[r]       for tokens in the row's history
  *   x - frequency[r] * c - presence[r]                  for those c > 0 times in it behind the prompt
  *   x + the row's biases of the token                   (added up in their order first)

@@ -1529,12 +1529,12 @@ size_t pmi_paged_attention_shared_workspace_bytes(int64_t T, int64_t R, int64_t 
 namespace {
 
 int paged_attention(const char* fn, const int32_t* runs, const int32_t* run_lens, const void* q, int dtype,
-                    int64_t q_stride, int64_t q_head_stride, const void* k_cache,
-                        const void* v_cache, const float* k_scale, const float* v_scale, int code_dtype,
-                        int64_t n_pages, int64_t page_size, const int32_t* tables, int64_t table_stride,
-                        const int32_t* kv_lens, const int32_t* q_starts, void* out, int64_t T, int64_t R,
-                        int64_t width, int64_t H, int64_t KV, int64_t D, int64_t max_q, int64_t max_kv,
-                        int64_t window, float scale, void* workspace, size_t workspace_bytes, void* stream) {
+                    int64_t q_stride, int64_t q_head_stride, const void* k_cache, const void* v_cache,
+                    const float* k_scale, const float* v_scale, int code_dtype, int64_t n_pages, int64_t page_size,
+                    const int32_t* tables, int64_t table_stride, const int32_t* kv_lens, const int32_t* q_starts,
+                    void* out, int64_t T, int64_t R, int64_t width, int64_t H, int64_t KV, int64_t D, int64_t max_q,
+                    int64_t max_kv, int64_t window, float scale, void* workspace, size_t workspace_bytes,
+                    void* stream) {
   if (int rc = check_cache(k_cache, v_cache, k_scale, v_scale, code_dtype, n_pages, page_size, H, KV, D, fn)) return rc;
   if (dtype != PMI_F16 && dtype != PMI_BF16)
     return fail(PMI_ERR_INVALID, "%s: dtype must be PMI_F16 or PMI_BF16 (got %d)", fn, dtype);
@@ -1587,22 +1587,23 @@ int pmi_paged_attention(const void* q, int dtype, int64_t q_stride, int64_t q_he
                         const int32_t* kv_lens, const int32_t* q_starts, void* out, int64_t T, int64_t R,
                         int64_t width, int64_t H, int64_t KV, int64_t D, int64_t max_q, int64_t max_kv,
                         int64_t window, float scale, void* workspace, size_t workspace_bytes, void* stream) {
-  return paged_attention("pmi_paged_attention", nullptr, nullptr, q, dtype, q_stride, q_head_stride, k_cache, v_cache, k_scale, v_scale, code_dtype,
-                         n_pages, page_size, tables, table_stride, kv_lens, q_starts, out, T, R, width, H, KV, D, max_q, max_kv,
-                         window, scale, workspace, workspace_bytes, stream);
+  return paged_attention("pmi_paged_attention", nullptr, nullptr, q, dtype, q_stride, q_head_stride, k_cache, v_cache,
+                         k_scale, v_scale, code_dtype, n_pages, page_size, tables, table_stride, kv_lens, q_starts,
+                         out, T, R, width, H, KV, D, max_q, max_kv, window, scale, workspace, workspace_bytes, stream);
 }
 
 int pmi_paged_attention_shared(const void* q, int dtype, int64_t q_stride, int64_t q_head_stride, const void* k_cache,
-                        const void* v_cache, const float* k_scale, const float* v_scale, int code_dtype,
-                        int64_t n_pages, int64_t page_size, const int32_t* tables, int64_t table_stride,
-                        const int32_t* kv_lens, const int32_t* q_starts, const int32_t* runs, const int32_t* run_lens, void* out, int64_t T, int64_t R,
-                        int64_t width, int64_t H, int64_t KV, int64_t D, int64_t max_q, int64_t max_kv,
-                        int64_t window, float scale, void* workspace, size_t workspace_bytes, void* stream) {
+                               const void* v_cache, const float* k_scale, const float* v_scale, int code_dtype,
+                               int64_t n_pages, int64_t page_size, const int32_t* tables, int64_t table_stride,
+                               const int32_t* kv_lens, const int32_t* q_starts, const int32_t* runs,
+                               const int32_t* run_lens, void* out, int64_t T, int64_t R, int64_t width, int64_t H,
+                               int64_t KV, int64_t D, int64_t max_q, int64_t max_kv, int64_t window, float scale,
+                               void* workspace, size_t workspace_bytes, void* stream) {
   const char* fn = "pmi_paged_attention_shared";
   if (R > 0 && (!runs || !run_lens || !aligned(runs, 16))) return fail(PMI_ERR_INVALID, "%s: null buffer", fn);
-  return paged_attention(fn, runs, run_lens, q, dtype, q_stride, q_head_stride, k_cache, v_cache, k_scale, v_scale, code_dtype,
-                         n_pages, page_size, tables, table_stride, kv_lens, q_starts, out, T, R, width, H, KV, D, max_q, max_kv,
-                         window, scale, workspace, workspace_bytes, stream);
+  return paged_attention(fn, runs, run_lens, q, dtype, q_stride, q_head_stride, k_cache, v_cache, k_scale, v_scale,
+                         code_dtype, n_pages, page_size, tables, table_stride, kv_lens, q_starts, out, T, R, width, H,
+                         KV, D, max_q, max_kv, window, scale, workspace, workspace_bytes, stream);
 }
 
 int pmi_fork_block_tables(int32_t* tables, int64_t table_stride, int32_t* kv_lens, const int32_t* parents,
@@ -1724,6 +1725,14 @@ int pmi_process_logits(const void* logits, int dtype, int64_t stride, const int3
   if (R == 0 || V == 0) return ok();
   if (!out || !aligned(out, dtype == PMI_F32 ? 4 : 2))
     return fail(PMI_ERR_INVALID, "%s: out is null or not aligned to its type", fn);
+  // out is the logits, or shares no value with them: beside them in rows of the same stride, or apart
+  const int64_t size = dtype == PMI_F32 ? 4 : 2, apart = ((intptr_t)out - (intptr_t)logits) / size;
+  if (apart < (R - 1) * stride + V && -apart < (R - 1) * out_stride + V) {
+    const int64_t beside = (apart % stride + stride) % stride;
+    const bool same = apart == 0 && (R == 1 || out_stride == stride);
+    if (!same && (R == 1 || out_stride != stride || beside < V || beside > stride - V))
+      return fail(PMI_ERR_INVALID, "%s: out overlaps the logits, but is not them", fn);
+  }
   return from_hip(pmi::launch_process_logits(f, out, out_stride, (hipStream_t)stream), fn);
 }
 

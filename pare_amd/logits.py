@@ -123,7 +123,8 @@ def process_logits(logits: torch.Tensor, *, history: torch.Tensor | None = None,
       is; a row without such a mask (-1) allows all.
 
     The penalties are fp32 [R], each optional. Tokens outside 0 .. V - 1 are skipped (-1: none).
-    Rounded once. ``out`` may be ``logits``. Logits that need a gradient are refused."""
+    Rounded once. ``out`` may be ``logits``, or a tensor that shares no value with them. Logits that
+    need a gradient are refused."""
     if logits.requires_grad and torch.is_grad_enabled():
         raise RuntimeError("process_logits has no backward pass: detach the logits or call it under no_grad, their "
                            "gradient would be left out")

@@ -106,6 +106,13 @@ def test_process_logits_refuses(change):
     assert _lib.lib().pmi_process_logits(*_args(**change)) in (_lib.PMI_ERR_INVALID, _lib.PMI_ERR_UNSUPPORTED)
 
 
+@pytest.mark.parametrize("change", [dict(out=P8 + 2), dict(out=P8 - 2), dict(out=P8 + 398), dict(out=P8 - 398),
+                                    dict(ostride=101), dict(out=P8 + 200, ostride=101), dict(out=P8 + 2, R=1),
+                                    dict(out=P8 + 198, stride=201, ostride=201), dict(out=P8 + 204, stride=201, ostride=201)])
+def test_an_output_that_overlaps_the_logits_is_refused(change):
+    assert _lib.lib().pmi_process_logits(*_args(**change)) == _lib.PMI_ERR_INVALID
+
+
 @pytest.mark.parametrize("change", BOTH + [dict(tokens=None), dict(tstride=0), dict(V=0, words=0), dict(R=16385), dict(ws=None),
                                            dict(ws=P8 + 16), dict(ws_bytes=100)])
 def test_greedy_tokens_refuses(change):
@@ -334,6 +341,22 @@ def test_logits_past_2_31_values():
     assert torch.equal(got, (at == 0).long())
     P.process_logits(x, history=h, presence=torch.full((R,), 6.0, device=DEV), out=x)
     assert (x.gather(1, at[:, None]) == -1).all() and int((x != 0).sum()) == R
+
+
+@gpu
+def test_an_output_beside_the_logits():
+    """Halves of one buffer, and rows behind the logits' rows."""
+    x = torch.randn(4, 100, device=DEV)
+    want = P.process_logits(x)
+    both = torch.cat([x, x * 0], 1)
+    P.process_logits(both[:, :100], out=both[:, 100:])
+    assert torch.equal(both[:, 100:], want) and torch.equal(both[:, :100], x)
+    rows = torch.cat([x, x * 0])
+    P.process_logits(rows[:4], out=rows[4:])
+    assert torch.equal(rows[4:], want) and torch.equal(rows[:4], x)
+    one = torch.cat([x[0], x[0] * 0]).view(1, 200)
+    P.process_logits(one[:, :100], out=one[:, 100:])
+    assert torch.equal(one[0, 100:], want[0])
 
 
 @gpu
