@@ -243,7 +243,8 @@ def compact_block_tables(block_tables: torch.Tensor, kv_lens: torch.Tensor, free
     0 .. n - 1, in place: those from n on, in order, take the places of the free ones before it, in order.
     Pages n, n + 1, .. are the ring's free ones afterwards, in that order, also pages that
     neither a request nor the ring held. The returned moves ([pages / 2], as many as ``count``
-    says) are for ``copy_kv_pages``, on the same stream. ``shares``: as in ``fork_block_tables``, or
+    says) are for ``copy_kv_pages``, on the same stream. It is for between two steps: slots of a plan made
+    before are of the old places. ``shares``: as in ``fork_block_tables``, or
     None."""
     dev = _hip(block_tables, "compact_block_tables")
     moves = _lib.host().compact_tables(block_tables, kv_lens, free_pages, pool, shares, page_size, *_here())
@@ -335,8 +336,9 @@ def shared_prefixes(block_tables: torch.Tensor, kv_lens: torch.Tensor, q_starts:
         _lib.check(L.pmi_shared_prefixes(
             block_tables.data_ptr(), _row_stride(block_tables), kv_lens.data_ptr(),
             q_starts.data_ptr() if q_starts is not None else None, starts.data_ptr(), lens.data_ptr(),
-            runs.data_ptr(), R, width, page_size, -(-least // max(page_size, 1)), ws.data_ptr() if ws is not None else None,
-            ws.numel() if ws is not None else 0, stream), "pmi_shared_prefixes")
+            runs.data_ptr(), R, width, page_size, -(-least // max(page_size, 1)),
+            ws.data_ptr() if ws is not None else None, ws.numel() if ws is not None else 0, stream),
+            "pmi_shared_prefixes")
     return SharedPrefixes(starts, lens, runs.view(R, 4))
 
 
@@ -540,7 +542,8 @@ class PagedKVCache:
                                      self.page_size, lengths=lengths))
 
     def compact(self) -> None:
-        """``compact_block_tables`` in place, with the copies of all layers."""
+        """``compact_block_tables`` in place, with the copies of all layers; not between a step's ``extend``
+        and its last ``append``, whose plan has the old slots."""
         self._copy(compact_block_tables(self.block_tables, self.kv_lens, self.free_pages, self.pool, self.shares,
                                         self.page_size))
 

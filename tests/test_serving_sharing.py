@@ -139,6 +139,46 @@ def test_a_serving_loop_of_forks(code, page_size, seed):
     _consistent(cache)
 
 
+@pytest.mark.parametrize("sharing", [True, False])
+def test_compaction_and_sizes_of_a_cache(sharing):
+    """Both kinds of cache are compacted, shrunk and grown, and serve on; a plan's slots are those of
+    the places at its making."""
+    cache = P.PagedKVCache(2, 4, 128, 2, 64, DEV, page_size=16, sharing=sharing)
+    cos, sin = _rope(128, 64)
+    g = torch.Generator(device=DEV).manual_seed(int(sharing))
+
+    def step(lens):
+        total = sum(lens)
+        plan = cache.extend(_ints(lens), total)
+        for i in range(2):
+            cache.append(i, torch.randn(total, 8 * 64, generator=g, device=DEV).half(), cos, sin, plan)
+        return plan
+
+    step([40, 100, 16, 33])
+    cache.release(torch.tensor([False, True, False, False], device=DEV))
+    for change in (cache.compact, lambda: cache.resize(8), lambda: cache.resize(40), cache.compact):
+        lens = cache.kv_lens.tolist()
+        want = [_values(cache, r, n) for r, n in enumerate(lens) if n]
+        change()
+        assert cache.kv_lens.tolist() == lens
+        for a, b in zip(want, [_values(cache, r, n) for r, n in enumerate(lens) if n]):
+            assert torch.equal(a, b)
+        live = sum(-(-n // 16) for n in lens)
+        assert sorted(p for r, n in enumerate(lens) for p in cache.block_tables[r, :-(-n // 16)].tolist()) == [*range(live)]
+        pages = cache.free_pages.numel()
+        assert cache.pool.tolist()[:2] == [0, pages - live]
+        assert cache.free_pages.tolist() == [(live + i) % pages for i in range(pages)]
+    with pytest.raises(ValueError, match="hold 7 pages"):
+        cache.resize(6)
+    plan = step([3, 20, 1, 0])
+    assert plan.kv_lens.tolist() == [43, 20, 17, 33] and cache.pool.tolist()[2] == 0
+    q = torch.randn(24, 4, 64, generator=g, device=DEV).half()
+    for i in range(2):
+        _against_64_bits(q, cache.attend(i, q, plan, scale=0.125), cache, i, plan, 0.125)
+    if sharing:
+        _consistent(cache)
+
+
 def test_forks_that_the_pool_cannot_hold_are_refused_whole():
     cache = P.PagedKVCache(1, 4, 64, 1, 64, DEV, page_size=16, pages=4, sharing=True)
     cache.extend(_ints([40, 0, 0, 0]), 40)
