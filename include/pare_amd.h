@@ -769,7 +769,7 @@ PMI_API size_t pmi_shared_prefixes_workspace_bytes(int64_t R);
  *   x - frequency[r] * c - presence[r]                  for those c > 0 times in it behind the prompt
  *   x + the row's biases of the token                   (added up in their order first)
  *   -inf                                                for tokens without a bit in the row's mask
- * history int32 [R, L] (nullable), of which history_lens[r] (int32 [R], nullable: L) tokens count,
+ * history int32 [R, L] (nullable, L < 2^30), of which history_lens[r] (int32 [R], nullable: L) tokens count,
  * the first prompt_lens[r] (nullable: 0) of them as the prompt; repetition, presence and
  * frequency fp32 [R], each nullable. bias_ids int32 and bias fp32 [R, n_bias]. Tokens outside
  * 0 .. V - 1 are skipped in both. allowed int32 [masks, words] (nullable): bit t % 32 of word t / 32 allows

@@ -132,9 +132,10 @@ int check_logits(const pmi::Logits& f, const char* fn) {
     return fail(PMI_ERR_INVALID, "%s: dtype must be PMI_F16, PMI_BF16 or PMI_F32 (got %d)", fn, f.dtype);
   if (f.R < 0 || f.V < 0 || f.stride < f.V || f.L < 0 || f.history_stride < f.L || f.n_bias < 0 || f.masks < 0)
     return fail(PMI_ERR_INVALID, "%s: R, V, L, n_bias and masks may not be negative, rows not overlap", fn);
-  if (f.V >= (1ll << 30) || f.L >= (1ll << 31) || f.n_bias >= (1ll << 30) || f.masks >= (1ll << 31) ||
+  if (f.V >= (1ll << 30) || f.L >= (1ll << 30) || f.n_bias >= (1ll << 30) || f.masks >= (1ll << 31) ||
       pmi::logits_workgroups(f.R < (1ll << 31) ? f.R : 1ll << 31, f.V, f.dtype) >= (1ll << 24))
-    return fail(PMI_ERR_UNSUPPORTED, "%s: too large (R=%lld V=%lld)", fn, (long long)f.R, (long long)f.V);
+    return fail(PMI_ERR_UNSUPPORTED, "%s: too large (R=%lld V=%lld L=%lld)", fn, (long long)f.R, (long long)f.V,
+                (long long)f.L);
   if (f.R == 0 || f.V == 0) return PMI_OK;
   if (!f.x) return fail(PMI_ERR_INVALID, "%s: null buffer", fn);
   if (f.n_bias && (!f.bias_ids || !f.bias))

@@ -10,7 +10,7 @@ struct Logits {
   const void* x;  // [R, V], rows `stride` elements apart
   int64_t stride;
   const int32_t* history;  // [R, L] tokens, or null
-  int64_t history_stride, L;
+  int64_t history_stride, L;  // L < 2^30: the kernel's 32-bit index goes up to a stride of its threads past it
   const int32_t* history_lens;  // [R], or null: L
   const int32_t* prompt_lens;   // [R], or null: 0
   const float* repetition;      // [R] each, or null

@@ -113,7 +113,8 @@ def process_logits(logits: torch.Tensor, *, history: torch.Tensor | None = None,
     """Logits [R, V] (fp16, bf16 or fp32, contiguous rows) with, in this order and in fp32:
 
     - x / ``repetition[r]`` where x > 0, else x * ``repetition[r]``, for the tokens of the row's
-      history: the first ``history_lens[r]`` (int32 [R], default all) of ``history`` int32 [R, L];
+      history: the first ``history_lens[r]`` (int32 [R], default all) of ``history`` int32 [R, L]
+      (L < 2^30; a count past 2^24 is rounded to fp32);
     - x - ``frequency[r]`` * c - ``presence[r]`` for tokens that are c > 0 times in it behind the
       first ``prompt_lens[r]`` (int32 [R], default 0);
     - x + ``bias[r, i]`` for token ``bias_ids[r, i]`` (int32 and fp32 [R, n]; a token's biases

@@ -378,3 +378,14 @@ def test_many_rows(rows):
     if rows == 16384:
         with pytest.raises(_lib.PmiError):
             P.greedy_tokens(torch.zeros(rows + 1, 8, device=DEV))
+
+
+# --- limits of a launch ---------------------------------------------------------------------
+
+@pytest.mark.parametrize("L", [1 << 30, (1 << 31) - 4096, (1 << 31) - 1])
+def test_histories_past_2_30_are_refused(L):
+    """The kernel goes through a history in steps of 4096 tokens with a 32-bit index: in one of more than 2^31 - 4096 it
+    would go negative, and read before the row."""
+    change = dict(L=L, hstride=L)
+    assert _lib.lib().pmi_process_logits(*_args(**change)) == _lib.PMI_ERR_UNSUPPORTED
+    assert _lib.lib().pmi_greedy_tokens(*_args(True, **change)) == _lib.PMI_ERR_UNSUPPORTED
