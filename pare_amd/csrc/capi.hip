@@ -133,7 +133,7 @@ int check_logits(const pmi::Logits& f, const char* fn) {
   if (f.R < 0 || f.V < 0 || f.stride < f.V || f.L < 0 || f.history_stride < f.L || f.n_bias < 0 || f.masks < 0)
     return fail(PMI_ERR_INVALID, "%s: R, V, L, n_bias and masks may not be negative, rows not overlap", fn);
   if (f.V >= (1ll << 30) || f.L >= (1ll << 30) || f.n_bias >= (1ll << 30) || f.masks >= (1ll << 31) ||
-      pmi::logits_workgroups(f.R < (1ll << 31) ? f.R : 1ll << 31, f.V, f.dtype) >= (1ll << 24))
+      !pmi::logits_launch_fits(f))
     return fail(PMI_ERR_UNSUPPORTED, "%s: too large (R=%lld V=%lld L=%lld)", fn, (long long)f.R, (long long)f.V,
                 (long long)f.L);
   if (f.R == 0 || f.V == 0) return PMI_OK;

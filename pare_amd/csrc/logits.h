@@ -25,7 +25,7 @@ struct Logits {
   int64_t R, V;
   int dtype;  // PMI_F16, PMI_BF16 or PMI_F32
 };
-int64_t logits_workgroups(int64_t R, int64_t V, int dtype);  // of a launch, at most
+bool logits_launch_fits(const Logits& f);  // its threads in 32 bits
 hipError_t launch_process_logits(const Logits& f, void* out, int64_t out_stride, hipStream_t stream);
 
 constexpr int64_t kGreedyMaxRows = 16384;  // a counter each

@@ -241,6 +241,13 @@ int64_t size_of(int dtype) { return dtype == 2 ? 4 : 2; }
 int64_t slices_of(int64_t V, int64_t size, bool aligned, int slice) {
   return (V + (aligned ? 0 : 16 / size - 1) + slice - 1) / slice;
 }
+// Whether the threads of a launch of this form pass no 2^32.
+template <typename F>
+bool fits(const Logits& f) {
+  const int64_t rows = f.R < (1ll << 31) ? f.R : 1ll << 31;
+  return rows * slices_of(f.V, size_of(f.dtype), false, F::kSlice) * F::kThreads < (1ll << 32);
+}
+bool wide(const Logits& f) { return f.L >= 1 << 15 || f.n_bias >= (1 << 16) - 1; }
 
 template <typename T, bool WRITE, typename F>
 hipError_t launch_form(const Logits& f, void* out, int64_t out_stride, int64_t* tokens, int64_t token_stride, void* ws,
@@ -256,9 +263,8 @@ hipError_t launch_form(const Logits& f, void* out, int64_t out_stride, int64_t* 
 template <typename T, bool WRITE>
 hipError_t launch_t(const Logits& f, void* out, int64_t out_stride, int64_t* tokens, int64_t token_stride, void* ws,
                     hipStream_t stream) {
-  if (f.L >= 1 << 15 || f.n_bias >= (1 << 16) - 1)
-    return launch_form<T, WRITE, Wide>(f, out, out_stride, tokens, token_stride, ws, stream);
-  if (f.R * ((f.V + Large::kSlice - 1) / Large::kSlice) >= device_cu_count())
+  if (wide(f)) return launch_form<T, WRITE, Wide>(f, out, out_stride, tokens, token_stride, ws, stream);
+  if (f.R * ((f.V + Large::kSlice - 1) / Large::kSlice) >= device_cu_count() && fits<Large>(f))
     return launch_form<T, WRITE, Large>(f, out, out_stride, tokens, token_stride, ws, stream);
   return launch_form<T, WRITE, Small>(f, out, out_stride, tokens, token_stride, ws, stream);
 }
@@ -273,16 +279,14 @@ hipError_t launch(const Logits& f, void* out, int64_t out_stride, int64_t* token
 
 }  // namespace
 
-int64_t logits_workgroups(int64_t R, int64_t V, int dtype) {
-  return R * slices_of(V, size_of(dtype), false, Small::kSlice);
-}
+bool logits_launch_fits(const Logits& f) { return wide(f) ? fits<Wide>(f) : fits<Small>(f); }
 
 hipError_t launch_process_logits(const Logits& f, void* out, int64_t out_stride, hipStream_t stream) {
   return launch<true>(f, out, out_stride, nullptr, 0, nullptr, stream);
 }
 
 size_t greedy_ws_bytes(int64_t R, int64_t V, int dtype) {
-  return kWsCounterBytes + (size_t)logits_workgroups(R, V, dtype) * 8;
+  return kWsCounterBytes + (size_t)(R * slices_of(V, size_of(dtype), false, Small::kSlice)) * 8;
 }
 
 hipError_t launch_greedy_tokens(const Logits& f, int64_t* tokens, int64_t token_stride, void* workspace,

@@ -389,3 +389,24 @@ def test_histories_past_2_30_are_refused(L):
     change = dict(L=L, hstride=L)
     assert _lib.lib().pmi_process_logits(*_args(**change)) == _lib.PMI_ERR_UNSUPPORTED
     assert _lib.lib().pmi_greedy_tokens(*_args(True, **change)) == _lib.PMI_ERR_UNSUPPORTED
+
+
+@pytest.mark.parametrize("change", [dict(L=1 << 15, hstride=1 << 15), dict(n_bias=(1 << 16) - 1)])
+def test_more_rows_than_a_launch_of_the_wide_form_holds_are_refused(change):
+    """2^23 workgroups of 512 threads are 2^32 threads: the library's refusal, not the runtime's error."""
+    for rows in (1 << 23, 1 << 31):
+        assert _lib.lib().pmi_process_logits(*_args(R=rows, **change)) == _lib.PMI_ERR_UNSUPPORTED
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_rows_past_a_launch_of_large_slices(dtype):
+    """Rows that are workgroups enough take 1024 threads each, up to 2^22 of them; more are done in the form of 256.
+    One fp32 sum and its rounding: the same bits."""
+    for R in ((1 << 22) - 1, 1 << 22, (1 << 22) + 3):
+        g = torch.Generator(device=DEV).manual_seed(R)
+        x = torch.randn(R, 5, generator=g, device=DEV).to(dtype)
+        at = torch.randint(0, 5, (R, 1), generator=g, device=DEV)
+        value = torch.randn(R, 1, generator=g, device=DEV)
+        got = P.process_logits(x, bias_ids=at.int(), bias=value)
+        assert torch.equal(got, x.float().scatter_add(1, at, value).to(dtype))
