@@ -17,6 +17,7 @@
 // points arrive as addresses, the stream as its handle.
 #include <ATen/ATen.h>
 #include <ATen/TensorSubclassLikeUtils.h>
+#include <c10/core/GradMode.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/utils/pybind.h>
 
@@ -198,6 +199,11 @@ bool rows(const at::Tensor& t, int64_t& stride) {
   return (t.size(1) <= 1 || t.stride(1) == 1) && (t.size(0) <= 1 || t.stride(0) >= t.size(1));
 }
 
+// A tensor whose gradient, or whose tangent, somebody waits for.
+bool differentiated(const at::Tensor& t) {
+  return (t.requires_grad() && c10::GradMode::is_enabled()) || t._fw_grad(0).defined();
+}
+
 // The processed logits, or with `greedy` their tokens: the arguments of pare_amd.process_logits and
 // pare_amd.greedy_tokens in their order.
 py::object logits(bool greedy, const at::Tensor& x, const Maybe& history, const Maybe& history_lens,
@@ -239,6 +245,11 @@ py::object logits(bool greedy, const at::Tensor& x, const Maybe& history, const 
     if (!none_or(allowed, dev, at::kInt, {masks, words}) || (!allowed_rows && masks != R)) return py::none();
   }
   if (!none_or(allowed_rows, dev, at::kInt, {R}) || (allowed_rows && !allowed)) return py::none();
+  if (!greedy) {
+    if (differentiated(x)) return py::none();
+    for (const Maybe* t : {&repetition, &presence, &frequency, &bias, &out})
+      if (*t && differentiated(**t)) return py::none();
+  }
   at::Tensor y, ws;
   int64_t out_stride = greedy ? 1 : V;
   if (out) {

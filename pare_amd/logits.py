@@ -12,6 +12,7 @@ from __future__ import annotations
 from typing import NamedTuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from .kernels import _DeviceGuard, _raw_stream, _workspace
@@ -104,6 +105,18 @@ def _host(greedy, logits, *rest):
                               lambda nbytes: _workspace(logits.device, stream, nbytes))
 
 
+def _no_gradient(**tensors: torch.Tensor | None) -> None:
+    """Refuses tensors whose gradient or tangent would be left out."""
+    for name, t in tensors.items():
+        if t is None:
+            continue
+        if t.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError(f"process_logits has no backward pass: detach {name} or call it under no_grad, the "
+                               "gradient would be left out")
+        if forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError(f"process_logits has no forward-mode derivative: the tangent of {name} would be left out")
+
+
 def process_logits(logits: torch.Tensor, *, history: torch.Tensor | None = None,
                    history_lens: torch.Tensor | None = None, prompt_lens: torch.Tensor | None = None,
                    repetition: torch.Tensor | None = None, presence: torch.Tensor | None = None,
@@ -124,15 +137,13 @@ def process_logits(logits: torch.Tensor, *, history: torch.Tensor | None = None,
       is; a row without such a mask (-1) allows all.
 
     The penalties are fp32 [R], each optional. Tokens outside 0 .. V - 1 are skipped (-1: none).
-    Rounded once. ``out`` may be ``logits``, or a tensor that shares no value with them. Logits that
-    need a gradient are refused."""
-    if logits.requires_grad and torch.is_grad_enabled():
-        raise RuntimeError("process_logits has no backward pass: detach the logits or call it under no_grad, their "
-                           "gradient would be left out")
+    Rounded once. ``out`` may be ``logits``, or a tensor that shares no value with them. Logits, penalties,
+    biases and an ``out`` that need a gradient are refused, and so are forward-mode tangents."""
     y = _host(False, logits, history, history_lens, prompt_lens, repetition, presence, frequency, bias_ids, bias,
               allowed, allowed_rows, out)
     if y is not None:
         return y if out is None else out
+    _no_gradient(logits=logits, repetition=repetition, presence=presence, frequency=frequency, bias=bias, out=out)
     args = _arguments("process_logits", logits, history, history_lens, prompt_lens, repetition, presence, frequency,
                       bias_ids, bias, allowed, allowed_rows)
     R, V = logits.shape

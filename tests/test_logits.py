@@ -410,3 +410,51 @@ def test_rows_past_a_launch_of_large_slices(dtype):
         value = torch.randn(R, 1, generator=g, device=DEV)
         got = P.process_logits(x, bias_ids=at.int(), bias=value)
         assert torch.equal(got, x.float().scatter_add(1, at, value).to(dtype))
+
+
+# --- derivatives ------------------------------------------------------------------------------
+
+def _float_arguments(dev):
+    a = dict(logits=torch.zeros(2, 64), history=torch.zeros(2, 3, dtype=torch.int32), repetition=torch.ones(2),
+             presence=torch.ones(2), frequency=torch.ones(2), bias_ids=torch.zeros(2, 3, dtype=torch.int32),
+             bias=torch.ones(2, 3), out=torch.zeros(2, 64))
+    return {k: v.to(dev) for k, v in a.items()}
+
+
+DERIVED = ["logits", "repetition", "presence", "frequency", "bias", "out"]
+
+
+def _refuses_derivatives(name, dev):
+    a = _float_arguments(dev)
+    a[name].requires_grad_()
+    with pytest.raises(RuntimeError, match="backward"):
+        P.process_logits(**a)
+    a = _float_arguments(dev)
+    with torch.autograd.forward_ad.dual_level():
+        a[name] = torch.autograd.forward_ad.make_dual(a[name], torch.ones_like(a[name]))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            P.process_logits(**a)
+
+
+@pytest.mark.parametrize("name", DERIVED)
+def test_a_derivative_that_would_be_left_out_is_refused(name):
+    _refuses_derivatives(name, "cpu")
+
+
+@gpu
+@pytest.mark.parametrize("name", DERIVED)
+def test_a_derivative_of_any_argument_is_refused(name):
+    """On the way through the host extension too; without a derivative, and for tokens, the call is done."""
+    _refuses_derivatives(name, DEV)
+    a = _float_arguments(DEV)
+    want = P.process_logits(**a).clone()
+    a[name].requires_grad_()
+    with torch.no_grad():
+        assert torch.equal(P.process_logits(**a), want)
+    a = _float_arguments(DEV)
+    with torch.autograd.forward_ad.dual_level():
+        assert torch.equal(P.process_logits(**a), want)
+    if name != "out":
+        del a["out"]
+        a[name].requires_grad_()
+        assert P.greedy_tokens(**a).tolist() == [1, 1]
