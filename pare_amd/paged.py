@@ -447,7 +447,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     L = _lib.lib()
     if shared is not None:
         _ints(dev, R, lens=shared.lens)
-        _ints(dev, 4 * R, runs=shared.runs.reshape(-1))
+        assert shared.runs.is_contiguous(), "runs must be contiguous"
+        _ints(dev, 4 * R, runs=shared.runs.view(-1))
         with _DeviceGuard(dev):
             stream = _raw_stream(dev)
             ws = _workspace(dev, stream, L.pmi_paged_attention_shared_workspace_bytes(T, R, H, KV, D, max_q, max_kv,

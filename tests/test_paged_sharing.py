@@ -734,3 +734,17 @@ def test_python_checks():
         P.fork_block_tables(t, two, two, free, four, free, 24)
     with pytest.raises(RuntimeError):
         P.PagedKVCache(1, 2, 64, 1, 64, DEV).fork(two)
+
+
+def test_runs_in_other_strides_are_refused(monkeypatch):
+    """Their address is handed over as that of R rows of 4: rows that lie apart, or one that stands for all, would be
+    read as others, and past their memory. (Checks come before anything of the device's.)"""
+    monkeypatch.setattr(P.paged, "_hip", lambda t, fn: t.device)
+    k, s = torch.zeros(4, 1, 16, 64, dtype=torch.int8), torch.zeros(4, 1)
+    args = (torch.zeros(3, 1, 64, dtype=torch.float16), k, k.view(4, 1, 1, 64, 16), s, s,
+            torch.zeros(3, 2, dtype=torch.int32), torch.zeros(3, dtype=torch.int32))
+    rows = torch.zeros(3, 8, dtype=torch.int32)
+    for runs in (rows[:, :4], rows[:1, :4].expand(3, 4), torch.zeros(4, 3, dtype=torch.int32).t()):
+        shared = P.SharedPrefixes(torch.zeros(4, dtype=torch.int32), torch.zeros(3, dtype=torch.int32), runs)
+        with pytest.raises(AssertionError, match="runs must be contiguous"):
+            P.paged_attention(*args, scale=0.125, shared=shared)
