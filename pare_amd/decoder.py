@@ -622,7 +622,7 @@ class QuantizedDecoder(nn.Module):
         row is ``eos``.
 
         ``prefix`` (1-D) stands before every prompt: it is prefilled once, and the requests
-        begin as forks of it. With ``rules`` (of one row a prompt) the tokens are those of
+        begin as forks of it; the cache has its whole pages once. With ``rules`` (of one row a prompt) the tokens are those of
         ``greedy_tokens``, each request's history its prefix, prompt and answer, of which only
         the answer counts for presence and frequency."""
         if not prompts or any(p.dim() != 1 or p.numel() == 0 for p in prompts):
@@ -637,7 +637,12 @@ class QuantizedDecoder(nn.Module):
         longest, total = max(lens), sum(lens)
         L = before + longest + n_generate
         cos, sin = self.rope_tables(L)
-        cache = self.new_paged_cache(R, L, page_size=page_size, dtype=dtype, sharing=prefix is not None)
+        # the prefix's whole pages once, and all else of every request
+        pages = None
+        if prefix is not None and page_size > 0:
+            common = before // page_size
+            pages = common + R * (-(-L // page_size) - common)
+        cache = self.new_paged_cache(R, L, page_size=page_size, pages=pages, dtype=dtype, sharing=prefix is not None)
         out = torch.empty(R, n_generate, dtype=torch.long, device=dev)
         tok = torch.zeros(R, 1, dtype=torch.long, device=dev)
         live = torch.ones(R, dtype=torch.int32, device=dev)

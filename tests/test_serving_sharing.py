@@ -393,6 +393,37 @@ def test_generation_with_rules(model, before):
             new = [1] * R
 
 
+@pytest.mark.parametrize("before,lens", [(16, [24, 24]), (37, [27] * 5), (300, [4] * 6), (15, [1, 9])])
+def test_a_prefix_takes_its_pages_once(model, before, lens, monkeypatch):
+    """The cache holds a prefix's whole pages once and everything else of every request, of whom none is refused: the
+    tokens are those of a cache with room for all of them at full length."""
+    prefix, prompts, n, ps = _prompts([before], seed=9)[0], _prompts(lens), 9, 16
+    R, width, common = len(lens), -(-(before + max(lens) + n) // ps), before // ps
+    make = model.new_paged_cache
+    for use_graph in (False, True):
+        got = []
+        for whole in (False, True):
+            caches = []
+
+            def recorded(*args, pages=None, **kw):
+                caches.append(make(*args, pages=None if whole else pages, **kw))
+                return caches[-1]
+
+            monkeypatch.setattr(model, "new_paged_cache", recorded)
+            got.append(model.generate_ragged(prompts, n, prefix=prefix, page_size=ps, use_graph=use_graph)[0])
+            assert caches[0].free_pages.numel() == (R * width if whole else common + R * (width - common))
+            assert caches[0].kv_lens.tolist() == [before + m + n - 1 for m in lens]
+            assert caches[0].pool.tolist()[2] == 0
+            _consistent(caches[0])
+        assert torch.equal(*got)
+    # every page is needed where the requests are as long as each other
+    if len(set(lens)) == 1 and (before + lens[0] + n - 2) // ps == width - 1:
+        cache = caches[0]
+        cache.compact()
+        cache.resize(common + R * (width - common))
+        assert int(cache.pool[1]) == 0
+
+
 def test_refusals(model):
     prompts = _prompts([9, 2])
     for bad in (torch.zeros(0, dtype=torch.long), torch.zeros(1, 2, dtype=torch.long)):
@@ -400,3 +431,10 @@ def test_refusals(model):
             model.generate_ragged(prompts, 4, prefix=bad)
     with pytest.raises(AssertionError):
         model.generate_ragged(prompts, 4, rules=P.LogitRules(repetition=torch.ones(3, device=DEV)))
+
+
+@pytest.mark.parametrize("page_size", [0, -16, 24])
+def test_page_sizes_that_no_cache_has_are_refused(model, page_size):
+    for prefix in (None, *_prompts([30])):
+        with pytest.raises(ValueError, match="page_size"):
+            model.generate_ragged(_prompts([9, 2]), 4, prefix=prefix, page_size=page_size)
