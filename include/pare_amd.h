@@ -703,7 +703,9 @@ PMI_API size_t pmi_paged_attention_shared_workspace_bytes(int64_t T, int64_t R, 
  * (nullable: all) how many of them; a request's parent is what it was before the call. With n tokens
  * the n / page_size whole pages are shared; if any are left, the page that holds them
  * is to be copied: a page from the ring becomes the fork's, and (src[r], dst[r]) int32 [R]
- * say what to copy where (-1, -1: nothing). Refused, and counted in pool[2]: a request that holds
+ * say what to copy where (-1, -1: nothing). With the page go its scales: the fork's tokens in it
+ * are read as its parent's are, as coarse as larger tokens behind them have made them, and as NaN
+ * where one of those is an infinity or NaN. Refused, and counted in pool[2]: a request that holds
  * tokens already, and one that needs a page when the needs up to it exceed the pool. scratch:
  * device memory of 4 R bytes. A page with several owners is whole, so that no token is
  * written to it. */

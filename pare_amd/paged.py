@@ -210,7 +210,10 @@ def fork_block_tables(block_tables: torch.Tensor, kv_lens: torch.Tensor, parents
 
     Their whole pages are owned by both from now on (``shares`` int32 [pages] counts a page's
     owners beyond the first); a last page that they do not fill is copied to a page from the ring:
-    the returned moves ([R]) are for ``copy_kv_pages``, on the same stream. A parent is what it was
+    the returned moves ([R]) are for ``copy_kv_pages``, on the same stream. The copy is of the whole
+    page with its scales, so a fork that ends inside a page reads its tokens as its parent does, bit for
+    bit: as coarse as larger tokens behind them in that page have made them, and as NaN where
+    one of those is an infinity or NaN (their own codes were lost with it). A parent is what it was
     before the call. Refused, and counted in ``pool[2]``, is a request that holds tokens, or that
     needs a page when the needs up to it exceed the pool."""
     dev = _hip(block_tables, "fork_block_tables")
@@ -313,7 +316,10 @@ def shared_prefixes(block_tables: torch.Tensor, kv_lens: torch.Tensor, q_starts:
     ``kv_lens`` int32 [R] with the new tokens that ``q_starts`` int32 [R + 1] counts (None: one
     each). A request joins the run of the request with new tokens before it if at least
     ``least`` positions of theirs, in whole pages before their new tokens, lie in the same pages;
-    the members of a run share what all of them have in common."""
+    the members of a run share what all of them have in common. Where groups of requests share more with
+    each other than with their neighbours (a document each, behind one system prompt), ``least`` has to be
+    above what all have in common for each group to be a run; else they are one run, which
+    shares that alone."""
     dev = _hip(block_tables, "shared_prefixes")
     here, stream = _here()
     runs = _lib.host().shared_prefixes(block_tables, kv_lens, q_starts, page_size, -(-least // max(page_size, 1)), here,
@@ -417,7 +423,9 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     ``shared``: what ``shared_prefixes`` says of the same tables, lengths and queries. The result
     is the same but for roundings; keys that a run of requests shares are read once for all of it
     where that pays: from 2048 keys (``max_kv_len``) and 2^27 bytes of all requests' keys and values on, up
-    to 32 query rows a request (``max_q_len`` H / KV), without a window."""
+    to 32 query rows a request (``max_q_len`` H / KV), without a window. The bounds decide for the whole
+    call, whatever the requests hold: with ``q_starts`` and no ``max_q_len`` the one is all of q, and one
+    request of many new tokens among single ones takes the sharing from all."""
     dev = _hip(q, "paged_attention")
     pages, KV, ps, D, code = _cache(dev, k_cache, v_cache, k_scale, v_scale)
     assert q.dim() == 3 and q.shape[2] == D and q.dtype in (torch.float16, torch.bfloat16), (

@@ -438,3 +438,25 @@ def test_page_sizes_that_no_cache_has_are_refused(model, page_size):
     for prefix in (None, *_prompts([30])):
         with pytest.raises(ValueError, match="page_size"):
             model.generate_ragged(_prompts([9, 2]), 4, prefix=prefix, page_size=page_size)
+
+
+@pytest.mark.parametrize("code", CODES)
+def test_a_fork_inside_a_page_has_its_parents_scale(code):
+    """Tokens behind the fork's, in the page where it ends, have made the page what it is: coarse for large ones, NaN
+    for an infinity. Its whole pages, and the page's other heads, are not touched by that."""
+    cache = P.PagedKVCache(1, 4, 64, 2, 64, DEV, page_size=16, dtype=code, sharing=True)
+    cos, sin = _rope(64, 64)
+    qkv = torch.randn(60, 6 * 64, generator=torch.Generator().manual_seed(2)).half()
+    qkv[28, 4 * 64:5 * 64] = 1000            # values of head 0, behind the first fork's 24 tokens
+    qkv[45, 5 * 64:] = float("inf")          # of head 1, behind the second's 40
+    plan = cache.extend(_ints([60, 0, 0, 0]), 60)
+    cache.append(0, qkv.to(DEV), cos, sin, plan)
+    cache.fork(_ints([-1, 0, 0, 0]), _ints([0, 24, 40, 32]))
+    for r, n in ((1, 24), (2, 40), (3, 32)):
+        mine, parent = _values(cache, r, n), _values(cache, 0, n)
+        assert torch.equal(mine.isnan(), parent.isnan()) and torch.equal(mine.nan_to_num(), parent.nan_to_num())
+    values = _values(cache, 2, 40)[1]
+    assert values[32:, 1].isnan().all() and not values[:32].isnan().any() and not values[32:, 0].isnan().any()
+    page = int(cache.block_tables[1, 1])
+    top = 127 if code == torch.int8 else 448
+    assert abs(float(cache.v_scale[0][page, 0]) * top / 1000 - 1) < 1e-6
