@@ -458,3 +458,76 @@ def test_a_derivative_of_any_argument_is_refused(name):
         del a["out"]
         a[name].requires_grad_()
         assert P.greedy_tokens(**a).tolist() == [1, 1]
+
+
+# --- the forms that large batches, long histories and many biases take ---------------------------
+
+def _laid_out(x, stride):
+    """x with rows `stride` values apart."""
+    room = torch.zeros(x.shape[0], stride, dtype=x.dtype, device=x.device)
+    return room[:, :x.shape[1]].copy_(x)
+
+
+def _check_forms(a, strides):
+    """Logits of several strides, written and in place, and their tokens."""
+    d = _on(a)
+    first = None
+    for stride in strides:
+        x = _laid_out(d["logits"], stride)
+        got = P.process_logits(**dict(d, logits=x))
+        if first is None:
+            first = got
+            _check(got, a)
+            tokens = _first_largest(got).tolist()
+        assert torch.equal(got, first)
+        assert P.greedy_tokens(**dict(d, logits=x)).tolist() == tokens
+        assert P.process_logits(**dict(d, logits=x), out=x) is x and torch.equal(x, first)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("R,V", [(64, 70001), (300, 1003)])
+def test_rows_that_are_workgroups_enough(R, V, dtype):
+    """Slices of 16384 tokens: histories with prompts, repeated biases and masks; rows that are aligned, and that are not."""
+    _check_forms(_case(R, V, 300, 30, 4, dtype, seed=R), (V, V + 8 - V % 8, V + 3))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("R", [3, 40])
+def test_long_histories_with_biases_and_masks(R, dtype):
+    """Counts in 32 bits, in slices of 8192 tokens."""
+    V = 20001
+    a = _case(R, V, 40000, 30, 2, dtype, seed=R)
+    a["history_lens"][0], a["prompt_lens"][0] = 40000, 39000
+    a["history_lens"][1], a["prompt_lens"][1] = 33000, 0
+    _check_forms(a, (V, V + 7, V + 2))
+
+
+@gpu
+@pytest.mark.parametrize("R", [2, 64])
+@pytest.mark.parametrize("L", [(1 << 15) - 1, 1 << 15])
+def test_one_token_that_fills_its_history(L, R):
+    """The most that 16 bits with the prompt's flag count, and one more."""
+    V, token = 70001, 65537
+    h = torch.full((R, L), token, dtype=torch.int32)
+    a = dict(_case(R, V, None, 5, 2, torch.float32, seed=L), history=h, prompt_lens=torch.arange(R).int() % 2,
+             repetition=torch.full((R,), 1.5), frequency=torch.full((R,), 0.25), presence=torch.full((R,), 1.0))
+    a["allowed"][1, token // 32] |= 1 << (token % 32)
+    a["allowed_rows"][:2] = 1
+    _check_forms(a, (V, V + 3))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("R", [2, 64])
+@pytest.mark.parametrize("n", [(1 << 16) - 2, (1 << 16) - 1])
+def test_as_many_biases_as_16_bits_name_and_more(n, R, dtype):
+    """The last entry of each form; a token with a first and a last bias, and none with more."""
+    V = 70001
+    a = _case(R, V, 20, 0, 1, dtype, seed=n)
+    rows = [torch.randperm(V, generator=torch.Generator().manual_seed(r))[:n].int() for r in range(2)]
+    ids = torch.stack([rows[r % 2] for r in range(R)])
+    ids[0, n - 1] = ids[0, 0]
+    a.update(bias_ids=ids, bias=5 * torch.randn(R, n, generator=torch.Generator().manual_seed(n)))
+    _check_forms(a, (V,))
