@@ -12,6 +12,7 @@ import torch
 
 import pare_amd as P
 from oracle import serving_oracle as S
+from pare_amd import _lib
 from pare_amd.decoder import DecoderConfig, QuantizedDecoder, add_rmsnorm
 
 pytestmark = pytest.mark.gpu
@@ -460,3 +461,35 @@ def test_a_fork_inside_a_page_has_its_parents_scale(code):
     page = int(cache.block_tables[1, 1])
     top = 127 if code == torch.int8 else 448
     assert abs(float(cache.v_scale[0][page, 0]) * top / 1000 - 1) < 1e-6
+
+
+def test_generation_whose_shared_pages_are_read_once(model, monkeypatch):
+    """As many requests behind as long a prefix as the rule wants: every layer's attention of the prompts' step and of
+    the tokens' is the one of parts, and within its tolerance; captured steps give the same tokens."""
+    before, n = 7300, 3
+    lens = [1 + i * 5 % 8 for i in range(36)]
+    prefix, prompts = _prompts([before], seed=9)[0], _prompts(lens)
+    make, seen = model.new_paged_cache, []
+    L, R, H, KV, D = _lib.lib(), len(lens), SMALL.heads, SMALL.kv_heads, SMALL.head_dim
+
+    def recorded(*args, **kw):
+        cache = make(*args, **kw)
+        attend = cache.attend
+
+        def check(layer, q, plan, *, max_q_len, max_kv_len, shared, **kw):
+            out = attend(layer, q, plan, max_q_len=max_q_len, max_kv_len=max_kv_len, shared=shared, **kw)
+            if shared is not None:
+                sizes = (q.shape[0], R, H, KV, D, max_q_len, max_kv_len, 0)
+                assert L.pmi_paged_attention_shared_workspace_bytes(*sizes) > L.pmi_paged_attention_workspace_bytes(*sizes)
+                assert shared.lens.tolist() == [before // 64 * 64] * R and shared.runs[0, 2] == q.shape[0]
+                _against_64_bits(q, out, cache, layer, plan, kw["scale"])
+                seen.append(layer)
+            return out
+        monkeypatch.setattr(cache, "attend", check)
+        return cache
+
+    with monkeypatch.context() as m:
+        m.setattr(model, "new_paged_cache", recorded)
+        eager, _ = model.generate_ragged(prompts, n, prefix=prefix, use_graph=False)
+    assert seen == [0, 1] * n
+    assert torch.equal(model.generate_ragged(prompts, n, prefix=prefix)[0], eager)
