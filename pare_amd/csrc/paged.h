@@ -6,7 +6,8 @@
 
 namespace pmi {
 
-constexpr int kTablesMaxRequests = 4096;  // a workgroup's LDS holds three ints a request
+// The LDS of a workgroup holds up to four ints a request (shared_runs_kernel: 64 KB and its waves' sums).
+constexpr int kTablesMaxRequests = 4096;
 
 struct PagedTables {
   int32_t* tables;  // [R, width], row stride `stride`

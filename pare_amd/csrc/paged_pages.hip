@@ -125,9 +125,9 @@ __global__ __launch_bounds__(256) void share_pages_kernel(PagedFork f) {
 // ---- caches of few pages, in one workgroup ----------------------------------------------
 
 // Releases and compactions of few table entries and pages are bound by their launches and the chain of
-// loads: one workgroup of 1024 threads then does all, with a bit or a count of each page in LDS (5 us each).
-// us, both with a copy of pages and what else a step does, in a graph, so / in the launches below: 12
-// requests of up to 19 pages 21.8 / 30.5, 64 of up to 222 (14208 entries) 49 / 34.
+// loads. One workgroup of 1024 threads then does all, with a bit or a count of each page in LDS, 5 us each.
+// A release and a compaction with its copies, in a graph, took in this form / in the launches further down
+// (us): 12 requests of up to 19 pages 21.8 / 30.5, 64 of up to 222 (14208 entries) 49 / 34.
 constexpr int kSmallPages = 16384, kSmallEntries = 4096, kSmallThreads = 1024;
 
 // f(r, j, page) for the entries of all requests that `use(r)` tells to take, eight of a thread in flight.
@@ -564,6 +564,8 @@ __global__ __launch_bounds__(kRunThreads) void shared_runs_kernel(PagedRuns f) {
 
 unsigned row_pieces(int64_t width) { return (unsigned)((width + kRowEntries - 1) / kRowEntries); }
 
+bool one_workgroup(int64_t R, int64_t width, int64_t ring) { return ring <= kSmallPages && R * width <= kSmallEntries; }
+
 }  // namespace
 
 hipError_t launch_fork_tables(const PagedFork& f, hipStream_t stream) {
@@ -577,10 +579,8 @@ hipError_t launch_fork_tables(const PagedFork& f, hipStream_t stream) {
 
 int64_t page_chunks(int64_t ring) { return (ring + kChunk - 1) / kChunk; }
 
-bool small(int64_t R, int64_t width, int64_t ring) { return ring <= kSmallPages && R * width <= kSmallEntries; }
-
 hipError_t launch_release_shared(const PagedRelease& f, hipStream_t stream) {
-  if (small(f.R, f.width, f.ring)) {
+  if (one_workgroup(f.R, f.width, f.ring)) {
     hipLaunchKernelGGL(release_small_kernel, dim3(1), dim3(kSmallThreads), 0, stream, f);
     return hipGetLastError();
   }
@@ -594,7 +594,7 @@ hipError_t launch_release_shared(const PagedRelease& f, hipStream_t stream) {
 }
 
 hipError_t launch_compact_tables(const PagedCompact& f, hipStream_t stream) {
-  if (small(f.R, f.width, f.ring)) {
+  if (one_workgroup(f.R, f.width, f.ring)) {
     hipLaunchKernelGGL(compact_small_kernel, dim3(1), dim3(kSmallThreads), 0, stream, f);
     return hipGetLastError();
   }
