@@ -544,7 +544,8 @@ class PagedKVCache:
                              shares=self.shares)
 
     def fork(self, parents: torch.Tensor, lengths: torch.Tensor | None = None) -> None:
-        """``fork_block_tables`` in place, with the copies of all layers."""
+        """``fork_block_tables`` in place, with the copies of all layers; not between a step's ``extend`` and its
+        last ``append``, when the parents' lengths count tokens that are not there to be copied."""
         if self.shares is None:
             raise RuntimeError("fork needs a cache made with sharing=True")
         self._copy(fork_block_tables(self.block_tables, self.kv_lens, parents, self.free_pages, self.pool, self.shares,

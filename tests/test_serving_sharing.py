@@ -253,6 +253,59 @@ def test_a_step_of_all_operators_captured_and_on_another_stream():
     assert (sa["history"][0, :int(sa["lens"][0])] != 0).all()  # token 0 is not allowed for every second request
 
 
+@pytest.mark.parametrize("R,L", [(6, 300), (40, 4000)])
+def test_forks_releases_and_compactions_captured(R, L):
+    """The tables' small forms and the large ones, with their copies, in a graph: replays leave the cache as the same
+    calls do eagerly, bit for bit, with other requests each time."""
+    KV, D, ps = 2, 64, 16
+
+    def make():
+        cache = P.PagedKVCache(2, R, L, KV, D, DEV, page_size=ps, sharing=True)
+        s = dict(new=_ints([0] * R), parents=_ints([-1] * R), at=_ints([0] * R),
+                 done=torch.zeros(R, dtype=torch.bool, device=DEV))
+        qkv = torch.randn(8 * R, (2 + 2 * KV) * D, generator=torch.Generator(device=DEV).manual_seed(1), device=DEV).half()
+        cos, sin = _rope(L, D)
+
+        def step():
+            plan = cache.extend(s["new"], 8 * R)
+            for layer in range(2):
+                cache.append(layer, qkv, cos, sin, plan)
+            cache.fork(s["parents"], s["at"])
+            cache.release(s["done"])
+            cache.compact()
+        return cache, s, step
+
+    (a, sa, eager), (b, sb, captured) = make(), make()
+    stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        eager(), captured()
+        with torch.cuda.graph(graph, stream=stream):
+            captured()
+    torch.cuda.current_stream().wait_stream(stream)
+    rng, lens, forks = random.Random(R), [0] * R, 0
+    for i in range(25):
+        held = [r for r, n in enumerate(lens) if n]
+        new = [rng.randint(0, 8) if n or rng.random() < 0.2 else 0 for n in lens]
+        parents = [rng.choice(held) if held and not lens[r] and not new[r] and rng.random() < 0.5 else -1 for r in range(R)]
+        at = [rng.choice([L, rng.randint(0, L)]) for _ in range(R)]
+        done = [rng.random() < 0.15 for _ in range(R)]
+        for s in (sa, sb):
+            for t, x in zip(s.values(), (new, parents, at, done)):
+                t.copy_(torch.tensor(x, dtype=t.dtype))
+        eager()
+        torch.randn(1000, device=DEV).sum().item()
+        graph.replay()
+        torch.cuda.synchronize()
+        for x, y in zip((a.block_tables, a.kv_lens, a.pool, a.shares, a.free_pages, *a.k, *a.v, *a.k_scale, *a.v_scale),
+                        (b.block_tables, b.kv_lens, b.pool, b.shares, b.free_pages, *b.k, *b.v, *b.k_scale, *b.v_scale)):
+            assert torch.equal(x, y)
+        lens = a.kv_lens.tolist()
+        forks += sum(0 <= p and lens[r] > 0 for r, p in enumerate(parents))
+    assert forks > 3
+    _consistent(a)
+
+
 def test_two_streams_at_once():
     """Calls that interleave on two streams have workspaces of their own."""
     x = [torch.randn(64, 50000, device=DEV) for _ in range(2)]
