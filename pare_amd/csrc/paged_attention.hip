@@ -771,8 +771,9 @@ PMI_DEV void many_rows(const AttnArgs& a, uint8_t* lds, int& s_last, int wg) {
   }
   const int all_tiles = __builtin_amdgcn_readlane(upto, 63);
   if constexpr (MODE == kParts) {
-    // (the host does not know how many runs there are, nor what they share)
-    splits = all_tiles > 0 ? max(1, a.many_wgs / (all_tiles * a.KV)) : 1;
+    // (the host does not know how many runs there are, nor what they share. Runs that no batch has may be so many
+    // that the product passes 32 bits: it is made only where the ranges' parts have room for it)
+    splits = all_tiles > 0 && all_tiles <= a.many_wgs / a.KV ? a.many_wgs / (all_tiles * a.KV) : 1;
     sp = rest % splits, index = rest / splits;
   }
   if (index >= all_tiles) return;

@@ -748,3 +748,30 @@ def test_runs_in_other_strides_are_refused(monkeypatch):
         shared = P.SharedPrefixes(torch.zeros(4, dtype=torch.int32), torch.zeros(3, dtype=torch.int32), runs)
         with pytest.raises(AssertionError, match="runs must be contiguous"):
             P.paged_attention(*args, scale=0.125, shared=shared)
+
+
+@gpu
+def test_runs_whose_row_tiles_pass_32_bits_stay_inside_the_buffers():
+    """Runs that no batch has, each of all queries: 2^28 + 2 row tiles of 16 KV heads, 2^32 + 32 together, which are
+    not the 32 that 32 bits say (16 ranges each would be written past the parts). No request is said to share anything:
+    the bits are those without runs."""
+    R, KV, H, D, ps = 100000, 16, 64, 64, 16
+    g = torch.Generator(device=DEV).manual_seed(0)
+    k = torch.randint(-127, 128, (4, KV, ps, D), generator=g, device=DEV, dtype=torch.int8)
+    scale = torch.full((4, KV), 0.01, device=DEV)
+    tables = torch.randint(0, 4, (R, 2048 // ps), generator=g, device=DEV, dtype=torch.int32)
+    lens = torch.randint(1, 2 * ps, (R,), generator=g, device=DEV, dtype=torch.int32)
+    q = torch.randn(R, H, D, generator=g, device=DEV).half()
+    args = (q, k, k.view(4, KV, 1, D, 16), scale, scale, tables, lens)
+    tiles = -(-R * (H // KV) // 128)
+    n = 2 ** 28 // tiles
+    runs = torch.zeros(R, 4, dtype=torch.int32, device=DEV)
+    runs[:n, 2], runs[:n, 3] = R, ps
+    last = 2 ** 28 + 2 - n * tiles
+    runs[n, 2], runs[n, 3] = last * 128 // (H // KV), ps
+    assert 0 < last <= tiles and n * tiles + last == 2 ** 28 + 2 and n < R
+    sizes, L = (R, R, H, KV, D, 1, 2048, 0), _lib.lib()
+    assert L.pmi_paged_attention_shared_workspace_bytes(*sizes) > L.pmi_paged_attention_workspace_bytes(*sizes)
+    want = P.paged_attention(*args, scale=0.125)
+    got = P.paged_attention(*args, scale=0.125, shared=P.SharedPrefixes(runs[:, 0], torch.zeros_like(lens), runs))
+    assert torch.equal(got, want)
