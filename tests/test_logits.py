@@ -531,3 +531,27 @@ def test_as_many_biases_as_16_bits_name_and_more(n, R, dtype):
     ids[0, n - 1] = ids[0, 0]
     a.update(bias_ids=ids, bias=5 * torch.randn(R, n, generator=torch.Generator().manual_seed(n)))
     _check_forms(a, (V,))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("R,V,n", [(2, 9000, 700), (64, 70001, 3000), (2, 70001, (1 << 16) + 50)])
+def test_tokens_with_one_bias_beside_those_with_several(R, V, n, dtype):
+    """Bits of the sums in the entries' order, in each form: every third entry is of a token that has another one."""
+    g = torch.Generator().manual_seed(n)
+    ids = torch.stack([torch.randperm(V, generator=g)[torch.arange(n) % V].int() for _ in range(2)])
+    few = torch.randint(0, n // 5, ids[:, ::3].shape, generator=g)
+    ids[:, ::3] = ids.gather(1, few - few % 3 + 1)
+    bias = torch.randn(2, n, generator=g)
+    pick = torch.arange(R) % 2
+    x = torch.zeros(R, V, dtype=dtype, device=DEV)
+    got = P.process_logits(x, bias_ids=ids[pick].to(DEV), bias=bias[pick].to(DEV))
+    want = np.zeros((2, V), np.float32)
+    for r in range(2):
+        seen = set()
+        for t, b in zip(ids[r].tolist(), bias[r].numpy()):
+            want[r, t] = np.float32(want[r, t] + b) if t in seen else b
+            seen.add(t)
+    assert torch.equal(got.cpu(), torch.from_numpy(want).to(dtype)[pick])
+    tokens = P.greedy_tokens(x, bias_ids=ids[pick].to(DEV), bias=bias[pick].to(DEV))
+    assert tokens.tolist() == _first_largest(got).tolist()
