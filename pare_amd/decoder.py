@@ -622,9 +622,9 @@ class QuantizedDecoder(nn.Module):
         row is ``eos``.
 
         ``prefix`` (1-D) stands before every prompt: it is prefilled once, and the requests
-        begin as forks of it; the cache has its whole pages once. With ``rules`` (of one row a prompt) the tokens are those of
-        ``greedy_tokens``, each request's history its prefix, prompt and answer, of which only
-        the answer counts for presence and frequency."""
+        begin as forks of it; the cache has its whole pages once. With ``rules`` (of one row a
+        prompt) the tokens are those of ``greedy_tokens``, each request's history its prefix,
+        prompt and answer, of which only the answer counts for presence and frequency."""
         if not prompts or any(p.dim() != 1 or p.numel() == 0 for p in prompts):
             raise ValueError("prompts must be 1-D tensors of at least one token")
         if n_generate < 1:
